@@ -56,6 +56,15 @@ enum b200kv_status {
   B200KV_ERR_CUDA = 4,          /* a CUDA runtime / driver call failed       */
 };
 
+/* Element types of the entry points that take more than one. */
+enum b200kv_dtype {
+  B200KV_F16 = 0,
+  B200KV_BF16 = 1,
+  B200KV_F32 = 2,
+  B200KV_I8 = 3,    /* signed steps of a row's fp32 scale */
+  B200KV_E4M3 = 4,  /* float8 e4m3 steps of a row's fp32 scale */
+};
+
 /* Bits OR-ed into the optional device-side error flag. */
 #define B200KV_DEVERR_BAD_BLOCK 0x1 /* block id outside [0, num_blocks)       */
 #define B200KV_DEVERR_BAD_SLOT 0x2  /* slot outside [0, num_blocks * 64)      */
@@ -572,6 +581,121 @@ B200KV_API int b200kv_oproj_allreduce_f16(const void *attn, int64_t attn_stride_
                                           void *const *peer_buffers, int32_t rank, int32_t world,
                                           int64_t capacity_elems, int32_t *error_flag,
                                           void *stream);
+
+/* ------------------------------------------------------------------------ *
+ * Speculative verification over the paged cache: rotary positions, K/V rows
+ * quantised as they are written, attention for a tree of drafted tokens, and
+ * the move of the accepted path.  (No counterpart in the reference.)
+ *
+ * Pools: 16-bit (fp16 or bf16) [num_blocks, Hkv, D/64, 64, 64] for D = 64 or
+ * 128, or 8-bit (int8 or e4m3) [num_blocks, Hkv, 1, 64, 128] for D = 128 with
+ * one fp32 scale per row, [num_blocks, Hkv, 64]: element d of token row t
+ * stands for value(d) * scale(t).
+ * ------------------------------------------------------------------------ */
+
+/* Rotary positions.  Row (t, h) of x starts at x[t * x_stride_t + h *
+ * x_stride_h] (D contiguous elements of `dtype`: fp16, bf16 or fp32); out is
+ * contiguous [num_tokens, num_heads, head_dim].  Pair i < rotary_dim / 2 is
+ * elements (i, i + rotary_dim / 2), or (2i, 2i + 1) when interleaved:
+ *   a' = a c - b s,  b' = b c + a s,  (c, s) = table[positions[t]][i]
+ * (table fp32 [max_pos, rotary_dim / 2, 2]), in fp32, rounded once; elements
+ * from rotary_dim on are copied.  transpose != 0 turns by the opposite angle,
+ * the transposed map (the gradient).  A position outside [0, max_pos) is
+ * clamped and sets B200KV_DEVERR_BAD_LEN.  out must not overlap x.  16-byte
+ * vectors are used where base, strides and pairs fall on them; any other
+ * layout is taken element by element. */
+B200KV_API int b200kv_rotary(const void *x, int32_t dtype, int64_t x_stride_t, int64_t x_stride_h,
+                             void *out, const float *table, int64_t max_pos, int64_t rotary_dim,
+                             const int32_t *positions, int64_t num_tokens, int64_t num_heads,
+                             int64_t head_dim, int32_t interleaved, int32_t transpose,
+                             int32_t *error_flag, void *stream);
+
+/* Writes K/V rows to their slots, in one launch.  Row n, head h of k starts at
+ * k[n * k_stride_n + h * k_stride_h] (v, q likewise; row_dtype fp16 or bf16;
+ * 16-byte aligned, strides multiples of 8).  With a table (as above; half
+ * layout: rotary_dim a multiple of 16) k is turned by positions[n] first, and
+ * so is q into q_out (contiguous [N, Hq, D]; num_q_heads 0: no q).  A 16-bit
+ * pool has the rows' dtype and takes them rounded once.  An 8-bit pool takes
+ *   s = max|x| / qmax (127 or 448),  round_to_nearest(clamp(x * (1 / s)))
+ * in fp32 and s in k_scales / v_scales; a row whose s is not a normal number
+ * (all zeros) is stored as zeros with s = 0, a row with NaN or inf as zeros
+ * with s = NaN, so that it reads back as NaN.  Slots must be distinct;
+ * negative: the row is skipped; past the pool: skipped, B200KV_DEVERR_BAD_SLOT. */
+B200KV_API int b200kv_kv_store(const void *q, int64_t q_stride_n, int64_t q_stride_h, void *q_out,
+                               const void *k, int64_t k_stride_n, int64_t k_stride_h, const void *v,
+                               int64_t v_stride_n, int64_t v_stride_h, int32_t row_dtype,
+                               void *k_pool, void *v_pool, int32_t pool_dtype, float *k_scales,
+                               float *v_scales, const int64_t *slots, const float *table,
+                               int64_t max_pos, int64_t rotary_dim, const int32_t *positions,
+                               int32_t interleaved, int64_t num_tokens, int64_t num_q_heads,
+                               int64_t num_kv_heads, int64_t head_dim, int64_t num_blocks,
+                               int32_t *error_flag, void *stream);
+
+/* Gathers rows by slot into out, contiguous [N, Hkv, D] of out_dtype (fp16,
+ * bf16 or fp32), value * scale in fp32 rounded once.  Negative slots give rows
+ * of zeros, slots past the pool too (B200KV_DEVERR_BAD_SLOT). */
+B200KV_API int b200kv_kv_load(const void *pool, int32_t pool_dtype, const float *scales,
+                              const int64_t *slots, void *out, int32_t out_dtype,
+                              int64_t num_tokens, int64_t num_kv_heads, int64_t head_dim,
+                              int64_t num_blocks, int32_t *error_flag, void *stream);
+
+/* Tree masks from parents: node i of sequence b (nodes q_indptr[b] ..
+ * q_indptr[b + 1] - 1, indexes inside the sequence) sees itself and its
+ * ancestors; parents[i] is -1 for a root, -2 for a pruned node, which sees
+ * nothing, and less than i otherwise (else B200KV_DEVERR_BAD_LEN, and the walk
+ * ends there).  mask int64 [total_q, mask_words]: bit j % 64 of word j / 64. */
+B200KV_API int b200kv_tree_mask(const int32_t *parents, const int32_t *q_indptr, int64_t batch,
+                                int64_t total_q, int64_t mask_words, int64_t *mask,
+                                int32_t *error_flag, void *stream);
+
+/* Workspace bytes of b200kv_tree_attention (-1: unsupported shape).  It needs
+ * no initial contents; calls that share it must be ordered on one stream. */
+B200KV_API int64_t b200kv_tree_workspace_bytes(int64_t total_q, int64_t batch, int64_t num_q_heads,
+                                               int64_t num_kv_heads, int64_t head_dim);
+
+/* Attention of every sequence's drafted tokens over its cache.  Sequence b has
+ * context_lens[b] committed tokens, which all its nodes see, and
+ * T_b = q_indptr[b + 1] - q_indptr[b] nodes (at most max_nodes), whose K/V rows
+ * are already in the cache at positions context_lens[b] + 0 .. T_b - 1.  Node i
+ * sees node j where its mask has bit j (tree_mask NULL: where j <= i, a chain).
+ *   q    fp16 or bf16, row (t, h) at q[t * q_stride_t + h * q_stride_h],
+ *        16-byte aligned, strides positive multiples of 8; t counts the nodes
+ *        of all sequences (q_indptr[0] = 0, q_indptr[batch] = total_q)
+ *   pools  of q's dtype, or int8 / e4m3 with scales (see above)
+ *   out  contiguous [total_q, Hq, D] of q's dtype; lse fp32 [total_q, Hq] or
+ *        NULL, the natural-log logsumexp of the scaled scores
+ * A node that sees nothing gives a zero row and lse = -inf.  Lengths outside
+ * the block table or max_nodes are clamped and set B200KV_DEVERR_BAD_LEN, block
+ * ids outside the pool read as zeros and set B200KV_DEVERR_BAD_BLOCK.
+ * Supported: Hq / Hkv <= 128, batch <= 1024, D = 128 (64 in 16-bit pools). */
+B200KV_API int b200kv_tree_attention(const void *q, int32_t q_dtype, int64_t q_stride_t,
+                                     int64_t q_stride_h, const void *k_pool, const void *v_pool,
+                                     int32_t pool_dtype, const float *k_scales,
+                                     const float *v_scales, const int32_t *block_table,
+                                     int64_t block_table_stride, const int32_t *context_lens,
+                                     const int32_t *q_indptr, const int64_t *tree_mask,
+                                     int64_t mask_words, void *out, float *lse, int64_t total_q,
+                                     int64_t batch, int64_t num_q_heads, int64_t num_kv_heads,
+                                     int64_t head_dim, int64_t num_blocks,
+                                     int64_t max_blocks_per_seq, int64_t max_nodes, float scale,
+                                     void *workspace, int64_t workspace_bytes, int32_t *error_flag,
+                                     void *stream);
+
+/* Moves the accepted path: for i < path_lens[b], the K/V rows (and scales) of
+ * node path[b][i] go to position context_lens[b] + i, every row read before it
+ * is overwritten; new_lens[b] = context_lens[b] + path_lens[b].  The path
+ * ascends (a node comes after its ancestors); an entry that does not, or lies
+ * outside the block table, is skipped and sets B200KV_DEVERR_BAD_SLOT; bad
+ * lengths move nothing and set B200KV_DEVERR_BAD_LEN (new_lens[b] is then
+ * context_lens[b]). */
+B200KV_API int b200kv_tree_commit(void *k_pool, void *v_pool, int32_t pool_dtype, float *k_scales,
+                                  float *v_scales, const int32_t *block_table,
+                                  int64_t block_table_stride, const int32_t *context_lens,
+                                  const int32_t *path, int64_t path_stride,
+                                  const int32_t *path_lens, int32_t *new_lens, int64_t batch,
+                                  int64_t num_kv_heads, int64_t head_dim, int64_t num_blocks,
+                                  int64_t max_blocks_per_seq, int64_t max_path,
+                                  int32_t *error_flag, void *stream);
 
 #ifdef __cplusplus
 }

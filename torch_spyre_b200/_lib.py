@@ -22,6 +22,8 @@ STATUS_NAMES = {
     4: "B200KV_ERR_CUDA",
 }
 
+DTYPES = {"float16": 0, "bfloat16": 1, "float32": 2, "int8": 3, "float8_e4m3fn": 4}  # enum b200kv_dtype
+
 DEVERR_BAD_BLOCK = 0x1
 DEVERR_BAD_SLOT = 0x2
 DEVERR_BAD_LEN = 0x4
@@ -247,6 +249,45 @@ SIGNATURES = {
             _i64, _i64,  # num_blocks, max_blocks_per_seq
             _f32, _i64,  # scale, num_splits
             _p, _i64,  # workspace, workspace_bytes
+            _p, _p,  # error_flag, stream
+        ],
+    ),
+    "b200kv_rotary": (
+        ctypes.c_int,
+        [_p, _i32, _i64, _i64, _p, _p, _i64, _i64, _p, _i64, _i64, _i64, _i32, _i32, _p, _p],
+    ),
+    "b200kv_kv_store": (
+        ctypes.c_int,
+        [
+            _p, _i64, _i64, _p,  # q, q_stride_n, q_stride_h, q_out
+            _p, _i64, _i64, _p, _i64, _i64,  # k and v with their strides
+            _i32, _p, _p, _i32, _p, _p,  # row_dtype, pools, pool_dtype, scales
+            _p, _p, _i64, _i64, _p, _i32,  # slots, table, max_pos, rotary_dim, positions, interleaved
+            _i64, _i64, _i64, _i64, _i64,  # num_tokens, Hq, Hkv, head_dim, num_blocks
+            _p, _p,  # error_flag, stream
+        ],
+    ),
+    "b200kv_kv_load": (ctypes.c_int, [_p, _i32, _p, _p, _p, _i32, _i64, _i64, _i64, _i64, _p, _p]),
+    "b200kv_tree_mask": (ctypes.c_int, [_p, _p, _i64, _i64, _i64, _p, _p, _p]),
+    "b200kv_tree_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _i64]),
+    "b200kv_tree_attention": (
+        ctypes.c_int,
+        [
+            _p, _i32, _i64, _i64,  # q, q_dtype, q_stride_t, q_stride_h
+            _p, _p, _i32, _p, _p,  # pools, pool_dtype, scales
+            _p, _i64, _p, _p,  # block_table, block_table_stride, context_lens, q_indptr
+            _p, _i64, _p, _p,  # tree_mask, mask_words, out, lse
+            _i64, _i64, _i64, _i64, _i64,  # total_q, batch, Hq, Hkv, head_dim
+            _i64, _i64, _i64, _f32,  # num_blocks, max_blocks_per_seq, max_nodes, scale
+            _p, _i64, _p, _p,  # workspace, workspace_bytes, error_flag, stream
+        ],
+    ),
+    "b200kv_tree_commit": (
+        ctypes.c_int,
+        [
+            _p, _p, _i32, _p, _p,  # pools, pool_dtype, scales
+            _p, _i64, _p, _p, _i64, _p, _p,  # block_table, stride, context_lens, path, stride, path_lens, new_lens
+            _i64, _i64, _i64, _i64, _i64, _i64,  # batch, Hkv, head_dim, num_blocks, max_blocks_per_seq, max_path
             _p, _p,  # error_flag, stream
         ],
     ),

@@ -31,6 +31,9 @@ SOURCES = [
     "peer_allreduce.cu",
     "nvls_allreduce.cu",
     "rope.cu",
+    "rotary.cu",
+    "kv_rows.cu",
+    "tree_attention.cu",
     "lse_combine.cu",
     "oproj_allreduce.cu",
 ]

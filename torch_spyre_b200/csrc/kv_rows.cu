@@ -1,0 +1,574 @@
+// K/V rows into and out of the paged stick cache, with one scale per row for
+// 8-bit pools:
+//   store   k is turned by its rotary position (optional, q beside it), then
+//           s = max |x| / qmax, q = round(x * (1 / s)) clamped to +-qmax and
+//           written to the row's slot, s beside it (16-bit pools: rounded once);
+//   load    rows gathered by slot, q * s rounded once;
+//   commit  the accepted path of a drafted tree moved to the end of the
+//           committed tokens, bytes and scales as they are.
+// All three are bound by HBM (or, for a few rows, by a chain of 2-3 dependent
+// loads): one pass over the rows, 16-byte vectors, K and V in one launch.
+#include "rows.cuh"
+
+namespace b200kv {
+namespace {
+
+constexpr float kQMaxInt8 = 127.f, kQMaxE4M3 = 448.f;
+
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// ------------------------------------------------------------------ store --
+struct StoreArgs {
+  const void *q, *k, *v;
+  int64_t q_sn, q_sh, k_sn, k_sh, v_sn, v_sh;
+  void *q_out;  // contiguous [N, Hq, D]
+  void *k_pool, *v_pool;
+  float *k_scales, *v_scales;
+  const int64_t *slots;
+  const float2 *table;
+  int64_t max_pos;
+  const int32_t *positions;
+  int64_t tokens, num_slots;
+  int hq, hkv, half;
+  int32_t *error_flag;
+};
+
+// Eight fp32 -> eight 8-bit steps of 1 / inv.  fp32 arithmetic, each operation
+// rounded by itself, so the same steps as x * (1 / s) computed anywhere else.
+__device__ __forceinline__ uint2 steps8_int8(const float (&f)[8], float inv) {
+  uint32_t w[2] = {0, 0};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float c = fminf(fmaxf(__fmul_rn(f[i], inv), -kQMaxInt8), kQMaxInt8);
+    w[i >> 2] |= (static_cast<uint32_t>(__float2int_rn(c)) & 0xffu) << (8 * (i & 3));
+  }
+  return make_uint2(w[0], w[1]);
+}
+__device__ __forceinline__ uint2 steps8_e4m3(const float (&f)[8], float inv) {
+  uint32_t w[2] = {0, 0};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 p = make_float2(fminf(fmaxf(__fmul_rn(f[2 * i], inv), -kQMaxE4M3), kQMaxE4M3),
+                                 fminf(fmaxf(__fmul_rn(f[2 * i + 1], inv), -kQMaxE4M3), kQMaxE4M3));
+    w[i >> 1] |= static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(p, __NV_SATFINITE, __NV_E4M3)) << (16 * (i & 1));
+  }
+  return make_uint2(w[0], w[1]);
+}
+
+// A group of D / 8 lanes takes one row, kRows rows of a token one after the
+// other (q heads, then K heads, then V heads), its vector's cos / sin in
+// registers.  The half layout's partner vector comes by shuffle (rotary_dim / 2
+// is a multiple of 8, so the partner is a whole lane away).
+// kCache: B200KV_F16 (= the row type), B200KV_I8 or B200KV_E4M3.
+template <typename T, int D, int kCache, int kTurn, int kRows>  // kTurn 0 none, 1 half, 2 interleaved
+__global__ void __launch_bounds__(256) kv_store_kernel(const StoreArgs a) {
+  constexpr int kLanes = D / 8;
+  constexpr int kStick = kCache == B200KV_F16 ? 64 : 128;
+  const int lane = threadIdx.x % kLanes, e = lane * 8;
+  const int heads = a.hq + 2 * a.hkv;
+  const int groups = (heads + kRows - 1) / kRows;
+  const int64_t unit = (int64_t(blockIdx.x) * 256 + threadIdx.x) / kLanes;
+  const int64_t t = unit / groups;
+  const int r0 = static_cast<int>(unit - t * groups) * kRows;
+  const bool live_t = t < a.tokens;  // dead lanes stay for the shuffles
+
+  uint4 raw[kRows];
+  if (live_t) {
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+      const int r = r0 + i;
+      if (r >= heads) break;
+      const T *src;
+      if (r < a.hq)
+        src = static_cast<const T *>(a.q) + t * a.q_sn + r * a.q_sh;
+      else if (r < a.hq + a.hkv)
+        src = static_cast<const T *>(a.k) + t * a.k_sn + (r - a.hq) * a.k_sh;
+      else
+        src = static_cast<const T *>(a.v) + t * a.v_sn + (r - a.hq - a.hkv) * a.v_sh;
+      raw[i] = __ldg(reinterpret_cast<const uint4 *>(src + e));
+    }
+  }
+  int64_t slot = -1;
+  if (live_t && r0 + kRows > a.hq) {
+    slot = __ldg(a.slots + t);
+    if (slot >= a.num_slots) {
+      if (a.error_flag && lane == 0) atomicOr(a.error_flag, B200KV_DEVERR_BAD_SLOT);
+      slot = -1;
+    }
+  }
+  // cos / sin of this lane's elements: 8 pairs in the half layout (elements of
+  // the second half use the same pairs), 4 interleaved
+  constexpr int kPairs = kTurn == 2 ? 4 : 8;
+  float cosv[kPairs], sinv[kPairs];
+  const bool turn_lane = kTurn != 0 && e < 2 * a.half;
+  const bool second = kTurn == 1 && e >= a.half;
+  if (kTurn != 0) {
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) cosv[i] = 1.f, sinv[i] = 0.f;
+    if (live_t && turn_lane && r0 < a.hq + a.hkv) {
+      int64_t pos = __ldg(a.positions + t);
+      if (pos < 0 || pos >= a.max_pos) {
+        if (a.error_flag && lane == 0) atomicOr(a.error_flag, B200KV_DEVERR_BAD_LEN);
+        pos = pos < 0 ? 0 : a.max_pos - 1;
+      }
+      const float2 *row = a.table + pos * a.half + (kTurn == 2 ? e / 2 : (second ? e - a.half : e));
+#pragma unroll
+      for (int i = 0; i < kPairs; ++i) {
+        // an interleaved vector cut by rotary_dim: the identity past it
+        const bool in = kTurn == 1 || e / 2 + i < a.half;
+        const float2 cs = in ? __ldg(row + i) : make_float2(1.f, 0.f);
+        cosv[i] = cs.x;
+        sinv[i] = cs.y;
+      }
+    }
+  }
+  const int shift = kTurn == 1 ? a.half / 8 : 0;
+  const int partner = second ? lane - shift : lane + shift;
+
+#pragma unroll
+  for (int i = 0; i < kRows; ++i) {
+    const int r = r0 + i;
+    const bool live = live_t && r < heads;
+    float f[8];
+    if (live) unpack8(raw[i], f, T());
+    if (kTurn == 1) {
+      uint4 o;  // every lane takes part in the shuffles
+      o.x = __shfl_sync(0xffffffffu, raw[i].x, partner, kLanes);
+      o.y = __shfl_sync(0xffffffffu, raw[i].y, partner, kLanes);
+      o.z = __shfl_sync(0xffffffffu, raw[i].z, partner, kLanes);
+      o.w = __shfl_sync(0xffffffffu, raw[i].w, partner, kLanes);
+      if (live && turn_lane && r < a.hq + a.hkv) {
+        float p[8], unused;
+        unpack8(o, p, T());
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          if (second)
+            turn_pair(p[j], f[j], cosv[j], sinv[j], unused, f[j]);
+          else
+            turn_pair(f[j], p[j], cosv[j], sinv[j], f[j], unused);
+        }
+      }
+    } else if (kTurn == 2) {
+      if (live && turn_lane && r < a.hq + a.hkv) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (e / 2 + j < a.half) turn_pair(f[2 * j], f[2 * j + 1], cosv[j], sinv[j], f[2 * j], f[2 * j + 1]);
+      }
+    }
+    if (live && r < a.hq) {
+      T *dst = static_cast<T *>(a.q_out) + (t * a.hq + r) * D + e;
+      *reinterpret_cast<uint4 *>(dst) = pack8(f, T());
+    }
+    const bool is_k = r < a.hq + a.hkv;
+    const int h = r - a.hq - (is_k ? 0 : a.hkv);
+    const bool write = live && r >= a.hq && slot >= 0;
+    const int64_t page = (slot >> 6) * a.hkv + h;
+    const int in_page = static_cast<int>(slot & 63);
+    const int64_t at = (page * (D / kStick) + e / kStick) * (64 * kStick) + int64_t(in_page) * kStick + e % kStick;
+    void *pool = is_k ? a.k_pool : a.v_pool;
+    if (kCache == B200KV_F16) {
+      if (write) *reinterpret_cast<uint4 *>(static_cast<T *>(pool) + at) = pack8(f, T());
+    } else {
+      float amax = 0.f;
+      if (live) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) amax = max_nan(amax, fabsf(f[j]));
+      }
+#pragma unroll
+      for (int m = kLanes / 2; m >= 1; m >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, m, kLanes));
+      if (write) {
+        // a row without a normal scale (all zeros, or subnormal steps) is stored
+        // as zeros; a row that holds NaN or inf reads back as NaN throughout
+        float s = __fdiv_rn(amax, kCache == B200KV_I8 ? kQMaxInt8 : kQMaxE4M3);
+        if (s < 1.17549435e-38f) s = 0.f;
+        const bool finite = s < CUDART_INF_F;
+        const float inv = s > 0.f && finite ? __fdiv_rn(1.f, s) : 0.f;
+        const uint2 w = !finite ? make_uint2(0, 0)
+                        : kCache == B200KV_I8 ? steps8_int8(f, inv) : steps8_e4m3(f, inv);
+        *reinterpret_cast<uint2 *>(static_cast<uint8_t *>(pool) + at) = w;
+        if (lane == 0) (is_k ? a.k_scales : a.v_scales)[page * 64 + in_page] = finite ? s : CUDART_NAN_F;
+      }
+    }
+  }
+}
+
+template <typename T, int D, int kCache, int kTurn>
+int launch_store(const StoreArgs &a, cudaStream_t stream) {
+  int dev = 0, sms = 0;
+  int st = current_device_sm_count(&dev, &sms);
+  if (st != B200KV_OK) return st;
+  constexpr int kLanes = D / 8;
+  const int heads = a.hq + 2 * a.hkv;
+  // Four rows per lane group once every SM still gets its 2048 threads; with
+  // fewer rows one each, as the latency of the loads counts.
+  const bool deep = a.tokens * heads * kLanes >= int64_t(sms) * 2048 * 4;
+  const int64_t units = a.tokens * ((heads + (deep ? 3 : 0)) / (deep ? 4 : 1));
+  const int64_t blocks = (units * kLanes + 255) / 256;
+  if (blocks >= (int64_t{1} << 31)) return set_error(B200KV_ERR_UNSUPPORTED, "too many rows (%lld tokens)", (long long)a.tokens);
+  if (deep)
+    kv_store_kernel<T, D, kCache, kTurn, 4><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(a);
+  else
+    kv_store_kernel<T, D, kCache, kTurn, 1><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(a);
+  B200KV_CUDA_TRY(cudaGetLastError());
+  return B200KV_OK;
+}
+template <typename T, int D, int kCache>
+int store_turn(const StoreArgs &a, int turn, cudaStream_t s) {
+  return turn == 0 ? launch_store<T, D, kCache, 0>(a, s)
+                   : turn == 1 ? launch_store<T, D, kCache, 1>(a, s) : launch_store<T, D, kCache, 2>(a, s);
+}
+template <typename T>
+int store_cache(const StoreArgs &a, int64_t dim, int cache, int turn, cudaStream_t s) {
+  if (cache == B200KV_I8) return store_turn<T, 128, B200KV_I8>(a, turn, s);
+  if (cache == B200KV_E4M3) return store_turn<T, 128, B200KV_E4M3>(a, turn, s);
+  return dim == 64 ? store_turn<T, 64, B200KV_F16>(a, turn, s) : store_turn<T, 128, B200KV_F16>(a, turn, s);
+}
+
+// ------------------------------------------------------------------- load --
+struct LoadArgs {
+  const void *pool;
+  const float *scales;
+  const int64_t *slots;
+  void *out;  // contiguous [N, Hkv, D]
+  int64_t total, num_slots;
+  int hkv;
+  int32_t *error_flag;
+};
+
+// kElems elements per thread: 16 bytes of output.  Four of them in flight.
+template <int kCache, typename TIn, typename TOut, int D>
+__global__ void __launch_bounds__(256) kv_load_kernel(const LoadArgs a) {
+  constexpr bool k8 = kCache != B200KV_F16;
+  constexpr int kElems = 16 / sizeof(TOut);
+  constexpr int kStick = k8 ? 128 : 64;
+  constexpr int kChunks = D / kElems;
+  constexpr int kUnroll = 4;
+  const int64_t step = int64_t(gridDim.x) * blockDim.x;
+  for (int64_t base = blockIdx.x * int64_t(blockDim.x) + threadIdx.x; base < a.total; base += step * kUnroll) {
+    uint32_t w[kUnroll][4];
+    float sc[kUnroll];
+    bool live[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int64_t i = base + u * step;
+      live[u] = false;
+      sc[u] = 1.f;
+      if (i >= a.total) continue;
+      const int e = static_cast<int>(i % kChunks) * kElems;
+      const int64_t nh = i / kChunks;
+      const int64_t n = nh / a.hkv;
+      const int h = static_cast<int>(nh - n * a.hkv);
+      const int64_t slot = __ldg(a.slots + n);
+      if (slot < 0) continue;  // padding: a row of zeros
+      if (slot >= a.num_slots) {
+        if (a.error_flag && e == 0 && h == 0) atomicOr(a.error_flag, B200KV_DEVERR_BAD_SLOT);
+        continue;
+      }
+      live[u] = true;
+      const int64_t page = (slot >> 6) * a.hkv + h;
+      const int in_page = static_cast<int>(slot & 63);
+      const TIn *src = static_cast<const TIn *>(a.pool) +
+                       (page * (D / kStick) + e / kStick) * (64 * kStick) + int64_t(in_page) * kStick + e % kStick;
+      if constexpr (kElems * sizeof(TIn) == 16) {
+        const uint4 v = __ldcs(reinterpret_cast<const uint4 *>(src));
+        w[u][0] = v.x, w[u][1] = v.y, w[u][2] = v.z, w[u][3] = v.w;
+      } else if constexpr (kElems * sizeof(TIn) == 8) {
+        const uint2 v = __ldcs(reinterpret_cast<const uint2 *>(src));
+        w[u][0] = v.x, w[u][1] = v.y;
+      } else {
+        w[u][0] = __ldcs(reinterpret_cast<const uint32_t *>(src));
+      }
+      if (k8) sc[u] = __ldg(a.scales + page * 64 + in_page);
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int64_t i = base + u * step;
+      if (i >= a.total) continue;
+      float f[kElems];
+#pragma unroll
+      for (int j = 0; j < kElems; ++j) {
+        f[j] = 0.f;
+        if (!live[u]) continue;
+        if constexpr (kCache == B200KV_I8) {
+          f[j] = __fmul_rn(static_cast<float>(static_cast<int8_t>(w[u][j >> 2] >> (8 * (j & 3)))), sc[u]);
+        } else if constexpr (kCache == B200KV_E4M3) {
+          const __nv_fp8_storage_t b = static_cast<__nv_fp8_storage_t>(w[u][j >> 2] >> (8 * (j & 3)));
+          f[j] = __fmul_rn(__half2float(__half(__nv_cvt_fp8_to_halfraw(b, __NV_E4M3))), sc[u]);
+        } else {
+          const uint16_t b = static_cast<uint16_t>(w[u][j >> 1] >> (16 * (j & 1)));
+          f[j] = to_float(*reinterpret_cast<const TIn *>(&b));
+        }
+      }
+      TOut o[kElems];
+#pragma unroll
+      for (int j = 0; j < kElems; ++j) from_float(o[j], f[j]);
+      __stcs(reinterpret_cast<uint4 *>(static_cast<TOut *>(a.out) + i * kElems), *reinterpret_cast<uint4 *>(o));
+    }
+  }
+}
+
+template <int kCache, typename TIn, typename TOut, int D>
+int launch_load(LoadArgs a, int64_t rows, cudaStream_t stream) {
+  int dev = 0, sms = 0;
+  int st = current_device_sm_count(&dev, &sms);
+  if (st != B200KV_OK) return st;
+  a.total = rows * (D / (16 / static_cast<int>(sizeof(TOut))));
+  const int64_t want = (a.total + 1023) / 1024, cap = int64_t(sms) * 8;
+  kv_load_kernel<kCache, TIn, TOut, D><<<static_cast<unsigned>(want < cap ? want : cap), 256, 0, stream>>>(a);
+  B200KV_CUDA_TRY(cudaGetLastError());
+  return B200KV_OK;
+}
+template <int kCache, typename TIn, int D>
+int load_out(const LoadArgs &a, int64_t rows, int dtype, cudaStream_t s) {
+  switch (dtype) {
+    case B200KV_F16: return launch_load<kCache, TIn, __half, D>(a, rows, s);
+    case B200KV_BF16: return launch_load<kCache, TIn, __nv_bfloat16, D>(a, rows, s);
+    default: return launch_load<kCache, TIn, float, D>(a, rows, s);
+  }
+}
+
+// ----------------------------------------------------------------- commit --
+struct CommitArgs {
+  void *pool[2];
+  float *scales[2];
+  const int32_t *block_table;
+  int64_t bt_stride;
+  const int32_t *ctx, *path, *path_lens;
+  int64_t path_stride;
+  int32_t *new_lens;
+  int hkv, max_blocks, max_path;
+  int64_t num_blocks;
+  int32_t *error_flag;
+};
+
+constexpr int kCommitThreads = 256, kCommitBatch = 8;
+
+// One CTA per (KV head, K or V, sequence).  A row is kRow bytes, one 16-byte
+// vector per thread, kCommitBatch rows per thread and batch.  A batch is read
+// whole before any of it is written; the path ascends, so path[i] >= i and a
+// later batch never reads what an earlier one wrote.
+template <int kRow, int kStickRow, bool kScaled>  // bytes of a row, of a row inside one stick (128)
+__global__ void __launch_bounds__(kCommitThreads) tree_commit_kernel(const CommitArgs a) {
+  constexpr int kLanes = kRow / 16;
+  constexpr int kPerPass = kCommitThreads / kLanes;
+  const int h = blockIdx.x >> 1, kv = blockIdx.x & 1, b = blockIdx.y;
+  const int lane = threadIdx.x % kLanes, row = threadIdx.x / kLanes;
+  const int cap = a.max_blocks * kPageTokens;
+  const int ctx = __ldg(a.ctx + b);
+  const int n_in = __ldg(a.path_lens + b);
+  const bool bad = ctx < 0 || ctx > cap || n_in < 0 || n_in > a.max_path || ctx + n_in > cap;
+  const int n = bad ? 0 : n_in;
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    if (bad && a.error_flag) atomicOr(a.error_flag, B200KV_DEVERR_BAD_LEN);
+    a.new_lens[b] = bad ? ctx : ctx + n;
+  }
+  const int32_t *path = a.path + b * a.path_stride;
+  const int32_t *table = a.block_table + b * a.bt_stride;
+  uint8_t *pool = static_cast<uint8_t *>(a.pool[kv]);
+  // byte offset of this thread's vector of token `tok`, -1 (flagged) outside
+  auto offset = [&](int tok, int64_t *scale_at) -> int64_t {
+    if (tok < 0 || tok >= cap) {
+      if (a.error_flag && lane == 0) atomicOr(a.error_flag, B200KV_DEVERR_BAD_SLOT);
+      return -1;
+    }
+    const int blk = __ldg(table + (tok >> 6));
+    if (blk < 0 || blk >= a.num_blocks) {
+      if (a.error_flag && lane == 0) atomicOr(a.error_flag, B200KV_DEVERR_BAD_BLOCK);
+      return -1;
+    }
+    const int64_t page = int64_t(blk) * a.hkv + h;
+    *scale_at = page * 64 + (tok & 63);
+    const int byte = lane * 16;
+    return (page * (kRow / kStickRow) + byte / kStickRow) * (64 * kStickRow) + int64_t(tok & 63) * kStickRow +
+           byte % kStickRow;
+  };
+  for (int base = 0; base < n; base += kPerPass * kCommitBatch) {
+    uint4 v[kCommitBatch];
+    float s[kCommitBatch];
+    int64_t dst[kCommitBatch], dst_s[kCommitBatch];
+#pragma unroll
+    for (int u = 0; u < kCommitBatch; ++u) {
+      const int i = base + u * kPerPass + row;
+      dst[u] = -1;
+      if (i >= n) continue;
+      const int p = __ldg(path + i);
+      const int before = i > 0 ? __ldg(path + i - 1) : -1;
+      if (p <= before) {  // not ascending: the row stays where it is
+        if (a.error_flag && lane == 0) atomicOr(a.error_flag, B200KV_DEVERR_BAD_SLOT);
+        continue;
+      }
+      if (p == i) continue;  // in place
+      int64_t src_s = 0;
+      const int64_t src = p < cap - ctx ? offset(ctx + p, &src_s) : offset(cap, &src_s);
+      const int64_t to = offset(ctx + i, &dst_s[u]);
+      if (src < 0 || to < 0) continue;
+      dst[u] = to;
+      v[u] = *reinterpret_cast<const uint4 *>(pool + src);
+      if (kScaled && lane == 0) s[u] = a.scales[kv][src_s];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < kCommitBatch; ++u) {
+      if (dst[u] < 0) continue;
+      *reinterpret_cast<uint4 *>(pool + dst[u]) = v[u];
+      if (kScaled && lane == 0) a.scales[kv][dst_s[u]] = s[u];
+    }
+    __syncthreads();
+  }
+}
+
+int check_cache(int32_t dtype, int64_t head_dim, const char *what) {
+  const bool k8 = dtype == B200KV_I8 || dtype == B200KV_E4M3;
+  if (!k8 && dtype != B200KV_F16 && dtype != B200KV_BF16)
+    return set_error(B200KV_ERR_INVALID_ARG, "%s dtype %d is not fp16, bf16, int8 or e4m3", what, dtype);
+  if (head_dim != 128 && !(head_dim == 64 && !k8))
+    return set_error(B200KV_ERR_UNSUPPORTED, "head_dim %lld unsupported (128, or 64 in 16-bit pools)",
+                     (long long)head_dim);
+  return B200KV_OK;
+}
+
+}  // namespace
+}  // namespace b200kv
+
+using namespace b200kv;
+
+extern "C" int b200kv_kv_store(const void *q, int64_t q_stride_n, int64_t q_stride_h, void *q_out, const void *k,
+                               int64_t k_stride_n, int64_t k_stride_h, const void *v, int64_t v_stride_n,
+                               int64_t v_stride_h, int32_t row_dtype, void *k_pool, void *v_pool, int32_t pool_dtype,
+                               float *k_scales, float *v_scales, const int64_t *slots, const float *table,
+                               int64_t max_pos, int64_t rotary_dim, const int32_t *positions, int32_t interleaved,
+                               int64_t num_tokens, int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim,
+                               int64_t num_blocks, int32_t *error_flag, void *stream) {
+  clear_error();
+  B200KV_CHECK_ARG(row_dtype == B200KV_F16 || row_dtype == B200KV_BF16, "row dtype %d is not fp16 or bf16", row_dtype);
+  int st = check_cache(pool_dtype, head_dim, "pool");
+  if (st != B200KV_OK) return st;
+  const bool k8 = pool_dtype == B200KV_I8 || pool_dtype == B200KV_E4M3;
+  B200KV_CHECK_ARG(k8 || pool_dtype == row_dtype, "a 16-bit pool must have the rows' dtype");
+  B200KV_CHECK_ARG(num_tokens >= 0, "num_tokens must be >= 0 (got %lld)", (long long)num_tokens);
+  B200KV_CHECK_ARG(num_kv_heads > 0 && num_kv_heads <= 65536 && num_q_heads >= 0 && num_q_heads <= 65536 &&
+                       num_blocks > 0 && num_blocks < (int64_t{1} << 40),
+                   "head counts or num_blocks out of range");
+  if (table) {
+    B200KV_CHECK_ARG(max_pos > 0, "max_pos must be > 0");
+    B200KV_CHECK_ARG(rotary_dim > 0 && rotary_dim % 2 == 0 && rotary_dim <= head_dim,
+                     "rotary_dim (%lld) must be even and in (0, head_dim]", (long long)rotary_dim);
+    if (!interleaved && rotary_dim % 16 != 0)
+      return set_error(B200KV_ERR_UNSUPPORTED, "rotary_dim %lld unsupported in the half layout (multiples of 16)",
+                       (long long)rotary_dim);
+  } else {
+    B200KV_CHECK_ARG(num_q_heads == 0, "q is only taken to be turned: a table is needed");
+  }
+  if (num_tokens == 0) return B200KV_OK;
+  B200KV_CHECK_ARG(k && v && k_pool && v_pool && slots, "null pointer argument");
+  B200KV_CHECK_ARG(num_q_heads == 0 || (q && q_out), "null q or q_out");
+  B200KV_CHECK_ARG(!k8 || (k_scales && v_scales), "8-bit pools need k_scales and v_scales");
+  B200KV_CHECK_ARG(!table || positions, "a table needs positions");
+  B200KV_CHECK_ARG(aligned_to(k, 16) && aligned_to(v, 16) && aligned_to(k_pool, 16) && aligned_to(v_pool, 16) &&
+                       (num_q_heads == 0 || (aligned_to(q, 16) && aligned_to(q_out, 16))) && aligned_to(table, 8),
+                   "buffers must be 16-byte aligned");
+  B200KV_CHECK_ARG(k_stride_n % 8 == 0 && k_stride_h % 8 == 0 && v_stride_n % 8 == 0 && v_stride_h % 8 == 0 &&
+                       (num_q_heads == 0 || (q_stride_n % 8 == 0 && q_stride_h % 8 == 0)),
+                   "row strides must be multiples of 8 elements");
+  StoreArgs a{};
+  a.q = q, a.q_sn = q_stride_n, a.q_sh = q_stride_h, a.q_out = q_out;
+  a.k = k, a.k_sn = k_stride_n, a.k_sh = k_stride_h;
+  a.v = v, a.v_sn = v_stride_n, a.v_sh = v_stride_h;
+  a.k_pool = k_pool, a.v_pool = v_pool, a.k_scales = k_scales, a.v_scales = v_scales;
+  a.slots = slots;
+  a.table = reinterpret_cast<const float2 *>(table);
+  a.max_pos = max_pos;
+  a.positions = positions;
+  a.tokens = num_tokens;
+  a.num_slots = num_blocks * kPageTokens;
+  a.hq = static_cast<int>(num_q_heads);
+  a.hkv = static_cast<int>(num_kv_heads);
+  a.half = table ? static_cast<int>(rotary_dim / 2) : 0;
+  a.error_flag = error_flag;
+  const int turn = !table ? 0 : (interleaved ? 2 : 1);
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return row_dtype == B200KV_F16 ? store_cache<__half>(a, head_dim, pool_dtype, turn, s)
+                                 : store_cache<__nv_bfloat16>(a, head_dim, pool_dtype, turn, s);
+}
+
+extern "C" int b200kv_kv_load(const void *pool, int32_t pool_dtype, const float *scales, const int64_t *slots,
+                              void *out, int32_t out_dtype, int64_t num_tokens, int64_t num_kv_heads,
+                              int64_t head_dim, int64_t num_blocks, int32_t *error_flag, void *stream) {
+  clear_error();
+  int st = check_cache(pool_dtype, head_dim, "pool");
+  if (st != B200KV_OK) return st;
+  const bool k8 = pool_dtype == B200KV_I8 || pool_dtype == B200KV_E4M3;
+  B200KV_CHECK_ARG(out_dtype == B200KV_F16 || out_dtype == B200KV_BF16 || out_dtype == B200KV_F32,
+                   "out dtype %d is not fp16, bf16 or fp32", out_dtype);
+  B200KV_CHECK_ARG(num_tokens >= 0, "num_tokens must be >= 0 (got %lld)", (long long)num_tokens);
+  B200KV_CHECK_ARG(num_kv_heads > 0 && num_kv_heads <= 65536 && num_blocks > 0 && num_blocks < (int64_t{1} << 40),
+                   "num_kv_heads or num_blocks out of range");
+  if (num_tokens == 0) return B200KV_OK;
+  B200KV_CHECK_ARG(pool && slots && out, "null pointer argument");
+  B200KV_CHECK_ARG(!k8 || scales, "8-bit pools need their scales");
+  B200KV_CHECK_ARG(aligned_to(pool, 16) && aligned_to(out, 16), "buffers must be 16-byte aligned");
+  LoadArgs a{};
+  a.pool = pool, a.scales = scales, a.slots = slots, a.out = out;
+  a.num_slots = num_blocks * kPageTokens;
+  a.hkv = static_cast<int>(num_kv_heads);
+  a.error_flag = error_flag;
+  const int64_t rows = num_tokens * num_kv_heads;
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  switch (pool_dtype) {
+    case B200KV_I8: return load_out<B200KV_I8, int8_t, 128>(a, rows, out_dtype, s);
+    case B200KV_E4M3: return load_out<B200KV_E4M3, uint8_t, 128>(a, rows, out_dtype, s);
+    case B200KV_F16:
+      return head_dim == 64 ? load_out<B200KV_F16, __half, 64>(a, rows, out_dtype, s)
+                            : load_out<B200KV_F16, __half, 128>(a, rows, out_dtype, s);
+    default:
+      return head_dim == 64 ? load_out<B200KV_F16, __nv_bfloat16, 64>(a, rows, out_dtype, s)
+                            : load_out<B200KV_F16, __nv_bfloat16, 128>(a, rows, out_dtype, s);
+  }
+}
+
+extern "C" int b200kv_tree_commit(void *k_pool, void *v_pool, int32_t pool_dtype, float *k_scales, float *v_scales,
+                                  const int32_t *block_table, int64_t block_table_stride, const int32_t *context_lens,
+                                  const int32_t *path, int64_t path_stride, const int32_t *path_lens,
+                                  int32_t *new_lens, int64_t batch, int64_t num_kv_heads, int64_t head_dim,
+                                  int64_t num_blocks, int64_t max_blocks_per_seq, int64_t max_path,
+                                  int32_t *error_flag, void *stream) {
+  clear_error();
+  int st = check_cache(pool_dtype, head_dim, "pool");
+  if (st != B200KV_OK) return st;
+  const bool k8 = pool_dtype == B200KV_I8 || pool_dtype == B200KV_E4M3;
+  B200KV_CHECK_ARG(batch >= 0 && batch <= 65535, "batch %lld out of range", (long long)batch);
+  B200KV_CHECK_ARG(num_kv_heads > 0 && num_kv_heads <= 65536 && num_blocks > 0 && num_blocks < (int64_t{1} << 40) &&
+                       max_blocks_per_seq > 0 && max_blocks_per_seq * kPageTokens < (int64_t{1} << 30),
+                   "num_kv_heads, num_blocks or max_blocks_per_seq out of range");
+  B200KV_CHECK_ARG(block_table_stride >= max_blocks_per_seq, "block_table_stride < max_blocks_per_seq");
+  B200KV_CHECK_ARG(max_path >= 0 && max_path < (int64_t{1} << 30) && path_stride >= max_path,
+                   "max_path out of range or path_stride < max_path");
+  if (batch == 0) return B200KV_OK;
+  B200KV_CHECK_ARG(k_pool && v_pool && block_table && context_lens && path_lens && new_lens && (path || max_path == 0),
+                   "null pointer argument");
+  B200KV_CHECK_ARG(!k8 || (k_scales && v_scales), "8-bit pools need k_scales and v_scales");
+  B200KV_CHECK_ARG(aligned_to(k_pool, 16) && aligned_to(v_pool, 16), "pools must be 16-byte aligned");
+  CommitArgs a{};
+  a.pool[0] = k_pool, a.pool[1] = v_pool, a.scales[0] = k_scales, a.scales[1] = v_scales;
+  a.block_table = block_table, a.bt_stride = block_table_stride;
+  a.ctx = context_lens, a.path = path, a.path_stride = path_stride, a.path_lens = path_lens, a.new_lens = new_lens;
+  a.hkv = static_cast<int>(num_kv_heads);
+  a.max_blocks = static_cast<int>(max_blocks_per_seq);
+  a.max_path = static_cast<int>(max_path);
+  a.num_blocks = num_blocks;
+  a.error_flag = error_flag;
+  const dim3 grid(static_cast<unsigned>(2 * num_kv_heads), static_cast<unsigned>(batch));
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (k8)
+    tree_commit_kernel<128, 128, true><<<grid, kCommitThreads, 0, s>>>(a);
+  else if (head_dim == 64)
+    tree_commit_kernel<128, 128, false><<<grid, kCommitThreads, 0, s>>>(a);
+  else
+    tree_commit_kernel<256, 128, false><<<grid, kCommitThreads, 0, s>>>(a);
+  B200KV_CUDA_TRY(cudaGetLastError());
+  return B200KV_OK;
+}
