@@ -34,6 +34,8 @@ SOURCES = [
     "rotary.cu",
     "kv_rows.cu",
     "tree_attention.cu",
+    "tree_mma_f16.cu",
+    "tree_mma_bf16.cu",
     "lse_combine.cu",
     "oproj_allreduce.cu",
 ]
@@ -66,6 +68,7 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         *ARCH_FLAGS,
         "-lineinfo",
         "-O3",
+        "-t0",
         "-std=c++17",
         "--expt-relaxed-constexpr",
         "-Xcompiler",

@@ -5,32 +5,17 @@
 //   out[t, h] = sum_p exp(s_p - m) v_p / sum_p exp(s_p - m),
 //   s_p = scale * q[t, h] . k_p,  m = max_p s_p   over the visible p;
 // a row that sees nothing is zero with lse = -inf.
+//
+// tree_mma.cuh has the kernels; here are the C entries, the masks and the
+// tensor maps.
 #include <cmath>
 
+#include "decode_common.cuh"
 #include "rows.cuh"
+#include "tree_attention.h"
 
 namespace b200kv {
 namespace {
-
-constexpr float kLog2e = 1.44269504088896341f;
-
-struct TreeArgs {
-  const void *q;
-  int64_t q_st, q_sh;
-  const void *k_pool, *v_pool;
-  const float *k_scales, *v_scales;
-  const int32_t *block_table;
-  int64_t bt_stride;
-  const int32_t *ctx, *indptr;
-  const uint64_t *mask;  // [N, words], null: a chain
-  int64_t words;
-  void *out;  // contiguous [N, Hq, D]
-  float *lse;
-  int64_t total_q, num_blocks;
-  int batch, hq, hkv, max_blocks, max_nodes;
-  float scale;
-  int32_t *error_flag;
-};
 
 // ------------------------------------------------------------------- masks --
 __global__ void __launch_bounds__(128) tree_mask_kernel(const int32_t *parents, const int32_t *indptr, int batch,
@@ -65,104 +50,44 @@ __global__ void __launch_bounds__(128) tree_mask_kernel(const int32_t *parents, 
   }
 }
 
-// -------------------------------------------------------------- attention --
-template <typename T, int kCache>
-__device__ __forceinline__ float cache_value(const void *pool, int64_t at) {
-  if constexpr (kCache == B200KV_I8) {
-    return static_cast<float>(static_cast<const int8_t *>(pool)[at]);
-  } else if constexpr (kCache == B200KV_E4M3) {
-    return __half2float(__half(__nv_cvt_fp8_to_halfraw(static_cast<const uint8_t *>(pool)[at], __NV_E4M3)));
-  } else {
-    return to_float(static_cast<const T *>(pool)[at]);
-  }
-}
+// --------------------------------------------------------------------- maps --
+constexpr int kBoxElems = 64;  // 16-bit elements of a 128-byte operand row
 
-// One warp per (node, query head); lane l owns dims l, l + 32, ...
-template <typename T, int D, int kCache>
-__global__ void __launch_bounds__(256) tree_rows_kernel(const TreeArgs a) {
-  constexpr int kStick = kCache == B200KV_F16 ? 64 : 128;
-  constexpr int kPer = D / 32;
-  const int lane = threadIdx.x & 31;
-  const int64_t row = int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  if (row >= a.total_q * a.hq) return;
-  const int64_t t = row / a.hq;
-  const int h = static_cast<int>(row - t * a.hq), kvh = h / (a.hq / a.hkv);
-  int lo = 0, hi = a.batch - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (__ldg(a.indptr + mid) <= t) lo = mid; else hi = mid - 1;
-  }
-  const int b = lo;
-  const int64_t first = __ldg(a.indptr + b);
-  const int cap = a.max_blocks * kPageTokens;
-  int ctx = __ldg(a.ctx + b);
-  int nodes = static_cast<int>(__ldg(a.indptr + b + 1) - first);
-  const int node = static_cast<int>(t - first);
-  if (ctx < 0 || ctx > cap || nodes > a.max_nodes || ctx + nodes > cap || node < 0 || node >= nodes) {
-    if (lane == 0 && a.error_flag) atomicOr(a.error_flag, B200KV_DEVERR_BAD_LEN);
-    ctx = ctx < 0 ? 0 : min(ctx, cap);
-    nodes = max(0, min(min(nodes, a.max_nodes), cap - ctx));
-  }
-  float q[kPer], o[kPer];
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    q[i] = to_float(static_cast<const T *>(a.q)[t * a.q_st + h * a.q_sh + lane + 32 * i]) * (a.scale * kLog2e);
-    o[i] = 0.f;
-  }
-  float m = -CUDART_INF_F, l = 0.f;
-  for (int p = 0; p < ctx + nodes; ++p) {
-    if (p >= ctx) {
-      const int j = p - ctx;
-      const bool see = a.mask ? (j < a.words * 64 && ((__ldg(a.mask + t * a.words + (j >> 6)) >> (j & 63)) & 1)) : j <= node;
-      if (!see) continue;
-    }
-    const int blk = __ldg(a.block_table + b * a.bt_stride + (p >> 6));
-    if (blk < 0 || blk >= a.num_blocks) {
-      if (lane == 0 && a.error_flag) atomicOr(a.error_flag, B200KV_DEVERR_BAD_BLOCK);
-      continue;
-    }
-    const int64_t page = int64_t(blk) * a.hkv + kvh;
-    float s = 0.f;
-    int64_t at[kPer];
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int d = lane + 32 * i;
-      at[i] = (page * (D / kStick) + d / kStick) * (64 * kStick) + int64_t(p & 63) * kStick + d % kStick;
-      s += q[i] * cache_value<T, kCache>(a.k_pool, at[i]);
-    }
-#pragma unroll
-    for (int k = 16; k >= 1; k >>= 1) s += __shfl_xor_sync(0xffffffffu, s, k);
-    float vs = 1.f;
-    if (kCache != B200KV_F16) {
-      s *= __ldg(a.k_scales + page * 64 + (p & 63));
-      vs = __ldg(a.v_scales + page * 64 + (p & 63));
-    }
-    const float mn = fmaxf(m, s);
-    const float keep = exp2f(m - mn), w = exp2f(s - mn);
-    m = mn;
-    l = l * keep + w;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) o[i] = o[i] * keep + w * vs * cache_value<T, kCache>(a.v_pool, at[i]);
-  }
-  const float inv = l > 0.f ? 1.f / l : 0.f;
-  T *out = static_cast<T *>(a.out) + row * D;
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) from_float(out[lane + 32 * i], l == 0.f ? 0.f : o[i] * inv);
-  if (lane == 0 && a.lse) a.lse[row] = l == 0.f ? -CUDART_INF_F : (m + log2f(l)) / kLog2e;
-}
-
-template <typename T, int D, int kCache>
-int launch_tree(const TreeArgs &a, cudaStream_t s) {
-  const int64_t blocks = (a.total_q * a.hq + 7) / 8;
-  tree_rows_kernel<T, D, kCache><<<static_cast<unsigned>(blocks), 256, 0, s>>>(a);
-  B200KV_CUDA_TRY(cudaGetLastError());
+int encode(CUtensorMap *map, CUtensorMapDataType type, const void *base, const cuuint64_t (&dims)[3],
+           const cuuint64_t (&strides)[2], const cuuint32_t (&box)[3], CUtensorMapSwizzle swizzle) {
+  EncodeTiledFn enc = encode_tiled_fn();
+  if (!enc) return set_error(B200KV_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
+  const cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r = enc(map, type, 3, const_cast<void *>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return set_error(B200KV_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", static_cast<int>(r));
   return B200KV_OK;
 }
-template <typename T>
-int tree_cache(const TreeArgs &a, int64_t dim, int cache, cudaStream_t s) {
-  if (cache == B200KV_I8) return launch_tree<T, 128, B200KV_I8>(a, s);
-  if (cache == B200KV_E4M3) return launch_tree<T, 128, B200KV_E4M3>(a, s);
-  return dim == 64 ? launch_tree<T, 64, B200KV_F16>(a, s) : launch_tree<T, 128, B200KV_F16>(a, s);
+
+// Pages of a pool, one box per page and 64-element stick column (16-bit: into
+// the 128-byte swizzle of an operand tile) or per page (8-bit: as it is).
+int pool_map(CUtensorMap *map, const void *pool, int64_t pages, int64_t dim, bool k8, CUtensorMapDataType type) {
+  const cuuint64_t stick = k8 ? 128 : 64, rows = k8 ? kPageTokens : dim / 64 * kPageTokens;
+  const cuuint64_t dims[3] = {stick, rows, static_cast<cuuint64_t>(pages)};
+  const cuuint64_t strides[2] = {128, rows * 128};
+  const cuuint32_t box[3] = {static_cast<cuuint32_t>(stick), kPageTokens, 1};
+  return encode(map, k8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : type, pool, dims, strides, box,
+                k8 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+struct Workspace {
+  int64_t joins, ml, o, total;
+};
+// After the decode kernels' counters, which calls on a shared workspace find as
+// they left them.
+Workspace workspace_of(int64_t dim) {
+  auto up = [](int64_t x) { return (x + 255) & ~int64_t(255); };
+  Workspace w;
+  w.joins = kMaxCounters * 4;
+  w.ml = up(w.joins + tree::kMaxCtas * static_cast<int64_t>(sizeof(tree::Join)));
+  w.o = up(w.ml + 2 * tree::kMaxCtas * 256 * 8);
+  w.total = up(w.o + 2 * tree::kMaxCtas * 256 * dim * 4);
+  return w;
 }
 
 }  // namespace
@@ -175,7 +100,7 @@ extern "C" int64_t b200kv_tree_workspace_bytes(int64_t total_q, int64_t batch, i
   if (total_q < 0 || batch < 0 || num_q_heads <= 0 || num_kv_heads <= 0 || num_q_heads % num_kv_heads != 0 ||
       (head_dim != 64 && head_dim != 128))
     return -1;
-  return 256;
+  return workspace_of(head_dim).total;
 }
 
 extern "C" int b200kv_tree_mask(const int32_t *parents, const int32_t *q_indptr, int64_t batch, int64_t total_q,
@@ -230,26 +155,60 @@ extern "C" int b200kv_tree_attention(const void *q, int32_t q_dtype, int64_t q_s
   B200KV_CHECK_ARG(batch > 0, "nodes without a sequence");
   B200KV_CHECK_ARG(q && k_pool && v_pool && block_table && context_lens && q_indptr && out, "null pointer argument");
   B200KV_CHECK_ARG(!k8 || (k_scales && v_scales), "8-bit pools need k_scales and v_scales");
-  B200KV_CHECK_ARG(aligned_to(q, 16) && q_stride_t % 8 == 0 && q_stride_h % 8 == 0 && q_stride_t > 0 && q_stride_h > 0,
+  B200KV_CHECK_ARG(!k8 || (aligned_to(k_scales, 16) && aligned_to(v_scales, 16)), "scales must be 16-byte aligned");
+  B200KV_CHECK_ARG(aligned_to(q, 16) && (total_q == 1 || (q_stride_t % 8 == 0 && q_stride_t > 0)) &&
+                       (num_q_heads == 1 || (q_stride_h % 8 == 0 && q_stride_h > 0)),
                    "q must be 16-byte aligned with positive strides that are multiples of 8 elements");
   B200KV_CHECK_ARG(aligned_to(k_pool, 16) && aligned_to(v_pool, 16) && aligned_to(out, 16), "pools and out must be 16-byte aligned");
   const int64_t need = b200kv_tree_workspace_bytes(total_q, batch, num_q_heads, num_kv_heads, head_dim);
   if (!workspace || workspace_bytes < need)
     return set_error(B200KV_ERR_WORKSPACE, "workspace of %lld bytes required (got %lld)", (long long)need,
                      (long long)workspace_bytes);
-  TreeArgs a{};
-  a.q = q, a.q_st = q_stride_t, a.q_sh = q_stride_h;
-  a.k_pool = k_pool, a.v_pool = v_pool, a.k_scales = k_scales, a.v_scales = v_scales;
+  if ((reinterpret_cast<uintptr_t>(workspace) & 255u) != 0)
+    return set_error(B200KV_ERR_WORKSPACE, "workspace must be 256-byte aligned");
+  int dev = 0, sms = 0;
+  int st = current_device_sm_count(&dev, &sms);
+  if (st != B200KV_OK) return st;
+  const int group = static_cast<int>(num_q_heads / num_kv_heads);
+  tree::Args a{};
   a.block_table = block_table, a.bt_stride = block_table_stride;
   a.ctx = context_lens, a.indptr = q_indptr;
   a.mask = reinterpret_cast<const uint64_t *>(tree_mask), a.words = mask_words;
+  a.k_scales = k_scales, a.v_scales = v_scales, a.v_pool = v_pool;
   a.out = out, a.lse = lse;
-  a.total_q = total_q, a.num_blocks = num_blocks;
-  a.batch = static_cast<int>(batch), a.hq = static_cast<int>(num_q_heads), a.hkv = static_cast<int>(num_kv_heads);
+  a.total_q = static_cast<int>(total_q), a.batch = static_cast<int>(batch);
+  a.hq = static_cast<int>(num_q_heads), a.hkv = static_cast<int>(num_kv_heads), a.group = group;
   a.max_blocks = static_cast<int>(max_blocks_per_seq), a.max_nodes = static_cast<int>(max_nodes);
+  a.num_blocks = static_cast<int>(num_blocks);
+  a.tile_nodes = 128 / group;
+  a.most_rows = max_nodes > a.tile_nodes ? 256 : 128;
   a.scale = scale;
   a.error_flag = error_flag;
+  const Workspace ws = workspace_of(head_dim);
+  uint8_t *base = static_cast<uint8_t *>(workspace);
+  a.joins = reinterpret_cast<tree::Join *>(base + ws.joins);
+  a.part_ml = reinterpret_cast<float2 *>(base + ws.ml);
+  a.part_o = reinterpret_cast<float *>(base + ws.o);
+
+  const CUtensorMapDataType type = q_dtype == B200KV_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  // Q: 64 elements x the KV head's query heads x the nodes of a tile (no more
+  // than a sequence can have), rows node-major
+  const int64_t box_nodes = max_nodes < a.tile_nodes ? max_nodes : a.tile_nodes;
+  a.q_box_bytes = static_cast<uint32_t>(box_nodes * group * 128);
+  CUtensorMap qm, km, vm;
+  // a dimension of one element may have any stride
+  const int64_t qs_h = num_q_heads == 1 ? head_dim : q_stride_h, qs_t = total_q == 1 ? num_q_heads * head_dim : q_stride_t;
+  st = encode(&qm, type, q,
+              {static_cast<cuuint64_t>(head_dim), static_cast<cuuint64_t>(num_q_heads), static_cast<cuuint64_t>(total_q)},
+              {static_cast<cuuint64_t>(qs_h * 2), static_cast<cuuint64_t>(qs_t * 2)},
+              {kBoxElems, static_cast<cuuint32_t>(group), static_cast<cuuint32_t>(box_nodes)}, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (st != B200KV_OK) return st;
+  st = pool_map(&km, k_pool, num_blocks * num_kv_heads, head_dim, k8, type);
+  if (st != B200KV_OK) return st;
+  st = pool_map(&vm, v_pool, num_blocks * num_kv_heads, head_dim, k8, type);
+  if (st != B200KV_OK) return st;
+  const int ctas = sms < tree::kMaxCtas ? sms : tree::kMaxCtas;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return q_dtype == B200KV_F16 ? tree_cache<__half>(a, head_dim, pool_dtype, s)
-                               : tree_cache<__nv_bfloat16>(a, head_dim, pool_dtype, s);
+  return q_dtype == B200KV_F16 ? tree::launch_f16(qm, km, vm, a, static_cast<int>(head_dim), pool_dtype, ctas, s)
+                               : tree::launch_bf16(qm, km, vm, a, static_cast<int>(head_dim), pool_dtype, ctas, s);
 }

@@ -1,0 +1,1063 @@
+// Tensor-core kernel of tree attention (tree_attention.cu has the operator).
+//
+// Rows: the nodes of a sequence and the G = Hq / Hkv query heads of a KV head
+// are the rows of one matrix (node-major, so row = node * G + head), cut into Q
+// tiles of floor(128 / G) nodes.  Two consecutive Q tiles of the same sequence
+// and KV head form a block; a block's cached tokens are cut into tiles of 128
+// (two pages).  The blocks' tiles, all sequences and KV heads one after the
+// other, form one line that is cut into equal shares, one per CTA; a block cut
+// by a share's end is joined by tree_join_kernel.
+//
+// Inside a CTA two streams run side by side, each with its own warpgroup, score
+// buffer S and accumulator O in TMEM.  A block of two Q tiles gives each stream
+// one of them, both over every token tile; a block of one Q tile (the usual
+// draft) gives the streams alternate token tiles, and their two states are
+// merged when the block ends.  Per tile: S = Q K^T (tcgen05.mma, fp32), the
+// warpgroup (thread = row) masks and exponentiates, P goes back into S's TMEM
+// columns in 16 bits, O += P V with P as the TMEM operand.  While one stream's
+// warpgroup works on its scores the tensor pipe works for the other.  O is only
+// rescaled when a row's maximum has risen by more than 2^8 (weights then stay
+// below 2^8, far from fp16's range), so most tiles touch it in the MMA alone.
+//
+// Bound: with up to 128 rows a 128-token tile costs the tensor pipe 0.55 us
+// (2 x 128^3 products at 8192 FLOP per clock) and HBM 1.5 us per SM, so drafts
+// run at the cache's bandwidth; blocks of two Q tiles are bound by the tensor
+// pipe and the exponentials (16 per clock and SM, as long as the products).
+//
+// Warps: 0-3 and 4-7 the two softmax warpgroups, 8 the TMA producer, 9 the MMA
+// issuer (owns the TMEM), 8-bit caches: 10-13 converters, which turn 8-bit
+// pages into 16-bit operand tiles (K as its exact steps, its scales multiply
+// the scores; V times its scale, rounded to the compute type).
+#pragma once
+
+#include <type_traits>
+
+#include "rows.cuh"
+#include "tree_attention.h"
+
+namespace b200kv {
+namespace tree {
+
+constexpr int kTileRows = 128, kTileTokens = 128;
+constexpr float kLazyLog2 = 8.f;
+
+template <typename T, int D, int kCache>
+struct Cfg {
+  static constexpr bool k8 = kCache != B200KV_F16;
+  static constexpr int kThreads = k8 ? 448 : 320;
+  static constexpr int kSticks = D / 64;
+  static constexpr int kStickTile = kTileTokens * 128;      // one 64-element column of 128 rows
+  static constexpr int kTile = kSticks * kStickTile;        // a Q, K or V tile
+  static constexpr int kSlots = k8 ? 3 : (D == 64 ? 8 : 5);  // operand tiles in flight
+  static constexpr int kRaw = k8 ? 7 : 0;                   // 8-bit pages in flight
+  static constexpr int kRawPage = kPageTokens * 128;
+  static constexpr int kRawScales = kPageTokens * 4;
+  static constexpr int kCtrl = k8 ? 8192 : 3072;
+  static constexpr int kOffQ = kCtrl;
+  static constexpr int kOffSlots = kOffQ + 2 * kTile;
+  static constexpr int kOffRaw = kOffSlots + kSlots * kTile;
+  static constexpr int kOffRawScales = kOffRaw + kRaw * kRawPage;
+  static constexpr int kSmem = kOffRawScales + kRaw * kRawScales;
+  static constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+  // kind::f16: fp32 accumulator, A and B both fp16 or both bf16, M = 128
+  static constexpr uint32_t kIdesc = (1u << 4) | (kBf16 ? (1u << 7) | (1u << 10) : 0u) | (uint32_t(kTileRows >> 4) << 24);
+  static constexpr uint32_t kIdescQK = kIdesc | (uint32_t(kTileTokens >> 3) << 17);
+  static constexpr uint32_t kIdescPV = kIdesc | (1u << 16) | (uint32_t(D >> 3) << 17);  // V: N-major
+  static_assert(kSmem <= 227 * 1024, "shared memory per CTA");
+};
+
+// TMEM columns
+constexpr uint32_t kTmemCols = 512;
+__device__ __forceinline__ uint32_t col_s(int w) { return uint32_t(w) * 128u; }
+__device__ __forceinline__ uint32_t col_o(int w) { return 256u + uint32_t(w) * 128u; }
+
+struct Ctrl {
+  uint64_t full[8], empty[8];          // operand tiles
+  uint64_t raw_full[8], raw_empty[8];  // 8-bit pages
+  uint64_t q_full, q_empty;
+  uint64_t s_full[2], p_ready[2], o_full[2];
+  uint32_t tmem;
+  int start_b;
+  long long start_rem, per, total;
+  long long scan[16];
+  int raw_rows[8];
+  unsigned bad_piece;       // last piece (counted from 1) that met a non-finite value in a node's V row
+  float2 ml[2][kTileRows];  // (maximum, sum) of the streams' rows
+};
+constexpr int kOffKScale = 3072;  // 8-bit caches: [8 warps][128] score factors of a tile
+static_assert(sizeof(Ctrl) <= kOffKScale, "control block");
+
+// ------------------------------------------------------------------- waits --
+// Bounded: after kWaitLimitNs the error flag is set and this thread waits no
+// more (its later waits return at once), so a lost transfer ends the kernel.
+__device__ __forceinline__ void wait(uint64_t *bar, uint32_t parity, bool &dead, int32_t *flag) {
+  if (mbar_try_wait(bar, parity) || dead) return;
+  const uint64_t t0 = global_timer_ns();
+  for (uint32_t i = 1;; ++i) {
+    if (mbar_try_wait(bar, parity)) return;
+    if ((i & 255u) == 0 && global_timer_ns() - t0 > kWaitLimitNs) break;
+  }
+  dead = true;
+  if (flag) atomicOr(flag, B200KV_DEVERR_TIMEOUT);
+}
+__device__ __forceinline__ void arrive(uint64_t *bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void commit(uint64_t *bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
+               : "memory");
+}
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void bar_pair() { asm volatile("bar.sync 1, 256;" ::: "memory"); }  // both warpgroups
+
+// -------------------------------------------------------------- TMEM moves --
+#define B200KV_R8(r, i) "=r"(r[i]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3]), "=r"(r[i + 4]), "=r"(r[i + 5]), \
+                        "=r"(r[i + 6]), "=r"(r[i + 7])
+#define B200KV_W8(r, i) "r"(r[i]), "r"(r[i + 1]), "r"(r[i + 2]), "r"(r[i + 3]), "r"(r[i + 4]), "r"(r[i + 5]), \
+                        "r"(r[i + 6]), "r"(r[i + 7])
+__device__ __forceinline__ void tmem_ld32(uint32_t at, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
+      "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : B200KV_R8(r, 0), B200KV_R8(r, 8), B200KV_R8(r, 16), B200KV_R8(r, 24)
+      : "r"(at));
+}
+#define B200KV_RW8(r, i) "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]), \
+                         "+r"(r[i + 6]), "+r"(r[i + 7])
+// The loaded registers go through the wait, so that no use of them is moved before it.
+__device__ __forceinline__ void wait_ld(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : B200KV_RW8(r, 0), B200KV_RW8(r, 8), B200KV_RW8(r, 16), B200KV_RW8(r, 24)::"memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t at, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
+      "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(at),
+      B200KV_W8(r, 0), B200KV_W8(r, 8), B200KV_W8(r, 16), B200KV_W8(r, 24)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(at),
+      B200KV_W8(r, 0), B200KV_W8(r, 8)
+      : "memory");
+}
+
+// ---------------------------------------------------------------- operands --
+// 128-byte swizzle, descriptor version 1.  K-major (Q, K): rows of 128 bytes,
+// groups of 8 rows 1024 bytes apart.  N-major (V): 64 head elements of a token
+// are 128 contiguous bytes; groups of 8 tokens 1024 bytes apart, the next 64
+// elements one stick column (128 tokens) on.
+__device__ __forceinline__ uint64_t desc_kmajor(uint32_t addr) {
+  return static_cast<uint64_t>((addr >> 4) & 0x3FFFu) | (uint64_t(1) << 16) | (uint64_t(1024 >> 4) << 32) |
+         (uint64_t(1) << 46) | (uint64_t(2) << 61);
+}
+__device__ __forceinline__ uint64_t desc_nmajor(uint32_t addr) {
+  return static_cast<uint64_t>((addr >> 4) & 0x3FFFu) | (uint64_t((kTileTokens * 128) >> 4) << 16) |
+         (uint64_t(1024 >> 4) << 32) | (uint64_t(1) << 46) | (uint64_t(2) << 61);
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+
+// -------------------------------------------------------------------- plan --
+struct Seq {
+  int ctx, nodes, q0, blocks, qtiles;
+};
+__device__ __forceinline__ Seq load_seq(const Args &a, int b, bool report) {
+  const int cap = a.max_blocks * kPageTokens;
+  Seq s;
+  s.ctx = __ldg(a.ctx + b);
+  s.q0 = __ldg(a.indptr + b);
+  const int end = __ldg(a.indptr + b + 1);
+  bool bad = s.ctx < 0 || s.ctx > cap || s.q0 < 0 || end < s.q0 || end > a.total_q || (b == 0 && s.q0 != 0) ||
+             (b == a.batch - 1 && end != a.total_q);
+  s.ctx = min(max(s.ctx, 0), cap);
+  s.q0 = min(max(s.q0, 0), a.total_q);
+  s.nodes = min(max(end, s.q0), a.total_q) - s.q0;
+  const int most = min(a.max_nodes, cap - s.ctx);
+  bad = bad || s.nodes > most;
+  s.nodes = min(s.nodes, most);
+  if (bad && report && a.error_flag) atomicOr(a.error_flag, B200KV_DEVERR_BAD_LEN);
+  s.qtiles = (s.nodes + a.tile_nodes - 1) / a.tile_nodes;
+  s.blocks = (s.qtiles + 1) >> 1;
+  return s;
+}
+// Token tiles of block k: what its last node can see.
+__device__ __forceinline__ int block_tiles(const Args &a, const Seq &s, int k) {
+  const int nodes = a.mask ? s.nodes : min(s.nodes, (2 * k + 2) * a.tile_nodes);
+  return (s.ctx + nodes + kTileTokens - 1) / kTileTokens;
+}
+__device__ __forceinline__ long long head_units(const Args &a, const Seq &s) {
+  if (a.mask) return static_cast<long long>(s.blocks) * (s.blocks ? block_tiles(a, s, 0) : 0);
+  long long n = 0;
+  for (int k = 0; k < s.blocks; ++k) n += block_tiles(a, s, k);
+  return n;
+}
+
+// The blocks of a CTA's share, one piece (a block, or the part of it in this
+// share) at a time.  Every role walks the same sequence.
+struct Walk {
+  Seq s;
+  int b, kvh, block, tiles, t0, t1;  // piece: token tiles [t0, t1) of `tiles`
+  int next_tile;
+  long long left;
+
+  __device__ __forceinline__ void init(const Args &a, const Ctrl &c) {
+    b = c.start_b;
+    left = min(c.per, c.total - static_cast<long long>(blockIdx.x) * c.per);
+    if (left <= 0) return;
+    s = load_seq(a, b, false);
+    const long long hu = head_units(a, s);
+    kvh = static_cast<int>(c.start_rem / hu);
+    long long rem = c.start_rem - kvh * hu;
+    block = 0;
+    if (a.mask) {
+      tiles = block_tiles(a, s, 0);
+      block = static_cast<int>(rem / tiles);
+      rem -= static_cast<long long>(block) * tiles;
+    } else {
+      while (rem >= (tiles = block_tiles(a, s, block))) rem -= tiles, ++block;
+    }
+    next_tile = static_cast<int>(rem);
+  }
+  // The next piece, false when the share is done.
+  __device__ __forceinline__ bool next(const Args &a) {
+    if (left <= 0) return false;
+    t0 = next_tile;
+    t1 = static_cast<int>(min(static_cast<long long>(tiles), t0 + left));
+    left -= t1 - t0;
+    return true;
+  }
+  __device__ __forceinline__ void advance(const Args &a) {
+    next_tile = 0;
+    if (left <= 0) return;
+    if (++block >= s.blocks) {
+      block = 0;
+      if (++kvh >= a.hkv) {
+        kvh = 0;
+        do s = load_seq(a, ++b, false);
+        while (s.nodes == 0);
+      }
+    }
+    tiles = block_tiles(a, s, block);
+  }
+  __device__ __forceinline__ bool two() const { return 2 * block + 1 < s.qtiles; }
+};
+
+// First unit, share and total of the line; all threads of the CTA call it.
+template <int kThreads>
+__device__ __forceinline__ void make_plan(const Args &a, Ctrl &c) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int each = (a.batch + kThreads - 1) / kThreads;
+  const int b0 = tid * each, b1 = min(b0 + each, a.batch);
+  long long mine = 0;
+  for (int b = b0; b < b1; ++b) mine += head_units(a, load_seq(a, b, blockIdx.x == 0)) * a.hkv;
+  long long incl = mine;
+#pragma unroll
+  for (int m = 1; m < 32; m <<= 1) {
+    const long long y = __shfl_up_sync(0xffffffffu, incl, m);
+    if (lane >= m) incl += y;
+  }
+  if (lane == 31) c.scan[warp] = incl;
+  __syncthreads();
+  long long total = 0, before = 0;
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) {
+    if (w < warp) before += c.scan[w];
+    total += c.scan[w];
+  }
+  const long long per = (total + gridDim.x - 1) / gridDim.x;
+  const long long first = static_cast<long long>(blockIdx.x) * per;
+  long long at = before + incl - mine;
+  if (first >= at && first < at + mine) {
+    for (int b = b0; b < b1; ++b) {
+      const long long n = head_units(a, load_seq(a, b, false)) * a.hkv;
+      if (first < at + n) {
+        c.start_b = b;
+        c.start_rem = first - at;
+        break;
+      }
+      at += n;
+    }
+  }
+  if (tid == 0) {
+    c.per = per;
+    c.total = total;
+  }
+}
+
+// Page ids of a sequence, 32 at a time in a warp's lanes.  Invalid ids are
+// flagged and become -1.
+__device__ __forceinline__ int load_ids(const Args &a, int b, int window, int pages) {
+  const int p = window * 32 + (threadIdx.x & 31);
+  if (p >= pages) return -1;
+  const int id = __ldg(a.block_table + static_cast<int64_t>(b) * a.bt_stride + p);
+  if (id < 0 || id >= a.num_blocks) {
+    if (a.error_flag) atomicOr(a.error_flag, B200KV_DEVERR_BAD_BLOCK);
+    return -1;
+  }
+  return id;
+}
+
+__device__ __forceinline__ void tma_3d(void *dst, const CUtensorMap *map, uint64_t *bar, int c0, int c1, int c2) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], "
+      "[%2];" ::"r"(smem_u32(dst)),
+      "l"(map), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
+      : "memory");
+}
+
+// ------------------------------------------------------------------ roles --
+template <typename C>
+__device__ __forceinline__ void producer(const Args &a, Ctrl &c, uint8_t *smem, const CUtensorMap *qm,
+                                         const CUtensorMap *km, const CUtensorMap *vm) {
+  const int lane = threadIdx.x & 31;
+  const uint64_t policy = l2_policy_evict_first();
+  bool dead = false;
+  uint32_t slot = 0, ring = 0, pieces = 0;  // tiles (16-bit) or pages (8-bit) issued, pieces begun
+  Walk w;
+  w.init(a, c);
+  while (w.next(a)) {
+    const bool two = w.two();
+    const int pages = (w.s.ctx + w.s.nodes + kPageTokens - 1) / kPageTokens;
+    if (lane == 0) {
+      wait(&c.q_empty, (pieces & 1u) ^ 1u, dead, a.error_flag);
+      mbar_arrive_expect_tx(&c.q_full, (two ? 2u : 1u) * C::kSticks * a.q_box_bytes);
+      for (int i = 0; i < (two ? 2 : 1); ++i)
+        for (int st = 0; st < C::kSticks; ++st)
+          tma_3d(smem + C::kOffQ + i * C::kTile + st * C::kStickTile, qm, &c.q_full, st * 64, w.kvh * a.group,
+                 w.s.q0 + (2 * w.block + i) * a.tile_nodes);
+    }
+    ++pieces;
+    int window = w.t0 / 16, ids = load_ids(a, w.b, window, pages), ids_next = load_ids(a, w.b, window + 1, pages);
+    int ids_before = ids;
+    auto issue = [&](bool is_v, int t) {
+      if (t / 16 > window) {  // K leads, V follows by at most two tiles
+        ids_before = ids;
+        ids = ids_next;
+        ids_next = load_ids(a, w.b, ++window + 1, pages);
+      }
+      const int have = t / 16 == window ? ids : ids_before;
+      const int id0 = __shfl_sync(0xffffffffu, have, (2 * t) & 31), id1 = __shfl_sync(0xffffffffu, have, (2 * t + 1) & 31);
+      const int n = min(2, pages - 2 * t);
+      const CUtensorMap *map = is_v ? vm : km;
+      if constexpr (!C::k8) {
+        if (lane == 0) {
+          const uint32_t s = slot % C::kSlots;
+          wait(&c.empty[s], ((slot / C::kSlots) & 1u) ^ 1u, dead, a.error_flag);
+          mbar_arrive_expect_tx(&c.full[s], uint32_t(n) * C::kSticks * (kPageTokens * 128));
+          uint8_t *dst = smem + C::kOffSlots + s * C::kTile;
+          for (int i = 0; i < n; ++i) {
+            const int id = i ? id1 : id0;
+            // an invalid id reads past the last page: zeros
+            const int page = id < 0 ? a.num_blocks * a.hkv : id * a.hkv + w.kvh;
+            for (int st = 0; st < C::kSticks; ++st)
+              tma_load_3d(dst + st * C::kStickTile + i * (kPageTokens * 128), map, &c.full[s], 0, st * kPageTokens, page,
+                          policy);
+          }
+        }
+        ++slot;
+      } else {
+        for (int i = 0; i < n; ++i) {
+          if (lane == 0) {
+            const uint32_t r = ring % C::kRaw;
+            wait(&c.raw_empty[r], ((ring / C::kRaw) & 1u) ^ 1u, dead, a.error_flag);
+            const int id = i ? id1 : id0;
+            // rows past the context, and whole pages with an invalid id, count as zeros
+            c.raw_rows[r] = id < 0 ? 0 : min(kPageTokens, w.s.ctx + w.s.nodes - (2 * t + i) * kPageTokens);
+            if (id < 0) {
+              arrive(&c.raw_full[r]);
+            } else {
+              const int page = id * a.hkv + w.kvh;
+              mbar_arrive_expect_tx(&c.raw_full[r], C::kRawPage + (is_v ? C::kRawScales : 0));
+              tma_load_3d(smem + C::kOffRaw + r * C::kRawPage, map, &c.raw_full[r], 0, 0, page, policy);
+              if (is_v)
+                bulk_load(smem + C::kOffRawScales + r * C::kRawScales, a.v_scales + static_cast<int64_t>(page) * kPageTokens,
+                          C::kRawScales, &c.raw_full[r]);
+            }
+          }
+          ++ring;
+        }
+      }
+    };
+    // K leads V by one tile per stream that needs it: the order the MMA warp
+    // consumes them in
+    const int lead = two ? 1 : 2;
+    for (int t = w.t0; t < min(w.t0 + lead, w.t1); ++t) issue(false, t);
+    for (int t = w.t0; t < w.t1; ++t) {
+      issue(true, t);
+      if (t + lead < w.t1) issue(false, t + lead);
+    }
+    w.advance(a);
+  }
+  // the last arrival that the MMAs owe this CTA: not before it may the CTA end
+  if (lane == 0 && pieces > 0) wait(&c.q_empty, (pieces & 1u) ^ 1u, dead, a.error_flag);
+  __syncwarp();
+}
+
+// Non-finite values of drafted nodes.  A weight of zero does not keep an inf or
+// NaN of V out of a matrix product, and a node may be hidden from some rows of
+// a tile only.  So the nodes' V rows are looked through in shared memory:
+// non-finite elements become zeros there, and when the block ends the rows that
+// see such a node get its elements added from the cache (non_finite_sum).
+template <typename T>
+__device__ __forceinline__ uint32_t drop_non_finite(uint32_t w) {
+  constexpr uint32_t e = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+  if ((w & e) == e) w &= 0xffff0000u;
+  if ((w & (e << 16)) == (e << 16)) w &= 0xffffu;
+  return w;
+}
+template <typename T>
+__device__ __forceinline__ bool drop_non_finite(uint4 &v) {
+  const uint4 x = make_uint4(drop_non_finite<T>(v.x), drop_non_finite<T>(v.y), drop_non_finite<T>(v.z),
+                             drop_non_finite<T>(v.w));
+  const bool hit = x.x != v.x || x.y != v.y || x.z != v.z || x.w != v.w;
+  v = x;
+  return hit;
+}
+
+// Eight-bit pages -> operand tiles.  Thread: 16 bytes of a row, 4 rows per
+// warp and step; the two 16-byte results of lanes 4-7 of a row are written in
+// swapped order so that the eight lanes of a row hit eight different 16-byte
+// bank groups in the swizzled tile.
+template <typename T, int kCache>
+__device__ __forceinline__ void widen16(uint4 v, float scale, bool scaled, uint4 &lo, uint4 &hi) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  uint32_t o[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float f[4];
+    if constexpr (kCache == B200KV_I8) {
+      // 2^23 + 128 + b as a float: b's byte, its sign bit flipped, under 0x4B0000
+      const uint32_t u = w[i] ^ 0x80808080u;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        f[j] = __fadd_rn(__uint_as_float(__byte_perm(u, 0x4B000000u, 0x7540 | j)), -8388736.f);
+    } else {
+      const __half2_raw a = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w[i] & 0xffffu), __NV_E4M3);
+      const __half2_raw b = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w[i] >> 16), __NV_E4M3);
+      const float2 fa = __half22float2(__half2(a)), fb = __half22float2(__half2(b));
+      f[0] = fa.x, f[1] = fa.y, f[2] = fb.x, f[3] = fb.y;
+    }
+    if (scaled) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) f[j] *= scale;
+    }
+    o[2 * i] = pack2(f[0], f[1], T());
+    o[2 * i + 1] = pack2(f[2], f[3], T());
+  }
+  lo = make_uint4(o[0], o[1], o[2], o[3]);
+  hi = make_uint4(o[4], o[5], o[6], o[7]);
+}
+
+template <typename C, typename T, int kCache>
+__device__ __forceinline__ void converter(const Args &a, Ctrl &c, uint8_t *smem, int warp) {
+  const int lane = threadIdx.x & 31, sub = lane & 7;
+  bool dead = false;
+  uint32_t slot = 0, ring = 0;
+  unsigned piece = 0;
+  auto tile = [&](bool is_v, int t, int pages, int ctx) {
+    const uint32_t s = slot % C::kSlots;
+    wait(&c.empty[s], ((slot / C::kSlots) & 1u) ^ 1u, dead, a.error_flag);
+    uint8_t *dst = smem + C::kOffSlots + s * C::kTile + (sub >> 2) * C::kStickTile;
+    for (int i = 0; i < 2; ++i) {
+      const bool page = 2 * t + i < pages;
+      const uint32_t r = ring % C::kRaw;
+      int rows = 0;
+      if (page) {
+        wait(&c.raw_full[r], (ring / C::kRaw) & 1u, dead, a.error_flag);
+        rows = c.raw_rows[r];
+      }
+      const uint8_t *src = smem + C::kOffRaw + r * C::kRawPage;
+      const float *scales = reinterpret_cast<const float *>(smem + C::kOffRawScales + r * C::kRawScales);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int row = warp * 16 + k * 4 + (lane >> 3), trow = i * kPageTokens + row;
+        uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
+        if (row < rows) {
+          widen16<T, kCache>(*reinterpret_cast<const uint4 *>(src + row * 128 + sub * 16), is_v ? scales[row] : 1.f, is_v,
+                             lo, hi);
+          if (is_v && t * kTileTokens + trow >= ctx) {  // a node's row
+            const bool hit = drop_non_finite<T>(lo);
+            if (drop_non_finite<T>(hi) || hit) atomicMax(&c.bad_piece, piece);
+          }
+        }
+        const int c0 = (sub & 3) * 2, first = sub >> 2;  // lanes 4-7 write their second half first
+        uint8_t *line = dst + trow * 128;
+        *reinterpret_cast<uint4 *>(line + (((c0 + first) ^ (trow & 7)) << 4)) = first ? hi : lo;
+        *reinterpret_cast<uint4 *>(line + (((c0 + 1 - first) ^ (trow & 7)) << 4)) = first ? lo : hi;
+      }
+      if (page) {
+        __syncwarp();
+        if (lane == 0) arrive(&c.raw_empty[r]);
+        ++ring;
+      }
+    }
+    fence_async_smem();
+    __syncwarp();
+    if (lane == 0) arrive(&c.full[s]);
+    ++slot;
+  };
+  Walk w;
+  w.init(a, c);
+  while (w.next(a)) {
+    ++piece;
+    const int pages = (w.s.ctx + w.s.nodes + kPageTokens - 1) / kPageTokens;
+    const int lead = w.two() ? 1 : 2;
+    for (int t = w.t0; t < min(w.t0 + lead, w.t1); ++t) tile(false, t, pages, w.s.ctx);
+    for (int t = w.t0; t < w.t1; ++t) {
+      tile(true, t, pages, w.s.ctx);
+      if (t + lead < w.t1) tile(false, t + lead, pages, w.s.ctx);
+    }
+    w.advance(a);
+  }
+}
+
+// One thread issues every MMA.
+template <typename C, int D>
+__device__ __forceinline__ void mma_issuer(const Args &a, Ctrl &c, uint8_t *smem, uint32_t tmem) {
+  bool dead = false;
+  uint32_t slot = 0, pieces = 0, p_uses[2] = {0, 0};
+  const uint32_t qbase = smem_u32(smem + C::kOffQ), sbase = smem_u32(smem + C::kOffSlots);
+  const uint32_t negate = a.scale < 0.f ? 1u << 13 : 0u;  // a negative scale turns Q's sign
+  auto ready = [&](uint32_t n) {
+    wait(&c.full[n % C::kSlots], (n / C::kSlots) & 1u, dead, a.error_flag);
+    fence_after();
+    return sbase + (n % C::kSlots) * C::kTile;
+  };
+  auto qk = [&](int w, int qtile, uint32_t k) {
+    const uint32_t q = qbase + qtile * C::kTile;
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) {
+      const uint32_t off = (i >> 2) * C::kStickTile + (i & 3) * 32;
+      mma_ss(tmem + col_s(w), desc_kmajor(q + off), desc_kmajor(k + off), C::kIdescQK | negate, i > 0);
+    }
+    commit(&c.s_full[w]);
+  };
+  auto pv = [&](int w, uint32_t v, bool first) {
+    wait(&c.p_ready[w], p_uses[w]++ & 1u, dead, a.error_flag);
+    fence_after();
+#pragma unroll
+    for (int i = 0; i < kTileTokens / 16; ++i)
+      mma_ts(tmem + col_o(w), tmem + col_s(w) + i * 8, desc_nmajor(v + i * 2048), C::kIdescPV, !first || i > 0);
+  };
+  Walk w;
+  w.init(a, c);
+  while (w.next(a)) {
+    wait(&c.q_full, pieces++ & 1u, dead, a.error_flag);
+    fence_after();
+    const int n = w.t1 - w.t0;
+    if (w.two()) {
+      // both streams over every tile; a slot is free when the second has used it
+      uint32_t k = ready(slot);
+      qk(0, 0, k);
+      qk(1, 1, k);
+      commit(&c.empty[slot++ % C::kSlots]);
+      for (int t = 0; t < n; ++t) {
+        const uint32_t vs = slot++, v = ready(vs);
+        const bool more = t + 1 < n;
+        pv(0, v, t == 0);
+        if (more)
+          qk(0, 0, k = ready(slot));
+        else
+          commit(&c.o_full[0]);
+        pv(1, v, t == 0);
+        commit(&c.empty[vs % C::kSlots]);
+        if (more) {
+          qk(1, 1, k);
+          commit(&c.empty[slot++ % C::kSlots]);
+        } else {
+          commit(&c.o_full[1]);
+        }
+      }
+    } else {
+      // stream t & 1 takes tile t
+      for (int t = 0; t < min(2, n); ++t) {
+        qk(t & 1, 0, ready(slot));
+        commit(&c.empty[slot++ % C::kSlots]);
+      }
+      for (int t = 0; t < n; ++t) {
+        pv(t & 1, ready(slot), t < 2);
+        commit(&c.empty[slot++ % C::kSlots]);
+        if (t + 2 < n) {
+          qk(t & 1, 0, ready(slot));
+          commit(&c.empty[slot++ % C::kSlots]);
+        } else {
+          commit(&c.o_full[t & 1]);
+        }
+      }
+    }
+    commit(&c.q_empty);
+    w.advance(a);
+  }
+}
+
+__device__ __forceinline__ uint32_t low_bits(int n) { return n >= 32 ? ~0u : (n <= 0 ? 0u : (1u << n) - 1u); }
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// Which of the tokens pos .. pos + 31 row `node` sees.
+__device__ __forceinline__ uint32_t visible32(const Args &a, const Seq &s, int node, int pos) {
+  if (!a.mask) return low_bits(s.ctx + node + 1 - pos);
+  uint32_t bits = low_bits(s.ctx - pos);
+  const int off = pos - s.ctx;
+  if (off > -32) {
+    const uint64_t *row = a.mask + static_cast<int64_t>(s.q0 + node) * a.words;
+    const int w = max(off, 0) >> 6;
+    uint64_t m = w < a.words ? __ldg(row + w) : 0;
+    if (off < 0) {
+      m <<= -off;
+    } else {
+      const int sh = off & 63;
+      m >>= sh;
+      if (sh > 32 && w + 1 < a.words) m |= __ldg(row + w + 1) << (64 - sh);
+    }
+    bits |= static_cast<uint32_t>(m) & low_bits(s.ctx + s.nodes - pos);
+  }
+  return bits;
+}
+
+// 32 scores of an 8-bit cache times their K scales (and the softmax scale).
+__device__ __forceinline__ void scale_scores(uint32_t (&r)[32], const float4 *factors) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float4 f = factors[j];
+    r[4 * j] = __float_as_uint(__uint_as_float(r[4 * j]) * f.x);
+    r[4 * j + 1] = __float_as_uint(__uint_as_float(r[4 * j + 1]) * f.y);
+    r[4 * j + 2] = __float_as_uint(__uint_as_float(r[4 * j + 2]) * f.z);
+    r[4 * j + 3] = __float_as_uint(__uint_as_float(r[4 * j + 3]) * f.w);
+  }
+}
+
+// Element d of a cached V row in the compute type's rounding.
+template <typename T, int D, int kCache>
+__device__ float cached_v(const Args &a, const void *pool, int id, int kvh, int row, int d) {
+  constexpr int kStick = kCache == B200KV_F16 ? 64 : 128;
+  const int64_t page = static_cast<int64_t>(id) * a.hkv + kvh;
+  const int64_t at = (page * (D / kStick) + d / kStick) * (kPageTokens * kStick) + row * kStick + d % kStick;
+  if constexpr (kCache == B200KV_F16) {
+    return to_float(static_cast<const T *>(pool)[at]);
+  } else {
+    float x;
+    if constexpr (kCache == B200KV_I8)
+      x = static_cast<float>(static_cast<const int8_t *>(pool)[at]);
+    else
+      x = __half2float(__half(__nv_cvt_fp8_to_halfraw(static_cast<const uint8_t *>(pool)[at], __NV_E4M3)));
+    T r;
+    from_float(r, x * __ldg(a.v_scales + page * kPageTokens + row));
+    return to_float(r);
+  }
+}
+// What the non-finite elements d of the visible nodes in [from, to) add to a row.
+template <typename T, int D, int kCache>
+__device__ __noinline__ float non_finite_sum(const Args &a, const Seq &s, int b, int kvh, int node, int from, int to,
+                                             int d) {
+  float sum = 0.f;
+  for (int p = max(from, s.ctx); p < min(to, s.ctx + s.nodes); ++p) {
+    if (!(visible32(a, s, node, p) & 1u)) continue;
+    const int id = __ldg(a.block_table + static_cast<int64_t>(b) * a.bt_stride + p / kPageTokens);
+    if (id < 0 || id >= a.num_blocks) continue;
+    const float v = cached_v<T, D, kCache>(a, a.v_pool, id, kvh, p % kPageTokens, d);
+    if (!(fabsf(v) < CUDART_INF_F)) sum += v;
+  }
+  return sum;
+}
+
+// One softmax warpgroup (w = 0 or 1); thread = row of its Q tile.
+template <typename C, typename T, int D, int kCache>
+__device__ __forceinline__ void softmax(const Args &a, Ctrl &c, uint8_t *smem, uint32_t tmem, int w) {
+  const int tid = threadIdx.x & 127, lane = tid & 31, warp = tid >> 5;
+  const uint32_t quad = tmem + (uint32_t(warp * 32) << 16);
+  const uint32_t ts = quad + col_s(w), to = quad + col_o(w);
+  const float cl = fabsf(a.scale) * 1.44269504088896341f;
+  float4 *kscale = reinterpret_cast<float4 *>(smem + kOffKScale) + (w * 4 + warp) * (kTileTokens / 4);
+  bool dead = false;
+  uint32_t s_uses = 0, o_uses[2] = {0, 0}, slot = 0;
+  unsigned piece = 0;
+  Walk wk;
+  wk.init(a, c);
+  while (wk.next(a)) {
+    ++piece;
+    const bool two = wk.two();
+    const int n = wk.t1 - wk.t0, lead = two ? 1 : 2;
+    const int len = wk.s.ctx + wk.s.nodes;
+    const int qt = 2 * wk.block + (two ? w : 0);
+    const int node = qt * a.tile_nodes + tid / a.group;
+    const bool live = tid < a.tile_nodes * a.group && node < wk.s.nodes;
+    const bool warp_live = __any_sync(0xffffffffu, live);
+    float m = -CUDART_INF_F, l = 0.f;
+    // 8-bit caches: the K scales of this stream's next tile, four per lane
+    auto scales_of = [&](int t) {
+      const int page = 2 * t + (lane >> 4);
+      if (page * kPageTokens >= len) return make_float4(0.f, 0.f, 0.f, 0.f);
+      const int id = __ldg(a.block_table + static_cast<int64_t>(wk.b) * a.bt_stride + page);
+      if (id < 0 || id >= a.num_blocks) return make_float4(0.f, 0.f, 0.f, 0.f);
+      return __ldg(reinterpret_cast<const float4 *>(a.k_scales + (static_cast<int64_t>(id) * a.hkv + wk.kvh) * kPageTokens) +
+                   (lane & 15));
+    };
+    const int step = two ? 1 : 2;
+    float4 ks = make_float4(0.f, 0.f, 0.f, 0.f);
+    const int tfirst = wk.t0 + (two ? 0 : w);
+    if (C::k8 && warp_live && tfirst < wk.t1) ks = scales_of(tfirst);
+    for (int t = tfirst; t < wk.t1; t += step) {
+      const int pos = t * kTileTokens;
+      const bool tail = pos + kTileTokens > wk.s.ctx + (a.mask ? 0 : 1);
+      uint32_t vis[4] = {~0u, ~0u, ~0u, ~0u};
+      if (tail && live) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) vis[i] = visible32(a, wk.s, node, pos + 32 * i);
+      }
+      if (C::k8 && warp_live) {
+        __syncwarp();
+        kscale[lane] = make_float4(ks.x * cl, ks.y * cl, ks.z * cl, ks.w * cl);
+        if (t + step < wk.t1) ks = scales_of(t + step);
+        __syncwarp();
+      }
+      wait(&c.s_full[w], s_uses++ & 1u, dead, a.error_flag);
+      fence_after();
+      if (warp_live) {
+        // maximum of the tile's scores, in units of log2
+        float mt = -CUDART_INF_F;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          uint32_t r[32];
+          tmem_ld32(ts + 32 * i, r);
+          wait_ld(r);
+          if (C::k8) scale_scores(r, kscale + 8 * i);
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            mt = fmaxf(mt, !tail || (vis[i] >> j & 1u) ? __uint_as_float(r[j]) : -CUDART_INF_F);
+        }
+        if (!C::k8 && mt != -CUDART_INF_F) mt *= cl;
+        const bool first = t == tfirst;
+        const bool rise = mt > m + (first ? 0.f : kLazyLog2);
+        if (!first && __any_sync(0xffffffffu, rise && live)) {
+          const float keep = rise ? ex2(m - mt) : 1.f;
+          l *= keep;
+#pragma unroll
+          for (int i = 0; i < D / 32; ++i) {
+            uint32_t r[32];
+            tmem_ld32(to + 32 * i, r);
+            wait_ld(r);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * keep);
+            tmem_st32(to + 32 * i, r);
+          }
+        }
+        if (rise) m = mt;
+        const float mm = m == -CUDART_INF_F ? 0.f : m;
+        float sum[2] = {0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          uint32_t r[32], p[16];
+          tmem_ld32(ts + 32 * i, r);
+          wait_ld(r);
+          if (C::k8) scale_scores(r, kscale + 8 * i);
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            const float x = __uint_as_float(r[j]);
+            float e = ex2(C::k8 ? x - mm : fmaf(x, cl, -mm));
+            if (tail) e = vis[i] >> j & 1u ? e : 0.f;
+            sum[j & 1] += e;
+            r[j] = __float_as_uint(e);
+          }
+#pragma unroll
+          for (int j = 0; j < 16; ++j) p[j] = pack2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1]), T());
+          tmem_st16(ts + 16 * i, p);
+        }
+        l += sum[0] + sum[1];
+        wait_st();
+      }
+      if (!C::k8 && pos + kTileTokens > wk.s.ctx) {
+        // the pool's rows past the sequence's end hold anything and become
+        // zeros, so that weights of zero meet finite values; so do non-finite
+        // elements of nodes
+        const int i = t - wk.t0;
+        const uint32_t vslot = slot + i + min(n, i + lead);
+        wait(&c.full[vslot % C::kSlots], (vslot / C::kSlots) & 1u, dead, a.error_flag);
+        uint8_t *v = smem + C::kOffSlots + (vslot % C::kSlots) * C::kTile;
+        const int node0 = max(wk.s.ctx - pos, 0), end = len - pos;
+        for (int k = node0 * 8 + tid; k < kTileTokens * 8; k += 128) {
+          for (int st = 0; st < C::kSticks; ++st) {
+            uint4 *at = reinterpret_cast<uint4 *>(v + st * C::kStickTile + k * 16);
+            uint4 x = make_uint4(0, 0, 0, 0);
+            if (k < end * 8) {
+              x = *at;
+              if (!drop_non_finite<T>(x)) continue;
+              atomicMax(&c.bad_piece, piece);  // before the element goes: the other stream looks too
+              __threadfence_block();
+            }
+            *at = x;
+          }
+        }
+        fence_async_smem();
+      }
+      fence_before();
+      __syncwarp();
+      if (lane == 0) arrive(&c.p_ready[w]);
+    }
+    slot += 2 * n;
+
+    // -------------------------------------------------------- end of piece --
+    const bool split = wk.t0 > 0 || wk.t1 < wk.tiles;
+    const int pslot = 2 * blockIdx.x + (wk.t0 > 0 || wk.left + n == c.per ? 0 : 1);
+    auto o_wait = [&](int k) {
+      wait(&c.o_full[k], o_uses[k]++ & 1u, dead, a.error_flag);
+      fence_after();
+    };
+    float keep0 = 1.f, keep1 = 0.f;
+    const bool both = !two && n > 1;
+    int d0 = 0, d1 = D;
+    if (two) {
+      o_wait(w);
+      ++o_uses[1 - w];
+    } else {
+      c.ml[w][tid] = make_float2(m, l);
+      o_wait(0);
+      if (both) o_wait(1);
+      bar_pair();
+      const float2 x = c.ml[0][tid], y = c.ml[1][tid];
+      m = fmaxf(x.x, y.x);
+      const float mm = m == -CUDART_INF_F ? 0.f : m;
+      keep0 = ex2(x.x - mm);
+      keep1 = ex2(y.x - mm);
+      l = x.y * keep0 + (both ? y.y * keep1 : 0.f);
+      d0 = w * (D / 2);
+      d1 = d0 + D / 2;
+    }
+    if (warp_live) {
+      const int64_t orow = static_cast<int64_t>(wk.s.q0 + node) * a.hq + wk.kvh * a.group + tid % a.group;
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      const bool repair = *reinterpret_cast<volatile unsigned *>(&c.bad_piece) >= piece;
+      const int prow = (two ? w : 0) * kTileRows + tid;
+#pragma unroll 1
+      for (int d = d0; d < d1; d += 32) {
+        uint32_t r[32];
+        tmem_ld32(two ? to + d : quad + col_o(0) + d, r);
+        wait_ld(r);
+        if (!two) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * keep0);
+          if (both) {
+            uint32_t r1[32];
+            tmem_ld32(quad + col_o(1) + d, r1);
+            wait_ld(r1);
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              r[j] = __float_as_uint(fmaf(__uint_as_float(r1[j]), keep1, __uint_as_float(r[j])));
+          }
+        }
+        if (live && repair) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            r[j] = __float_as_uint(__uint_as_float(r[j]) +
+                                   non_finite_sum<T, D, kCache>(a, wk.s, wk.b, wk.kvh, node, wk.t0 * kTileTokens,
+                                                                wk.t1 * kTileTokens, d + j));
+        }
+        if (live && split) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            *reinterpret_cast<uint4 *>(a.part_o + ((static_cast<int64_t>(pslot) * (D / 4) + d / 4 + j) * 256 + prow) * 4) =
+                make_uint4(r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
+        } else if (live) {
+          T *out = static_cast<T *>(a.out) + orow * D + d;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            float f[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) f[k] = l == 0.f ? 0.f : __uint_as_float(r[8 * j + k]) * inv;
+            *reinterpret_cast<uint4 *>(out + 8 * j) = pack8(f, T());
+          }
+        }
+        __syncwarp();
+      }
+      if (live && (two || w == 0)) {
+        if (split)
+          a.part_ml[static_cast<int64_t>(pslot) * 256 + prow] = make_float2(m, l);
+        else if (a.lse)
+          a.lse[orow] = l == 0.f ? -CUDART_INF_F : (m + log2f(l)) * 0.69314718055994530942f;
+      }
+    }
+    // the first CTA boundary inside a split block describes it to the join
+    if (split && wk.t0 > 0 && w == 0 && tid == 0 && wk.t0 <= c.per) {
+      Join j;
+      j.rows0 = static_cast<int64_t>(wk.s.q0);
+      j.node0 = 2 * wk.block * a.tile_nodes;
+      j.nodes = min(wk.s.nodes - j.node0, 2 * a.tile_nodes);
+      j.kvh = wk.kvh;
+      // pieces: the CTA before this one, this one, and on to the block's end
+      j.first_slot = 2 * (static_cast<int>(blockIdx.x) - 1) + (wk.t0 == c.per ? 0 : 1);
+      j.last_cta = static_cast<int>((static_cast<long long>(blockIdx.x) * c.per - wk.t0 + wk.tiles - 1) / c.per);
+      a.joins[blockIdx.x] = j;
+    }
+    fence_before();
+    if (!two) bar_pair();  // both have read O and ml before either goes on
+    fence_after();
+    wk.advance(a);
+  }
+}
+
+template <typename T, int D, int kCache>
+__global__ void __launch_bounds__((Cfg<T, D, kCache>::kThreads), 1)
+    tree_kernel(const __grid_constant__ CUtensorMap qm, const __grid_constant__ CUtensorMap km,
+                const __grid_constant__ CUtensorMap vm, const __grid_constant__ Args a) {
+  using C = Cfg<T, D, kCache>;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  Ctrl &c = *reinterpret_cast<Ctrl *>(smem);
+  const int tid = threadIdx.x, warp = tid >> 5;
+  if (tid == 0) {
+    prefetch_tensormap(&qm);
+    prefetch_tensormap(&km);
+    prefetch_tensormap(&vm);
+    for (int i = 0; i < C::kSlots; ++i) {
+      mbar_init(&c.full[i], C::k8 ? 4 : 1);
+      mbar_init(&c.empty[i], 1);
+    }
+    for (int i = 0; i < C::kRaw; ++i) {
+      mbar_init(&c.raw_full[i], 1);
+      mbar_init(&c.raw_empty[i], 4);
+    }
+    mbar_init(&c.q_full, 1);
+    mbar_init(&c.q_empty, 1);
+    for (int w = 0; w < 2; ++w) {
+      mbar_init(&c.s_full[w], 1);
+      mbar_init(&c.p_ready[w], 4);
+      mbar_init(&c.o_full[w], 1);
+    }
+    fence_mbar_init();
+    c.bad_piece = 0;
+  }
+  if (warp == 9) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&c.tmem)),
+                 "r"(kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (tid == 0) a.joins[blockIdx.x].nodes = 0;  // no block begins to be split here, unless the epilogue says so
+  make_plan<C::kThreads>(a, c);
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = c.tmem;
+  if (warp < 8) {
+    softmax<C, T, D, kCache>(a, c, smem, tmem, warp >> 2);
+  } else if (warp == 8) {
+    producer<C>(a, c, smem, &qm, &km, &vm);
+  } else if (warp == 9) {
+    if ((tid & 31) == 0) mma_issuer<C, D>(a, c, smem, tmem);
+    __syncwarp();
+  } else {
+    if constexpr (C::k8) converter<C, T, kCache>(a, c, smem, warp - 10);
+  }
+  fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+  }
+}
+
+// ------------------------------------------------------------------- join --
+// Blocks cut by CTA boundaries: out = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i
+// over the pieces in order (the same bits every time).  One CTA per boundary and
+// 32 rows; lane = row, warp = an eighth of the head.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) tree_join_kernel(const __grid_constant__ Args a) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const Join j = a.joins[blockIdx.x];
+  const int tile_rows = a.tile_nodes * a.group;
+  const int prow = blockIdx.y * 32 + (threadIdx.x & 31);
+  const int in_tile = prow & (kTileRows - 1), tile = prow / kTileRows;
+  const int node = tile * a.tile_nodes + in_tile / a.group;
+  if (in_tile >= tile_rows || node >= j.nodes) return;
+  const int first_cta = j.first_slot >> 1;
+  auto slot_of = [&](int cta) { return cta == first_cta ? j.first_slot : 2 * cta; };
+  float M = -CUDART_INF_F;
+  for (int x = first_cta; x <= j.last_cta; ++x)
+    M = fmaxf(M, a.part_ml[static_cast<int64_t>(slot_of(x)) * 256 + prow].x);
+  const float mm = M == -CUDART_INF_F ? 0.f : M;
+  constexpr int kPer = D / 8 / 4;
+  const int d4 = (threadIdx.x >> 5) * kPer;
+  float l = 0.f, o[4 * kPer];
+#pragma unroll
+  for (int i = 0; i < 4 * kPer; ++i) o[i] = 0.f;
+#pragma unroll 2
+  for (int x = first_cta; x <= j.last_cta; ++x) {
+    const int64_t s = slot_of(x);
+    const float2 ml = a.part_ml[s * 256 + prow];
+    const float keep = exp2f(ml.x - mm);
+    l = fmaf(ml.y, keep, l);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const float4 v = *reinterpret_cast<const float4 *>(a.part_o + ((s * (D / 4) + d4 + i) * 256 + prow) * 4);
+      o[4 * i] = fmaf(v.x, keep, o[4 * i]);
+      o[4 * i + 1] = fmaf(v.y, keep, o[4 * i + 1]);
+      o[4 * i + 2] = fmaf(v.z, keep, o[4 * i + 2]);
+      o[4 * i + 3] = fmaf(v.w, keep, o[4 * i + 3]);
+    }
+  }
+  const int64_t orow = (j.rows0 + j.node0 + node) * a.hq + j.kvh * a.group + in_tile % a.group;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  T *out = static_cast<T *>(a.out) + orow * D + 4 * d4;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const uint32_t lo = pack2(l == 0.f ? 0.f : o[4 * i] * inv, l == 0.f ? 0.f : o[4 * i + 1] * inv, T());
+    const uint32_t hi = pack2(l == 0.f ? 0.f : o[4 * i + 2] * inv, l == 0.f ? 0.f : o[4 * i + 3] * inv, T());
+    *reinterpret_cast<uint2 *>(out + 4 * i) = make_uint2(lo, hi);
+  }
+  if (threadIdx.x < 32 && a.lse) a.lse[orow] = l == 0.f ? -CUDART_INF_F : (M + log2f(l)) * 0.69314718055994530942f;
+}
+
+// ----------------------------------------------------------------- launch --
+template <typename T, int D, int kCache>
+int launch(const CUtensorMap &qm, const CUtensorMap &km, const CUtensorMap &vm, const Args &a, int ctas,
+           cudaStream_t stream) {
+  using C = Cfg<T, D, kCache>;
+  static int configured[64] = {0};
+  int dev = 0;
+  B200KV_CUDA_TRY(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= 64) return set_error(B200KV_ERR_UNSUPPORTED, "device ordinal %d", dev);
+  if (!__atomic_load_n(&configured[dev], __ATOMIC_ACQUIRE)) {
+    B200KV_CUDA_TRY(cudaFuncSetAttribute(tree_kernel<T, D, kCache>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
+    __atomic_store_n(&configured[dev], 1, __ATOMIC_RELEASE);
+  }
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(ctas));
+  cfg.blockDim = dim3(C::kThreads);
+  cfg.dynamicSmemBytes = C::kSmem;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  B200KV_CUDA_TRY(cudaLaunchKernelEx(&cfg, tree_kernel<T, D, kCache>, qm, km, vm, a));
+  cfg.gridDim = dim3(static_cast<unsigned>(ctas), a.most_rows > kTileRows ? 8 : 4);
+  cfg.blockDim = dim3(256);
+  cfg.dynamicSmemBytes = 0;
+  B200KV_CUDA_TRY(cudaLaunchKernelEx(&cfg, tree_join_kernel<T, D>, a));
+  return B200KV_OK;
+}
+
+}  // namespace tree
+}  // namespace b200kv
