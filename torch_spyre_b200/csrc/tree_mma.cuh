@@ -25,9 +25,8 @@
 // pipe and the exponentials (16 per clock and SM, as long as the products).
 //
 // Warps: 0-3 and 4-7 the two softmax warpgroups, 8 the TMA producer, 9 the MMA
-// issuer (owns the TMEM), 8-bit caches: 10-13 converters, which turn 8-bit
-// pages into 16-bit operand tiles (K as its exact steps, its scales multiply
-// the scores; V times its scale, rounded to the compute type).
+// issuer (owns the TMEM), 8-bit caches: 12-15 converters, which turn 8-bit
+// pages into 16-bit operand tiles of exact steps (the scales: see Factors).
 #pragma once
 
 #include <type_traits>
@@ -44,25 +43,32 @@ constexpr float kLazyLog2 = 8.f;
 template <typename T, int D, int kCache>
 struct Cfg {
   static constexpr bool k8 = kCache != B200KV_F16;
-  static constexpr int kThreads = k8 ? 448 : 320;
+  static constexpr int kThreads = k8 ? 512 : 384;
+  // Registers a thread, warpgroups 0-1 / 2 / 3, after setmaxnreg: a softmax
+  // thread holds its row's 128 scores.  Sums within the launch's own: 384
+  // threads of 168, or 512 of 128.
+  static constexpr int kRegsSoftmax = k8 ? 176 : 208, kRegsIssue = k8 ? 72 : 80, kRegsConvert = 88;
   static constexpr int kSticks = D / 64;
   static constexpr int kStickTile = kTileTokens * 128;      // one 64-element column of 128 rows
   static constexpr int kTile = kSticks * kStickTile;        // a Q, K or V tile
   static constexpr int kSlots = k8 ? 3 : (D == 64 ? 8 : 5);  // operand tiles in flight
-  static constexpr int kRaw = k8 ? 7 : 0;                   // 8-bit pages in flight
+  static constexpr int kRaw = k8 ? 6 : 0;                   // 8-bit pages in flight
   static constexpr int kRawPage = kPageTokens * 128;
-  static constexpr int kRawScales = kPageTokens * 4;
-  static constexpr int kCtrl = k8 ? 8192 : 3072;
+  static constexpr int kCtrl = k8 ? 15360 : 3072;
   static constexpr int kOffQ = kCtrl;
   static constexpr int kOffSlots = kOffQ + 2 * kTile;
   static constexpr int kOffRaw = kOffSlots + kSlots * kTile;
-  static constexpr int kOffRawScales = kOffRaw + kRaw * kRawPage;
-  static constexpr int kSmem = kOffRawScales + kRaw * kRawScales;
-  static constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+  static constexpr int kSmem = kOffRaw + kRaw * kRawPage;
+  // The type of P and V: an 8-bit cache's steps are exact in fp16, whatever q's
+  // type, and fp16 keeps three bits more of each weight than bf16.
+  using P = typename std::conditional<k8, __half, T>::type;
   // kind::f16: fp32 accumulator, A and B both fp16 or both bf16, M = 128
-  static constexpr uint32_t kIdesc = (1u << 4) | (kBf16 ? (1u << 7) | (1u << 10) : 0u) | (uint32_t(kTileRows >> 4) << 24);
-  static constexpr uint32_t kIdescQK = kIdesc | (uint32_t(kTileTokens >> 3) << 17);
-  static constexpr uint32_t kIdescPV = kIdesc | (1u << 16) | (uint32_t(D >> 3) << 17);  // V: N-major
+  static constexpr uint32_t kIdesc = (1u << 4) | (uint32_t(kTileRows >> 4) << 24);
+  static constexpr uint32_t kBf16 = (1u << 7) | (1u << 10);
+  static constexpr uint32_t kIdescQK =
+      kIdesc | (std::is_same<T, __half>::value ? 0u : kBf16) | (uint32_t(kTileTokens >> 3) << 17);
+  static constexpr uint32_t kIdescPV =  // V: N-major
+      kIdesc | (std::is_same<P, __half>::value ? 0u : kBf16) | (1u << 16) | (uint32_t(D >> 3) << 17);
   static_assert(kSmem <= 227 * 1024, "shared memory per CTA");
 };
 
@@ -84,8 +90,9 @@ struct Ctrl {
   unsigned bad_piece;       // last piece (counted from 1) that met a non-finite value in a node's V row
   float2 ml[2][kTileRows];  // (maximum, sum) of the streams' rows
 };
-constexpr int kOffKScale = 3072;  // 8-bit caches: [8 warps][128] score factors of a tile
-static_assert(sizeof(Ctrl) <= kOffKScale, "control block");
+// 8-bit caches: [8 warps][3][128] factors of a tile's tokens, see Factors
+constexpr int kOffFactors = 3072;
+static_assert(sizeof(Ctrl) <= kOffFactors, "control block");
 
 // ------------------------------------------------------------------- waits --
 // Bounded: after kWaitLimitNs the error flag is set and this thread waits no
@@ -109,7 +116,6 @@ __device__ __forceinline__ void commit(uint64_t *bar) {
 }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void bar_pair() { asm volatile("bar.sync 1, 256;" ::: "memory"); }  // both warpgroups
 
@@ -125,6 +131,12 @@ __device__ __forceinline__ void tmem_ld32(uint32_t at, uint32_t (&r)[32]) {
       : B200KV_R8(r, 0), B200KV_R8(r, 8), B200KV_R8(r, 16), B200KV_R8(r, 24)
       : "r"(at));
 }
+__device__ __forceinline__ void tmem_ld16(uint32_t at, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : B200KV_R8(r, 0), B200KV_R8(r, 8)
+      : "r"(at));
+}
 #define B200KV_RW8(r, i) "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]), \
                          "+r"(r[i + 6]), "+r"(r[i + 7])
 // The loaded registers go through the wait, so that no use of them is moved before it.
@@ -132,12 +144,8 @@ __device__ __forceinline__ void wait_ld(uint32_t (&r)[32]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;"
                : B200KV_RW8(r, 0), B200KV_RW8(r, 8), B200KV_RW8(r, 16), B200KV_RW8(r, 24)::"memory");
 }
-__device__ __forceinline__ void tmem_st32(uint32_t at, const uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
-      "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(at),
-      B200KV_W8(r, 0), B200KV_W8(r, 8), B200KV_W8(r, 16), B200KV_W8(r, 24)
-      : "memory");
+__device__ __forceinline__ void wait_ld(uint32_t (&r)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" : B200KV_RW8(r, 0), B200KV_RW8(r, 8)::"memory");
 }
 __device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t (&r)[16]) {
   asm volatile(
@@ -384,11 +392,8 @@ __device__ __forceinline__ void producer(const Args &a, Ctrl &c, uint8_t *smem, 
               arrive(&c.raw_full[r]);
             } else {
               const int page = id * a.hkv + w.kvh;
-              mbar_arrive_expect_tx(&c.raw_full[r], C::kRawPage + (is_v ? C::kRawScales : 0));
+              mbar_arrive_expect_tx(&c.raw_full[r], C::kRawPage);
               tma_load_3d(smem + C::kOffRaw + r * C::kRawPage, map, &c.raw_full[r], 0, 0, page, policy);
-              if (is_v)
-                bulk_load(smem + C::kOffRawScales + r * C::kRawScales, a.v_scales + static_cast<int64_t>(page) * kPageTokens,
-                          C::kRawScales, &c.raw_full[r]);
             }
           }
           ++ring;
@@ -435,31 +440,42 @@ __device__ __forceinline__ bool drop_non_finite(uint4 &v) {
 // warp and step; the two 16-byte results of lanes 4-7 of a row are written in
 // swapped order so that the eight lanes of a row hit eight different 16-byte
 // bank groups in the swizzled tile.
+//
+// Every step is exact in the operand type.  int8 -> fp16: 0x64xx is 1024 + xx,
+// taken as b + 128, less 1152.  int8 -> bf16: b = (b & 127) - (b & 128), both
+// over 128 as 0x43xx.  e4m3 -> fp16 in hardware, on to bf16 by way of fp32, of
+// whose mantissa at most three bits are set.
 template <typename T, int kCache>
-__device__ __forceinline__ void widen16(uint4 v, float scale, bool scaled, uint4 &lo, uint4 &hi) {
+__device__ __forceinline__ void widen16(uint4 v, uint4 &lo, uint4 &hi) {
+  constexpr bool kHalf = std::is_same<T, __half>::value;
   const uint32_t w[4] = {v.x, v.y, v.z, v.w};
   uint32_t o[8];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    float f[4];
-    if constexpr (kCache == B200KV_I8) {
-      // 2^23 + 128 + b as a float: b's byte, its sign bit flipped, under 0x4B0000
-      const uint32_t u = w[i] ^ 0x80808080u;
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        f[j] = __fadd_rn(__uint_as_float(__byte_perm(u, 0x4B000000u, 0x7540 | j)), -8388736.f);
-    } else {
-      const __half2_raw a = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w[i] & 0xffffu), __NV_E4M3);
-      const __half2_raw b = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w[i] >> 16), __NV_E4M3);
-      const float2 fa = __half22float2(__half2(a)), fb = __half22float2(__half2(b));
-      f[0] = fa.x, f[1] = fa.y, f[2] = fb.x, f[3] = fb.y;
+    for (int k = 0; k < 2; ++k) {
+      uint32_t &r = o[2 * i + k];
+      if constexpr (kCache == B200KV_I8 && kHalf) {
+        const uint32_t u = __byte_perm(w[i] ^ 0x80808080u, 0x64646464u, k ? 0x4342 : 0x4140);
+        const __half2 h = __hsub2(*reinterpret_cast<const __half2 *>(&u), __half2half2(__ushort_as_half(0x6480)));
+        r = *reinterpret_cast<const uint32_t *>(&h);
+      } else if constexpr (kCache == B200KV_I8) {
+        const uint32_t u = __byte_perm(w[i], 0u, k ? 0x4342 : 0x4140);
+        const uint32_t a = (u & 0x007f007fu) | 0x43004300u, b = (u & 0x00800080u) | 0x43004300u;
+        const __nv_bfloat162 h =
+            __hsub2(*reinterpret_cast<const __nv_bfloat162 *>(&a), *reinterpret_cast<const __nv_bfloat162 *>(&b));
+        r = *reinterpret_cast<const uint32_t *>(&h);
+      } else {
+        const __half2_raw h =
+            __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(k ? w[i] >> 16 : w[i] & 0xffffu), __NV_E4M3);
+        if constexpr (kHalf) {
+          r = static_cast<uint32_t>(h.x) | static_cast<uint32_t>(h.y) << 16;
+        } else {
+          const float2 f = __half22float2(__half2(h));
+          r = __byte_perm(__float_as_uint(f.x), __float_as_uint(f.y), 0x7632);
+        }
+      }
     }
-    if (scaled) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) f[j] *= scale;
-    }
-    o[2 * i] = pack2(f[0], f[1], T());
-    o[2 * i + 1] = pack2(f[2], f[3], T());
   }
   lo = make_uint4(o[0], o[1], o[2], o[3]);
   hi = make_uint4(o[4], o[5], o[6], o[7]);
@@ -484,17 +500,20 @@ __device__ __forceinline__ void converter(const Args &a, Ctrl &c, uint8_t *smem,
         rows = c.raw_rows[r];
       }
       const uint8_t *src = smem + C::kOffRaw + r * C::kRawPage;
-      const float *scales = reinterpret_cast<const float *>(smem + C::kOffRawScales + r * C::kRawScales);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const int row = warp * 16 + k * 4 + (lane >> 3), trow = i * kPageTokens + row;
         uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
         if (row < rows) {
-          widen16<T, kCache>(*reinterpret_cast<const uint4 *>(src + row * 128 + sub * 16), is_v ? scales[row] : 1.f, is_v,
-                             lo, hi);
-          if (is_v && t * kTileTokens + trow >= ctx) {  // a node's row
-            const bool hit = drop_non_finite<T>(lo);
-            if (drop_non_finite<T>(hi) || hit) atomicMax(&c.bad_piece, piece);
+          const uint4 x = *reinterpret_cast<const uint4 *>(src + row * 128 + sub * 16);
+          if (is_v) {
+            widen16<__half, kCache>(x, lo, hi);
+            if (kCache == B200KV_E4M3 && t * kTileTokens + trow >= ctx) {  // a node's row: e4m3 has NaN
+              const bool hit = drop_non_finite<__half>(lo);
+              if (drop_non_finite<__half>(hi) || hit) atomicMax(&c.bad_piece, piece);
+            }
+          } else {
+            widen16<T, kCache>(x, lo, hi);
           }
         }
         const int c0 = (sub & 3) * 2, first = sub >> 2;  // lanes 4-7 write their second half first
@@ -635,36 +654,127 @@ __device__ __forceinline__ uint32_t visible32(const Args &a, const Seq &s, int n
   return bits;
 }
 
-// 32 scores of an 8-bit cache times their K scales (and the softmax scale).
-__device__ __forceinline__ void scale_scores(uint32_t (&r)[32], const float4 *factors) {
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const float4 f = factors[j];
-    r[4 * j] = __float_as_uint(__uint_as_float(r[4 * j]) * f.x);
-    r[4 * j + 1] = __float_as_uint(__uint_as_float(r[4 * j + 1]) * f.y);
-    r[4 * j + 2] = __float_as_uint(__uint_as_float(r[4 * j + 2]) * f.z);
-    r[4 * j + 3] = __float_as_uint(__uint_as_float(r[4 * j + 3]) * f.w);
-  }
+// Two fp32 at a time.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+      "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 d, a, b;\n\t"
+      "mov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
 }
 
-// Element d of a cached V row in the compute type's rounding.
+// Per-token factors of an 8-bit cache.  The scales leave the products: K and V
+// enter them as exact steps, and the weight that V's steps get is
+//   p v = 2^(k_factor s + log2 v) = 2^y,   y = s * (scale * log2(e) * k) + log2 v,
+// so the running maximum is that of y, and the softmax's own sum takes 2^y / v.
+// Scales below 1e-30 count as that: their rows stay zero to any purpose.
+struct Factors {
+  float4 k[kTileTokens / 4], log2v[kTileTokens / 4], inv_v[kTileTokens / 4];
+};
+__device__ __forceinline__ float floor_scale(float v) { return v < 1e-30f ? 1e-30f : v; }
+// (a NaN scale makes 2^y NaN where the token is seen; 0 / v must stay 0 where not)
+__device__ __forceinline__ float inv_scale(float v) { return v < CUDART_INF_F ? 1.f / v : 1.f; }
+
+// Scores of a row's 128 tokens -> weights, in place in TMEM.  kTail: vis tells
+// which tokens the row sees.
+template <typename C, int D, bool kTail>
+__device__ __forceinline__ void weigh(uint32_t ts, uint32_t to, const uint32_t (&vis)[4], float cl, const Factors *fac,
+                                      bool first, bool live, float &m, float &l) {
+  uint32_t s[4][32];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) tmem_ld32(ts + 32 * i, s[i]);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) wait_ld(s[i]);
+  float top[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (C::k8) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float4 k = fac->k[8 * i + j], v = fac->log2v[8 * i + j];
+        uint32_t *r = &s[i][4 * j];
+        const float2 lo = fma2(make_float2(__uint_as_float(r[0]), __uint_as_float(r[1])), make_float2(k.x, k.y),
+                               make_float2(v.x, v.y));
+        const float2 hi = fma2(make_float2(__uint_as_float(r[2]), __uint_as_float(r[3])), make_float2(k.z, k.w),
+                               make_float2(v.z, v.w));
+        r[0] = __float_as_uint(lo.x), r[1] = __float_as_uint(lo.y);
+        r[2] = __float_as_uint(hi.x), r[3] = __float_as_uint(hi.y);
+      }
+    }
+    if (kTail) {
+#pragma unroll
+      for (int j = 0; j < 32; ++j) s[i][j] = vis[i] >> j & 1u ? s[i][j] : 0xff800000u;  // -inf
+    }
+    float t = __uint_as_float(s[i][0]);
+#pragma unroll
+    for (int j = 1; j < 31; j += 2) t = fmaxf(fmaxf(t, __uint_as_float(s[i][j])), __uint_as_float(s[i][j + 1]));
+    top[i] = fmaxf(t, __uint_as_float(s[i][31]));
+  }
+  float mt = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+  if (!C::k8) mt *= cl;
+  const bool rise = mt > m + (first ? 0.f : kLazyLog2);
+  if (!first && __any_sync(0xffffffffu, rise && live)) {
+    const float keep = rise ? ex2(m - mt) : 1.f;
+    l *= keep;
+#pragma unroll 1
+    for (int i = 0; i < D; i += 16) {
+      uint32_t r[16];
+      tmem_ld16(to + i, r);
+      wait_ld(r);
+#pragma unroll
+      for (int j = 0; j < 16; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * keep);
+      tmem_st16(to + i, r);
+    }
+  }
+  if (rise) m = mt;
+  const float minus = m == -CUDART_INF_F ? 0.f : -m;
+  float2 sum[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    sum[i] = make_float2(0.f, 0.f);
+    uint32_t p[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const float2 x = make_float2(__uint_as_float(s[i][2 * j]), __uint_as_float(s[i][2 * j + 1]));
+      const float2 y = C::k8 ? add2(x, make_float2(minus, minus))
+                             : fma2(x, make_float2(cl, cl), make_float2(minus, minus));
+      const float2 e = make_float2(ex2(y.x), ex2(y.y));
+      if constexpr (C::k8) {
+        const float4 v = fac->inv_v[8 * i + j / 2];
+        sum[i] = fma2(e, j & 1 ? make_float2(v.z, v.w) : make_float2(v.x, v.y), sum[i]);
+      } else {
+        sum[i] = add2(sum[i], e);
+      }
+      p[j] = pack2(e.x, e.y, typename C::P());
+    }
+    tmem_st16(ts + 16 * i, p);
+  }
+  const float2 t = add2(add2(sum[0], sum[1]), add2(sum[2], sum[3]));
+  l += t.x + t.y;
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+
+// Element d of a cached V row (8-bit caches: its steps).
 template <typename T, int D, int kCache>
 __device__ float cached_v(const Args &a, const void *pool, int id, int kvh, int row, int d) {
   constexpr int kStick = kCache == B200KV_F16 ? 64 : 128;
   const int64_t page = static_cast<int64_t>(id) * a.hkv + kvh;
   const int64_t at = (page * (D / kStick) + d / kStick) * (kPageTokens * kStick) + row * kStick + d % kStick;
-  if constexpr (kCache == B200KV_F16) {
+  if constexpr (kCache == B200KV_F16)
     return to_float(static_cast<const T *>(pool)[at]);
-  } else {
-    float x;
-    if constexpr (kCache == B200KV_I8)
-      x = static_cast<float>(static_cast<const int8_t *>(pool)[at]);
-    else
-      x = __half2float(__half(__nv_cvt_fp8_to_halfraw(static_cast<const uint8_t *>(pool)[at], __NV_E4M3)));
-    T r;
-    from_float(r, x * __ldg(a.v_scales + page * kPageTokens + row));
-    return to_float(r);
-  }
+  else if constexpr (kCache == B200KV_I8)
+    return static_cast<float>(static_cast<const int8_t *>(pool)[at]);
+  else
+    return __half2float(__half(__nv_cvt_fp8_to_halfraw(static_cast<const uint8_t *>(pool)[at], __NV_E4M3)));
 }
 // What the non-finite elements d of the visible nodes in [from, to) add to a row.
 template <typename T, int D, int kCache>
@@ -687,8 +797,9 @@ __device__ __forceinline__ void softmax(const Args &a, Ctrl &c, uint8_t *smem, u
   const int tid = threadIdx.x & 127, lane = tid & 31, warp = tid >> 5;
   const uint32_t quad = tmem + (uint32_t(warp * 32) << 16);
   const uint32_t ts = quad + col_s(w), to = quad + col_o(w);
-  const float cl = fabsf(a.scale) * 1.44269504088896341f;
-  float4 *kscale = reinterpret_cast<float4 *>(smem + kOffKScale) + (w * 4 + warp) * (kTileTokens / 4);
+  // (a scale of zero: too small to move a score, and -inf stays -inf)
+  const float cl = fmaxf(fabsf(a.scale) * 1.44269504088896341f, 1e-37f);
+  Factors *fac = reinterpret_cast<Factors *>(smem + kOffFactors) + (w * 4 + warp);
   bool dead = false;
   uint32_t s_uses = 0, o_uses[2] = {0, 0}, slot = 0;
   unsigned piece = 0;
@@ -704,19 +815,21 @@ __device__ __forceinline__ void softmax(const Args &a, Ctrl &c, uint8_t *smem, u
     const bool live = tid < a.tile_nodes * a.group && node < wk.s.nodes;
     const bool warp_live = __any_sync(0xffffffffu, live);
     float m = -CUDART_INF_F, l = 0.f;
-    // 8-bit caches: the K scales of this stream's next tile, four per lane
-    auto scales_of = [&](int t) {
+    // 8-bit caches: the scales of this stream's next tile, four tokens per lane
+    auto scales_of = [&](int t, float4 &k, float4 &v) {
       const int page = 2 * t + (lane >> 4);
-      if (page * kPageTokens >= len) return make_float4(0.f, 0.f, 0.f, 0.f);
+      k = v = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (page * kPageTokens >= len) return;
       const int id = __ldg(a.block_table + static_cast<int64_t>(wk.b) * a.bt_stride + page);
-      if (id < 0 || id >= a.num_blocks) return make_float4(0.f, 0.f, 0.f, 0.f);
-      return __ldg(reinterpret_cast<const float4 *>(a.k_scales + (static_cast<int64_t>(id) * a.hkv + wk.kvh) * kPageTokens) +
-                   (lane & 15));
+      if (id < 0 || id >= a.num_blocks) return;
+      const int64_t at = (static_cast<int64_t>(id) * a.hkv + wk.kvh) * kPageTokens;
+      k = __ldg(reinterpret_cast<const float4 *>(a.k_scales + at) + (lane & 15));
+      v = __ldg(reinterpret_cast<const float4 *>(a.v_scales + at) + (lane & 15));
     };
     const int step = two ? 1 : 2;
-    float4 ks = make_float4(0.f, 0.f, 0.f, 0.f);
     const int tfirst = wk.t0 + (two ? 0 : w);
-    if (C::k8 && warp_live && tfirst < wk.t1) ks = scales_of(tfirst);
+    float4 ks, vs;
+    if (C::k8 && warp_live && tfirst < wk.t1) scales_of(tfirst, ks, vs);
     for (int t = tfirst; t < wk.t1; t += step) {
       const int pos = t * kTileTokens;
       const bool tail = pos + kTileTokens > wk.s.ctx + (a.mask ? 0 : 1);
@@ -727,64 +840,20 @@ __device__ __forceinline__ void softmax(const Args &a, Ctrl &c, uint8_t *smem, u
       }
       if (C::k8 && warp_live) {
         __syncwarp();
-        kscale[lane] = make_float4(ks.x * cl, ks.y * cl, ks.z * cl, ks.w * cl);
-        if (t + step < wk.t1) ks = scales_of(t + step);
+        fac->k[lane] = make_float4(ks.x * cl, ks.y * cl, ks.z * cl, ks.w * cl);
+        vs = make_float4(floor_scale(vs.x), floor_scale(vs.y), floor_scale(vs.z), floor_scale(vs.w));
+        fac->log2v[lane] = make_float4(__log2f(vs.x), __log2f(vs.y), __log2f(vs.z), __log2f(vs.w));
+        fac->inv_v[lane] = make_float4(inv_scale(vs.x), inv_scale(vs.y), inv_scale(vs.z), inv_scale(vs.w));
+        if (t + step < wk.t1) scales_of(t + step, ks, vs);
         __syncwarp();
       }
       wait(&c.s_full[w], s_uses++ & 1u, dead, a.error_flag);
       fence_after();
       if (warp_live) {
-        // maximum of the tile's scores, in units of log2
-        float mt = -CUDART_INF_F;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          uint32_t r[32];
-          tmem_ld32(ts + 32 * i, r);
-          wait_ld(r);
-          if (C::k8) scale_scores(r, kscale + 8 * i);
-#pragma unroll
-          for (int j = 0; j < 32; ++j)
-            mt = fmaxf(mt, !tail || (vis[i] >> j & 1u) ? __uint_as_float(r[j]) : -CUDART_INF_F);
-        }
-        if (!C::k8 && mt != -CUDART_INF_F) mt *= cl;
-        const bool first = t == tfirst;
-        const bool rise = mt > m + (first ? 0.f : kLazyLog2);
-        if (!first && __any_sync(0xffffffffu, rise && live)) {
-          const float keep = rise ? ex2(m - mt) : 1.f;
-          l *= keep;
-#pragma unroll
-          for (int i = 0; i < D / 32; ++i) {
-            uint32_t r[32];
-            tmem_ld32(to + 32 * i, r);
-            wait_ld(r);
-#pragma unroll
-            for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * keep);
-            tmem_st32(to + 32 * i, r);
-          }
-        }
-        if (rise) m = mt;
-        const float mm = m == -CUDART_INF_F ? 0.f : m;
-        float sum[2] = {0.f, 0.f};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          uint32_t r[32], p[16];
-          tmem_ld32(ts + 32 * i, r);
-          wait_ld(r);
-          if (C::k8) scale_scores(r, kscale + 8 * i);
-#pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            const float x = __uint_as_float(r[j]);
-            float e = ex2(C::k8 ? x - mm : fmaf(x, cl, -mm));
-            if (tail) e = vis[i] >> j & 1u ? e : 0.f;
-            sum[j & 1] += e;
-            r[j] = __float_as_uint(e);
-          }
-#pragma unroll
-          for (int j = 0; j < 16; ++j) p[j] = pack2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1]), T());
-          tmem_st16(ts + 16 * i, p);
-        }
-        l += sum[0] + sum[1];
-        wait_st();
+        if (tail)
+          weigh<C, D, true>(ts, to, vis, cl, fac, t == tfirst, live, m, l);
+        else
+          weigh<C, D, false>(ts, to, vis, cl, fac, t == tfirst, live, m, l);
       }
       if (!C::k8 && pos + kTileTokens > wk.s.ctx) {
         // the pool's rows past the sequence's end hold anything and become
@@ -801,7 +870,7 @@ __device__ __forceinline__ void softmax(const Args &a, Ctrl &c, uint8_t *smem, u
             uint4 x = make_uint4(0, 0, 0, 0);
             if (k < end * 8) {
               x = *at;
-              if (!drop_non_finite<T>(x)) continue;
+              if (!drop_non_finite<typename C::P>(x)) continue;
               atomicMax(&c.bad_piece, piece);  // before the element goes: the other stream looks too
               __threadfence_block();
             }
@@ -960,14 +1029,21 @@ __global__ void __launch_bounds__((Cfg<T, D, kCache>::kThreads), 1)
   fence_after();
   const uint32_t tmem = c.tmem;
   if (warp < 8) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kRegsSoftmax));
     softmax<C, T, D, kCache>(a, c, smem, tmem, warp >> 2);
-  } else if (warp == 8) {
-    producer<C>(a, c, smem, &qm, &km, &vm);
-  } else if (warp == 9) {
-    if ((tid & 31) == 0) mma_issuer<C, D>(a, c, smem, tmem);
-    __syncwarp();
+  } else if (warp < 12) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kRegsIssue));
+    if (warp == 8) {
+      producer<C>(a, c, smem, &qm, &km, &vm);
+    } else if (warp == 9) {
+      if ((tid & 31) == 0) mma_issuer<C, D>(a, c, smem, tmem);
+      __syncwarp();
+    }
   } else {
-    if constexpr (C::k8) converter<C, T, kCache>(a, c, smem, warp - 10);
+    if constexpr (C::k8) {
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kRegsConvert));
+      converter<C, T, kCache>(a, c, smem, warp - 12);
+    }
   }
   fence_before();
   __syncthreads();
