@@ -181,7 +181,6 @@ extern "C" int b200kv_tree_attention(const void *q, int32_t q_dtype, int64_t q_s
   a.max_blocks = static_cast<int>(max_blocks_per_seq), a.max_nodes = static_cast<int>(max_nodes);
   a.num_blocks = static_cast<int>(num_blocks);
   a.tile_nodes = 128 / group;
-  a.most_rows = max_nodes > a.tile_nodes ? 256 : 128;
   a.scale = scale;
   a.error_flag = error_flag;
   const Workspace ws = workspace_of(head_dim);

@@ -29,7 +29,6 @@ struct Args {
   int total_q, batch, hq, hkv, group, max_blocks, max_nodes, num_blocks;
   int tile_nodes;        // nodes of a Q tile: floor(128 / group)
   uint32_t q_box_bytes;  // bytes one TMA box of Q brings
-  int most_rows;         // most rows a block can have
   float scale;
   int32_t *error_flag;
   Join *joins;      // [CTAs]

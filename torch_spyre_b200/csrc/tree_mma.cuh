@@ -47,16 +47,17 @@ struct Cfg {
   // Registers a thread, warpgroups 0-1 / 2 / 3, after setmaxnreg: a softmax
   // thread holds its row's 128 scores.  Sums within the launch's own: 384
   // threads of 168, or 512 of 128.
-  static constexpr int kRegsSoftmax = k8 ? 176 : 208, kRegsIssue = k8 ? 72 : 80, kRegsConvert = 88;
+  static constexpr int kRegsSoftmax = k8 ? 192 : 208, kRegsIssue = k8 ? 56 : 80, kRegsConvert = 72;
   static constexpr int kSticks = D / 64;
   static constexpr int kStickTile = kTileTokens * 128;      // one 64-element column of 128 rows
   static constexpr int kTile = kSticks * kStickTile;        // a Q, K or V tile
-  static constexpr int kSlots = k8 ? 3 : (D == 64 ? 8 : 5);  // operand tiles in flight
+  static constexpr int kQ = k8 ? 1 : 2;                      // most Q tiles of a block
+  static constexpr int kSlots = k8 ? 4 : (D == 64 ? 8 : 5);  // operand tiles in flight
   static constexpr int kRaw = k8 ? 6 : 0;                   // 8-bit pages in flight
   static constexpr int kRawPage = kPageTokens * 128;
   static constexpr int kCtrl = k8 ? 15360 : 3072;
   static constexpr int kOffQ = kCtrl;
-  static constexpr int kOffSlots = kOffQ + 2 * kTile;
+  static constexpr int kOffSlots = kOffQ + kQ * kTile;
   static constexpr int kOffRaw = kOffSlots + kSlots * kTile;
   static constexpr int kSmem = kOffRaw + kRaw * kRawPage;
   // The type of P and V: an 8-bit cache's steps are exact in fp16, whatever q's
@@ -159,33 +160,41 @@ __device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t (&r)[16]) 
 // groups of 8 rows 1024 bytes apart.  N-major (V): 64 head elements of a token
 // are 128 contiguous bytes; groups of 8 tokens 1024 bytes apart, the next 64
 // elements one stick column (128 tokens) on.
-__device__ __forceinline__ uint64_t desc_kmajor(uint32_t addr) {
-  return static_cast<uint64_t>((addr >> 4) & 0x3FFFu) | (uint64_t(1) << 16) | (uint64_t(1024 >> 4) << 32) |
-         (uint64_t(1) << 46) | (uint64_t(2) << 61);
+constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);  // group stride, version 1, 128-byte swizzle
+__device__ __forceinline__ uint32_t desc_kmajor(uint32_t addr) { return (addr >> 4) | (1u << 16); }
+__device__ __forceinline__ uint32_t desc_nmajor(uint32_t addr) {
+  return (addr >> 4) | (uint32_t((kTileTokens * 128) >> 4) << 16);
 }
-__device__ __forceinline__ uint64_t desc_nmajor(uint32_t addr) {
-  return static_cast<uint64_t>((addr >> 4) & 0x3FFFu) | (uint64_t((kTileTokens * 128) >> 4) << 16) |
-         (uint64_t(1024 >> 4) << 32) | (uint64_t(1) << 46) | (uint64_t(2) << 61);
-}
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+// One lane of the converged warp issues (`go`); every operand is the same in
+// all lanes, so that it lives in a uniform register and costs no move per MMA.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc, uint32_t go) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      "{\n\t.reg .pred p, e;\n\t.reg .b64 a, b;\n\tsetp.ne.b32 p, %5, 0;\n\tsetp.ne.b32 e, %6, 0;\n\t"
+      "mov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(kDescHi), "r"(idesc), "r"(acc), "r"(go)
       : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc, uint32_t go) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(acc)
+      "{\n\t.reg .pred p, e;\n\t.reg .b64 b;\n\tsetp.ne.b32 p, %5, 0;\n\tsetp.ne.b32 e, %6, 0;\n\t"
+      "mov.b64 b, {%2, %3};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(kDescHi), "r"(idesc), "r"(acc), "r"(go)
       : "memory");
 }
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t e;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(e));
+  return e;
+}
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return __shfl_sync(0xffffffffu, x, 0); }
 
 // -------------------------------------------------------------------- plan --
 struct Seq {
   int ctx, nodes, q0, blocks, qtiles;
 };
+template <int kQ>
 __device__ __forceinline__ Seq load_seq(const Args &a, int b, bool report) {
   const int cap = a.max_blocks * kPageTokens;
   Seq s;
@@ -202,23 +211,26 @@ __device__ __forceinline__ Seq load_seq(const Args &a, int b, bool report) {
   s.nodes = min(s.nodes, most);
   if (bad && report && a.error_flag) atomicOr(a.error_flag, B200KV_DEVERR_BAD_LEN);
   s.qtiles = (s.nodes + a.tile_nodes - 1) / a.tile_nodes;
-  s.blocks = (s.qtiles + 1) >> 1;
+  s.blocks = (s.qtiles + kQ - 1) / kQ;
   return s;
 }
 // Token tiles of block k: what its last node can see.
+template <int kQ>
 __device__ __forceinline__ int block_tiles(const Args &a, const Seq &s, int k) {
-  const int nodes = a.mask ? s.nodes : min(s.nodes, (2 * k + 2) * a.tile_nodes);
+  const int nodes = a.mask ? s.nodes : min(s.nodes, (k + 1) * kQ * a.tile_nodes);
   return (s.ctx + nodes + kTileTokens - 1) / kTileTokens;
 }
+template <int kQ>
 __device__ __forceinline__ long long head_units(const Args &a, const Seq &s) {
-  if (a.mask) return static_cast<long long>(s.blocks) * (s.blocks ? block_tiles(a, s, 0) : 0);
+  if (a.mask) return static_cast<long long>(s.blocks) * (s.blocks ? block_tiles<kQ>(a, s, 0) : 0);
   long long n = 0;
-  for (int k = 0; k < s.blocks; ++k) n += block_tiles(a, s, k);
+  for (int k = 0; k < s.blocks; ++k) n += block_tiles<kQ>(a, s, k);
   return n;
 }
 
 // The blocks of a CTA's share, one piece (a block, or the part of it in this
 // share) at a time.  Every role walks the same sequence.
+template <int kQ>
 struct Walk {
   Seq s;
   int b, kvh, block, tiles, t0, t1;  // piece: token tiles [t0, t1) of `tiles`
@@ -229,17 +241,17 @@ struct Walk {
     b = c.start_b;
     left = min(c.per, c.total - static_cast<long long>(blockIdx.x) * c.per);
     if (left <= 0) return;
-    s = load_seq(a, b, false);
-    const long long hu = head_units(a, s);
+    s = load_seq<kQ>(a, b, false);
+    const long long hu = head_units<kQ>(a, s);
     kvh = static_cast<int>(c.start_rem / hu);
     long long rem = c.start_rem - kvh * hu;
     block = 0;
     if (a.mask) {
-      tiles = block_tiles(a, s, 0);
+      tiles = block_tiles<kQ>(a, s, 0);
       block = static_cast<int>(rem / tiles);
       rem -= static_cast<long long>(block) * tiles;
     } else {
-      while (rem >= (tiles = block_tiles(a, s, block))) rem -= tiles, ++block;
+      while (rem >= (tiles = block_tiles<kQ>(a, s, block))) rem -= tiles, ++block;
     }
     next_tile = static_cast<int>(rem);
   }
@@ -258,23 +270,23 @@ struct Walk {
       block = 0;
       if (++kvh >= a.hkv) {
         kvh = 0;
-        do s = load_seq(a, ++b, false);
+        do s = load_seq<kQ>(a, ++b, false);
         while (s.nodes == 0);
       }
     }
-    tiles = block_tiles(a, s, block);
+    tiles = block_tiles<kQ>(a, s, block);
   }
-  __device__ __forceinline__ bool two() const { return 2 * block + 1 < s.qtiles; }
+  __device__ __forceinline__ bool two() const { return kQ == 2 && 2 * block + 1 < s.qtiles; }
 };
 
 // First unit, share and total of the line; all threads of the CTA call it.
-template <int kThreads>
+template <int kThreads, int kQ>
 __device__ __forceinline__ void make_plan(const Args &a, Ctrl &c) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int each = (a.batch + kThreads - 1) / kThreads;
   const int b0 = tid * each, b1 = min(b0 + each, a.batch);
   long long mine = 0;
-  for (int b = b0; b < b1; ++b) mine += head_units(a, load_seq(a, b, blockIdx.x == 0)) * a.hkv;
+  for (int b = b0; b < b1; ++b) mine += head_units<kQ>(a, load_seq<kQ>(a, b, blockIdx.x == 0)) * a.hkv;
   long long incl = mine;
 #pragma unroll
   for (int m = 1; m < 32; m <<= 1) {
@@ -294,7 +306,7 @@ __device__ __forceinline__ void make_plan(const Args &a, Ctrl &c) {
   long long at = before + incl - mine;
   if (first >= at && first < at + mine) {
     for (int b = b0; b < b1; ++b) {
-      const long long n = head_units(a, load_seq(a, b, false)) * a.hkv;
+      const long long n = head_units<kQ>(a, load_seq<kQ>(a, b, false)) * a.hkv;
       if (first < at + n) {
         c.start_b = b;
         c.start_rem = first - at;
@@ -338,7 +350,7 @@ __device__ __forceinline__ void producer(const Args &a, Ctrl &c, uint8_t *smem, 
   const uint64_t policy = l2_policy_evict_first();
   bool dead = false;
   uint32_t slot = 0, ring = 0, pieces = 0;  // tiles (16-bit) or pages (8-bit) issued, pieces begun
-  Walk w;
+  Walk<C::kQ> w;
   w.init(a, c);
   while (w.next(a)) {
     const bool two = w.two();
@@ -349,7 +361,7 @@ __device__ __forceinline__ void producer(const Args &a, Ctrl &c, uint8_t *smem, 
       for (int i = 0; i < (two ? 2 : 1); ++i)
         for (int st = 0; st < C::kSticks; ++st)
           tma_3d(smem + C::kOffQ + i * C::kTile + st * C::kStickTile, qm, &c.q_full, st * 64, w.kvh * a.group,
-                 w.s.q0 + (2 * w.block + i) * a.tile_nodes);
+                 w.s.q0 + (C::kQ * w.block + i) * a.tile_nodes);
     }
     ++pieces;
     int window = w.t0 / 16, ids = load_ids(a, w.b, window, pages), ids_next = load_ids(a, w.b, window + 1, pages);
@@ -484,13 +496,21 @@ __device__ __forceinline__ void widen16(uint4 v, uint4 &lo, uint4 &hi) {
 template <typename C, typename T, int kCache>
 __device__ __forceinline__ void converter(const Args &a, Ctrl &c, uint8_t *smem, int warp) {
   const int lane = threadIdx.x & 31, sub = lane & 7;
+  const int first = sub >> 2, c0 = (sub & 3) * 2;
   bool dead = false;
   uint32_t slot = 0, ring = 0;
   unsigned piece = 0;
-  auto tile = [&](bool is_v, int t, int pages, int ctx) {
+  // one tile of K (To the compute type) or V (to fp16)
+  auto tile = [&](auto to, bool is_v, int t, int pages, int ctx) {
+    using To = decltype(to);
     const uint32_t s = slot % C::kSlots;
     wait(&c.empty[s], ((slot / C::kSlots) & 1u) ^ 1u, dead, a.error_flag);
-    uint8_t *dst = smem + C::kOffSlots + s * C::kTile + (sub >> 2) * C::kStickTile;
+    uint8_t *dst = smem + C::kOffSlots + s * C::kTile + first * C::kStickTile;
+    auto put = [&](int trow, uint4 lo, uint4 hi) {
+      uint8_t *line = dst + trow * 128;
+      *reinterpret_cast<uint4 *>(line + (((c0 + first) ^ (trow & 7)) << 4)) = first ? hi : lo;
+      *reinterpret_cast<uint4 *>(line + (((c0 + 1 - first) ^ (trow & 7)) << 4)) = first ? lo : hi;
+    };
     for (int i = 0; i < 2; ++i) {
       const bool page = 2 * t + i < pages;
       const uint32_t r = ring % C::kRaw;
@@ -499,32 +519,34 @@ __device__ __forceinline__ void converter(const Args &a, Ctrl &c, uint8_t *smem,
         wait(&c.raw_full[r], (ring / C::kRaw) & 1u, dead, a.error_flag);
         rows = c.raw_rows[r];
       }
-      const uint8_t *src = smem + C::kOffRaw + r * C::kRawPage;
+      const uint8_t *src = smem + C::kOffRaw + r * C::kRawPage + sub * 16;
+      const int row0 = warp * 16 + (lane >> 3);
+      const bool plain = rows == kPageTokens &&
+                         (kCache == B200KV_I8 || !is_v || t * kTileTokens + (i + 1) * kPageTokens <= ctx);
+      uint4 x[4];
+      if (plain) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int row = warp * 16 + k * 4 + (lane >> 3), trow = i * kPageTokens + row;
-        uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
-        if (row < rows) {
-          const uint4 x = *reinterpret_cast<const uint4 *>(src + row * 128 + sub * 16);
-          if (is_v) {
-            widen16<__half, kCache>(x, lo, hi);
-            if (kCache == B200KV_E4M3 && t * kTileTokens + trow >= ctx) {  // a node's row: e4m3 has NaN
-              const bool hit = drop_non_finite<__half>(lo);
-              if (drop_non_finite<__half>(hi) || hit) atomicMax(&c.bad_piece, piece);
-            }
-          } else {
-            widen16<T, kCache>(x, lo, hi);
-          }
-        }
-        const int c0 = (sub & 3) * 2, first = sub >> 2;  // lanes 4-7 write their second half first
-        uint8_t *line = dst + trow * 128;
-        *reinterpret_cast<uint4 *>(line + (((c0 + first) ^ (trow & 7)) << 4)) = first ? hi : lo;
-        *reinterpret_cast<uint4 *>(line + (((c0 + 1 - first) ^ (trow & 7)) << 4)) = first ? lo : hi;
+        for (int k = 0; k < 4; ++k) x[k] = *reinterpret_cast<const uint4 *>(src + (row0 + 4 * k) * 128);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          x[k] = row0 + 4 * k < rows ? *reinterpret_cast<const uint4 *>(src + (row0 + 4 * k) * 128) : make_uint4(0, 0, 0, 0);
       }
       if (page) {
         __syncwarp();
         if (lane == 0) arrive(&c.raw_empty[r]);
         ++ring;
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int trow = i * kPageTokens + row0 + 4 * k;
+        uint4 lo, hi;
+        widen16<To, kCache>(x[k], lo, hi);
+        if (!plain && kCache == B200KV_E4M3 && is_v && t * kTileTokens + trow >= ctx) {  // a node's row: e4m3 has NaN
+          const bool hit = drop_non_finite<__half>(lo);
+          if (drop_non_finite<__half>(hi) || hit) atomicMax(&c.bad_piece, piece);
+        }
+        put(trow, lo, hi);
       }
     }
     fence_async_smem();
@@ -532,50 +554,55 @@ __device__ __forceinline__ void converter(const Args &a, Ctrl &c, uint8_t *smem,
     if (lane == 0) arrive(&c.full[s]);
     ++slot;
   };
-  Walk w;
+  Walk<C::kQ> w;
   w.init(a, c);
   while (w.next(a)) {
     ++piece;
     const int pages = (w.s.ctx + w.s.nodes + kPageTokens - 1) / kPageTokens;
     const int lead = w.two() ? 1 : 2;
-    for (int t = w.t0; t < min(w.t0 + lead, w.t1); ++t) tile(false, t, pages, w.s.ctx);
+    for (int t = w.t0; t < min(w.t0 + lead, w.t1); ++t) tile(T(), false, t, pages, w.s.ctx);
     for (int t = w.t0; t < w.t1; ++t) {
-      tile(true, t, pages, w.s.ctx);
-      if (t + lead < w.t1) tile(false, t + lead, pages, w.s.ctx);
+      tile(__half(), true, t, pages, w.s.ctx);
+      if (t + lead < w.t1) tile(T(), false, t + lead, pages, w.s.ctx);
     }
     w.advance(a);
   }
 }
 
-// One thread issues every MMA.
+// One warp, converged, issues every MMA from an elected lane.
 template <typename C, int D>
-__device__ __forceinline__ void mma_issuer(const Args &a, Ctrl &c, uint8_t *smem, uint32_t tmem) {
+__device__ __forceinline__ void mma_issuer(const Args &a, Ctrl &c, uint8_t *smem, uint32_t tmem_any) {
   bool dead = false;
   uint32_t slot = 0, pieces = 0, p_uses[2] = {0, 0};
+  const uint32_t go = elect_one(), tmem = uniform(tmem_any);
   const uint32_t qbase = smem_u32(smem + C::kOffQ), sbase = smem_u32(smem + C::kOffSlots);
   const uint32_t negate = a.scale < 0.f ? 1u << 13 : 0u;  // a negative scale turns Q's sign
+  auto done = [&](uint64_t *bar) {
+    if (go) commit(bar);
+  };
   auto ready = [&](uint32_t n) {
     wait(&c.full[n % C::kSlots], (n / C::kSlots) & 1u, dead, a.error_flag);
     fence_after();
-    return sbase + (n % C::kSlots) * C::kTile;
+    return uniform(sbase + (n % C::kSlots) * C::kTile);
   };
   auto qk = [&](int w, int qtile, uint32_t k) {
-    const uint32_t q = qbase + qtile * C::kTile;
+    const uint32_t qd = desc_kmajor(qbase + qtile * C::kTile), kd = desc_kmajor(k);
 #pragma unroll
     for (int i = 0; i < D / 16; ++i) {
-      const uint32_t off = (i >> 2) * C::kStickTile + (i & 3) * 32;
-      mma_ss(tmem + col_s(w), desc_kmajor(q + off), desc_kmajor(k + off), C::kIdescQK | negate, i > 0);
+      const uint32_t off = ((i >> 2) * C::kStickTile + (i & 3) * 32) >> 4;
+      mma_ss(tmem + col_s(w), qd + off, kd + off, C::kIdescQK | negate, i > 0, go);
     }
-    commit(&c.s_full[w]);
+    done(&c.s_full[w]);
   };
   auto pv = [&](int w, uint32_t v, bool first) {
     wait(&c.p_ready[w], p_uses[w]++ & 1u, dead, a.error_flag);
     fence_after();
+    const uint32_t vd = desc_nmajor(v);
 #pragma unroll
     for (int i = 0; i < kTileTokens / 16; ++i)
-      mma_ts(tmem + col_o(w), tmem + col_s(w) + i * 8, desc_nmajor(v + i * 2048), C::kIdescPV, !first || i > 0);
+      mma_ts(tmem + col_o(w), tmem + col_s(w) + i * 8, vd + (i * 2048 >> 4), C::kIdescPV, !first || i > 0, go);
   };
-  Walk w;
+  Walk<C::kQ> w;
   w.init(a, c);
   while (w.next(a)) {
     wait(&c.q_full, pieces++ & 1u, dead, a.error_flag);
@@ -586,7 +613,7 @@ __device__ __forceinline__ void mma_issuer(const Args &a, Ctrl &c, uint8_t *smem
       uint32_t k = ready(slot);
       qk(0, 0, k);
       qk(1, 1, k);
-      commit(&c.empty[slot++ % C::kSlots]);
+      done(&c.empty[slot++ % C::kSlots]);
       for (int t = 0; t < n; ++t) {
         const uint32_t vs = slot++, v = ready(vs);
         const bool more = t + 1 < n;
@@ -594,36 +621,43 @@ __device__ __forceinline__ void mma_issuer(const Args &a, Ctrl &c, uint8_t *smem
         if (more)
           qk(0, 0, k = ready(slot));
         else
-          commit(&c.o_full[0]);
+          done(&c.o_full[0]);
         pv(1, v, t == 0);
-        commit(&c.empty[vs % C::kSlots]);
+        done(&c.empty[vs % C::kSlots]);
         if (more) {
           qk(1, 1, k);
-          commit(&c.empty[slot++ % C::kSlots]);
+          done(&c.empty[slot++ % C::kSlots]);
         } else {
-          commit(&c.o_full[1]);
+          done(&c.o_full[1]);
         }
       }
     } else {
       // stream t & 1 takes tile t
-      for (int t = 0; t < min(2, n); ++t) {
-        qk(t & 1, 0, ready(slot));
-        commit(&c.empty[slot++ % C::kSlots]);
-      }
-      for (int t = 0; t < n; ++t) {
-        pv(t & 1, ready(slot), t < 2);
-        commit(&c.empty[slot++ % C::kSlots]);
+      auto pair = [&](int w0, int t) {
+        pv(w0, ready(slot), t < 2);
+        done(&c.empty[slot++ % C::kSlots]);
         if (t + 2 < n) {
-          qk(t & 1, 0, ready(slot));
-          commit(&c.empty[slot++ % C::kSlots]);
+          qk(w0, 0, ready(slot));
+          done(&c.empty[slot++ % C::kSlots]);
         } else {
-          commit(&c.o_full[t & 1]);
+          done(&c.o_full[w0]);
         }
+      };
+      qk(0, 0, ready(slot));
+      done(&c.empty[slot++ % C::kSlots]);
+      if (n > 1) {
+        qk(1, 0, ready(slot));
+        done(&c.empty[slot++ % C::kSlots]);
+      }
+      for (int t = 0; t < n; t += 2) {
+        pair(0, t);
+        if (t + 1 < n) pair(1, t + 1);
       }
     }
-    commit(&c.q_empty);
+    done(&c.q_empty);
     w.advance(a);
   }
+  __syncwarp();
 }
 
 __device__ __forceinline__ uint32_t low_bits(int n) { return n >= 32 ? ~0u : (n <= 0 ? 0u : (1u << n) - 1u); }
@@ -690,22 +724,29 @@ template <typename C, int D, bool kTail>
 __device__ __forceinline__ void weigh(uint32_t ts, uint32_t to, const uint32_t (&vis)[4], float cl, const Factors *fac,
                                       bool first, bool live, float &m, float &l) {
   uint32_t s[4][32];
+  if constexpr (!C::k8) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) tmem_ld32(ts + 32 * i, s[i]);
+    for (int i = 0; i < 4; ++i) tmem_ld32(ts + 32 * i, s[i]);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) wait_ld(s[i]);
+    for (int i = 0; i < 4; ++i) wait_ld(s[i]);
+  }
   float top[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     if constexpr (C::k8) {
+      // a quarter at a time, so that registers are left to fetch its factors ahead
+      tmem_ld32(ts + 32 * i, s[i]);
+      float4 k[8], v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) k[j] = fac->k[8 * i + j], v[j] = fac->log2v[8 * i + j];
+      wait_ld(s[i]);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float4 k = fac->k[8 * i + j], v = fac->log2v[8 * i + j];
         uint32_t *r = &s[i][4 * j];
-        const float2 lo = fma2(make_float2(__uint_as_float(r[0]), __uint_as_float(r[1])), make_float2(k.x, k.y),
-                               make_float2(v.x, v.y));
-        const float2 hi = fma2(make_float2(__uint_as_float(r[2]), __uint_as_float(r[3])), make_float2(k.z, k.w),
-                               make_float2(v.z, v.w));
+        const float2 lo = fma2(make_float2(__uint_as_float(r[0]), __uint_as_float(r[1])), make_float2(k[j].x, k[j].y),
+                               make_float2(v[j].x, v[j].y));
+        const float2 hi = fma2(make_float2(__uint_as_float(r[2]), __uint_as_float(r[3])), make_float2(k[j].z, k[j].w),
+                               make_float2(v[j].z, v[j].w));
         r[0] = __float_as_uint(lo.x), r[1] = __float_as_uint(lo.y);
         r[2] = __float_as_uint(hi.x), r[3] = __float_as_uint(hi.y);
       }
@@ -803,14 +844,14 @@ __device__ __forceinline__ void softmax(const Args &a, Ctrl &c, uint8_t *smem, u
   bool dead = false;
   uint32_t s_uses = 0, o_uses[2] = {0, 0}, slot = 0;
   unsigned piece = 0;
-  Walk wk;
+  Walk<C::kQ> wk;
   wk.init(a, c);
   while (wk.next(a)) {
     ++piece;
     const bool two = wk.two();
     const int n = wk.t1 - wk.t0, lead = two ? 1 : 2;
     const int len = wk.s.ctx + wk.s.nodes;
-    const int qt = 2 * wk.block + (two ? w : 0);
+    const int qt = C::kQ * wk.block + (two ? w : 0);
     const int node = qt * a.tile_nodes + tid / a.group;
     const bool live = tid < a.tile_nodes * a.group && node < wk.s.nodes;
     const bool warp_live = __any_sync(0xffffffffu, live);
@@ -969,8 +1010,8 @@ __device__ __forceinline__ void softmax(const Args &a, Ctrl &c, uint8_t *smem, u
     if (split && wk.t0 > 0 && w == 0 && tid == 0 && wk.t0 <= c.per) {
       Join j;
       j.rows0 = static_cast<int64_t>(wk.s.q0);
-      j.node0 = 2 * wk.block * a.tile_nodes;
-      j.nodes = min(wk.s.nodes - j.node0, 2 * a.tile_nodes);
+      j.node0 = C::kQ * wk.block * a.tile_nodes;
+      j.nodes = min(wk.s.nodes - j.node0, C::kQ * a.tile_nodes);
       j.kvh = wk.kvh;
       // pieces: the CTA before this one, this one, and on to the block's end
       j.first_slot = 2 * (static_cast<int>(blockIdx.x) - 1) + (wk.t0 == c.per ? 0 : 1);
@@ -1023,7 +1064,7 @@ __global__ void __launch_bounds__((Cfg<T, D, kCache>::kThreads), 1)
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (tid == 0) a.joins[blockIdx.x].nodes = 0;  // no block begins to be split here, unless the epilogue says so
-  make_plan<C::kThreads>(a, c);
+  make_plan<C::kThreads, C::kQ>(a, c);
   fence_before();
   __syncthreads();
   fence_after();
@@ -1036,8 +1077,7 @@ __global__ void __launch_bounds__((Cfg<T, D, kCache>::kThreads), 1)
     if (warp == 8) {
       producer<C>(a, c, smem, &qm, &km, &vm);
     } else if (warp == 9) {
-      if ((tid & 31) == 0) mma_issuer<C, D>(a, c, smem, tmem);
-      __syncwarp();
+      mma_issuer<C, D>(a, c, smem, tmem);
     }
   } else {
     if constexpr (C::k8) {
@@ -1128,7 +1168,7 @@ int launch(const CUtensorMap &qm, const CUtensorMap &km, const CUtensorMap &vm, 
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   B200KV_CUDA_TRY(cudaLaunchKernelEx(&cfg, tree_kernel<T, D, kCache>, qm, km, vm, a));
-  cfg.gridDim = dim3(static_cast<unsigned>(ctas), a.most_rows > kTileRows ? 8 : 4);
+  cfg.gridDim = dim3(static_cast<unsigned>(ctas), C::kQ == 2 && a.max_nodes > a.tile_nodes ? 8 : 4);
   cfg.blockDim = dim3(256);
   cfg.dynamicSmemBytes = 0;
   B200KV_CUDA_TRY(cudaLaunchKernelEx(&cfg, tree_join_kernel<T, D>, a));
