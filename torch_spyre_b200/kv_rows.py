@@ -17,10 +17,10 @@ from typing import Optional
 
 import torch
 
-from . import _lib
+from ._eager import direct, launch, written
 from .layout import PAGE_TOKENS
-from .ops import _maybe_check_flag, _ptr, _require_cuda, _stream_ptr
-from .rotations import check_table, dtype_code
+from .ops import _maybe_check_flag, _ptr, _require_cuda
+from .rotations import DTYPE_CODES, ROTARY_DTYPES, check_table
 
 DTYPES_16 = (torch.float16, torch.bfloat16)
 DTYPES_8 = (torch.int8, torch.float8_e4m3fn)
@@ -41,20 +41,22 @@ def empty_row_pool(num_blocks: int, num_kv_heads: int, head_dim: int = 128, dtyp
 
 def check_row_pool(pool: torch.Tensor, scales: Optional[torch.Tensor], name: str) -> tuple[int, int, int]:
     """(num_blocks, Hkv, D) of a pool, its scales checked."""
-    stick = 128 if pool.dtype in DTYPES_8 else 64
-    if pool.dtype not in DTYPES_8 + DTYPES_16 or pool.dim() != 5 or pool.shape[3:] != (PAGE_TOKENS, stick) \
-            or pool.shape[2] * stick not in (64, 128) or not pool.is_contiguous():
+    dtype, shape = pool.dtype, pool.shape
+    k8 = dtype in DTYPES_8
+    stick = 128 if k8 else 64
+    if not (k8 or dtype in DTYPES_16) or len(shape) != 5 or shape[3] != PAGE_TOKENS or shape[4] != stick \
+            or shape[2] * stick not in (64, 128) or not pool.is_contiguous():
         raise ValueError(f"{name}_pool must be contiguous [num_blocks, Hkv, D/64, 64, 64] (fp16, bf16) or "
-                         f"[num_blocks, Hkv, 1, 64, 128] (int8, float8_e4m3fn), got {tuple(pool.shape)} {pool.dtype}")
-    if pool.dtype in DTYPES_8:
+                         f"[num_blocks, Hkv, 1, 64, 128] (int8, float8_e4m3fn), got {tuple(shape)} {dtype}")
+    if k8:
         if scales is None:
             raise ValueError(f"8-bit pools need {name}_scales")
-        if scales.dtype != torch.float32 or scales.shape != (pool.shape[0], pool.shape[1], PAGE_TOKENS) \
+        if scales.dtype != torch.float32 or scales.shape != (shape[0], shape[1], PAGE_TOKENS) \
                 or not scales.is_contiguous() or scales.device != pool.device:
             raise ValueError(f"{name}_scales must be contiguous fp32 [num_blocks, Hkv, 64] on the pool's device")
     elif scales is not None:
         raise ValueError(f"a 16-bit pool takes no {name}_scales")
-    return pool.shape[0], pool.shape[1], pool.shape[2] * stick
+    return shape[0], shape[1], shape[2] * stick
 
 
 def check_row_pools(k_pool, v_pool, k_scales, v_scales) -> tuple[int, int, int]:
@@ -66,13 +68,11 @@ def check_row_pools(k_pool, v_pool, k_scales, v_scales) -> tuple[int, int, int]:
 
 
 def _check_slots(slots: torch.Tensor, tokens: int, device: torch.device) -> None:
-    if slots.dtype != torch.int64 or slots.shape != (tokens,) or not slots.is_contiguous() or slots.device != device:
+    if slots.dtype != torch.int64 or slots.dim() != 1 or len(slots) != tokens or not slots.is_contiguous() or slots.device != device:
         raise ValueError("slots must be a contiguous int64 [N] tensor on the pool's device")
 
 
-@torch.library.custom_op("b200kv::kv_store", mutates_args=("k_pool", "v_pool", "k_scales", "v_scales"),
-                         device_types="cuda")
-def _kv_store_op(
+def _kv_store_impl(
     k_new: torch.Tensor,
     v_new: torch.Tensor,
     k_pool: torch.Tensor,
@@ -88,37 +88,45 @@ def _kv_store_op(
 ) -> torch.Tensor:
     _require_cuda(k_new, v_new, k_pool, v_pool, slots)
     NB, Hkv, D = check_row_pools(k_pool, v_pool, k_scales, v_scales)
+    device, dtype = k_pool.device, k_new.dtype
     N = k_new.shape[0] if k_new.dim() == 3 else -1
     for rows, name in ((k_new, "k_new"), (v_new, "v_new")):
-        if rows.shape != (N, Hkv, D) or rows.dtype not in DTYPES_16 or rows.dtype != k_new.dtype \
-                or rows.stride(2) != 1 or rows.device != k_pool.device:
+        if rows.shape != (N, Hkv, D) or dtype not in DTYPES_16 or rows.dtype != dtype or rows.stride(2) != 1 \
+                or rows.device != device:
             raise ValueError(f"{name} must be fp16 or bf16 [N, {Hkv}, {D}] with a contiguous head_dim on the pools' "
                              f"device, got {tuple(rows.shape)} {rows.dtype}")
-    if k_pool.dtype in DTYPES_16 and k_pool.dtype != k_new.dtype:
-        raise ValueError(f"a {k_pool.dtype} pool cannot take {k_new.dtype} rows")
-    _check_slots(slots, N, k_pool.device)
+    if k_scales is None and k_pool.dtype != dtype:
+        raise ValueError(f"a {k_pool.dtype} pool cannot take {dtype} rows")
+    _check_slots(slots, N, device)
     if q is not None:
         if table is None:
             raise ValueError("q is taken to be turned: it needs a table")
-        if q.dim() != 3 or q.shape[0] != N or q.shape[2] != D or q.dtype != k_new.dtype or q.stride(2) != 1 \
-                or q.device != k_pool.device:
+        if q.dim() != 3 or q.shape[0] != N or q.shape[2] != D or q.dtype != dtype or q.stride(2) != 1 \
+                or q.device != device:
             raise ValueError(f"q must be [N, Hq, {D}] of the rows' dtype with a contiguous head_dim")
+        Hq, out, q_args = q.shape[1], torch.empty_like(q, memory_format=torch.contiguous_format), (
+            q.data_ptr(), q.stride(0), q.stride(1))
+    else:
+        Hq, out, q_args = 0, k_new.new_empty((N, 0, D)), (None, 0, 0)
     if table is not None:
         if positions is None:
             raise ValueError("a table needs positions")
-        check_table(table, positions, N, D, k_pool.device)
-    out = k_new.new_empty((N, 0 if q is None else q.shape[1], D))
-    _lib.call(
-        "b200kv_kv_store",
-        _ptr(q), 0 if q is None else q.stride(0), 0 if q is None else q.stride(1), out.data_ptr(),
+        check_table(table, positions, N, D, device)
+        turn = (table.data_ptr(), table.shape[0], 2 * table.shape[1], positions.data_ptr())
+    else:
+        turn = (None, 0, 0, None)
+    launch(
+        "b200kv_kv_store", device, *q_args, out.data_ptr(),
         k_new.data_ptr(), k_new.stride(0), k_new.stride(1), v_new.data_ptr(), v_new.stride(0), v_new.stride(1),
-        dtype_code(k_new.dtype), k_pool.data_ptr(), v_pool.data_ptr(), dtype_code(k_pool.dtype),
-        _ptr(k_scales), _ptr(v_scales), slots.data_ptr(),
-        _ptr(table), 0 if table is None else table.shape[0], 0 if table is None else 2 * table.shape[1],
-        _ptr(positions), int(interleaved), N, out.shape[1], Hkv, D, NB, _ptr(error_flag), _stream_ptr(k_new.device),
+        DTYPE_CODES[dtype], k_pool.data_ptr(), v_pool.data_ptr(), DTYPE_CODES[k_pool.dtype],
+        _ptr(k_scales), _ptr(v_scales), slots.data_ptr(), *turn, interleaved, N, Hq, Hkv, D, NB, _ptr(error_flag),
     )
     _maybe_check_flag(error_flag, "kv_store")
     return out
+
+
+_kv_store_op = torch.library.custom_op("b200kv::kv_store", _kv_store_impl, device_types="cuda",
+                                       mutates_args=("k_pool", "v_pool", "k_scales", "v_scales"))
 
 
 @_kv_store_op.register_fake
@@ -149,25 +157,32 @@ def kv_store(
     (:func:`torch_spyre_b200.rotary_table`) k is turned first (not rounded
     in between); ``q`` [N, Hq, D] is turned by the same launch and returned.
     Slots must be distinct; negative slots skip their row."""
-    out = torch.ops.b200kv.kv_store(k_new, v_new, k_pool, v_pool, slots, k_scales, v_scales, q, table, positions,
-                                    bool(interleaved), error_flag)
+    args = (k_new, v_new, k_pool, v_pool, slots, k_scales, v_scales, q, table, positions, bool(interleaved), error_flag)
+    if direct(k_new):
+        out = _kv_store_impl(*args)
+        written(k_pool, v_pool, k_scales, v_scales)
+    else:
+        out = torch.ops.b200kv.kv_store(*args)
     return None if q is None else out
 
 
-@torch.library.custom_op("b200kv::kv_load", mutates_args=(), device_types="cuda")
-def _kv_load_op(pool: torch.Tensor, slots: torch.Tensor, scales: Optional[torch.Tensor], dtype: torch.dtype,
-                error_flag: Optional[torch.Tensor]) -> torch.Tensor:
+def _kv_load_impl(pool: torch.Tensor, slots: torch.Tensor, scales: Optional[torch.Tensor], dtype: torch.dtype,
+                  error_flag: Optional[torch.Tensor]) -> torch.Tensor:
     _require_cuda(pool, slots)
     NB, Hkv, D = check_row_pool(pool, scales, "")
     N = slots.shape[0] if slots.dim() == 1 else -1
-    _check_slots(slots, N, pool.device)
-    if dtype not in DTYPES_16 + (torch.float32,):
+    device = pool.device
+    _check_slots(slots, N, device)
+    if dtype not in ROTARY_DTYPES:
         raise ValueError(f"dtype must be fp16, bf16 or fp32, got {dtype}")
-    out = torch.empty((N, Hkv, D), dtype=dtype, device=pool.device)
-    _lib.call("b200kv_kv_load", pool.data_ptr(), dtype_code(pool.dtype), _ptr(scales), slots.data_ptr(),
-              out.data_ptr(), dtype_code(dtype), N, Hkv, D, NB, _ptr(error_flag), _stream_ptr(pool.device))
+    out = torch.empty((N, Hkv, D), dtype=dtype, device=device)
+    launch("b200kv_kv_load", device, pool.data_ptr(), DTYPE_CODES[pool.dtype], _ptr(scales), slots.data_ptr(),
+           out.data_ptr(), DTYPE_CODES[dtype], N, Hkv, D, NB, _ptr(error_flag))
     _maybe_check_flag(error_flag, "kv_load")
     return out
+
+
+_kv_load_op = torch.library.custom_op("b200kv::kv_load", _kv_load_impl, mutates_args=(), device_types="cuda")
 
 
 @_kv_load_op.register_fake
@@ -182,4 +197,5 @@ def kv_load(pool: torch.Tensor, slots: torch.Tensor, scales: Optional[torch.Tens
     Negative slots give rows of zeros."""
     if dtype is None:
         dtype = pool.dtype if pool.dtype in DTYPES_16 else torch.float16
-    return torch.ops.b200kv.kv_load(pool, slots, scales, dtype, error_flag)
+    op = _kv_load_impl if direct(pool) else torch.ops.b200kv.kv_load
+    return op(pool, slots, scales, dtype, error_flag)

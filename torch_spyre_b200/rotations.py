@@ -18,17 +18,15 @@ from typing import Optional
 import torch
 
 from . import _lib
-from .ops import _maybe_check_flag, _ptr, _require_cuda, _stream_ptr
+from ._eager import direct, launch
+from .ops import _maybe_check_flag, _ptr, _require_cuda
 
 ROTARY_SCALINGS = ("none", "linear", "ntk", "yarn")
 
 
-def dtype_code(dtype: torch.dtype) -> int:
-    """enum b200kv_dtype of a torch dtype (ValueError if the library has none)."""
-    code = _lib.DTYPES.get(str(dtype).removeprefix("torch."))
-    if code is None:
-        raise ValueError(f"unsupported dtype {dtype}")
-    return code
+# enum b200kv_dtype of the torch dtypes
+DTYPE_CODES = {getattr(torch, name): code for name, code in _lib.DTYPES.items()}
+ROTARY_DTYPES = {d: DTYPE_CODES[d] for d in (torch.float16, torch.bfloat16, torch.float32)}
 
 
 def rotary_table(max_pos: int, rotary_dim: int, base: float = 10000.0, scaling: str = "none", factor: float = 1.0,
@@ -80,38 +78,47 @@ def rotary_table(max_pos: int, rotary_dim: int, base: float = 10000.0, scaling: 
 
 def check_table(table: torch.Tensor, positions: torch.Tensor, tokens: int, head_dim: int,
                 device: torch.device) -> None:
-    if table.dtype != torch.float32 or table.dim() != 3 or table.shape[2] != 2 or not table.is_contiguous() \
+    shape = table.shape
+    if table.dtype != torch.float32 or len(shape) != 3 or shape[2] != 2 or not table.is_contiguous() \
             or table.device != device:
         raise ValueError("table must be a contiguous fp32 [max_pos, rotary_dim / 2, 2] tensor on the rows' device, "
                          f"got {tuple(table.shape)} {table.dtype} on {table.device}")
-    if not 0 < 2 * table.shape[1] <= head_dim:
-        raise ValueError(f"the table turns {2 * table.shape[1]} elements of a head of {head_dim}")
-    if positions.dtype != torch.int32 or positions.shape != (tokens,) or not positions.is_contiguous() \
-            or positions.device != device:
+    if not 0 < 2 * shape[1] <= head_dim:
+        raise ValueError(f"the table turns {2 * shape[1]} elements of a head of {head_dim}")
+    if positions.dtype != torch.int32 or positions.dim() != 1 or len(positions) != tokens \
+            or not positions.is_contiguous() or positions.device != device:
         raise ValueError("positions must be a contiguous int32 [T] tensor on the rows' device")
 
 
-@torch.library.custom_op("b200kv::rotary", mutates_args=(), device_types="cuda")
-def _rotary_op(x: torch.Tensor, table: torch.Tensor, positions: torch.Tensor, interleaved: bool, transpose: bool,
-               error_flag: Optional[torch.Tensor]) -> torch.Tensor:
+def _rotary_impl(x: torch.Tensor, table: torch.Tensor, positions: torch.Tensor, interleaved: bool, transpose: bool,
+                 error_flag: Optional[torch.Tensor]) -> torch.Tensor:
     _require_cuda(x, table, positions)
-    if x.dim() != 3 or x.dtype not in (torch.float16, torch.bfloat16, torch.float32) or (x.stride(2) != 1
-                                                                                         and x.shape[2] != 1):
+    if x.dim() != 3 or x.dtype not in ROTARY_DTYPES or (x.stride(2) != 1 and x.shape[2] != 1):
         raise ValueError("x must be fp16, bf16 or fp32 [T, H, D] with a contiguous head_dim, "
                          f"got {tuple(x.shape)} {x.dtype}")
     T, H, D = x.shape
-    check_table(table, positions, T, D, x.device)
-    out = torch.empty((T, H, D), dtype=x.dtype, device=x.device)
-    _lib.call("b200kv_rotary", x.data_ptr(), dtype_code(x.dtype), x.stride(0), x.stride(1), out.data_ptr(),
-              table.data_ptr(), table.shape[0], 2 * table.shape[1], positions.data_ptr(), T, H, D, int(interleaved),
-              int(transpose), _ptr(error_flag), _stream_ptr(x.device))
+    device = x.device
+    check_table(table, positions, T, D, device)
+    out = torch.empty_like(x, memory_format=torch.contiguous_format)
+    launch("b200kv_rotary", device, x.data_ptr(), ROTARY_DTYPES[x.dtype], x.stride(0), x.stride(1), out.data_ptr(),
+           table.data_ptr(), table.shape[0], 2 * table.shape[1], positions.data_ptr(), T, H, D, interleaved, transpose,
+           _ptr(error_flag))
     _maybe_check_flag(error_flag, "rotary")
     return out
+
+
+_rotary_op = torch.library.custom_op("b200kv::rotary", _rotary_impl, mutates_args=(), device_types="cuda")
 
 
 @_rotary_op.register_fake
 def _(x, table, positions, interleaved, transpose, error_flag):
     return x.new_empty(x.shape)
+
+
+def _turn_back(grad, table, positions, interleaved, transpose, error_flag):
+    if grad.stride(-1) != 1:  # e.g. the expanded gradient of a sum
+        grad = grad.contiguous()
+    return _turn(grad, table, positions, interleaved, not transpose, error_flag)
 
 
 def _rotary_setup(ctx, inputs, output):
@@ -121,15 +128,30 @@ def _rotary_setup(ctx, inputs, output):
 
 
 def _rotary_backward(ctx, grad):
-    table, positions = ctx.saved_tensors
-    interleaved, transpose, error_flag = ctx.turn
-    if grad.stride(-1) != 1:  # e.g. the expanded gradient of a sum
-        grad = grad.contiguous()
-    return (torch.ops.b200kv.rotary(grad, table, positions, interleaved, not transpose, error_flag), None, None, None,
-            None, None)
+    return (_turn_back(grad, *ctx.saved_tensors, *ctx.turn), None, None, None, None, None)
 
 
 _rotary_op.register_autograd(_rotary_backward, setup_context=_rotary_setup)
+
+
+class _Rotary(torch.autograd.Function):
+    """The operator's gradient without the dispatcher (the same map turned the other way)."""
+
+    @staticmethod
+    def forward(ctx, x, table, positions, interleaved, transpose, error_flag):
+        ctx.save_for_backward(table, positions)
+        ctx.turn = (interleaved, transpose, error_flag)
+        return _rotary_impl(x, table, positions, interleaved, transpose, error_flag)
+
+    backward = staticmethod(_rotary_backward)
+
+
+def _turn(x, table, positions, interleaved, transpose, error_flag):
+    if not direct(x):
+        return torch.ops.b200kv.rotary(x, table, positions, interleaved, transpose, error_flag)
+    if x.requires_grad and torch.is_grad_enabled():
+        return _Rotary.apply(x, table, positions, interleaved, transpose, error_flag)
+    return _rotary_impl(x, table, positions, interleaved, transpose, error_flag)
 
 
 def rotary(x: torch.Tensor, table: torch.Tensor, positions: torch.Tensor, interleaved: bool = False,
@@ -140,4 +162,4 @@ def rotary(x: torch.Tensor, table: torch.Tensor, positions: torch.Tensor, interl
     (2i, 2i + 1) when ``interleaved``; the other elements are copied.  fp32
     arithmetic, rounded once.  Differentiable in x (the table is a constant).  A
     position outside the table is clamped and sets ``DEVERR_BAD_LEN``."""
-    return torch.ops.b200kv.rotary(x, table, positions, bool(interleaved), False, error_flag)
+    return _turn(x, table, positions, bool(interleaved), False, error_flag)
