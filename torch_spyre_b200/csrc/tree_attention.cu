@@ -174,7 +174,7 @@ extern "C" int b200kv_tree_attention(const void *q, int32_t q_dtype, int64_t q_s
   a.block_table = block_table, a.bt_stride = block_table_stride;
   a.ctx = context_lens, a.indptr = q_indptr;
   a.mask = reinterpret_cast<const uint64_t *>(tree_mask), a.words = mask_words;
-  a.k_scales = k_scales, a.v_scales = v_scales, a.v_pool = v_pool;
+  a.k_scales = k_scales, a.v_scales = v_scales, a.k_pool = k_pool, a.v_pool = v_pool;
   a.out = out, a.lse = lse;
   a.total_q = static_cast<int>(total_q), a.batch = static_cast<int>(batch);
   a.hq = static_cast<int>(num_q_heads), a.hkv = static_cast<int>(num_kv_heads), a.group = group;

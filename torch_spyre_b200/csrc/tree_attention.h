@@ -23,7 +23,7 @@ struct Args {
   const uint64_t *mask;  // [N, words], null: a chain
   int64_t words;
   const float *k_scales, *v_scales;
-  const void *v_pool;
+  const void *k_pool, *v_pool;
   void *out;  // contiguous [N, Hq, D]
   float *lse;
   int total_q, batch, hq, hkv, group, max_blocks, max_nodes, num_blocks;

@@ -405,7 +405,10 @@ __device__ __forceinline__ void producer(const Args &a, Ctrl &c, uint8_t *smem, 
             } else {
               const int page = id * a.hkv + w.kvh;
               mbar_arrive_expect_tx(&c.raw_full[r], C::kRawPage);
-              tma_load_3d(smem + C::kOffRaw + r * C::kRawPage, map, &c.raw_full[r], 0, 0, page, policy);
+              // a page is one contiguous run of 8 KiB
+              bulk_load(smem + C::kOffRaw + r * C::kRawPage,
+                        static_cast<const uint8_t *>(is_v ? a.v_pool : a.k_pool) + static_cast<int64_t>(page) * C::kRawPage,
+                        C::kRawPage, &c.raw_full[r]);
             }
           }
           ++ring;
@@ -448,10 +451,10 @@ __device__ __forceinline__ bool drop_non_finite(uint4 &v) {
   return hit;
 }
 
-// Eight-bit pages -> operand tiles.  Thread: 16 bytes of a row, 4 rows per
-// warp and step; the two 16-byte results of lanes 4-7 of a row are written in
-// swapped order so that the eight lanes of a row hit eight different 16-byte
-// bank groups in the swizzled tile.
+// Eight-bit pages -> operand tiles.  A lane takes 16 bytes of a row and writes
+// the two 16-byte vectors they become.  Lanes 0-3 of eight take the first half
+// of row r, lanes 4-7 the second half of row r ^ 1: the swizzle then puts the
+// eight vectors of a store on eight different bank groups, as it does the reads.
 //
 // Every step is exact in the operand type.  int8 -> fp16: 0x64xx is 1024 + xx,
 // taken as b + 128, less 1152.  int8 -> bf16: b = (b & 127) - (b & 128), both
@@ -496,7 +499,12 @@ __device__ __forceinline__ void widen16(uint4 v, uint4 &lo, uint4 &hi) {
 template <typename C, typename T, int kCache>
 __device__ __forceinline__ void converter(const Args &a, Ctrl &c, uint8_t *smem, int warp) {
   const int lane = threadIdx.x & 31, sub = lane & 7;
-  const int first = sub >> 2, c0 = (sub & 3) * 2;
+  // this lane's rows of a page are row0, row0 + 4, + 8, + 12; rows four apart
+  // differ in bit 2 of the swizzle's XOR
+  const int row0 = warp * 16 + ((lane >> 3) ^ (sub >> 2));
+  const int chunk = (sub & 3) * 2;
+  const uint32_t from = row0 * 128 + sub * 16;
+  const uint32_t even = (sub >> 2) * C::kStickTile + row0 * 128, at0 = (chunk ^ (row0 & 7)) << 4;
   bool dead = false;
   uint32_t slot = 0, ring = 0;
   unsigned piece = 0;
@@ -505,12 +513,7 @@ __device__ __forceinline__ void converter(const Args &a, Ctrl &c, uint8_t *smem,
     using To = decltype(to);
     const uint32_t s = slot % C::kSlots;
     wait(&c.empty[s], ((slot / C::kSlots) & 1u) ^ 1u, dead, a.error_flag);
-    uint8_t *dst = smem + C::kOffSlots + s * C::kTile + first * C::kStickTile;
-    auto put = [&](int trow, uint4 lo, uint4 hi) {
-      uint8_t *line = dst + trow * 128;
-      *reinterpret_cast<uint4 *>(line + (((c0 + first) ^ (trow & 7)) << 4)) = first ? hi : lo;
-      *reinterpret_cast<uint4 *>(line + (((c0 + 1 - first) ^ (trow & 7)) << 4)) = first ? lo : hi;
-    };
+    uint8_t *dst = smem + C::kOffSlots + s * C::kTile + even;
     for (int i = 0; i < 2; ++i) {
       const bool page = 2 * t + i < pages;
       const uint32_t r = ring % C::kRaw;
@@ -519,18 +522,17 @@ __device__ __forceinline__ void converter(const Args &a, Ctrl &c, uint8_t *smem,
         wait(&c.raw_full[r], (ring / C::kRaw) & 1u, dead, a.error_flag);
         rows = c.raw_rows[r];
       }
-      const uint8_t *src = smem + C::kOffRaw + r * C::kRawPage + sub * 16;
-      const int row0 = warp * 16 + (lane >> 3);
+      const uint8_t *src = smem + C::kOffRaw + r * C::kRawPage + from;
       const bool plain = rows == kPageTokens &&
                          (kCache == B200KV_I8 || !is_v || t * kTileTokens + (i + 1) * kPageTokens <= ctx);
       uint4 x[4];
       if (plain) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) x[k] = *reinterpret_cast<const uint4 *>(src + (row0 + 4 * k) * 128);
+        for (int k = 0; k < 4; ++k) x[k] = *reinterpret_cast<const uint4 *>(src + k * 512);
       } else {
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-          x[k] = row0 + 4 * k < rows ? *reinterpret_cast<const uint4 *>(src + (row0 + 4 * k) * 128) : make_uint4(0, 0, 0, 0);
+          x[k] = row0 + 4 * k < rows ? *reinterpret_cast<const uint4 *>(src + k * 512) : make_uint4(0, 0, 0, 0);
       }
       if (page) {
         __syncwarp();
@@ -539,14 +541,16 @@ __device__ __forceinline__ void converter(const Args &a, Ctrl &c, uint8_t *smem,
       }
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const int trow = i * kPageTokens + row0 + 4 * k;
         uint4 lo, hi;
         widen16<To, kCache>(x[k], lo, hi);
-        if (!plain && kCache == B200KV_E4M3 && is_v && t * kTileTokens + trow >= ctx) {  // a node's row: e4m3 has NaN
+        if (!plain && kCache == B200KV_E4M3 && is_v && t * kTileTokens + i * kPageTokens + row0 + 4 * k >= ctx) {  // a node's row: e4m3 has NaN
           const bool hit = drop_non_finite<__half>(lo);
           if (drop_non_finite<__half>(hi) || hit) atomicMax(&c.bad_piece, piece);
         }
-        put(trow, lo, hi);
+        uint8_t *line = dst + i * (kPageTokens * 128) + k * 512;
+        const uint32_t at = k & 1 ? at0 ^ 64 : at0;
+        *reinterpret_cast<uint4 *>(line + at) = lo;
+        *reinterpret_cast<uint4 *>(line + (at ^ 16)) = hi;
       }
     }
     fence_async_smem();
