@@ -192,7 +192,9 @@ extern "C" int b200kv_tree_attention(const void *q, int32_t q_dtype, int64_t q_s
   const CUtensorMapDataType type = q_dtype == B200KV_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   // Q: 64 elements x the KV head's query heads x the nodes of a tile (no more
   // than a sequence can have), rows node-major
-  const int64_t box_nodes = max_nodes < a.tile_nodes ? max_nodes : a.tile_nodes;
+  a.small_boxes = k8 && 32 % group == 0;
+  const int64_t box_nodes = a.small_boxes ? 32 / group : (max_nodes < a.tile_nodes ? max_nodes : a.tile_nodes);
+  a.box_nodes = static_cast<int>(box_nodes);
   a.q_box_bytes = static_cast<uint32_t>(box_nodes * group * 128);
   CUtensorMap qm, km, vm;
   // a dimension of one element may have any stride

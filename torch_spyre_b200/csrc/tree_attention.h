@@ -28,7 +28,9 @@ struct Args {
   float *lse;
   int total_q, batch, hq, hkv, group, max_blocks, max_nodes, num_blocks;
   int tile_nodes;        // nodes of a Q tile: floor(128 / group)
-  uint32_t q_box_bytes;  // bytes one TMA box of Q brings
+  int box_nodes;         // nodes of a TMA box of Q
+  int small_boxes;       // the boxes are of 32 rows, as many as are needed; else one box a tile
+  uint32_t q_box_bytes;  // bytes of a box
   float scale;
   int32_t *error_flag;
   Join *joins;      // [CTAs]

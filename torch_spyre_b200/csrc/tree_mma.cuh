@@ -25,7 +25,7 @@
 // pipe and the exponentials (16 per clock and SM, as long as the products).
 //
 // Warps: 0-3 and 4-7 the two softmax warpgroups, 8 the TMA producer, 9 the MMA
-// issuer (owns the TMEM), 8-bit caches: 12-15 converters, which turn 8-bit
+// issuer (owns the TMEM), 8-bit caches: 12-19 converters, which turn 8-bit
 // pages into 16-bit operand tiles of exact steps (the scales: see Factors).
 #pragma once
 
@@ -43,11 +43,12 @@ constexpr float kLazyLog2 = 8.f;
 template <typename T, int D, int kCache>
 struct Cfg {
   static constexpr bool k8 = kCache != B200KV_F16;
-  static constexpr int kThreads = k8 ? 512 : 384;
-  // Registers a thread, warpgroups 0-1 / 2 / 3, after setmaxnreg: a softmax
-  // thread holds its row's 128 scores.  Sums within the launch's own: 384
-  // threads of 168, or 512 of 128.
-  static constexpr int kRegsSoftmax = k8 ? 192 : 208, kRegsIssue = k8 ? 56 : 80, kRegsConvert = 72;
+  static constexpr int kThreads = k8 ? 640 : 384;
+  // Registers a thread, softmax / issue / converter warpgroups, after
+  // setmaxnreg (a 16-bit cache's softmax thread holds its row's 128 scores).
+  // Sums within the launch's own: 384 threads of 168, or 640 of 96.
+  static constexpr int kRegsSoftmax = k8 ? 144 : 208, kRegsIssue = k8 ? 64 : 80, kRegsConvert = 64;
+  static constexpr int kConverters = 8;  // warps
   static constexpr int kSticks = D / 64;
   static constexpr int kStickTile = kTileTokens * 128;      // one 64-element column of 128 rows
   static constexpr int kTile = kSticks * kStickTile;        // a Q, K or V tile
@@ -55,7 +56,7 @@ struct Cfg {
   static constexpr int kSlots = k8 ? 4 : (D == 64 ? 8 : 5);  // operand tiles in flight
   static constexpr int kRaw = k8 ? 6 : 0;                   // 8-bit pages in flight
   static constexpr int kRawPage = kPageTokens * 128;
-  static constexpr int kCtrl = k8 ? 15360 : 3072;
+  static constexpr int kCtrl = k8 ? 19456 : 3072;
   static constexpr int kOffQ = kCtrl;
   static constexpr int kOffSlots = kOffQ + kQ * kTile;
   static constexpr int kOffRaw = kOffSlots + kSlots * kTile;
@@ -91,7 +92,8 @@ struct Ctrl {
   unsigned bad_piece;       // last piece (counted from 1) that met a non-finite value in a node's V row
   float2 ml[2][kTileRows];  // (maximum, sum) of the streams' rows
 };
-// 8-bit caches: [8 warps][3][128] factors of a tile's tokens, see Factors
+// 8-bit caches: [8 warps][3][128] factors of a tile's tokens (see Factors), or,
+// when a block ends, [2 warpgroups][4][128] float4 of its rows' copies
 constexpr int kOffFactors = 3072;
 static_assert(sizeof(Ctrl) <= kOffFactors, "control block");
 
@@ -118,6 +120,12 @@ __device__ __forceinline__ void commit(uint64_t *bar) {
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void bar_group(int w) {  // one warpgroup
+  if (w == 0)
+    asm volatile("bar.sync 2, 128;" ::: "memory");
+  else
+    asm volatile("bar.sync 3, 128;" ::: "memory");
+}
 __device__ __forceinline__ void bar_pair() { asm volatile("bar.sync 1, 256;" ::: "memory"); }  // both warpgroups
 
 // -------------------------------------------------------------- TMEM moves --
@@ -148,6 +156,14 @@ __device__ __forceinline__ void wait_ld(uint32_t (&r)[32]) {
 __device__ __forceinline__ void wait_ld(uint32_t (&r)[16]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" : B200KV_RW8(r, 0), B200KV_RW8(r, 8)::"memory");
 }
+__device__ __forceinline__ void tmem_st32(uint32_t at, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
+      "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(at),
+      B200KV_W8(r, 0), B200KV_W8(r, 8), B200KV_W8(r, 16), B200KV_W8(r, 24)
+      : "memory");
+}
+__device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t (&r)[16]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(at),
@@ -226,6 +242,24 @@ __device__ __forceinline__ long long head_units(const Args &a, const Seq &s) {
   long long n = 0;
   for (int k = 0; k < s.blocks; ++k) n += block_tiles<kQ>(a, s, k);
   return n;
+}
+
+// An 8-bit cache's Q tile holds its rows several times where they are few: 4
+// times up to 32 rows, twice up to 64.  Every copy meets all tokens in the
+// products, but weighs only its share of them (the rest get zeros), so that all
+// four warps of a warpgroup work on a tile and a thread takes 32 or 64 scores
+// of it.  The copies are separate states of the softmax until the block ends.
+struct Copies {
+  int copies, rows, boxes;  // rows: of the tile, per copy; boxes: TMA boxes of a copy
+};
+__device__ __forceinline__ Copies copies_of(const Args &a, const Seq &s, int block) {
+  const int live = min(a.tile_nodes, s.nodes - block * a.tile_nodes) * a.group;
+  Copies c;
+  c.boxes = a.small_boxes ? (live + 31) / 32 : 1;
+  const int held = a.small_boxes ? c.boxes * 32 : a.box_nodes * a.group;
+  c.copies = held <= 32 ? 4 : (held <= 64 ? 2 : 1);
+  c.rows = kTileRows / c.copies;
+  return c;
 }
 
 // The blocks of a CTA's share, one piece (a block, or the part of it in this
@@ -357,11 +391,21 @@ __device__ __forceinline__ void producer(const Args &a, Ctrl &c, uint8_t *smem, 
     const int pages = (w.s.ctx + w.s.nodes + kPageTokens - 1) / kPageTokens;
     if (lane == 0) {
       wait(&c.q_empty, (pieces & 1u) ^ 1u, dead, a.error_flag);
-      mbar_arrive_expect_tx(&c.q_full, (two ? 2u : 1u) * C::kSticks * a.q_box_bytes);
-      for (int i = 0; i < (two ? 2 : 1); ++i)
-        for (int st = 0; st < C::kSticks; ++st)
-          tma_3d(smem + C::kOffQ + i * C::kTile + st * C::kStickTile, qm, &c.q_full, st * 64, w.kvh * a.group,
-                 w.s.q0 + (C::kQ * w.block + i) * a.tile_nodes);
+      if constexpr (C::k8) {
+        const Copies q = copies_of(a, w.s, w.block);
+        mbar_arrive_expect_tx(&c.q_full, uint32_t(q.copies * q.boxes) * C::kSticks * a.q_box_bytes);
+        for (int k = 0; k < q.copies; ++k)
+          for (int i = 0; i < q.boxes; ++i)
+            for (int st = 0; st < C::kSticks; ++st)
+              tma_3d(smem + C::kOffQ + st * C::kStickTile + (k * q.rows + i * 32) * 128, qm, &c.q_full, st * 64,
+                     w.kvh * a.group, w.s.q0 + w.block * a.tile_nodes + i * a.box_nodes);
+      } else {
+        mbar_arrive_expect_tx(&c.q_full, (two ? 2u : 1u) * C::kSticks * a.q_box_bytes);
+        for (int i = 0; i < (two ? 2 : 1); ++i)
+          for (int st = 0; st < C::kSticks; ++st)
+            tma_3d(smem + C::kOffQ + i * C::kTile + st * C::kStickTile, qm, &c.q_full, st * 64, w.kvh * a.group,
+                   w.s.q0 + (C::kQ * w.block + i) * a.tile_nodes);
+      }
     }
     ++pieces;
     int window = w.t0 / 16, ids = load_ids(a, w.b, window, pages), ids_next = load_ids(a, w.b, window + 1, pages);
@@ -499,9 +543,9 @@ __device__ __forceinline__ void widen16(uint4 v, uint4 &lo, uint4 &hi) {
 template <typename C, typename T, int kCache>
 __device__ __forceinline__ void converter(const Args &a, Ctrl &c, uint8_t *smem, int warp) {
   const int lane = threadIdx.x & 31, sub = lane & 7;
-  // this lane's rows of a page are row0, row0 + 4, + 8, + 12; rows four apart
-  // differ in bit 2 of the swizzle's XOR
-  const int row0 = warp * 16 + ((lane >> 3) ^ (sub >> 2));
+  // this lane's rows of a page are row0 and row0 + 4, which differ in bit 2 of
+  // the swizzle's XOR
+  const int row0 = warp * 8 + ((lane >> 3) ^ (sub >> 2));
   const int chunk = (sub & 3) * 2;
   const uint32_t from = row0 * 128 + sub * 16;
   const uint32_t even = (sub >> 2) * C::kStickTile + row0 * 128, at0 = (chunk ^ (row0 & 7)) << 4;
@@ -525,25 +569,21 @@ __device__ __forceinline__ void converter(const Args &a, Ctrl &c, uint8_t *smem,
       const uint8_t *src = smem + C::kOffRaw + r * C::kRawPage + from;
       const bool plain = rows == kPageTokens &&
                          (kCache == B200KV_I8 || !is_v || t * kTileTokens + (i + 1) * kPageTokens <= ctx);
-      uint4 x[4];
-      if (plain) {
+      uint4 x[2];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) x[k] = *reinterpret_cast<const uint4 *>(src + k * 512);
-      } else {
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          x[k] = row0 + 4 * k < rows ? *reinterpret_cast<const uint4 *>(src + k * 512) : make_uint4(0, 0, 0, 0);
-      }
+      for (int k = 0; k < 2; ++k)
+        x[k] = plain || row0 + 4 * k < rows ? *reinterpret_cast<const uint4 *>(src + k * 512) : make_uint4(0, 0, 0, 0);
       if (page) {
         __syncwarp();
         if (lane == 0) arrive(&c.raw_empty[r]);
         ++ring;
       }
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
+      for (int k = 0; k < 2; ++k) {
         uint4 lo, hi;
         widen16<To, kCache>(x[k], lo, hi);
-        if (!plain && kCache == B200KV_E4M3 && is_v && t * kTileTokens + i * kPageTokens + row0 + 4 * k >= ctx) {  // a node's row: e4m3 has NaN
+        // a node's row: e4m3 has NaN
+        if (!plain && kCache == B200KV_E4M3 && is_v && t * kTileTokens + i * kPageTokens + row0 + 4 * k >= ctx) {
           const bool hit = drop_non_finite<__half>(lo);
           if (drop_non_finite<__half>(hi) || hit) atomicMax(&c.bad_piece, piece);
         }
@@ -722,50 +762,9 @@ __device__ __forceinline__ float floor_scale(float v) { return v < 1e-30f ? 1e-3
 // (a NaN scale makes 2^y NaN where the token is seen; 0 / v must stay 0 where not)
 __device__ __forceinline__ float inv_scale(float v) { return v < CUDART_INF_F ? 1.f / v : 1.f; }
 
-// Scores of a row's 128 tokens -> weights, in place in TMEM.  kTail: vis tells
-// which tokens the row sees.
-template <typename C, int D, bool kTail>
-__device__ __forceinline__ void weigh(uint32_t ts, uint32_t to, const uint32_t (&vis)[4], float cl, const Factors *fac,
-                                      bool first, bool live, float &m, float &l) {
-  uint32_t s[4][32];
-  if constexpr (!C::k8) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) tmem_ld32(ts + 32 * i, s[i]);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) wait_ld(s[i]);
-  }
-  float top[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if constexpr (C::k8) {
-      // a quarter at a time, so that registers are left to fetch its factors ahead
-      tmem_ld32(ts + 32 * i, s[i]);
-      float4 k[8], v[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) k[j] = fac->k[8 * i + j], v[j] = fac->log2v[8 * i + j];
-      wait_ld(s[i]);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        uint32_t *r = &s[i][4 * j];
-        const float2 lo = fma2(make_float2(__uint_as_float(r[0]), __uint_as_float(r[1])), make_float2(k[j].x, k[j].y),
-                               make_float2(v[j].x, v[j].y));
-        const float2 hi = fma2(make_float2(__uint_as_float(r[2]), __uint_as_float(r[3])), make_float2(k[j].z, k[j].w),
-                               make_float2(v[j].z, v[j].w));
-        r[0] = __float_as_uint(lo.x), r[1] = __float_as_uint(lo.y);
-        r[2] = __float_as_uint(hi.x), r[3] = __float_as_uint(hi.y);
-      }
-    }
-    if (kTail) {
-#pragma unroll
-      for (int j = 0; j < 32; ++j) s[i][j] = vis[i] >> j & 1u ? s[i][j] : 0xff800000u;  // -inf
-    }
-    float t = __uint_as_float(s[i][0]);
-#pragma unroll
-    for (int j = 1; j < 31; j += 2) t = fmaxf(fmaxf(t, __uint_as_float(s[i][j])), __uint_as_float(s[i][j + 1]));
-    top[i] = fmaxf(t, __uint_as_float(s[i][31]));
-  }
-  float mt = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-  if (!C::k8) mt *= cl;
+// Moves the running maximum when a row's has risen far enough, O and l with it.
+template <int D>
+__device__ __forceinline__ void follow(uint32_t to, float mt, bool first, bool live, float &m, float &l) {
   const bool rise = mt > m + (first ? 0.f : kLazyLog2);
   if (!first && __any_sync(0xffffffffu, rise && live)) {
     const float keep = rise ? ex2(m - mt) : 1.f;
@@ -781,6 +780,34 @@ __device__ __forceinline__ void weigh(uint32_t ts, uint32_t to, const uint32_t (
     }
   }
   if (rise) m = mt;
+}
+
+template <bool kTail>
+__device__ __forceinline__ float mask_max(uint32_t (&s)[32], uint32_t vis) {
+  if (kTail) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) s[j] = vis >> j & 1u ? s[j] : 0xff800000u;  // -inf
+  }
+  float t = __uint_as_float(s[0]);
+#pragma unroll
+  for (int j = 1; j < 31; j += 2) t = fmaxf(fmaxf(t, __uint_as_float(s[j])), __uint_as_float(s[j + 1]));
+  return fmaxf(t, __uint_as_float(s[31]));
+}
+
+// Scores of a row's 128 tokens -> weights, in place in TMEM.  kTail: vis tells
+// which tokens the row sees.
+template <typename P, int D, bool kTail>
+__device__ __forceinline__ void weigh(uint32_t ts, uint32_t to, const uint32_t (&vis)[4], float cl, bool first, bool live,
+                                      float &m, float &l) {
+  uint32_t s[4][32];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) tmem_ld32(ts + 32 * i, s[i]);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) wait_ld(s[i]);
+  float top[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) top[i] = mask_max<kTail>(s[i], vis[i]);
+  follow<D>(to, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * cl, first, live, m, l);
   const float minus = m == -CUDART_INF_F ? 0.f : -m;
   float2 sum[4];
 #pragma unroll
@@ -790,22 +817,95 @@ __device__ __forceinline__ void weigh(uint32_t ts, uint32_t to, const uint32_t (
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
       const float2 x = make_float2(__uint_as_float(s[i][2 * j]), __uint_as_float(s[i][2 * j + 1]));
-      const float2 y = C::k8 ? add2(x, make_float2(minus, minus))
-                             : fma2(x, make_float2(cl, cl), make_float2(minus, minus));
+      const float2 y = fma2(x, make_float2(cl, cl), make_float2(minus, minus));
       const float2 e = make_float2(ex2(y.x), ex2(y.y));
-      if constexpr (C::k8) {
-        const float4 v = fac->inv_v[8 * i + j / 2];
-        sum[i] = fma2(e, j & 1 ? make_float2(v.z, v.w) : make_float2(v.x, v.y), sum[i]);
-      } else {
-        sum[i] = add2(sum[i], e);
-      }
-      p[j] = pack2(e.x, e.y, typename C::P());
+      sum[i] = add2(sum[i], e);
+      p[j] = pack2(e.x, e.y, P());
     }
     tmem_st16(ts + 16 * i, p);
   }
   const float2 t = add2(add2(sum[0], sum[1]), add2(sum[2], sum[3]));
   l += t.x + t.y;
-  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+  wait_st();
+}
+
+// The same for an 8-bit cache: the 32 * kN tokens that this copy of the row
+// weighs, from token 32 * kN * copy on.
+template <int kN, int D, bool kTail>
+__device__ __forceinline__ void weigh8(uint32_t ts, uint32_t to, const uint32_t (&vis)[4], const Factors *fac, int copy,
+                                       bool first, bool live, float &m, float &l) {
+  constexpr bool kKeep = kN <= 2;  // scores stay in registers (else they go back to TMEM for the second pass)
+  const int c0 = copy * kN;
+  uint32_t y[kKeep ? kN : 1][32];
+  float mt = -CUDART_INF_F;
+#pragma unroll
+  for (int i = 0; i < kN; ++i) {
+    uint32_t(&s)[32] = y[kKeep ? i : 0];
+    tmem_ld32(ts + 32 * (c0 + i), s);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {  // factors of 16 tokens are fetched together
+      const float4 *kf = fac->k + 8 * (c0 + i) + 4 * h, *vf = fac->log2v + 8 * (c0 + i) + 4 * h;
+      float4 k[4], v[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) k[j] = kf[j], v[j] = vf[j];
+      if (h == 0) wait_ld(s);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        uint32_t *r = &s[16 * h + 4 * j];
+        const float2 lo = fma2(make_float2(__uint_as_float(r[0]), __uint_as_float(r[1])), make_float2(k[j].x, k[j].y),
+                               make_float2(v[j].x, v[j].y));
+        const float2 hi = fma2(make_float2(__uint_as_float(r[2]), __uint_as_float(r[3])), make_float2(k[j].z, k[j].w),
+                               make_float2(v[j].z, v[j].w));
+        r[0] = __float_as_uint(lo.x), r[1] = __float_as_uint(lo.y);
+        r[2] = __float_as_uint(hi.x), r[3] = __float_as_uint(hi.y);
+      }
+    }
+    mt = fmaxf(mt, mask_max<kTail>(s, vis[i]));
+    if (!kKeep) tmem_st32(ts + 32 * i, s);
+  }
+  if (!kKeep) wait_st();
+  follow<D>(to, mt, first, live, m, l);
+  const float minus = m == -CUDART_INF_F ? 0.f : -m;
+  float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+  for (int i = 0; i < kN; ++i) {
+    uint32_t(&s)[32] = y[kKeep ? i : 0];
+    if (!kKeep) tmem_ld32(ts + 32 * i, s);
+    if (!kKeep) wait_ld(s);
+    uint32_t p[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const float2 x = add2(make_float2(__uint_as_float(s[2 * j]), __uint_as_float(s[2 * j + 1])), make_float2(minus, minus));
+      const float2 e = make_float2(ex2(x.x), ex2(x.y));
+      const float4 f = fac->inv_v[8 * (c0 + i) + j / 2];
+      sum[j & 1] = fma2(e, j & 1 ? make_float2(f.z, f.w) : make_float2(f.x, f.y), sum[j & 1]);
+      p[j] = pack2(e.x, e.y, __half());
+    }
+    tmem_st16(ts + 16 * (c0 + i), p);
+  }
+  if (kN < 4) {
+    // the tokens of the other copies
+    uint32_t zero[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) zero[j] = 0;
+#pragma unroll
+    for (int i = 1; i < 4 / kN; ++i)
+#pragma unroll
+      for (int k = 0; k < kN; ++k) tmem_st16(ts + 16 * (((copy + i) % (4 / kN)) * kN + k), zero);
+  }
+  const float2 t = add2(sum[0], sum[1]);
+  l += t.x + t.y;
+  wait_st();
+}
+template <int D, bool kTail>
+__device__ __forceinline__ void weigh8(uint32_t ts, uint32_t to, const uint32_t (&vis)[4], const Factors *fac, int copies,
+                                       int copy, bool first, bool live, float &m, float &l) {
+  if (copies == 4)
+    weigh8<1, D, kTail>(ts, to, vis, fac, copy, first, live, m, l);
+  else if (copies == 2)
+    weigh8<2, D, kTail>(ts, to, vis, fac, copy, first, live, m, l);
+  else
+    weigh8<4, D, kTail>(ts, to, vis, fac, copy, first, live, m, l);
 }
 
 // Element d of a cached V row (8-bit caches: its steps).
@@ -856,8 +956,11 @@ __device__ __forceinline__ void softmax(const Args &a, Ctrl &c, uint8_t *smem, u
     const int n = wk.t1 - wk.t0, lead = two ? 1 : 2;
     const int len = wk.s.ctx + wk.s.nodes;
     const int qt = C::kQ * wk.block + (two ? w : 0);
-    const int node = qt * a.tile_nodes + tid / a.group;
-    const bool live = tid < a.tile_nodes * a.group && node < wk.s.nodes;
+    Copies q{1, kTileRows, 1};
+    if (C::k8) q = copies_of(a, wk.s, wk.block);
+    const int row = tid & (q.rows - 1), copy = tid / q.rows;
+    const int node = qt * a.tile_nodes + row / a.group;
+    const bool live = row < a.tile_nodes * a.group && node < wk.s.nodes;
     const bool warp_live = __any_sync(0xffffffffu, live);
     float m = -CUDART_INF_F, l = 0.f;
     // 8-bit caches: the scales of this stream's next tile, four tokens per lane
@@ -881,7 +984,8 @@ __device__ __forceinline__ void softmax(const Args &a, Ctrl &c, uint8_t *smem, u
       uint32_t vis[4] = {~0u, ~0u, ~0u, ~0u};
       if (tail && live) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) vis[i] = visible32(a, wk.s, node, pos + 32 * i);
+        for (int i = 0; i < 4; ++i)
+          if (i < 4 / q.copies) vis[i] = visible32(a, wk.s, node, pos + copy * q.rows + 32 * i);
       }
       if (C::k8 && warp_live) {
         __syncwarp();
@@ -895,10 +999,18 @@ __device__ __forceinline__ void softmax(const Args &a, Ctrl &c, uint8_t *smem, u
       wait(&c.s_full[w], s_uses++ & 1u, dead, a.error_flag);
       fence_after();
       if (warp_live) {
-        if (tail)
-          weigh<C, D, true>(ts, to, vis, cl, fac, t == tfirst, live, m, l);
-        else
-          weigh<C, D, false>(ts, to, vis, cl, fac, t == tfirst, live, m, l);
+        const bool first = t == tfirst;
+        if constexpr (C::k8) {
+          if (tail)
+            weigh8<D, true>(ts, to, vis, fac, q.copies, copy, first, live, m, l);
+          else
+            weigh8<D, false>(ts, to, vis, fac, q.copies, copy, first, live, m, l);
+        } else {
+          if (tail)
+            weigh<typename C::P, D, true>(ts, to, vis, cl, first, live, m, l);
+          else
+            weigh<typename C::P, D, false>(ts, to, vis, cl, first, live, m, l);
+        }
       }
       if (!C::k8 && pos + kTileTokens > wk.s.ctx) {
         // the pool's rows past the sequence's end hold anything and become
@@ -950,18 +1062,74 @@ __device__ __forceinline__ void softmax(const Args &a, Ctrl &c, uint8_t *smem, u
       bar_pair();
       const float2 x = c.ml[0][tid], y = c.ml[1][tid];
       m = fmaxf(x.x, y.x);
+      for (int k = 1; k < q.copies; ++k) {
+        const int at = tid ^ (k * q.rows);
+        m = fmaxf(m, fmaxf(c.ml[0][at].x, c.ml[1][at].x));
+      }
       const float mm = m == -CUDART_INF_F ? 0.f : m;
       keep0 = ex2(x.x - mm);
       keep1 = ex2(y.x - mm);
-      l = x.y * keep0 + (both ? y.y * keep1 : 0.f);
+      l = 0.f;
+      for (int k = 0; k < q.copies; ++k) {
+        const float2 xk = c.ml[0][row + k * q.rows], yk = c.ml[1][row + k * q.rows];
+        l = fmaf(xk.y, ex2(xk.x - mm), l);
+        if (both) l = fmaf(yk.y, ex2(yk.x - mm), l);
+      }
       d0 = w * (D / 2);
       d1 = d0 + D / 2;
     }
-    if (warp_live) {
-      const int64_t orow = static_cast<int64_t>(wk.s.q0 + node) * a.hq + wk.kvh * a.group + tid % a.group;
-      const float inv = l == 0.f ? 0.f : 1.f / l;
-      const bool repair = *reinterpret_cast<volatile unsigned *>(&c.bad_piece) >= piece;
-      const int prow = (two ? w : 0) * kTileRows + tid;
+    const int64_t orow = static_cast<int64_t>(wk.s.q0 + node) * a.hq + wk.kvh * a.group + row % a.group;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const bool repair = *reinterpret_cast<volatile unsigned *>(&c.bad_piece) >= piece;
+    const int prow = (two ? w : 0) * kTileRows + row;
+    if (C::k8 && q.copies > 1) {
+      // add the copies up, 16 columns at a time through shared memory
+      float4 *red = reinterpret_cast<float4 *>(smem + kOffFactors) + w * 4 * kTileRows;
+#pragma unroll 1
+      for (int d = d0; d < d1; d += 16) {
+        uint32_t r[16], r1[16];
+        tmem_ld16(quad + col_o(0) + d, r);
+        wait_ld(r);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * keep0);
+        if (both) {
+          tmem_ld16(quad + col_o(1) + d, r1);
+          wait_ld(r1);
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            r[j] = __float_as_uint(fmaf(__uint_as_float(r1[j]), keep1, __uint_as_float(r[j])));
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          red[j * kTileRows + tid] = make_float4(__uint_as_float(r[4 * j]), __uint_as_float(r[4 * j + 1]),
+                                                 __uint_as_float(r[4 * j + 2]), __uint_as_float(r[4 * j + 3]));
+        bar_group(w);
+        for (int j = copy; live && j < 4; j += q.copies) {
+          float4 o = red[j * kTileRows + row];
+          for (int k = 1; k < q.copies; ++k) {
+            const float4 x = red[j * kTileRows + row + k * q.rows];
+            o = make_float4(o.x + x.x, o.y + x.y, o.z + x.z, o.w + x.w);
+          }
+          const int dj = d + 4 * j;
+          if (repair) {
+            auto more = [&](int i) {
+              return non_finite_sum<T, D, kCache>(a, wk.s, wk.b, wk.kvh, node, wk.t0 * kTileTokens, wk.t1 * kTileTokens,
+                                                  dj + i);
+            };
+            o = make_float4(o.x + more(0), o.y + more(1), o.z + more(2), o.w + more(3));
+          }
+          if (split) {
+            *reinterpret_cast<float4 *>(a.part_o + ((static_cast<int64_t>(pslot) * (D / 4) + dj / 4) * 256 + prow) * 4) = o;
+          } else {
+            const bool none = l == 0.f;
+            *reinterpret_cast<uint2 *>(static_cast<T *>(a.out) + orow * D + dj) =
+                none ? make_uint2(0u, 0u)
+                     : make_uint2(pack2(o.x * inv, o.y * inv, T()), pack2(o.z * inv, o.w * inv, T()));
+          }
+        }
+        bar_group(w);
+      }
+    } else if (warp_live) {
 #pragma unroll 1
       for (int d = d0; d < d1; d += 32) {
         uint32_t r[32];
@@ -1003,12 +1171,12 @@ __device__ __forceinline__ void softmax(const Args &a, Ctrl &c, uint8_t *smem, u
         }
         __syncwarp();
       }
-      if (live && (two || w == 0)) {
-        if (split)
-          a.part_ml[static_cast<int64_t>(pslot) * 256 + prow] = make_float2(m, l);
-        else if (a.lse)
-          a.lse[orow] = l == 0.f ? -CUDART_INF_F : (m + log2f(l)) * 0.69314718055994530942f;
-      }
+    }
+    if (live && copy == 0 && (two || w == 0)) {
+      if (split)
+        a.part_ml[static_cast<int64_t>(pslot) * 256 + prow] = make_float2(m, l);
+      else if (a.lse)
+        a.lse[orow] = l == 0.f ? -CUDART_INF_F : (m + log2f(l)) * 0.69314718055994530942f;
     }
     // the first CTA boundary inside a split block describes it to the join
     if (split && wk.t0 > 0 && w == 0 && tid == 0 && wk.t0 <= c.per) {
@@ -1042,12 +1210,12 @@ __global__ void __launch_bounds__((Cfg<T, D, kCache>::kThreads), 1)
     prefetch_tensormap(&km);
     prefetch_tensormap(&vm);
     for (int i = 0; i < C::kSlots; ++i) {
-      mbar_init(&c.full[i], C::k8 ? 4 : 1);
+      mbar_init(&c.full[i], C::k8 ? C::kConverters : 1);
       mbar_init(&c.empty[i], 1);
     }
     for (int i = 0; i < C::kRaw; ++i) {
       mbar_init(&c.raw_full[i], 1);
-      mbar_init(&c.raw_empty[i], 4);
+      mbar_init(&c.raw_empty[i], C::kConverters);
     }
     mbar_init(&c.q_full, 1);
     mbar_init(&c.q_empty, 1);
