@@ -39,6 +39,10 @@ namespace tree {
 
 constexpr int kTileRows = 128, kTileTokens = 128;
 constexpr float kLazyLog2 = 8.f;
+#ifndef TS8
+#define TS8 4
+#define TR8 3
+#endif
 
 template <typename T, int D, int kCache>
 struct Cfg {
@@ -53,14 +57,14 @@ struct Cfg {
   static constexpr int kStickTile = kTileTokens * 128;      // one 64-element column of 128 rows
   static constexpr int kTile = kSticks * kStickTile;        // a Q, K or V tile
   static constexpr int kQ = k8 ? 1 : 2;                      // most Q tiles of a block
-  static constexpr int kSlots = k8 ? 4 : (D == 64 ? 8 : 5);  // operand tiles in flight
-  static constexpr int kRaw = k8 ? 6 : 0;                   // 8-bit pages in flight
-  static constexpr int kRawPage = kPageTokens * 128;
+  static constexpr int kSlots = k8 ? TS8 : (D == 64 ? 8 : 5);  // operand tiles in flight
+  static constexpr int kRaw = k8 ? TR8 : 0;                   // 8-bit tiles in flight
+  static constexpr int kRawTile = kTileTokens * 128;
   static constexpr int kCtrl = k8 ? 19456 : 3072;
   static constexpr int kOffQ = kCtrl;
   static constexpr int kOffSlots = kOffQ + kQ * kTile;
   static constexpr int kOffRaw = kOffSlots + kSlots * kTile;
-  static constexpr int kSmem = kOffRaw + kRaw * kRawPage;
+  static constexpr int kSmem = kOffRaw + kRaw * kRawTile;
   // The type of P and V: an 8-bit cache's steps are exact in fp16, whatever q's
   // type, and fp16 keeps three bits more of each weight than bf16.
   using P = typename std::conditional<k8, __half, T>::type;
@@ -81,14 +85,13 @@ __device__ __forceinline__ uint32_t col_o(int w) { return 256u + uint32_t(w) * 1
 
 struct Ctrl {
   uint64_t full[8], empty[8];          // operand tiles
-  uint64_t raw_full[8], raw_empty[8];  // 8-bit pages
+  uint64_t raw_full[8], raw_empty[8];  // 8-bit tiles
   uint64_t q_full, q_empty;
   uint64_t s_full[2], p_ready[2], o_full[2];
   uint32_t tmem;
   int start_b;
   long long start_rem, per, total;
   long long scan[16];
-  int raw_rows[8];
   unsigned bad_piece;       // last piece (counted from 1) that met a non-finite value in a node's V row
   float2 ml[2][kTileRows];  // (maximum, sum) of the streams' rows
 };
@@ -151,24 +154,22 @@ __device__ __forceinline__ void tmem_ld16(uint32_t at, uint32_t (&r)[16]) {
 // The loaded registers go through the wait, so that no use of them is moved before it.
 __device__ __forceinline__ void wait_ld(uint32_t (&r)[32]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : B200KV_RW8(r, 0), B200KV_RW8(r, 8), B200KV_RW8(r, 16), B200KV_RW8(r, 24)::"memory");
+               : B200KV_RW8(r, 0), B200KV_RW8(r, 8), B200KV_RW8(r, 16), B200KV_RW8(r, 24));
 }
 __device__ __forceinline__ void wait_ld(uint32_t (&r)[16]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;" : B200KV_RW8(r, 0), B200KV_RW8(r, 8)::"memory");
+  asm volatile("tcgen05.wait::ld.sync.aligned;" : B200KV_RW8(r, 0), B200KV_RW8(r, 8));
 }
 __device__ __forceinline__ void tmem_st32(uint32_t at, const uint32_t (&r)[32]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
       "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(at),
-      B200KV_W8(r, 0), B200KV_W8(r, 8), B200KV_W8(r, 16), B200KV_W8(r, 24)
-      : "memory");
+      B200KV_W8(r, 0), B200KV_W8(r, 8), B200KV_W8(r, 16), B200KV_W8(r, 24));
 }
-__device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;"); }
 __device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t (&r)[16]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(at),
-      B200KV_W8(r, 0), B200KV_W8(r, 8)
-      : "memory");
+      B200KV_W8(r, 0), B200KV_W8(r, 8));
 }
 
 // ---------------------------------------------------------------- operands --
@@ -383,7 +384,7 @@ __device__ __forceinline__ void producer(const Args &a, Ctrl &c, uint8_t *smem, 
   const int lane = threadIdx.x & 31;
   const uint64_t policy = l2_policy_evict_first();
   bool dead = false;
-  uint32_t slot = 0, ring = 0, pieces = 0;  // tiles (16-bit) or pages (8-bit) issued, pieces begun
+  uint32_t slot = 0, ring = 0, pieces = 0;  // tiles issued (16-bit, 8-bit), pieces begun
   Walk<C::kQ> w;
   w.init(a, c);
   while (w.next(a)) {
@@ -416,47 +417,36 @@ __device__ __forceinline__ void producer(const Args &a, Ctrl &c, uint8_t *smem, 
         ids = ids_next;
         ids_next = load_ids(a, w.b, ++window + 1, pages);
       }
+      // lane: a page of the tile and, in 16-bit pools, one of its stick columns
+      constexpr int kParts = C::k8 ? 1 : C::kSticks;
       const int have = t / 16 == window ? ids : ids_before;
-      const int id0 = __shfl_sync(0xffffffffu, have, (2 * t) & 31), id1 = __shfl_sync(0xffffffffu, have, (2 * t + 1) & 31);
+      const int part = lane % kParts, at = lane / kParts;
+      const int id = __shfl_sync(0xffffffffu, have, (2 * t + (at & 1)) & 31);
       const int n = min(2, pages - 2 * t);
-      const CUtensorMap *map = is_v ? vm : km;
       if constexpr (!C::k8) {
-        if (lane == 0) {
-          const uint32_t s = slot % C::kSlots;
-          wait(&c.empty[s], ((slot / C::kSlots) & 1u) ^ 1u, dead, a.error_flag);
-          mbar_arrive_expect_tx(&c.full[s], uint32_t(n) * C::kSticks * (kPageTokens * 128));
-          uint8_t *dst = smem + C::kOffSlots + s * C::kTile;
-          for (int i = 0; i < n; ++i) {
-            const int id = i ? id1 : id0;
-            // an invalid id reads past the last page: zeros
-            const int page = id < 0 ? a.num_blocks * a.hkv : id * a.hkv + w.kvh;
-            for (int st = 0; st < C::kSticks; ++st)
-              tma_load_3d(dst + st * C::kStickTile + i * (kPageTokens * 128), map, &c.full[s], 0, st * kPageTokens, page,
-                          policy);
-          }
-        }
+        const uint32_t s = slot % C::kSlots;
+        wait(&c.empty[s], ((slot / C::kSlots) & 1u) ^ 1u, dead, a.error_flag);
+        if (lane == 0) mbar_arrive_expect_tx(&c.full[s], uint32_t(n) * C::kSticks * (kPageTokens * 128));
+        __syncwarp();
+        // an invalid id reads past the last page: zeros
+        const int page = id < 0 ? a.num_blocks * a.hkv : id * a.hkv + w.kvh;
+        if (at < n)
+          tma_load_3d(smem + C::kOffSlots + s * C::kTile + part * C::kStickTile + at * (kPageTokens * 128), is_v ? vm : km,
+                      &c.full[s], 0, part * kPageTokens, page, policy);
         ++slot;
       } else {
-        for (int i = 0; i < n; ++i) {
-          if (lane == 0) {
-            const uint32_t r = ring % C::kRaw;
-            wait(&c.raw_empty[r], ((ring / C::kRaw) & 1u) ^ 1u, dead, a.error_flag);
-            const int id = i ? id1 : id0;
-            // rows past the context, and whole pages with an invalid id, count as zeros
-            c.raw_rows[r] = id < 0 ? 0 : min(kPageTokens, w.s.ctx + w.s.nodes - (2 * t + i) * kPageTokens);
-            if (id < 0) {
-              arrive(&c.raw_full[r]);
-            } else {
-              const int page = id * a.hkv + w.kvh;
-              mbar_arrive_expect_tx(&c.raw_full[r], C::kRawPage);
-              // a page is one contiguous run of 8 KiB
-              bulk_load(smem + C::kOffRaw + r * C::kRawPage,
-                        static_cast<const uint8_t *>(is_v ? a.v_pool : a.k_pool) + static_cast<int64_t>(page) * C::kRawPage,
-                        C::kRawPage, &c.raw_full[r]);
-            }
-          }
-          ++ring;
-        }
+        const uint32_t r = ring % C::kRaw;
+        wait(&c.raw_empty[r], ((ring / C::kRaw) & 1u) ^ 1u, dead, a.error_flag);
+        if (lane == 0) mbar_arrive_expect_tx(&c.raw_full[r], uint32_t(n) * (kPageTokens * 128));
+        __syncwarp();
+        // a page is one contiguous run; an invalid id reads page 0, and scales
+        // of zero make zeros of it
+        const int64_t page = id < 0 ? 0 : id * a.hkv + w.kvh;
+        if (at < n)
+          bulk_load(smem + C::kOffRaw + r * C::kRawTile + at * (kPageTokens * 128),
+                    static_cast<const uint8_t *>(is_v ? a.v_pool : a.k_pool) + page * (kPageTokens * 128),
+                    kPageTokens * 128, &c.raw_full[r]);
+        ++ring;
       }
     };
     // K leads V by one tile per stream that needs it: the order the MMA warp
@@ -478,7 +468,7 @@ __device__ __forceinline__ void producer(const Args &a, Ctrl &c, uint8_t *smem, 
 // NaN of V out of a matrix product, and a node may be hidden from some rows of
 // a tile only.  So the nodes' V rows are looked through in shared memory:
 // non-finite elements become zeros there, and when the block ends the rows that
-// see such a node get its elements added from the cache (non_finite_sum).
+// see such a node get its elements added from the cache (repair_row).
 template <typename T>
 __device__ __forceinline__ uint32_t drop_non_finite(uint32_t w) {
   constexpr uint32_t e = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
@@ -543,9 +533,8 @@ __device__ __forceinline__ void widen16(uint4 v, uint4 &lo, uint4 &hi) {
 template <typename C, typename T, int kCache>
 __device__ __forceinline__ void converter(const Args &a, Ctrl &c, uint8_t *smem, int warp) {
   const int lane = threadIdx.x & 31, sub = lane & 7;
-  // this lane's rows of a page are row0 and row0 + 4, which differ in bit 2 of
-  // the swizzle's XOR
-  const int row0 = warp * 8 + ((lane >> 3) ^ (sub >> 2));
+  // this lane's rows of a tile are row0, row0 + 32, + 64 and + 96
+  const int row0 = warp * 4 + ((lane >> 3) ^ (sub >> 2));
   const int chunk = (sub & 3) * 2;
   const uint32_t from = row0 * 128 + sub * 16;
   const uint32_t even = (sub >> 2) * C::kStickTile + row0 * 128, at0 = (chunk ^ (row0 & 7)) << 4;
@@ -553,45 +542,32 @@ __device__ __forceinline__ void converter(const Args &a, Ctrl &c, uint8_t *smem,
   uint32_t slot = 0, ring = 0;
   unsigned piece = 0;
   // one tile of K (To the compute type) or V (to fp16)
-  auto tile = [&](auto to, bool is_v, int t, int pages, int ctx) {
+  auto tile = [&](auto to, bool is_v, int t, int len, int ctx) {
     using To = decltype(to);
     const uint32_t s = slot % C::kSlots;
     wait(&c.empty[s], ((slot / C::kSlots) & 1u) ^ 1u, dead, a.error_flag);
     uint8_t *dst = smem + C::kOffSlots + s * C::kTile + even;
-    for (int i = 0; i < 2; ++i) {
-      const bool page = 2 * t + i < pages;
-      const uint32_t r = ring % C::kRaw;
-      int rows = 0;
-      if (page) {
-        wait(&c.raw_full[r], (ring / C::kRaw) & 1u, dead, a.error_flag);
-        rows = c.raw_rows[r];
-      }
-      const uint8_t *src = smem + C::kOffRaw + r * C::kRawPage + from;
-      const bool plain = rows == kPageTokens &&
-                         (kCache == B200KV_I8 || !is_v || t * kTileTokens + (i + 1) * kPageTokens <= ctx);
-      uint4 x[2];
+    const uint32_t r = ring % C::kRaw;
+    wait(&c.raw_full[r], (ring / C::kRaw) & 1u, dead, a.error_flag);
+    const uint8_t *src = smem + C::kOffRaw + r * C::kRawTile + from;
+    const int rows = len - t * kTileTokens;  // those from the sequence's end on become zeros
+    uint4 x[4];
 #pragma unroll
-      for (int k = 0; k < 2; ++k)
-        x[k] = plain || row0 + 4 * k < rows ? *reinterpret_cast<const uint4 *>(src + k * 512) : make_uint4(0, 0, 0, 0);
-      if (page) {
-        __syncwarp();
-        if (lane == 0) arrive(&c.raw_empty[r]);
-        ++ring;
-      }
+    for (int k = 0; k < 4; ++k)
+      x[k] = row0 + 32 * k < rows ? *reinterpret_cast<const uint4 *>(src + k * 4096) : make_uint4(0, 0, 0, 0);
+    __syncwarp();
+    if (lane == 0) arrive(&c.raw_empty[r]);
+    ++ring;
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        uint4 lo, hi;
-        widen16<To, kCache>(x[k], lo, hi);
-        // a node's row: e4m3 has NaN
-        if (!plain && kCache == B200KV_E4M3 && is_v && t * kTileTokens + i * kPageTokens + row0 + 4 * k >= ctx) {
-          const bool hit = drop_non_finite<__half>(lo);
-          if (drop_non_finite<__half>(hi) || hit) atomicMax(&c.bad_piece, piece);
-        }
-        uint8_t *line = dst + i * (kPageTokens * 128) + k * 512;
-        const uint32_t at = k & 1 ? at0 ^ 64 : at0;
-        *reinterpret_cast<uint4 *>(line + at) = lo;
-        *reinterpret_cast<uint4 *>(line + (at ^ 16)) = hi;
+    for (int k = 0; k < 4; ++k) {
+      uint4 lo, hi;
+      widen16<To, kCache>(x[k], lo, hi);
+      if (kCache == B200KV_E4M3 && is_v && t * kTileTokens + row0 + 32 * k >= ctx) {  // a node's row: e4m3 has NaN
+        const bool hit = drop_non_finite<__half>(lo);
+        if (drop_non_finite<__half>(hi) || hit) atomicMax(&c.bad_piece, piece);
       }
+      *reinterpret_cast<uint4 *>(dst + k * 4096 + at0) = lo;
+      *reinterpret_cast<uint4 *>(dst + k * 4096 + (at0 ^ 16)) = hi;
     }
     fence_async_smem();
     __syncwarp();
@@ -602,12 +578,12 @@ __device__ __forceinline__ void converter(const Args &a, Ctrl &c, uint8_t *smem,
   w.init(a, c);
   while (w.next(a)) {
     ++piece;
-    const int pages = (w.s.ctx + w.s.nodes + kPageTokens - 1) / kPageTokens;
+    const int len = w.s.ctx + w.s.nodes;
     const int lead = w.two() ? 1 : 2;
-    for (int t = w.t0; t < min(w.t0 + lead, w.t1); ++t) tile(T(), false, t, pages, w.s.ctx);
+    for (int t = w.t0; t < min(w.t0 + lead, w.t1); ++t) tile(T(), false, t, len, w.s.ctx);
     for (int t = w.t0; t < w.t1; ++t) {
-      tile(__half(), true, t, pages, w.s.ctx);
-      if (t + lead < w.t1) tile(T(), false, t + lead, pages, w.s.ctx);
+      tile(__half(), true, t, len, w.s.ctx);
+      if (t + lead < w.t1) tile(T(), false, t + lead, len, w.s.ctx);
     }
     w.advance(a);
   }
@@ -831,24 +807,26 @@ __device__ __forceinline__ void weigh(uint32_t ts, uint32_t to, const uint32_t (
 
 // The same for an 8-bit cache: the 32 * kN tokens that this copy of the row
 // weighs, from token 32 * kN * copy on.
-template <int kN, int D, bool kTail>
+template <int kN, int D, bool kTail, typename Arrived>
 __device__ __forceinline__ void weigh8(uint32_t ts, uint32_t to, const uint32_t (&vis)[4], const Factors *fac, int copy,
-                                       bool first, bool live, float &m, float &l) {
+                                       Arrived arrived, bool first, bool live, float &m, float &l) {
   constexpr bool kKeep = kN <= 2;  // scores stay in registers (else they go back to TMEM for the second pass)
   const int c0 = copy * kN;
   uint32_t y[kKeep ? kN : 1][32];
   float mt = -CUDART_INF_F;
+  // factors of 16 tokens are fetched together, the first before the scores are there
+  const float4 *kf = fac->k + 8 * c0, *vf = fac->log2v + 8 * c0, *inv = fac->inv_v + 8 * c0;
+  float4 k[4], v[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) k[j] = kf[j], v[j] = vf[j];
+  arrived();
 #pragma unroll
   for (int i = 0; i < kN; ++i) {
     uint32_t(&s)[32] = y[kKeep ? i : 0];
     tmem_ld32(ts + 32 * (c0 + i), s);
+    wait_ld(s);
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {  // factors of 16 tokens are fetched together
-      const float4 *kf = fac->k + 8 * (c0 + i) + 4 * h, *vf = fac->log2v + 8 * (c0 + i) + 4 * h;
-      float4 k[4], v[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) k[j] = kf[j], v[j] = vf[j];
-      if (h == 0) wait_ld(s);
+    for (int h = 0; h < 2; ++h) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         uint32_t *r = &s[16 * h + 4 * j];
@@ -858,6 +836,10 @@ __device__ __forceinline__ void weigh8(uint32_t ts, uint32_t to, const uint32_t 
                                make_float2(v[j].z, v[j].w));
         r[0] = __float_as_uint(lo.x), r[1] = __float_as_uint(lo.y);
         r[2] = __float_as_uint(hi.x), r[3] = __float_as_uint(hi.y);
+      }
+      if (i < kN - 1 || h == 0) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) k[j] = kf[8 * i + 4 * h + 4 + j], v[j] = vf[8 * i + 4 * h + 4 + j];
       }
     }
     mt = fmaxf(mt, mask_max<kTail>(s, vis[i]));
@@ -877,7 +859,7 @@ __device__ __forceinline__ void weigh8(uint32_t ts, uint32_t to, const uint32_t 
     for (int j = 0; j < 16; ++j) {
       const float2 x = add2(make_float2(__uint_as_float(s[2 * j]), __uint_as_float(s[2 * j + 1])), make_float2(minus, minus));
       const float2 e = make_float2(ex2(x.x), ex2(x.y));
-      const float4 f = fac->inv_v[8 * (c0 + i) + j / 2];
+      const float4 f = inv[8 * i + j / 2];
       sum[j & 1] = fma2(e, j & 1 ? make_float2(f.z, f.w) : make_float2(f.x, f.y), sum[j & 1]);
       p[j] = pack2(e.x, e.y, __half());
     }
@@ -897,15 +879,15 @@ __device__ __forceinline__ void weigh8(uint32_t ts, uint32_t to, const uint32_t 
   l += t.x + t.y;
   wait_st();
 }
-template <int D, bool kTail>
+template <int D, bool kTail, typename Arrived>
 __device__ __forceinline__ void weigh8(uint32_t ts, uint32_t to, const uint32_t (&vis)[4], const Factors *fac, int copies,
-                                       int copy, bool first, bool live, float &m, float &l) {
+                                       int copy, Arrived arrived, bool first, bool live, float &m, float &l) {
   if (copies == 4)
-    weigh8<1, D, kTail>(ts, to, vis, fac, copy, first, live, m, l);
+    weigh8<1, D, kTail>(ts, to, vis, fac, copy, arrived, first, live, m, l);
   else if (copies == 2)
-    weigh8<2, D, kTail>(ts, to, vis, fac, copy, first, live, m, l);
+    weigh8<2, D, kTail>(ts, to, vis, fac, copy, arrived, first, live, m, l);
   else
-    weigh8<4, D, kTail>(ts, to, vis, fac, copy, first, live, m, l);
+    weigh8<4, D, kTail>(ts, to, vis, fac, copy, arrived, first, live, m, l);
 }
 
 // Element d of a cached V row (8-bit caches: its steps).
@@ -921,19 +903,24 @@ __device__ float cached_v(const Args &a, const void *pool, int id, int kvh, int 
   else
     return __half2float(__half(__nv_cvt_fp8_to_halfraw(static_cast<const uint8_t *>(pool)[at], __NV_E4M3)));
 }
-// What the non-finite elements d of the visible nodes in [from, to) add to a row.
+// Adds the non-finite elements of the piece's visible nodes to elements
+// [d0, d1) of a row that has been written, to its partial sums or its output.
 template <typename T, int D, int kCache>
-__device__ __noinline__ float non_finite_sum(const Args &a, const Seq &s, int b, int kvh, int node, int from, int to,
-                                             int d) {
-  float sum = 0.f;
+__device__ __noinline__ void repair_row(const Args &a, const Seq &s, int b, int kvh, int node, int from, int to, int d0,
+                                        int d1, float *part, T *out) {
   for (int p = max(from, s.ctx); p < min(to, s.ctx + s.nodes); ++p) {
     if (!(visible32(a, s, node, p) & 1u)) continue;
     const int id = __ldg(a.block_table + static_cast<int64_t>(b) * a.bt_stride + p / kPageTokens);
     if (id < 0 || id >= a.num_blocks) continue;
-    const float v = cached_v<T, D, kCache>(a, a.v_pool, id, kvh, p % kPageTokens, d);
-    if (!(fabsf(v) < CUDART_INF_F)) sum += v;
+    for (int d = d0; d < d1; ++d) {
+      const float v = cached_v<T, D, kCache>(a, a.v_pool, id, kvh, p % kPageTokens, d);
+      if (fabsf(v) < CUDART_INF_F) continue;
+      if (part)
+        part[d / 4 * 1024 + d % 4] += v;
+      else
+        from_float(out[d], to_float(out[d]) + v);
+    }
   }
-  return sum;
 }
 
 // One softmax warpgroup (w = 0 or 1); thread = row of its Q tile.
@@ -996,15 +983,18 @@ __device__ __forceinline__ void softmax(const Args &a, Ctrl &c, uint8_t *smem, u
         if (t + step < wk.t1) scales_of(t + step, ks, vs);
         __syncwarp();
       }
-      wait(&c.s_full[w], s_uses++ & 1u, dead, a.error_flag);
-      fence_after();
+      auto arrived = [&] {
+        wait(&c.s_full[w], s_uses++ & 1u, dead, a.error_flag);
+        fence_after();
+      };
+      if (!C::k8 || !warp_live) arrived();
       if (warp_live) {
         const bool first = t == tfirst;
         if constexpr (C::k8) {
           if (tail)
-            weigh8<D, true>(ts, to, vis, fac, q.copies, copy, first, live, m, l);
+            weigh8<D, true>(ts, to, vis, fac, q.copies, copy, arrived, first, live, m, l);
           else
-            weigh8<D, false>(ts, to, vis, fac, q.copies, copy, first, live, m, l);
+            weigh8<D, false>(ts, to, vis, fac, q.copies, copy, arrived, first, live, m, l);
         } else {
           if (tail)
             weigh<typename C::P, D, true>(ts, to, vis, cl, first, live, m, l);
@@ -1080,7 +1070,6 @@ __device__ __forceinline__ void softmax(const Args &a, Ctrl &c, uint8_t *smem, u
     }
     const int64_t orow = static_cast<int64_t>(wk.s.q0 + node) * a.hq + wk.kvh * a.group + row % a.group;
     const float inv = l == 0.f ? 0.f : 1.f / l;
-    const bool repair = *reinterpret_cast<volatile unsigned *>(&c.bad_piece) >= piece;
     const int prow = (two ? w : 0) * kTileRows + row;
     if (C::k8 && q.copies > 1) {
       // add the copies up, 16 columns at a time through shared memory
@@ -1111,13 +1100,6 @@ __device__ __forceinline__ void softmax(const Args &a, Ctrl &c, uint8_t *smem, u
             o = make_float4(o.x + x.x, o.y + x.y, o.z + x.z, o.w + x.w);
           }
           const int dj = d + 4 * j;
-          if (repair) {
-            auto more = [&](int i) {
-              return non_finite_sum<T, D, kCache>(a, wk.s, wk.b, wk.kvh, node, wk.t0 * kTileTokens, wk.t1 * kTileTokens,
-                                                  dj + i);
-            };
-            o = make_float4(o.x + more(0), o.y + more(1), o.z + more(2), o.w + more(3));
-          }
           if (split) {
             *reinterpret_cast<float4 *>(a.part_o + ((static_cast<int64_t>(pslot) * (D / 4) + dj / 4) * 256 + prow) * 4) = o;
           } else {
@@ -1147,13 +1129,6 @@ __device__ __forceinline__ void softmax(const Args &a, Ctrl &c, uint8_t *smem, u
               r[j] = __float_as_uint(fmaf(__uint_as_float(r1[j]), keep1, __uint_as_float(r[j])));
           }
         }
-        if (live && repair) {
-#pragma unroll
-          for (int j = 0; j < 32; ++j)
-            r[j] = __float_as_uint(__uint_as_float(r[j]) +
-                                   non_finite_sum<T, D, kCache>(a, wk.s, wk.b, wk.kvh, node, wk.t0 * kTileTokens,
-                                                                wk.t1 * kTileTokens, d + j));
-        }
         if (live && split) {
 #pragma unroll
           for (int j = 0; j < 8; ++j)
@@ -1172,6 +1147,10 @@ __device__ __forceinline__ void softmax(const Args &a, Ctrl &c, uint8_t *smem, u
         __syncwarp();
       }
     }
+    if (live && copy == 0 && *reinterpret_cast<volatile unsigned *>(&c.bad_piece) >= piece)
+      repair_row<T, D, kCache>(a, wk.s, wk.b, wk.kvh, node, wk.t0 * kTileTokens, wk.t1 * kTileTokens, d0, d1,
+                               split ? a.part_o + (static_cast<int64_t>(pslot) * (D / 4) * 256 + prow) * 4 : nullptr,
+                               static_cast<T *>(a.out) + orow * D);
     if (live && copy == 0 && (two || w == 0)) {
       if (split)
         a.part_ml[static_cast<int64_t>(pslot) * 256 + prow] = make_float2(m, l);
