@@ -70,10 +70,11 @@ __global__ void __launch_bounds__(256) kv_store_kernel(const StoreArgs a) {
   constexpr int kStick = kCache == B200KV_F16 ? 64 : 128;
   const int lane = threadIdx.x % kLanes, e = lane * 8;
   const int heads = a.hq + 2 * a.hkv;
-  const int groups = (heads + kRows - 1) / kRows;
-  const int64_t unit = (int64_t(blockIdx.x) * 256 + threadIdx.x) / kLanes;
-  const int64_t t = unit / groups;
-  const int r0 = static_cast<int>(unit - t * groups) * kRows;
+  const uint32_t groups = (heads + kRows - 1) / kRows;
+  const uint32_t unit = blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes;
+  const uint32_t t32 = unit / groups;
+  const int r0 = static_cast<int>(unit - t32 * groups) * kRows;
+  const int64_t t = t32;
   const bool live_t = t < a.tokens;  // dead lanes stay for the shuffles
 
   uint4 raw[kRows];
@@ -208,7 +209,8 @@ int launch_store(const StoreArgs &a, cudaStream_t stream) {
   const bool deep = a.tokens * heads * kLanes >= int64_t(sms) * 2048 * 4;
   const int64_t units = a.tokens * ((heads + (deep ? 3 : 0)) / (deep ? 4 : 1));
   const int64_t blocks = (units * kLanes + 255) / 256;
-  if (blocks >= (int64_t{1} << 31)) return set_error(B200KV_ERR_UNSUPPORTED, "too many rows (%lld tokens)", (long long)a.tokens);
+  if (units >= (int64_t{1} << 31))  // the kernel counts them in 32 bits
+    return set_error(B200KV_ERR_UNSUPPORTED, "%lld tokens of %d heads: 2^31 rows or more", (long long)a.tokens, heads);
   if (deep)
     kv_store_kernel<T, D, kCache, kTurn, 4><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(a);
   else
@@ -234,100 +236,107 @@ struct LoadArgs {
   const float *scales;
   const int64_t *slots;
   void *out;  // contiguous [N, Hkv, D]
-  int64_t total, num_slots;
-  int hkv;
+  int64_t num_slots;
+  uint32_t rows, hkv;
   int32_t *error_flag;
 };
 
-// kElems elements per thread: 16 bytes of output.  Four of them in flight.
-template <int kCache, typename TIn, typename TOut, int D>
+// A thread makes 16 bytes of output (kElems elements) of kUnroll rows; the
+// kChunks threads of a row are neighbours, so reads and writes are whole lines.
+// All kUnroll slots, then all rows and scales, are in flight together.  Row
+// numbers are 32-bit (the host checks): a 64-bit division per row cost as much
+// as the row's memory traffic.
+template <int kCache, typename TIn, typename TOut, int D, int kUnroll>
 __global__ void __launch_bounds__(256) kv_load_kernel(const LoadArgs a) {
   constexpr bool k8 = kCache != B200KV_F16;
   constexpr int kElems = 16 / sizeof(TOut);
   constexpr int kStick = k8 ? 128 : 64;
   constexpr int kChunks = D / kElems;
-  constexpr int kUnroll = 4;
-  const int64_t step = int64_t(gridDim.x) * blockDim.x;
-  for (int64_t base = blockIdx.x * int64_t(blockDim.x) + threadIdx.x; base < a.total; base += step * kUnroll) {
-    uint32_t w[kUnroll][4];
-    float sc[kUnroll];
-    bool live[kUnroll];
+  constexpr int kRows = 256 / kChunks;
+  const int e = static_cast<int>(threadIdx.x % kChunks) * kElems;
+  const uint32_t row0 = blockIdx.x * (kRows * kUnroll) + threadIdx.x / kChunks;
+  int64_t slot[kUnroll];
+  uint32_t head[kUnroll];
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const int64_t i = base + u * step;
-      live[u] = false;
-      sc[u] = 1.f;
-      if (i >= a.total) continue;
-      const int e = static_cast<int>(i % kChunks) * kElems;
-      const int64_t nh = i / kChunks;
-      const int64_t n = nh / a.hkv;
-      const int h = static_cast<int>(nh - n * a.hkv);
-      const int64_t slot = __ldg(a.slots + n);
-      if (slot < 0) continue;  // padding: a row of zeros
-      if (slot >= a.num_slots) {
-        if (a.error_flag && e == 0 && h == 0) atomicOr(a.error_flag, B200KV_DEVERR_BAD_SLOT);
-        continue;
-      }
-      live[u] = true;
-      const int64_t page = (slot >> 6) * a.hkv + h;
-      const int in_page = static_cast<int>(slot & 63);
-      const TIn *src = static_cast<const TIn *>(a.pool) +
-                       (page * (D / kStick) + e / kStick) * (64 * kStick) + int64_t(in_page) * kStick + e % kStick;
-      if constexpr (kElems * sizeof(TIn) == 16) {
-        const uint4 v = __ldcs(reinterpret_cast<const uint4 *>(src));
-        w[u][0] = v.x, w[u][1] = v.y, w[u][2] = v.z, w[u][3] = v.w;
-      } else if constexpr (kElems * sizeof(TIn) == 8) {
-        const uint2 v = __ldcs(reinterpret_cast<const uint2 *>(src));
-        w[u][0] = v.x, w[u][1] = v.y;
+  for (int u = 0; u < kUnroll; ++u) {
+    const uint32_t row = row0 + u * kRows;
+    slot[u] = -1;
+    if (row < a.rows) {
+      const uint32_t n = row / a.hkv;
+      head[u] = row - n * a.hkv;
+      slot[u] = __ldg(a.slots + n);
+    }
+  }
+  uint32_t w[kUnroll][4];
+  float sc[kUnroll];
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u) {
+    w[u][0] = w[u][1] = w[u][2] = w[u][3] = 0;  // padding, and past the pool: a row of zeros
+    sc[u] = 0.f;
+    if (slot[u] < 0) continue;
+    if (slot[u] >= a.num_slots) {
+      if (a.error_flag && e == 0 && head[u] == 0) atomicOr(a.error_flag, B200KV_DEVERR_BAD_SLOT);
+      continue;
+    }
+    const int64_t page = (slot[u] >> 6) * a.hkv + head[u];
+    const int in_page = static_cast<int>(slot[u] & 63);
+    const TIn *src = static_cast<const TIn *>(a.pool) +
+                     (page * (D / kStick) + e / kStick) * (64 * kStick) + int64_t(in_page) * kStick + e % kStick;
+    if constexpr (kElems * sizeof(TIn) == 16) {
+      const uint4 v = __ldcs(reinterpret_cast<const uint4 *>(src));
+      w[u][0] = v.x, w[u][1] = v.y, w[u][2] = v.z, w[u][3] = v.w;
+    } else if constexpr (kElems * sizeof(TIn) == 8) {
+      const uint2 v = __ldcs(reinterpret_cast<const uint2 *>(src));
+      w[u][0] = v.x, w[u][1] = v.y;
+    } else {
+      w[u][0] = __ldcs(reinterpret_cast<const uint32_t *>(src));
+    }
+    if (k8) sc[u] = __ldg(a.scales + page * 64 + in_page);
+  }
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u) {
+    const uint32_t row = row0 + u * kRows;
+    if (row >= a.rows) continue;
+    TOut o[kElems];
+#pragma unroll
+    for (int j = 0; j < kElems; ++j) {
+      if constexpr (kCache == B200KV_I8) {
+        from_float(o[j], __fmul_rn(static_cast<float>(static_cast<int8_t>(w[u][j >> 2] >> (8 * (j & 3)))), sc[u]));
+      } else if constexpr (kCache == B200KV_E4M3) {
+        const __nv_fp8_storage_t b = static_cast<__nv_fp8_storage_t>(w[u][j >> 2] >> (8 * (j & 3)));
+        from_float(o[j], __fmul_rn(__half2float(__half(__nv_cvt_fp8_to_halfraw(b, __NV_E4M3))), sc[u]));
       } else {
-        w[u][0] = __ldcs(reinterpret_cast<const uint32_t *>(src));
+        const uint16_t b = static_cast<uint16_t>(w[u][j >> 1] >> (16 * (j & 1)));
+        from_float(o[j], to_float(*reinterpret_cast<const TIn *>(&b)));
       }
-      if (k8) sc[u] = __ldg(a.scales + page * 64 + in_page);
     }
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const int64_t i = base + u * step;
-      if (i >= a.total) continue;
-      float f[kElems];
-#pragma unroll
-      for (int j = 0; j < kElems; ++j) {
-        f[j] = 0.f;
-        if (!live[u]) continue;
-        if constexpr (kCache == B200KV_I8) {
-          f[j] = __fmul_rn(static_cast<float>(static_cast<int8_t>(w[u][j >> 2] >> (8 * (j & 3)))), sc[u]);
-        } else if constexpr (kCache == B200KV_E4M3) {
-          const __nv_fp8_storage_t b = static_cast<__nv_fp8_storage_t>(w[u][j >> 2] >> (8 * (j & 3)));
-          f[j] = __fmul_rn(__half2float(__half(__nv_cvt_fp8_to_halfraw(b, __NV_E4M3))), sc[u]);
-        } else {
-          const uint16_t b = static_cast<uint16_t>(w[u][j >> 1] >> (16 * (j & 1)));
-          f[j] = to_float(*reinterpret_cast<const TIn *>(&b));
-        }
-      }
-      TOut o[kElems];
-#pragma unroll
-      for (int j = 0; j < kElems; ++j) from_float(o[j], f[j]);
-      __stcs(reinterpret_cast<uint4 *>(static_cast<TOut *>(a.out) + i * kElems), *reinterpret_cast<uint4 *>(o));
-    }
+    __stcs(reinterpret_cast<uint4 *>(static_cast<TOut *>(a.out) + int64_t(row) * D + e), *reinterpret_cast<uint4 *>(o));
   }
 }
 
 template <int kCache, typename TIn, typename TOut, int D>
-int launch_load(LoadArgs a, int64_t rows, cudaStream_t stream) {
+int launch_load(const LoadArgs &a, cudaStream_t stream) {
   int dev = 0, sms = 0;
   int st = current_device_sm_count(&dev, &sms);
   if (st != B200KV_OK) return st;
-  a.total = rows * (D / (16 / static_cast<int>(sizeof(TOut))));
-  const int64_t want = (a.total + 1023) / 1024, cap = int64_t(sms) * 8;
-  kv_load_kernel<kCache, TIn, TOut, D><<<static_cast<unsigned>(want < cap ? want : cap), 256, 0, stream>>>(a);
+  constexpr int kRows = 256 / (D / (16 / static_cast<int>(sizeof(TOut))));
+  // Eight rows per thread once every SM still gets its 2048 threads, else one.
+  const bool deep = a.rows >= static_cast<uint32_t>(sms) * 8 * kRows * 8;
+  const unsigned per = kRows * (deep ? 8 : 1);
+  const unsigned grid = (a.rows + per - 1) / per;
+  if (deep)
+    kv_load_kernel<kCache, TIn, TOut, D, 8><<<grid, 256, 0, stream>>>(a);
+  else
+    kv_load_kernel<kCache, TIn, TOut, D, 1><<<grid, 256, 0, stream>>>(a);
   B200KV_CUDA_TRY(cudaGetLastError());
   return B200KV_OK;
 }
 template <int kCache, typename TIn, int D>
-int load_out(const LoadArgs &a, int64_t rows, int dtype, cudaStream_t s) {
+int load_out(const LoadArgs &a, int dtype, cudaStream_t s) {
   switch (dtype) {
-    case B200KV_F16: return launch_load<kCache, TIn, __half, D>(a, rows, s);
-    case B200KV_BF16: return launch_load<kCache, TIn, __nv_bfloat16, D>(a, rows, s);
-    default: return launch_load<kCache, TIn, float, D>(a, rows, s);
+    case B200KV_F16: return launch_load<kCache, TIn, __half, D>(a, s);
+    case B200KV_BF16: return launch_load<kCache, TIn, __nv_bfloat16, D>(a, s);
+    default: return launch_load<kCache, TIn, float, D>(a, s);
   }
 }
 
@@ -505,8 +514,12 @@ extern "C" int b200kv_kv_load(const void *pool, int32_t pool_dtype, const float 
   B200KV_CHECK_ARG(out_dtype == B200KV_F16 || out_dtype == B200KV_BF16 || out_dtype == B200KV_F32,
                    "out dtype %d is not fp16, bf16 or fp32", out_dtype);
   B200KV_CHECK_ARG(num_tokens >= 0, "num_tokens must be >= 0 (got %lld)", (long long)num_tokens);
-  B200KV_CHECK_ARG(num_kv_heads > 0 && num_kv_heads <= 65536 && num_blocks > 0 && num_blocks < (int64_t{1} << 40),
-                   "num_kv_heads or num_blocks out of range");
+  B200KV_CHECK_ARG(num_kv_heads > 0 && num_kv_heads <= 65536 && num_blocks > 0 && num_blocks < (int64_t{1} << 40) &&
+                       num_tokens < (int64_t{1} << 31),
+                   "num_kv_heads, num_blocks or num_tokens out of range");
+  if (num_tokens * num_kv_heads >= (int64_t{1} << 31))
+    return set_error(B200KV_ERR_UNSUPPORTED, "%lld tokens of %lld heads: 2^31 rows or more", (long long)num_tokens,
+                     (long long)num_kv_heads);
   if (num_tokens == 0) return B200KV_OK;
   B200KV_CHECK_ARG(pool && slots && out, "null pointer argument");
   B200KV_CHECK_ARG(!k8 || scales, "8-bit pools need their scales");
@@ -514,19 +527,19 @@ extern "C" int b200kv_kv_load(const void *pool, int32_t pool_dtype, const float 
   LoadArgs a{};
   a.pool = pool, a.scales = scales, a.slots = slots, a.out = out;
   a.num_slots = num_blocks * kPageTokens;
-  a.hkv = static_cast<int>(num_kv_heads);
+  a.rows = static_cast<uint32_t>(num_tokens * num_kv_heads);
+  a.hkv = static_cast<uint32_t>(num_kv_heads);
   a.error_flag = error_flag;
-  const int64_t rows = num_tokens * num_kv_heads;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   switch (pool_dtype) {
-    case B200KV_I8: return load_out<B200KV_I8, int8_t, 128>(a, rows, out_dtype, s);
-    case B200KV_E4M3: return load_out<B200KV_E4M3, uint8_t, 128>(a, rows, out_dtype, s);
+    case B200KV_I8: return load_out<B200KV_I8, int8_t, 128>(a, out_dtype, s);
+    case B200KV_E4M3: return load_out<B200KV_E4M3, uint8_t, 128>(a, out_dtype, s);
     case B200KV_F16:
-      return head_dim == 64 ? load_out<B200KV_F16, __half, 64>(a, rows, out_dtype, s)
-                            : load_out<B200KV_F16, __half, 128>(a, rows, out_dtype, s);
+      return head_dim == 64 ? load_out<B200KV_F16, __half, 64>(a, out_dtype, s)
+                            : load_out<B200KV_F16, __half, 128>(a, out_dtype, s);
     default:
-      return head_dim == 64 ? load_out<B200KV_F16, __nv_bfloat16, 64>(a, rows, out_dtype, s)
-                            : load_out<B200KV_F16, __nv_bfloat16, 128>(a, rows, out_dtype, s);
+      return head_dim == 64 ? load_out<B200KV_F16, __nv_bfloat16, 64>(a, out_dtype, s)
+                            : load_out<B200KV_F16, __nv_bfloat16, 128>(a, out_dtype, s);
   }
 }
 
