@@ -1,14 +1,24 @@
-"""The short way from a public function to its C entry.
+"""The short ways from a public function to its C entry.
 
 A ``torch.library.custom_op`` costs 15-25 us of host time per call (dispatcher,
 autograd and in-place bookkeeping), several times the kernels of a decode step.
-In plain eager mode the public functions therefore call their implementation
-directly; under torch.compile, fake tensors, dispatch modes or functorch
-transforms they go through the registered operator, whose kernel is the same
-implementation.
+So in plain eager mode, with nothing to differentiate, the public functions of
+the verification operators take one of two shorter ways:
+
+* the ``_fast`` module (csrc/fast_call.cpp) checks, allocates and launches
+  without Python; it returns None when anything is not plain or not as the
+  operator wants it;
+* then the Python implementation runs directly (it raises for what is wrong).
+
+Under torch.compile, fake tensors, dispatch modes, functorch transforms and for
+inputs that require a gradient they go through the registered operator, whose
+kernel is the same Python implementation.
 """
 
 from __future__ import annotations
+
+import ctypes
+import importlib.util
 
 import torch
 
@@ -19,12 +29,43 @@ _modes = torch._C._len_torch_dispatch_stack
 _interpreter = torch._C._functorch.peek_interpreter_stack
 _stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 _device = getattr(torch._C, "_cuda_getDevice", None)
+compiling = torch.compiler.is_compiling
+
+# the order of Entries in csrc/fast_call.cpp
+_ENTRIES = ("b200kv_rotary", "b200kv_kv_store", "b200kv_kv_load", "b200kv_tree_mask", "b200kv_tree_workspace_bytes",
+            "b200kv_tree_attention", "b200kv_tree_commit")
 
 
-def direct(x: torch.Tensor) -> bool:
-    """Whether a call on x may skip the dispatcher."""
-    return (type(x) in _PLAIN and x.is_cuda and not _modes() and _interpreter() is None
-            and not torch.compiler.is_compiling())
+class _Unbound:
+    """Stands in until the first call: loads the library and binds the module to it."""
+
+    def __getattr__(self, name):
+        global fast
+        path = _lib.LIB_PATH.parent / "_fast.so"
+        if not path.exists():
+            raise ImportError(f"{path} is missing: build it with `python -m torch_spyre_b200.build`")
+        spec = importlib.util.spec_from_file_location("_fast", path)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        handle = _lib.lib()
+        module.bind(*(ctypes.cast(getattr(handle, e), ctypes.c_void_p).value for e in _ENTRIES))
+        fast = module
+        return getattr(module, name)
+
+
+fast = _Unbound()
+
+
+def plain(t: torch.Tensor) -> bool:
+    return type(t) in _PLAIN and t.is_cuda
+
+
+def direct(*tensors) -> bool:
+    """Whether a call on these tensors (None among them) may skip the dispatcher."""
+    if _modes() or _interpreter() is not None or compiling():
+        return False
+    grad = torch.is_grad_enabled()
+    return all(t is None or (plain(t) and not (grad and t.requires_grad)) for t in tensors)
 
 
 def launch(name: str, device: torch.device, *args) -> None:
@@ -41,4 +82,4 @@ def launch(name: str, device: torch.device, *args) -> None:
 
 def written(*tensors) -> None:
     """Marks tensors as changed in place, as the registered operator does."""
-    torch.autograd.graph.increment_version([t for t in tensors if t is not None])
+    torch.autograd.graph.increment_version([t for t in tensors if t is not None and not t.is_inference()])

@@ -11,12 +11,14 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG_DIR = Path(__file__).resolve().parent
 CSRC = PKG_DIR / "csrc"
 LIB_DIR = PKG_DIR / "lib"
 LIB_PATH = LIB_DIR / "libb200kv.so"
+FAST_PATH = LIB_DIR / "_fast.so"  # the Python module of csrc/fast_call.cpp
 INCLUDE = PKG_DIR.parent / "include"
 
 SOURCES = [
@@ -57,11 +59,35 @@ def _needs_rebuild() -> bool:
     return any(p.stat().st_mtime > mtime for p in deps)
 
 
+def build_fast(force: bool = False) -> Path:
+    """Compiles the module that calls the library without Python in between."""
+    src = CSRC / "fast_call.cpp"
+    if not force and FAST_PATH.exists() and FAST_PATH.stat().st_mtime >= src.stat().st_mtime:
+        return FAST_PATH
+    import torch
+
+    root = Path(torch.__file__).resolve().parent
+    cuda_home = Path(nvcc_path()).resolve().parent.parent
+    includes = [root / "include", root / "include" / "torch" / "csrc" / "api" / "include",
+                sysconfig.get_paths()["include"], cuda_home / "include"]
+    tmp = FAST_PATH.with_suffix(".so.tmp")
+    cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *[f"-I{p}" for p in includes], str(src),
+           "-o", str(tmp), f"-L{root / 'lib'}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"]
+    proc = subprocess.run(cmd, capture_output=True, text=True)
+    if proc.returncode != 0:
+        raise RuntimeError(f"g++ failed ({proc.returncode}):\n{' '.join(cmd)}\n{proc.stderr}")
+    os.replace(tmp, FAST_PATH)
+    return FAST_PATH
+
+
 def build(force: bool = False, verbose: bool = False) -> Path:
-    """Compiles every CUDA source of the library into one shared object."""
+    """Compiles every CUDA source of the library into one shared object, and the
+    module that calls it."""
+    LIB_DIR.mkdir(exist_ok=True)
+    build_fast(force)
     if not force and not _needs_rebuild():
         return LIB_PATH
-    LIB_DIR.mkdir(exist_ok=True)
     tmp = LIB_PATH.with_suffix(".so.tmp")
     cmd = [
         nvcc_path(),

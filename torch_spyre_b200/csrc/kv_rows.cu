@@ -39,24 +39,25 @@ struct StoreArgs {
 
 // Eight fp32 -> eight 8-bit steps of 1 / inv.  fp32 arithmetic, each operation
 // rounded by itself, so the same steps as x * (1 / s) computed anywhere else.
+// |x * inv| exceeds qmax by a few 2^-24 at most (inv and s are rounded), which
+// rounds to qmax: no clamp is needed.
 __device__ __forceinline__ uint2 steps8_int8(const float (&f)[8], float inv) {
-  uint32_t w[2] = {0, 0};
+  // 1.5 * 2^23 + x: the nearest integer (ties to even) is in the low byte
+  uint32_t b[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float c = fminf(fmaxf(__fmul_rn(f[i], inv), -kQMaxInt8), kQMaxInt8);
-    w[i >> 2] |= (static_cast<uint32_t>(__float2int_rn(c)) & 0xffu) << (8 * (i & 3));
-  }
-  return make_uint2(w[0], w[1]);
+  for (int i = 0; i < 8; ++i) b[i] = __float_as_uint(__fadd_rn(__fmul_rn(f[i], inv), 12582912.f));
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = __byte_perm(b[2 * i], b[2 * i + 1], 0x0040);
+  return make_uint2(__byte_perm(w[0], w[1], 0x5410), __byte_perm(w[2], w[3], 0x5410));
 }
 __device__ __forceinline__ uint2 steps8_e4m3(const float (&f)[8], float inv) {
-  uint32_t w[2] = {0, 0};
+  uint32_t w[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 p = make_float2(fminf(fmaxf(__fmul_rn(f[2 * i], inv), -kQMaxE4M3), kQMaxE4M3),
-                                 fminf(fmaxf(__fmul_rn(f[2 * i + 1], inv), -kQMaxE4M3), kQMaxE4M3));
-    w[i >> 1] |= static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(p, __NV_SATFINITE, __NV_E4M3)) << (16 * (i & 1));
-  }
-  return make_uint2(w[0], w[1]);
+  for (int i = 0; i < 4; ++i)
+    w[i] = __nv_cvt_float2_to_fp8x2(make_float2(__fmul_rn(f[2 * i], inv), __fmul_rn(f[2 * i + 1], inv)), __NV_SATFINITE,
+                                    __NV_E4M3);
+  return make_uint2(__byte_perm(w[0], w[1], 0x5410), __byte_perm(w[2], w[3], 0x5410));
 }
 
 // A group of D / 8 lanes takes one row, kRows rows of a token one after the
@@ -65,7 +66,7 @@ __device__ __forceinline__ uint2 steps8_e4m3(const float (&f)[8], float inv) {
 // is a multiple of 8, so the partner is a whole lane away).
 // kCache: B200KV_F16 (= the row type), B200KV_I8 or B200KV_E4M3.
 template <typename T, int D, int kCache, int kTurn, int kRows>  // kTurn 0 none, 1 half, 2 interleaved
-__global__ void __launch_bounds__(256) kv_store_kernel(const StoreArgs a) {
+__global__ void __launch_bounds__(256, kRows > 1 ? 5 : 1) kv_store_kernel(const StoreArgs a) {
   constexpr int kLanes = D / 8;
   constexpr int kStick = kCache == B200KV_F16 ? 64 : 128;
   const int lane = threadIdx.x % kLanes, e = lane * 8;
@@ -117,13 +118,20 @@ __global__ void __launch_bounds__(256) kv_store_kernel(const StoreArgs a) {
         pos = pos < 0 ? 0 : a.max_pos - 1;
       }
       const float2 *row = a.table + pos * a.half + (kTurn == 2 ? e / 2 : (second ? e - a.half : e));
+      if (kTurn == 1 || (a.half % 2 == 0 && e / 2 + 4 <= a.half)) {  // 16-byte aligned, all inside
 #pragma unroll
-      for (int i = 0; i < kPairs; ++i) {
-        // an interleaved vector cut by rotary_dim: the identity past it
-        const bool in = kTurn == 1 || e / 2 + i < a.half;
-        const float2 cs = in ? __ldg(row + i) : make_float2(1.f, 0.f);
-        cosv[i] = cs.x;
-        sinv[i] = cs.y;
+        for (int i = 0; i < kPairs; i += 2) {
+          const float4 cs = __ldg(reinterpret_cast<const float4 *>(row + i));
+          cosv[i] = cs.x, sinv[i] = cs.y, cosv[i + 1] = cs.z, sinv[i + 1] = cs.w;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) {
+          // an interleaved vector cut by rotary_dim: the identity past it
+          const float2 cs = e / 2 + i < a.half ? __ldg(row + i) : make_float2(1.f, 0.f);
+          cosv[i] = cs.x;
+          sinv[i] = cs.y;
+        }
       }
     }
   }
@@ -136,7 +144,8 @@ __global__ void __launch_bounds__(256) kv_store_kernel(const StoreArgs a) {
     const bool live = live_t && r < heads;
     float f[8];
     if (live) unpack8(raw[i], f, T());
-    if (kTurn == 1) {
+    // (rows of two kinds can meet in a warp: it skips what none of them needs)
+    if (kTurn == 1 && __any_sync(0xffffffffu, live && r < a.hq + a.hkv)) {
       uint4 o;  // every lane takes part in the shuffles
       o.x = __shfl_sync(0xffffffffu, raw[i].x, partner, kLanes);
       o.y = __shfl_sync(0xffffffffu, raw[i].y, partner, kLanes);
@@ -164,6 +173,7 @@ __global__ void __launch_bounds__(256) kv_store_kernel(const StoreArgs a) {
       T *dst = static_cast<T *>(a.q_out) + (t * a.hq + r) * D + e;
       *reinterpret_cast<uint4 *>(dst) = pack8(f, T());
     }
+    if (!__any_sync(0xffffffffu, live && r >= a.hq)) continue;
     const bool is_k = r < a.hq + a.hkv;
     const int h = r - a.hq - (is_k ? 0 : a.hkv);
     const bool write = live && r >= a.hq && slot >= 0;
@@ -205,7 +215,10 @@ int launch_store(const StoreArgs &a, cudaStream_t stream) {
   constexpr int kLanes = D / 8;
   const int heads = a.hq + 2 * a.hkv;
   // Four rows per lane group once every SM still gets its 2048 threads; with
-  // fewer rows one each, as the latency of the loads counts.
+  // fewer rows one each, as the latency of the loads counts.  (16381 tokens of
+  // 32 + 16 heads into e4m3, us with two readings back: two rows 131 at four
+  // blocks per SM and 113 at six, four rows 117 at four and 116 at five, eight
+  // rows 116 at four; int8 in the half layout 143, 156, 124, 127 and 135.)
   const bool deep = a.tokens * heads * kLanes >= int64_t(sms) * 2048 * 4;
   const int64_t units = a.tokens * ((heads + (deep ? 3 : 0)) / (deep ? 4 : 1));
   const int64_t blocks = (units * kLanes + 255) / 256;
@@ -478,7 +491,7 @@ extern "C" int b200kv_kv_store(const void *q, int64_t q_stride_n, int64_t q_stri
   B200KV_CHECK_ARG(!k8 || (k_scales && v_scales), "8-bit pools need k_scales and v_scales");
   B200KV_CHECK_ARG(!table || positions, "a table needs positions");
   B200KV_CHECK_ARG(aligned_to(k, 16) && aligned_to(v, 16) && aligned_to(k_pool, 16) && aligned_to(v_pool, 16) &&
-                       (num_q_heads == 0 || (aligned_to(q, 16) && aligned_to(q_out, 16))) && aligned_to(table, 8),
+                       (num_q_heads == 0 || (aligned_to(q, 16) && aligned_to(q_out, 16))) && aligned_to(table, 16),
                    "buffers must be 16-byte aligned");
   B200KV_CHECK_ARG(k_stride_n % 8 == 0 && k_stride_h % 8 == 0 && v_stride_n % 8 == 0 && v_stride_h % 8 == 0 &&
                        (num_q_heads == 0 || (q_stride_n % 8 == 0 && q_stride_h % 8 == 0)),

@@ -17,6 +17,7 @@ from typing import Optional
 
 import torch
 
+from . import _eager
 from ._eager import direct, launch, written
 from .layout import PAGE_TOKENS
 from .ops import _maybe_check_flag, _ptr, _require_cuda
@@ -158,11 +159,13 @@ def kv_store(
     in between); ``q`` [N, Hq, D] is turned by the same launch and returned.
     Slots must be distinct; negative slots skip their row."""
     args = (k_new, v_new, k_pool, v_pool, slots, k_scales, v_scales, q, table, positions, bool(interleaved), error_flag)
-    if direct(k_new):
-        out = _kv_store_impl(*args)
-        written(k_pool, v_pool, k_scales, v_scales)
-    else:
-        out = torch.ops.b200kv.kv_store(*args)
+    out = None if _eager.compiling() else _eager.fast.kv_store(*args)
+    if out is None:
+        if direct(k_new, v_new, k_pool, v_pool, slots, k_scales, v_scales, q, table, positions):
+            out = _kv_store_impl(*args)
+            written(k_pool, v_pool, k_scales, v_scales)
+        else:
+            out = torch.ops.b200kv.kv_store(*args)
     return None if q is None else out
 
 
@@ -197,5 +200,9 @@ def kv_load(pool: torch.Tensor, slots: torch.Tensor, scales: Optional[torch.Tens
     Negative slots give rows of zeros."""
     if dtype is None:
         dtype = pool.dtype if pool.dtype in DTYPES_16 else torch.float16
-    op = _kv_load_impl if direct(pool) else torch.ops.b200kv.kv_load
+    if not _eager.compiling():
+        out = _eager.fast.kv_load(pool, slots, scales, DTYPE_CODES.get(dtype, -1), error_flag)
+        if out is not None:
+            return out
+    op = _kv_load_impl if direct(pool, slots, scales) else torch.ops.b200kv.kv_load
     return op(pool, slots, scales, dtype, error_flag)

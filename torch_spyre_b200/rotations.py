@@ -17,8 +17,8 @@ from typing import Optional
 
 import torch
 
-from . import _lib
-from ._eager import direct, launch
+from . import _eager, _lib
+from ._eager import launch
 from .ops import _maybe_check_flag, _ptr, _require_cuda
 
 ROTARY_SCALINGS = ("none", "linear", "ntk", "yarn")
@@ -141,17 +141,21 @@ class _Rotary(torch.autograd.Function):
     def forward(ctx, x, table, positions, interleaved, transpose, error_flag):
         ctx.save_for_backward(table, positions)
         ctx.turn = (interleaved, transpose, error_flag)
-        return _rotary_impl(x, table, positions, interleaved, transpose, error_flag)
+        y = _eager.fast.rotary(x, table, positions, interleaved, transpose, error_flag)
+        return _rotary_impl(x, table, positions, interleaved, transpose, error_flag) if y is None else y
 
     backward = staticmethod(_rotary_backward)
 
 
 def _turn(x, table, positions, interleaved, transpose, error_flag):
-    if not direct(x):
-        return torch.ops.b200kv.rotary(x, table, positions, interleaved, transpose, error_flag)
-    if x.requires_grad and torch.is_grad_enabled():
-        return _Rotary.apply(x, table, positions, interleaved, transpose, error_flag)
-    return _rotary_impl(x, table, positions, interleaved, transpose, error_flag)
+    args = (x, table, positions, interleaved, transpose, error_flag)
+    if not _eager.compiling():
+        y = _eager.fast.rotary(*args)
+        if y is not None:
+            return y
+        if _eager.plain(x) and _eager.direct(table, positions):
+            return _Rotary.apply(*args) if x.requires_grad and torch.is_grad_enabled() else _rotary_impl(*args)
+    return torch.ops.b200kv.rotary(*args)
 
 
 def rotary(x: torch.Tensor, table: torch.Tensor, positions: torch.Tensor, interleaved: bool = False,

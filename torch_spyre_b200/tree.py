@@ -20,7 +20,7 @@ from typing import Optional
 
 import torch
 
-from . import _lib
+from . import _eager, _lib
 from ._eager import direct, launch, written
 from .kv_rows import DTYPES_16, check_row_pools
 from .ops import _maybe_check_flag, _ptr, _require_cuda, workspace_for
@@ -73,8 +73,11 @@ def tree_mask(parents: torch.Tensor, q_indptr: torch.Tensor, max_nodes: int,
     itself and its ancestors.  parents int32 [N] are indexes inside the node's
     own sequence (nodes q_indptr[b] .. q_indptr[b + 1] - 1), smaller than the
     node's; -1 marks a root, -2 a pruned node, which sees nothing."""
-    op = _tree_mask_impl if direct(parents) else torch.ops.b200kv.tree_mask
-    return op(parents, q_indptr, max(1, -(-int(max_nodes) // 64)), error_flag)
+    args = (parents, q_indptr, max(1, -(-int(max_nodes) // 64)), error_flag)
+    mask = None if _eager.compiling() else _eager.fast.tree_mask(*args)
+    if mask is None:
+        mask = _tree_mask_impl(*args) if direct(parents, q_indptr) else torch.ops.b200kv.tree_mask(*args)
+    return mask
 
 
 # ---------------------------------------------------------------- attention --
@@ -122,6 +125,8 @@ def _attend(q, k_pool, v_pool, block_table, context_lens, q_indptr, tree_mask, s
     wbytes = _lib.lib().b200kv_tree_workspace_bytes(N, B, Hq, Hkv, D)
     # An unsupported shape has no workspace size; the call below then reports why.
     ws = workspace_for(device, wbytes) if wbytes > 0 else torch.empty(0, dtype=torch.uint8, device=device)
+    if wbytes > 0:
+        _eager.fast.set_workspace(ws)  # where the next call finds it
     launch(
         "b200kv_tree_attention", device, q.data_ptr(), DTYPE_CODES[dtype], q.stride(0), q.stride(1),
         k_pool.data_ptr(), v_pool.data_ptr(), DTYPE_CODES[k_pool.dtype], _ptr(k_scales), _ptr(v_scales),
@@ -177,7 +182,11 @@ def tree_attention(
         max_nodes = q.shape[0] if tree_mask is None else min(q.shape[0], 64 * tree_mask.shape[1])
     args = (q, k_pool, v_pool, block_table, context_lens, q_indptr, tree_mask, float(scale), max(1, int(max_nodes)),
             k_scales, v_scales, error_flag)
-    out, lse = _attend(*args, return_lse) if direct(q) else torch.ops.b200kv.tree_attention(*args)
+    pair = None if _eager.compiling() else _eager.fast.tree_attention(*args, bool(return_lse))
+    if pair is None:
+        plain = direct(q, k_pool, v_pool, block_table, context_lens, q_indptr, tree_mask, k_scales, v_scales)
+        pair = _attend(*args, return_lse) if plain else torch.ops.b200kv.tree_attention(*args)
+    out, lse = pair
     return (out, lse) if return_lse else out
 
 
@@ -240,8 +249,10 @@ def tree_commit(
     their sequence, in place, and returns the new lengths
     context_lens + path_lens (int32 [B])."""
     args = (k_pool, v_pool, block_table, context_lens, path, path_lens, k_scales, v_scales, error_flag)
-    if not direct(k_pool):
-        return torch.ops.b200kv.tree_commit(*args)
-    new_lens = _tree_commit_impl(*args)
-    written(k_pool, v_pool, k_scales, v_scales)
+    new_lens = None if _eager.compiling() else _eager.fast.tree_commit(*args)
+    if new_lens is None:
+        if not direct(k_pool, v_pool, block_table, context_lens, path, path_lens, k_scales, v_scales):
+            return torch.ops.b200kv.tree_commit(*args)
+        new_lens = _tree_commit_impl(*args)
+        written(k_pool, v_pool, k_scales, v_scales)
     return new_lens
