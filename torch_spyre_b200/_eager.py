@@ -19,6 +19,7 @@ from __future__ import annotations
 
 import ctypes
 import importlib.util
+from pathlib import Path
 
 import torch
 
@@ -41,7 +42,7 @@ class _Unbound:
 
     def __getattr__(self, name):
         global fast
-        path = _lib.LIB_PATH.parent / "_fast.so"
+        path = Path(__file__).resolve().parent / "lib" / "_fast.so"
         if not path.exists():
             raise ImportError(f"{path} is missing: build it with `python -m torch_spyre_b200.build`")
         spec = importlib.util.spec_from_file_location("_fast", path)

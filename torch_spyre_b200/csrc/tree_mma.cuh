@@ -83,15 +83,24 @@ constexpr uint32_t kTmemCols = 512;
 __device__ __forceinline__ uint32_t col_s(int w) { return uint32_t(w) * 128u; }
 __device__ __forceinline__ uint32_t col_o(int w) { return 256u + uint32_t(w) * 128u; }
 
+struct Seq {
+  int ctx, nodes, q0, blocks, qtiles;
+};
+// Where a CTA's share of the line begins: a block's token tile.
+struct Start {
+  Seq s;
+  int b, kvh, block, tiles, tile;
+};
+
 struct Ctrl {
   uint64_t full[8], empty[8];          // operand tiles
   uint64_t raw_full[8], raw_empty[8];  // 8-bit tiles
   uint64_t q_full, q_empty;
   uint64_t s_full[2], p_ready[2], o_full[2];
   uint32_t tmem;
-  int start_b;
-  long long start_rem, per, total;
-  long long scan[16];
+  int per, total;  // tiles of a share, of the line
+  Start start;
+  int scan[32];
   unsigned bad_piece;       // last piece (counted from 1) that met a non-finite value in a node's V row
   float2 ml[2][kTileRows];  // (maximum, sum) of the streams' rows
 };
@@ -208,9 +217,6 @@ __device__ __forceinline__ uint32_t elect_one() {
 __device__ __forceinline__ uint32_t uniform(uint32_t x) { return __shfl_sync(0xffffffffu, x, 0); }
 
 // -------------------------------------------------------------------- plan --
-struct Seq {
-  int ctx, nodes, q0, blocks, qtiles;
-};
 template <int kQ>
 __device__ __forceinline__ Seq load_seq(const Args &a, int b, bool report) {
   const int cap = a.max_blocks * kPageTokens;
@@ -238,9 +244,9 @@ __device__ __forceinline__ int block_tiles(const Args &a, const Seq &s, int k) {
   return (s.ctx + nodes + kTileTokens - 1) / kTileTokens;
 }
 template <int kQ>
-__device__ __forceinline__ long long head_units(const Args &a, const Seq &s) {
-  if (a.mask) return static_cast<long long>(s.blocks) * (s.blocks ? block_tiles<kQ>(a, s, 0) : 0);
-  long long n = 0;
+__device__ __forceinline__ int head_units(const Args &a, const Seq &s) {
+  if (a.mask) return s.blocks * (s.blocks ? block_tiles<kQ>(a, s, 0) : 0);
+  int n = 0;
   for (int k = 0; k < s.blocks; ++k) n += block_tiles<kQ>(a, s, k);
   return n;
 }
@@ -269,32 +275,18 @@ template <int kQ>
 struct Walk {
   Seq s;
   int b, kvh, block, tiles, t0, t1;  // piece: token tiles [t0, t1) of `tiles`
-  int next_tile;
-  long long left;
+  int next_tile, left;
 
   __device__ __forceinline__ void init(const Args &a, const Ctrl &c) {
-    b = c.start_b;
-    left = min(c.per, c.total - static_cast<long long>(blockIdx.x) * c.per);
-    if (left <= 0) return;
-    s = load_seq<kQ>(a, b, false);
-    const long long hu = head_units<kQ>(a, s);
-    kvh = static_cast<int>(c.start_rem / hu);
-    long long rem = c.start_rem - kvh * hu;
-    block = 0;
-    if (a.mask) {
-      tiles = block_tiles<kQ>(a, s, 0);
-      block = static_cast<int>(rem / tiles);
-      rem -= static_cast<long long>(block) * tiles;
-    } else {
-      while (rem >= (tiles = block_tiles<kQ>(a, s, block))) rem -= tiles, ++block;
-    }
-    next_tile = static_cast<int>(rem);
+    left = min(c.per, c.total - static_cast<int>(blockIdx.x) * c.per);
+    const Start &f = c.start;
+    s = f.s, b = f.b, kvh = f.kvh, block = f.block, tiles = f.tiles, next_tile = f.tile;
   }
   // The next piece, false when the share is done.
   __device__ __forceinline__ bool next(const Args &a) {
     if (left <= 0) return false;
     t0 = next_tile;
-    t1 = static_cast<int>(min(static_cast<long long>(tiles), t0 + left));
+    t1 = min(tiles, t0 + left);
     left -= t1 - t0;
     return true;
   }
@@ -314,41 +306,55 @@ struct Walk {
   __device__ __forceinline__ bool two() const { return kQ == 2 && 2 * block + 1 < s.qtiles; }
 };
 
-// First unit, share and total of the line; all threads of the CTA call it.
+// The line's length, a share's, and where this CTA's begins; all threads of the
+// CTA call it, a barrier follows.  The counts fit 31 bits (the host checks).
 template <int kThreads, int kQ>
 __device__ __forceinline__ void make_plan(const Args &a, Ctrl &c) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int each = (a.batch + kThreads - 1) / kThreads;
   const int b0 = tid * each, b1 = min(b0 + each, a.batch);
-  long long mine = 0;
-  for (int b = b0; b < b1; ++b) mine += head_units<kQ>(a, load_seq<kQ>(a, b, blockIdx.x == 0)) * a.hkv;
-  long long incl = mine;
+  Seq s{};
+  int mine = 0;
+  for (int b = b0; b < b1; ++b) {
+    s = load_seq<kQ>(a, b, blockIdx.x == 0);
+    mine += head_units<kQ>(a, s) * a.hkv;
+  }
+  int incl = mine;
 #pragma unroll
   for (int m = 1; m < 32; m <<= 1) {
-    const long long y = __shfl_up_sync(0xffffffffu, incl, m);
+    const int y = __shfl_up_sync(0xffffffffu, incl, m);
     if (lane >= m) incl += y;
   }
   if (lane == 31) c.scan[warp] = incl;
   __syncthreads();
-  long long total = 0, before = 0;
+  int total = 0, before = 0;
 #pragma unroll
   for (int w = 0; w < kThreads / 32; ++w) {
     if (w < warp) before += c.scan[w];
     total += c.scan[w];
   }
-  const long long per = (total + gridDim.x - 1) / gridDim.x;
-  const long long first = static_cast<long long>(blockIdx.x) * per;
-  long long at = before + incl - mine;
+  const int per = static_cast<int>((static_cast<unsigned>(total) + gridDim.x - 1) / gridDim.x);
+  const int first = static_cast<int>(blockIdx.x) * per;
+  int at = before + incl - mine;
   if (first >= at && first < at + mine) {
-    for (int b = b0; b < b1; ++b) {
-      const long long n = head_units<kQ>(a, load_seq<kQ>(a, b, false)) * a.hkv;
-      if (first < at + n) {
-        c.start_b = b;
-        c.start_rem = first - at;
-        break;
-      }
-      at += n;
+    int b = b0, hu = 0;
+    for (;; ++b) {
+      if (each > 1) s = load_seq<kQ>(a, b, false);
+      hu = head_units<kQ>(a, s);
+      if (first < at + hu * a.hkv) break;
+      at += hu * a.hkv;
     }
+    int rem = first - at, block = 0, tiles;
+    const int kvh = rem / hu;
+    rem -= kvh * hu;
+    if (a.mask) {
+      tiles = block_tiles<kQ>(a, s, 0);
+      block = rem / tiles;
+      rem -= block * tiles;
+    } else {
+      while (rem >= (tiles = block_tiles<kQ>(a, s, block))) rem -= tiles, ++block;
+    }
+    c.start = Start{s, b, kvh, block, tiles, rem};
   }
   if (tid == 0) {
     c.per = per;
@@ -390,26 +396,28 @@ __device__ __forceinline__ void producer(const Args &a, Ctrl &c, uint8_t *smem, 
   while (w.next(a)) {
     const bool two = w.two();
     const int pages = (w.s.ctx + w.s.nodes + kPageTokens - 1) / kPageTokens;
-    if (lane == 0) {
-      wait(&c.q_empty, (pieces & 1u) ^ 1u, dead, a.error_flag);
-      if constexpr (C::k8) {
-        const Copies q = copies_of(a, w.s, w.block);
-        mbar_arrive_expect_tx(&c.q_full, uint32_t(q.copies * q.boxes) * C::kSticks * a.q_box_bytes);
-        for (int k = 0; k < q.copies; ++k)
-          for (int i = 0; i < q.boxes; ++i)
-            for (int st = 0; st < C::kSticks; ++st)
-              tma_3d(smem + C::kOffQ + st * C::kStickTile + (k * q.rows + i * 32) * 128, qm, &c.q_full, st * 64,
-                     w.kvh * a.group, w.s.q0 + w.block * a.tile_nodes + i * a.box_nodes);
-      } else {
-        mbar_arrive_expect_tx(&c.q_full, (two ? 2u : 1u) * C::kSticks * a.q_box_bytes);
-        for (int i = 0; i < (two ? 2 : 1); ++i)
-          for (int st = 0; st < C::kSticks; ++st)
-            tma_3d(smem + C::kOffQ + i * C::kTile + st * C::kStickTile, qm, &c.q_full, st * 64, w.kvh * a.group,
-                   w.s.q0 + (C::kQ * w.block + i) * a.tile_nodes);
-      }
+    int window = w.t0 / 16, ids = load_ids(a, w.b, window, pages), ids_next = load_ids(a, w.b, window + 1, pages);
+    wait(&c.q_empty, (pieces & 1u) ^ 1u, dead, a.error_flag);
+    // lane: a box of Q (16-bit pools: of one or two Q tiles; 8-bit: of the
+    // tile's copies) and stick column
+    const int st = lane % C::kSticks, box = lane / C::kSticks;
+    if constexpr (C::k8) {
+      const Copies q = copies_of(a, w.s, w.block);
+      const int n = q.copies * q.boxes, k = box / q.boxes, i = box - k * q.boxes;
+      if (lane == 0) mbar_arrive_expect_tx(&c.q_full, uint32_t(n) * C::kSticks * a.q_box_bytes);
+      __syncwarp();
+      if (box < n)
+        tma_3d(smem + C::kOffQ + st * C::kStickTile + (k * q.rows + i * 32) * 128, qm, &c.q_full, st * 64,
+               w.kvh * a.group, w.s.q0 + w.block * a.tile_nodes + i * a.box_nodes);
+    } else {
+      const int n = two ? 2 : 1;
+      if (lane == 0) mbar_arrive_expect_tx(&c.q_full, uint32_t(n) * C::kSticks * a.q_box_bytes);
+      __syncwarp();
+      if (box < n)
+        tma_3d(smem + C::kOffQ + box * C::kTile + st * C::kStickTile, qm, &c.q_full, st * 64, w.kvh * a.group,
+               w.s.q0 + (C::kQ * w.block + box) * a.tile_nodes);
     }
     ++pieces;
-    int window = w.t0 / 16, ids = load_ids(a, w.b, window, pages), ids_next = load_ids(a, w.b, window + 1, pages);
     int ids_before = ids;
     auto issue = [&](bool is_v, int t) {
       if (t / 16 > window) {  // K leads, V follows by at most two tiles
@@ -1112,35 +1120,38 @@ __device__ __forceinline__ void softmax(const Args &a, Ctrl &c, uint8_t *smem, u
         bar_group(w);
       }
     } else if (warp_live) {
+      // (short steps: this code runs once per piece, mostly out of a cold
+      // instruction cache)
 #pragma unroll 1
-      for (int d = d0; d < d1; d += 32) {
-        uint32_t r[32];
-        tmem_ld32(two ? to + d : quad + col_o(0) + d, r);
+      for (int d = d0; d < d1; d += 16) {
+        uint32_t r[16];
+        tmem_ld16(two ? to + d : quad + col_o(0) + d, r);
         wait_ld(r);
         if (!two) {
 #pragma unroll
-          for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * keep0);
+          for (int j = 0; j < 16; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * keep0);
           if (both) {
-            uint32_t r1[32];
-            tmem_ld32(quad + col_o(1) + d, r1);
+            uint32_t r1[16];
+            tmem_ld16(quad + col_o(1) + d, r1);
             wait_ld(r1);
 #pragma unroll
-            for (int j = 0; j < 32; ++j)
+            for (int j = 0; j < 16; ++j)
               r[j] = __float_as_uint(fmaf(__uint_as_float(r1[j]), keep1, __uint_as_float(r[j])));
           }
         }
         if (live && split) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
+          for (int j = 0; j < 4; ++j)
             *reinterpret_cast<uint4 *>(a.part_o + ((static_cast<int64_t>(pslot) * (D / 4) + d / 4 + j) * 256 + prow) * 4) =
                 make_uint4(r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
         } else if (live) {
           T *out = static_cast<T *>(a.out) + orow * D + d;
+          const bool none = l == 0.f;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
+          for (int j = 0; j < 2; ++j) {
             float f[8];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) f[k] = l == 0.f ? 0.f : __uint_as_float(r[8 * j + k]) * inv;
+            for (int k = 0; k < 8; ++k) f[k] = none ? 0.f : __uint_as_float(r[8 * j + k]) * inv;
             *reinterpret_cast<uint4 *>(out + 8 * j) = pack8(f, T());
           }
         }
@@ -1166,7 +1177,7 @@ __device__ __forceinline__ void softmax(const Args &a, Ctrl &c, uint8_t *smem, u
       j.kvh = wk.kvh;
       // pieces: the CTA before this one, this one, and on to the block's end
       j.first_slot = 2 * (static_cast<int>(blockIdx.x) - 1) + (wk.t0 == c.per ? 0 : 1);
-      j.last_cta = static_cast<int>((static_cast<long long>(blockIdx.x) * c.per - wk.t0 + wk.tiles - 1) / c.per);
+      j.last_cta = (static_cast<int>(blockIdx.x) * c.per - wk.t0 + wk.tiles - 1) / c.per;
       a.joins[blockIdx.x] = j;
     }
     fence_before();
@@ -1250,6 +1261,7 @@ __global__ void __launch_bounds__((Cfg<T, D, kCache>::kThreads), 1)
 // 32 rows; lane = row, warp = an eighth of the head.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) tree_join_kernel(const __grid_constant__ Args a) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const Join j = a.joins[blockIdx.x];
   const int tile_rows = a.tile_nodes * a.group;
@@ -1258,29 +1270,46 @@ __global__ void __launch_bounds__(256) tree_join_kernel(const __grid_constant__ 
   const int node = tile * a.tile_nodes + in_tile / a.group;
   if (in_tile >= tile_rows || node >= j.nodes) return;
   const int first_cta = j.first_slot >> 1;
-  auto slot_of = [&](int cta) { return cta == first_cta ? j.first_slot : 2 * cta; };
-  float M = -CUDART_INF_F;
-  for (int x = first_cta; x <= j.last_cta; ++x)
-    M = fmaxf(M, a.part_ml[static_cast<int64_t>(slot_of(x)) * 256 + prow].x);
-  const float mm = M == -CUDART_INF_F ? 0.f : M;
-  constexpr int kPer = D / 8 / 4;
+  constexpr int kPer = D / 8 / 4, kAhead = 4;
   const int d4 = (threadIdx.x >> 5) * kPer;
-  float l = 0.f, o[4 * kPer];
+  float M = -CUDART_INF_F, l = 0.f, o[4 * kPer];
 #pragma unroll
   for (int i = 0; i < 4 * kPer; ++i) o[i] = 0.f;
-#pragma unroll 2
-  for (int x = first_cta; x <= j.last_cta; ++x) {
-    const int64_t s = slot_of(x);
-    const float2 ml = a.part_ml[s * 256 + prow];
-    const float keep = exp2f(ml.x - mm);
-    l = fmaf(ml.y, keep, l);
+  for (int x0 = first_cta; x0 <= j.last_cta; x0 += kAhead) {
+    float2 ml[kAhead];
+    float4 v[kAhead][kPer];
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const float4 v = *reinterpret_cast<const float4 *>(a.part_o + ((s * (D / 4) + d4 + i) * 256 + prow) * 4);
-      o[4 * i] = fmaf(v.x, keep, o[4 * i]);
-      o[4 * i + 1] = fmaf(v.y, keep, o[4 * i + 1]);
-      o[4 * i + 2] = fmaf(v.z, keep, o[4 * i + 2]);
-      o[4 * i + 3] = fmaf(v.w, keep, o[4 * i + 3]);
+    for (int k = 0; k < kAhead; ++k) {
+      ml[k] = make_float2(-CUDART_INF_F, 0.f);
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) v[k][i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (x0 + k > j.last_cta) continue;
+      const int64_t s = x0 + k == first_cta ? j.first_slot : 2 * (x0 + k);
+      ml[k] = a.part_ml[s * 256 + prow];
+#pragma unroll
+      for (int i = 0; i < kPer; ++i)
+        v[k][i] = *reinterpret_cast<const float4 *>(a.part_o + ((s * (D / 4) + d4 + i) * 256 + prow) * 4);
+    }
+    float top = M;
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) top = fmaxf(top, ml[k].x);
+    const float mm = top == -CUDART_INF_F ? 0.f : top;
+    const float old = exp2f(M - mm);
+    M = top;
+    l *= old;
+#pragma unroll
+    for (int i = 0; i < 4 * kPer; ++i) o[i] *= old;
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const float keep = exp2f(ml[k].x - mm);
+      l = fmaf(ml[k].y, keep, l);
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        o[4 * i] = fmaf(v[k][i].x, keep, o[4 * i]);
+        o[4 * i + 1] = fmaf(v[k][i].y, keep, o[4 * i + 1]);
+        o[4 * i + 2] = fmaf(v[k][i].z, keep, o[4 * i + 2]);
+        o[4 * i + 3] = fmaf(v[k][i].w, keep, o[4 * i + 3]);
+      }
     }
   }
   const int64_t orow = (j.rows0 + j.node0 + node) * a.hq + j.kvh * a.group + in_tile % a.group;
