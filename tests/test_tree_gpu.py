@@ -213,6 +213,16 @@ def test_repeat_graph_and_streams():
     assert torch.equal(captured, tsb.tree_attention(*case.args(), **case.kwargs()))
 
 
+@pytest.mark.parametrize("cache", [F16, I8, F8])
+def test_long_contexts_give_the_same_bits_every_time(cache):
+    # a cache that stays in L2, so that loads come back fast, and blocks of every width
+    for nodes in (3, 12, 200):
+        case = TreeCase([33000, 700], [nodes, 3], 8, 2, cache=cache, seed=6)
+        first = check(case)
+        for _ in range(10):
+            assert torch.equal(tsb.tree_attention(*case.args(), **case.kwargs()), first)
+
+
 def test_one_node_agrees_with_decode_attention():
     case = TreeCase([900, 17, 64], [1, 1, 1], 32, 8, seed=21)
     out = tsb.tree_attention(*case.args(), **case.kwargs())

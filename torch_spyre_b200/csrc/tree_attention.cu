@@ -151,10 +151,10 @@ extern "C" int b200kv_tree_attention(const void *q, int32_t q_dtype, int64_t q_s
   B200KV_CHECK_ARG(!tree_mask || mask_words * 64 >= max_nodes, "mask_words (%lld) cover fewer than max_nodes (%lld)",
                    (long long)mask_words, (long long)max_nodes);
   B200KV_CHECK_ARG(std::isfinite(scale), "scale must be finite");
-  // blocks of rows x tiles of tokens, counted in 31 bits on the device
-  if ((batch + total_q * (num_q_heads / num_kv_heads) / 64 + 1) * num_kv_heads * (max_blocks_per_seq / 2 + 1) >=
+  // the kernel counts its units of work in 31 bits
+  if ((batch + total_q * (num_q_heads / num_kv_heads) / 64 + 1) * num_kv_heads * (max_blocks_per_seq + 8) >=
       (int64_t{1} << 31))
-    return set_error(B200KV_ERR_UNSUPPORTED, "2^31 or more tiles of rows and tokens");
+    return set_error(B200KV_ERR_UNSUPPORTED, "2^31 or more steps of rows and tokens");
   if (total_q == 0) return B200KV_OK;
   B200KV_CHECK_ARG(batch > 0, "nodes without a sequence");
   B200KV_CHECK_ARG(q && k_pool && v_pool && block_table && context_lens && q_indptr && out, "null pointer argument");

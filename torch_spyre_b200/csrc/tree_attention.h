@@ -9,11 +9,11 @@ namespace tree {
 
 constexpr int kMaxCtas = 148;  // shares of a launch: one CTA per SM of a B200
 
-// A block of rows whose token tiles are spread over CTAs first_slot / 2 ..
-// last_cta; its partials are in first_slot and then in slots 2 * cta.
+// A block of rows whose token tiles are spread over CTAs first_cta .. last_cta;
+// its partials are in slot 2 * first_cta + 1 and then in slots 2 * cta.
 struct Join {
   int64_t rows0;
-  int node0, nodes, kvh, first_slot, last_cta, pad;
+  int node0, nodes, kvh, first_cta, last_cta, pad;
 };
 
 struct Args {

@@ -39,10 +39,6 @@ namespace tree {
 
 constexpr int kTileRows = 128, kTileTokens = 128;
 constexpr float kLazyLog2 = 8.f;
-#ifndef TS8
-#define TS8 4
-#define TR8 3
-#endif
 
 template <typename T, int D, int kCache>
 struct Cfg {
@@ -57,8 +53,8 @@ struct Cfg {
   static constexpr int kStickTile = kTileTokens * 128;      // one 64-element column of 128 rows
   static constexpr int kTile = kSticks * kStickTile;        // a Q, K or V tile
   static constexpr int kQ = k8 ? 1 : 2;                      // most Q tiles of a block
-  static constexpr int kSlots = k8 ? TS8 : (D == 64 ? 8 : 5);  // operand tiles in flight
-  static constexpr int kRaw = k8 ? TR8 : 0;                   // 8-bit tiles in flight
+  static constexpr int kSlots = k8 ? 4 : (D == 64 ? 8 : 5);  // operand tiles in flight
+  static constexpr int kRaw = k8 ? 3 : 0;                   // 8-bit tiles in flight
   static constexpr int kRawTile = kTileTokens * 128;
   static constexpr int kCtrl = k8 ? 19456 : 3072;
   static constexpr int kOffQ = kCtrl;
@@ -86,10 +82,11 @@ __device__ __forceinline__ uint32_t col_o(int w) { return 256u + uint32_t(w) * 1
 struct Seq {
   int ctx, nodes, q0, blocks, qtiles;
 };
-// Where a CTA's share of the line begins: a block's token tile.
+// Where a CTA's share of the line begins: in block `block`, whose units begin at
+// unit u0 of the line.
 struct Start {
   Seq s;
-  int b, kvh, block, tiles, tile;
+  int b, kvh, block, u0;
 };
 
 struct Ctrl {
@@ -98,7 +95,7 @@ struct Ctrl {
   uint64_t q_full, q_empty;
   uint64_t s_full[2], p_ready[2], o_full[2];
   uint32_t tmem;
-  int per, total;  // tiles of a share, of the line
+  int per, total;  // units of a share, of the line
   Start start;
   int scan[32];
   unsigned bad_piece;       // last piece (counted from 1) that met a non-finite value in a node's V row
@@ -243,11 +240,28 @@ __device__ __forceinline__ int block_tiles(const Args &a, const Seq &s, int k) {
   const int nodes = a.mask ? s.nodes : min(s.nodes, (k + 1) * kQ * a.tile_nodes);
   return (s.ctx + nodes + kTileTokens - 1) / kTileTokens;
 }
+// The line is cut by cost, in units of a one-Q-tile step over a token tile: a
+// step of two Q tiles counts as two (2.6 us against 1.25 measured), and a block
+// begins with kBlockUnits for what every piece costs besides its steps (Q, the
+// first products, the epilogue: about 5 us).  16 ragged sequences of 1 to 64
+// nodes: 90 us cut by steps alone, 77, 75 and 73 us with 3, 4 and 5 units; 16
+// sequences of 100 to 300 tokens: 47 us, and 36, 40 and 40.
+constexpr int kBlockUnits = 4;
+template <int kQ>
+__device__ __forceinline__ int step_units(const Seq &s, int k) {
+  return kQ == 2 && 2 * k + 1 < s.qtiles ? 2 : 1;
+}
+template <int kQ>
+__device__ __forceinline__ int block_units(const Args &a, const Seq &s, int k) {
+  return kBlockUnits + step_units<kQ>(s, k) * block_tiles<kQ>(a, s, k);
+}
 template <int kQ>
 __device__ __forceinline__ int head_units(const Args &a, const Seq &s) {
-  if (a.mask) return s.blocks * (s.blocks ? block_tiles<kQ>(a, s, 0) : 0);
+  if (s.blocks == 0) return 0;
+  // with a mask all blocks have as many tiles, and only the last may be of one Q tile
+  if (a.mask) return (s.blocks - 1) * block_units<kQ>(a, s, 0) + block_units<kQ>(a, s, s.blocks - 1);
   int n = 0;
-  for (int k = 0; k < s.blocks; ++k) n += block_tiles<kQ>(a, s, k);
+  for (int k = 0; k < s.blocks; ++k) n += block_units<kQ>(a, s, k);
   return n;
 }
 
@@ -274,25 +288,35 @@ __device__ __forceinline__ Copies copies_of(const Args &a, const Seq &s, int blo
 template <int kQ>
 struct Walk {
   Seq s;
-  int b, kvh, block, tiles, t0, t1;  // piece: token tiles [t0, t1) of `tiles`
-  int next_tile, left;
+  int b, kvh, block, u0, tiles, t0, t1;  // piece: token tiles [t0, t1) of `tiles`
+  int end;                               // of the share
 
   __device__ __forceinline__ void init(const Args &a, const Ctrl &c) {
-    left = min(c.per, c.total - static_cast<int>(blockIdx.x) * c.per);
     const Start &f = c.start;
-    s = f.s, b = f.b, kvh = f.kvh, block = f.block, tiles = f.tiles, next_tile = f.tile;
+    s = f.s, b = f.b, kvh = f.kvh, block = f.block, u0 = f.u0;
+    t1 = 0;
+    end = min(c.total, (static_cast<int>(blockIdx.x) + 1) * c.per);
+  }
+  // Tile t belongs to the share that holds its first unit.
+  __device__ __forceinline__ int tile_from(int unit) const {
+    const int w = step_units<kQ>(s, block), x = unit - u0 - kBlockUnits;
+    return x <= 0 ? 0 : min(tiles, (x + w - 1) / w);
   }
   // The next piece, false when the share is done.
-  __device__ __forceinline__ bool next(const Args &a) {
-    if (left <= 0) return false;
-    t0 = next_tile;
-    t1 = min(tiles, t0 + left);
-    left -= t1 - t0;
-    return true;
+  __device__ __forceinline__ bool next(const Args &a, const Ctrl &c) {
+    const int first = static_cast<int>(blockIdx.x) * c.per;
+    for (;;) {
+      if (u0 >= end || first >= c.total) return false;
+      tiles = block_tiles<kQ>(a, s, block);
+      t0 = tile_from(first);
+      t1 = tile_from(end);
+      if (t0 < t1) return true;
+      advance(a);
+    }
   }
   __device__ __forceinline__ void advance(const Args &a) {
-    next_tile = 0;
-    if (left <= 0) return;
+    u0 += block_units<kQ>(a, s, block);
+    if (u0 >= end) return;
     if (++block >= s.blocks) {
       block = 0;
       if (++kvh >= a.hkv) {
@@ -301,9 +325,12 @@ struct Walk {
         while (s.nodes == 0);
       }
     }
-    tiles = block_tiles<kQ>(a, s, block);
   }
   __device__ __forceinline__ bool two() const { return kQ == 2 && 2 * block + 1 < s.qtiles; }
+  // The share that holds the first unit of tile t.
+  __device__ __forceinline__ int share_of(int t, int per) const {
+    return (u0 + kBlockUnits + t * step_units<kQ>(s, block)) / per;
+  }
 };
 
 // The line's length, a share's, and where this CTA's begins; all threads of the
@@ -333,7 +360,8 @@ __device__ __forceinline__ void make_plan(const Args &a, Ctrl &c) {
     if (w < warp) before += c.scan[w];
     total += c.scan[w];
   }
-  const int per = static_cast<int>((static_cast<unsigned>(total) + gridDim.x - 1) / gridDim.x);
+  // (at least 2, so that a share inside a block holds the start of a tile)
+  const int per = max(2, static_cast<int>((static_cast<unsigned>(total) + gridDim.x - 1) / gridDim.x));
   const int first = static_cast<int>(blockIdx.x) * per;
   int at = before + incl - mine;
   if (first >= at && first < at + mine) {
@@ -344,17 +372,17 @@ __device__ __forceinline__ void make_plan(const Args &a, Ctrl &c) {
       if (first < at + hu * a.hkv) break;
       at += hu * a.hkv;
     }
-    int rem = first - at, block = 0, tiles;
-    const int kvh = rem / hu;
-    rem -= kvh * hu;
+    const int kvh = (first - at) / hu;
+    at += kvh * hu;
+    int block = 0;
     if (a.mask) {
-      tiles = block_tiles<kQ>(a, s, 0);
-      block = rem / tiles;
-      rem -= block * tiles;
+      const int n = block_units<kQ>(a, s, 0);
+      block = min((first - at) / n, s.blocks - 1);
+      at += block * n;
     } else {
-      while (rem >= (tiles = block_tiles<kQ>(a, s, block))) rem -= tiles, ++block;
+      for (int n; first >= at + (n = block_units<kQ>(a, s, block)); ++block) at += n;
     }
-    c.start = Start{s, b, kvh, block, tiles, rem};
+    c.start = Start{s, b, kvh, block, at};
   }
   if (tid == 0) {
     c.per = per;
@@ -393,7 +421,7 @@ __device__ __forceinline__ void producer(const Args &a, Ctrl &c, uint8_t *smem, 
   uint32_t slot = 0, ring = 0, pieces = 0;  // tiles issued (16-bit, 8-bit), pieces begun
   Walk<C::kQ> w;
   w.init(a, c);
-  while (w.next(a)) {
+  while (w.next(a, c)) {
     const bool two = w.two();
     const int pages = (w.s.ctx + w.s.nodes + kPageTokens - 1) / kPageTokens;
     int window = w.t0 / 16, ids = load_ids(a, w.b, window, pages), ids_next = load_ids(a, w.b, window + 1, pages);
@@ -563,8 +591,6 @@ __device__ __forceinline__ void converter(const Args &a, Ctrl &c, uint8_t *smem,
 #pragma unroll
     for (int k = 0; k < 4; ++k)
       x[k] = row0 + 32 * k < rows ? *reinterpret_cast<const uint4 *>(src + k * 4096) : make_uint4(0, 0, 0, 0);
-    __syncwarp();
-    if (lane == 0) arrive(&c.raw_empty[r]);
     ++ring;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -579,12 +605,16 @@ __device__ __forceinline__ void converter(const Args &a, Ctrl &c, uint8_t *smem,
     }
     fence_async_smem();
     __syncwarp();
+    // The raw tile is released here and not right after its loads: an arrival
+    // can overtake shared-memory loads whose values nothing has used yet, and
+    // the next bulk copy then overwrites what they were to read.
+    if (lane == 0) arrive(&c.raw_empty[r]);
     if (lane == 0) arrive(&c.full[s]);
     ++slot;
   };
   Walk<C::kQ> w;
   w.init(a, c);
-  while (w.next(a)) {
+  while (w.next(a, c)) {
     ++piece;
     const int len = w.s.ctx + w.s.nodes;
     const int lead = w.two() ? 1 : 2;
@@ -632,7 +662,7 @@ __device__ __forceinline__ void mma_issuer(const Args &a, Ctrl &c, uint8_t *smem
   };
   Walk<C::kQ> w;
   w.init(a, c);
-  while (w.next(a)) {
+  while (w.next(a, c)) {
     wait(&c.q_full, pieces++ & 1u, dead, a.error_flag);
     fence_after();
     const int n = w.t1 - w.t0;
@@ -945,7 +975,7 @@ __device__ __forceinline__ void softmax(const Args &a, Ctrl &c, uint8_t *smem, u
   unsigned piece = 0;
   Walk<C::kQ> wk;
   wk.init(a, c);
-  while (wk.next(a)) {
+  while (wk.next(a, c)) {
     ++piece;
     const bool two = wk.two();
     const int n = wk.t1 - wk.t0, lead = two ? 1 : 2;
@@ -1042,7 +1072,7 @@ __device__ __forceinline__ void softmax(const Args &a, Ctrl &c, uint8_t *smem, u
 
     // -------------------------------------------------------- end of piece --
     const bool split = wk.t0 > 0 || wk.t1 < wk.tiles;
-    const int pslot = 2 * blockIdx.x + (wk.t0 > 0 || wk.left + n == c.per ? 0 : 1);
+    const int pslot = 2 * blockIdx.x + (wk.t0 > 0 ? 0 : 1);  // one of each kind per share
     auto o_wait = [&](int k) {
       wait(&c.o_full[k], o_uses[k]++ & 1u, dead, a.error_flag);
       fence_after();
@@ -1168,17 +1198,19 @@ __device__ __forceinline__ void softmax(const Args &a, Ctrl &c, uint8_t *smem, u
       else if (a.lse)
         a.lse[orow] = l == 0.f ? -CUDART_INF_F : (m + log2f(l)) * 0.69314718055994530942f;
     }
-    // the first CTA boundary inside a split block describes it to the join
-    if (split && wk.t0 > 0 && w == 0 && tid == 0 && wk.t0 <= c.per) {
-      Join j;
-      j.rows0 = static_cast<int64_t>(wk.s.q0);
-      j.node0 = C::kQ * wk.block * a.tile_nodes;
-      j.nodes = min(wk.s.nodes - j.node0, C::kQ * a.tile_nodes);
-      j.kvh = wk.kvh;
-      // pieces: the CTA before this one, this one, and on to the block's end
-      j.first_slot = 2 * (static_cast<int>(blockIdx.x) - 1) + (wk.t0 == c.per ? 0 : 1);
-      j.last_cta = (static_cast<int>(blockIdx.x) * c.per - wk.t0 + wk.tiles - 1) / c.per;
-      a.joins[blockIdx.x] = j;
+    // the second share of a split block describes it to the join
+    if (wk.t0 > 0 && w == 0 && tid == 0) {
+      const int first = wk.share_of(0, c.per);
+      if (static_cast<int>(blockIdx.x) == first + 1) {
+        Join j;
+        j.rows0 = wk.s.q0;
+        j.node0 = C::kQ * wk.block * a.tile_nodes;
+        j.nodes = min(wk.s.nodes - j.node0, C::kQ * a.tile_nodes);
+        j.kvh = wk.kvh;
+        j.first_cta = first;
+        j.last_cta = wk.share_of(wk.tiles - 1, c.per);
+        a.joins[blockIdx.x] = j;
+      }
     }
     fence_before();
     if (!two) bar_pair();  // both have read O and ml before either goes on
@@ -1269,13 +1301,12 @@ __global__ void __launch_bounds__(256) tree_join_kernel(const __grid_constant__ 
   const int in_tile = prow & (kTileRows - 1), tile = prow / kTileRows;
   const int node = tile * a.tile_nodes + in_tile / a.group;
   if (in_tile >= tile_rows || node >= j.nodes) return;
-  const int first_cta = j.first_slot >> 1;
   constexpr int kPer = D / 8 / 4, kAhead = 4;
   const int d4 = (threadIdx.x >> 5) * kPer;
   float M = -CUDART_INF_F, l = 0.f, o[4 * kPer];
 #pragma unroll
   for (int i = 0; i < 4 * kPer; ++i) o[i] = 0.f;
-  for (int x0 = first_cta; x0 <= j.last_cta; x0 += kAhead) {
+  for (int x0 = j.first_cta; x0 <= j.last_cta; x0 += kAhead) {
     float2 ml[kAhead];
     float4 v[kAhead][kPer];
 #pragma unroll
@@ -1284,7 +1315,7 @@ __global__ void __launch_bounds__(256) tree_join_kernel(const __grid_constant__ 
 #pragma unroll
       for (int i = 0; i < kPer; ++i) v[k][i] = make_float4(0.f, 0.f, 0.f, 0.f);
       if (x0 + k > j.last_cta) continue;
-      const int64_t s = x0 + k == first_cta ? j.first_slot : 2 * (x0 + k);
+      const int64_t s = 2 * (x0 + k) + (x0 + k == j.first_cta ? 1 : 0);
       ml[k] = a.part_ml[s * 256 + prow];
 #pragma unroll
       for (int i = 0; i < kPer; ++i)
