@@ -505,6 +505,14 @@ __device__ __forceinline__ void producer(const Args &a, Ctrl &c, uint8_t *smem, 
 // a tile only.  So the nodes' V rows are looked through in shared memory:
 // non-finite elements become zeros there, and when the block ends the rows that
 // see such a node get its elements added from the cache (repair_row).
+// (An exponent of all ones, and no other, carries into the sign bit when its
+// lowest bit is added.)
+template <typename T>
+__device__ __forceinline__ bool any_non_finite(uint4 v) {
+  constexpr uint32_t e = std::is_same<T, __half>::value ? 0x7c007c00u : 0x7f807f80u;
+  constexpr uint32_t one = std::is_same<T, __half>::value ? 0x04000400u : 0x00800080u;
+  return ((((v.x & e) + one) | ((v.y & e) + one) | ((v.z & e) + one) | ((v.w & e) + one)) & 0x80008000u) != 0;
+}
 template <typename T>
 __device__ __forceinline__ uint32_t drop_non_finite(uint32_t w) {
   constexpr uint32_t e = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
@@ -987,6 +995,8 @@ __device__ __forceinline__ void softmax(const Args &a, Ctrl &c, uint8_t *smem, u
     const int node = qt * a.tile_nodes + row / a.group;
     const bool live = row < a.tile_nodes * a.group && node < wk.s.nodes;
     const bool warp_live = __any_sync(0xffffffffu, live);
+    // tokens before this one are seen by every row of the Q tile
+    const int common = wk.s.ctx + (a.mask ? 0 : qt * a.tile_nodes + 1);
     float m = -CUDART_INF_F, l = 0.f;
     // 8-bit caches: the scales of this stream's next tile, four tokens per lane
     auto scales_of = [&](int t, float4 &k, float4 &v) {
@@ -1005,7 +1015,7 @@ __device__ __forceinline__ void softmax(const Args &a, Ctrl &c, uint8_t *smem, u
     if (C::k8 && warp_live && tfirst < wk.t1) scales_of(tfirst, ks, vs);
     for (int t = tfirst; t < wk.t1; t += step) {
       const int pos = t * kTileTokens;
-      const bool tail = pos + kTileTokens > wk.s.ctx + (a.mask ? 0 : 1);
+      const bool tail = pos + kTileTokens > common;
       uint32_t vis[4] = {~0u, ~0u, ~0u, ~0u};
       if (tail && live) {
 #pragma unroll
@@ -1040,26 +1050,31 @@ __device__ __forceinline__ void softmax(const Args &a, Ctrl &c, uint8_t *smem, u
             weigh<typename C::P, D, false>(ts, to, vis, cl, first, live, m, l);
         }
       }
-      if (!C::k8 && pos + kTileTokens > wk.s.ctx) {
+      if (!C::k8 && pos + kTileTokens > min(common, len)) {
         // the pool's rows past the sequence's end hold anything and become
         // zeros, so that weights of zero meet finite values; so do non-finite
-        // elements of nodes
+        // elements of nodes that not every row sees
         const int i = t - wk.t0;
         const uint32_t vslot = slot + i + min(n, i + lead);
         wait(&c.full[vslot % C::kSlots], (vslot / C::kSlots) & 1u, dead, a.error_flag);
-        uint8_t *v = smem + C::kOffSlots + (vslot % C::kSlots) * C::kTile;
-        const int node0 = max(wk.s.ctx - pos, 0), end = len - pos;
-        for (int k = node0 * 8 + tid; k < kTileTokens * 8; k += 128) {
-          for (int st = 0; st < C::kSticks; ++st) {
-            uint4 *at = reinterpret_cast<uint4 *>(v + st * C::kStickTile + k * 16);
-            uint4 x = make_uint4(0, 0, 0, 0);
-            if (k < end * 8) {
-              x = *at;
-              if (!drop_non_finite<typename C::P>(x)) continue;
+        uint8_t *v = smem + C::kOffSlots + (vslot % C::kSlots) * C::kTile + tid * 16;
+        // 16 bytes per thread: row = 16 k + tid / 8
+        const int from = max(common - pos, 0), end = len - pos;
+        for (int st = 0; st < C::kSticks; ++st) {
+#pragma unroll 1
+          for (int k = from / 16; k < 8; ++k) {
+            uint4 *at = reinterpret_cast<uint4 *>(v + st * C::kStickTile + k * 2048);
+            const int vrow = 16 * k + (tid >> 3);
+            if (vrow >= end) {
+              *at = make_uint4(0, 0, 0, 0);
+            } else if (vrow >= from) {
+              uint4 x = *at;
+              if (!any_non_finite<T>(x)) continue;
               atomicMax(&c.bad_piece, piece);  // before the element goes: the other stream looks too
               __threadfence_block();
+              drop_non_finite<T>(x);
+              *at = x;
             }
-            *at = x;
           }
         }
         fence_async_smem();
