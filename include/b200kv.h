@@ -589,8 +589,9 @@ B200KV_API int b200kv_oproj_allreduce_f16(const void *attn, int64_t attn_stride_
  *
  * Pools: 16-bit (fp16 or bf16) [num_blocks, Hkv, D/64, 64, 64] for D = 64 or
  * 128, or 8-bit (int8 or e4m3) [num_blocks, Hkv, 1, 64, 128] for D = 128 with
- * one fp32 scale per row, [num_blocks, Hkv, 64]: element d of token row t
- * stands for value(d) * scale(t).
+ * one fp32 scale per row, [num_blocks, Hkv, 64], not negative: element d of
+ * token row t stands for value(d) * scale(t).  Pools, scales and contiguous
+ * outputs are 16-byte aligned.
  * ------------------------------------------------------------------------ */
 
 /* Rotary positions.  Row (t, h) of x starts at x[t * x_stride_t + h *
@@ -612,8 +613,8 @@ B200KV_API int b200kv_rotary(const void *x, int32_t dtype, int64_t x_stride_t, i
 
 /* Writes K/V rows to their slots, in one launch.  Row n, head h of k starts at
  * k[n * k_stride_n + h * k_stride_h] (v, q likewise; row_dtype fp16 or bf16;
- * 16-byte aligned, strides multiples of 8).  With a table (as above; half
- * layout: rotary_dim a multiple of 16) k is turned by positions[n] first, and
+ * 16-byte aligned, strides multiples of 8).  With a table (as above, 16-byte
+ * aligned; half layout: rotary_dim a multiple of 16) k is turned by positions[n] first, and
  * so is q into q_out (contiguous [N, Hq, D]; num_q_heads 0: no q).  A 16-bit
  * pool has the rows' dtype and takes them rounded once.  An 8-bit pool takes
  *   s = max|x| / qmax (127 or 448),  round_to_nearest(clamp(x * (1 / s)))
@@ -667,7 +668,9 @@ B200KV_API int64_t b200kv_tree_workspace_bytes(int64_t total_q, int64_t batch, i
  * A node that sees nothing gives a zero row and lse = -inf.  Lengths outside
  * the block table or max_nodes are clamped and set B200KV_DEVERR_BAD_LEN, block
  * ids outside the pool read as zeros and set B200KV_DEVERR_BAD_BLOCK.
- * Supported: Hq / Hkv <= 128, batch <= 1024, D = 128 (64 in 16-bit pools). */
+ * Supported: Hq / Hkv <= 128, batch <= 1024, D = 128 (64 in 16-bit pools),
+ * total_q * Hq < 2^31, max_blocks_per_seq < 2^24 and
+ * (batch + total_q * (Hq / Hkv) / 64 + 1) * Hkv * (max_blocks_per_seq + 8) < 2^31. */
 B200KV_API int b200kv_tree_attention(const void *q, int32_t q_dtype, int64_t q_stride_t,
                                      int64_t q_stride_h, const void *k_pool, const void *v_pool,
                                      int32_t pool_dtype, const float *k_scales,

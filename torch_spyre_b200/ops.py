@@ -43,6 +43,7 @@ DECODE_INPUTS_READY = 1  # B200KV_DECODE_INPUTS_READY
 
 # ---------------------------------------------------------------- helpers ---
 _workspaces: dict[tuple[int, int], torch.Tensor] = {}
+_outgrown: list[torch.Tensor] = []
 
 
 def _stream_ptr(device: torch.device) -> int:
@@ -66,12 +67,16 @@ def workspace_for(device: torch.device, nbytes: int) -> torch.Tensor:
     """Zero-initialised decode workspace cached per (device, stream).
 
     The decode kernel leaves its completion counters at zero after every call,
-    so one buffer serves every call ordered on the same stream.
+    so one buffer serves every call ordered on the same stream.  A buffer that
+    became too small is kept: a captured graph may still write to it.  (Sizes are
+    powers of two, so those kept are together smaller than the one in use.)
     """
     key = (device.index if device.index is not None else torch.cuda.current_device(), _stream_ptr(device))
     ws = _workspaces.get(key)
     if ws is None or ws.numel() < nbytes:
-        ws = torch.zeros(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
+        if ws is not None:
+            _outgrown.append(ws)
+        ws = torch.zeros(1 << max(nbytes - 1, (1 << 20) - 1).bit_length(), dtype=torch.uint8, device=device)
         _workspaces[key] = ws
     return ws
 
