@@ -367,77 +367,88 @@ struct CommitArgs {
   int32_t *error_flag;
 };
 
-constexpr int kCommitThreads = 256, kCommitBatch = 8;
+constexpr int kCommitThreads = 128, kCommitRows = 64;
 
-// One CTA per (KV head, K or V, sequence).  A row is kRow bytes, one 16-byte
-// vector per thread, kCommitBatch rows per thread and batch.  A batch is read
+// One CTA per sequence and KV head, K and V one after the other.  The path is
+// taken 64 rows at a time: thread i finds where row i comes from and goes to, and
+// moves its scale; then the rows move, 16 bytes per thread.  A batch is read
 // whole before any of it is written; the path ascends, so path[i] >= i and a
 // later batch never reads what an earlier one wrote.
+//
+// Bound: bytes, each moved row read and written once; few rows: the chain length
+// -> path -> block table -> row.  128 sequences, 8 KV heads, 32 rows each on
+// average (33.6 MB): 6.2 us, 0.84 of the copy rate.  A CTA for K and one for V
+// (every one walks that chain): 9.7 us; four heads' CTAs in one: 6.1 us, but
+// 6.0 in place of 4.2 us for 4 sequences.
 template <int kRow, int kStickRow, bool kScaled>  // bytes of a row, of a row inside one stick (128)
 __global__ void __launch_bounds__(kCommitThreads) tree_commit_kernel(const CommitArgs a) {
-  constexpr int kLanes = kRow / 16;
-  constexpr int kPerPass = kCommitThreads / kLanes;
-  const int h = blockIdx.x >> 1, kv = blockIdx.x & 1, b = blockIdx.y;
-  const int lane = threadIdx.x % kLanes, row = threadIdx.x / kLanes;
+  constexpr int kLanes = kRow / 16, kGroups = kCommitThreads / kLanes, kEach = kCommitRows / kGroups;
+  constexpr int64_t kPage = 64 * kRow;
+  __shared__ int64_t from[kCommitRows], to[kCommitRows];  // byte offsets of KV head 0's rows, to: -1 = stays
+  const int tid = threadIdx.x, h = blockIdx.x, b = blockIdx.y;
   const int cap = a.max_blocks * kPageTokens;
   const int ctx = __ldg(a.ctx + b);
   const int n_in = __ldg(a.path_lens + b);
   const bool bad = ctx < 0 || ctx > cap || n_in < 0 || n_in > a.max_path || ctx + n_in > cap;
   const int n = bad ? 0 : n_in;
-  if (blockIdx.x == 0 && threadIdx.x == 0) {
+  if (h == 0 && tid == 0) {
     if (bad && a.error_flag) atomicOr(a.error_flag, B200KV_DEVERR_BAD_LEN);
     a.new_lens[b] = bad ? ctx : ctx + n;
   }
   const int32_t *path = a.path + b * a.path_stride;
   const int32_t *table = a.block_table + b * a.bt_stride;
-  uint8_t *pool = static_cast<uint8_t *>(a.pool[kv]);
-  // byte offset of this thread's vector of token `tok`, -1 (flagged) outside
-  auto offset = [&](int tok, int64_t *scale_at) -> int64_t {
-    if (tok < 0 || tok >= cap) {
-      if (a.error_flag && lane == 0) atomicOr(a.error_flag, B200KV_DEVERR_BAD_SLOT);
+  auto offset = [&](int tok, bool inside) -> int64_t {  // -1 (flagged) outside
+    if (!inside) {
+      if (a.error_flag) atomicOr(a.error_flag, B200KV_DEVERR_BAD_SLOT);
       return -1;
     }
     const int blk = __ldg(table + (tok >> 6));
     if (blk < 0 || blk >= a.num_blocks) {
-      if (a.error_flag && lane == 0) atomicOr(a.error_flag, B200KV_DEVERR_BAD_BLOCK);
+      if (a.error_flag) atomicOr(a.error_flag, B200KV_DEVERR_BAD_BLOCK);
       return -1;
     }
-    const int64_t page = int64_t(blk) * a.hkv + h;
-    *scale_at = page * 64 + (tok & 63);
-    const int byte = lane * 16;
-    return (page * (kRow / kStickRow) + byte / kStickRow) * (64 * kStickRow) + int64_t(tok & 63) * kStickRow +
-           byte % kStickRow;
+    return int64_t(blk) * a.hkv * kPage + (tok & 63) * kStickRow;
   };
-  for (int base = 0; base < n; base += kPerPass * kCommitBatch) {
-    uint4 v[kCommitBatch];
-    float s[kCommitBatch];
-    int64_t dst[kCommitBatch], dst_s[kCommitBatch];
-#pragma unroll
-    for (int u = 0; u < kCommitBatch; ++u) {
-      const int i = base + u * kPerPass + row;
-      dst[u] = -1;
-      if (i >= n) continue;
-      const int p = __ldg(path + i);
-      const int before = i > 0 ? __ldg(path + i - 1) : -1;
-      if (p <= before) {  // not ascending: the row stays where it is
-        if (a.error_flag && lane == 0) atomicOr(a.error_flag, B200KV_DEVERR_BAD_SLOT);
-        continue;
+  const int byte = (tid % kLanes) * 16, group = tid / kLanes;
+  const int64_t part = h * kPage + byte / kStickRow * (64 * kStickRow) + byte % kStickRow;
+  auto scale_at = [&](int64_t off) { return off / kPage * 64 + off % kPage / kStickRow + h * 64; };
+  for (int base = 0; base < n; base += kCommitRows) {
+    int64_t src = -1, dst = -1;
+    if (tid < kCommitRows) {
+      const int i = base + tid;
+      if (i < n) {
+        const int p = __ldg(path + i), before = i > 0 ? __ldg(path + i - 1) : -1;
+        if (p <= before) {  // not ascending: the row stays where it is
+          if (a.error_flag) atomicOr(a.error_flag, B200KV_DEVERR_BAD_SLOT);
+        } else if (p != i) {
+          src = offset(ctx + p, p < cap - ctx);
+          dst = offset(ctx + i, true);
+          if (src < 0) dst = -1;
+        }
       }
-      if (p == i) continue;  // in place
-      int64_t src_s = 0;
-      const int64_t src = p < cap - ctx ? offset(ctx + p, &src_s) : offset(cap, &src_s);
-      const int64_t to = offset(ctx + i, &dst_s[u]);
-      if (src < 0 || to < 0) continue;
-      dst[u] = to;
-      v[u] = *reinterpret_cast<const uint4 *>(pool + src);
-      if (kScaled && lane == 0) s[u] = a.scales[kv][src_s];
+      from[tid] = src;
+      to[tid] = dst;
     }
     __syncthreads();
 #pragma unroll
-    for (int u = 0; u < kCommitBatch; ++u) {
-      if (dst[u] < 0) continue;
-      *reinterpret_cast<uint4 *>(pool + dst[u]) = v[u];
-      if (kScaled && lane == 0) a.scales[kv][dst_s[u]] = s[u];
+    for (int kv = 0; kv < 2; ++kv) {
+      uint8_t *pool = static_cast<uint8_t *>(a.pool[kv]) + part;
+      uint4 v[kEach];
+      int64_t at[kEach];
+#pragma unroll
+      for (int u = 0; u < kEach; ++u) {
+        const int r = u * kGroups + group;
+        at[u] = to[r];
+        if (at[u] >= 0) v[u] = *reinterpret_cast<const uint4 *>(pool + from[r]);
+      }
+      float s = 0.f;
+      const bool scaled = kScaled && dst >= 0;
+      if (scaled) s = a.scales[kv][scale_at(src)];
+      __syncthreads();
+#pragma unroll
+      for (int u = 0; u < kEach; ++u)
+        if (at[u] >= 0) *reinterpret_cast<uint4 *>(pool + at[u]) = v[u];
+      if (scaled) a.scales[kv][scale_at(dst)] = s;
     }
     __syncthreads();
   }
@@ -587,7 +598,7 @@ extern "C" int b200kv_tree_commit(void *k_pool, void *v_pool, int32_t pool_dtype
   a.max_path = static_cast<int>(max_path);
   a.num_blocks = num_blocks;
   a.error_flag = error_flag;
-  const dim3 grid(static_cast<unsigned>(2 * num_kv_heads), static_cast<unsigned>(batch));
+  const dim3 grid(static_cast<unsigned>(num_kv_heads), static_cast<unsigned>(batch));
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (k8)
     tree_commit_kernel<128, 128, true><<<grid, kCommitThreads, 0, s>>>(a);
