@@ -670,7 +670,7 @@ B200KV_API int64_t b200kv_tree_workspace_bytes(int64_t total_q, int64_t batch, i
  * ids outside the pool read as zeros and set B200KV_DEVERR_BAD_BLOCK.
  * Supported: Hq / Hkv <= 128, batch <= 1024, D = 128 (64 in 16-bit pools),
  * total_q * Hq < 2^31, max_blocks_per_seq < 2^24 and
- * (batch + total_q * (Hq / Hkv) / 64 + 1) * Hkv * (max_blocks_per_seq + 8) < 2^31. */
+ * (batch + total_q * (Hq / Hkv) / 64 + 1) * Hkv * (2 * max_blocks_per_seq + 17) < 2^31. */
 B200KV_API int b200kv_tree_attention(const void *q, int32_t q_dtype, int64_t q_stride_t,
                                      int64_t q_stride_h, const void *k_pool, const void *v_pool,
                                      int32_t pool_dtype, const float *k_scales,

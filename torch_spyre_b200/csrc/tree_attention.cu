@@ -152,7 +152,8 @@ extern "C" int b200kv_tree_attention(const void *q, int32_t q_dtype, int64_t q_s
                    (long long)mask_words, (long long)max_nodes);
   B200KV_CHECK_ARG(std::isfinite(scale), "scale must be finite");
   // the kernel counts its units of work in 31 bits
-  if ((batch + total_q * (num_q_heads / num_kv_heads) / 64 + 1) * num_kv_heads * (max_blocks_per_seq + 8) >=
+  // (a block of one Q tile holds at least 65 of total_q * group rows, and 9 + 2 a tile units; of two 130, and 13 + 4)
+  if ((batch + total_q * (num_q_heads / num_kv_heads) / 64 + 1) * num_kv_heads * (2 * max_blocks_per_seq + 17) >=
       (int64_t{1} << 31))
     return set_error(B200KV_ERR_UNSUPPORTED, "2^31 or more steps of rows and tokens");
   if (total_q == 0) return B200KV_OK;

@@ -240,20 +240,26 @@ __device__ __forceinline__ int block_tiles(const Args &a, const Seq &s, int k) {
   const int nodes = a.mask ? s.nodes : min(s.nodes, (k + 1) * kQ * a.tile_nodes);
   return (s.ctx + nodes + kTileTokens - 1) / kTileTokens;
 }
-// The line is cut by cost, in units of a one-Q-tile step over a token tile: a
-// step of two Q tiles counts as two (2.6 us against 1.25 measured), and a block
-// begins with kBlockUnits for what every piece costs besides its steps (Q, the
-// first products, the epilogue: about 5 us).  16 ragged sequences of 1 to 64
-// nodes: 90 us cut by steps alone, 77, 75 and 73 us with 3, 4 and 5 units; 16
-// sequences of 100 to 300 tokens: 47 us, and 36, 40 and 40.
-constexpr int kBlockUnits = 4;
+// The line is cut by cost, in units of half a microsecond: a step over a token
+// tile takes 1.1 us with one Q tile and 2.05 with two, and a block begins with
+// what every piece costs besides its steps (Q, the first products, the epilogue),
+// 5 and 7 us (least squares over the CTAs' times of eight batches of 1 to 16
+// sequences; they are within 1 to 2 us of it).
+template <int kQ>
+__device__ __forceinline__ bool two_tiles(const Seq &s, int k) {
+  return kQ == 2 && 2 * k + 1 < s.qtiles;
+}
 template <int kQ>
 __device__ __forceinline__ int step_units(const Seq &s, int k) {
-  return kQ == 2 && 2 * k + 1 < s.qtiles ? 2 : 1;
+  return two_tiles<kQ>(s, k) ? 4 : 2;
+}
+template <int kQ>
+__device__ __forceinline__ int begin_units(const Seq &s, int k) {
+  return two_tiles<kQ>(s, k) ? 13 : 9;
 }
 template <int kQ>
 __device__ __forceinline__ int block_units(const Args &a, const Seq &s, int k) {
-  return kBlockUnits + step_units<kQ>(s, k) * block_tiles<kQ>(a, s, k);
+  return begin_units<kQ>(s, k) + step_units<kQ>(s, k) * block_tiles<kQ>(a, s, k);
 }
 template <int kQ>
 __device__ __forceinline__ int head_units(const Args &a, const Seq &s) {
@@ -299,7 +305,7 @@ struct Walk {
   }
   // Tile t belongs to the share that holds its first unit.
   __device__ __forceinline__ int tile_from(int unit) const {
-    const int w = step_units<kQ>(s, block), x = unit - u0 - kBlockUnits;
+    const int w = step_units<kQ>(s, block), x = unit - u0 - begin_units<kQ>(s, block);
     return x <= 0 ? 0 : min(tiles, (x + w - 1) / w);
   }
   // The next piece, false when the share is done.
@@ -326,10 +332,10 @@ struct Walk {
       }
     }
   }
-  __device__ __forceinline__ bool two() const { return kQ == 2 && 2 * block + 1 < s.qtiles; }
+  __device__ __forceinline__ bool two() const { return two_tiles<kQ>(s, block); }
   // The share that holds the first unit of tile t.
   __device__ __forceinline__ int share_of(int t, int per) const {
-    return (u0 + kBlockUnits + t * step_units<kQ>(s, block)) / per;
+    return (u0 + begin_units<kQ>(s, block) + t * step_units<kQ>(s, block)) / per;
   }
 };
 
@@ -360,8 +366,8 @@ __device__ __forceinline__ void make_plan(const Args &a, Ctrl &c) {
     if (w < warp) before += c.scan[w];
     total += c.scan[w];
   }
-  // (at least 2, so that a share inside a block holds the start of a tile)
-  const int per = max(2, static_cast<int>((static_cast<unsigned>(total) + gridDim.x - 1) / gridDim.x));
+  // (at least a step, so that a share inside a block holds the start of a tile)
+  const int per = max(4, static_cast<int>((static_cast<unsigned>(total) + gridDim.x - 1) / gridDim.x));
   const int first = static_cast<int>(blockIdx.x) * per;
   int at = before + incl - mine;
   if (first >= at && first < at + mine) {
