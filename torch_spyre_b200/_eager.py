@@ -10,9 +10,10 @@ the verification operators take one of two shorter ways:
   operator wants it;
 * then the Python implementation runs directly (it raises for what is wrong).
 
-Under torch.compile, fake tensors, dispatch modes, functorch transforms and for
-inputs that require a gradient they go through the registered operator, whose
-kernel is the same Python implementation.
+Under torch.compile, fake tensors, dispatch modes, functorch transforms, forward
+derivatives and for inputs that require a gradient they go through the registered
+operator, whose kernel is the same Python implementation (rotary has its gradient
+in the shorter ways too).
 """
 
 from __future__ import annotations
@@ -22,6 +23,7 @@ import importlib.util
 from pathlib import Path
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -63,7 +65,7 @@ def plain(t: torch.Tensor) -> bool:
 
 def direct(*tensors) -> bool:
     """Whether a call on these tensors (None among them) may skip the dispatcher."""
-    if _modes() or _interpreter() is not None or compiling():
+    if compiling() or _modes() or _interpreter() is not None or forward_ad._current_level >= 0:
         return False
     grad = torch.is_grad_enabled()
     return all(t is None or (plain(t) and not (grad and t.requires_grad)) for t in tensors)

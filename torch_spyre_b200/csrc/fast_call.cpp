@@ -1,8 +1,9 @@
 // The plain case of the verification operators' Python calls, without Python:
 // tensors that are all as the operator wants them, in eager mode with nothing
-// to differentiate.  A function here checks that much, allocates the result and
-// calls the C entry on the current stream; in every other case it returns None,
-// and the caller takes the Python path, which raises or handles what was met.
+// to differentiate (rotary: with its gradient).  A function here checks that
+// much, allocates the result and calls the C entry on the current stream; in
+// every other case it returns None, and the caller takes the Python path, which
+// raises or handles what was met.
 // (Host time of rotary on 16 tokens: 12 us by the Python path, 4 by this one.)
 #include <Python.h>
 
@@ -13,6 +14,7 @@
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cstdlib>
@@ -74,13 +76,15 @@ struct Call {
     ok = ok && !c10::impl::TorchDispatchModeTLS::any_modes_set() &&
          !c10::impl::tls_local_dispatch_key_set().included_.has(DispatchKey::FuncTorchDynamicLayerFrontMode);
   }
-  const at::Tensor *tensor(PyObject *o) {
+  const at::Tensor *tensor(PyObject *o, bool with_grad = false) {
     if (!ok || !THPVariable_CheckExact(o)) {
       ok = false;
       return nullptr;
     }
     const at::Tensor &t = THPVariable_Unpack(o);
-    if (!t.is_cuda() || t.layout() != c10::kStrided || (t.requires_grad() && c10::GradMode::is_enabled()) ||
+    const bool grad = t.requires_grad() && c10::GradMode::is_enabled();
+    const bool tangent = t.unsafeGetTensorImpl()->autograd_meta() && t._fw_grad(0).defined();
+    if (!t.is_cuda() || t.layout() != c10::kStrided || (grad && !with_grad) || tangent ||
         (has_device && t.device() != device)) {
       ok = false;
       return nullptr;
@@ -155,22 +159,65 @@ void *stream_of(const Call &c) { return c10::cuda::getCurrentCUDAStream(c.device
     return nullptr;                                            \
   }
 
+// x turned, undefined if the entry refuses.
+at::Tensor turn(const at::Tensor &x, const at::Tensor &table, const at::Tensor &pos, bool interleaved, bool transpose,
+                int32_t *flag) {
+  const c10::cuda::CUDAGuard guard(x.device());
+  at::Tensor out = at::empty(x.sizes(), x.options());
+  const int st = entries.rotary(x.data_ptr(), code_of(x.scalar_type()), x.stride(0), x.stride(1), out.data_ptr(),
+                                static_cast<const float *>(table.data_ptr()), table.size(0), 2 * table.size(1),
+                                static_cast<const int32_t *>(pos.data_ptr()), x.size(0), x.size(1), x.size(2),
+                                interleaved, transpose, flag,
+                                c10::cuda::getCurrentCUDAStream(x.device().index()).stream());
+  return st == 0 ? out : at::Tensor();
+}
+
+// rotary with its gradient: the same map turned the other way.
+struct Turn : torch::autograd::Function<Turn> {
+  static at::Tensor forward(torch::autograd::AutogradContext *ctx, const at::Tensor &x, const at::Tensor &table,
+                            const at::Tensor &pos, bool interleaved, bool transpose,
+                            const std::optional<at::Tensor> &flag) {
+    ctx->save_for_backward({table, pos});
+    ctx->saved_data["interleaved"] = interleaved;
+    ctx->saved_data["transpose"] = transpose;
+    ctx->saved_data["flag"] = flag;
+    at::Tensor out = turn(x, table, pos, interleaved, transpose, flag ? flag->data_ptr<int32_t>() : nullptr);
+    TORCH_CHECK(out.defined(), "b200kv_rotary failed");
+    return out;
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx,
+                                                 torch::autograd::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    at::Tensor g = grads[0];
+    if (g.dim() == 3 && g.stride(2) != 1) g = g.contiguous();  // e.g. the expanded gradient of a sum
+    at::Tensor none;
+    return {Turn::apply(g, saved[0], saved[1], ctx->saved_data["interleaved"].toBool(),
+                        !ctx->saved_data["transpose"].toBool(), ctx->saved_data["flag"].toOptional<at::Tensor>()),
+            none, none, none, none, none};
+  }
+};
+
 // rotary(x, table, positions, interleaved, transpose, error_flag)
 PyObject *rotary(PyObject *, PyObject *const *a, Py_ssize_t n) {
   B200KV_ARGS(6)
   Call c;
-  const at::Tensor *x = c.tensor(a[0]), *table = c.tensor(a[1]), *pos = c.tensor(a[2]);
+  const at::Tensor *x = c.tensor(a[0], true), *table = c.tensor(a[1]), *pos = c.tensor(a[2]);
   int32_t *flag = c.flag(a[5]);
   if (!c.ok || !rows_ok(x)) Py_RETURN_NONE;
   const int code = code_of(x->scalar_type());
   if (code < 0 || code > 2 || !table_ok(table, pos, x->size(0), x->size(2))) Py_RETURN_NONE;
-  const c10::cuda::CUDAGuard guard(c.device);
-  at::Tensor out = at::empty(x->sizes(), x->options());
-  const int st = entries.rotary(x->data_ptr(), code, x->stride(0), x->stride(1), out.data_ptr(),
-                                static_cast<const float *>(data(table)), table->size(0), 2 * table->size(1),
-                                static_cast<const int32_t *>(data(pos)), x->size(0), x->size(1), x->size(2),
-                                a[3] == Py_True, a[4] == Py_True, flag, stream_of(c));
-  if (st != 0) Py_RETURN_NONE;
+  const bool interleaved = a[3] == Py_True, transpose = a[4] == Py_True;
+  at::Tensor out;
+  if (!x->requires_grad() || !c10::GradMode::is_enabled()) {
+    out = turn(*x, *table, *pos, interleaved, transpose, flag);
+  } else {
+    // (a head_dim that the entry refuses goes to the Python path, which says so)
+    if (x->size(2) > 4096 || x->size(1) > 65536 || x->size(0) >= int64_t(1) << 31 || x->numel() == 0) Py_RETURN_NONE;
+    std::optional<at::Tensor> kept;
+    if (flag) kept = THPVariable_Unpack(a[5]);
+    out = Turn::apply(*x, *table, *pos, interleaved, transpose, kept);
+  }
+  if (!out.defined()) Py_RETURN_NONE;
   return THPVariable_Wrap(std::move(out));
 }
 
