@@ -60,42 +60,38 @@ __device__ __forceinline__ uint2 steps8_e4m3(const float (&f)[8], float inv) {
   return make_uint2(__byte_perm(w[0], w[1], 0x5410), __byte_perm(w[2], w[3], 0x5410));
 }
 
-// A group of D / 8 lanes takes one row, kRows rows of a token one after the
-// other (q heads, then K heads, then V heads), its vector's cos / sin in
-// registers.  The half layout's partner vector comes by shuffle (rotary_dim / 2
-// is a multiple of 8, so the partner is a whole lane away).
+// A group of D / 8 lanes takes one row, kRows rows of a token and kind (q, K or
+// V heads) one after the other, its vector's cos / sin in registers.  The half
+// layout's partner vector comes by shuffle (rotary_dim / 2 is a multiple of 8,
+// so the partner is a whole lane away).
 // kCache: B200KV_F16 (= the row type), B200KV_I8 or B200KV_E4M3.
 template <typename T, int D, int kCache, int kTurn, int kRows>  // kTurn 0 none, 1 half, 2 interleaved
 __global__ void __launch_bounds__(256, kRows > 1 ? 5 : 1) kv_store_kernel(const StoreArgs a) {
   constexpr int kLanes = D / 8;
   constexpr int kStick = kCache == B200KV_F16 ? 64 : 128;
   const int lane = threadIdx.x % kLanes, e = lane * 8;
-  const int heads = a.hq + 2 * a.hkv;
-  const uint32_t groups = (heads + kRows - 1) / kRows;
+  const uint32_t of_q = (a.hq + kRows - 1) / kRows, of_kv = (a.hkv + kRows - 1) / kRows;  // units of a kind
   const uint32_t unit = blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes;
-  const uint32_t t32 = unit / groups;
-  const int r0 = static_cast<int>(unit - t32 * groups) * kRows;
+  const uint32_t t32 = unit / (of_q + 2 * of_kv);
+  uint32_t u = unit - t32 * (of_q + 2 * of_kv);
+  const int kind = u < of_q ? 0 : (u < of_q + of_kv ? 1 : 2);  // q, K, V
+  u -= kind == 0 ? 0 : (kind == 1 ? of_q : of_q + of_kv);
+  const int h0 = static_cast<int>(u) * kRows;
   const int64_t t = t32;
   const bool live_t = t < a.tokens;  // dead lanes stay for the shuffles
+  const int rows = live_t ? min(kRows, (kind == 0 ? a.hq : a.hkv) - h0) : 0;
 
   uint4 raw[kRows];
-  if (live_t) {
+  {
+    const int64_t sn = kind == 0 ? a.q_sn : (kind == 1 ? a.k_sn : a.v_sn);
+    const int64_t sh = kind == 0 ? a.q_sh : (kind == 1 ? a.k_sh : a.v_sh);
+    const T *src = static_cast<const T *>(kind == 0 ? a.q : (kind == 1 ? a.k : a.v)) + t * sn + h0 * sh + e;
 #pragma unroll
-    for (int i = 0; i < kRows; ++i) {
-      const int r = r0 + i;
-      if (r >= heads) break;
-      const T *src;
-      if (r < a.hq)
-        src = static_cast<const T *>(a.q) + t * a.q_sn + r * a.q_sh;
-      else if (r < a.hq + a.hkv)
-        src = static_cast<const T *>(a.k) + t * a.k_sn + (r - a.hq) * a.k_sh;
-      else
-        src = static_cast<const T *>(a.v) + t * a.v_sn + (r - a.hq - a.hkv) * a.v_sh;
-      raw[i] = __ldg(reinterpret_cast<const uint4 *>(src + e));
-    }
+    for (int i = 0; i < kRows; ++i)
+      if (i < rows) raw[i] = __ldg(reinterpret_cast<const uint4 *>(src + i * sh));
   }
   int64_t slot = -1;
-  if (live_t && r0 + kRows > a.hq) {
+  if (rows > 0 && kind > 0) {
     slot = __ldg(a.slots + t);
     if (slot >= a.num_slots) {
       if (a.error_flag && lane == 0) atomicOr(a.error_flag, B200KV_DEVERR_BAD_SLOT);
@@ -106,52 +102,57 @@ __global__ void __launch_bounds__(256, kRows > 1 ? 5 : 1) kv_store_kernel(const 
   // the second half use the same pairs), 4 interleaved
   constexpr int kPairs = kTurn == 2 ? 4 : 8;
   float cosv[kPairs], sinv[kPairs];
-  const bool turn_lane = kTurn != 0 && e < 2 * a.half;
+  const bool turn_lane = kTurn != 0 && rows > 0 && kind < 2 && e < 2 * a.half;
   const bool second = kTurn == 1 && e >= a.half;
-  if (kTurn != 0) {
+  const bool whole = kTurn == 1 || e / 2 + 4 <= a.half;  // no pair past rotary_dim
+  if (turn_lane) {
+    int64_t pos = __ldg(a.positions + t);
+    if (pos < 0 || pos >= a.max_pos) {
+      if (a.error_flag && lane == 0) atomicOr(a.error_flag, B200KV_DEVERR_BAD_LEN);
+      pos = pos < 0 ? 0 : a.max_pos - 1;
+    }
+    const float2 *row = a.table + pos * a.half + (kTurn == 2 ? e / 2 : (second ? e - a.half : e));
+    if (kTurn == 1 || (a.half % 2 == 0 && whole)) {  // 16-byte aligned, all inside
 #pragma unroll
-    for (int i = 0; i < kPairs; ++i) cosv[i] = 1.f, sinv[i] = 0.f;
-    if (live_t && turn_lane && r0 < a.hq + a.hkv) {
-      int64_t pos = __ldg(a.positions + t);
-      if (pos < 0 || pos >= a.max_pos) {
-        if (a.error_flag && lane == 0) atomicOr(a.error_flag, B200KV_DEVERR_BAD_LEN);
-        pos = pos < 0 ? 0 : a.max_pos - 1;
+      for (int i = 0; i < kPairs; i += 2) {
+        const float4 cs = __ldg(reinterpret_cast<const float4 *>(row + i));
+        cosv[i] = cs.x, sinv[i] = cs.y, cosv[i + 1] = cs.z, sinv[i + 1] = cs.w;
       }
-      const float2 *row = a.table + pos * a.half + (kTurn == 2 ? e / 2 : (second ? e - a.half : e));
-      if (kTurn == 1 || (a.half % 2 == 0 && e / 2 + 4 <= a.half)) {  // 16-byte aligned, all inside
+    } else {
 #pragma unroll
-        for (int i = 0; i < kPairs; i += 2) {
-          const float4 cs = __ldg(reinterpret_cast<const float4 *>(row + i));
-          cosv[i] = cs.x, sinv[i] = cs.y, cosv[i + 1] = cs.z, sinv[i + 1] = cs.w;
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < kPairs; ++i) {
-          // an interleaved vector cut by rotary_dim: the identity past it
-          const float2 cs = e / 2 + i < a.half ? __ldg(row + i) : make_float2(1.f, 0.f);
-          cosv[i] = cs.x;
-          sinv[i] = cs.y;
-        }
+      for (int i = 0; i < kPairs; ++i) {
+        // an interleaved vector cut by rotary_dim: nothing past it is used
+        const float2 cs = e / 2 + i < a.half ? __ldg(row + i) : make_float2(1.f, 0.f);
+        cosv[i] = cs.x;
+        sinv[i] = cs.y;
       }
     }
   }
   const int shift = kTurn == 1 ? a.half / 8 : 0;
   const int partner = second ? lane - shift : lane + shift;
+  // of the first row; the next head's is D elements (q) or a page on
+  T *q_out = static_cast<T *>(a.q_out) + (t * a.hq + h0) * D + e;
+  const int64_t page = (slot >> 6) * a.hkv + h0;
+  const int in_page = static_cast<int>(slot & 63);
+  const int64_t at = page * (64 * D) + e / kStick * (64 * kStick) + in_page * kStick + e % kStick;
+  void *pool = kind == 1 ? a.k_pool : a.v_pool;
+  float *scale = (kind == 1 ? a.k_scales : a.v_scales) + page * 64 + in_page;
+  // (units of two kinds can meet in a warp: it skips what none of them needs)
+  const bool any_turned = kTurn == 1 && __any_sync(0xffffffffu, rows > 0 && kind < 2);
+  const bool any_stored = __any_sync(0xffffffffu, rows > 0 && kind > 0);
 
 #pragma unroll
   for (int i = 0; i < kRows; ++i) {
-    const int r = r0 + i;
-    const bool live = live_t && r < heads;
+    const bool live = i < rows;
     float f[8];
     if (live) unpack8(raw[i], f, T());
-    // (rows of two kinds can meet in a warp: it skips what none of them needs)
-    if (kTurn == 1 && __any_sync(0xffffffffu, live && r < a.hq + a.hkv)) {
+    if (any_turned) {
       uint4 o;  // every lane takes part in the shuffles
       o.x = __shfl_sync(0xffffffffu, raw[i].x, partner, kLanes);
       o.y = __shfl_sync(0xffffffffu, raw[i].y, partner, kLanes);
       o.z = __shfl_sync(0xffffffffu, raw[i].z, partner, kLanes);
       o.w = __shfl_sync(0xffffffffu, raw[i].w, partner, kLanes);
-      if (live && turn_lane && r < a.hq + a.hkv) {
+      if (live && turn_lane) {
         float p[8], unused;
         unpack8(o, p, T());
 #pragma unroll
@@ -162,27 +163,21 @@ __global__ void __launch_bounds__(256, kRows > 1 ? 5 : 1) kv_store_kernel(const 
             turn_pair(f[j], p[j], cosv[j], sinv[j], f[j], unused);
         }
       }
-    } else if (kTurn == 2) {
-      if (live && turn_lane && r < a.hq + a.hkv) {
+    } else if (kTurn == 2 && live && turn_lane) {
+      if (whole) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) turn_pair(f[2 * j], f[2 * j + 1], cosv[j], sinv[j], f[2 * j], f[2 * j + 1]);
+      } else {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
           if (e / 2 + j < a.half) turn_pair(f[2 * j], f[2 * j + 1], cosv[j], sinv[j], f[2 * j], f[2 * j + 1]);
       }
     }
-    if (live && r < a.hq) {
-      T *dst = static_cast<T *>(a.q_out) + (t * a.hq + r) * D + e;
-      *reinterpret_cast<uint4 *>(dst) = pack8(f, T());
-    }
-    if (!__any_sync(0xffffffffu, live && r >= a.hq)) continue;
-    const bool is_k = r < a.hq + a.hkv;
-    const int h = r - a.hq - (is_k ? 0 : a.hkv);
-    const bool write = live && r >= a.hq && slot >= 0;
-    const int64_t page = (slot >> 6) * a.hkv + h;
-    const int in_page = static_cast<int>(slot & 63);
-    const int64_t at = (page * (D / kStick) + e / kStick) * (64 * kStick) + int64_t(in_page) * kStick + e % kStick;
-    void *pool = is_k ? a.k_pool : a.v_pool;
+    if (live && kind == 0) *reinterpret_cast<uint4 *>(q_out + i * D) = pack8(f, T());
+    if (!any_stored) continue;
+    const bool write = live && kind > 0 && slot >= 0;
     if (kCache == B200KV_F16) {
-      if (write) *reinterpret_cast<uint4 *>(static_cast<T *>(pool) + at) = pack8(f, T());
+      if (write) *reinterpret_cast<uint4 *>(static_cast<T *>(pool) + at + i * (64 * D)) = pack8(f, T());
     } else {
       float amax = 0.f;
       if (live) {
@@ -200,8 +195,8 @@ __global__ void __launch_bounds__(256, kRows > 1 ? 5 : 1) kv_store_kernel(const 
         const float inv = s > 0.f && finite ? __fdiv_rn(1.f, s) : 0.f;
         const uint2 w = !finite ? make_uint2(0, 0)
                         : kCache == B200KV_I8 ? steps8_int8(f, inv) : steps8_e4m3(f, inv);
-        *reinterpret_cast<uint2 *>(static_cast<uint8_t *>(pool) + at) = w;
-        if (lane == 0) (is_k ? a.k_scales : a.v_scales)[page * 64 + in_page] = finite ? s : CUDART_NAN_F;
+        *reinterpret_cast<uint2 *>(static_cast<uint8_t *>(pool) + at + i * (64 * D)) = w;
+        if (lane == 0) scale[i * 64] = finite ? s : CUDART_NAN_F;
       }
     }
   }
@@ -220,7 +215,7 @@ int launch_store(const StoreArgs &a, cudaStream_t stream) {
   // blocks per SM and 113 at six, four rows 117 at four and 116 at five, eight
   // rows 116 at four; int8 in the half layout 143, 156, 124, 127 and 135.)
   const bool deep = a.tokens * heads * kLanes >= int64_t(sms) * 2048 * 4;
-  const int64_t units = a.tokens * ((heads + (deep ? 3 : 0)) / (deep ? 4 : 1));
+  const int64_t units = a.tokens * (deep ? (a.hq + 3) / 4 + 2 * ((a.hkv + 3) / 4) : heads);
   const int64_t blocks = (units * kLanes + 255) / 256;
   if (units >= (int64_t{1} << 31))  // the kernel counts them in 32 bits
     return set_error(B200KV_ERR_UNSUPPORTED, "%lld tokens of %d heads: 2^31 rows or more", (long long)a.tokens, heads);

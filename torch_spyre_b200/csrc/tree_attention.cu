@@ -21,6 +21,8 @@ namespace {
 __global__ void __launch_bounds__(128) tree_mask_kernel(const int32_t *parents, const int32_t *indptr, int batch,
                                                         int64_t total, int64_t words, uint64_t *mask,
                                                         int32_t *error_flag) {
+  // (the attention that comes next sets itself up meanwhile; it waits for the mask)
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int64_t i = int64_t(blockIdx.x) * blockDim.x + threadIdx.x;
   if (i >= total) return;
   uint64_t *row = mask + i * words;
