@@ -60,16 +60,28 @@ __device__ __forceinline__ uint2 steps8_e4m3(const float (&f)[8], float inv) {
   return make_uint2(__byte_perm(w[0], w[1], 0x5410), __byte_perm(w[2], w[3], 0x5410));
 }
 
-// A group of D / 8 lanes takes one row, kRows rows of a token and kind (q, K or
-// V heads) one after the other, its vector's cos / sin in registers.  The half
-// layout's partner vector comes by shuffle (rotary_dim / 2 is a multiple of 8,
-// so the partner is a whole lane away).
+// A group of lanes takes one row, kRows rows of a token and kind (q, K or V
+// heads) one after the other, the cos / sin of its elements in registers.  A
+// lane has one 16-byte vector, or in the half layout two: a vector and the one
+// that holds its pairs' other elements (rotary_dim / 2 is a multiple of 8), or
+// two neighbours past rotary_dim.
 // kCache: B200KV_F16 (= the row type), B200KV_I8 or B200KV_E4M3.
+//
+// Bound: bytes, and the instructions of the conversions right behind them.  16381
+// tokens of 32 + 16 heads, 128 elements of which 96 are turned, bf16 into e4m3
+// (369 MB): 73 us, 0.78 of the copy rate, and 101 with two readings back; into
+// bf16 100, in the half layout 102 (into int8 105).  Rows and blocks per SM, us
+// with the readings: interleaved four and five 101, eight and five 121; half
+// layout two and four 105, two and three 114, four and three 100, four and two
+// 112.  A lane of the half layout with one vector, its partner's by shuffle: 127.
 template <typename T, int D, int kCache, int kTurn, int kRows>  // kTurn 0 none, 1 half, 2 interleaved
-__global__ void __launch_bounds__(256, kRows > 1 ? 5 : 1) kv_store_kernel(const StoreArgs a) {
-  constexpr int kLanes = D / 8;
+__global__ void __launch_bounds__(256, kRows > 1 ? (kTurn == 1 ? 3 : 5) : 1) kv_store_kernel(const StoreArgs a) {
+  constexpr int kVecs = kTurn == 1 ? 2 : 1, kLanes = D / 8 / kVecs;
   constexpr int kStick = kCache == B200KV_F16 ? 64 : 128;
-  const int lane = threadIdx.x % kLanes, e = lane * 8;
+  const int lane = threadIdx.x % kLanes;
+  const bool paired = kTurn == 1 && lane < a.half / 8;
+  const int e = kTurn == 1 && !paired ? 16 * lane : 8 * lane;  // the first vector's elements
+  const int beside = paired ? a.half : 8;                      // from the first vector to the second
   const uint32_t of_q = (a.hq + kRows - 1) / kRows, of_kv = (a.hkv + kRows - 1) / kRows;  // units of a kind
   const uint32_t unit = blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes;
   const uint32_t t32 = unit / (of_q + 2 * of_kv);
@@ -81,14 +93,16 @@ __global__ void __launch_bounds__(256, kRows > 1 ? 5 : 1) kv_store_kernel(const 
   const bool live_t = t < a.tokens;  // dead lanes stay for the shuffles
   const int rows = live_t ? min(kRows, (kind == 0 ? a.hq : a.hkv) - h0) : 0;
 
-  uint4 raw[kRows];
+  uint4 raw[kRows][kVecs];
   {
     const int64_t sn = kind == 0 ? a.q_sn : (kind == 1 ? a.k_sn : a.v_sn);
     const int64_t sh = kind == 0 ? a.q_sh : (kind == 1 ? a.k_sh : a.v_sh);
     const T *src = static_cast<const T *>(kind == 0 ? a.q : (kind == 1 ? a.k : a.v)) + t * sn + h0 * sh + e;
 #pragma unroll
     for (int i = 0; i < kRows; ++i)
-      if (i < rows) raw[i] = __ldg(reinterpret_cast<const uint4 *>(src + i * sh));
+#pragma unroll
+      for (int x = 0; x < kVecs; ++x)
+        if (i < rows) raw[i][x] = __ldg(reinterpret_cast<const uint4 *>(src + i * sh + x * beside));
   }
   int64_t slot = -1;
   if (rows > 0 && kind > 0) {
@@ -98,20 +112,18 @@ __global__ void __launch_bounds__(256, kRows > 1 ? 5 : 1) kv_store_kernel(const 
       slot = -1;
     }
   }
-  // cos / sin of this lane's elements: 8 pairs in the half layout (elements of
-  // the second half use the same pairs), 4 interleaved
+  // cos / sin of this lane's pairs: 8 in the half layout, 4 interleaved
   constexpr int kPairs = kTurn == 2 ? 4 : 8;
   float cosv[kPairs], sinv[kPairs];
-  const bool turn_lane = kTurn != 0 && rows > 0 && kind < 2 && e < 2 * a.half;
-  const bool second = kTurn == 1 && e >= a.half;
+  const bool turned = rows > 0 && kind < 2 && (kTurn == 1 ? paired : kTurn == 2 && e < 2 * a.half);
   const bool whole = kTurn == 1 || e / 2 + 4 <= a.half;  // no pair past rotary_dim
-  if (turn_lane) {
+  if (turned) {
     int64_t pos = __ldg(a.positions + t);
     if (pos < 0 || pos >= a.max_pos) {
       if (a.error_flag && lane == 0) atomicOr(a.error_flag, B200KV_DEVERR_BAD_LEN);
       pos = pos < 0 ? 0 : a.max_pos - 1;
     }
-    const float2 *row = a.table + pos * a.half + (kTurn == 2 ? e / 2 : (second ? e - a.half : e));
+    const float2 *row = a.table + pos * a.half + (kTurn == 2 ? e / 2 : e);
     if (kTurn == 1 || (a.half % 2 == 0 && whole)) {  // 16-byte aligned, all inside
 #pragma unroll
       for (int i = 0; i < kPairs; i += 2) {
@@ -128,61 +140,56 @@ __global__ void __launch_bounds__(256, kRows > 1 ? 5 : 1) kv_store_kernel(const 
       }
     }
   }
-  const int shift = kTurn == 1 ? a.half / 8 : 0;
-  const int partner = second ? lane - shift : lane + shift;
   // of the first row; the next head's is D elements (q) or a page on
   T *q_out = static_cast<T *>(a.q_out) + (t * a.hq + h0) * D + e;
   const int64_t page = (slot >> 6) * a.hkv + h0;
   const int in_page = static_cast<int>(slot & 63);
-  const int64_t at = page * (64 * D) + e / kStick * (64 * kStick) + in_page * kStick + e % kStick;
+  const int64_t at = page * (64 * D) + in_page * kStick;
+  int in_row[kVecs];  // a vector's place in the pool, from its row's
+#pragma unroll
+  for (int x = 0; x < kVecs; ++x) {
+    const int ex = e + x * beside;
+    in_row[x] = ex / kStick * (64 * kStick) + ex % kStick;
+  }
   void *pool = kind == 1 ? a.k_pool : a.v_pool;
   float *scale = (kind == 1 ? a.k_scales : a.v_scales) + page * 64 + in_page;
   // (units of two kinds can meet in a warp: it skips what none of them needs)
-  const bool any_turned = kTurn == 1 && __any_sync(0xffffffffu, rows > 0 && kind < 2);
   const bool any_stored = __any_sync(0xffffffffu, rows > 0 && kind > 0);
 
 #pragma unroll
   for (int i = 0; i < kRows; ++i) {
     const bool live = i < rows;
-    float f[8];
-    if (live) unpack8(raw[i], f, T());
-    if (any_turned) {
-      uint4 o;  // every lane takes part in the shuffles
-      o.x = __shfl_sync(0xffffffffu, raw[i].x, partner, kLanes);
-      o.y = __shfl_sync(0xffffffffu, raw[i].y, partner, kLanes);
-      o.z = __shfl_sync(0xffffffffu, raw[i].z, partner, kLanes);
-      o.w = __shfl_sync(0xffffffffu, raw[i].w, partner, kLanes);
-      if (live && turn_lane) {
-        float p[8], unused;
-        unpack8(o, p, T());
+    float f[kVecs][8];
+    if (live) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          if (second)
-            turn_pair(p[j], f[j], cosv[j], sinv[j], unused, f[j]);
-          else
-            turn_pair(f[j], p[j], cosv[j], sinv[j], f[j], unused);
-        }
-      }
-    } else if (kTurn == 2 && live && turn_lane) {
-      if (whole) {
+      for (int x = 0; x < kVecs; ++x) unpack8(raw[i][x], f[x], T());
+      if (kTurn == 1 && turned) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) turn_pair(f[2 * j], f[2 * j + 1], cosv[j], sinv[j], f[2 * j], f[2 * j + 1]);
-      } else {
+        for (int j = 0; j < 8; ++j) turn_pair(f[0][j], f[kVecs - 1][j], cosv[j], sinv[j], f[0][j], f[kVecs - 1][j]);
+      } else if (kTurn == 2 && turned) {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          if (e / 2 + j < a.half) turn_pair(f[2 * j], f[2 * j + 1], cosv[j], sinv[j], f[2 * j], f[2 * j + 1]);
+          if (whole || e / 2 + j < a.half)
+            turn_pair(f[0][2 * j], f[0][2 * j + 1], cosv[j], sinv[j], f[0][2 * j], f[0][2 * j + 1]);
       }
     }
-    if (live && kind == 0) *reinterpret_cast<uint4 *>(q_out + i * D) = pack8(f, T());
+    if (live && kind == 0) {
+#pragma unroll
+      for (int x = 0; x < kVecs; ++x) *reinterpret_cast<uint4 *>(q_out + i * D + x * beside) = pack8(f[x], T());
+    }
     if (!any_stored) continue;
     const bool write = live && kind > 0 && slot >= 0;
     if (kCache == B200KV_F16) {
-      if (write) *reinterpret_cast<uint4 *>(static_cast<T *>(pool) + at + i * (64 * D)) = pack8(f, T());
+#pragma unroll
+      for (int x = 0; x < kVecs; ++x)
+        if (write) *reinterpret_cast<uint4 *>(static_cast<T *>(pool) + at + in_row[x] + i * (64 * D)) = pack8(f[x], T());
     } else {
       float amax = 0.f;
       if (live) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) amax = max_nan(amax, fabsf(f[j]));
+        for (int x = 0; x < kVecs; ++x)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) amax = max_nan(amax, fabsf(f[x][j]));
       }
 #pragma unroll
       for (int m = kLanes / 2; m >= 1; m >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, m, kLanes));
@@ -193,9 +200,12 @@ __global__ void __launch_bounds__(256, kRows > 1 ? 5 : 1) kv_store_kernel(const 
         if (s < 1.17549435e-38f) s = 0.f;
         const bool finite = s < CUDART_INF_F;
         const float inv = s > 0.f && finite ? __fdiv_rn(1.f, s) : 0.f;
-        const uint2 w = !finite ? make_uint2(0, 0)
-                        : kCache == B200KV_I8 ? steps8_int8(f, inv) : steps8_e4m3(f, inv);
-        *reinterpret_cast<uint2 *>(static_cast<uint8_t *>(pool) + at + i * (64 * D)) = w;
+#pragma unroll
+        for (int x = 0; x < kVecs; ++x) {
+          const uint2 w = !finite ? make_uint2(0, 0)
+                          : kCache == B200KV_I8 ? steps8_int8(f[x], inv) : steps8_e4m3(f[x], inv);
+          *reinterpret_cast<uint2 *>(static_cast<uint8_t *>(pool) + at + in_row[x] + i * (64 * D)) = w;
+        }
         if (lane == 0) scale[i * 64] = finite ? s : CUDART_NAN_F;
       }
     }
@@ -207,20 +217,18 @@ int launch_store(const StoreArgs &a, cudaStream_t stream) {
   int dev = 0, sms = 0;
   int st = current_device_sm_count(&dev, &sms);
   if (st != B200KV_OK) return st;
-  constexpr int kLanes = D / 8;
-  const int heads = a.hq + 2 * a.hkv;
+  constexpr int kVecs = kTurn == 1 ? 2 : 1, kLanes = D / 8 / kVecs;
   // Four rows per lane group once every SM still gets its 2048 threads; with
-  // fewer rows one each, as the latency of the loads counts.  (16381 tokens of
-  // 32 + 16 heads into e4m3, us with two readings back: two rows 131 at four
-  // blocks per SM and 113 at six, four rows 117 at four and 116 at five, eight
-  // rows 116 at four; int8 in the half layout 143, 156, 124, 127 and 135.)
-  const bool deep = a.tokens * heads * kLanes >= int64_t(sms) * 2048 * 4;
-  const int64_t units = a.tokens * (deep ? (a.hq + 3) / 4 + 2 * ((a.hkv + 3) / 4) : heads);
+  // fewer rows one each, as the latency of the loads counts.
+  constexpr int kDeep = 4;
+  const int heads = a.hq + 2 * a.hkv;
+  const bool deep = a.tokens * heads * (D / 8) >= int64_t(sms) * 2048 * 4;
+  const int64_t units = a.tokens * (deep ? (a.hq + kDeep - 1) / kDeep + 2 * ((a.hkv + kDeep - 1) / kDeep) : heads);
   const int64_t blocks = (units * kLanes + 255) / 256;
   if (units >= (int64_t{1} << 31))  // the kernel counts them in 32 bits
     return set_error(B200KV_ERR_UNSUPPORTED, "%lld tokens of %d heads: 2^31 rows or more", (long long)a.tokens, heads);
   if (deep)
-    kv_store_kernel<T, D, kCache, kTurn, 4><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(a);
+    kv_store_kernel<T, D, kCache, kTurn, kDeep><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(a);
   else
     kv_store_kernel<T, D, kCache, kTurn, 1><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(a);
   B200KV_CUDA_TRY(cudaGetLastError());
