@@ -60,7 +60,7 @@ struct Vec {
 };
 
 // kHeads heads per thread.  Half layout: item c < half / kN is the pair of
-// vectors at c * kN and half + c * kN, later items are single copied vectors.
+// vectors at c * kN and half + c * kN, a later item two copied neighbours.
 // Interleaved: every item is one vector, its pairs before rotary_dim turned.
 template <typename T, bool kInterleaved, int kHeads>
 __global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a) {
@@ -80,7 +80,9 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a) {
   T *out = static_cast<T *>(a.out) + t * a.heads * a.dim;
   const int pair_items = kInterleaved ? 0 : a.half / kN;
   const bool pair = !kInterleaved && c < pair_items;
-  const int e = kInterleaved || pair ? c * kN : 2 * a.half + (c - pair_items) * kN;
+  const int e = kInterleaved || pair ? c * kN : 2 * a.half + (c - pair_items) * 2 * kN;
+  const int beside = pair ? a.half : kN;
+  const bool second = pair || (!kInterleaved && e + kN < a.dim);
   const bool turn = kInterleaved ? e < 2 * a.half : pair;
 
   uint4 va[kHeads], vb[kHeads];
@@ -88,7 +90,7 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a) {
   for (int i = 0; i < kHeads; ++i) {
     if (h0 + i < a.heads) {
       va[i] = __ldg(reinterpret_cast<const uint4 *>(x + (h0 + i) * a.xs_h + e));
-      if (pair) vb[i] = __ldg(reinterpret_cast<const uint4 *>(x + (h0 + i) * a.xs_h + a.half + e));
+      if (second) vb[i] = __ldg(reinterpret_cast<const uint4 *>(x + (h0 + i) * a.xs_h + beside + e));
     }
   }
   float cosv[kPairs], sinv[kPairs];
@@ -126,6 +128,7 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a) {
       __stcs(reinterpret_cast<uint4 *>(o), Vec<T>::store(f));
     } else {
       __stcs(reinterpret_cast<uint4 *>(o), va[i]);
+      if (second) __stcs(reinterpret_cast<uint4 *>(o + beside), vb[i]);
     }
   }
 }
@@ -171,7 +174,7 @@ int launch_rotary(RotaryArgs a, cudaStream_t stream) {
     B200KV_CUDA_TRY(cudaGetLastError());
     return B200KV_OK;
   }
-  a.items = kInterleaved ? a.dim / kN : (a.dim - a.half) / kN;
+  a.items = kInterleaved ? a.dim / kN : a.half / kN + ((a.dim - 2 * a.half) / kN + 1) / 2;
   // Four heads per thread once that still leaves every SM its 2048 threads;
   // below, one head per thread: with few rows the latency of one load counts.
   const bool deep = a.tokens * a.heads * a.items >= int64_t(sms) * 2048 * 4;
