@@ -261,7 +261,8 @@ struct LoadArgs {
 // kChunks threads of a row are neighbours, so reads and writes are whole lines.
 // All kUnroll slots, then all rows and scales, are in flight together.  Row
 // numbers are 32-bit (the host checks): a 64-bit division per row cost as much
-// as the row's memory traffic.
+// as the row's memory traffic.  131072 tokens of 8 heads, e4m3 to bf16 (408 MB):
+// 70 us, 0.91 of the copy rate; int8 67.
 template <int kCache, typename TIn, typename TOut, int D, int kUnroll>
 __global__ void __launch_bounds__(256) kv_load_kernel(const LoadArgs a) {
   constexpr bool k8 = kCache != B200KV_F16;

@@ -19,10 +19,27 @@
 // rescaled when a row's maximum has risen by more than 2^8 (weights then stay
 // below 2^8, far from fp16's range), so most tiles touch it in the MMA alone.
 //
-// Bound: with up to 128 rows a 128-token tile costs the tensor pipe 0.55 us
-// (2 x 128^3 products at 8192 FLOP per clock) and HBM 1.5 us per SM, so drafts
-// run at the cache's bandwidth; blocks of two Q tiles are bound by the tensor
-// pipe and the exponentials (16 per clock and SM, as long as the products).
+// Bound, 16-bit caches: with up to 128 rows a 128-token tile costs the tensor pipe
+// 0.55 us (2 x 128^3 products at 8192 FLOP per clock) and HBM 1.5 us per SM, so
+// drafts run at the cache's bandwidth (4 sequences of 118k tokens, 16 nodes, 32/8
+// heads, fp16, 1.93 GB: 237 us); short ones by what a piece costs besides its
+// steps (16 sequences of 4.3k tokens and up to 64 nodes, bf16, 285 MB: 75 us, the
+// copy rate would be 44).  Blocks of two Q tiles are bound by the tensor pipe and
+// the exponentials (16 per clock and SM, as long as the products), which follow
+// one another within a stream: 4096 tokens of a prompt in two sequences, 64/8
+// heads, 578 GFLOP: 590 us, 0.58 of the matrix rate; without the softmax it took
+// 440, without the products 480.
+//
+// 8-bit caches: widening (2 x 16 KB a tile), softmax and products take 0.6 to 0.7
+// us a tile and SM each and are a chain with handshakes, which 3 raw and 4
+// operand tiles let overlap in part only: 1.7 us a tile, 4 sequences of 118k
+// tokens, int8, 1.0 GB: 327 us (e4m3, whose widening goes through the
+// conversion unit: 426).  Without widening 0.88 of that, without softmax 0.77,
+// without products 0.92.  More than 128 rows: every Q tile widens the tile
+// again.  (Tried: two Q tiles a block with three operand tiles, 0.93 of the time
+// with all blocks full but 1.08 with ragged drafts; widening by 16 warps in two
+// groups, 1.2; by two groups of four, one for K and one for V, 1.1; scores in
+// matrix fragments, a quarter of the factors' reads, 1.0.)
 //
 // Warps: 0-3 and 4-7 the two softmax warpgroups, 8 the TMA producer, 9 the MMA
 // issuer (owns the TMEM), 8-bit caches: 12-19 converters, which turn 8-bit
@@ -54,7 +71,7 @@ struct Cfg {
   static constexpr int kTile = kSticks * kStickTile;        // a Q, K or V tile
   static constexpr int kQ = k8 ? 1 : 2;                      // most Q tiles of a block
   static constexpr int kSlots = k8 ? 4 : (D == 64 ? 8 : 5);  // operand tiles in flight
-  static constexpr int kRaw = k8 ? 3 : 0;                   // 8-bit tiles in flight
+  static constexpr int kRaw = k8 ? 3 : 0;                    // 8-bit tiles in flight
   static constexpr int kRawTile = kTileTokens * 128;
   static constexpr int kCtrl = k8 ? 19456 : 3072;
   static constexpr int kOffQ = kCtrl;
@@ -297,7 +314,7 @@ struct Walk {
   int b, kvh, block, u0, tiles, t0, t1;  // piece: token tiles [t0, t1) of `tiles`
   int end;                               // of the share
 
-  __device__ __forceinline__ void init(const Args &a, const Ctrl &c) {
+  __device__ __forceinline__ void init(const Ctrl &c) {
     const Start &f = c.start;
     s = f.s, b = f.b, kvh = f.kvh, block = f.block, u0 = f.u0;
     t1 = 0;
@@ -426,7 +443,7 @@ __device__ __forceinline__ void producer(const Args &a, Ctrl &c, uint8_t *smem, 
   bool dead = false;
   uint32_t slot = 0, ring = 0, pieces = 0;  // tiles issued (16-bit, 8-bit), pieces begun
   Walk<C::kQ> w;
-  w.init(a, c);
+  w.init(c);
   while (w.next(a, c)) {
     const bool two = w.two();
     const int pages = (w.s.ctx + w.s.nodes + kPageTokens - 1) / kPageTokens;
@@ -627,7 +644,7 @@ __device__ __forceinline__ void converter(const Args &a, Ctrl &c, uint8_t *smem,
     ++slot;
   };
   Walk<C::kQ> w;
-  w.init(a, c);
+  w.init(c);
   while (w.next(a, c)) {
     ++piece;
     const int len = w.s.ctx + w.s.nodes;
@@ -675,7 +692,7 @@ __device__ __forceinline__ void mma_issuer(const Args &a, Ctrl &c, uint8_t *smem
       mma_ts(tmem + col_o(w), tmem + col_s(w) + i * 8, vd + (i * 2048 >> 4), C::kIdescPV, !first || i > 0, go);
   };
   Walk<C::kQ> w;
-  w.init(a, c);
+  w.init(c);
   while (w.next(a, c)) {
     wait(&c.q_full, pieces++ & 1u, dead, a.error_flag);
     fence_after();
@@ -988,7 +1005,7 @@ __device__ __forceinline__ void softmax(const Args &a, Ctrl &c, uint8_t *smem, u
   uint32_t s_uses = 0, o_uses[2] = {0, 0}, slot = 0;
   unsigned piece = 0;
   Walk<C::kQ> wk;
-  wk.init(a, c);
+  wk.init(c);
   while (wk.next(a, c)) {
     ++piece;
     const bool two = wk.two();
