@@ -33,8 +33,8 @@
 // 8-bit caches: widening (2 x 16 KB a tile), softmax and products take 0.6 to 0.7
 // us a tile and SM each and are a chain with handshakes, which 3 raw and 4
 // operand tiles let overlap in part only: 1.7 us a tile, 4 sequences of 118k
-// tokens, int8, 1.0 GB: 327 us (e4m3, whose widening goes through the
-// conversion unit: 426).  Without widening 0.88 of that, without softmax 0.77,
+// tokens, int8, 1.0 GB: 327 us (e4m3, which the conversion unit widens with fewer
+// instructions: 296).  Without widening 0.88 of that, without softmax 0.77,
 // without products 0.92.  More than 128 rows: every Q tile widens the tile
 // again.  (Tried: two Q tiles a block with three operand tiles, 0.93 of the time
 // with all blocks full but 1.08 with ragged drafts; widening by 16 warps in two
