@@ -26,9 +26,8 @@
 // steps (16 sequences of 4.3k tokens and up to 64 nodes, bf16, 285 MB: 75 us, the
 // copy rate would be 44).  Blocks of two Q tiles are bound by the tensor pipe and
 // the exponentials (16 per clock and SM, as long as the products), which follow
-// one another within a stream: 4096 tokens of a prompt in two sequences, 64/8
-// heads, 578 GFLOP: 590 us, 0.58 of the matrix rate; without the softmax it took
-// 440, without the products 480.
+// one another within a stream: two prompts' chunks of 1024 tokens over 8.1k, 64/8
+// heads, 578 GFLOP: 528 us, 0.64 of the matrix rate.
 //
 // 8-bit caches: widening (2 x 16 KB a tile), softmax and products take 0.6 to 0.7
 // us a tile and SM each and are a chain with handshakes, which 3 raw and 4
@@ -439,13 +438,19 @@ template <typename C>
 __device__ __forceinline__ void producer(const Args &a, Ctrl &c, uint8_t *smem, const CUtensorMap *qm,
                                          const CUtensorMap *km, const CUtensorMap *vm) {
   const int lane = threadIdx.x & 31;
-  const uint64_t policy = l2_policy_evict_first();
+  // Pages are read once and leave L2 first, unless more than two blocks read them
+  // (two prompts' chunks of 1024 tokens: 582 us, 528 with the plain policy; with
+  // two blocks, drafts up to 64 nodes of 64/8 heads, 116 and 118).
+  const uint64_t policy_once = l2_policy_evict_first();
+  uint64_t policy_again;
+  asm volatile("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(policy_again));
   bool dead = false;
   uint32_t slot = 0, ring = 0, pieces = 0;  // tiles issued (16-bit, 8-bit), pieces begun
   Walk<C::kQ> w;
   w.init(c);
   while (w.next(a, c)) {
     const bool two = w.two();
+    const uint64_t policy = w.s.blocks > 2 ? policy_again : policy_once;
     const int pages = (w.s.ctx + w.s.nodes + kPageTokens - 1) / kPageTokens;
     int window = w.t0 / 16, ids = load_ids(a, w.b, window, pages), ids_next = load_ids(a, w.b, window + 1, pages);
     wait(&c.q_empty, (pieces & 1u) ^ 1u, dead, a.error_flag);
