@@ -687,8 +687,9 @@ B200KV_API int b200kv_tree_attention(const void *q, int32_t q_dtype, int64_t q_s
 /* Moves the accepted path: for i < path_lens[b], the K/V rows (and scales) of
  * node path[b][i] go to position context_lens[b] + i, every row read before it
  * is overwritten; new_lens[b] = context_lens[b] + path_lens[b].  The path
- * ascends (a node comes after its ancestors); an entry that does not, or lies
- * outside the block table, is skipped and sets B200KV_DEVERR_BAD_SLOT; bad
+ * ascends from 0 on (a node comes after its ancestors); an entry that does not
+ * (not above the one before it, or below its own index i), or that lies outside
+ * the block table, is skipped and sets B200KV_DEVERR_BAD_SLOT; bad
  * lengths move nothing and set B200KV_DEVERR_BAD_LEN (new_lens[b] is then
  * context_lens[b]). */
 B200KV_API int b200kv_tree_commit(void *k_pool, void *v_pool, int32_t pool_dtype, float *k_scales,

@@ -1,0 +1,52 @@
+"""Edges of the verification operators: inputs that are out of range or out of order, extreme scales,
+rows that no sequence has, and calls from several host threads."""
+
+import pytest
+import torch
+
+import torch_spyre_b200 as tsb
+from tests.verify_ref import make_cache
+from torch_spyre_b200 import _lib
+
+pytestmark = pytest.mark.gpu
+
+F16, BF16, I8, F8 = torch.float16, torch.bfloat16, torch.int8, torch.float8_e4m3fn
+
+
+def int32(*values):
+    return torch.tensor(values, dtype=torch.int32, device="cuda")
+
+
+# ------------------------------------------------------------------ commit --
+@pytest.mark.parametrize("cache", [F16, I8])
+@pytest.mark.parametrize("ctx", [0, 3, 100])
+@pytest.mark.parametrize("path,kept", [
+    # (path, the entries that move): a run of negatives that ascends, entries below their own index
+    ([0, -5, -4, 9], [0, 3]),
+    ([-7, -6, -2, 3, 8], [3, 4]),
+    ([5, 1, 2, 3, 7], [0, 3, 4]),
+    (list(range(0, 140, 2)) + [0, 1, 2, 500], list(range(70)) + [73]),
+    (list(range(1, 65)) + [-1000, -999, -998, 70], list(range(64)) + [67]),
+])
+def test_commit_skips_entries_that_do_not_ascend(cache, ctx, path, kept):
+    g = torch.Generator(device="cuda").manual_seed(1)
+    (kp, ks), (vp, vs) = (make_cache(24, 2, 128, cache, g) for _ in range(2))
+    # the sequence's row of the table comes first, then one that must not be read
+    table = torch.stack([torch.arange(10), torch.arange(10, 20)]).int().cuda()
+    before = [None if t is None else t.clone() for t in (kp, vp, ks, vs)]
+    flag = torch.zeros(1, dtype=torch.int32, device="cuda")
+    paths = torch.tensor([path, [0] * len(path)], dtype=torch.int32, device="cuda")
+    new = tsb.tree_commit(kp, vp, table, int32(ctx, 0), paths, int32(len(path), 0), ks, vs, error_flag=flag)
+    assert int(flag.item()) == _lib.DEVERR_BAD_SLOT and new.tolist() == [ctx + len(path), 0]
+    for now, was, is_pool in zip((kp, vp, ks, vs), before, (True, True, False, False)):
+        if now is None:
+            continue
+        now, was = (t.view(torch.uint8) if is_pool else t for t in (now, was))
+        want = was.clone()
+        for i in kept:
+            src, dst = ctx + path[i], ctx + i
+            if is_pool:
+                want[dst // 64, :, :, dst % 64] = was[src // 64, :, :, src % 64]
+            else:
+                want[dst // 64, :, dst % 64] = was[src // 64, :, src % 64]
+        assert torch.equal(now, want)

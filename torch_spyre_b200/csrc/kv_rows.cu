@@ -376,8 +376,8 @@ constexpr int kCommitThreads = 128, kCommitRows = 64;
 // One CTA per sequence and KV head, K and V one after the other.  The path is
 // taken 64 rows at a time: thread i finds where row i comes from and goes to, and
 // moves its scale; then the rows move, 16 bytes per thread.  A batch is read
-// whole before any of it is written; the path ascends, so path[i] >= i and a
-// later batch never reads what an earlier one wrote.
+// whole before any of it is written; path[i] >= i (checked), so a later batch
+// never reads what an earlier one wrote.
 //
 // Bound: bytes, each moved row read and written once; few rows: the chain length
 // -> path -> block table -> row.  128 sequences, 8 KV heads, 32 rows each on
@@ -422,7 +422,9 @@ __global__ void __launch_bounds__(kCommitThreads) tree_commit_kernel(const Commi
       const int i = base + tid;
       if (i < n) {
         const int p = __ldg(path + i), before = i > 0 ? __ldg(path + i - 1) : -1;
-        if (p <= before) {  // not ascending: the row stays where it is
+        // (p < i: not ascending from 0 on, and so neither is any negative entry;
+        // its row may have been overwritten already)
+        if (p <= before || p < i) {  // the row stays where it is
           if (a.error_flag) atomicOr(a.error_flag, B200KV_DEVERR_BAD_SLOT);
         } else if (p != i) {
           src = offset(ctx + p, p < cap - ctx);
