@@ -686,7 +686,8 @@ B200KV_API int b200kv_tree_attention(const void *q, int32_t q_dtype, int64_t q_s
 
 /* Moves the accepted path: for i < path_lens[b], the K/V rows (and scales) of
  * node path[b][i] go to position context_lens[b] + i, every row read before it
- * is overwritten; new_lens[b] = context_lens[b] + path_lens[b].  The path
+ * is overwritten; new_lens[b] = context_lens[b] + path_lens[b].  path[b][i] is
+ * path[b * path_stride + i] (stride 0: one path for all sequences).  The path
  * ascends from 0 on (a node comes after its ancestors); an entry that does not
  * (not above the one before it, or below its own index i), or that lies outside
  * the block table, is skipped and sets B200KV_DEVERR_BAD_SLOT; bad

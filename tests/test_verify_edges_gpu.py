@@ -50,3 +50,29 @@ def test_commit_skips_entries_that_do_not_ascend(cache, ctx, path, kept):
             else:
                 want[dst // 64, :, dst % 64] = was[src // 64, :, src % 64]
         assert torch.equal(now, want)
+
+
+@pytest.mark.parametrize("registered", [False, True])
+@pytest.mark.parametrize("view", ["expanded", "wider", "one column", "overlapping"])
+def test_commit_takes_paths_of_any_row_stride(view, registered):
+    g = torch.Generator(device="cuda").manual_seed(2)
+    table = torch.arange(9, dtype=torch.int32, device="cuda").view(3, 3)
+    rows = int32(*range(2, 40))
+    path = {"expanded": lambda: int32(1, 4, 9).expand(3, 3), "wider": lambda: rows[:36].view(3, 12)[:, :5],
+            "one column": lambda: int32(7).expand(3, 1), "overlapping": lambda: rows.as_strided((3, 5), (2, 1))}[view]()
+    tight = path.contiguous()
+    lens, n = int32(3, 60, 100), torch.full((3,), path.shape[1], dtype=torch.int32, device="cuda")
+    pools = [make_cache(9, 2, 128, I8, g) for _ in range(2)]
+    after = []
+    commit = torch.ops.b200kv.tree_commit if registered else lambda *a: tsb.tree_commit(*a[:-1], error_flag=a[-1])
+    for p in (path, tight):
+        flag = torch.zeros(1, dtype=torch.int32, device="cuda")
+        (kp, ks), (vp, vs) = ((a.clone(), s.clone()) for a, s in pools)
+        if view == "overlapping" and p is path:  # refused: rows of one path must not run into the next's
+            with pytest.raises(tsb.B200KVError, match="path_stride"):
+                commit(kp, vp, table, lens, p, n, ks, vs, flag)
+            return
+        new = commit(kp, vp, table, lens, p, n, ks, vs, flag)
+        assert int(flag.item()) == 0
+        after.append((kp, ks, vp, vs, new))
+    assert all(torch.equal(x, y) for x, y in zip(*after))

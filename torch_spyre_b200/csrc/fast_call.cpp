@@ -365,7 +365,7 @@ PyObject *tree_commit(PyObject *, PyObject *const *a, Py_ssize_t n) {
   const int st = entries.tree_commit(
       kp->data_ptr(), vp->data_ptr(), p.code, static_cast<float *>(data(ks)), static_cast<float *>(data(vs)),
       static_cast<const int32_t *>(data(table)), table->stride(0), static_cast<const int32_t *>(data(lens)),
-      static_cast<const int32_t *>(data(path)), std::max(path->stride(0), path->size(1)),
+      static_cast<const int32_t *>(data(path)), batch > 1 ? path->stride(0) : path->size(1),
       static_cast<const int32_t *>(data(plens)), static_cast<int32_t *>(out.data_ptr()), batch, p.heads, p.dim, p.blocks,
       table->size(1), path->size(1), flag, stream_of(c));
   if (st != 0) Py_RETURN_NONE;

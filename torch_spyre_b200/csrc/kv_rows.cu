@@ -588,7 +588,7 @@ extern "C" int b200kv_tree_commit(void *k_pool, void *v_pool, int32_t pool_dtype
                        max_blocks_per_seq > 0 && max_blocks_per_seq * kPageTokens < (int64_t{1} << 30),
                    "num_kv_heads, num_blocks or max_blocks_per_seq out of range");
   B200KV_CHECK_ARG(block_table_stride >= max_blocks_per_seq, "block_table_stride < max_blocks_per_seq");
-  B200KV_CHECK_ARG(max_path >= 0 && max_path < (int64_t{1} << 30) && path_stride >= max_path,
+  B200KV_CHECK_ARG(max_path >= 0 && max_path < (int64_t{1} << 30) && (path_stride >= max_path || path_stride == 0),
                    "max_path out of range or path_stride < max_path");
   if (batch == 0) return B200KV_OK;
   B200KV_CHECK_ARG(k_pool && v_pool && block_table && context_lens && path_lens && new_lens && (path || max_path == 0),

@@ -217,7 +217,7 @@ def _tree_commit_impl(
         "b200kv_tree_commit", device,
         k_pool.data_ptr(), v_pool.data_ptr(), DTYPE_CODES[k_pool.dtype], _ptr(k_scales), _ptr(v_scales),
         block_table.data_ptr(), block_table.stride(0), context_lens.data_ptr(), path.data_ptr(),
-        max(path.stride(0), path.shape[1]), path_lens.data_ptr(), new_lens.data_ptr(),
+        path.stride(0) if B > 1 else path.shape[1], path_lens.data_ptr(), new_lens.data_ptr(),
         B, Hkv, D, NB, block_table.shape[1], path.shape[1], _ptr(error_flag),
     )
     _maybe_check_flag(error_flag, "tree_commit")
@@ -245,7 +245,7 @@ def tree_commit(
     error_flag: Optional[torch.Tensor] = None,
 ) -> torch.Tensor:
     """Moves the K/V rows (and scales) of the accepted nodes path[b, :path_lens[b]]
-    (int32, ascending) to positions context_lens[b], context_lens[b] + 1, ... of
+    (int32, ascending; one path expanded over the batch will do) to positions context_lens[b], context_lens[b] + 1, ... of
     their sequence, in place, and returns the new lengths
     context_lens + path_lens (int32 [B])."""
     args = (k_pool, v_pool, block_table, context_lens, path, path_lens, k_scales, v_scales, error_flag)
