@@ -1,11 +1,13 @@
 """Edges of the verification operators: inputs that are out of range or out of order, extreme scales,
 rows that no sequence has, and calls from several host threads."""
 
+import threading
+
 import pytest
 import torch
 
 import torch_spyre_b200 as tsb
-from tests.verify_ref import make_cache
+from tests.verify_ref import TreeCase, make_cache
 from torch_spyre_b200 import _lib
 
 pytestmark = pytest.mark.gpu
@@ -76,3 +78,41 @@ def test_commit_takes_paths_of_any_row_stride(view, registered):
         assert int(flag.item()) == 0
         after.append((kp, ks, vp, vs, new))
     assert all(torch.equal(x, y) for x, y in zip(*after))
+
+
+# ----------------------------------------------------------------- threads --
+def in_threads(calls):
+    """What the calls return (or raise), each by a thread of its own."""
+    results = [None] * len(calls)
+
+    def run(i):
+        try:
+            results[i] = calls[i]()
+        except Exception as e:  # noqa: BLE001 (shown by the caller)
+            results[i] = e
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(len(calls))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for r in results:
+        if isinstance(r, Exception):
+            raise r
+    return results
+
+
+@pytest.mark.parametrize("cache", [F16, I8])
+def test_first_call_of_a_host_thread(cache):
+    """A thread's first use of CUDA can be a call that encodes tensor maps."""
+    case = TreeCase([300, 7], [9, 3], 8, 2, cache=cache, seed=1)
+    want = tsb.tree_attention(*case.args(), **case.kwargs())
+    torch.cuda.synchronize()
+    (got,) = in_threads([lambda: tsb.tree_attention(*case.args(), **case.kwargs())])
+    assert torch.equal(got, want)
+    if cache == F16:
+        one = TreeCase([300, 7], [1, 1], 8, 2, seed=1)
+        args = (one.q, one.k_pool, one.v_pool, one.block_table.clamp_min(0), one.context_lens + 1)
+        want = tsb.decode_attention(*args)
+        torch.cuda.synchronize()
+        assert torch.equal(in_threads([lambda: tsb.decode_attention(*args)])[0], want)

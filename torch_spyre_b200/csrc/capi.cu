@@ -49,6 +49,29 @@ int current_device_sm_count(int *device_out, int *sms_out) {
   return B200KV_OK;
 }
 
+namespace {
+EncodeTiledFn g_encode_tiled = nullptr;
+
+// A host thread that has not used CUDA yet has no context for the driver call;
+// the runtime gives it the current device's.
+CUresult encode_tiled(CUtensorMap *map, CUtensorMapDataType type, cuuint32_t rank, void *base,
+                      const cuuint64_t *dims, const cuuint64_t *strides, const cuuint32_t *box,
+                      const cuuint32_t *elem_strides, CUtensorMapInterleave interleave,
+                      CUtensorMapSwizzle swizzle, CUtensorMapL2promotion promotion,
+                      CUtensorMapFloatOOBfill fill) {
+  auto encode = [&] {
+    return g_encode_tiled(map, type, rank, base, dims, strides, box, elem_strides, interleave,
+                          swizzle, promotion, fill);
+  };
+  const CUresult r = encode();
+  int dev = 0;
+  if (r != CUDA_ERROR_INVALID_CONTEXT || cudaGetDevice(&dev) != cudaSuccess ||
+      cudaSetDevice(dev) != cudaSuccess)
+    return r;
+  return encode();
+}
+}  // namespace
+
 EncodeTiledFn encode_tiled_fn() {
   static EncodeTiledFn fn = nullptr;
   static std::once_flag once;
@@ -57,8 +80,10 @@ EncodeTiledFn encode_tiled_fn() {
     cudaDriverEntryPointQueryResult q;
     if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) ==
             cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<EncodeTiledFn>(p);
+        q == cudaDriverEntryPointSuccess) {
+      g_encode_tiled = reinterpret_cast<EncodeTiledFn>(p);
+      fn = encode_tiled;
+    }
   });
   return fn;
 }
