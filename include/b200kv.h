@@ -650,7 +650,10 @@ B200KV_API int b200kv_tree_mask(const int32_t *parents, const int32_t *q_indptr,
                                 int32_t *error_flag, void *stream);
 
 /* Workspace bytes of b200kv_tree_attention (-1: unsupported shape).  It needs
- * no initial contents; calls that share it must be ordered on one stream. */
+ * no initial contents; calls that share it must be ordered on one stream.  (The
+ * call is two launches; several host threads may make calls on one stream and
+ * workspace, decode's among them: each enqueues its launches without another's
+ * in between.) */
 B200KV_API int64_t b200kv_tree_workspace_bytes(int64_t total_q, int64_t batch, int64_t num_q_heads,
                                                int64_t num_kv_heads, int64_t head_dim);
 

@@ -116,3 +116,32 @@ def test_first_call_of_a_host_thread(cache):
         want = tsb.decode_attention(*args)
         torch.cuda.synchronize()
         assert torch.equal(in_threads([lambda: tsb.decode_attention(*args)])[0], want)
+
+
+def test_host_threads_share_a_stream():
+    """Calls of several host threads on one stream and workspace, of the widest difference in rows, beside
+    decode calls: each gives the bits that it gives alone."""
+    cases = [TreeCase([5000], [3], 8, 2, seed=1), TreeCase([900, 0, 3000], [300, 200, 500], 8, 2, seed=2),
+             TreeCase([20000, 70], [16, 1], 8, 2, cache=I8, seed=3), TreeCase([64], [1], 8, 2, cache=F8, seed=4)]
+    decode = TreeCase([4000] * 20, [1] * 20, 8, 2, seed=5)
+    table, lens = decode.block_table.clamp_min(0), decode.context_lens + 1
+    stream = torch.cuda.current_stream()
+
+    def tree_call(c):  # the registered operator: its entry is called without the interpreter lock
+        return torch.ops.b200kv.tree_attention(*c.args(), c.mask, 128**-0.5, c.max_nodes, c.k_scales, c.v_scales, None)
+
+    def decode_call(c):
+        return torch.ops.b200kv.decode_attention(c.q, c.k_pool, c.v_pool, table, lens, 128**-0.5, 0, None)
+
+    work = [(tree_call, c) for c in cases] + [(decode_call, decode)] * 2
+    want = [call(c) for call, c in work]
+    torch.cuda.synchronize()
+
+    def run(call, c):
+        with torch.cuda.stream(stream):
+            got = [call(c) for _ in range(60)]
+            stream.synchronize()
+        return got
+
+    for got, one in zip(in_threads([lambda call=call, c=c: run(call, c) for call, c in work]), want):
+        assert all(torch.equal(x, y) for pair in got for x, y in zip(pair, one))

@@ -50,6 +50,17 @@ int current_device_sm_count(int *device_out, int *sms_out) {
 }
 
 namespace {
+constexpr int kWorkspaceLocks = 64;
+std::mutex g_workspace_locks[kWorkspaceLocks];
+}  // namespace
+
+WorkspaceLock::WorkspaceLock(const void *workspace)
+    : index_(static_cast<int>((reinterpret_cast<uintptr_t>(workspace) >> 20) % kWorkspaceLocks)) {
+  g_workspace_locks[index_].lock();
+}
+WorkspaceLock::~WorkspaceLock() { g_workspace_locks[index_].unlock(); }
+
+namespace {
 EncodeTiledFn g_encode_tiled = nullptr;
 
 // A host thread that has not used CUDA yet has no context for the driver call;

@@ -48,6 +48,22 @@ int cuda_status(cudaError_t err, const char *what);
 // Number of SMs of the current device (cached per device ordinal).
 int current_device_sm_count(int *device_out, int *sms_out);
 
+// Held by a call while it enqueues the launches that use a workspace.  Tree
+// attention is two launches, the second of which reads what the first one left
+// there; without this, calls of two host threads on one stream could come to
+// A1 B1 A2 B2 (or a decode between A1 and A2), and A2 would take B's rows for
+// its own.  (A lock serves all workspaces that hash to it.)
+class WorkspaceLock {
+ public:
+  explicit WorkspaceLock(const void *workspace);
+  ~WorkspaceLock();
+  WorkspaceLock(const WorkspaceLock &) = delete;
+  WorkspaceLock &operator=(const WorkspaceLock &) = delete;
+
+ private:
+  int index_;
+};
+
 // cuTensorMapEncodeTiled resolved through the runtime's driver entry point
 // (no link-time dependency on libcuda).
 using EncodeTiledFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t,

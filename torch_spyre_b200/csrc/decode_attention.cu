@@ -170,6 +170,7 @@ static int decode_entry(
     }
   }
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const WorkspaceLock lock(workspace);
   if (use_simt_kernel()) {
     // CUDA-core variant: num_splits is its target number of work items per CTA
     const int per_cta = num_splits > 0 ? static_cast<int>(num_splits < 64 ? num_splits : 64)

@@ -219,6 +219,7 @@ extern "C" int b200kv_tree_attention(const void *q, int32_t q_dtype, int64_t q_s
   if (st != B200KV_OK) return st;
   const int ctas = sms < tree::kMaxCtas ? sms : tree::kMaxCtas;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const WorkspaceLock lock(workspace);
   return q_dtype == B200KV_F16 ? tree::launch_f16(qm, km, vm, a, static_cast<int>(head_dim), pool_dtype, ctas, s)
                                : tree::launch_bf16(qm, km, vm, a, static_cast<int>(head_dim), pool_dtype, ctas, s);
 }
