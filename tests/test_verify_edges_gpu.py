@@ -19,6 +19,26 @@ def int32(*values):
     return torch.tensor(values, dtype=torch.int32, device="cuda")
 
 
+@pytest.mark.parametrize("flag", [torch.zeros(1, dtype=torch.int32), torch.zeros(1, dtype=torch.int64),
+                                  torch.zeros(0, dtype=torch.int32)])
+def test_flags_that_a_kernel_cannot_write_are_refused(flag):
+    if flag.dtype == torch.int64 or flag.numel() == 0:
+        flag = flag.cuda()
+    case = TreeCase([10], [2], 2, 1, cache=I8, seed=1)
+    rows = torch.randn(2, 1, 128, device="cuda", dtype=F16)
+    slots, pos, table = torch.arange(2, device="cuda"), int32(0, 1), tsb.rotary_table(4, 128, device="cuda")
+    kv = (case.k_pool, case.v_pool)
+    for call in (lambda: tsb.rotary(rows, table, pos, error_flag=flag),
+                 lambda: tsb.kv_store(rows, rows, *kv, slots, case.k_scales, case.v_scales, error_flag=flag),
+                 lambda: tsb.kv_load(case.k_pool, slots, case.k_scales, error_flag=flag),
+                 lambda: tsb.tree_mask(int32(-1, 0), int32(0, 2), 2, error_flag=flag),
+                 lambda: tsb.tree_attention(*case.args(), **case.kwargs(), error_flag=flag),
+                 lambda: tsb.tree_commit(*kv, case.block_table, case.context_lens, int32(0).view(1, 1), int32(1),
+                                         case.k_scales, case.v_scales, error_flag=flag)):
+        with pytest.raises(ValueError, match="error_flag"):
+            call()
+
+
 # ------------------------------------------------------------------ commit --
 @pytest.mark.parametrize("cache", [F16, I8])
 @pytest.mark.parametrize("ctx", [0, 3, 100])

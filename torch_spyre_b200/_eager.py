@@ -21,6 +21,7 @@ from __future__ import annotations
 import ctypes
 import importlib.util
 from pathlib import Path
+from typing import Optional
 
 import torch
 from torch.autograd import forward_ad
@@ -69,6 +70,16 @@ def direct(*tensors) -> bool:
         return False
     grad = torch.is_grad_enabled()
     return all(t is None or (plain(t) and not (grad and t.requires_grad)) for t in tensors)
+
+
+def flag_ptr(flag: Optional[torch.Tensor], device: torch.device) -> Optional[int]:
+    """Address of an error flag, which a kernel on ``device`` may write to."""
+    if flag is None:
+        return None
+    if flag.dtype != torch.int32 or flag.device != device or flag.numel() < 1:
+        raise ValueError(f"error_flag must be an int32 tensor on {device}, got {flag.numel()} elements of {flag.dtype} "
+                         f"on {flag.device}")
+    return flag.data_ptr()
 
 
 def launch(name: str, device: torch.device, *args) -> None:

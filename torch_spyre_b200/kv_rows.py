@@ -18,7 +18,7 @@ from typing import Optional
 import torch
 
 from . import _eager
-from ._eager import direct, launch, written
+from ._eager import direct, flag_ptr, launch, written
 from .layout import PAGE_TOKENS
 from .ops import _maybe_check_flag, _ptr, _require_cuda
 from .rotations import DTYPE_CODES, ROTARY_DTYPES, check_table
@@ -120,7 +120,8 @@ def _kv_store_impl(
         "b200kv_kv_store", device, *q_args, out.data_ptr(),
         k_new.data_ptr(), k_new.stride(0), k_new.stride(1), v_new.data_ptr(), v_new.stride(0), v_new.stride(1),
         DTYPE_CODES[dtype], k_pool.data_ptr(), v_pool.data_ptr(), DTYPE_CODES[k_pool.dtype],
-        _ptr(k_scales), _ptr(v_scales), slots.data_ptr(), *turn, interleaved, N, Hq, Hkv, D, NB, _ptr(error_flag),
+        _ptr(k_scales), _ptr(v_scales), slots.data_ptr(), *turn, interleaved, N, Hq, Hkv, D, NB,
+        flag_ptr(error_flag, device),
     )
     _maybe_check_flag(error_flag, "kv_store")
     return out
@@ -180,7 +181,7 @@ def _kv_load_impl(pool: torch.Tensor, slots: torch.Tensor, scales: Optional[torc
         raise ValueError(f"dtype must be fp16, bf16 or fp32, got {dtype}")
     out = torch.empty((N, Hkv, D), dtype=dtype, device=device)
     launch("b200kv_kv_load", device, pool.data_ptr(), DTYPE_CODES[pool.dtype], _ptr(scales), slots.data_ptr(),
-           out.data_ptr(), DTYPE_CODES[dtype], N, Hkv, D, NB, _ptr(error_flag))
+           out.data_ptr(), DTYPE_CODES[dtype], N, Hkv, D, NB, flag_ptr(error_flag, device))
     _maybe_check_flag(error_flag, "kv_load")
     return out
 

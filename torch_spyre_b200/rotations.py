@@ -18,8 +18,8 @@ from typing import Optional
 import torch
 
 from . import _eager, _lib
-from ._eager import launch
-from .ops import _maybe_check_flag, _ptr, _require_cuda
+from ._eager import flag_ptr, launch
+from .ops import _maybe_check_flag, _require_cuda
 
 ROTARY_SCALINGS = ("none", "linear", "ntk", "yarn")
 
@@ -102,7 +102,7 @@ def _rotary_impl(x: torch.Tensor, table: torch.Tensor, positions: torch.Tensor, 
     out = torch.empty_like(x, memory_format=torch.contiguous_format)
     launch("b200kv_rotary", device, x.data_ptr(), ROTARY_DTYPES[x.dtype], x.stride(0), x.stride(1), out.data_ptr(),
            table.data_ptr(), table.shape[0], 2 * table.shape[1], positions.data_ptr(), T, H, D, interleaved, transpose,
-           _ptr(error_flag))
+           flag_ptr(error_flag, device))
     _maybe_check_flag(error_flag, "rotary")
     return out
 

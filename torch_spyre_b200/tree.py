@@ -21,7 +21,7 @@ from typing import Optional
 import torch
 
 from . import _eager, _lib
-from ._eager import direct, launch, written
+from ._eager import direct, flag_ptr, launch, written
 from .kv_rows import DTYPES_16, check_row_pools
 from .ops import _maybe_check_flag, _ptr, _require_cuda, workspace_for
 from .rotations import DTYPE_CODES
@@ -54,7 +54,7 @@ def _tree_mask_impl(parents: torch.Tensor, q_indptr: torch.Tensor, mask_words: i
     _check_indptr(q_indptr, q_indptr.shape[0] - 1, parents.device)
     mask = torch.empty((parents.shape[0], mask_words), dtype=torch.int64, device=parents.device)
     launch("b200kv_tree_mask", parents.device, parents.data_ptr(), q_indptr.data_ptr(), q_indptr.shape[0] - 1,
-           parents.shape[0], mask_words, mask.data_ptr(), _ptr(error_flag))
+           parents.shape[0], mask_words, mask.data_ptr(), flag_ptr(error_flag, parents.device))
     _maybe_check_flag(error_flag, "tree_mask")
     return mask
 
@@ -132,7 +132,8 @@ def _attend(q, k_pool, v_pool, block_table, context_lens, q_indptr, tree_mask, s
         k_pool.data_ptr(), v_pool.data_ptr(), DTYPE_CODES[k_pool.dtype], _ptr(k_scales), _ptr(v_scales),
         block_table.data_ptr(), block_table.stride(0), context_lens.data_ptr(), q_indptr.data_ptr(),
         _ptr(tree_mask), words, out.data_ptr(), _ptr(lse),
-        N, B, Hq, Hkv, D, NB, block_table.shape[1], max_nodes, scale, ws.data_ptr(), ws.numel(), _ptr(error_flag),
+        N, B, Hq, Hkv, D, NB, block_table.shape[1], max_nodes, scale, ws.data_ptr(), ws.numel(),
+        flag_ptr(error_flag, device),
     )
     _maybe_check_flag(error_flag, "tree_attention")
     return out, lse
@@ -218,7 +219,7 @@ def _tree_commit_impl(
         k_pool.data_ptr(), v_pool.data_ptr(), DTYPE_CODES[k_pool.dtype], _ptr(k_scales), _ptr(v_scales),
         block_table.data_ptr(), block_table.stride(0), context_lens.data_ptr(), path.data_ptr(),
         path.stride(0) if B > 1 else path.shape[1], path_lens.data_ptr(), new_lens.data_ptr(),
-        B, Hkv, D, NB, block_table.shape[1], path.shape[1], _ptr(error_flag),
+        B, Hkv, D, NB, block_table.shape[1], path.shape[1], flag_ptr(error_flag, device),
     )
     _maybe_check_flag(error_flag, "tree_commit")
     return new_lens
