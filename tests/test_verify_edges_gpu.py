@@ -1,6 +1,7 @@
 """Edges of the verification operators: inputs that are out of range or out of order, extreme scales,
 rows that no sequence has, and calls from several host threads."""
 
+import math
 import threading
 
 import pytest
@@ -9,6 +10,7 @@ import torch
 import torch_spyre_b200 as tsb
 from tests.verify_ref import TreeCase, make_cache
 from torch_spyre_b200 import _lib
+from torch_spyre_b200.rotations import DTYPE_CODES
 
 pytestmark = pytest.mark.gpu
 
@@ -19,6 +21,51 @@ def int32(*values):
     return torch.tensor(values, dtype=torch.int32, device="cuda")
 
 
+# --------------------------------------------------------------------- rows --
+def attend_into(case, out, lse, context_lens=None, q_indptr=None, max_nodes=None):
+    """The C entry with outputs that the caller has filled; returns the error flag."""
+    ctx = case.context_lens if context_lens is None else context_lens
+    indptr = case.q_indptr if q_indptr is None else q_indptr
+    N, Hq, D = case.q.shape
+    batch = len(ctx)
+    size = _lib.lib().b200kv_tree_workspace_bytes(N, batch, Hq, case.hkv, D)
+    ws = torch.empty(size, dtype=torch.uint8, device="cuda")
+    flag = torch.zeros(1, dtype=torch.int32, device="cuda")
+    sc = [None if s is None else s.data_ptr() for s in (case.k_scales, case.v_scales)]
+    mask, words = (None, 0) if case.mask is None else (case.mask.data_ptr(), case.mask.shape[1])
+    table = case.block_table
+    st = _lib.lib().b200kv_tree_attention(
+        case.q.data_ptr(), DTYPE_CODES[case.q.dtype], case.q.stride(0), case.q.stride(1), case.k_pool.data_ptr(),
+        case.v_pool.data_ptr(), DTYPE_CODES[case.k_pool.dtype], *sc, table.data_ptr(), table.stride(0), ctx.data_ptr(),
+        indptr.data_ptr(), mask, words, out.data_ptr(), lse.data_ptr(), N, batch, Hq, case.hkv, D, case.k_pool.shape[0],
+        table.shape[1], max_nodes or case.max_nodes, D**-0.5, ws.data_ptr(), size, flag.data_ptr(),
+        torch.cuda.current_stream().cuda_stream)
+    assert st == 0, _lib.last_error()
+    torch.cuda.synchronize()
+    return int(flag.item())
+
+
+@pytest.mark.parametrize("cache", [F16, I8])
+@pytest.mark.parametrize("over,cut", [
+    (dict(max_nodes=20), range(32, 52)),
+    (dict(context_lens=(100, 128)), range(12, 52)),
+    (dict(context_lens=(100, 120)), range(20, 52)),
+    (dict(q_indptr=(0, 12, 45)), range(45, 52)),
+    (dict(q_indptr=(3, 12, 52)), range(0, 3)),
+])
+def test_rows_that_no_sequence_has_are_zero(cache, over, cut):
+    case = TreeCase([100, 30], [12, 40], 8, 2, cache=cache, seed=19, poison=False)
+    over = {k: v if isinstance(v, int) else int32(*v) for k, v in over.items()}
+    out, lse = torch.full_like(case.q, math.nan), torch.full((52, 8), math.nan, device="cuda")
+    assert attend_into(case, out, lse, **over) & _lib.DEVERR_BAD_LEN
+    cut = torch.tensor(list(cut), device="cuda")
+    assert bool((out[cut] == 0).all()) and bool((lse[cut] == -math.inf).all())
+    kept = torch.ones(52, dtype=torch.bool, device="cuda")
+    kept[cut] = False
+    assert bool(torch.isfinite(lse[kept]).all())
+
+
+# -------------------------------------------------------------------- flags --
 @pytest.mark.parametrize("flag", [torch.zeros(1, dtype=torch.int32), torch.zeros(1, dtype=torch.int64),
                                   torch.zeros(0, dtype=torch.int32)])
 def test_flags_that_a_kernel_cannot_write_are_refused(flag):

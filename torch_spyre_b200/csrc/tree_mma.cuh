@@ -355,18 +355,41 @@ struct Walk {
   }
 };
 
+// Rows of q that no sequence has (all of them flagged): before the first
+// sequence's, past a sequence's nodes as they were clamped, after the last's.
+// They see nothing.  Every CTA takes some.
+__device__ __forceinline__ int rows_end(const Args &a, int b) {  // of sequence b and what follows it unclaimed
+  return b == a.batch - 1 ? a.total_q : min(max(__ldg(a.indptr + b + 1), 0), a.total_q);
+}
+template <typename T, int D, int kQ>
+__device__ __noinline__ void clear_rows(const Args &a) {
+  for (int b = 0; b < a.batch; ++b) {
+    const Seq s = load_seq<kQ>(a, b, false);
+    const int first = b == 0 ? 0 : s.q0, end = rows_end(a, b);
+    for (int t = first + blockIdx.x; t < end; t += gridDim.x) {
+      if (t >= s.q0 && t < s.q0 + s.nodes) continue;
+      uint4 *out = reinterpret_cast<uint4 *>(static_cast<T *>(a.out) + static_cast<int64_t>(t) * a.hq * D);
+      for (int i = threadIdx.x; i < a.hq * (D / 8); i += blockDim.x) out[i] = make_uint4(0, 0, 0, 0);
+      if (!a.lse) continue;
+      for (int h = threadIdx.x; h < a.hq; h += blockDim.x) a.lse[static_cast<int64_t>(t) * a.hq + h] = -CUDART_INF_F;
+    }
+  }
+}
+
 // The line's length, a share's, and where this CTA's begins; all threads of the
 // CTA call it, a barrier follows.  The counts fit 31 bits (the host checks).
-template <int kThreads, int kQ>
+template <typename T, int D, int kThreads, int kQ>
 __device__ __forceinline__ void make_plan(const Args &a, Ctrl &c) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int each = (a.batch + kThreads - 1) / kThreads;
   const int b0 = tid * each, b1 = min(b0 + each, a.batch);
   Seq s{};
   int mine = 0;
+  bool unclaimed = false;
   for (int b = b0; b < b1; ++b) {
     s = load_seq<kQ>(a, b, blockIdx.x == 0);
     mine += head_units<kQ>(a, s) * a.hkv;
+    unclaimed = unclaimed || (b == 0 && s.q0 > 0) || s.q0 + s.nodes < rows_end(a, b);
   }
   int incl = mine;
 #pragma unroll
@@ -375,7 +398,7 @@ __device__ __forceinline__ void make_plan(const Args &a, Ctrl &c) {
     if (lane >= m) incl += y;
   }
   if (lane == 31) c.scan[warp] = incl;
-  __syncthreads();
+  if (__syncthreads_or(unclaimed)) clear_rows<T, D, kQ>(a);
   int total = 0, before = 0;
 #pragma unroll
   for (int w = 0; w < kThreads / 32; ++w) {
@@ -1302,7 +1325,7 @@ __global__ void __launch_bounds__((Cfg<T, D, kCache>::kThreads), 1)
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (tid == 0) a.joins[blockIdx.x].nodes = 0;  // no block begins to be split here, unless the epilogue says so
-  make_plan<C::kThreads, C::kQ>(a, c);
+  make_plan<T, D, C::kThreads, C::kQ>(a, c);
   fence_before();
   __syncthreads();
   fence_after();
