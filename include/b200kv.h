@@ -671,7 +671,7 @@ B200KV_API int64_t b200kv_tree_workspace_bytes(int64_t total_q, int64_t batch, i
  * A node that sees nothing gives a zero row and lse = -inf.  Lengths outside
  * the block table or max_nodes are clamped and set B200KV_DEVERR_BAD_LEN, and
  * rows of q that no sequence has then are given as those of nodes that see
- * nothing; block ids outside the pool read as zeros and set B200KV_DEVERR_BAD_BLOCK.
+ * nothing (all rows, where q_indptr descends); block ids outside the pool read as zeros and set B200KV_DEVERR_BAD_BLOCK.
  * Supported: Hq / Hkv <= 128, batch <= 1024, D = 128 (64 in 16-bit pools),
  * total_q * Hq < 2^31, max_blocks_per_seq < 2^24 and
  * (batch + total_q * (Hq / Hkv) / 64 + 1) * Hkv * (2 * max_blocks_per_seq + 17) < 2^31. */

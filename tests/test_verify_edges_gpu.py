@@ -52,6 +52,7 @@ def attend_into(case, out, lse, context_lens=None, q_indptr=None, max_nodes=None
     (dict(context_lens=(100, 120)), range(20, 52)),
     (dict(q_indptr=(0, 12, 45)), range(45, 52)),
     (dict(q_indptr=(3, 12, 52)), range(0, 3)),
+    (dict(q_indptr=(0, 53, 52)), range(28, 52)),  # 100 committed tokens leave 28 of the two pages
 ])
 def test_rows_that_no_sequence_has_are_zero(cache, over, cut):
     case = TreeCase([100, 30], [12, 40], 8, 2, cache=cache, seed=19, poison=False)
@@ -63,6 +64,15 @@ def test_rows_that_no_sequence_has_are_zero(cache, over, cut):
     kept = torch.ones(52, dtype=torch.bool, device="cuda")
     kept[cut] = False
     assert bool(torch.isfinite(lse[kept]).all())
+
+
+@pytest.mark.parametrize("cache", [F16, I8])
+@pytest.mark.parametrize("indptr", [(0, 40, 12, 52), (52, 0, 0, 52), (0, 60, -3, 52), (0, 52, 0, 52)])
+def test_no_row_has_a_sequence_where_the_offsets_descend(cache, indptr):
+    case = TreeCase([100, 30, 7], [12, 30, 10], 8, 2, cache=cache, seed=19, poison=False)
+    out, lse = torch.full_like(case.q, math.nan), torch.full((52, 8), math.nan, device="cuda")
+    assert attend_into(case, out, lse, q_indptr=int32(*indptr), max_nodes=64) & _lib.DEVERR_BAD_LEN
+    assert bool((out == 0).all()) and bool((lse == -math.inf).all())
 
 
 # -------------------------------------------------------------------- flags --

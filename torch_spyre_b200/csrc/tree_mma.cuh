@@ -357,17 +357,17 @@ struct Walk {
 
 // Rows of q that no sequence has (all of them flagged): before the first
 // sequence's, past a sequence's nodes as they were clamped, after the last's.
-// They see nothing.  Every CTA takes some.
+// They see nothing.  Every CTA takes some.  `all`: no row has a sequence.
 __device__ __forceinline__ int rows_end(const Args &a, int b) {  // of sequence b and what follows it unclaimed
   return b == a.batch - 1 ? a.total_q : min(max(__ldg(a.indptr + b + 1), 0), a.total_q);
 }
 template <typename T, int D, int kQ>
-__device__ __noinline__ void clear_rows(const Args &a) {
+__device__ __noinline__ void clear_rows(const Args &a, bool all) {
   for (int b = 0; b < a.batch; ++b) {
     const Seq s = load_seq<kQ>(a, b, false);
-    const int first = b == 0 ? 0 : s.q0, end = rows_end(a, b);
+    const int first = b == 0 ? 0 : s.q0, end = all ? (b == 0 ? a.total_q : 0) : rows_end(a, b);
     for (int t = first + blockIdx.x; t < end; t += gridDim.x) {
-      if (t >= s.q0 && t < s.q0 + s.nodes) continue;
+      if (!all && t >= s.q0 && t < s.q0 + s.nodes) continue;
       uint4 *out = reinterpret_cast<uint4 *>(static_cast<T *>(a.out) + static_cast<int64_t>(t) * a.hq * D);
       for (int i = threadIdx.x; i < a.hq * (D / 8); i += blockDim.x) out[i] = make_uint4(0, 0, 0, 0);
       if (!a.lse) continue;
@@ -377,7 +377,9 @@ __device__ __noinline__ void clear_rows(const Args &a) {
 }
 
 // The line's length, a share's, and where this CTA's begins; all threads of the
-// CTA call it, a barrier follows.  The counts fit 31 bits (the host checks).
+// CTA call it, a barrier follows.  The counts fit 31 bits (the host checks) where
+// no two sequences have the same row: a q_indptr that descends could make them
+// anything, so then nothing has a sequence.
 template <typename T, int D, int kThreads, int kQ>
 __device__ __forceinline__ void make_plan(const Args &a, Ctrl &c) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -385,11 +387,13 @@ __device__ __forceinline__ void make_plan(const Args &a, Ctrl &c) {
   const int b0 = tid * each, b1 = min(b0 + each, a.batch);
   Seq s{};
   int mine = 0;
-  bool unclaimed = false;
+  bool unclaimed = false, descends = false;
   for (int b = b0; b < b1; ++b) {
     s = load_seq<kQ>(a, b, blockIdx.x == 0);
     mine += head_units<kQ>(a, s) * a.hkv;
-    unclaimed = unclaimed || (b == 0 && s.q0 > 0) || s.q0 + s.nodes < rows_end(a, b);
+    const int end = rows_end(a, b);
+    unclaimed = unclaimed || (b == 0 && s.q0 > 0) || s.q0 + s.nodes < end;
+    descends = descends || end < s.q0;
   }
   int incl = mine;
 #pragma unroll
@@ -398,13 +402,18 @@ __device__ __forceinline__ void make_plan(const Args &a, Ctrl &c) {
     if (lane >= m) incl += y;
   }
   if (lane == 31) c.scan[warp] = incl;
-  if (__syncthreads_or(unclaimed)) clear_rows<T, D, kQ>(a);
+  bool none = false;
+  if (__syncthreads_or(unclaimed || descends)) {
+    none = __syncthreads_or(descends);
+    clear_rows<T, D, kQ>(a, none);
+  }
   int total = 0, before = 0;
 #pragma unroll
   for (int w = 0; w < kThreads / 32; ++w) {
     if (w < warp) before += c.scan[w];
     total += c.scan[w];
   }
+  if (none) total = mine = 0;
   // (at least a step, so that a share inside a block holds the start of a tile)
   const int per = max(4, static_cast<int>((static_cast<unsigned>(total) + gridDim.x - 1) / gridDim.x));
   const int first = static_cast<int>(blockIdx.x) * per;
