@@ -40,7 +40,8 @@ def rotary_table(max_pos: int, rotary_dim: int, base: float = 10000.0, scaling: 
       unchanged, the slowest interpolated;
     * ``yarn`` -- pairs that turn more than ``beta_fast`` times over
       ``original_max_pos`` keep inv_i, those under ``beta_slow`` turns take
-      inv_i / factor, a linear ramp between them; cos and sin are multiplied by
+      inv_i / factor, a ramp linear in the pair's index (it may end past the
+      last pair) between them; cos and sin are multiplied by
       ``attention_factor`` (default 0.1 ln(factor) + 1).
 
     Angles are computed in fp64 and rounded once: at position 131071 an fp32
@@ -66,7 +67,7 @@ def rotary_table(max_pos: int, rotary_dim: int, base: float = 10000.0, scaling: 
         def pair_of(turns: float) -> float:  # the (real) pair index that turns this often over original_max_pos
             return rotary_dim * math.log(original_max_pos / (turns * 2.0 * math.pi)) / (2.0 * math.log(base))
 
-        lo, hi = max(math.floor(pair_of(beta_fast)), 0), min(math.ceil(pair_of(beta_slow)), half - 1)
+        lo, hi = max(math.floor(pair_of(beta_fast)), 0), min(math.ceil(pair_of(beta_slow)), rotary_dim - 1)
         ramp = ((i - lo) / max(hi - lo, 0.001)).clamp(0.0, 1.0)
         inv = inv * (1.0 - ramp) + inv / factor * ramp
         scale = 0.1 * math.log(factor) + 1.0
