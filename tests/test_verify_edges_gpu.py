@@ -8,6 +8,7 @@ import pytest
 import torch
 
 import torch_spyre_b200 as tsb
+from tests.test_verify_paths_gpu import Step, same
 from tests.verify_ref import TreeCase, make_cache
 from torch_spyre_b200 import _lib
 from torch_spyre_b200.rotations import DTYPE_CODES
@@ -222,3 +223,31 @@ def test_host_threads_share_a_stream():
 
     for got, one in zip(in_threads([lambda call=call, c=c: run(call, c) for call, c in work]), want):
         assert all(torch.equal(x, y) for pair in got for x, y in zip(pair, one))
+
+
+# ------------------------------------------------------------------ traces --
+def test_traced_calls_are_recorded():
+    first = Step()
+    first.public()
+
+    def run(step, q, k, v):
+        step.q, step.k, step.v = q, k, v
+        return step.public()
+
+    step = Step()
+    traced = torch.jit.trace(lambda q, k, v: run(step, q, k, v), (step.q, step.k, step.v), check_trace=False)
+    kinds = {n.kind() for n in traced.graph.nodes()}
+    assert {f"b200kv::{n}" for n in ("kv_store", "kv_load", "tree_mask", "tree_attention", "tree_commit", "rotary")} <= kinds
+    fresh = Step()
+    for t, s in ((step.kp, fresh.kp), (step.vp, fresh.vp), (step.ks, fresh.ks), (step.vs, fresh.vs)):
+        t.copy_(s)
+    assert same(traced(fresh.q, fresh.k, fresh.v), Step().public())
+
+
+def test_traced_gradient():
+    step = Step()
+    x = step.k.clone().requires_grad_(True)
+    traced = torch.jit.trace(lambda x: tsb.rotary(x, step.turn, step.pos), (x,), check_trace=False)
+    w = torch.randn_like(x)
+    assert torch.equal(torch.autograd.grad(traced(x), x, w)[0],
+                       torch.autograd.grad(tsb.rotary(x, step.turn, step.pos), x, w)[0])

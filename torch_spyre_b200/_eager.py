@@ -10,9 +10,9 @@ the verification operators take one of two shorter ways:
   operator wants it;
 * then the Python implementation runs directly (it raises for what is wrong).
 
-Under torch.compile, fake tensors, dispatch modes, functorch transforms, forward
-derivatives and for inputs that require a gradient they go through the registered
-operator, whose kernel is the same Python implementation (rotary has its gradient
+Under torch.compile, torch.jit.trace, fake tensors, dispatch modes, functorch
+transforms, forward derivatives and for inputs that require a gradient they go
+through the registered operator, whose kernel is the same Python implementation (rotary has its gradient
 in the shorter ways too).
 """
 
@@ -31,6 +31,7 @@ from . import _lib
 _PLAIN = (torch.Tensor, torch.nn.Parameter)
 _modes = torch._C._len_torch_dispatch_stack
 _interpreter = torch._C._functorch.peek_interpreter_stack
+_tracing = torch._C._get_tracing_state
 _stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 _device = getattr(torch._C, "_cuda_getDevice", None)
 compiling = torch.compiler.is_compiling
@@ -66,7 +67,7 @@ def plain(t: torch.Tensor) -> bool:
 
 def direct(*tensors) -> bool:
     """Whether a call on these tensors (None among them) may skip the dispatcher."""
-    if compiling() or _modes() or _interpreter() is not None or forward_ad._current_level >= 0:
+    if compiling() or _modes() or _interpreter() is not None or forward_ad._current_level >= 0 or _tracing() is not None:
         return False
     grad = torch.is_grad_enabled()
     return all(t is None or (plain(t) and not (grad and t.requires_grad)) for t in tensors)

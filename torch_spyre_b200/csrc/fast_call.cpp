@@ -73,8 +73,9 @@ struct Call {
 
   Call() {
     using c10::DispatchKey;
+    const c10::DispatchKeySet included = c10::impl::tls_local_dispatch_key_set().included_;
     ok = ok && !c10::impl::TorchDispatchModeTLS::any_modes_set() &&
-         !c10::impl::tls_local_dispatch_key_set().included_.has(DispatchKey::FuncTorchDynamicLayerFrontMode);
+         !included.has(DispatchKey::FuncTorchDynamicLayerFrontMode) && !included.has(DispatchKey::Tracer);
   }
   const at::Tensor *tensor(PyObject *o, bool with_grad = false) {
     if (!ok || !THPVariable_CheckExact(o)) {
