@@ -643,7 +643,7 @@ B200KV_API int b200kv_kv_load(const void *pool, int32_t pool_dtype, const float 
 /* Tree masks from parents: node i of sequence b (nodes q_indptr[b] ..
  * q_indptr[b + 1] - 1, indexes inside the sequence) sees itself and its
  * ancestors; parents[i] is -1 for a root, -2 for a pruned node, which sees
- * nothing, and less than i otherwise (else B200KV_DEVERR_BAD_LEN, and the walk
+ * nothing, nor do its descendants, and less than i otherwise (else B200KV_DEVERR_BAD_LEN, and the walk
  * ends there).  mask int64 [total_q, mask_words]: bit j % 64 of word j / 64. */
 B200KV_API int b200kv_tree_mask(const int32_t *parents, const int32_t *q_indptr, int64_t batch,
                                 int64_t total_q, int64_t mask_words, int64_t *mask,

@@ -97,6 +97,23 @@ def test_flags_that_a_kernel_cannot_write_are_refused(flag):
             call()
 
 
+# ------------------------------------------------------------------- masks --
+def test_descendants_of_a_pruned_node_see_nothing():
+    parents = [-1, -2, 1, 2, 0] + [-1] + list(range(5, 100)) + [70, -2]  # a second sequence of several mask words
+    parents = parents[:5] + [p if p < 0 else p - 5 for p in parents[5:]]
+    parents[5 + 66] = -2
+    flag = torch.zeros(1, dtype=torch.int32, device="cuda")
+    mask = tsb.tree_mask(int32(*parents), int32(0, 5, len(parents)), len(parents) - 5, error_flag=flag).cpu()
+    assert int(flag.item()) == 0
+    assert mask[:5].tolist() == [[1, 0], [0, 0], [0, 0], [0, 0], [17, 0]]
+    for i in range(len(parents) - 5):  # a chain as far as node 65, pruned from 66 on; then a child of node 65
+        want = [0, 0]
+        if i < 66 or parents[5 + i] == 65:
+            for j in list(range(min(i, 65) + 1)) + [i]:
+                want[j // 64] |= 1 << (j % 64)
+        assert [w & (2**64 - 1) for w in mask[5 + i].tolist()] == want, i
+
+
 # ------------------------------------------------------------------ commit --
 @pytest.mark.parametrize("cache", [F16, I8])
 @pytest.mark.parametrize("ctx", [0, 3, 100])

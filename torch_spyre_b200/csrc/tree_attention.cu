@@ -41,8 +41,11 @@ __global__ void __launch_bounds__(128) tree_mask_kernel(const int32_t *parents, 
     return;
   }
   int parent = __ldg(parents + i);
-  if (parent == -2) return;  // pruned: sees nothing
   for (;;) {
+    if (parent == -2) {  // pruned, itself or by an ancestor: sees nothing
+      for (int64_t w = 0; w < words; ++w) row[w] = 0;
+      return;
+    }
     row[j >> 6] |= uint64_t{1} << (j & 63);
     if (parent == -1) return;
     if (parent < 0 || parent >= j) {  // parents come before their children

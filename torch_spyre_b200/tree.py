@@ -72,7 +72,8 @@ def tree_mask(parents: torch.Tensor, q_indptr: torch.Tensor, max_nodes: int,
     """Mask bits int64 [N, ceil(max_nodes / 64)] of drafted trees: node i sees
     itself and its ancestors.  parents int32 [N] are indexes inside the node's
     own sequence (nodes q_indptr[b] .. q_indptr[b + 1] - 1), smaller than the
-    node's; -1 marks a root, -2 a pruned node, which sees nothing."""
+    node's; -1 marks a root, -2 a pruned node, which sees nothing, nor do the
+    nodes that descend from it."""
     args = (parents, q_indptr, max(1, -(-int(max_nodes) // 64)), error_flag)
     mask = None if _eager.compiling() else _eager.fast.tree_mask(*args)
     if mask is None:
