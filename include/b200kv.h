@@ -590,7 +590,9 @@ B200KV_API int b200kv_oproj_allreduce_f16(const void *attn, int64_t attn_stride_
  * Pools: 16-bit (fp16 or bf16) [num_blocks, Hkv, D/64, 64, 64] for D = 64 or
  * 128, or 8-bit (int8 or e4m3) [num_blocks, Hkv, 1, 64, 128] for D = 128 with
  * one fp32 scale per row, [num_blocks, Hkv, 64], not negative: element d of
- * token row t stands for value(d) * scale(t).  Pools, scales and contiguous
+ * token row t stands for value(d) * scale(t).  (Attention tells V's scales apart
+ * down to 2^-70 of the largest of their sequence and head; smaller ones may
+ * count as that.)  Pools, scales and contiguous
  * outputs are 16-byte aligned.
  * ------------------------------------------------------------------------ */
 

@@ -9,7 +9,7 @@ import torch
 
 import torch_spyre_b200 as tsb
 from tests.test_verify_paths_gpu import Step, same
-from tests.verify_ref import TreeCase, make_cache
+from tests.verify_ref import TreeCase, make_cache, unit_roundoff
 from torch_spyre_b200 import _lib
 from torch_spyre_b200.rotations import DTYPE_CODES
 
@@ -95,6 +95,51 @@ def test_flags_that_a_kernel_cannot_write_are_refused(flag):
                                          case.k_scales, case.v_scales, error_flag=flag)):
         with pytest.raises(ValueError, match="error_flag"):
             call()
+
+
+# ------------------------------------------------------------------ scales --
+def scaled_case(ctx, nodes, hq, hkv, cache, v_scales, seed=0):
+    """An 8-bit cache whose V rows have scales v_scales(number of rows)."""
+    case = TreeCase(ctx, nodes, hq, hkv, dtype=BF16, cache=cache, seed=seed)
+    for b, (c, t) in enumerate(zip(ctx, nodes)):
+        sl = case.slots(b, 0, c + t)
+        case.v_scales[sl // 64, :, sl % 64] = v_scales(c + t).float().cuda()[:, None].expand(-1, hkv)
+    return case
+
+
+def uniform(n):
+    return (torch.rand(n, generator=torch.Generator().manual_seed(n)) + 0.2) * 0.02
+
+
+RAMPS = {
+    "tiny": lambda n: uniform(n) * 2.0**-115,
+    "large": lambda n: uniform(n) * 2.0**100,
+    "tiny first": lambda n: uniform(n) * torch.where(torch.arange(n) < 200, 2.0**-116, 1.0),
+    "tiny last": lambda n: uniform(n) * torch.where(torch.arange(n) < n - 200, 1.0, 2.0**-80),
+    "rising": lambda n: uniform(n) * torch.exp2(-115.0 + 10.0 * (torch.arange(n) // 128).clamp(max=12)),
+    "zeros first": lambda n: uniform(n) * torch.where(torch.arange(n) < 200, 0.0, 2.0**-100),
+    "zeros between large": lambda n: uniform(n) * torch.where(torch.arange(n) % 2 == 0, 0.0, 2.0**30),
+    "all zero": lambda n: torch.zeros(n),
+}
+
+
+@pytest.mark.parametrize("cache", [I8, F8])
+@pytest.mark.parametrize("ramp", RAMPS)
+@pytest.mark.parametrize("ctx,nodes,hq,hkv", [([300, 5], [3, 1], 4, 2), ([1700, 64], [16, 9], 8, 2),
+                                              ([257, 40], [60, 40], 4, 1), ([9000], [11], 8, 1)])
+def test_scales_of_v_over_their_whole_range(cache, ramp, ctx, nodes, hq, hkv):
+    """The result is right relative to the rows' own size (the bound: rounding of out and of the weights), and the
+    lse does not know V at all."""
+    case = scaled_case(ctx, nodes, hq, hkv, cache, RAMPS[ramp])
+    flag = torch.zeros(1, dtype=torch.int32, device="cuda")
+    out, lse = tsb.tree_attention(*case.args(), **case.kwargs(), return_lse=True, error_flag=flag)
+    assert int(flag.item()) == 0
+    ref, ref_lse, spread = case.reference()
+    u = unit_roundoff(BF16)
+    bound = u * ref.abs() + (2 * u + 2.0**-17) * spread + 2.0**-133
+    err = (out.double() - ref).abs()
+    assert bool((err <= bound).all()), float((err / bound).max())
+    assert bool(((lse - ref_lse).abs() <= 2e-4 * (1 + ref_lse.abs())).all())
 
 
 # ------------------------------------------------------------------- masks --

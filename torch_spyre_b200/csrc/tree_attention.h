@@ -35,7 +35,7 @@ struct Args {
   int32_t *error_flag;
   Join *joins;      // [CTAs]
   float2 *part_ml;  // [2 * CTAs][256] (maximum in log2 units, sum)
-  float *part_o;    // [2 * CTAs][D / 4][256][4]
+  float *part_o;    // [2 * CTAs][D / 4][256][4] (8-bit caches: divided by the sum)
 };
 
 int launch_f16(const CUtensorMap &qm, const CUtensorMap &km, const CUtensorMap &vm, const Args &a, int dim, int cache,

@@ -116,6 +116,7 @@ struct Ctrl {
   int scan[32];
   unsigned bad_piece;       // last piece (counted from 1) that met a non-finite value in a node's V row
   float2 ml[2][kTileRows];  // (maximum, sum) of the streams' rows
+  float unit[2][4];         // 8-bit caches: what O counts in (see Factors), by stream and warp
 };
 // 8-bit caches: [8 warps][3][128] factors of a tile's tokens (see Factors), or,
 // when a block ends, [2 warpgroups][4][128] float4 of its rows' copies
@@ -837,13 +838,53 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
 // enter them as exact steps, and the weight that V's steps get is
 //   p v = 2^(k_factor s + log2 v) = 2^y,   y = s * (scale * log2(e) * k) + log2 v,
 // so the running maximum is that of y, and the softmax's own sum takes 2^y / v.
-// Scales below 1e-30 count as that: their rows stay zero to any purpose.
+// Scales may be any normal number, and 2^y / v has to stay one: v is taken in
+// units of a power of two, so O counts in it too, and m and l do not depend on it.
+// The unit is 1 if the scales of a warp's first tile are within 2^-20 .. 2^30 (no
+// tile of such a cache needs more than a look at its scales), else the power of the
+// largest of them, and follows when scales 2^30 times as large come up (O with it).
+// In that unit
+//   a row of zeros (v = 0) weighs in the sum alone: v = 2^-60, small enough not
+//     to move the maximum and large enough for 2^(y - m) to stay normal for
+//     whatever matters in the sum;
+//   others below 2^-90 count as that, next to rows more than 2^70 times their size.
 struct Factors {
   float4 k[kTileTokens / 4], log2v[kTileTokens / 4], inv_v[kTileTokens / 4];
 };
-__device__ __forceinline__ float floor_scale(float v) { return v < 1e-30f ? 1e-30f : v; }
-// (a NaN scale makes 2^y NaN where the token is seen; 0 / v must stay 0 where not)
-__device__ __forceinline__ float inv_scale(float v) { return v < CUDART_INF_F ? 1.f / v : 1.f; }
+constexpr uint32_t kExp = 1u << 23;  // of a float's exponent
+constexpr uint32_t kMostUnits = 157u * kExp, kLeastUnits = 37u * kExp, kLeastFirst = 107u * kExp;  // 2^30, 2^-90, 2^-20
+__device__ __forceinline__ float inverse_of_power(float x) { return __uint_as_float(254u * kExp - __float_as_uint(x)); }
+// Whether a lane's four scales, in units, are positive numbers within the bounds
+// (compared as integers: NaN, inf and negative numbers are above all others).
+__device__ __forceinline__ bool ordinary(float4 u, uint32_t least) {
+  const uint32_t x = __float_as_uint(u.x), y = __float_as_uint(u.y), z = __float_as_uint(u.z), w = __float_as_uint(u.w);
+  return max(max(x, y), max(z, w)) <= kMostUnits && min(min(x, y), min(z, w)) >= least;
+}
+__device__ __forceinline__ void put_v(Factors *fac, float4 u) {
+  const int lane = threadIdx.x & 31;
+  fac->log2v[lane] = make_float4(__log2f(u.x), __log2f(u.y), __log2f(u.z), __log2f(u.w));
+  fac->inv_v[lane] = make_float4(__fdividef(1.f, u.x), __fdividef(1.f, u.y), __fdividef(1.f, u.z), __fdividef(1.f, u.w));
+}
+// V's factors of a tile whose scales are not all ordinary in units of 1 / per, four to a lane (`have`: so many of
+// them are of the sequence's rows).  Returns 1 / unit from this tile on, 0 as long as all rows were zero.
+static __device__ __noinline__ float odd_scales(Factors *fac, float4 v, int have, float per) {
+  auto of = [&](float x, int i) { return i < have && x > 0.f && x < CUDART_INF_F ? x : 0.f; };
+  const float mine = fmaxf(fmaxf(of(v.x, 0), of(v.y, 1)), fmaxf(of(v.z, 2), of(v.w, 3)));
+  const uint32_t largest = __reduce_max_sync(0xffffffffu, __float_as_uint(mine));
+  if (largest != 0 && (per == 0.f || __uint_as_float(largest) * per > __uint_as_float(kMostUnits)))
+    // (bounds that keep a row's sum and its inverse, times the unit, normal)
+    per = inverse_of_power(__uint_as_float(min(max(largest & (255u * kExp), 27u * kExp), 217u * kExp)));  // 2^-100, 2^90
+  auto in_units = [&](float x) {
+    const float u = x * (per == 0.f ? 1.f : per);
+    return x == 0.f ? 8.67361738e-19f : u < __uint_as_float(kLeastUnits) ? __uint_as_float(kLeastUnits) : u;
+  };
+  const float4 u = make_float4(in_units(v.x), in_units(v.y), in_units(v.z), in_units(v.w));
+  put_v(fac, u);
+  // (a NaN scale makes 2^y NaN where the token is seen; 0 / v must stay 0 where not)
+  auto inv = [](float x) { return x < CUDART_INF_F ? 1.f / x : 1.f; };
+  fac->inv_v[threadIdx.x & 31] = make_float4(inv(u.x), inv(u.y), inv(u.z), inv(u.w));
+  return per;
+}
 
 // Moves the running maximum when a row's has risen far enough, O and l with it.
 template <int D>
@@ -863,6 +904,20 @@ __device__ __forceinline__ void follow(uint32_t to, float mt, bool first, bool l
     }
   }
   if (rise) m = mt;
+}
+
+template <int D>
+__device__ __noinline__ void rescale(uint32_t to, float by) {
+#pragma unroll 1
+  for (int i = 0; i < D; i += 16) {
+    uint32_t r[16];
+    tmem_ld16(to + i, r);
+    wait_ld(r);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * by);
+    tmem_st16(to + i, r);
+  }
+  wait_st();
 }
 
 template <bool kTail>
@@ -1059,11 +1114,13 @@ __device__ __forceinline__ void softmax(const Args &a, Ctrl &c, uint8_t *smem, u
     // tokens before this one are seen by every row of the Q tile
     const int common = wk.s.ctx + (a.mask ? 0 : qt * a.tile_nodes + 1);
     float m = -CUDART_INF_F, l = 0.f;
+    float per = 1.f;  // 8-bit caches: the inverse of what O counts in, 0 as long as all rows were zero
     // 8-bit caches: the scales of this stream's next tile, four tokens per lane
     auto scales_of = [&](int t, float4 &k, float4 &v) {
       const int page = 2 * t + (lane >> 4);
-      k = v = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (page * kPageTokens >= len) return;
+      k = make_float4(0.f, 0.f, 0.f, 0.f), v = make_float4(1.f, 1.f, 1.f, 1.f);
+      if (page * kPageTokens >= len) return;  // (what is past the end weighs nothing, and 1 is an ordinary scale)
+      v = k;
       const int id = __ldg(a.block_table + static_cast<int64_t>(wk.b) * a.bt_stride + page);
       if (id < 0 || id >= a.num_blocks) return;
       const int64_t at = (static_cast<int64_t>(id) * a.hkv + wk.kvh) * kPageTokens;
@@ -1083,18 +1140,25 @@ __device__ __forceinline__ void softmax(const Args &a, Ctrl &c, uint8_t *smem, u
         for (int i = 0; i < 4; ++i)
           if (i < 4 / q.copies) vis[i] = visible32(a, wk.s, node, pos + copy * q.rows + 32 * i);
       }
+      float regain = 1.f;  // the factor that O takes when its unit moves
       if (C::k8 && warp_live) {
+        const float4 u = make_float4(vs.x * per, vs.y * per, vs.z * per, vs.w * per);
         __syncwarp();
         fac->k[lane] = make_float4(ks.x * cl, ks.y * cl, ks.z * cl, ks.w * cl);
-        vs = make_float4(floor_scale(vs.x), floor_scale(vs.y), floor_scale(vs.z), floor_scale(vs.w));
-        fac->log2v[lane] = make_float4(__log2f(vs.x), __log2f(vs.y), __log2f(vs.z), __log2f(vs.w));
-        fac->inv_v[lane] = make_float4(inv_scale(vs.x), inv_scale(vs.y), inv_scale(vs.z), inv_scale(vs.w));
+        if (__all_sync(0xffffffffu, ordinary(u, t == tfirst ? kLeastFirst : kLeastUnits))) {
+          put_v(fac, u);
+        } else {
+          const float now = odd_scales(fac, vs, len - pos - 4 * lane, t == tfirst ? 0.f : per);
+          if (now != per && t != tfirst) regain = per == 0.f ? 0.f : now * inverse_of_power(per);
+          per = now;
+        }
         if (t + step < wk.t1) scales_of(t + step, ks, vs);
         __syncwarp();
       }
       auto arrived = [&] {
         wait(&c.s_full[w], s_uses++ & 1u, dead, a.error_flag);
         fence_after();
+        if (C::k8 && regain != 1.f) rescale<D>(to, regain);
       };
       if (!C::k8 || !warp_live) arrived();
       if (warp_live) {
@@ -1153,7 +1217,7 @@ __device__ __forceinline__ void softmax(const Args &a, Ctrl &c, uint8_t *smem, u
       wait(&c.o_full[k], o_uses[k]++ & 1u, dead, a.error_flag);
       fence_after();
     };
-    float keep0 = 1.f, keep1 = 0.f;
+    float keep0 = 1.f, keep1 = 0.f, unit = 0.f;
     const bool both = !two && n > 1;
     int d0 = 0, d1 = D;
     if (two) {
@@ -1161,6 +1225,7 @@ __device__ __forceinline__ void softmax(const Args &a, Ctrl &c, uint8_t *smem, u
       ++o_uses[1 - w];
     } else {
       c.ml[w][tid] = make_float2(m, l);
+      if (C::k8 && lane == 0) c.unit[w][warp] = per == 0.f || tfirst >= wk.t1 || !warp_live ? 0.f : inverse_of_power(per);
       o_wait(0);
       if (both) o_wait(1);
       bar_pair();
@@ -1173,6 +1238,13 @@ __device__ __forceinline__ void softmax(const Args &a, Ctrl &c, uint8_t *smem, u
       const float mm = m == -CUDART_INF_F ? 0.f : m;
       keep0 = ex2(x.x - mm);
       keep1 = ex2(y.x - mm);
+      if (C::k8) {  // O of both, and of the row's copies, in the largest of their units
+#pragma unroll
+        for (int k = 0; k < 4; ++k) unit = fmaxf(unit, fmaxf(c.unit[0][k], c.unit[1][k]));
+        const float per_unit = unit > 0.f ? inverse_of_power(unit) : 0.f;
+        keep0 *= c.unit[0][warp] * per_unit;
+        keep1 *= c.unit[1][warp] * per_unit;
+      }
       l = 0.f;
       for (int k = 0; k < q.copies; ++k) {
         const float2 xk = c.ml[0][row + k * q.rows], yk = c.ml[1][row + k * q.rows];
@@ -1183,7 +1255,8 @@ __device__ __forceinline__ void softmax(const Args &a, Ctrl &c, uint8_t *smem, u
       d1 = d0 + D / 2;
     }
     const int64_t orow = static_cast<int64_t>(wk.s.q0 + node) * a.hq + wk.kvh * a.group + row % a.group;
-    const float inv = l == 0.f ? 0.f : 1.f / l;
+    float inv = l == 0.f ? 0.f : 1.f / l;
+    if (C::k8) inv *= unit;
     const int prow = (two ? w : 0) * kTileRows + row;
     if (C::k8 && q.copies > 1) {
       // add the copies up, 16 columns at a time through shared memory
@@ -1214,14 +1287,13 @@ __device__ __forceinline__ void softmax(const Args &a, Ctrl &c, uint8_t *smem, u
             o = make_float4(o.x + x.x, o.y + x.y, o.z + x.z, o.w + x.w);
           }
           const int dj = d + 4 * j;
-          if (split) {
+          const bool none = l == 0.f;
+          o = none ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+          if (split)
             *reinterpret_cast<float4 *>(a.part_o + ((static_cast<int64_t>(pslot) * (D / 4) + dj / 4) * 256 + prow) * 4) = o;
-          } else {
-            const bool none = l == 0.f;
+          else
             *reinterpret_cast<uint2 *>(static_cast<T *>(a.out) + orow * D + dj) =
-                none ? make_uint2(0u, 0u)
-                     : make_uint2(pack2(o.x * inv, o.y * inv, T()), pack2(o.z * inv, o.w * inv, T()));
-          }
+                make_uint2(pack2(o.x, o.y, T()), pack2(o.z, o.w, T()));
         }
         bar_group(w);
       }
@@ -1245,6 +1317,11 @@ __device__ __forceinline__ void softmax(const Args &a, Ctrl &c, uint8_t *smem, u
               r[j] = __float_as_uint(fmaf(__uint_as_float(r1[j]), keep1, __uint_as_float(r[j])));
           }
         }
+        const bool none = l == 0.f;
+        if (C::k8 && split) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) r[j] = none ? 0u : __float_as_uint(__uint_as_float(r[j]) * inv);
+        }
         if (live && split) {
 #pragma unroll
           for (int j = 0; j < 4; ++j)
@@ -1252,7 +1329,6 @@ __device__ __forceinline__ void softmax(const Args &a, Ctrl &c, uint8_t *smem, u
                 make_uint4(r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
         } else if (live) {
           T *out = static_cast<T *>(a.out) + orow * D + d;
-          const bool none = l == 0.f;
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
             float f[8];
@@ -1365,9 +1441,10 @@ __global__ void __launch_bounds__((Cfg<T, D, kCache>::kThreads), 1)
 
 // ------------------------------------------------------------------- join --
 // Blocks cut by CTA boundaries: out = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i
-// over the pieces in order (the same bits every time).  One CTA per boundary and
-// 32 rows; lane = row, warp = an eighth of the head.
-template <typename T, int D>
+// over the pieces in order (the same bits every time).  The pieces of an 8-bit
+// cache have units of their own and come divided by their l (kDivided).  One CTA
+// per boundary and 32 rows; lane = row, warp = an eighth of the head.
+template <typename T, int D, bool kDivided>
 __global__ void __launch_bounds__(256) tree_join_kernel(const __grid_constant__ Args a) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -1410,12 +1487,13 @@ __global__ void __launch_bounds__(256) tree_join_kernel(const __grid_constant__ 
     for (int k = 0; k < kAhead; ++k) {
       const float keep = exp2f(ml[k].x - mm);
       l = fmaf(ml[k].y, keep, l);
+      const float weight = kDivided ? ml[k].y * keep : keep;
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
-        o[4 * i] = fmaf(v[k][i].x, keep, o[4 * i]);
-        o[4 * i + 1] = fmaf(v[k][i].y, keep, o[4 * i + 1]);
-        o[4 * i + 2] = fmaf(v[k][i].z, keep, o[4 * i + 2]);
-        o[4 * i + 3] = fmaf(v[k][i].w, keep, o[4 * i + 3]);
+        o[4 * i] = fmaf(v[k][i].x, weight, o[4 * i]);
+        o[4 * i + 1] = fmaf(v[k][i].y, weight, o[4 * i + 1]);
+        o[4 * i + 2] = fmaf(v[k][i].z, weight, o[4 * i + 2]);
+        o[4 * i + 3] = fmaf(v[k][i].w, weight, o[4 * i + 3]);
       }
     }
   }
@@ -1458,7 +1536,7 @@ int launch(const CUtensorMap &qm, const CUtensorMap &km, const CUtensorMap &vm, 
   cfg.gridDim = dim3(static_cast<unsigned>(ctas), C::kQ == 2 && a.max_nodes > a.tile_nodes ? 8 : 4);
   cfg.blockDim = dim3(256);
   cfg.dynamicSmemBytes = 0;
-  B200KV_CUDA_TRY(cudaLaunchKernelEx(&cfg, tree_join_kernel<T, D>, a));
+  B200KV_CUDA_TRY(cudaLaunchKernelEx(&cfg, tree_join_kernel<T, D, C::k8>, a));
   return B200KV_OK;
 }
 
