@@ -142,6 +142,22 @@ def test_scales_of_v_over_their_whole_range(cache, ramp, ctx, nodes, hq, hkv):
     assert bool(((lse - ref_lse).abs() <= 2e-4 * (1 + ref_lse.abs())).all())
 
 
+@pytest.mark.parametrize("cache", [I8, F8])
+@pytest.mark.parametrize("nodes,hq", [(3, 4), (12, 8), (60, 4)])
+@pytest.mark.parametrize("where", ["committed", "node"])
+def test_a_nan_v_row_leaves_the_lse(cache, nodes, hq, where):
+    case = TreeCase([1000, 40], [nodes, 2], hq, 2, cache=cache, seed=23)
+    at = 700 if where == "committed" else 1000 + nodes // 2
+    sl = case.slots(0, at, at + 1)[0]
+    case.v_scales[sl // 64, :, sl % 64] = math.nan
+    out, lse = tsb.tree_attention(*case.args(), **case.kwargs(), return_lse=True)
+    _, ref_lse, _ = case.reference()
+    sees = torch.ones(nodes, dtype=torch.bool) if where == "committed" else case.see[0][:, nodes // 2]
+    sees = torch.cat([sees, torch.zeros(2, dtype=torch.bool)]).cuda()
+    assert bool(torch.isnan(out[sees]).all()) and bool(torch.isfinite(out[~sees]).all())
+    assert bool(((lse - ref_lse).abs() <= 2e-4 * (1 + ref_lse.abs())).all())
+
+
 # ------------------------------------------------------------------- masks --
 def test_descendants_of_a_pruned_node_see_nothing():
     parents = [-1, -2, 1, 2, 0] + [-1] + list(range(5, 100)) + [70, -2]  # a second sequence of several mask words

@@ -117,6 +117,7 @@ struct Ctrl {
   unsigned bad_piece;       // last piece (counted from 1) that met a non-finite value in a node's V row
   float2 ml[2][kTileRows];  // (maximum, sum) of the streams' rows
   float unit[2][4];         // 8-bit caches: what O counts in (see Factors), by stream and warp
+  unsigned spoilt_piece;    // last piece (counted from 1) that met a V scale that is not finite
 };
 // 8-bit caches: [8 warps][3][128] factors of a tile's tokens (see Factors), or,
 // when a block ends, [2 warpgroups][4][128] float4 of its rows' copies
@@ -865,9 +866,14 @@ __device__ __forceinline__ void put_v(Factors *fac, float4 u) {
   fac->log2v[lane] = make_float4(__log2f(u.x), __log2f(u.y), __log2f(u.z), __log2f(u.w));
   fac->inv_v[lane] = make_float4(__fdividef(1.f, u.x), __fdividef(1.f, u.y), __fdividef(1.f, u.z), __fdividef(1.f, u.w));
 }
-// V's factors of a tile whose scales are not all ordinary in units of 1 / per, four to a lane (`have`: so many of
-// them are of the sequence's rows).  Returns 1 / unit from this tile on, 0 as long as all rows were zero.
-static __device__ __noinline__ float odd_scales(Factors *fac, float4 v, int have, float per) {
+// V's factors of a tile whose scales are not all ordinary in units of 1 / per, four
+// to a lane (`have`: so many of them are of the sequence's rows).  Returns 1 / unit
+// from this tile on, 0 as long as all rows were zero.
+// A scale that is not finite makes NaN of whoever sees its row (see sees_spoilt), but
+// not of the sums, which go by K alone: the row weighs as one of zeros.
+static __device__ __noinline__ float odd_scales(Factors *fac, float4 v, int have, float per, unsigned piece,
+                                                unsigned *spoilt_piece) {
+  const int lane = threadIdx.x & 31;
   auto of = [&](float x, int i) { return i < have && x > 0.f && x < CUDART_INF_F ? x : 0.f; };
   const float mine = fmaxf(fmaxf(of(v.x, 0), of(v.y, 1)), fmaxf(of(v.z, 2), of(v.w, 3)));
   const uint32_t largest = __reduce_max_sync(0xffffffffu, __float_as_uint(mine));
@@ -876,13 +882,11 @@ static __device__ __noinline__ float odd_scales(Factors *fac, float4 v, int have
     per = inverse_of_power(__uint_as_float(min(max(largest & (255u * kExp), 27u * kExp), 217u * kExp)));  // 2^-100, 2^90
   auto in_units = [&](float x) {
     const float u = x * (per == 0.f ? 1.f : per);
-    return x == 0.f ? 8.67361738e-19f : u < __uint_as_float(kLeastUnits) ? __uint_as_float(kLeastUnits) : u;
+    return x == 0.f || !(x < CUDART_INF_F) ? 8.67361738e-19f : u < __uint_as_float(kLeastUnits) ? __uint_as_float(kLeastUnits) : u;
   };
-  const float4 u = make_float4(in_units(v.x), in_units(v.y), in_units(v.z), in_units(v.w));
-  put_v(fac, u);
-  // (a NaN scale makes 2^y NaN where the token is seen; 0 / v must stay 0 where not)
-  auto inv = [](float x) { return x < CUDART_INF_F ? 1.f / x : 1.f; };
-  fac->inv_v[threadIdx.x & 31] = make_float4(inv(u.x), inv(u.y), inv(u.z), inv(u.w));
+  put_v(fac, make_float4(in_units(v.x), in_units(v.y), in_units(v.z), in_units(v.w)));
+  auto spoilt = [&](float x, int i) { return i < have && !(x < CUDART_INF_F); };
+  if (spoilt(v.x, 0) || spoilt(v.y, 1) || spoilt(v.z, 2) || spoilt(v.w, 3)) *spoilt_piece = piece;
   return per;
 }
 
@@ -1065,6 +1069,28 @@ __device__ float cached_v(const Args &a, const void *pool, int id, int kvh, int 
   else
     return __half2float(__half(__nv_cvt_fp8_to_halfraw(static_cast<const uint8_t *>(pool)[at], __NV_E4M3)));
 }
+// Whether row `node` (-1: none) sees a V row whose scale is not finite, in tiles [t0, t1); the whole warp calls it.
+static __device__ __noinline__ bool sees_spoilt(const Args &a, const Seq s, int b, int kvh, int node, int t0, int t1) {
+  const int lane = threadIdx.x & 31;
+  bool sees = false;
+  for (int t = t0; t < t1; ++t) {
+    const int page = 2 * t + (lane >> 4), have = s.ctx + s.nodes - t * kTileTokens - 4 * lane;
+    const int id = have > 0 ? __ldg(a.block_table + static_cast<int64_t>(b) * a.bt_stride + page) : -1;
+    uint32_t bad = 0;
+    if (id >= 0 && id < a.num_blocks) {
+      const float4 v = __ldg(reinterpret_cast<const float4 *>(
+                                 a.v_scales + (static_cast<int64_t>(id) * a.hkv + kvh) * kPageTokens) + (lane & 15));
+      auto bit = [&](float x, int i) { return i < have && !(x < CUDART_INF_F) ? 1u << i : 0u; };
+      bad = bit(v.x, 0) | bit(v.y, 1) | bit(v.z, 2) | bit(v.w, 3);
+    }
+    if (!__any_sync(0xffffffffu, bad != 0)) continue;
+    for (int g = 0; g < 4; ++g) {
+      const uint32_t word = __reduce_or_sync(0xffffffffu, lane / 8 == g ? bad << (4 * (lane & 7)) : 0u);
+      if (node >= 0 && (word & visible32(a, s, node, t * kTileTokens + 32 * g))) sees = true;
+    }
+  }
+  return sees;
+}
 // Adds the non-finite elements of the piece's visible nodes to elements
 // [d0, d1) of a row that has been written, to its partial sums or its output.
 template <typename T, int D, int kCache>
@@ -1148,7 +1174,7 @@ __device__ __forceinline__ void softmax(const Args &a, Ctrl &c, uint8_t *smem, u
         if (__all_sync(0xffffffffu, ordinary(u, t == tfirst ? kLeastFirst : kLeastUnits))) {
           put_v(fac, u);
         } else {
-          const float now = odd_scales(fac, vs, len - pos - 4 * lane, t == tfirst ? 0.f : per);
+          const float now = odd_scales(fac, vs, len - pos - 4 * lane, t == tfirst ? 0.f : per, piece, &c.spoilt_piece);
           if (now != per && t != tfirst) regain = per == 0.f ? 0.f : now * inverse_of_power(per);
           per = now;
         }
@@ -1256,7 +1282,12 @@ __device__ __forceinline__ void softmax(const Args &a, Ctrl &c, uint8_t *smem, u
     }
     const int64_t orow = static_cast<int64_t>(wk.s.q0 + node) * a.hq + wk.kvh * a.group + row % a.group;
     float inv = l == 0.f ? 0.f : 1.f / l;
-    if (C::k8) inv *= unit;
+    if (C::k8) {
+      inv *= unit;
+      if (*reinterpret_cast<volatile unsigned *>(&c.spoilt_piece) == piece &&
+          sees_spoilt(a, wk.s, wk.b, wk.kvh, live ? node : -1, wk.t0, wk.t1))
+        inv = CUDART_NAN_F;
+    }
     const int prow = (two ? w : 0) * kTileRows + row;
     if (C::k8 && q.copies > 1) {
       // add the copies up, 16 columns at a time through shared memory
@@ -1399,7 +1430,7 @@ __global__ void __launch_bounds__((Cfg<T, D, kCache>::kThreads), 1)
       mbar_init(&c.o_full[w], 1);
     }
     fence_mbar_init();
-    c.bad_piece = 0;
+    c.bad_piece = c.spoilt_piece = 0;
   }
   if (warp == 9) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&c.tmem)),
