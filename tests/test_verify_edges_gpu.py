@@ -158,6 +158,39 @@ def test_a_nan_v_row_leaves_the_lse(cache, nodes, hq, where):
     assert bool(((lse - ref_lse).abs() <= 2e-4 * (1 + ref_lse.abs())).all())
 
 
+# ------------------------------------------------------------------- pages --
+@pytest.mark.parametrize("cache", [F16, I8, F8])
+@pytest.mark.parametrize("bad", [-1, -(1 << 31), 1 << 20])
+@pytest.mark.parametrize("ctx,at", [([700, 30], 3), ([9000, 64], 64), ([40, 5], 0)])
+def test_a_page_outside_the_pool_reads_as_zeros(cache, bad, ctx, at):
+    """The same bits as with a page of zeros in its place, whatever the pool's first page holds."""
+    case = TreeCase(ctx, [9, 2], 8, 2, cache=cache, seed=29)
+    zeros = int((set(range(case.k_pool.shape[0])) - set(case.block_table.flatten().tolist()) - {0}).pop())
+    if (case.block_table == 0).any():  # page 0 moves to a free place, so that no sequence has it
+        free = int((set(range(case.k_pool.shape[0])) - set(case.block_table.flatten().tolist()) - {0, zeros}).pop())
+        case.block_table[case.block_table == 0] = free
+    else:
+        free = zeros
+    for pool, scales in ((case.k_pool, case.k_scales), (case.v_pool, case.v_scales)):
+        raw = pool.view(torch.uint8)
+        if free != zeros:
+            raw[free] = raw[0]
+            if scales is not None:
+                scales[free] = scales[0]
+        raw[0], raw[zeros] = 0x7F, 0  # NaN in e4m3 and fp16
+        if scales is not None:
+            scales[0], scales[zeros] = 1.0, 0.0
+    table = case.block_table.clone()
+    case.block_table[0, at] = zeros
+    want = tsb.tree_attention(*case.args(), **case.kwargs(), return_lse=True)
+    assert all(bool(torch.isfinite(x).all()) for x in want)
+    table[0, at] = bad
+    case.block_table = table
+    flag = torch.zeros(1, dtype=torch.int32, device="cuda")
+    got = tsb.tree_attention(*case.args(), **case.kwargs(), return_lse=True, error_flag=flag)
+    assert int(flag.item()) == _lib.DEVERR_BAD_BLOCK and all(torch.equal(x, y) for x, y in zip(got, want))
+
+
 # ------------------------------------------------------------------- masks --
 def test_descendants_of_a_pruned_node_see_nothing():
     parents = [-1, -2, 1, 2, 0] + [-1] + list(range(5, 100)) + [70, -2]  # a second sequence of several mask words

@@ -467,6 +467,15 @@ __device__ __forceinline__ void tma_3d(void *dst, const CUtensorMap *map, uint64
       : "memory");
 }
 
+// The pages of a raw tile that are not among `valid`; the whole warp calls it.
+static __device__ __noinline__ void zero_pages(uint8_t *tile, uint32_t valid) {
+  uint4 *at = reinterpret_cast<uint4 *>(tile);
+  for (int i = threadIdx.x & 31; i < 2 * kPageTokens * 8; i += 32)
+    if (!(valid >> (i / (kPageTokens * 8)) & 1u)) at[i] = make_uint4(0, 0, 0, 0);
+  fence_async_smem();
+  __syncwarp();
+}
+
 // ------------------------------------------------------------------ roles --
 template <typename C>
 __device__ __forceinline__ void producer(const Args &a, Ctrl &c, uint8_t *smem, const CUtensorMap *qm,
@@ -535,12 +544,13 @@ __device__ __forceinline__ void producer(const Args &a, Ctrl &c, uint8_t *smem, 
       } else {
         const uint32_t r = ring % C::kRaw;
         wait(&c.raw_empty[r], ((ring / C::kRaw) & 1u) ^ 1u, dead, a.error_flag);
-        if (lane == 0) mbar_arrive_expect_tx(&c.raw_full[r], uint32_t(n) * (kPageTokens * 128));
+        // a page is one contiguous run; one with an invalid id is written as zeros
+        const uint32_t valid = __ballot_sync(0xffffffffu, at < n && id >= 0);
+        if (valid != (1u << n) - 1u) zero_pages(smem + C::kOffRaw + r * C::kRawTile, valid);
+        if (lane == 0) mbar_arrive_expect_tx(&c.raw_full[r], __popc(valid) * (kPageTokens * 128));
         __syncwarp();
-        // a page is one contiguous run; an invalid id reads page 0, and scales
-        // of zero make zeros of it
-        const int64_t page = id < 0 ? 0 : id * a.hkv + w.kvh;
-        if (at < n)
+        const int64_t page = id * a.hkv + w.kvh;
+        if (at < n && id >= 0)
           bulk_load(smem + C::kOffRaw + r * C::kRawTile + at * (kPageTokens * 128),
                     static_cast<const uint8_t *>(is_v ? a.v_pool : a.k_pool) + page * (kPageTokens * 128),
                     kPageTokens * 128, &c.raw_full[r]);
