@@ -61,25 +61,22 @@ __global__ void __launch_bounds__(128) tree_mask_kernel(const int32_t *parents, 
 constexpr int kBoxElems = 64;  // 16-bit elements of a 128-byte operand row
 
 int encode(CUtensorMap *map, CUtensorMapDataType type, const void *base, const cuuint64_t (&dims)[3],
-           const cuuint64_t (&strides)[2], const cuuint32_t (&box)[3], CUtensorMapSwizzle swizzle) {
+           const cuuint64_t (&strides)[2], const cuuint32_t (&box)[3]) {
   EncodeTiledFn enc = encode_tiled_fn();
   if (!enc) return set_error(B200KV_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
   const cuuint32_t estr[3] = {1, 1, 1};
   const CUresult r = enc(map, type, 3, const_cast<void *>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                         swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return set_error(B200KV_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", static_cast<int>(r));
   return B200KV_OK;
 }
 
-// Pages of a pool, one box per page and 64-element stick column (16-bit: into
-// the 128-byte swizzle of an operand tile) or per page (8-bit: as it is).
-int pool_map(CUtensorMap *map, const void *pool, int64_t pages, int64_t dim, bool k8, CUtensorMapDataType type) {
-  const cuuint64_t stick = k8 ? 128 : 64, rows = k8 ? kPageTokens : dim / 64 * kPageTokens;
-  const cuuint64_t dims[3] = {stick, rows, static_cast<cuuint64_t>(pages)};
-  const cuuint64_t strides[2] = {128, rows * 128};
-  const cuuint32_t box[3] = {static_cast<cuuint32_t>(stick), kPageTokens, 1};
-  return encode(map, k8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : type, pool, dims, strides, box,
-                k8 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B);
+// Pages of a 16-bit pool, one box per page and 64-element stick column, into the
+// 128-byte swizzle of an operand tile.  (8-bit pages come by plain bulk copies.)
+int pool_map(CUtensorMap *map, const void *pool, int64_t pages, int64_t dim, CUtensorMapDataType type) {
+  const cuuint64_t rows = dim / kBoxElems * kPageTokens;
+  return encode(map, type, pool, {kBoxElems, rows, static_cast<cuuint64_t>(pages)}, {128, rows * 128},
+                {kBoxElems, kPageTokens, 1});
 }
 
 struct Workspace {
@@ -208,18 +205,20 @@ extern "C" int b200kv_tree_attention(const void *q, int32_t q_dtype, int64_t q_s
   const int64_t box_nodes = a.small_boxes ? 32 / group : (max_nodes < a.tile_nodes ? max_nodes : a.tile_nodes);
   a.box_nodes = static_cast<int>(box_nodes);
   a.q_box_bytes = static_cast<uint32_t>(box_nodes * group * 128);
-  CUtensorMap qm, km, vm;
+  CUtensorMap qm, km{}, vm{};
   // a dimension of one element may have any stride
   const int64_t qs_h = num_q_heads == 1 ? head_dim : q_stride_h, qs_t = total_q == 1 ? num_q_heads * head_dim : q_stride_t;
   st = encode(&qm, type, q,
               {static_cast<cuuint64_t>(head_dim), static_cast<cuuint64_t>(num_q_heads), static_cast<cuuint64_t>(total_q)},
               {static_cast<cuuint64_t>(qs_h * 2), static_cast<cuuint64_t>(qs_t * 2)},
-              {kBoxElems, static_cast<cuuint32_t>(group), static_cast<cuuint32_t>(box_nodes)}, CU_TENSOR_MAP_SWIZZLE_128B);
+              {kBoxElems, static_cast<cuuint32_t>(group), static_cast<cuuint32_t>(box_nodes)});
   if (st != B200KV_OK) return st;
-  st = pool_map(&km, k_pool, num_blocks * num_kv_heads, head_dim, k8, type);
-  if (st != B200KV_OK) return st;
-  st = pool_map(&vm, v_pool, num_blocks * num_kv_heads, head_dim, k8, type);
-  if (st != B200KV_OK) return st;
+  if (!k8) {
+    st = pool_map(&km, k_pool, num_blocks * num_kv_heads, head_dim, type);
+    if (st != B200KV_OK) return st;
+    st = pool_map(&vm, v_pool, num_blocks * num_kv_heads, head_dim, type);
+    if (st != B200KV_OK) return st;
+  }
   const int ctas = sms < tree::kMaxCtas ? sms : tree::kMaxCtas;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   const WorkspaceLock lock(workspace);

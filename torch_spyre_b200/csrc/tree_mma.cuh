@@ -1422,8 +1422,10 @@ __global__ void __launch_bounds__((Cfg<T, D, kCache>::kThreads), 1)
   const int tid = threadIdx.x, warp = tid >> 5;
   if (tid == 0) {
     prefetch_tensormap(&qm);
-    prefetch_tensormap(&km);
-    prefetch_tensormap(&vm);
+    if (!C::k8) {
+      prefetch_tensormap(&km);
+      prefetch_tensormap(&vm);
+    }
     for (int i = 0; i < C::kSlots; ++i) {
       mbar_init(&c.full[i], C::k8 ? C::kConverters : 1);
       mbar_init(&c.empty[i], 1);
