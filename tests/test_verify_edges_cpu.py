@@ -1,11 +1,13 @@
 """Edges of the verification operators' host-side parts (no GPU)."""
 
 import math
+import subprocess
 
 import pytest
 import torch
 
 import torch_spyre_b200 as tsb
+from torch_spyre_b200 import _eager, build
 
 
 # ------------------------------------------------------------------ tables --
@@ -36,3 +38,47 @@ def test_yarn_ramp(rotary_dim, base, original, factor):
         if turns > 1.0:  # a pair that turns is not interpolated whole
             assert float(got[i]) > inv / factor * (1 + 1e-6)
         assert math.isclose(float(t[1, i].double().norm()), 0.1 * math.log(factor) + 1, rel_tol=1e-6)
+
+
+# ------------------------------------------------------------------- build --
+class Tools:
+    """In place of subprocess.run: writes what the compilers would."""
+
+    def __init__(self, monkeypatch, tmp_path, gxx):
+        self.ran, self.gxx = [], gxx
+        for name in ("LIB_DIR", "LIB_PATH", "FAST_PATH"):
+            monkeypatch.setattr(build, name, tmp_path / "lib" / getattr(build, name).name if name != "LIB_DIR"
+                                else tmp_path / "lib")
+        monkeypatch.setattr(build.subprocess, "run", self.run)
+        monkeypatch.setattr(build, "nvcc_path", lambda: "/somewhere/bin/nvcc")
+
+    def run(self, cmd, **kw):
+        tool = cmd[0].split("/")[-1]
+        self.ran.append(tool)
+        if tool == "g++" and self.gxx != "works":
+            if self.gxx == "absent":
+                raise FileNotFoundError("g++")
+            return subprocess.CompletedProcess(cmd, 1, "", "Python.h: No such file or directory")
+        with open(cmd[cmd.index("-o") + 1], "w") as f:
+            f.write(tool)
+        return subprocess.CompletedProcess(cmd, 0, "", "")
+
+
+@pytest.mark.parametrize("gxx", ["absent", "fails", "works"])
+def test_the_library_is_built_without_a_host_compiler_of_torch_extensions(monkeypatch, tmp_path, gxx):
+    tools = Tools(monkeypatch, tmp_path, gxx)
+    if gxx == "works":
+        build.build()
+    else:
+        with pytest.warns(RuntimeWarning, match="through Python"):
+            build.build()
+    assert build.LIB_PATH.read_text() == "nvcc" and build.FAST_PATH.exists() == (gxx == "works")
+    assert tools.ran == ["nvcc", "g++"]
+
+
+def test_calls_without_the_module_take_the_python_way(monkeypatch, tmp_path):
+    monkeypatch.setattr(_eager, "__file__", str(tmp_path / "_eager.py"))
+    monkeypatch.setattr(_eager, "fast", _eager._Unbound())
+    with pytest.warns(RuntimeWarning, match="is missing"):
+        assert _eager.fast.rotary(1, 2, 3) is None
+    assert _eager.fast.tree_mask() is None and _eager.fast.set_workspace(None) is None

@@ -10,7 +10,7 @@ import torch
 import torch_spyre_b200 as tsb
 from tests.test_verify_paths_gpu import Step, same
 from tests.verify_ref import TreeCase, make_cache, unit_roundoff
-from torch_spyre_b200 import _lib
+from torch_spyre_b200 import _eager, _lib
 from torch_spyre_b200.rotations import DTYPE_CODES
 
 pytestmark = pytest.mark.gpu
@@ -362,3 +362,14 @@ def test_traced_gradient():
     w = torch.randn_like(x)
     assert torch.equal(torch.autograd.grad(traced(x), x, w)[0],
                        torch.autograd.grad(tsb.rotary(x, step.turn, step.pos), x, w)[0])
+
+
+# ------------------------------------------------------------- without _fast --
+def test_calls_without_the_module_give_the_same_bits(monkeypatch):
+    want = Step().public()
+    x = Step().k.clone().requires_grad_(True)
+    step, w = Step(), torch.randn_like(x)
+    grad = torch.autograd.grad(tsb.rotary(x, step.turn, step.pos), x, w)[0]
+    monkeypatch.setattr(_eager, "fast", _eager._Absent())
+    assert same(Step().public(), want)
+    assert torch.equal(torch.autograd.grad(tsb.rotary(x, step.turn, step.pos), x, w)[0], grad)

@@ -7,7 +7,7 @@ the verification operators take one of two shorter ways:
 
 * the ``_fast`` module (csrc/fast_call.cpp) checks, allocates and launches
   without Python; it returns None when anything is not plain or not as the
-  operator wants it;
+  operator wants it (or the module was not built);
 * then the Python implementation runs directly (it raises for what is wrong).
 
 Under torch.compile, torch.jit.trace, fake tensors, dispatch modes, functorch
@@ -20,6 +20,7 @@ from __future__ import annotations
 
 import ctypes
 import importlib.util
+import warnings
 from pathlib import Path
 from typing import Optional
 
@@ -41,19 +42,29 @@ _ENTRIES = ("b200kv_rotary", "b200kv_kv_store", "b200kv_kv_load", "b200kv_tree_m
             "b200kv_tree_attention", "b200kv_tree_commit")
 
 
+class _Absent:
+    """Stands in for the module where it was not built: every call takes the Python way."""
+
+    def __getattr__(self, name):
+        return lambda *args: None
+
+
 class _Unbound:
     """Stands in until the first call: loads the library and binds the module to it."""
 
     def __getattr__(self, name):
         global fast
         path = Path(__file__).resolve().parent / "lib" / "_fast.so"
-        if not path.exists():
-            raise ImportError(f"{path} is missing: build it with `python -m torch_spyre_b200.build`")
-        spec = importlib.util.spec_from_file_location("_fast", path)
-        module = importlib.util.module_from_spec(spec)
-        spec.loader.exec_module(module)
         handle = _lib.lib()
-        module.bind(*(ctypes.cast(getattr(handle, e), ctypes.c_void_p).value for e in _ENTRIES))
+        if path.exists():
+            spec = importlib.util.spec_from_file_location("_fast", path)
+            module = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(module)
+            module.bind(*(ctypes.cast(getattr(handle, e), ctypes.c_void_p).value for e in _ENTRIES))
+        else:
+            warnings.warn(f"{path} is missing, calls go through Python (three times the host time): build it with "
+                          "`python -m torch_spyre_b200.build`", RuntimeWarning, stacklevel=3)
+            module = _Absent()
         fast = module
         return getattr(module, name)
 

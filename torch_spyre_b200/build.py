@@ -12,6 +12,7 @@ import shutil
 import subprocess
 import sys
 import sysconfig
+import warnings
 from pathlib import Path
 
 PKG_DIR = Path(__file__).resolve().parent
@@ -74,7 +75,10 @@ def build_fast(force: bool = False) -> Path:
     cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *[f"-I{p}" for p in includes], str(src),
            "-o", str(tmp), f"-L{root / 'lib'}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"]
-    proc = subprocess.run(cmd, capture_output=True, text=True)
+    try:
+        proc = subprocess.run(cmd, capture_output=True, text=True)
+    except OSError as e:
+        raise RuntimeError(f"g++ could not be run: {e}") from e
     if proc.returncode != 0:
         raise RuntimeError(f"g++ failed ({proc.returncode}):\n{' '.join(cmd)}\n{proc.stderr}")
     os.replace(tmp, FAST_PATH)
@@ -83,11 +87,19 @@ def build_fast(force: bool = False) -> Path:
 
 def build(force: bool = False, verbose: bool = False) -> Path:
     """Compiles every CUDA source of the library into one shared object, and the
-    module that calls it."""
+    module that calls it.  Only nvcc is needed: without the module (no g++, no
+    Python headers) the same calls go through Python, which a warning says."""
     LIB_DIR.mkdir(exist_ok=True)
-    build_fast(force)
-    if not force and not _needs_rebuild():
-        return LIB_PATH
+    if force or _needs_rebuild():
+        _build_lib(verbose)
+    try:
+        build_fast(force)
+    except RuntimeError as e:
+        warnings.warn(f"the verification operators will be called through Python: {e}", RuntimeWarning, stacklevel=2)
+    return LIB_PATH
+
+
+def _build_lib(verbose: bool) -> None:
     tmp = LIB_PATH.with_suffix(".so.tmp")
     cmd = [
         nvcc_path(),
@@ -113,7 +125,6 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     if verbose:
         sys.stderr.write(proc.stderr)
     os.replace(tmp, LIB_PATH)
-    return LIB_PATH
 
 
 if __name__ == "__main__":
