@@ -82,3 +82,20 @@ def test_calls_without_the_module_take_the_python_way(monkeypatch, tmp_path):
     with pytest.warns(RuntimeWarning, match="is missing"):
         assert _eager.fast.rotary(1, 2, 3) is None
     assert _eager.fast.tree_mask() is None and _eager.fast.set_workspace(None) is None
+
+
+def test_a_module_built_for_another_torch_is_not_loaded(monkeypatch, tmp_path):
+    monkeypatch.setattr(torch, "__version__", torch.__version__ + ".other")
+    other = build.fast_name()
+    monkeypatch.undo()
+    assert other != build.fast_name() and build.FAST_PATH.name == build.fast_name()
+    tools = Tools(monkeypatch, tmp_path, "works")
+    build.build()
+    build.FAST_PATH.rename(build.FAST_PATH.with_name(other))  # left from before: is built anew, newer source or not
+    build.build()
+    assert tools.ran == ["nvcc", "g++", "g++"] and build.FAST_PATH.exists()
+    build.FAST_PATH.unlink()
+    monkeypatch.setattr(_eager, "__file__", str(tmp_path / "_eager.py"))
+    monkeypatch.setattr(_eager, "fast", _eager._Unbound())
+    with pytest.warns(RuntimeWarning, match="is missing"):
+        assert _eager.fast.kv_load() is None

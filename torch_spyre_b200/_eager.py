@@ -54,7 +54,9 @@ class _Unbound:
 
     def __getattr__(self, name):
         global fast
-        path = Path(__file__).resolve().parent / "lib" / "_fast.so"
+        from .build import fast_name  # (here, so that `python -m torch_spyre_b200.build` is its only import)
+
+        path = Path(__file__).resolve().parent / "lib" / fast_name()
         handle = _lib.lib()
         if path.exists():
             spec = importlib.util.spec_from_file_location("_fast", path)

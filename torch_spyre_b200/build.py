@@ -15,11 +15,21 @@ import sysconfig
 import warnings
 from pathlib import Path
 
+import torch
+
 PKG_DIR = Path(__file__).resolve().parent
 CSRC = PKG_DIR / "csrc"
 LIB_DIR = PKG_DIR / "lib"
 LIB_PATH = LIB_DIR / "libb200kv.so"
-FAST_PATH = LIB_DIR / "_fast.so"  # the Python module of csrc/fast_call.cpp
+
+
+def fast_name() -> str:
+    """File name of the Python module of csrc/fast_call.cpp: it fits one version of
+    torch and of Python, so one built for another is not taken for it."""
+    return f"_fast-{torch.__version__}-{sys.implementation.cache_tag}.so"
+
+
+FAST_PATH = LIB_DIR / fast_name()
 INCLUDE = PKG_DIR.parent / "include"
 
 SOURCES = [
@@ -65,13 +75,11 @@ def build_fast(force: bool = False) -> Path:
     src = CSRC / "fast_call.cpp"
     if not force and FAST_PATH.exists() and FAST_PATH.stat().st_mtime >= src.stat().st_mtime:
         return FAST_PATH
-    import torch
-
     root = Path(torch.__file__).resolve().parent
     cuda_home = Path(nvcc_path()).resolve().parent.parent
     includes = [root / "include", root / "include" / "torch" / "csrc" / "api" / "include",
                 sysconfig.get_paths()["include"], cuda_home / "include"]
-    tmp = FAST_PATH.with_suffix(".so.tmp")
+    tmp = FAST_PATH.with_name(FAST_PATH.name + ".tmp")
     cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *[f"-I{p}" for p in includes], str(src),
            "-o", str(tmp), f"-L{root / 'lib'}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"]
