@@ -615,7 +615,8 @@ B200KV_API int b200kv_rotary(const void *x, int32_t dtype, int64_t x_stride_t, i
 
 /* Writes K/V rows to their slots, in one launch.  Row n, head h of k starts at
  * k[n * k_stride_n + h * k_stride_h] (v, q likewise; row_dtype fp16 or bf16;
- * 16-byte aligned, strides multiples of 8).  With a table (as above, 16-byte
+ * 16-byte aligned, strides multiples of 8 where there is more than one row or
+ * head).  With a table (as above, 16-byte
  * aligned; half layout: rotary_dim a multiple of 16) k is turned by positions[n] first, and
  * so is q into q_out (contiguous [N, Hq, D]; num_q_heads 0: no q).  A 16-bit
  * pool has the rows' dtype and takes them rounded once.  An 8-bit pool takes

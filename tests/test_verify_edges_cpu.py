@@ -7,7 +7,8 @@ import pytest
 import torch
 
 import torch_spyre_b200 as tsb
-from torch_spyre_b200 import _eager, build
+from tests.test_verify_cpu import store
+from torch_spyre_b200 import _eager, _lib, build
 
 
 # ------------------------------------------------------------------ tables --
@@ -99,3 +100,9 @@ def test_a_module_built_for_another_torch_is_not_loaded(monkeypatch, tmp_path):
     monkeypatch.setattr(_eager, "fast", _eager._Unbound())
     with pytest.warns(RuntimeWarning, match="is missing"):
         assert _eager.fast.kv_load() is None
+
+
+# ---------------------------------------------------------------- refusals --
+def test_token_counts_that_the_product_with_the_heads_would_wrap():
+    for n in (1 << 31, 1 << 58, (1 << 63) - 1):
+        assert store(N=n) == 1 and "num_tokens" in _lib.last_error()

@@ -488,7 +488,7 @@ extern "C" int b200kv_kv_store(const void *q, int64_t q_stride_n, int64_t q_stri
   if (st != B200KV_OK) return st;
   const bool k8 = pool_dtype == B200KV_I8 || pool_dtype == B200KV_E4M3;
   B200KV_CHECK_ARG(k8 || pool_dtype == row_dtype, "a 16-bit pool must have the rows' dtype");
-  B200KV_CHECK_ARG(num_tokens >= 0, "num_tokens must be >= 0 (got %lld)", (long long)num_tokens);
+  B200KV_CHECK_ARG(num_tokens >= 0 && num_tokens < (int64_t{1} << 31), "num_tokens %lld out of range", (long long)num_tokens);
   B200KV_CHECK_ARG(num_kv_heads > 0 && num_kv_heads <= 65536 && num_q_heads >= 0 && num_q_heads <= 65536 &&
                        num_blocks > 0 && num_blocks < (int64_t{1} << 40),
                    "head counts or num_blocks out of range");
@@ -510,8 +510,11 @@ extern "C" int b200kv_kv_store(const void *q, int64_t q_stride_n, int64_t q_stri
   B200KV_CHECK_ARG(aligned_to(k, 16) && aligned_to(v, 16) && aligned_to(k_pool, 16) && aligned_to(v_pool, 16) &&
                        (num_q_heads == 0 || (aligned_to(q, 16) && aligned_to(q_out, 16))) && aligned_to(table, 16),
                    "buffers must be 16-byte aligned");
-  B200KV_CHECK_ARG(k_stride_n % 8 == 0 && k_stride_h % 8 == 0 && v_stride_n % 8 == 0 && v_stride_h % 8 == 0 &&
-                       (num_q_heads == 0 || (q_stride_n % 8 == 0 && q_stride_h % 8 == 0)),
+  // (a dimension of one element may have any stride)
+  const bool many = num_tokens > 1;
+  B200KV_CHECK_ARG((!many || (k_stride_n % 8 == 0 && v_stride_n % 8 == 0)) &&
+                       (num_kv_heads == 1 || (k_stride_h % 8 == 0 && v_stride_h % 8 == 0)) &&
+                       (num_q_heads == 0 || ((!many || q_stride_n % 8 == 0) && (num_q_heads == 1 || q_stride_h % 8 == 0))),
                    "row strides must be multiples of 8 elements");
   StoreArgs a{};
   a.q = q, a.q_sn = q_stride_n, a.q_sh = q_stride_h, a.q_out = q_out;
