@@ -208,6 +208,15 @@ def test_descendants_of_a_pruned_node_see_nothing():
         assert [w & (2**64 - 1) for w in mask[5 + i].tolist()] == want, i
 
 
+@pytest.mark.parametrize("grad", [False, True])
+def test_tables_that_the_entry_refuses(grad):
+    x = torch.randn(2, 1, 8, device="cuda", requires_grad=grad)
+    odd = torch.zeros(1 + 4 * 8, device="cuda")[1:].view(4, 4, 2)  # 4 bytes past an 8-byte boundary
+    for table, what in ((odd, "aligned"), (torch.zeros(0, 4, 2, device="cuda"), "max_pos")):
+        with pytest.raises(tsb.B200KVError, match=what):
+            tsb.rotary(x, table, int32(0, 1))
+
+
 # ------------------------------------------------------------------ commit --
 @pytest.mark.parametrize("cache", [F16, I8])
 @pytest.mark.parametrize("ctx", [0, 3, 100])

@@ -212,8 +212,10 @@ PyObject *rotary(PyObject *, PyObject *const *a, Py_ssize_t n) {
   if (!x->requires_grad() || !c10::GradMode::is_enabled()) {
     out = turn(*x, *table, *pos, interleaved, transpose, flag);
   } else {
-    // (a head_dim that the entry refuses goes to the Python path, which says so)
-    if (x->size(2) > 4096 || x->size(1) > 65536 || x->size(0) >= int64_t(1) << 31 || x->numel() == 0) Py_RETURN_NONE;
+    // (what the entry refuses goes to the Python path, which says so)
+    if (x->size(2) > 4096 || x->size(1) > 65536 || x->size(0) >= int64_t(1) << 31 || x->numel() == 0 ||
+        table->size(0) == 0 || reinterpret_cast<uintptr_t>(table->data_ptr()) % 8 != 0)
+      Py_RETURN_NONE;
     std::optional<at::Tensor> kept;
     if (flag) kept = THPVariable_Unpack(a[5]);
     out = Turn::apply(*x, *table, *pos, interleaved, transpose, kept);
