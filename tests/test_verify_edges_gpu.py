@@ -76,6 +76,21 @@ def test_no_row_has_a_sequence_where_the_offsets_descend(cache, indptr):
     assert bool((out == 0).all()) and bool((lse == -math.inf).all())
 
 
+@pytest.mark.parametrize("cache", [F16, I8])
+def test_store_takes_any_stride_of_a_single_row_or_head(cache):
+    g = torch.Generator(device="cuda").manual_seed(3)
+    fused = torch.randn(1, 6 * 128 + 3, generator=g, device="cuda").half()
+    q, k, v = (fused.as_strided((1, n, 128), (771, 128 if n > 1 else 771, 1), at * 128) for at, n in ((0, 4), (4, 1), (5, 1)))
+    tight = tuple(torch.empty(x.shape, dtype=F16, device="cuda").copy_(x) for x in (q, k, v))
+    table, pos, slots = tsb.rotary_table(8, 128, device="cuda"), int32(5), torch.tensor([70], device="cuda")
+    got = []
+    for q, k, v in ((q, k, v), tight):
+        (kp, ks), (vp, vs) = (tsb.empty_row_pool(2, 1, 128, cache, device="cuda") for _ in range(2))
+        out = tsb.kv_store(k, v, kp, vp, slots, ks, vs, q=q, table=table, positions=pos)
+        got.append((out, tsb.kv_load(kp, slots, ks), tsb.kv_load(vp, slots, vs)))
+    assert same(*got)
+
+
 # -------------------------------------------------------------------- flags --
 @pytest.mark.parametrize("flag", [torch.zeros(1, dtype=torch.int32), torch.zeros(1, dtype=torch.int64),
                                   torch.zeros(0, dtype=torch.int32)])
