@@ -126,7 +126,9 @@ static_assert(sizeof(Ctrl) <= kOffFactors, "control block");
 
 // ------------------------------------------------------------------- waits --
 // Bounded: after kWaitLimitNs the error flag is set and this thread waits no
-// more (its later waits return at once), so a lost transfer ends the kernel.
+// more (its later waits return at once), so a lost transfer ends the kernel.  The
+// producer then starts no more copies, and waits for those under way, with a limit
+// again, before the CTA ends.
 __device__ __forceinline__ void wait(uint64_t *bar, uint32_t parity, bool &dead, int32_t *flag) {
   if (mbar_try_wait(bar, parity) || dead) return;
   const uint64_t t0 = global_timer_ns();
@@ -477,6 +479,16 @@ static __device__ __noinline__ void zero_pages(uint8_t *tile, uint32_t valid) {
 }
 
 // ------------------------------------------------------------------ roles --
+// Waits, with a limit, for the copies that are under way: the last of `issued` tiles and Q of the last piece.
+template <typename C>
+__device__ __noinline__ void drain(const Args &a, Ctrl &c, uint32_t issued, uint32_t pieces) {
+  bool late = false;
+  if (pieces > 0) wait(&c.q_full, (pieces - 1) & 1u, late, a.error_flag);
+  constexpr uint32_t kDepth = C::k8 ? C::kRaw : C::kSlots;
+  for (uint32_t n = issued - min(issued, kDepth); n < issued; ++n)
+    wait(C::k8 ? &c.raw_full[n % kDepth] : &c.full[n % kDepth], (n / kDepth) & 1u, late, a.error_flag);
+}
+
 template <typename C>
 __device__ __forceinline__ void producer(const Args &a, Ctrl &c, uint8_t *smem, const CUtensorMap *qm,
                                          const CUtensorMap *km, const CUtensorMap *vm) {
@@ -497,6 +509,8 @@ __device__ __forceinline__ void producer(const Args &a, Ctrl &c, uint8_t *smem, 
     const int pages = (w.s.ctx + w.s.nodes + kPageTokens - 1) / kPageTokens;
     int window = w.t0 / 16, ids = load_ids(a, w.b, window, pages), ids_next = load_ids(a, w.b, window + 1, pages);
     wait(&c.q_empty, (pieces & 1u) ^ 1u, dead, a.error_flag);
+    dead = __any_sync(0xffffffffu, dead);
+    if (dead) break;
     // lane: a box of Q (16-bit pools: of one or two Q tiles; 8-bit: of the
     // tile's copies) and stick column
     const int st = lane % C::kSticks, box = lane / C::kSticks;
@@ -519,6 +533,7 @@ __device__ __forceinline__ void producer(const Args &a, Ctrl &c, uint8_t *smem, 
     ++pieces;
     int ids_before = ids;
     auto issue = [&](bool is_v, int t) {
+      if (dead) return;
       if (t / 16 > window) {  // K leads, V follows by at most two tiles
         ids_before = ids;
         ids = ids_next;
@@ -534,7 +549,7 @@ __device__ __forceinline__ void producer(const Args &a, Ctrl &c, uint8_t *smem, 
         const uint32_t s = slot % C::kSlots;
         wait(&c.empty[s], ((slot / C::kSlots) & 1u) ^ 1u, dead, a.error_flag);
         if (lane == 0) mbar_arrive_expect_tx(&c.full[s], uint32_t(n) * C::kSticks * (kPageTokens * 128));
-        __syncwarp();
+        if ((dead = __any_sync(0xffffffffu, dead))) return;
         // an invalid id reads past the last page: zeros
         const int page = id < 0 ? a.num_blocks * a.hkv : id * a.hkv + w.kvh;
         if (at < n)
@@ -548,7 +563,7 @@ __device__ __forceinline__ void producer(const Args &a, Ctrl &c, uint8_t *smem, 
         const uint32_t valid = __ballot_sync(0xffffffffu, at < n && id >= 0);
         if (valid != (1u << n) - 1u) zero_pages(smem + C::kOffRaw + r * C::kRawTile, valid);
         if (lane == 0) mbar_arrive_expect_tx(&c.raw_full[r], __popc(valid) * (kPageTokens * 128));
-        __syncwarp();
+        if ((dead = __any_sync(0xffffffffu, dead))) return;
         const int64_t page = id * a.hkv + w.kvh;
         if (at < n && id >= 0)
           bulk_load(smem + C::kOffRaw + r * C::kRawTile + at * (kPageTokens * 128),
@@ -567,8 +582,12 @@ __device__ __forceinline__ void producer(const Args &a, Ctrl &c, uint8_t *smem, 
     }
     w.advance(a);
   }
+  if (dead) drain<C>(a, c, C::k8 ? ring : slot, pieces);
   // the last arrival that the MMAs owe this CTA: not before it may the CTA end
-  if (lane == 0 && pieces > 0) wait(&c.q_empty, (pieces & 1u) ^ 1u, dead, a.error_flag);
+  if (lane == 0 && pieces > 0) {
+    bool late = false;
+    wait(&c.q_empty, (pieces & 1u) ^ 1u, late, a.error_flag);
+  }
   __syncwarp();
 }
 
