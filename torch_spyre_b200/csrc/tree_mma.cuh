@@ -97,6 +97,7 @@ __device__ __forceinline__ uint32_t col_o(int w) { return 256u + uint32_t(w) * 1
 
 struct Seq {
   int ctx, nodes, q0, blocks, qtiles;
+  int end;  // the first row of q that is a later sequence's
 };
 // Where a CTA's share of the line begins: in block `block`, whose units begin at
 // unit u0 of the line.
@@ -246,6 +247,7 @@ __device__ __forceinline__ Seq load_seq(const Args &a, int b, bool report) {
   s.ctx = min(max(s.ctx, 0), cap);
   s.q0 = min(max(s.q0, 0), a.total_q);
   s.nodes = min(max(end, s.q0), a.total_q) - s.q0;
+  s.end = b == a.batch - 1 ? a.total_q : min(max(end, 0), a.total_q);
   const int most = min(a.max_nodes, cap - s.ctx);
   bad = bad || s.nodes > most;
   s.nodes = min(s.nodes, most);
@@ -362,14 +364,11 @@ struct Walk {
 // Rows of q that no sequence has (all of them flagged): before the first
 // sequence's, past a sequence's nodes as they were clamped, after the last's.
 // They see nothing.  Every CTA takes some.  `all`: no row has a sequence.
-__device__ __forceinline__ int rows_end(const Args &a, int b) {  // of sequence b and what follows it unclaimed
-  return b == a.batch - 1 ? a.total_q : min(max(__ldg(a.indptr + b + 1), 0), a.total_q);
-}
 template <typename T, int D, int kQ>
 __device__ __noinline__ void clear_rows(const Args &a, bool all) {
   for (int b = 0; b < a.batch; ++b) {
     const Seq s = load_seq<kQ>(a, b, false);
-    const int first = b == 0 ? 0 : s.q0, end = all ? (b == 0 ? a.total_q : 0) : rows_end(a, b);
+    const int first = b == 0 ? 0 : s.q0, end = all ? (b == 0 ? a.total_q : 0) : s.end;
     for (int t = first + blockIdx.x; t < end; t += gridDim.x) {
       if (!all && t >= s.q0 && t < s.q0 + s.nodes) continue;
       uint4 *out = reinterpret_cast<uint4 *>(static_cast<T *>(a.out) + static_cast<int64_t>(t) * a.hq * D);
@@ -395,9 +394,8 @@ __device__ __forceinline__ void make_plan(const Args &a, Ctrl &c) {
   for (int b = b0; b < b1; ++b) {
     s = load_seq<kQ>(a, b, blockIdx.x == 0);
     mine += head_units<kQ>(a, s) * a.hkv;
-    const int end = rows_end(a, b);
-    unclaimed = unclaimed || (b == 0 && s.q0 > 0) || s.q0 + s.nodes < end;
-    descends = descends || end < s.q0;
+    unclaimed = unclaimed || (b == 0 && s.q0 > 0) || s.q0 + s.nodes < s.end;
+    descends = descends || s.end < s.q0;
   }
   int incl = mine;
 #pragma unroll
