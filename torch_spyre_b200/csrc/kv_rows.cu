@@ -381,9 +381,10 @@ constexpr int kCommitThreads = 128, kCommitRows = 64;
 //
 // Bound: bytes, each moved row read and written once; few rows: the chain length
 // -> path -> block table -> row.  128 sequences, 8 KV heads, 32 rows each on
-// average (33.6 MB): 6.2 us, 0.84 of the copy rate.  A CTA for K and one for V
-// (every one walks that chain): 9.7 us; four heads' CTAs in one: 6.1 us, but
-// 6.0 in place of 4.2 us for 4 sequences.
+// average (33.6 MB): 7.5 us from HBM, 0.69 of the copy rate, and 6.2 where part of
+// the rows is in L2.  There a CTA for K and one for V (every one walks that chain)
+// took 9.7 us; four heads' CTAs in one 6.1, but 6.0 in place of 4.2 us for 4
+// sequences.
 template <int kRow, int kStickRow, bool kScaled>  // bytes of a row, of a row inside one stick (128)
 __global__ void __launch_bounds__(kCommitThreads) tree_commit_kernel(const CommitArgs a) {
   constexpr int kLanes = kRow / 16, kGroups = kCommitThreads / kLanes, kEach = kCommitRows / kGroups;

@@ -22,9 +22,9 @@
 // Bound, 16-bit caches: with up to 128 rows a 128-token tile costs the tensor pipe
 // 0.55 us (2 x 128^3 products at 8192 FLOP per clock) and HBM 1.5 us per SM, so
 // drafts run at the cache's bandwidth (4 sequences of 118k tokens, 16 nodes, 32/8
-// heads, fp16, 1.93 GB: 237 us); short ones by what a piece costs besides its
-// steps (16 sequences of 4.3k tokens and up to 64 nodes, bf16, 285 MB: 75 us, the
-// copy rate would be 44).  Blocks of two Q tiles are bound by the tensor pipe and
+// heads, fp16, 1.93 GB: 288 to 303 us, the copy rate would be 300); short ones by
+// what a piece costs besides its steps (16 sequences of 4.3k tokens and up to 64
+// nodes, bf16, 295 MB: 75 us, the copy rate would be 46).  Blocks of two Q tiles are bound by the tensor pipe and
 // the exponentials (16 per clock and SM, as long as the products), which follow
 // one another within a stream: two prompts' chunks of 1024 tokens over 8.1k, 64/8
 // heads, 578 GFLOP: 528 us, 0.64 of the matrix rate.
@@ -32,8 +32,7 @@
 // 8-bit caches: widening (2 x 16 KB a tile), softmax and products take 0.6 to 0.7
 // us a tile and SM each and are a chain with handshakes, which 3 raw and 4
 // operand tiles let overlap in part only: 1.7 us a tile, 4 sequences of 118k
-// tokens, int8, 1.0 GB: 327 us (e4m3, which the conversion unit widens with fewer
-// instructions: 296).  Without widening 0.88 of that, without softmax 0.77,
+// tokens, 1.0 GB: 325 us over int8, 324 over e4m3.  Without widening 0.88 of that, without softmax 0.77,
 // without products 0.92.  More than 128 rows: every Q tile widens the tile
 // again.  (Tried: two Q tiles a block with three operand tiles, 0.93 of the time
 // with all blocks full but 1.08 with ragged drafts; widening by 16 warps in two
@@ -266,7 +265,9 @@ __device__ __forceinline__ int block_tiles(const Args &a, const Seq &s, int k) {
 // tile takes 1.1 us with one Q tile and 2.05 with two, and a block begins with
 // what every piece costs besides its steps (Q, the first products, the epilogue),
 // 5 and 7 us (least squares over the CTAs' times of eight batches of 1 to 16
-// sequences; they are within 1 to 2 us of it).
+// sequences over 16-bit caches; they are within 1 to 2 us of it).  8-bit caches are
+// cut by the same weights, although their steps take 1.75 to 2.4 us and their pieces
+// 10 to 14.
 template <int kQ>
 __device__ __forceinline__ bool two_tiles(const Seq &s, int k) {
   return kQ == 2 && 2 * k + 1 < s.qtiles;
