@@ -70,6 +70,8 @@ enum b200kv_dtype {
 #define B200KV_DEVERR_BAD_SLOT 0x2  /* slot outside [0, num_blocks * 64)      */
 #define B200KV_DEVERR_BAD_LEN 0x4   /* context_len < 0 or > capacity of table */
 #define B200KV_DEVERR_TIMEOUT 0x8   /* a bounded wait on a page transfer expired */
+#define B200KV_DEVERR_NO_PAGES 0x10 /* fewer free pages (or places for them) than needed */
+#define B200KV_DEVERR_BAD_TOKEN 0x20 /* a token outside the vocabulary, or no probability left */
 
 /* Library version: major * 10000 + minor * 100 + patch. */
 B200KV_API int b200kv_version(void);
@@ -708,6 +710,114 @@ B200KV_API int b200kv_tree_commit(void *k_pool, void *v_pool, int32_t pool_dtype
                                   int64_t num_kv_heads, int64_t head_dim, int64_t num_blocks,
                                   int64_t max_blocks_per_seq, int64_t max_path,
                                   int32_t *error_flag, void *stream);
+
+/* ------------------------------------------------------------------------ *
+ * A step's plan and its end, on the GPU: block tables, slots and positions from
+ * the requests' lengths, and the accepted path from probabilities.  (No
+ * counterpart in the reference.)
+ * ------------------------------------------------------------------------ */
+
+/* Block tables, slots and positions of the tokens a step adds.  Sequence b has
+ * context_lens[b] tokens and adds T_b = q_indptr[b + 1] - q_indptr[b] (q_indptr[0]
+ * = 0, q_indptr[batch] = num_tokens).  page_counts[b] pages are in its row of
+ * block_table; what ceil((context_lens[b] + T_b) / 64) needs beyond those is taken
+ * from the stack free_pages[0 .. free_count[0] - 1] (capacity entries), from its
+ * top, sequence after sequence; page_counts and free_count follow.  Then token i
+ * of b (t = q_indptr[b] + i) has
+ *   slots[t] = block_table[b][p / 64] * 64 + p % 64,  p = context_lens[b] + i,
+ *   positions[t] = context_lens[b] + depth,
+ * depth = i, or with tree_mask (int64 [num_tokens, mask_words], b200kv_tree_mask) the
+ * number of its bits less one (0 for a pruned node).  Where the stack runs out
+ * the sequence gets no page, nor do those after it that need any
+ * (B200KV_DEVERR_NO_PAGES), and tokens without a page have slot -1.  Lengths
+ * outside the table are clamped, tokens that no sequence has get slot -1 and
+ * position 0 (B200KV_DEVERR_BAD_LEN).  A page belongs to one sequence at a time.
+ * batch <= 1024, max_blocks_per_seq < 2^21. */
+B200KV_API int b200kv_extend_pages(int32_t *block_table, int64_t block_table_stride,
+                                   int32_t *page_counts, int32_t *free_pages, int64_t capacity,
+                                   int32_t *free_count, const int32_t *context_lens,
+                                   const int32_t *q_indptr, const int64_t *tree_mask,
+                                   int64_t mask_words, int64_t *slots, int32_t *positions,
+                                   int64_t num_tokens, int64_t batch, int64_t max_blocks_per_seq,
+                                   int32_t *error_flag, void *stream);
+
+/* Gives pages back: sequence b keeps ceil(keep_lens[b] / 64) pages (0: it ends),
+ * the others go back to the stack, in the order opposite to b200kv_extend_pages
+ * (an extend that is released whole leaves the stack as it was), and their table
+ * entries become -1.  A negative keep_lens keeps all (B200KV_DEVERR_BAD_LEN);
+ * what finds no place in free_pages stays (B200KV_DEVERR_NO_PAGES). */
+B200KV_API int b200kv_release_pages(int32_t *block_table, int64_t block_table_stride,
+                                    int32_t *page_counts, int32_t *free_pages, int64_t capacity,
+                                    int32_t *free_count, const int32_t *keep_lens, int64_t batch,
+                                    int64_t max_blocks_per_seq, int32_t *error_flag, void *stream);
+
+/* Accepts or rejects the drafted tokens of every sequence.  Sequence b has nodes
+ * q_indptr[b] .. q_indptr[b + 1] - 1 (at most 1024): node 0 is its last token, and
+ * is taken; node i > 0 is the drafted token tokens[i] after node parents[i]
+ * (index inside the sequence, below i; negative: never tried).
+ * target_probs row i (vocab elements of dtype fp16, bf16 or fp32, from target_probs
+ * + i * target_stride) is the target's distribution after node i, draft_probs
+ * row i (may be NULL) the one that node i's children were drawn from.  From node 0
+ * on, the children of the node reached are tried in their order with accept_u
+ * [total_q] (in [0, 1)):  x is accepted if u * S * q(x) < w(x), where w = p and
+ * S = 1 at first, and w = max(w - S q, 0), S = sum w after a rejection; without
+ * draft_probs, if u * S < w(x), and after a rejection w(x) = 0 and S falls by what
+ * w(x) was.  The next token is drawn from w where the walk ends, with sample_u
+ * [batch]: the first x with w(0) + .. + w(x) > u * sum w.  (This leaves the
+ * target's distribution as it is if children were drawn independently from the
+ * draft_probs row, or chosen without chance where there is none.)  All of it
+ * in 64 bits.  path int32 [batch, max_path] gets the nodes accepted, 0 first, -1
+ * behind them; a path of max_path nodes ends there.  path_lens [batch],
+ * next_tokens int64 [batch].  Elements that are not positive numbers have no
+ * weight; where nothing is left w = p again, and a row without any weight gives -1
+ * and B200KV_DEVERR_BAD_TOKEN, as does a token outside the vocabulary, which is
+ * not accepted.  A sequence without nodes has path length 0 and next token -1. */
+B200KV_API int b200kv_tree_verify(const int32_t *parents, const int64_t *tokens,
+                                  const int32_t *q_indptr, const void *target_probs,
+                                  int64_t target_stride, const void *draft_probs,
+                                  int64_t draft_stride, int32_t dtype, const float *accept_u,
+                                  const float *sample_u, int32_t *path, int32_t *path_lens,
+                                  int64_t *next_tokens, int64_t total_q, int64_t batch,
+                                  int64_t vocab, int64_t max_path, int32_t *error_flag,
+                                  void *stream);
+
+/* ------------------------------------------------------------------------ *
+ * Latent attention: a cache of one vector a token that all heads share.
+ *
+ * A row has 512 latent elements, which are key and value, and 64 rotary key
+ * elements: pool (fp16 or bf16, 16-byte aligned) [num_blocks, 1, 9, 64, 64], pages
+ * and slots as above with one head of nine sticks.  (b200kv_kv_load reads rows of it
+ * taken as [num_blocks, 9, 1, 64, 64], nine heads of 64 elements.)
+ * ------------------------------------------------------------------------ */
+#define B200KV_LATENT_RANK 512
+#define B200KV_LATENT_ROPE 64
+#define B200KV_LATENT_NOPE 128 /* a head's key and value elements, expanded */
+
+/* Writes rows to their slots, in one launch: latent row n (512 elements at latent
+ * + n * latent_stride_n), with norm_weight (512 elements of dtype, or NULL) as
+ * x / sqrt(mean(x^2) + eps) * weight; behind it k_rope row n (64 elements), with a
+ * table (fp32 [max_pos, 32, 2]) turned by positions[n] as b200kv_rotary does, half
+ * or interleaved pairs.  q_rope (64 elements of row n, head h, or num_q_heads 0) is
+ * turned into q_out, contiguous [num_tokens, num_q_heads, 64].  fp32, rounded once.
+ * Row strides are multiples of 8.  Slots must be distinct; negative: the row is
+ * skipped; past the pool: skipped, B200KV_DEVERR_BAD_SLOT.  A position outside the
+ * table is clamped (B200KV_DEVERR_BAD_LEN). */
+B200KV_API int b200kv_latent_store(const void *latent, int64_t latent_stride_n, const void *k_rope,
+                                   int64_t k_rope_stride_n, const void *q_rope, int64_t q_stride_n,
+                                   int64_t q_stride_h, void *q_out, int32_t dtype,
+                                   const void *norm_weight, float eps, void *pool,
+                                   const int64_t *slots, const float *table, int64_t max_pos,
+                                   const int32_t *positions, int32_t interleaved,
+                                   int64_t num_tokens, int64_t num_q_heads, int64_t num_blocks,
+                                   int32_t *error_flag, void *stream);
+
+/* b200kv_tree_commit for a latent pool. */
+B200KV_API int b200kv_latent_commit(void *pool, int32_t dtype, const int32_t *block_table,
+                                    int64_t block_table_stride, const int32_t *context_lens,
+                                    const int32_t *path, int64_t path_stride,
+                                    const int32_t *path_lens, int32_t *new_lens, int64_t batch,
+                                    int64_t num_blocks, int64_t max_blocks_per_seq,
+                                    int64_t max_path, int32_t *error_flag, void *stream);
 
 #ifdef __cplusplus
 }

@@ -5,16 +5,18 @@ CUDA library (``lib/libb200kv.so``, built by ``python -m torch_spyre_b200.build`
 is loaded on first use and is the only implementation.
 """
 
-from . import _lib, fp8, kv_rows, layout, ops, rotations, tree, workloads  # noqa: F401
+from . import _lib, fp8, kv_rows, latent, layout, ops, pages, rotations, tree, workloads  # noqa: F401
 from ._lib import B200KVError
 from .fp8 import dequantize_fp8_with_scale, empty_pool_fp8, pool_shape_fp8, quantize_fp8_with_scale
 from .kv_rows import empty_row_pool, kv_load, kv_store
+from .latent import empty_latent_pool, latent_commit, latent_load, latent_store
 from .layout import (SpyreTensorLayout, empty_pool, from_device_layout, page_layout, pool_shape, restickify,
                      restickify_layout, stick_layout, to_device_layout)
 from .ops import (decode_attention, decode_attention_append, kv_append, kv_relayout, kv_unrelayout,
                   merge_attention_states, rope, scaled_dot_product_fused_attention_overrideable, sdpa_decode)
+from .pages import extend_pages, release_pages
 from .rotations import rotary, rotary_table
-from .tree import tree_attention, tree_commit, tree_mask
+from .tree import tree_attention, tree_commit, tree_mask, tree_verify
 
 __all__ = [
     "B200KVError",
@@ -22,9 +24,11 @@ __all__ = [
     "decode_attention",
     "decode_attention_append",
     "dequantize_fp8_with_scale",
+    "empty_latent_pool",
     "empty_pool",
     "empty_pool_fp8",
     "empty_row_pool",
+    "extend_pages",
     "from_device_layout",
     "to_device_layout",
     "kv_append",
@@ -32,11 +36,15 @@ __all__ = [
     "kv_relayout",
     "kv_store",
     "kv_unrelayout",
+    "latent_commit",
+    "latent_load",
+    "latent_store",
     "merge_attention_states",
     "page_layout",
     "pool_shape",
     "pool_shape_fp8",
     "quantize_fp8_with_scale",
+    "release_pages",
     "restickify",
     "restickify_layout",
     "rope",
@@ -48,4 +56,5 @@ __all__ = [
     "tree_attention",
     "tree_commit",
     "tree_mask",
+    "tree_verify",
 ]

@@ -28,6 +28,8 @@ DEVERR_BAD_BLOCK = 0x1
 DEVERR_BAD_SLOT = 0x2
 DEVERR_BAD_LEN = 0x4
 DEVERR_TIMEOUT = 0x8
+DEVERR_NO_PAGES = 0x10
+DEVERR_BAD_TOKEN = 0x20
 
 
 class B200KVError(RuntimeError):
@@ -290,6 +292,36 @@ SIGNATURES = {
             _i64, _i64, _i64, _i64, _i64, _i64,  # batch, Hkv, head_dim, num_blocks, max_blocks_per_seq, max_path
             _p, _p,  # error_flag, stream
         ],
+    ),
+    "b200kv_extend_pages": (
+        ctypes.c_int,
+        [
+            _p, _i64, _p, _p, _i64, _p,  # block_table, stride, page_counts, free_pages, capacity, free_count
+            _p, _p, _p, _i64, _p, _p,  # context_lens, q_indptr, tree_mask, mask_words, slots, positions
+            _i64, _i64, _i64, _p, _p,  # num_tokens, batch, max_blocks_per_seq, error_flag, stream
+        ],
+    ),
+    "b200kv_release_pages": (ctypes.c_int, [_p, _i64, _p, _p, _i64, _p, _p, _i64, _i64, _p, _p]),
+    "b200kv_tree_verify": (
+        ctypes.c_int,
+        [
+            _p, _p, _p, _p, _i64, _p, _i64, _i32,  # parents, tokens, q_indptr, target, draft, dtype
+            _p, _p, _p, _p, _p,  # accept_u, sample_u, path, path_lens, next_tokens
+            _i64, _i64, _i64, _i64, _p, _p,  # total_q, batch, vocab, max_path, error_flag, stream
+        ],
+    ),
+    "b200kv_latent_store": (
+        ctypes.c_int,
+        [
+            _p, _i64, _p, _i64, _p, _i64, _i64, _p,  # latent, k_rope, q_rope with their strides, q_out
+            _i32, _p, _f32, _p, _p,  # dtype, norm_weight, eps, pool, slots
+            _p, _i64, _p, _i32, _i64, _i64, _i64,  # table, max_pos, positions, interleaved, tokens, heads, num_blocks
+            _p, _p,  # error_flag, stream
+        ],
+    ),
+    "b200kv_latent_commit": (
+        ctypes.c_int,
+        [_p, _i32, _p, _i64, _p, _p, _i64, _p, _p, _i64, _i64, _i64, _i64, _p, _p],
     ),
 }
 

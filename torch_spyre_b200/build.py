@@ -49,6 +49,9 @@ SOURCES = [
     "tree_attention.cu",
     "tree_mma_f16.cu",
     "tree_mma_bf16.cu",
+    "tree_verify.cu",
+    "pages.cu",
+    "latent_rows.cu",
     "lse_combine.cu",
     "oproj_allreduce.cu",
 ]

@@ -41,6 +41,18 @@ struct Entries {
   int (*tree_commit)(void *, void *, int32_t, float *, float *, const int32_t *, int64_t, const int32_t *,
                      const int32_t *, int64_t, const int32_t *, int32_t *, int64_t, int64_t, int64_t, int64_t, int64_t,
                      int64_t, int32_t *, void *);
+  int (*extend_pages)(int32_t *, int64_t, int32_t *, int32_t *, int64_t, int32_t *, const int32_t *, const int32_t *,
+                      const int64_t *, int64_t, int64_t *, int32_t *, int64_t, int64_t, int64_t, int32_t *, void *);
+  int (*release_pages)(int32_t *, int64_t, int32_t *, int32_t *, int64_t, int32_t *, const int32_t *, int64_t, int64_t,
+                       int32_t *, void *);
+  int (*tree_verify)(const int32_t *, const int64_t *, const int32_t *, const void *, int64_t, const void *, int64_t,
+                     int32_t, const float *, const float *, int32_t *, int32_t *, int64_t *, int64_t, int64_t, int64_t,
+                     int64_t, int32_t *, void *);
+  int (*latent_store)(const void *, int64_t, const void *, int64_t, const void *, int64_t, int64_t, void *, int32_t,
+                      const void *, float, void *, const int64_t *, const float *, int64_t, const int32_t *, int32_t,
+                      int64_t, int64_t, int64_t, int32_t *, void *);
+  int (*latent_commit)(void *, int32_t, const int32_t *, int64_t, const int32_t *, const int32_t *, int64_t,
+                       const int32_t *, int32_t *, int64_t, int64_t, int64_t, int64_t, int32_t *, void *);
 } entries;
 bool bound = false;
 
@@ -376,9 +388,176 @@ PyObject *tree_commit(PyObject *, PyObject *const *a, Py_ssize_t n) {
   return THPVariable_Wrap(std::move(out));
 }
 
+int32_t *ints(const at::Tensor *t) { return static_cast<int32_t *>(data(t)); }
+
+struct Table {  // of extend_pages and release_pages
+  const at::Tensor *table, *counts, *pages, *count;
+  int64_t batch = 0, stride = 0;
+  Table(Call &c, PyObject *const *a)
+      : table(c.tensor(a[0])), counts(c.tensor(a[1])), pages(c.tensor(a[2])), count(c.tensor(a[3])) {
+    if (!c.ok) return;
+    c.need(table->scalar_type() == at::kInt && table->dim() == 2 && (table->size(1) == 1 || table->stride(1) == 1));
+    if (!c.ok) return;
+    batch = table->size(0);
+    stride = batch > 1 ? table->stride(0) : table->size(1);
+    c.need(vector_of(counts, at::kInt, batch) && pages->dim() == 1 && vector_of(pages, at::kInt, pages->size(0)) &&
+           vector_of(count, at::kInt, 1));
+  }
+};
+
+PyObject *pack(std::initializer_list<at::Tensor> tensors) {
+  PyObject *tuple = PyTuple_New(static_cast<Py_ssize_t>(tensors.size()));
+  Py_ssize_t i = 0;
+  for (const at::Tensor &t : tensors) {
+    PyObject *o = tuple ? THPVariable_Wrap(t) : nullptr;
+    if (!o) {
+      Py_XDECREF(tuple);
+      return nullptr;
+    }
+    PyTuple_SET_ITEM(tuple, i++, o);
+  }
+  return tuple;
+}
+
+// extend_pages(block_table, page_counts, free_pages, free_count, context_lens, q_indptr, num_tokens, mask, error_flag)
+// -> (slots, positions)
+PyObject *extend_pages(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  B200KV_ARGS(9)
+  Call c;
+  const Table t(c, a);
+  const at::Tensor *lens = c.tensor(a[4]), *indptr = c.tensor(a[5]), *mask = c.optional(a[7]);
+  const int64_t tokens = c.integer(a[6]);
+  int32_t *flag = c.flag(a[8]);
+  if (!c.ok || tokens < 0 || !vector_of(lens, at::kInt, t.batch) || !vector_of(indptr, at::kInt, t.batch + 1)) Py_RETURN_NONE;
+  if (mask && (mask->scalar_type() != at::kLong || mask->dim() != 2 || mask->size(0) != tokens || !mask->is_contiguous()))
+    Py_RETURN_NONE;
+  const c10::cuda::CUDAGuard guard(c.device);
+  at::Tensor slots = at::empty({tokens}, t.table->options().dtype(at::kLong)), pos = at::empty({tokens}, t.table->options());
+  const int st = entries.extend_pages(
+      ints(t.table), t.stride, ints(t.counts), ints(t.pages), t.pages->size(0), ints(t.count), ints(lens), ints(indptr),
+      static_cast<const int64_t *>(data(mask)), mask ? mask->size(1) : 0, static_cast<int64_t *>(slots.data_ptr()),
+      static_cast<int32_t *>(pos.data_ptr()), tokens, t.batch, t.table->size(1), flag, stream_of(c));
+  if (st != 0) Py_RETURN_NONE;
+  for (const at::Tensor *x : {t.table, t.counts, t.count}) written(x);
+  return pack({slots, pos});
+}
+
+// release_pages(block_table, page_counts, free_pages, free_count, keep_lens, error_flag) -> True
+PyObject *release_pages(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  B200KV_ARGS(6)
+  Call c;
+  const Table t(c, a);
+  const at::Tensor *keep = c.tensor(a[4]);
+  int32_t *flag = c.flag(a[5]);
+  if (!c.ok || !vector_of(keep, at::kInt, t.batch)) Py_RETURN_NONE;
+  const c10::cuda::CUDAGuard guard(c.device);
+  const int st = entries.release_pages(ints(t.table), t.stride, ints(t.counts), ints(t.pages), t.pages->size(0),
+                                       ints(t.count), ints(keep), t.batch, t.table->size(1), flag, stream_of(c));
+  if (st != 0) Py_RETURN_NONE;
+  for (const at::Tensor *x : {t.table, t.counts, t.pages, t.count}) written(x);
+  Py_RETURN_TRUE;
+}
+
+// tree_verify(parents, tokens, q_indptr, target_probs, accept_u, sample_u, draft_probs, max_path, error_flag)
+// -> (path, path_lens, next_tokens)
+PyObject *tree_verify(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  B200KV_ARGS(9)
+  Call c;
+  const at::Tensor *parents = c.tensor(a[0]), *tokens = c.tensor(a[1]), *indptr = c.tensor(a[2]), *target = c.tensor(a[3]),
+                   *au = c.tensor(a[4]), *su = c.tensor(a[5]), *draft = c.optional(a[6]);
+  const int64_t max_path = c.integer(a[7]);
+  int32_t *flag = c.flag(a[8]);
+  if (!c.ok || parents->dim() != 1 || indptr->dim() != 1 || indptr->size(0) < 1 || max_path < 1) Py_RETURN_NONE;
+  const int64_t nodes = parents->size(0), batch = indptr->size(0) - 1;
+  auto rows = [&](const at::Tensor *p) {
+    return p->dim() == 2 && p->size(0) == nodes && p->size(1) >= 1 && (p->size(1) == 1 || p->stride(1) == 1);
+  };
+  const int code = code_of(target->scalar_type());
+  if (code < 0 || code > 2 || !vector_of(parents, at::kInt, nodes) || !vector_of(tokens, at::kLong, nodes) ||
+      !vector_of(indptr, at::kInt, batch + 1) || !vector_of(au, at::kFloat, nodes) || !vector_of(su, at::kFloat, batch) ||
+      !rows(target) || (draft && (!rows(draft) || draft->sizes() != target->sizes() ||
+                                  draft->scalar_type() != target->scalar_type())))
+    Py_RETURN_NONE;
+  const c10::cuda::CUDAGuard guard(c.device);
+  at::Tensor path = at::empty({batch, max_path}, parents->options()), lens = at::empty({batch}, parents->options()),
+             next = at::empty({batch}, tokens->options());
+  const int st = entries.tree_verify(
+      ints(parents), static_cast<const int64_t *>(data(tokens)), ints(indptr), data(target), target->stride(0), data(draft),
+      draft ? draft->stride(0) : 0, code, static_cast<const float *>(data(au)), static_cast<const float *>(data(su)),
+      static_cast<int32_t *>(path.data_ptr()), static_cast<int32_t *>(lens.data_ptr()),
+      static_cast<int64_t *>(next.data_ptr()), nodes, batch, target->size(1), max_path, flag, stream_of(c));
+  if (st != 0) Py_RETURN_NONE;
+  return pack({path, lens, next});
+}
+
+constexpr int64_t kRank = 512, kRope = 64, kSticks = (kRank + kRope) / 64;
+bool latent_pool_ok(const at::Tensor *p) {
+  return is16(code_of(p->scalar_type())) && p->dim() == 5 && p->size(1) == 1 && p->size(2) == kSticks && p->size(3) == 64 &&
+         p->size(4) == 64 && p->is_contiguous();
+}
+
+// latent_store(latent, k_rope, pool, slots, q_rope, norm_weight, eps, table, positions, interleaved, error_flag)
+// -> q_rope turned, or True
+PyObject *latent_store(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  B200KV_ARGS(11)
+  Call c;
+  const at::Tensor *latent = c.tensor(a[0]), *k = c.tensor(a[1]), *pool = c.tensor(a[2]), *slots = c.tensor(a[3]),
+                   *q = c.optional(a[4]), *weight = c.optional(a[5]), *table = c.optional(a[7]), *pos = c.optional(a[8]);
+  const double eps = PyFloat_AsDouble(a[6]);
+  if (eps == -1.0 && PyErr_Occurred()) {
+    PyErr_Clear();
+    Py_RETURN_NONE;
+  }
+  int32_t *flag = c.flag(a[10]);
+  if (!c.ok || !latent_pool_ok(pool) || latent->dim() != 2 || k->dim() != 2) Py_RETURN_NONE;
+  const int64_t tokens = latent->size(0);
+  const at::ScalarType type = pool->scalar_type();
+  c.need(latent->size(1) == kRank && latent->stride(1) == 1 && latent->scalar_type() == type && k->size(0) == tokens &&
+         k->size(1) == kRope && k->stride(1) == 1 && k->scalar_type() == type && vector_of(slots, at::kLong, tokens));
+  if (weight) c.need(vector_of(weight, type, kRank));
+  if (c.ok && table) c.need(pos && table_ok(table, pos, tokens, kRope) && table->size(1) == kRope / 2);
+  if (q) c.need(table && rows_ok(q) && q->scalar_type() == type && q->size(0) == tokens && q->size(2) == kRope);
+  if (!c.ok) Py_RETURN_NONE;
+  const c10::cuda::CUDAGuard guard(c.device);
+  at::Tensor out;
+  if (q) out = at::empty(q->sizes(), q->options());
+  const int st = entries.latent_store(
+      data(latent), latent->stride(0), data(k), k->stride(0), data(q), q ? q->stride(0) : 0, q ? q->stride(1) : 0,
+      q ? out.data_ptr() : nullptr, code_of(type), data(weight), static_cast<float>(eps), data(pool),
+      static_cast<const int64_t *>(data(slots)), static_cast<const float *>(data(table)), table ? table->size(0) : 0,
+      table ? ints(pos) : nullptr, a[9] == Py_True, tokens, q ? q->size(1) : 0, pool->size(0), flag, stream_of(c));
+  if (st != 0) Py_RETURN_NONE;
+  written(pool);
+  if (!q) Py_RETURN_TRUE;
+  return THPVariable_Wrap(std::move(out));
+}
+
+// latent_commit(pool, block_table, context_lens, path, path_lens, error_flag)
+PyObject *latent_commit(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  B200KV_ARGS(6)
+  Call c;
+  const at::Tensor *pool = c.tensor(a[0]), *table = c.tensor(a[1]), *lens = c.tensor(a[2]), *path = c.tensor(a[3]),
+                   *plens = c.tensor(a[4]);
+  int32_t *flag = c.flag(a[5]);
+  if (!c.ok || !latent_pool_ok(pool) || !sequences_ok(table, lens)) Py_RETURN_NONE;
+  const int64_t batch = table->size(0);
+  if (path->scalar_type() != at::kInt || path->dim() != 2 || path->size(0) != batch ||
+      (path->size(1) > 1 && path->stride(1) != 1) || !vector_of(plens, at::kInt, batch))
+    Py_RETURN_NONE;
+  const c10::cuda::CUDAGuard guard(c.device);
+  at::Tensor out = at::empty(lens->sizes(), lens->options());
+  const int st = entries.latent_commit(data(pool), code_of(pool->scalar_type()), ints(table), table->stride(0), ints(lens),
+                                       ints(path), batch > 1 ? path->stride(0) : path->size(1), ints(plens),
+                                       static_cast<int32_t *>(out.data_ptr()), batch, pool->size(0), table->size(1),
+                                       path->size(1), flag, stream_of(c));
+  if (st != 0) Py_RETURN_NONE;
+  written(pool);
+  return THPVariable_Wrap(std::move(out));
+}
+
 // bind(addresses): the C entries in the order of Entries
 PyObject *bind(PyObject *, PyObject *const *a, Py_ssize_t n) {
-  B200KV_ARGS(7)
+  B200KV_ARGS(static_cast<Py_ssize_t>(sizeof(Entries) / sizeof(void *)))
   void **slots = reinterpret_cast<void **>(&entries);
   for (Py_ssize_t i = 0; i < n; ++i) {
     slots[i] = PyLong_AsVoidPtr(a[i]);
@@ -417,6 +596,8 @@ PyObject *guarded(PyObject *self, PyObject *const *a, Py_ssize_t n) {
 
 PyMethodDef methods[] = {B200KV_METHOD(rotary),         B200KV_METHOD(kv_store),    B200KV_METHOD(kv_load),
                          B200KV_METHOD(tree_mask),      B200KV_METHOD(tree_attention), B200KV_METHOD(tree_commit),
+                         B200KV_METHOD(extend_pages),   B200KV_METHOD(release_pages), B200KV_METHOD(tree_verify),
+                         B200KV_METHOD(latent_store),   B200KV_METHOD(latent_commit),
                          B200KV_METHOD(bind),           B200KV_METHOD(set_workspace), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_fast", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -385,7 +385,8 @@ constexpr int kCommitThreads = 128, kCommitRows = 64;
 // the rows is in L2.  There a CTA for K and one for V (every one walks that chain)
 // took 9.7 us; four heads' CTAs in one 6.1, but 6.0 in place of 4.2 us for 4
 // sequences.
-template <int kRow, int kStickRow, bool kScaled>  // bytes of a row, of a row inside one stick (128)
+// (kPools = 1: a latent cache, its nine sticks taken as heads of 64 elements.)
+template <int kRow, int kStickRow, bool kScaled, int kPools = 2>  // bytes of a row, of a row inside one stick (128)
 __global__ void __launch_bounds__(kCommitThreads) tree_commit_kernel(const CommitArgs a) {
   constexpr int kLanes = kRow / 16, kGroups = kCommitThreads / kLanes, kEach = kCommitRows / kGroups;
   constexpr int64_t kPage = 64 * kRow;
@@ -438,7 +439,7 @@ __global__ void __launch_bounds__(kCommitThreads) tree_commit_kernel(const Commi
     }
     __syncthreads();
 #pragma unroll
-    for (int kv = 0; kv < 2; ++kv) {
+    for (int kv = 0; kv < kPools; ++kv) {
       uint8_t *pool = static_cast<uint8_t *>(a.pool[kv]) + part;
       uint4 v[kEach];
       int64_t at[kEach];
@@ -577,6 +578,34 @@ extern "C" int b200kv_kv_load(const void *pool, int32_t pool_dtype, const float 
   }
 }
 
+namespace {
+
+// What both caches' commits check, and the arguments that do not depend on the cache.
+int commit_args(CommitArgs &a, const int32_t *block_table, int64_t block_table_stride, const int32_t *context_lens,
+                const int32_t *path, int64_t path_stride, const int32_t *path_lens, int32_t *new_lens, int64_t batch,
+                int64_t num_kv_heads, int64_t num_blocks, int64_t max_blocks_per_seq, int64_t max_path,
+                int32_t *error_flag) {
+  B200KV_CHECK_ARG(batch >= 0 && batch <= 65535, "batch %lld out of range", (long long)batch);
+  B200KV_CHECK_ARG(num_kv_heads > 0 && num_kv_heads <= 65536 && num_blocks > 0 && num_blocks < (int64_t{1} << 40) &&
+                       max_blocks_per_seq > 0 && max_blocks_per_seq * kPageTokens < (int64_t{1} << 30),
+                   "num_kv_heads, num_blocks or max_blocks_per_seq out of range");
+  B200KV_CHECK_ARG(block_table_stride >= max_blocks_per_seq, "block_table_stride < max_blocks_per_seq");
+  B200KV_CHECK_ARG(max_path >= 0 && max_path < (int64_t{1} << 30) && (path_stride >= max_path || path_stride == 0),
+                   "max_path out of range or path_stride < max_path");
+  B200KV_CHECK_ARG(batch == 0 || (block_table && context_lens && path_lens && new_lens && (path || max_path == 0)),
+                   "null pointer argument");
+  a.block_table = block_table, a.bt_stride = block_table_stride;
+  a.ctx = context_lens, a.path = path, a.path_stride = path_stride, a.path_lens = path_lens, a.new_lens = new_lens;
+  a.hkv = static_cast<int>(num_kv_heads);
+  a.max_blocks = static_cast<int>(max_blocks_per_seq);
+  a.max_path = static_cast<int>(max_path);
+  a.num_blocks = num_blocks;
+  a.error_flag = error_flag;
+  return B200KV_OK;
+}
+
+}  // namespace
+
 extern "C" int b200kv_tree_commit(void *k_pool, void *v_pool, int32_t pool_dtype, float *k_scales, float *v_scales,
                                   const int32_t *block_table, int64_t block_table_stride, const int32_t *context_lens,
                                   const int32_t *path, int64_t path_stride, const int32_t *path_lens,
@@ -587,27 +616,14 @@ extern "C" int b200kv_tree_commit(void *k_pool, void *v_pool, int32_t pool_dtype
   int st = check_cache(pool_dtype, head_dim, "pool");
   if (st != B200KV_OK) return st;
   const bool k8 = pool_dtype == B200KV_I8 || pool_dtype == B200KV_E4M3;
-  B200KV_CHECK_ARG(batch >= 0 && batch <= 65535, "batch %lld out of range", (long long)batch);
-  B200KV_CHECK_ARG(num_kv_heads > 0 && num_kv_heads <= 65536 && num_blocks > 0 && num_blocks < (int64_t{1} << 40) &&
-                       max_blocks_per_seq > 0 && max_blocks_per_seq * kPageTokens < (int64_t{1} << 30),
-                   "num_kv_heads, num_blocks or max_blocks_per_seq out of range");
-  B200KV_CHECK_ARG(block_table_stride >= max_blocks_per_seq, "block_table_stride < max_blocks_per_seq");
-  B200KV_CHECK_ARG(max_path >= 0 && max_path < (int64_t{1} << 30) && (path_stride >= max_path || path_stride == 0),
-                   "max_path out of range or path_stride < max_path");
-  if (batch == 0) return B200KV_OK;
-  B200KV_CHECK_ARG(k_pool && v_pool && block_table && context_lens && path_lens && new_lens && (path || max_path == 0),
-                   "null pointer argument");
+  CommitArgs a{};
+  st = commit_args(a, block_table, block_table_stride, context_lens, path, path_stride, path_lens, new_lens, batch,
+                   num_kv_heads, num_blocks, max_blocks_per_seq, max_path, error_flag);
+  if (st != B200KV_OK || batch == 0) return st;
+  B200KV_CHECK_ARG(k_pool && v_pool, "null pointer argument");
   B200KV_CHECK_ARG(!k8 || (k_scales && v_scales), "8-bit pools need k_scales and v_scales");
   B200KV_CHECK_ARG(aligned_to(k_pool, 16) && aligned_to(v_pool, 16), "pools must be 16-byte aligned");
-  CommitArgs a{};
   a.pool[0] = k_pool, a.pool[1] = v_pool, a.scales[0] = k_scales, a.scales[1] = v_scales;
-  a.block_table = block_table, a.bt_stride = block_table_stride;
-  a.ctx = context_lens, a.path = path, a.path_stride = path_stride, a.path_lens = path_lens, a.new_lens = new_lens;
-  a.hkv = static_cast<int>(num_kv_heads);
-  a.max_blocks = static_cast<int>(max_blocks_per_seq);
-  a.max_path = static_cast<int>(max_path);
-  a.num_blocks = num_blocks;
-  a.error_flag = error_flag;
   const dim3 grid(static_cast<unsigned>(num_kv_heads), static_cast<unsigned>(batch));
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (k8)
@@ -616,6 +632,26 @@ extern "C" int b200kv_tree_commit(void *k_pool, void *v_pool, int32_t pool_dtype
     tree_commit_kernel<128, 128, false><<<grid, kCommitThreads, 0, s>>>(a);
   else
     tree_commit_kernel<256, 128, false><<<grid, kCommitThreads, 0, s>>>(a);
+  B200KV_CUDA_TRY(cudaGetLastError());
+  return B200KV_OK;
+}
+
+extern "C" int b200kv_latent_commit(void *pool, int32_t dtype, const int32_t *block_table, int64_t block_table_stride,
+                                    const int32_t *context_lens, const int32_t *path, int64_t path_stride,
+                                    const int32_t *path_lens, int32_t *new_lens, int64_t batch, int64_t num_blocks,
+                                    int64_t max_blocks_per_seq, int64_t max_path, int32_t *error_flag, void *stream) {
+  clear_error();
+  B200KV_CHECK_ARG(dtype == B200KV_F16 || dtype == B200KV_BF16, "pool dtype %d is not fp16 or bf16", dtype);
+  constexpr int kSticks = (B200KV_LATENT_RANK + B200KV_LATENT_ROPE) / 64;
+  CommitArgs a{};
+  const int st = commit_args(a, block_table, block_table_stride, context_lens, path, path_stride, path_lens, new_lens,
+                             batch, kSticks, num_blocks, max_blocks_per_seq, max_path, error_flag);
+  if (st != B200KV_OK || batch == 0) return st;
+  B200KV_CHECK_ARG(pool, "null pointer argument");
+  B200KV_CHECK_ARG(aligned_to(pool, 16), "the pool must be 16-byte aligned");
+  a.pool[0] = pool;
+  tree_commit_kernel<128, 128, false, 1><<<dim3(kSticks, static_cast<unsigned>(batch)), kCommitThreads, 0,
+                                           static_cast<cudaStream_t>(stream)>>>(a);
   B200KV_CUDA_TRY(cudaGetLastError());
   return B200KV_OK;
 }

@@ -1,0 +1,196 @@
+"""Latent attention over a paged cache of one vector a token.
+
+A token's row has 512 latent elements, which every head takes as key and value,
+and 64 rotary key elements, also shared: 1152 bytes a token in fp16 or bf16, for
+any number of heads.  A head's own key (128 elements) and value (128) are
+products of the latent vector with the head's weights W_k, W_v [512, 128]:
+
+* absorbed (few new tokens): W_k is multiplied into the query, q W_k^T . c = q . W_k^T c,
+  and W_v into the output, so attention runs over the rows as they are cached
+  (:func:`latent_attention`);
+* expanded (prompts): the rows are multiplied out, once for all queries
+  (:func:`latent_prompt_attention`).
+
+* ``b200kv::latent_store(latent, k_rope, pool!, slots, ...)`` -- rows normalised,
+  turned and written, the heads' rotary queries turned beside them;
+* :func:`latent_load` -- rows gathered by slot; ``b200kv::latent_commit`` -- the
+  accepted path of a drafted tree, as :func:`torch_spyre_b200.tree_commit`.
+"""
+
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+
+from . import _eager
+from ._eager import direct, flag_ptr, launch, written
+from .kv_rows import DTYPES_16, _check_slots, kv_load
+from .layout import PAGE_TOKENS
+from .ops import _maybe_check_flag, _ptr, _require_cuda
+from .rotations import DTYPE_CODES, check_table
+from .tree import _check_sequences
+
+RANK, ROPE, NOPE = 512, 64, 128
+STICKS = (RANK + ROPE) // 64
+
+
+def empty_latent_pool(num_blocks: int, dtype: torch.dtype = torch.bfloat16, device=None) -> torch.Tensor:
+    """Uninitialised pages [num_blocks, 1, 9, 64, 64] of 64 rows each."""
+    if dtype not in DTYPES_16:
+        raise ValueError(f"latent pools are fp16 or bf16, not {dtype}")
+    return torch.empty((num_blocks, 1, STICKS, PAGE_TOKENS, 64), dtype=dtype, device=device)
+
+
+def _check_pool(pool: torch.Tensor) -> int:
+    if pool.dtype not in DTYPES_16 or pool.dim() != 5 or pool.shape[1:] != (1, STICKS, PAGE_TOKENS, 64) \
+            or not pool.is_contiguous():
+        raise ValueError(f"pool must be contiguous fp16 or bf16 [num_blocks, 1, {STICKS}, 64, 64], got "
+                         f"{tuple(pool.shape)} {pool.dtype}")
+    return pool.shape[0]
+
+
+def _latent_store_impl(
+    latent: torch.Tensor,
+    k_rope: torch.Tensor,
+    pool: torch.Tensor,
+    slots: torch.Tensor,
+    q_rope: Optional[torch.Tensor],
+    norm_weight: Optional[torch.Tensor],
+    eps: float,
+    table: Optional[torch.Tensor],
+    positions: Optional[torch.Tensor],
+    interleaved: bool,
+    error_flag: Optional[torch.Tensor],
+) -> torch.Tensor:
+    _require_cuda(latent, k_rope, pool, slots)
+    NB, device, dtype = _check_pool(pool), pool.device, pool.dtype
+    N = latent.shape[0] if latent.dim() == 2 else -1
+    for rows, name, width in ((latent, "latent", RANK), (k_rope, "k_rope", ROPE)):
+        if rows.shape != (N, width) or rows.dtype != dtype or rows.stride(1) != 1 or rows.device != device:
+            raise ValueError(f"{name} must be [N, {width}] of the pool's dtype with contiguous rows on its device, got "
+                             f"{tuple(rows.shape)} {rows.dtype}")
+    _check_slots(slots, N, device)
+    if norm_weight is not None and (norm_weight.dtype != dtype or norm_weight.shape != (RANK,)
+                                    or not norm_weight.is_contiguous() or norm_weight.device != device):
+        raise ValueError(f"norm_weight must be contiguous [{RANK}] of the pool's dtype on its device")
+    if q_rope is not None:
+        if table is None:
+            raise ValueError("q_rope is taken to be turned: it needs a table")
+        if q_rope.dim() != 3 or q_rope.shape[0] != N or q_rope.shape[2] != ROPE or q_rope.dtype != dtype \
+                or q_rope.stride(2) != 1 or q_rope.device != device:
+            raise ValueError(f"q_rope must be [N, H, {ROPE}] of the pool's dtype with contiguous rows on its device")
+        H, q_args = q_rope.shape[1], (q_rope.data_ptr(), q_rope.stride(0), q_rope.stride(1))
+    else:
+        H, q_args = 0, (None, 0, 0)
+    out = latent.new_empty((N, H, ROPE))
+    if table is not None:
+        if positions is None:
+            raise ValueError("a table needs positions")
+        check_table(table, positions, N, ROPE, device)
+        if table.shape[1] != ROPE // 2:
+            raise ValueError(f"the table must turn all {ROPE} elements, it turns {2 * table.shape[1]}")
+    launch("b200kv_latent_store", device, latent.data_ptr(), latent.stride(0), k_rope.data_ptr(), k_rope.stride(0),
+           *q_args, out.data_ptr(), DTYPE_CODES[dtype], _ptr(norm_weight), eps, pool.data_ptr(), slots.data_ptr(),
+           _ptr(table), 0 if table is None else table.shape[0], _ptr(positions), interleaved, N, H, NB,
+           flag_ptr(error_flag, device))
+    _maybe_check_flag(error_flag, "latent_store")
+    return out
+
+
+_latent_store_op = torch.library.custom_op("b200kv::latent_store", _latent_store_impl, device_types="cuda",
+                                           mutates_args=("pool",))
+
+
+@_latent_store_op.register_fake
+def _(latent, k_rope, pool, slots, q_rope, norm_weight, eps, table, positions, interleaved, error_flag):
+    return latent.new_empty((latent.shape[0], 0 if q_rope is None else q_rope.shape[1], ROPE))
+
+
+def latent_store(
+    latent: torch.Tensor,
+    k_rope: torch.Tensor,
+    pool: torch.Tensor,
+    slots: torch.Tensor,
+    q_rope: Optional[torch.Tensor] = None,
+    norm_weight: Optional[torch.Tensor] = None,
+    eps: float = 1e-6,
+    table: Optional[torch.Tensor] = None,
+    positions: Optional[torch.Tensor] = None,
+    interleaved: bool = False,
+    error_flag: Optional[torch.Tensor] = None,
+) -> Optional[torch.Tensor]:
+    """Writes token n's row, latent[n] ([N, 512]) and k_rope[n] ([N, 64]), to slot
+    slots[n] of the pool, in one launch (strided rows will do, so both may be parts of
+    one projection's output).
+
+    With ``norm_weight`` [512] the latent part is x / sqrt(mean(x^2) + eps) * weight.
+    With ``table`` ([max_pos, 32, 2], :func:`torch_spyre_b200.rotary_table`) and
+    ``positions`` the key part is turned, and so is ``q_rope`` [N, H, 64] beside it,
+    which is returned.  fp32 arithmetic, rounded once.  Slots must be distinct;
+    negative slots skip their row."""
+    args = (latent, k_rope, pool, slots, q_rope, norm_weight, float(eps), table, positions, bool(interleaved), error_flag)
+    out = None if _eager.compiling() else _eager.fast.latent_store(*args)
+    if out is None:
+        if direct(latent, k_rope, pool, slots, q_rope, norm_weight, table, positions):
+            out = _latent_store_impl(*args)
+            written(pool)
+        else:
+            out = torch.ops.b200kv.latent_store(*args)
+    return None if q_rope is None else out
+
+
+def latent_load(pool: torch.Tensor, slots: torch.Tensor, dtype: Optional[torch.dtype] = None,
+                error_flag: Optional[torch.Tensor] = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """(latent [N, 512], k_rope [N, 64]) of the rows at ``slots``, two views of one
+    contiguous [N, 576] tensor (dtype fp16, bf16 or fp32; default the pool's).
+    Negative slots give rows of zeros."""
+    NB = _check_pool(pool)
+    rows = kv_load(pool.view(NB, STICKS, 1, PAGE_TOKENS, 64), slots, dtype=dtype, error_flag=error_flag)
+    rows = rows.view(-1, RANK + ROPE)
+    return rows[:, :RANK], rows[:, RANK:]
+
+
+# ------------------------------------------------------------------- commit --
+def _latent_commit_impl(pool: torch.Tensor, block_table: torch.Tensor, context_lens: torch.Tensor, path: torch.Tensor,
+                        path_lens: torch.Tensor, error_flag: Optional[torch.Tensor]) -> torch.Tensor:
+    _require_cuda(pool, block_table, context_lens, path, path_lens)
+    NB, device = _check_pool(pool), pool.device
+    B = _check_sequences(block_table, context_lens, device)
+    if path.dtype != torch.int32 or path.dim() != 2 or len(path) != B or (path.shape[1] > 1 and path.stride(1) != 1) \
+            or path.device != device:
+        raise ValueError("path must be int32 [B, max_path] with unit column stride on the pool's device")
+    if path_lens.dtype != torch.int32 or path_lens.dim() != 1 or len(path_lens) != B \
+            or not path_lens.is_contiguous() or path_lens.device != device:
+        raise ValueError("path_lens must be a contiguous int32 [B] tensor on the pool's device")
+    new_lens = torch.empty_like(context_lens)
+    launch("b200kv_latent_commit", device, pool.data_ptr(), DTYPE_CODES[pool.dtype], block_table.data_ptr(),
+           block_table.stride(0), context_lens.data_ptr(), path.data_ptr(), path.stride(0) if B > 1 else path.shape[1],
+           path_lens.data_ptr(), new_lens.data_ptr(), B, NB, block_table.shape[1], path.shape[1],
+           flag_ptr(error_flag, device))
+    _maybe_check_flag(error_flag, "latent_commit")
+    return new_lens
+
+
+_latent_commit_op = torch.library.custom_op("b200kv::latent_commit", _latent_commit_impl, device_types="cuda",
+                                            mutates_args=("pool",))
+
+
+@_latent_commit_op.register_fake
+def _(pool, block_table, context_lens, path, path_lens, error_flag):
+    return torch.empty_like(context_lens)
+
+
+def latent_commit(pool: torch.Tensor, block_table: torch.Tensor, context_lens: torch.Tensor, path: torch.Tensor,
+                  path_lens: torch.Tensor, error_flag: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """:func:`torch_spyre_b200.tree_commit` for a latent pool: moves the rows of the
+    accepted nodes path[b, :path_lens[b]] to positions context_lens[b] on, in place,
+    and returns the new lengths."""
+    args = (pool, block_table, context_lens, path, path_lens, error_flag)
+    new_lens = None if _eager.compiling() else _eager.fast.latent_commit(*args)
+    if new_lens is None:
+        if not direct(pool, block_table, context_lens, path, path_lens):
+            return torch.ops.b200kv.latent_commit(*args)
+        new_lens = _latent_commit_impl(*args)
+        written(pool)
+    return new_lens

@@ -9,6 +9,9 @@ their K/V rows sit in the cache right after the committed tokens
 * ``b200kv::tree_attention(q, k_pool, v_pool, block_table, context_lens, q_indptr, ...)``
   -- attention of all nodes over committed tokens and visible nodes; without a
   mask the nodes form a chain (several tokens of one sequence, a prompt chunk);
+* ``b200kv::tree_verify(parents, tokens, q_indptr, target_probs, ...)`` -- once per
+  step, the accepted path and the token that comes next, from the target's and
+  the drafter's probabilities and given random numbers;
 * ``b200kv::tree_commit(k_pool!, v_pool!, ...)`` -- the accepted path's rows moved
   to the end of the committed tokens.
 """
@@ -24,7 +27,7 @@ from . import _eager, _lib
 from ._eager import direct, flag_ptr, launch, written
 from .kv_rows import DTYPES_16, check_row_pools
 from .ops import _maybe_check_flag, _ptr, _require_cuda, workspace_for
-from .rotations import DTYPE_CODES
+from .rotations import DTYPE_CODES, ROTARY_DTYPES
 
 
 def _check_sequences(block_table: torch.Tensor, context_lens: torch.Tensor, device: torch.device) -> int:
@@ -190,6 +193,107 @@ def tree_attention(
         pair = _attend(*args, return_lse) if plain else torch.ops.b200kv.tree_attention(*args)
     out, lse = pair
     return (out, lse) if return_lse else out
+
+
+# ------------------------------------------------------------------- verify --
+def _check_probs(probs: torch.Tensor, name: str, nodes: int, device: torch.device) -> None:
+    if probs.dim() != 2 or len(probs) != nodes or probs.dtype not in ROTARY_DTYPES or probs.device != device \
+            or probs.shape[1] < 1 or (probs.shape[1] > 1 and probs.stride(1) != 1):
+        raise ValueError(f"{name} must be fp16, bf16 or fp32 [{nodes}, vocab] with contiguous rows on parents' device, "
+                         f"got {tuple(probs.shape)} {probs.dtype}")
+
+
+def _tree_verify_impl(
+    parents: torch.Tensor,
+    tokens: torch.Tensor,
+    q_indptr: torch.Tensor,
+    target_probs: torch.Tensor,
+    accept_u: torch.Tensor,
+    sample_u: torch.Tensor,
+    draft_probs: Optional[torch.Tensor],
+    max_path: int,
+    error_flag: Optional[torch.Tensor],
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    _require_cuda(parents, tokens, q_indptr, target_probs, accept_u, sample_u)
+    if parents.dtype != torch.int32 or parents.dim() != 1 or not parents.is_contiguous():
+        raise ValueError("parents must be a contiguous int32 [N] tensor")
+    N, device = parents.shape[0], parents.device
+    if q_indptr.dim() != 1 or q_indptr.shape[0] < 1:
+        raise ValueError("q_indptr must be int32 [B + 1]")
+    B = q_indptr.shape[0] - 1
+    _check_indptr(q_indptr, B, device)
+    for t, name, n, dtype in ((tokens, "tokens", N, torch.int64), (accept_u, "accept_u", N, torch.float32),
+                              (sample_u, "sample_u", B, torch.float32)):
+        if t.dtype != dtype or t.dim() != 1 or len(t) != n or not t.is_contiguous() or t.device != device:
+            raise ValueError(f"{name} must be a contiguous {str(dtype)[6:]} [{n}] tensor on parents' device")
+    _check_probs(target_probs, "target_probs", N, device)
+    if draft_probs is not None:
+        _check_probs(draft_probs, "draft_probs", N, device)
+        if draft_probs.dtype != target_probs.dtype or draft_probs.shape != target_probs.shape:
+            raise ValueError("draft_probs must have target_probs' dtype and shape")
+    if max_path < 1:
+        raise ValueError(f"max_path must be >= 1, got {max_path}")
+    path = torch.empty((B, max_path), dtype=torch.int32, device=device)
+    path_lens = torch.empty(B, dtype=torch.int32, device=device)
+    next_tokens = torch.empty(B, dtype=torch.int64, device=device)
+    launch("b200kv_tree_verify", device, parents.data_ptr(), tokens.data_ptr(), q_indptr.data_ptr(),
+           target_probs.data_ptr(), target_probs.stride(0), _ptr(draft_probs),
+           0 if draft_probs is None else draft_probs.stride(0), DTYPE_CODES[target_probs.dtype], accept_u.data_ptr(),
+           sample_u.data_ptr(), path.data_ptr(), path_lens.data_ptr(), next_tokens.data_ptr(), N, B,
+           target_probs.shape[1], max_path, flag_ptr(error_flag, device))
+    _maybe_check_flag(error_flag, "tree_verify")
+    return path, path_lens, next_tokens
+
+
+_tree_verify_op = torch.library.custom_op("b200kv::tree_verify", _tree_verify_impl, mutates_args=(), device_types="cuda")
+
+
+@_tree_verify_op.register_fake
+def _(parents, tokens, q_indptr, target_probs, accept_u, sample_u, draft_probs, max_path, error_flag):
+    B = q_indptr.shape[0] - 1
+    return parents.new_empty((B, max_path)), parents.new_empty(B), parents.new_empty(B, dtype=torch.int64)
+
+
+def tree_verify(
+    parents: torch.Tensor,
+    tokens: torch.Tensor,
+    q_indptr: torch.Tensor,
+    target_probs: torch.Tensor,
+    accept_u: torch.Tensor,
+    sample_u: torch.Tensor,
+    draft_probs: Optional[torch.Tensor] = None,
+    max_path: Optional[int] = None,
+    error_flag: Optional[torch.Tensor] = None,
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Which drafted tokens stay, and what comes after them.
+
+    Node 0 of a sequence is its last token (always taken), node i the drafted
+    tokens[i] (int64 [N]) after node parents[i] (int32 [N], as for
+    :func:`tree_mask`; negative: not tried).  target_probs [N, vocab] (fp16, bf16,
+    fp32): the target's distribution after each node; draft_probs (same type and
+    shape): the one its children were drawn from independently, None where
+    they were chosen without chance (a list of likely tokens).  accept_u fp32 [N]
+    and sample_u fp32 [B] are uniform random numbers in [0, 1).
+
+    From node 0 on a node's children are tried in their order: x stays if
+    u * q(x) < p(x); else p becomes max(p - q, 0) over its sum (without draft_probs:
+    p without x over its sum), and the next one is tried against that.  Where none
+    stays, the next token is drawn from the p of that moment.  So the
+    sequence's tokens have the target's distribution, whatever the drafter's is.
+    64-bit arithmetic.
+
+    Returns path int32 [B, max_path] (the nodes that stay, 0 first, then -1; at
+    most ``max_path``, default N), path_lens int32 [B], as :func:`tree_commit`
+    takes them, and next_tokens int64 [B].  At most 1024 nodes a sequence."""
+    if max_path is None:
+        max_path = max(1, parents.shape[0])
+    args = (parents, tokens, q_indptr, target_probs, accept_u, sample_u, draft_probs, int(max_path), error_flag)
+    out = None if _eager.compiling() else _eager.fast.tree_verify(*args)
+    if out is None:
+        op = _tree_verify_impl if direct(parents, tokens, q_indptr, target_probs, accept_u, sample_u, draft_probs) \
+            else torch.ops.b200kv.tree_verify
+        out = op(*args)
+    return out
 
 
 # ------------------------------------------------------------------- commit --
