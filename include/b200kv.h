@@ -819,6 +819,33 @@ B200KV_API int b200kv_latent_commit(void *pool, int32_t dtype, const int32_t *bl
                                     int64_t num_blocks, int64_t max_blocks_per_seq,
                                     int64_t max_path, int32_t *error_flag, void *stream);
 
+/* Workspace bytes of b200kv_latent_attention (-1: unsupported shape), under the
+ * rules of b200kv_tree_workspace_bytes (the two may share one). */
+B200KV_API int64_t b200kv_latent_workspace_bytes(int64_t total_q, int64_t batch, int64_t num_heads);
+
+/* Latent attention, absorbed form: b200kv_tree_attention over a latent pool.  Sequence
+ * b's nodes, which committed tokens and nodes they see, the mask, clamped lengths and
+ * rows that no sequence has are as there; every head of a node scores token p by
+ *   scale * (q_latent[t, h] . latent_p + q_rope[t, h] . k_rope_p)
+ * and gets the weighted sum of the latent parts.
+ *   q_latent  of the pool's dtype, row (t, h) of 512 elements at q_latent[t *
+ *             q_latent_stride_t + h * q_latent_stride_h]; q_rope likewise, 64
+ *             elements; 16-byte aligned, strides positive multiples of 8
+ *   out       contiguous [total_q, H, 512]; lse fp32 [total_q, H] or NULL
+ * Supported: H <= 512, batch <= 1024, total_q * H < 2^31, max_blocks_per_seq < 2^24
+ * and (batch + total_q / max(1, 64 / H) + 1) * (max_blocks_per_seq + 4) < 2^31. */
+B200KV_API int b200kv_latent_attention(const void *q_latent, int64_t q_latent_stride_t,
+                                       int64_t q_latent_stride_h, const void *q_rope,
+                                       int64_t q_rope_stride_t, int64_t q_rope_stride_h,
+                                       int32_t dtype, const void *pool, const int32_t *block_table,
+                                       int64_t block_table_stride, const int32_t *context_lens,
+                                       const int32_t *q_indptr, const int64_t *tree_mask,
+                                       int64_t mask_words, void *out, float *lse, int64_t total_q,
+                                       int64_t batch, int64_t num_heads, int64_t num_blocks,
+                                       int64_t max_blocks_per_seq, int64_t max_nodes, float scale,
+                                       void *workspace, int64_t workspace_bytes,
+                                       int32_t *error_flag, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

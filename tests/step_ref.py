@@ -4,6 +4,8 @@ import math
 
 import torch
 
+from tests.verify_ref import _weigh, pack_bits, random_tree, see_of
+
 
 # ------------------------------------------------------------------- pages --
 class Pages:
@@ -111,3 +113,74 @@ def turn(x, angle, interleaved):
     out[..., a] = x[..., a] * c - x[..., b] * s
     out[..., b] = x[..., b] * c + x[..., a] * s
     return out
+
+
+class LatentCase:
+    """One call's inputs: ragged contexts and drafts over a permuted pool, everything else in it NaN."""
+
+    def __init__(self, ctx, nodes, heads, dtype=torch.bfloat16, chain=False, dead=0.0, seed=0, qscale=1.0, poison=True,
+                 device="cuda"):
+        g = torch.Generator(device=device).manual_seed(seed)
+        gc = torch.Generator().manual_seed(seed + 1)
+        need = [-(-(c + t) // 64) for c, t in zip(ctx, nodes)]
+        nb = sum(need) + 3
+        order = torch.randperm(nb, generator=gc)
+        self.block_table = torch.full((len(ctx), max(max(need), 1)), -7, dtype=torch.int32)
+        at = 0
+        for b, n in enumerate(need):
+            self.block_table[b, :n] = order[at:at + n].int()
+            at += n
+        self.ctx, self.nodes, self.heads = ctx, nodes, heads
+        self.pool = torch.randn((nb, 1, 9, 64, 64), generator=g, device=device).to(dtype)
+        self.block_table = self.block_table.to(device)
+        if poison:
+            owned = torch.zeros(nb * 64, dtype=torch.bool, device=device)
+            for b, (c, t) in enumerate(zip(ctx, nodes)):
+                owned[self.slots(b, 0, c + t)] = True
+            self.pool.permute(0, 3, 1, 2, 4)[~owned.view(nb, 64)] = float("nan")
+        self.context_lens = torch.tensor(ctx, dtype=torch.int32, device=device)
+        self.indptr = [0]
+        for t in nodes:
+            self.indptr.append(self.indptr[-1] + t)
+        self.q_indptr = torch.tensor(self.indptr, dtype=torch.int32, device=device)
+        n = self.indptr[-1]
+        self.q_latent = (torch.randn((n, heads, 512), generator=g, device=device) * qscale).to(dtype)
+        self.q_rope = (torch.randn((n, heads, 64), generator=g, device=device) * qscale).to(dtype)
+        self.max_nodes = max(max(nodes), 1)
+        if chain:
+            self.see = [torch.ones(t, t, dtype=torch.bool).tril() for t in nodes]
+            self.mask = None
+        else:
+            self.see = [see_of(random_tree(t, gc, dead)) for t in nodes]
+            self.mask = torch.cat([pack_bits(s, -(-self.max_nodes // 64)) for s in self.see]).to(device)
+
+    def slots(self, b, start, stop):
+        p = torch.arange(start, stop, device=self.block_table.device)
+        return self.block_table[b].long()[p // 64] * 64 + p % 64
+
+    def args(self):
+        return self.q_latent, self.q_rope, self.pool, self.block_table, self.context_lens, self.q_indptr
+
+    def kwargs(self):
+        return dict(tree_mask=self.mask, max_nodes=self.max_nodes)
+
+    def reference(self, scale=None):
+        """(out, lse, spread) in 64 bits; spread = sum of weight * |latent|, what the error bound goes by."""
+        scale = 192**-0.5 if scale is None else scale
+        outs, lses, spreads = [], [], []
+        for b, (c, t) in enumerate(zip(self.ctx, self.nodes)):
+            if t == 0:
+                continue
+            rows = latent_rows(self.pool, self.slots(b, 0, c + t))
+            part = slice(self.indptr[b], self.indptr[b + 1])
+            q = torch.cat([self.q_latent[part], self.q_rope[part]], -1).double()
+            s = torch.einsum("thd,pd->htp", q, rows) * scale
+            see = torch.cat([torch.ones(t, c, dtype=torch.bool), self.see[b]], 1).to(s.device)
+            s = s.masked_fill(~see, -math.inf)
+            lse = torch.logsumexp(s, -1)
+            w = torch.where(see & (lse[..., None] > -math.inf), torch.exp(s - lse[..., None]), 0.0)
+            v = rows[:, None, :512].expand(-1, self.heads, -1)
+            outs.append(_weigh(w, v))
+            spreads.append(_weigh(w, v.abs()))
+            lses.append(lse.transpose(0, 1))
+        return torch.cat(outs), torch.cat(lses), torch.cat(spreads)

@@ -10,7 +10,7 @@ import pytest
 import torch
 
 import torch_spyre_b200 as tsb
-from step_ref import latent_rows, turn
+from tests.step_ref import latent_rows, turn
 from torch_spyre_b200 import _lib
 
 pytestmark = pytest.mark.gpu

@@ -12,7 +12,7 @@ import pytest
 import torch
 
 import torch_spyre_b200 as tsb
-from step_ref import Pages, verify
+from tests.step_ref import Pages, verify
 from torch_spyre_b200 import _lib
 
 pytestmark = pytest.mark.gpu

@@ -40,7 +40,8 @@ compiling = torch.compiler.is_compiling
 # the order of Entries in csrc/fast_call.cpp
 _ENTRIES = ("b200kv_rotary", "b200kv_kv_store", "b200kv_kv_load", "b200kv_tree_mask", "b200kv_tree_workspace_bytes",
             "b200kv_tree_attention", "b200kv_tree_commit", "b200kv_extend_pages", "b200kv_release_pages",
-            "b200kv_tree_verify", "b200kv_latent_store", "b200kv_latent_commit")
+            "b200kv_tree_verify", "b200kv_latent_store", "b200kv_latent_commit",
+            "b200kv_latent_workspace_bytes", "b200kv_latent_attention")
 
 
 class _Absent:

@@ -323,6 +323,17 @@ SIGNATURES = {
         ctypes.c_int,
         [_p, _i32, _p, _i64, _p, _p, _i64, _p, _p, _i64, _i64, _i64, _i64, _p, _p],
     ),
+    "b200kv_latent_workspace_bytes": (_i64, [_i64, _i64, _i64]),
+    "b200kv_latent_attention": (
+        ctypes.c_int,
+        [
+            _p, _i64, _i64, _p, _i64, _i64, _i32,  # q_latent, q_rope with their strides, dtype
+            _p, _p, _i64, _p, _p, _p, _i64,  # pool, block_table, stride, context_lens, q_indptr, tree_mask, words
+            _p, _p, _i64, _i64, _i64,  # out, lse, total_q, batch, heads
+            _i64, _i64, _i64, _f32,  # num_blocks, max_blocks_per_seq, max_nodes, scale
+            _p, _i64, _p, _p,  # workspace, workspace_bytes, error_flag, stream
+        ],
+    ),
 }
 
 

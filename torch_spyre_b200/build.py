@@ -52,6 +52,7 @@ SOURCES = [
     "tree_verify.cu",
     "pages.cu",
     "latent_rows.cu",
+    "latent_attention.cu",
     "lse_combine.cu",
     "oproj_allreduce.cu",
 ]

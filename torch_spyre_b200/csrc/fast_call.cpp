@@ -53,6 +53,11 @@ struct Entries {
                       int64_t, int64_t, int64_t, int32_t *, void *);
   int (*latent_commit)(void *, int32_t, const int32_t *, int64_t, const int32_t *, const int32_t *, int64_t,
                        const int32_t *, int32_t *, int64_t, int64_t, int64_t, int64_t, int32_t *, void *);
+  int64_t (*latent_workspace_bytes)(int64_t, int64_t, int64_t);
+  int (*latent_attention)(const void *, int64_t, int64_t, const void *, int64_t, int64_t, int32_t, const void *,
+                          const int32_t *, int64_t, const int32_t *, const int32_t *, const int64_t *, int64_t, void *,
+                          float *, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, float, void *, int64_t, int32_t *,
+                          void *);
 } entries;
 bool bound = false;
 
@@ -555,6 +560,52 @@ PyObject *latent_commit(PyObject *, PyObject *const *a, Py_ssize_t n) {
   return THPVariable_Wrap(std::move(out));
 }
 
+// (out, lse or None)
+PyObject *out_and_lse(at::Tensor &&out, at::Tensor &&lse) {
+  if (lse.defined()) return pack({out, lse});
+  PyObject *o = THPVariable_Wrap(std::move(out));
+  PyObject *pair = o ? PyTuple_Pack(2, o, Py_None) : nullptr;
+  Py_XDECREF(o);
+  return pair;
+}
+
+// latent_attention(q_latent, q_rope, pool, block_table, context_lens, q_indptr, mask, scale, max_nodes, error_flag,
+//                  want_lse) -> (out, lse or None)
+PyObject *latent_attention(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  B200KV_ARGS(11)
+  Call c;
+  const at::Tensor *q = c.tensor(a[0]), *qr = c.tensor(a[1]), *pool = c.tensor(a[2]), *table = c.tensor(a[3]),
+                   *lens = c.tensor(a[4]), *indptr = c.tensor(a[5]), *mask = c.optional(a[6]);
+  const double scale = PyFloat_AsDouble(a[7]);
+  if (scale == -1.0 && PyErr_Occurred()) {
+    PyErr_Clear();
+    Py_RETURN_NONE;
+  }
+  const int64_t max_nodes = c.integer(a[8]);
+  int32_t *flag = c.flag(a[9]);
+  if (!c.ok || !latent_pool_ok(pool) || !rows_ok(q) || !rows_ok(qr) || !sequences_ok(table, lens)) Py_RETURN_NONE;
+  const int64_t N = q->size(0), heads = q->size(1), batch = table->size(0);
+  const at::ScalarType type = pool->scalar_type();
+  c.need(q->scalar_type() == type && qr->scalar_type() == type && q->size(2) == kRank && qr->size(0) == N &&
+         qr->size(1) == heads && qr->size(2) == kRope && vector_of(indptr, at::kInt, batch + 1));
+  if (c.ok && mask) c.need(mask->scalar_type() == at::kLong && mask->dim() == 2 && mask->size(0) == N && mask->is_contiguous());
+  if (!c.ok || N == 0) Py_RETURN_NONE;
+  const c10::cuda::CUDAGuard guard(c.device);
+  void *stream = stream_of(c);
+  const auto ws = workspaces().find(Key(c.device.index(), stream));
+  const int64_t bytes = entries.latent_workspace_bytes(N, batch, heads);
+  if (ws == workspaces().end() || bytes <= 0 || ws->second.numel() < bytes) Py_RETURN_NONE;
+  at::Tensor out = at::empty({N, heads, kRank}, q->options()), lse;
+  if (a[10] == Py_True) lse = at::empty({N, heads}, q->options().dtype(at::kFloat));
+  const int st = entries.latent_attention(
+      data(q), q->stride(0), q->stride(1), data(qr), qr->stride(0), qr->stride(1), code_of(type), data(pool), ints(table),
+      table->stride(0), ints(lens), ints(indptr), static_cast<const int64_t *>(data(mask)), mask ? mask->size(1) : 0,
+      out.data_ptr(), lse.defined() ? static_cast<float *>(lse.data_ptr()) : nullptr, N, batch, heads, pool->size(0),
+      table->size(1), max_nodes, static_cast<float>(scale), ws->second.data_ptr(), ws->second.numel(), flag, stream);
+  if (st != 0) Py_RETURN_NONE;
+  return out_and_lse(std::move(out), std::move(lse));
+}
+
 // bind(addresses): the C entries in the order of Entries
 PyObject *bind(PyObject *, PyObject *const *a, Py_ssize_t n) {
   B200KV_ARGS(static_cast<Py_ssize_t>(sizeof(Entries) / sizeof(void *)))
@@ -597,7 +648,7 @@ PyObject *guarded(PyObject *self, PyObject *const *a, Py_ssize_t n) {
 PyMethodDef methods[] = {B200KV_METHOD(rotary),         B200KV_METHOD(kv_store),    B200KV_METHOD(kv_load),
                          B200KV_METHOD(tree_mask),      B200KV_METHOD(tree_attention), B200KV_METHOD(tree_commit),
                          B200KV_METHOD(extend_pages),   B200KV_METHOD(release_pages), B200KV_METHOD(tree_verify),
-                         B200KV_METHOD(latent_store),   B200KV_METHOD(latent_commit),
+                         B200KV_METHOD(latent_store),   B200KV_METHOD(latent_commit), B200KV_METHOD(latent_attention),
                          B200KV_METHOD(bind),           B200KV_METHOD(set_workspace), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_fast", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -1,0 +1,835 @@
+// Tensor-core kernel of latent attention in the absorbed form (latent_attention.cu
+// has the operator): cached rows c = (512 latent, 64 rotary) are key and value of
+// all heads, so the rows of one product are a sequence's nodes times its heads,
+// and a token's 1152 bytes serve all of them.
+//
+// A CTA holds a tile of up to 64 rows (node-major; more than 64 heads: 64 of them,
+// and `parts` neighbouring CTAs walk the same tokens, which L2 then serves but once
+// from memory) and goes over pages of 64 tokens:
+//   S [64 rows, 64 tokens]  = Q K^T        9 sticks of 64 elements
+//   O^T [512, rows]        += V^T P^T      4 products of 128 latent elements
+// O is kept transposed: as M = 128 latent elements by N = rows it takes 256 TMEM
+// columns and the products run at the full rate whatever the number of rows; with
+// rows on M it would take all 512.  V^T is the page as it lies (tokens are the
+// reduction, their 64-element sticks M-major), P goes through shared memory.
+//
+// The cache's page is loaded once, as four pairs of sticks and the rotary stick;
+// a pair is free again once O has taken it.  Eight pairs are held, so the MMA
+// warp takes whichever is ready first: the next page's scores, stick by stick as
+// they arrive, or this page's values, as soon as its weights are there.
+//
+// The blocks' pages, all sequences one after the other, form one line that is cut
+// into equal shares; blocks cut by a share's end are joined by latent_join_kernel.
+//
+// Warps: 0-3 softmax and output (thread = row: lanes 0-15 of warp w have rows
+// 16w .. 16w + 15, where an M = 64 accumulator lies), 4 TMA producer, 5 MMA issuer.
+#pragma once
+
+#include "latent_attention.h"
+#include "umma.cuh"
+
+namespace b200kv {
+namespace latent {
+
+using namespace umma;
+
+constexpr int kThreads = 192;
+constexpr int kTile = kPageTokens;
+constexpr int kStickTile = kTile * 128, kPair = 2 * kStickTile, kPairs = 4, kSlots = 8;
+constexpr float kLazyLog2 = 8.f;
+constexpr int kOffQ = 2048;
+constexpr int kOffP = kOffQ + kSticks * kStickTile;
+constexpr int kOffRope = kOffP + 2 * kStickTile;
+constexpr int kOffSlots = kOffRope + kStickTile;
+constexpr int kSmem = kOffSlots + kSlots * kPair;
+static_assert(kSmem <= 227 * 1024, "shared memory per CTA");
+
+// TMEM columns: O^T, 64 for each 128 latent elements, and two score buffers
+constexpr uint32_t kTmemCols = 512;
+__device__ __forceinline__ uint32_t col_o(int m) { return uint32_t(m) * 64u; }
+__device__ __forceinline__ uint32_t col_s(int b) { return 256u + uint32_t(b) * 64u; }
+
+struct Seq {
+  int ctx, nodes, q0, blocks;
+  int end;  // the first row of q that is a later sequence's
+};
+struct Start {  // where a share of the line begins: in block `block`, whose units begin at u0
+  Seq s;
+  int b, block, u0;
+};
+
+struct Ctrl {
+  uint64_t full[kSlots], empty[kSlots], rope_full, rope_empty;
+  uint64_t q_full, q_empty;
+  uint64_t s_full[2], p_ready[2], p_free[2], o_full, o_empty;
+  uint32_t tmem;
+  int per, total;  // units of a share, of the line
+  Start start;
+  int scan[kThreads / 32];
+  unsigned bad_piece;  // last piece (counted from 1) that met a non-finite value in a node's row
+  float factor[kTileRows];  // of O's columns
+  int row_at[kTileRows];    // row of out, -1: none
+};
+static_assert(sizeof(Ctrl) <= kOffQ, "control block");
+
+__device__ __forceinline__ bool mbar_test(uint64_t *bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ void bar_softmax() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+__device__ __forceinline__ bool any_softmax(bool x) {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+               : "=r"(r)
+               : "r"(uint32_t(x))
+               : "memory");
+  return r != 0;
+}
+
+// -------------------------------------------------------------------- plan --
+__device__ __forceinline__ Seq load_seq(const Args &a, int b, bool report) {
+  const int cap = a.max_blocks * kPageTokens;
+  Seq s;
+  s.ctx = __ldg(a.ctx + b);
+  s.q0 = __ldg(a.indptr + b);
+  const int end = __ldg(a.indptr + b + 1);
+  bool bad = s.ctx < 0 || s.ctx > cap || s.q0 < 0 || end < s.q0 || end > a.total_q || (b == 0 && s.q0 != 0) ||
+             (b == a.batch - 1 && end != a.total_q);
+  s.ctx = min(max(s.ctx, 0), cap);
+  s.q0 = min(max(s.q0, 0), a.total_q);
+  s.nodes = min(max(end, s.q0), a.total_q) - s.q0;
+  s.end = b == a.batch - 1 ? a.total_q : min(max(end, 0), a.total_q);
+  const int most = min(a.max_nodes, cap - s.ctx);
+  bad = bad || s.nodes > most;
+  s.nodes = min(s.nodes, most);
+  if (bad && report && a.error_flag) atomicOr(a.error_flag, B200KV_DEVERR_BAD_LEN);
+  s.blocks = (s.nodes + a.tile_nodes - 1) / a.tile_nodes;
+  return s;
+}
+// Pages of block k: what its last node can see.
+__device__ __forceinline__ int block_tiles(const Args &a, const Seq &s, int k) {
+  const int nodes = a.mask ? s.nodes : min(s.nodes, (k + 1) * a.tile_nodes);
+  return (s.ctx + nodes + kTile - 1) / kTile;
+}
+// The line is cut by cost: a page counts one, a block's beginning and end kBegin.
+constexpr int kBegin = 4;
+__device__ __forceinline__ int block_units(const Args &a, const Seq &s, int k) { return kBegin + block_tiles(a, s, k); }
+__device__ __forceinline__ int seq_units(const Args &a, const Seq &s) {
+  if (a.mask) return s.blocks > 0 ? s.blocks * block_units(a, s, 0) : 0;
+  int n = 0;
+  for (int k = 0; k < s.blocks; ++k) n += block_units(a, s, k);
+  return n;
+}
+
+// The blocks of a share, one piece (a block, or the part of it in this share) at
+// a time.  Every role walks the same sequence.
+struct Walk {
+  Seq s;
+  int b, block, u0, tiles, t0, t1;  // piece: pages [t0, t1) of `tiles`
+  int first, end;                   // of the share
+
+  __device__ __forceinline__ void init(const Args &a, const Ctrl &c) {
+    const Start &f = c.start;
+    s = f.s, b = f.b, block = f.block, u0 = f.u0;
+    t0 = t1 = 0;
+    const int share = static_cast<int>(blockIdx.x) / a.parts;
+    first = share * c.per;
+    end = min(c.total, first + c.per);
+  }
+  // Page t belongs to the share that holds its unit; the begin goes with the first.
+  __device__ __forceinline__ int tile_from(int unit) const { return min(max(unit - u0 - kBegin, 0), tiles); }
+  __device__ __forceinline__ bool next(const Args &a) {
+    for (;;) {
+      if (u0 >= end || first >= end) return false;
+      tiles = block_tiles(a, s, block);
+      t0 = tile_from(first);
+      t1 = tile_from(end);
+      if (t0 < t1) return true;
+      advance(a);
+    }
+  }
+  __device__ __forceinline__ void advance(const Args &a) {
+    u0 += block_units(a, s, block);
+    if (u0 >= end) return;
+    if (++block >= s.blocks) {
+      block = 0;
+      do s = load_seq(a, ++b, false);
+      while (s.nodes == 0);
+    }
+  }
+  __device__ __forceinline__ int share_of(int t, int per) const { return (u0 + kBegin + t) / per; }
+  __device__ __forceinline__ int rows(const Args &a) const {  // of the Q tile
+    return min(a.tile_nodes, s.nodes - block * a.tile_nodes) * a.head_box;
+  }
+};
+
+// Rows of q that no sequence has (all of them flagged): they see nothing.
+template <typename T>
+__device__ __noinline__ void clear_rows(const Args &a, bool all) {
+  for (int b = 0; b < a.batch; ++b) {
+    const Seq s = load_seq(a, b, false);
+    const int first = b == 0 ? 0 : s.q0, end = all ? (b == 0 ? a.total_q : 0) : s.end;
+    for (int t = first + blockIdx.x; t < end; t += gridDim.x) {
+      if (!all && t >= s.q0 && t < s.q0 + s.nodes) continue;
+      uint4 *out = reinterpret_cast<uint4 *>(static_cast<T *>(a.out) + static_cast<int64_t>(t) * a.heads * kRank);
+      for (int i = threadIdx.x; i < a.heads * (kRank / 8); i += blockDim.x) out[i] = make_uint4(0, 0, 0, 0);
+      if (!a.lse) continue;
+      for (int h = threadIdx.x; h < a.heads; h += blockDim.x) a.lse[static_cast<int64_t>(t) * a.heads + h] = -CUDART_INF_F;
+    }
+  }
+}
+
+// The line's length, a share's, and where this CTA's begins; all threads call it,
+// a barrier follows.  (With a q_indptr that descends nothing has a sequence: its
+// sequences could have the same rows, and the counts pass 31 bits.)
+template <typename T>
+__device__ __forceinline__ void make_plan(const Args &a, Ctrl &c) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int each = (a.batch + kThreads - 1) / kThreads;
+  const int b0 = tid * each, b1 = min(b0 + each, a.batch);
+  Seq s{};
+  int mine = 0;
+  bool unclaimed = false, descends = false;
+  for (int b = b0; b < b1; ++b) {
+    s = load_seq(a, b, blockIdx.x == 0);
+    mine += seq_units(a, s);
+    unclaimed = unclaimed || (b == 0 && s.q0 > 0) || s.q0 + s.nodes < s.end;
+    descends = descends || s.end < s.q0;
+  }
+  int incl = mine;
+#pragma unroll
+  for (int m = 1; m < 32; m <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, incl, m);
+    if (lane >= m) incl += y;
+  }
+  if (lane == 31) c.scan[warp] = incl;
+  bool none = false;
+  if (__syncthreads_or(unclaimed || descends)) {
+    none = __syncthreads_or(descends);
+    clear_rows<T>(a, none);
+  }
+  int total = 0, before = 0;
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) {
+    if (w < warp) before += c.scan[w];
+    total += c.scan[w];
+  }
+  if (none) total = mine = 0;
+  const int shares = static_cast<int>(gridDim.x) / a.parts;
+  const int per = max(2, static_cast<int>((static_cast<unsigned>(total) + shares - 1) / shares));
+  const int first = static_cast<int>(blockIdx.x) / a.parts * per;
+  int at = before + incl - mine;
+  if (first >= at && first < at + mine) {
+    int b = b0;
+    for (;; ++b) {
+      if (each > 1) s = load_seq(a, b, false);
+      const int n = seq_units(a, s);
+      if (first < at + n) break;
+      at += n;
+    }
+    int block = 0;
+    if (a.mask) {
+      const int n = block_units(a, s, 0);
+      block = (first - at) / n;
+      at += block * n;
+    } else {
+      for (int n; first >= at + (n = block_units(a, s, block)); ++block) at += n;
+    }
+    c.start = Start{s, b, block, at};
+  }
+  if (tid == 0) {
+    c.per = per;
+    c.total = total;
+  }
+}
+
+// ------------------------------------------------------------------- roles --
+// Page ids of a sequence, 32 at a time in a warp's lanes.  Invalid ids are flagged and become -1.
+__device__ __forceinline__ int load_ids(const Args &a, int b, int window, int pages) {
+  const int p = window * 32 + (threadIdx.x & 31);
+  if (p >= pages) return -1;
+  const int id = __ldg(a.block_table + static_cast<int64_t>(b) * a.bt_stride + p);
+  if (id < 0 || id >= a.num_blocks) {
+    if (a.error_flag) atomicOr(a.error_flag, B200KV_DEVERR_BAD_BLOCK);
+    return -1;
+  }
+  return id;
+}
+
+__device__ __forceinline__ void producer(const Args &a, Ctrl &c, uint8_t *smem, const CUtensorMap *qm,
+                                         const CUtensorMap *rm, const CUtensorMap *pm, const CUtensorMap *sm) {
+  const int lane = threadIdx.x & 31;
+  const int head0 = static_cast<int>(blockIdx.x) % a.parts * a.head_box;
+  const uint32_t q_bytes = static_cast<uint32_t>(a.box_nodes * a.head_box * 128);
+  const uint64_t policy_once = l2_policy_evict_first();
+  uint64_t policy_again;
+  asm volatile("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(policy_again));
+  bool dead = false;
+  uint32_t pairs = 0, tiles = 0, pieces = 0;  // issued
+  Walk w;
+  w.init(a, c);
+  while (w.next(a)) {
+    // pages that one block of one CTA reads leave L2 first
+    const uint64_t policy = a.parts > 1 || w.s.blocks > 1 ? policy_again : policy_once;
+    const int pages = (w.s.ctx + w.s.nodes + kPageTokens - 1) / kPageTokens;
+    int window = w.t0 / 32, ids = load_ids(a, w.b, window, pages), ids_next = load_ids(a, w.b, window + 1, pages);
+    wait(&c.q_empty, (pieces & 1u) ^ 1u, dead, a.error_flag);
+    if ((dead = __any_sync(0xffffffffu, dead))) break;
+    if (lane == 0) mbar_arrive_expect_tx(&c.q_full, kSticks * q_bytes);
+    __syncwarp();
+    if (lane < kSticks)
+      tma_3d(smem + kOffQ + lane * kStickTile, lane < kSticks - 1 ? qm : rm, &c.q_full, lane < kSticks - 1 ? lane * 64 : 0,
+             head0, w.s.q0 + w.block * a.tile_nodes);
+    ++pieces;
+    for (int t = w.t0; t < w.t1; ++t, ++tiles) {
+      if (t / 32 > window) {
+        ids = ids_next;
+        ids_next = load_ids(a, w.b, ++window + 1, pages);
+      }
+      const int id = __shfl_sync(0xffffffffu, ids, t & 31);
+      const int page = id < 0 ? a.num_blocks : id;  // an invalid id reads past the last page: zeros
+      wait(&c.rope_empty, (tiles & 1u) ^ 1u, dead, a.error_flag);
+      if ((dead = __any_sync(0xffffffffu, dead))) break;
+      if (lane == 0) {
+        mbar_arrive_expect_tx(&c.rope_full, kStickTile);
+        tma_load_3d(smem + kOffRope, sm, &c.rope_full, 0, (kSticks - 1) * kTile, page, policy);
+      }
+      for (int j = 0; j < kPairs; ++j, ++pairs) {
+        const uint32_t slot = pairs % kSlots;
+        wait(&c.empty[slot], ((pairs / kSlots) & 1u) ^ 1u, dead, a.error_flag);
+        if ((dead = __any_sync(0xffffffffu, dead))) break;
+        if (lane == 0) {
+          mbar_arrive_expect_tx(&c.full[slot], kPair);
+          tma_load_3d(smem + kOffSlots + slot * kPair, pm, &c.full[slot], 0, j * 2 * kTile, page, policy);
+        }
+      }
+      if (dead) {
+        ++tiles;
+        break;
+      }
+    }
+    if (dead) break;
+    w.advance(a);
+  }
+  if (dead) {  // the copies under way, with a limit
+    bool late = false;
+    if (pieces > 0) wait(&c.q_full, (pieces - 1) & 1u, late, a.error_flag);
+    if (tiles > 0) wait(&c.rope_full, (tiles - 1) & 1u, late, a.error_flag);
+    for (uint32_t n = pairs - min(pairs, uint32_t(kSlots)); n < pairs; ++n)
+      wait(&c.full[n % kSlots], (n / kSlots) & 1u, late, a.error_flag);
+  }
+  // the last arrival that the MMAs owe this CTA: not before it may the CTA end
+  if (lane == 0 && pieces > 0) {
+    bool late = false;
+    wait(&c.q_empty, (pieces & 1u) ^ 1u, late, a.error_flag);
+  }
+  __syncwarp();
+}
+
+// One warp, converged, issues every MMA from an elected lane.  Scores run up to
+// one page ahead of the values; of the two, what is ready goes first.
+template <typename T>
+__device__ __forceinline__ void mma_issuer(const Args &a, Ctrl &c, uint8_t *smem, uint32_t tmem_any) {
+  constexpr uint32_t kBase = (1u << 4) | (std::is_same<T, __half>::value ? 0u : (1u << 7) | (1u << 10));
+  constexpr uint32_t kIdescQK = kBase | (uint32_t(kTile >> 3) << 17) | (uint32_t(kTileRows >> 4) << 24);
+  constexpr uint32_t kIdescPV = kBase | (1u << 15) | (uint32_t(128 >> 4) << 24);  // A (V^T): M-major
+  const uint32_t go = elect_one(), tmem = uniform(tmem_any);
+  const uint32_t negate = a.scale < 0.f ? 1u << 13 : 0u;  // a negative scale turns Q's sign
+  const uint32_t qd = desc_kmajor(uniform(smem_u32(smem + kOffQ)));
+  const uint32_t pd = desc_kmajor(uniform(smem_u32(smem + kOffP)));
+  const uint32_t rd = desc_kmajor(uniform(smem_u32(smem + kOffRope)));
+  const uint32_t slots = uniform(smem_u32(smem + kOffSlots));
+  auto done = [&](uint64_t *bar) {
+    if (go) commit(bar);
+  };
+  Walk wq, wp;  // the pieces that scores and values are at
+  wq.init(a, c);
+  wp = wq;
+  bool more = wq.next(a), left = wp.next(a);
+  int tq = wq.t0, tp = wp.t0;
+  uint32_t nq = 0, np = 0;            // pages whose scores are complete, whose values are
+  uint32_t sub = 0;                   // the next part of page nq: the rotary stick, then the pairs
+  uint32_t piece_q = 0, piece_p = 0;
+  uint32_t idle = 0;
+  uint64_t since = 0;
+  while (left) {
+    bool moved = false;
+    if (np < nq) {
+      const bool first = tp == wp.t0;
+      bool ready = mbar_test(&c.p_ready[np & 1], (np >> 1) & 1u);
+      if (first) ready = ready && mbar_test(&c.o_empty, (piece_p & 1u) ^ 1u);
+      if (__all_sync(0xffffffffu, ready)) {
+        fence_after();
+        const uint32_t idesc = kIdescPV | (uint32_t((wp.rows(a) + 15) / 16 * 2) << 17);
+        const uint32_t p = pd + ((np & 1u) * kStickTile >> 4);
+#pragma unroll 1
+        for (int m = 0; m < kPairs; ++m) {
+          const uint32_t slot = (np * kPairs + m) % kSlots;
+          const uint32_t vd = ((slots + slot * kPair) >> 4) | (uint32_t(kStickTile >> 4) << 16);
+#pragma unroll
+          for (int k = 0; k < kTile / 16; ++k)
+            mma_ss(tmem + col_o(m), vd + (k * 2048 >> 4), p + (k * 32 >> 4), idesc, !first || k > 0, go);
+          done(&c.empty[slot]);
+        }
+        done(&c.p_free[np & 1]);
+        ++np;
+        if (++tp >= wp.t1) {
+          done(&c.o_full);
+          ++piece_p;
+          wp.advance(a);
+          left = wp.next(a);
+          tp = wp.t0;
+        }
+        moved = true;
+      }
+    }
+    if (!moved && more && nq <= np + 1) {
+      const uint32_t slot = (nq * kPairs + sub - 1) % kSlots;
+      bool ready;
+      if (sub == 0)
+        ready = mbar_test(&c.rope_full, nq & 1u) && (tq > wq.t0 || mbar_test(&c.q_full, piece_q & 1u));
+      else
+        ready = mbar_test(&c.full[slot], ((nq * kPairs + sub - 1) / kSlots) & 1u);
+      if (__all_sync(0xffffffffu, ready)) {
+        fence_after();
+        const uint32_t s = tmem + col_s(nq & 1);
+        if (sub == 0) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            mma_ss(s, qd + ((kSticks - 1) * kStickTile + k * 32 >> 4), rd + (k * 32 >> 4), kIdescQK | negate, k > 0, go);
+          done(&c.rope_empty);
+          ++sub;
+        } else {
+          const uint32_t q = qd + ((sub - 1) * kPair >> 4), kd = desc_kmajor(slots + slot * kPair);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const uint32_t off = ((k >> 2) * kStickTile + (k & 3) * 32) >> 4;
+            mma_ss(s, q + off, kd + off, kIdescQK | negate, 1, go);
+          }
+          if (++sub > kPairs) {
+            sub = 0;
+            done(&c.s_full[nq & 1]);
+            ++nq;
+            if (++tq >= wq.t1) {
+              done(&c.q_empty);
+              ++piece_q;
+              wq.advance(a);
+              more = wq.next(a);
+              tq = wq.t0;
+            }
+          }
+        }
+        moved = true;
+      }
+    }
+    if (moved) {
+      idle = 0;
+    } else if ((++idle & 1023u) == 0) {
+      const uint64_t now = global_timer_ns();
+      if (idle == 1024u) since = now;
+      if (__any_sync(0xffffffffu, now - since > kWaitLimitNs)) {
+        if (go && a.error_flag) atomicOr(a.error_flag, B200KV_DEVERR_TIMEOUT);
+        break;
+      }
+    }
+  }
+  __syncwarp();
+}
+
+// Which of the tokens pos .. pos + 31 node `node` sees.
+__device__ __forceinline__ uint32_t visible32(const Args &a, const Seq &s, int node, int pos) {
+  if (!a.mask) return low_bits(s.ctx + node + 1 - pos);
+  uint32_t bits = low_bits(s.ctx - pos);
+  const int off = pos - s.ctx;
+  if (off > -32) {
+    const uint64_t *row = a.mask + static_cast<int64_t>(s.q0 + node) * a.words;
+    const int w = max(off, 0) >> 6;
+    uint64_t m = w < a.words ? __ldg(row + w) : 0;
+    if (off < 0) {
+      m <<= -off;
+    } else {
+      const int sh = off & 63;
+      m >>= sh;
+      if (sh > 32 && w + 1 < a.words) m |= __ldg(row + w + 1) << (64 - sh);
+    }
+    bits |= static_cast<uint32_t>(m) & low_bits(s.ctx + s.nodes - pos);
+  }
+  return bits;
+}
+
+template <bool kTail>
+__device__ __forceinline__ float mask_max(uint32_t (&s)[32], uint32_t vis) {
+  if (kTail) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) s[j] = vis >> j & 1u ? s[j] : 0xff800000u;  // -inf
+  }
+  float t = __uint_as_float(s[0]);
+#pragma unroll
+  for (int j = 1; j < 31; j += 2) t = fmaxf(fmaxf(t, __uint_as_float(s[j])), __uint_as_float(s[j + 1]));
+  return fmaxf(t, __uint_as_float(s[31]));
+}
+
+// O's columns times their factors; the four warps call it.
+static __device__ __noinline__ void rescale(const Ctrl &c, uint32_t quad, int rows) {
+  for (int m = 0; m < kPairs; ++m)
+    for (int j0 = 0; j0 < rows; j0 += 32) {
+      uint32_t r[32];
+      tmem_ld32(quad + col_o(m) + j0, r);
+      wait_ld(r);
+#pragma unroll
+      for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * c.factor[j0 + j]);
+      tmem_st32(quad + col_o(m) + j0, r);
+    }
+  wait_st();
+}
+
+// Adds the non-finite elements of the piece's visible nodes to a row that has been
+// written, to its partial sums or its output.
+template <typename T>
+__device__ __noinline__ void repair_row(const Args &a, const Seq &s, int b, int node, int from, int to, float *part, T *out) {
+  for (int p = max(from, s.ctx); p < min(to, s.ctx + s.nodes); ++p) {
+    if (!(visible32(a, s, node, p) & 1u)) continue;
+    const int id = __ldg(a.block_table + static_cast<int64_t>(b) * a.bt_stride + p / kPageTokens);
+    if (id < 0 || id >= a.num_blocks) continue;
+    const T *page = static_cast<const T *>(a.pool) + static_cast<int64_t>(id) * kRow * kPageTokens;
+    for (int d = 0; d < kRank; ++d) {
+      const float v = to_float(page[(d / 64 * kPageTokens + p % kPageTokens) * 64 + d % 64]);
+      if (fabsf(v) < CUDART_INF_F) continue;
+      if (part)
+        part[d] += v;
+      else
+        from_float(out[d], to_float(out[d]) + v);
+    }
+  }
+}
+
+// Softmax of the CTA's rows, and their output.
+template <typename T>
+__device__ __forceinline__ void softmax(const Args &a, Ctrl &c, uint8_t *smem, uint32_t tmem) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int row = 16 * warp + (lane & 15);
+  const bool has_row = lane < 16;
+  const uint32_t quad = tmem + (uint32_t(warp * 32) << 16);
+  const int part = static_cast<int>(blockIdx.x) % a.parts;
+  // (a scale of zero: too small to move a score, and -inf stays -inf)
+  const float cl = fmaxf(fabsf(a.scale) * 1.44269504088896341f, 1e-37f);
+  bool dead = false;
+  uint32_t n = 0;  // pages
+  unsigned piece = 0;
+  Walk wk;
+  wk.init(a, c);
+  while (wk.next(a)) {
+    ++piece;
+    const int len = wk.s.ctx + wk.s.nodes, rows = wk.rows(a);
+    const int node = wk.block * a.tile_nodes + row / a.head_box;
+    const int head = part * a.head_box + row % a.head_box;
+    const bool live = has_row && row < rows && head < a.heads;
+    const bool warp_live = __any_sync(0xffffffffu, live);
+    // tokens before this one are seen by every row of the tile
+    const int common = wk.s.ctx + (a.mask ? 0 : wk.block * a.tile_nodes + 1);
+    float m = -CUDART_INF_F, l = 0.f;
+    for (int t = wk.t0; t < wk.t1; ++t, ++n) {
+      const int pos = t * kTile;
+      const bool first = t == wk.t0, tail = pos + kTile > common;
+      uint32_t vis[2] = {~0u, ~0u};
+      if (tail && live) {
+        vis[0] = visible32(a, wk.s, node, pos);
+        vis[1] = visible32(a, wk.s, node, pos + 32);
+      }
+      wait(&c.s_full[n & 1], (n >> 1) & 1u, dead, a.error_flag);
+      fence_after();
+      uint32_t s[2][32];
+      float mt = -CUDART_INF_F;
+      if (warp_live) {
+        tmem_ld32(quad + col_s(n & 1), s[0]);
+        tmem_ld32(quad + col_s(n & 1) + 32, s[1]);
+        wait_ld(s[0]);
+        wait_ld(s[1]);
+        if (tail)
+          mt = fmaxf(mask_max<true>(s[0], vis[0]), mask_max<true>(s[1], vis[1])) * cl;
+        else
+          mt = fmaxf(mask_max<false>(s[0], ~0u), mask_max<false>(s[1], ~0u)) * cl;
+      }
+      const bool rise = live && mt > m + (first ? 0.f : kLazyLog2);
+      if (!first && any_softmax(rise)) {
+        // O moves to the new maxima once the values before are in it
+        const float keep = rise ? ex2(m - mt) : 1.f;
+        l *= keep;
+        if (has_row) c.factor[row] = keep;
+        wait(&c.p_free[(n - 1) & 1], ((n - 1) >> 1) & 1u, dead, a.error_flag);
+        fence_after();
+        bar_softmax();
+        rescale(c, quad, rows);
+        bar_softmax();
+      }
+      if (rise) m = mt;
+      // P's buffer is free once the values of two pages before are in O
+      if (n >= 2) wait(&c.p_free[n & 1], ((n - 2) >> 1) & 1u, dead, a.error_flag);
+      if (warp_live) {
+        const float minus = m == -CUDART_INF_F ? 0.f : -m;
+        float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        uint8_t *at = smem + kOffP + (n & 1) * kStickTile + row * 128;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          uint32_t p[16];
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            const float2 x = make_float2(__uint_as_float(s[i][2 * j]), __uint_as_float(s[i][2 * j + 1]));
+            const float2 y = fma2(x, make_float2(cl, cl), make_float2(minus, minus));
+            const float2 e = make_float2(ex2(y.x), ex2(y.y));
+            sum[j & 1] = add2(sum[j & 1], e);
+            p[j] = pack2(e.x, e.y, T());
+          }
+          if (has_row) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              *reinterpret_cast<uint4 *>(at + (((4 * i + k) ^ (row & 7)) << 4)) =
+                  make_uint4(p[4 * k], p[4 * k + 1], p[4 * k + 2], p[4 * k + 3]);
+          }
+        }
+        const float2 x = add2(sum[0], sum[1]);
+        l += x.x + x.y;
+      }
+      if (pos + kTile > min(common, len)) {
+        // the pool's rows past the sequence's end hold anything and become zeros, so that
+        // weights of zero meet finite values; so do non-finite elements of nodes that not
+        // every row sees (repair_row)
+        const int from = max(common - pos, 0), end = len - pos;
+        for (int j = 0; j < kPairs; ++j) {
+          uint8_t *v = smem + kOffSlots + (n * kPairs + j) % kSlots * kPair + tid * 16;
+#pragma unroll 1
+          for (int k = min(from, end) / 16; k < 4; ++k)
+            for (int st = 0; st < 2; ++st) {
+              uint4 *cell = reinterpret_cast<uint4 *>(v + st * kStickTile + k * 2048);
+              const int vrow = 16 * k + (tid >> 3);
+              if (vrow >= end) {
+                *cell = make_uint4(0, 0, 0, 0);
+              } else if (vrow >= from) {
+                uint4 x = *cell;
+                if (!any_non_finite<T>(x)) continue;
+                atomicMax(&c.bad_piece, piece);
+                drop_non_finite<T>(x);
+                *cell = x;
+              }
+            }
+        }
+      }
+      fence_async_smem();
+      fence_before();
+      __syncwarp();
+      if (lane == 0) arrive(&c.p_ready[n & 1]);
+    }
+
+    // -------------------------------------------------------- end of piece --
+    const bool split = wk.t0 > 0 || wk.t1 < wk.tiles;
+    const int64_t pslot = 2 * blockIdx.x + (wk.t0 > 0 ? 0 : 1);  // one of each kind per share
+    const int64_t orow = static_cast<int64_t>(wk.s.q0 + node) * a.heads + head;
+    if (has_row) {
+      c.factor[row] = split ? 1.f : (l == 0.f ? 0.f : 1.f / l);
+      c.row_at[row] = live ? static_cast<int>(orow) : -1;
+      if (live && split)
+        a.part_ml[pslot * kTileRows + row] = make_float2(m, l);
+      else if (live && a.lse)
+        a.lse[orow] = l == 0.f ? -CUDART_INF_F : (m + log2f(l)) * 0.69314718055994530942f;
+    }
+    bar_softmax();
+    wait(&c.o_full, (piece - 1) & 1u, dead, a.error_flag);
+    fence_after();
+    for (int mblock = 0; mblock < kPairs; ++mblock)
+#pragma unroll 1
+      for (int j0 = 0; j0 < rows; j0 += 32) {
+        const int d = 128 * mblock + 32 * warp + lane;  // this lane's latent element
+        uint32_t r[32];
+        tmem_ld32(quad + col_o(mblock) + j0, r);
+        wait_ld(r);
+        if (split) {
+          float *to = a.part_o + (pslot * kTileRows + j0) * kRank + d;
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if (c.row_at[j0 + j] >= 0) to[j * kRank] = __uint_as_float(r[j]);
+        } else {
+          // lanes in pairs: two neighbouring elements of every other row each
+          T *out = static_cast<T *>(a.out) + (d & ~1);
+#pragma unroll
+          for (int j = 0; j < 32; j += 2) {
+            float x[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const float f = c.factor[j0 + j + i];
+              x[i] = f == 0.f ? 0.f : __uint_as_float(r[j + i]) * f;
+            }
+            const float other = __shfl_xor_sync(0xffffffffu, lane & 1 ? x[0] : x[1], 1);
+            const int to = c.row_at[j0 + j + (lane & 1)];
+            const uint32_t two = lane & 1 ? pack2(other, x[1], T()) : pack2(x[0], other, T());
+            if (to >= 0) *reinterpret_cast<uint32_t *>(out + static_cast<int64_t>(to) * kRank) = two;
+          }
+        }
+      }
+    fence_before();
+    bar_softmax();  // (the factors and rows are read)
+    if (lane == 0) arrive(&c.o_empty);
+    if (live && *reinterpret_cast<volatile unsigned *>(&c.bad_piece) >= piece)
+      repair_row<T>(a, wk.s, wk.b, node, wk.t0 * kTile, wk.t1 * kTile,
+                    split ? a.part_o + (pslot * kTileRows + row) * kRank : nullptr, static_cast<T *>(a.out) + orow * kRank);
+    // the second share of a split block describes it to the join
+    if (wk.t0 > 0 && tid == 0) {
+      const int first = wk.share_of(0, c.per), share = static_cast<int>(blockIdx.x) / a.parts;
+      if (share == first + 1) {
+        Join j;
+        j.rows0 = wk.s.q0;
+        j.node0 = wk.block * a.tile_nodes;
+        j.nodes = min(wk.s.nodes - j.node0, a.tile_nodes);
+        j.first = first;
+        j.last = wk.share_of(wk.tiles - 1, c.per);
+        a.joins[blockIdx.x] = j;
+      }
+    }
+    wk.advance(a);
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 1)
+    latent_kernel(const __grid_constant__ CUtensorMap qm, const __grid_constant__ CUtensorMap rm,
+                  const __grid_constant__ CUtensorMap pm, const __grid_constant__ CUtensorMap sm,
+                  const __grid_constant__ Args a) {
+  extern __shared__ __align__(1024) uint8_t smem[];
+  Ctrl &c = *reinterpret_cast<Ctrl *>(smem);
+  const int tid = threadIdx.x, warp = tid >> 5;
+  if (tid == 0) {
+    prefetch_tensormap(&qm);
+    prefetch_tensormap(&rm);
+    prefetch_tensormap(&pm);
+    prefetch_tensormap(&sm);
+    for (int i = 0; i < kSlots; ++i) {
+      mbar_init(&c.full[i], 1);
+      mbar_init(&c.empty[i], 1);
+    }
+    mbar_init(&c.rope_full, 1);
+    mbar_init(&c.rope_empty, 1);
+    mbar_init(&c.q_full, 1);
+    mbar_init(&c.q_empty, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&c.s_full[i], 1);
+      mbar_init(&c.p_ready[i], 4);
+      mbar_init(&c.p_free[i], 1);
+    }
+    mbar_init(&c.o_full, 1);
+    mbar_init(&c.o_empty, 4);
+    fence_mbar_init();
+    c.bad_piece = 0;
+  }
+  if (warp == 5) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&c.tmem)),
+                 "r"(kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (tid == 0) a.joins[blockIdx.x].nodes = 0;  // no block begins to be split here, unless the epilogue says so
+  make_plan<T>(a, c);
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = c.tmem;
+  if (warp < 4)
+    softmax<T>(a, c, smem, tmem);
+  else if (warp == 4)
+    producer(a, c, smem, &qm, &rm, &pm, &sm);
+  else
+    mma_issuer<T>(a, c, smem, tmem);
+  fence_before();
+  __syncthreads();
+  if (warp == 5) {
+    fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+  }
+}
+
+// ------------------------------------------------------------------- join --
+// Blocks cut by shares: out = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i over the
+// pieces in order (the same bits every time).  A warp per row, 8 rows a CTA.
+template <typename T>
+__global__ void __launch_bounds__(256) latent_join_kernel(const __grid_constant__ Args a) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const Join j = a.joins[blockIdx.x];
+  const int row = blockIdx.y * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const int part = static_cast<int>(blockIdx.x) % a.parts;
+  const int node = row / a.head_box, head = part * a.head_box + row % a.head_box;
+  if (node >= j.nodes || head >= a.heads) return;
+  float M = -CUDART_INF_F, l = 0.f;
+  float4 o[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int x = j.first; x <= j.last; ++x) {
+    const int64_t slot = 2 * (x * a.parts + part) + (x == j.first ? 1 : 0);
+    const float2 ml = a.part_ml[slot * kTileRows + row];
+    const float4 *v = reinterpret_cast<const float4 *>(a.part_o + (slot * kTileRows + row) * kRank) + lane;
+    float4 p[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) p[i] = v[32 * i];
+    const float top = fmaxf(M, ml.x), mm = top == -CUDART_INF_F ? 0.f : top;
+    const float old = exp2f(M - mm), keep = exp2f(ml.x - mm);
+    M = top;
+    l = fmaf(ml.y, keep, l * old);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      o[i].x = fmaf(p[i].x, keep, o[i].x * old), o[i].y = fmaf(p[i].y, keep, o[i].y * old);
+      o[i].z = fmaf(p[i].z, keep, o[i].z * old), o[i].w = fmaf(p[i].w, keep, o[i].w * old);
+    }
+  }
+  const int64_t orow = (j.rows0 + j.node0 + node) * a.heads + head;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  T *out = static_cast<T *>(a.out) + orow * kRank + 4 * lane;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const bool none = l == 0.f;
+    const uint32_t lo = pack2(none ? 0.f : o[i].x * inv, none ? 0.f : o[i].y * inv, T());
+    const uint32_t hi = pack2(none ? 0.f : o[i].z * inv, none ? 0.f : o[i].w * inv, T());
+    *reinterpret_cast<uint2 *>(out + 128 * i) = make_uint2(lo, hi);
+  }
+  if (lane == 0 && a.lse) a.lse[orow] = l == 0.f ? -CUDART_INF_F : (M + log2f(l)) * 0.69314718055994530942f;
+}
+
+// ----------------------------------------------------------------- launch --
+template <typename T>
+int launch(const CUtensorMap &qm, const CUtensorMap &rm, const CUtensorMap &pm, const CUtensorMap &sm, const Args &a,
+           int ctas, cudaStream_t stream) {
+  static int configured[64] = {0};
+  int dev = 0;
+  B200KV_CUDA_TRY(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= 64) return set_error(B200KV_ERR_UNSUPPORTED, "device ordinal %d", dev);
+  if (!__atomic_load_n(&configured[dev], __ATOMIC_ACQUIRE)) {
+    B200KV_CUDA_TRY(cudaFuncSetAttribute(latent_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
+    __atomic_store_n(&configured[dev], 1, __ATOMIC_RELEASE);
+  }
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(ctas));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kSmem;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  B200KV_CUDA_TRY(cudaLaunchKernelEx(&cfg, latent_kernel<T>, qm, rm, pm, sm, a));
+  const int rows = a.box_nodes * a.head_box;
+  cfg.gridDim = dim3(static_cast<unsigned>(ctas), static_cast<unsigned>((rows + 7) / 8));
+  cfg.blockDim = dim3(256);
+  cfg.dynamicSmemBytes = 0;
+  B200KV_CUDA_TRY(cudaLaunchKernelEx(&cfg, latent_join_kernel<T>, a));
+  return B200KV_OK;
+}
+
+}  // namespace latent
+}  // namespace b200kv

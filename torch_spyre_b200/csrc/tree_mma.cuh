@@ -46,11 +46,13 @@
 
 #include <type_traits>
 
-#include "rows.cuh"
 #include "tree_attention.h"
+#include "umma.cuh"
 
 namespace b200kv {
 namespace tree {
+
+using namespace umma;
 
 constexpr int kTileRows = 128, kTileTokens = 128;
 constexpr float kLazyLog2 = 8.f;
@@ -124,31 +126,6 @@ struct Ctrl {
 constexpr int kOffFactors = 3072;
 static_assert(sizeof(Ctrl) <= kOffFactors, "control block");
 
-// ------------------------------------------------------------------- waits --
-// Bounded: after kWaitLimitNs the error flag is set and this thread waits no
-// more (its later waits return at once), so a lost transfer ends the kernel.  The
-// producer then starts no more copies, and waits for those under way, with a limit
-// again, before the CTA ends.
-__device__ __forceinline__ void wait(uint64_t *bar, uint32_t parity, bool &dead, int32_t *flag) {
-  if (mbar_try_wait(bar, parity) || dead) return;
-  const uint64_t t0 = global_timer_ns();
-  for (uint32_t i = 1;; ++i) {
-    if (mbar_try_wait(bar, parity)) return;
-    if ((i & 255u) == 0 && global_timer_ns() - t0 > kWaitLimitNs) break;
-  }
-  dead = true;
-  if (flag) atomicOr(flag, B200KV_DEVERR_TIMEOUT);
-}
-__device__ __forceinline__ void arrive(uint64_t *bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
-__device__ __forceinline__ void commit(uint64_t *bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
-               : "memory");
-}
-__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void bar_group(int w) {  // one warpgroup
   if (w == 0)
     asm volatile("bar.sync 2, 128;" ::: "memory");
@@ -157,82 +134,14 @@ __device__ __forceinline__ void bar_group(int w) {  // one warpgroup
 }
 __device__ __forceinline__ void bar_pair() { asm volatile("bar.sync 1, 256;" ::: "memory"); }  // both warpgroups
 
-// -------------------------------------------------------------- TMEM moves --
-#define B200KV_R8(r, i) "=r"(r[i]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3]), "=r"(r[i + 4]), "=r"(r[i + 5]), \
-                        "=r"(r[i + 6]), "=r"(r[i + 7])
-#define B200KV_W8(r, i) "r"(r[i]), "r"(r[i + 1]), "r"(r[i + 2]), "r"(r[i + 3]), "r"(r[i + 4]), "r"(r[i + 5]), \
-                        "r"(r[i + 6]), "r"(r[i + 7])
-__device__ __forceinline__ void tmem_ld32(uint32_t at, uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
-      "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-      : B200KV_R8(r, 0), B200KV_R8(r, 8), B200KV_R8(r, 16), B200KV_R8(r, 24)
-      : "r"(at));
-}
-__device__ __forceinline__ void tmem_ld16(uint32_t at, uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-      : B200KV_R8(r, 0), B200KV_R8(r, 8)
-      : "r"(at));
-}
-#define B200KV_RW8(r, i) "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]), \
-                         "+r"(r[i + 6]), "+r"(r[i + 7])
-// The loaded registers go through the wait, so that no use of them is moved before it.
-__device__ __forceinline__ void wait_ld(uint32_t (&r)[32]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : B200KV_RW8(r, 0), B200KV_RW8(r, 8), B200KV_RW8(r, 16), B200KV_RW8(r, 24));
-}
-__device__ __forceinline__ void wait_ld(uint32_t (&r)[16]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;" : B200KV_RW8(r, 0), B200KV_RW8(r, 8));
-}
-__device__ __forceinline__ void tmem_st32(uint32_t at, const uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
-      "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(at),
-      B200KV_W8(r, 0), B200KV_W8(r, 8), B200KV_W8(r, 16), B200KV_W8(r, 24));
-}
-__device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;"); }
-__device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(at),
-      B200KV_W8(r, 0), B200KV_W8(r, 8));
-}
-
 // ---------------------------------------------------------------- operands --
 // 128-byte swizzle, descriptor version 1.  K-major (Q, K): rows of 128 bytes,
 // groups of 8 rows 1024 bytes apart.  N-major (V): 64 head elements of a token
 // are 128 contiguous bytes; groups of 8 tokens 1024 bytes apart, the next 64
 // elements one stick column (128 tokens) on.
-constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);  // group stride, version 1, 128-byte swizzle
-__device__ __forceinline__ uint32_t desc_kmajor(uint32_t addr) { return (addr >> 4) | (1u << 16); }
 __device__ __forceinline__ uint32_t desc_nmajor(uint32_t addr) {
   return (addr >> 4) | (uint32_t((kTileTokens * 128) >> 4) << 16);
 }
-// One lane of the converged warp issues (`go`); every operand is the same in
-// all lanes, so that it lives in a uniform register and costs no move per MMA.
-__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc, uint32_t go) {
-  asm volatile(
-      "{\n\t.reg .pred p, e;\n\t.reg .b64 a, b;\n\tsetp.ne.b32 p, %5, 0;\n\tsetp.ne.b32 e, %6, 0;\n\t"
-      "mov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\t"
-      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n\t}" ::"r"(d),
-      "r"(a), "r"(b), "r"(kDescHi), "r"(idesc), "r"(acc), "r"(go)
-      : "memory");
-}
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc, uint32_t go) {
-  asm volatile(
-      "{\n\t.reg .pred p, e;\n\t.reg .b64 b;\n\tsetp.ne.b32 p, %5, 0;\n\tsetp.ne.b32 e, %6, 0;\n\t"
-      "mov.b64 b, {%2, %3};\n\t"
-      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}" ::"r"(d),
-      "r"(a), "r"(b), "r"(kDescHi), "r"(idesc), "r"(acc), "r"(go)
-      : "memory");
-}
-__device__ __forceinline__ uint32_t elect_one() {
-  uint32_t e;
-  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(e));
-  return e;
-}
-__device__ __forceinline__ uint32_t uniform(uint32_t x) { return __shfl_sync(0xffffffffu, x, 0); }
-
 // -------------------------------------------------------------------- plan --
 template <int kQ>
 __device__ __forceinline__ Seq load_seq(const Args &a, int b, bool report) {
@@ -460,14 +369,6 @@ __device__ __forceinline__ int load_ids(const Args &a, int b, int window, int pa
   return id;
 }
 
-__device__ __forceinline__ void tma_3d(void *dst, const CUtensorMap *map, uint64_t *bar, int c0, int c1, int c2) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], "
-      "[%2];" ::"r"(smem_u32(dst)),
-      "l"(map), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
-      : "memory");
-}
-
 // The pages of a raw tile that are not among `valid`; the whole warp calls it.
 static __device__ __noinline__ void zero_pages(uint8_t *tile, uint32_t valid) {
   uint4 *at = reinterpret_cast<uint4 *>(tile);
@@ -595,30 +496,6 @@ __device__ __forceinline__ void producer(const Args &a, Ctrl &c, uint8_t *smem, 
 // a tile only.  So the nodes' V rows are looked through in shared memory:
 // non-finite elements become zeros there, and when the block ends the rows that
 // see such a node get its elements added from the cache (repair_row).
-// (An exponent of all ones, and no other, carries into the sign bit when its
-// lowest bit is added.)
-template <typename T>
-__device__ __forceinline__ bool any_non_finite(uint4 v) {
-  constexpr uint32_t e = std::is_same<T, __half>::value ? 0x7c007c00u : 0x7f807f80u;
-  constexpr uint32_t one = std::is_same<T, __half>::value ? 0x04000400u : 0x00800080u;
-  return ((((v.x & e) + one) | ((v.y & e) + one) | ((v.z & e) + one) | ((v.w & e) + one)) & 0x80008000u) != 0;
-}
-template <typename T>
-__device__ __forceinline__ uint32_t drop_non_finite(uint32_t w) {
-  constexpr uint32_t e = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
-  if ((w & e) == e) w &= 0xffff0000u;
-  if ((w & (e << 16)) == (e << 16)) w &= 0xffffu;
-  return w;
-}
-template <typename T>
-__device__ __forceinline__ bool drop_non_finite(uint4 &v) {
-  const uint4 x = make_uint4(drop_non_finite<T>(v.x), drop_non_finite<T>(v.y), drop_non_finite<T>(v.z),
-                             drop_non_finite<T>(v.w));
-  const bool hit = x.x != v.x || x.y != v.y || x.z != v.z || x.w != v.w;
-  v = x;
-  return hit;
-}
-
 // Eight-bit pages -> operand tiles.  A lane takes 16 bytes of a row and writes
 // the two 16-byte vectors they become.  Lanes 0-3 of eight take the first half
 // of row r, lanes 4-7 the second half of row r ^ 1: the swizzle then puts the
@@ -817,13 +694,6 @@ __device__ __forceinline__ void mma_issuer(const Args &a, Ctrl &c, uint8_t *smem
   __syncwarp();
 }
 
-__device__ __forceinline__ uint32_t low_bits(int n) { return n >= 32 ? ~0u : (n <= 0 ? 0u : (1u << n) - 1u); }
-__device__ __forceinline__ float ex2(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
-
 // Which of the tokens pos .. pos + 31 row `node` sees.
 __device__ __forceinline__ uint32_t visible32(const Args &a, const Seq &s, int node, int pos) {
   if (!a.mask) return low_bits(s.ctx + node + 1 - pos);
@@ -843,24 +713,6 @@ __device__ __forceinline__ uint32_t visible32(const Args &a, const Seq &s, int n
     bits |= static_cast<uint32_t>(m) & low_bits(s.ctx + s.nodes - pos);
   }
   return bits;
-}
-
-// Two fp32 at a time.
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  float2 d;
-  asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
-      "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
-      : "=f"(d.x), "=f"(d.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-  return d;
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-  float2 d;
-  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 d, a, b;\n\t"
-      "mov.b64 {%0, %1}, d;\n\t}"
-      : "=f"(d.x), "=f"(d.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return d;
 }
 
 // Per-token factors of an 8-bit cache.  The scales leave the products: K and V

@@ -11,6 +11,8 @@ products of the latent vector with the head's weights W_k, W_v [512, 128]:
 * expanded (prompts): the rows are multiplied out, once for all queries
   (:func:`latent_prompt_attention`).
 
+* ``b200kv::latent_attention(q_latent, q_rope, pool, block_table, ...)`` -- the
+  absorbed form: drafted trees, chains or single tokens over the paged rows;
 * ``b200kv::latent_store(latent, k_rope, pool!, slots, ...)`` -- rows normalised,
   turned and written, the heads' rotary queries turned beside them;
 * :func:`latent_load` -- rows gathered by slot; ``b200kv::latent_commit`` -- the
@@ -19,17 +21,18 @@ products of the latent vector with the head's weights W_k, W_v [512, 128]:
 
 from __future__ import annotations
 
+import math
 from typing import Optional
 
 import torch
 
-from . import _eager
+from . import _eager, _lib
 from ._eager import direct, flag_ptr, launch, written
 from .kv_rows import DTYPES_16, _check_slots, kv_load
 from .layout import PAGE_TOKENS
-from .ops import _maybe_check_flag, _ptr, _require_cuda
+from .ops import _maybe_check_flag, _ptr, _require_cuda, workspace_for
 from .rotations import DTYPE_CODES, check_table
-from .tree import _check_sequences
+from .tree import _check_indptr, _check_sequences
 
 RANK, ROPE, NOPE = 512, 64, 128
 STICKS = (RANK + ROPE) // 64
@@ -194,3 +197,102 @@ def latent_commit(pool: torch.Tensor, block_table: torch.Tensor, context_lens: t
         new_lens = _latent_commit_impl(*args)
         written(pool)
     return new_lens
+
+
+# ---------------------------------------------------------------- attention --
+def _latent_attention_impl(
+    q_latent: torch.Tensor,
+    q_rope: torch.Tensor,
+    pool: torch.Tensor,
+    block_table: torch.Tensor,
+    context_lens: torch.Tensor,
+    q_indptr: torch.Tensor,
+    tree_mask: Optional[torch.Tensor],
+    scale: float,
+    max_nodes: int,
+    error_flag: Optional[torch.Tensor],
+) -> tuple[torch.Tensor, torch.Tensor]:
+    return _attend(q_latent, q_rope, pool, block_table, context_lens, q_indptr, tree_mask, scale, max_nodes, error_flag,
+                   True)
+
+
+def _attend(q_latent, q_rope, pool, block_table, context_lens, q_indptr, tree_mask, scale, max_nodes, error_flag,
+            want_lse):
+    _require_cuda(q_latent, q_rope, pool, block_table, context_lens, q_indptr)
+    NB, device, dtype = _check_pool(pool), pool.device, pool.dtype
+    for q, name, width in ((q_latent, "q_latent", RANK), (q_rope, "q_rope", ROPE)):
+        if q.dim() != 3 or q.shape[:2] != q_latent.shape[:2] or q.shape[2] != width or q.dtype != dtype \
+                or q.stride(2) != 1 or q.device != device:
+            raise ValueError(f"{name} must be [N, H, {width}] of the pool's dtype with contiguous rows on its device, got "
+                             f"{tuple(q.shape)} {q.dtype}")
+    B = _check_sequences(block_table, context_lens, device)
+    _check_indptr(q_indptr, B, device)
+    N, H, _ = q_latent.shape
+    words = 0
+    if tree_mask is not None:
+        if tree_mask.dtype != torch.int64 or tree_mask.dim() != 2 or len(tree_mask) != N \
+                or not tree_mask.is_contiguous() or tree_mask.device != device:
+            raise ValueError("tree_mask must be a contiguous int64 [N, words] tensor on q's device")
+        words = tree_mask.shape[1]
+    out = torch.empty((N, H, RANK), dtype=dtype, device=device)
+    lse = torch.empty((N, H), dtype=torch.float32, device=device) if want_lse else None
+    if N == 0:
+        return out, lse
+    wbytes = _lib.lib().b200kv_latent_workspace_bytes(N, B, H)
+    # An unsupported shape has no workspace size; the call below then reports why.
+    ws = workspace_for(device, wbytes) if wbytes > 0 else torch.empty(0, dtype=torch.uint8, device=device)
+    if wbytes > 0:
+        _eager.fast.set_workspace(ws)  # where the next call finds it
+    launch("b200kv_latent_attention", device, q_latent.data_ptr(), q_latent.stride(0), q_latent.stride(1),
+           q_rope.data_ptr(), q_rope.stride(0), q_rope.stride(1), DTYPE_CODES[dtype], pool.data_ptr(),
+           block_table.data_ptr(), block_table.stride(0), context_lens.data_ptr(), q_indptr.data_ptr(), _ptr(tree_mask),
+           words, out.data_ptr(), _ptr(lse), N, B, H, NB, block_table.shape[1], max_nodes, scale, ws.data_ptr(),
+           ws.numel(), flag_ptr(error_flag, device))
+    _maybe_check_flag(error_flag, "latent_attention")
+    return out, lse
+
+
+_latent_attention_op = torch.library.custom_op("b200kv::latent_attention", _latent_attention_impl, mutates_args=(),
+                                               device_types="cuda")
+
+
+@_latent_attention_op.register_fake
+def _(q_latent, q_rope, pool, block_table, context_lens, q_indptr, tree_mask, scale, max_nodes, error_flag):
+    return q_latent.new_empty(q_latent.shape), q_latent.new_empty(q_latent.shape[:2], dtype=torch.float32)
+
+
+def latent_attention(
+    q_latent: torch.Tensor,
+    q_rope: torch.Tensor,
+    pool: torch.Tensor,
+    block_table: torch.Tensor,
+    context_lens: torch.Tensor,
+    q_indptr: torch.Tensor,
+    tree_mask: Optional[torch.Tensor] = None,
+    scale: Optional[float] = None,
+    max_nodes: Optional[int] = None,
+    return_lse: bool = False,
+    error_flag: Optional[torch.Tensor] = None,
+):
+    """Attention of every sequence's new tokens over its cached rows, absorbed form:
+    each head scores a token by scale * (q_latent . latent + q_rope . k_rope) and gets the
+    weighted sum of the latent parts.
+
+    q_latent [N, H, 512] is the head's own query times its W_k^T, q_rope [N, H, 64] the
+    turned part (:func:`latent_store` returns it), both of the pool's dtype; the
+    result [N, H, 512] is what W_v multiplies.  The nodes of all sequences come one
+    after the other; q_indptr, context_lens, tree_mask, max_nodes, the masks' meaning
+    and the returned log-sum-exps are those of :func:`torch_spyre_b200.tree_attention`.
+    scale defaults to that of the expanded head, 1 / sqrt(128 + 64)."""
+    if scale is None:
+        scale = 1.0 / math.sqrt(NOPE + ROPE)
+    if max_nodes is None:
+        max_nodes = q_latent.shape[0] if tree_mask is None else min(q_latent.shape[0], 64 * tree_mask.shape[1])
+    args = (q_latent, q_rope, pool, block_table, context_lens, q_indptr, tree_mask, float(scale), max(1, int(max_nodes)),
+            error_flag)
+    pair = None if _eager.compiling() else _eager.fast.latent_attention(*args, bool(return_lse))
+    if pair is None:
+        plain = direct(q_latent, q_rope, pool, block_table, context_lens, q_indptr, tree_mask)
+        pair = _attend(*args, return_lse) if plain else torch.ops.b200kv.latent_attention(*args)
+    out, lse = pair
+    return (out, lse) if return_lse else out
