@@ -846,6 +846,33 @@ B200KV_API int b200kv_latent_attention(const void *q_latent, int64_t q_latent_st
                                        void *workspace, int64_t workspace_bytes,
                                        int32_t *error_flag, void *stream);
 
+/* Workspace bytes of b200kv_latent_prompt_attention (-1: unsupported shape), under
+ * the rules of b200kv_tree_workspace_bytes (they may share one). */
+B200KV_API int64_t b200kv_prompt_workspace_bytes(int64_t total_q, int64_t total_kv, int64_t batch,
+                                                 int64_t num_heads);
+
+/* Latent attention, expanded form, for prompts.  Sequence b has rows q_indptr[b] ..
+ * q_indptr[b + 1] - 1 of q (q_indptr[0] = 0, q_indptr[batch] = total_q) and tokens
+ * kv_indptr[b] .. kv_indptr[b + 1] - 1, of which the last ones are its rows' own: with
+ * causal != 0 row i of n sees tokens 0 .. m - n + i of m, else all m.
+ *   q       fp16 or bf16, row (t, h) of 192 elements at q[t * q_stride_t + h * q_stride_h]:
+ *           128 for the head's own key part, 64 for the shared rotary one
+ *   k_nope  row (p, h) of 128 elements, v likewise; k_rope row p of 64, for all heads
+ *   out     contiguous [total_q, H, 128]; lse fp32 [total_q, H] or NULL
+ * Buffers are 16-byte aligned, strides positive multiples of 8 elements.  A row that
+ * sees nothing is zero with lse = -inf.  Offsets outside [0, total] are clamped and set
+ * B200KV_DEVERR_BAD_LEN; rows that no sequence has (all of them, where offsets descend)
+ * are given as rows that see nothing.  Supported: H <= 65536, batch <= 1024, total_q * H
+ * < 2^31, total_kv < 2^30 and, with T = total_kv / 128 + 1, (17 * (total_q / 256 + batch) +
+ * 4 * (total_q / 256 * T + T + batch)) * H < 2^31. */
+B200KV_API int b200kv_latent_prompt_attention(
+    const void *q, int64_t q_stride_t, int64_t q_stride_h, const void *k_nope, int64_t k_stride_t,
+    int64_t k_stride_h, const void *k_rope, int64_t k_rope_stride_t, const void *v,
+    int64_t v_stride_t, int64_t v_stride_h, int32_t dtype, const int32_t *q_indptr,
+    const int32_t *kv_indptr, void *out, float *lse, int64_t total_q, int64_t total_kv,
+    int64_t batch, int64_t num_heads, float scale, int32_t causal, void *workspace,
+    int64_t workspace_bytes, int32_t *error_flag, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -9,7 +9,8 @@ from . import _lib, fp8, kv_rows, latent, layout, ops, pages, rotations, tree, w
 from ._lib import B200KVError
 from .fp8 import dequantize_fp8_with_scale, empty_pool_fp8, pool_shape_fp8, quantize_fp8_with_scale
 from .kv_rows import empty_row_pool, kv_load, kv_store
-from .latent import empty_latent_pool, latent_attention, latent_commit, latent_load, latent_store
+from .latent import (empty_latent_pool, latent_attention, latent_commit, latent_load, latent_prompt_attention,
+                     latent_store)
 from .layout import (SpyreTensorLayout, empty_pool, from_device_layout, page_layout, pool_shape, restickify,
                      restickify_layout, stick_layout, to_device_layout)
 from .ops import (decode_attention, decode_attention_append, kv_append, kv_relayout, kv_unrelayout,
@@ -39,6 +40,7 @@ __all__ = [
     "latent_attention",
     "latent_commit",
     "latent_load",
+    "latent_prompt_attention",
     "latent_store",
     "merge_attention_states",
     "page_layout",

@@ -41,7 +41,8 @@ compiling = torch.compiler.is_compiling
 _ENTRIES = ("b200kv_rotary", "b200kv_kv_store", "b200kv_kv_load", "b200kv_tree_mask", "b200kv_tree_workspace_bytes",
             "b200kv_tree_attention", "b200kv_tree_commit", "b200kv_extend_pages", "b200kv_release_pages",
             "b200kv_tree_verify", "b200kv_latent_store", "b200kv_latent_commit",
-            "b200kv_latent_workspace_bytes", "b200kv_latent_attention")
+            "b200kv_latent_workspace_bytes", "b200kv_latent_attention",
+            "b200kv_prompt_workspace_bytes", "b200kv_latent_prompt_attention")
 
 
 class _Absent:

@@ -334,6 +334,15 @@ SIGNATURES = {
             _p, _i64, _p, _p,  # workspace, workspace_bytes, error_flag, stream
         ],
     ),
+    "b200kv_prompt_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64]),
+    "b200kv_latent_prompt_attention": (
+        ctypes.c_int,
+        [
+            _p, _i64, _i64, _p, _i64, _i64, _p, _i64, _p, _i64, _i64, _i32,  # q, k_nope, k_rope, v with strides, dtype
+            _p, _p, _p, _p, _i64, _i64, _i64, _i64,  # indptrs, out, lse, total_q, total_kv, batch, heads
+            _f32, _i32, _p, _i64, _p, _p,  # scale, causal, workspace, bytes, error_flag, stream
+        ],
+    ),
 }
 
 

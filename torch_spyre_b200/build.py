@@ -53,6 +53,7 @@ SOURCES = [
     "pages.cu",
     "latent_rows.cu",
     "latent_attention.cu",
+    "prompt_attention.cu",
     "lse_combine.cu",
     "oproj_allreduce.cu",
 ]

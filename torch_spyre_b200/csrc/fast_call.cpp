@@ -58,6 +58,10 @@ struct Entries {
                           const int32_t *, int64_t, const int32_t *, const int32_t *, const int64_t *, int64_t, void *,
                           float *, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, float, void *, int64_t, int32_t *,
                           void *);
+  int64_t (*prompt_workspace_bytes)(int64_t, int64_t, int64_t, int64_t);
+  int (*latent_prompt_attention)(const void *, int64_t, int64_t, const void *, int64_t, int64_t, const void *, int64_t,
+                                 const void *, int64_t, int64_t, int32_t, const int32_t *, const int32_t *, void *, float *,
+                                 int64_t, int64_t, int64_t, int64_t, float, int32_t, void *, int64_t, int32_t *, void *);
 } entries;
 bool bound = false;
 
@@ -606,6 +610,44 @@ PyObject *latent_attention(PyObject *, PyObject *const *a, Py_ssize_t n) {
   return out_and_lse(std::move(out), std::move(lse));
 }
 
+// latent_prompt_attention(q, k_nope, k_rope, v, q_indptr, kv_indptr, scale, causal, error_flag, want_lse)
+// -> (out, lse or None)
+PyObject *latent_prompt_attention(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  B200KV_ARGS(10)
+  Call c;
+  const at::Tensor *q = c.tensor(a[0]), *k = c.tensor(a[1]), *kr = c.tensor(a[2]), *v = c.tensor(a[3]),
+                   *qp = c.tensor(a[4]), *kp = c.tensor(a[5]);
+  const double scale = PyFloat_AsDouble(a[6]);
+  if (scale == -1.0 && PyErr_Occurred()) {
+    PyErr_Clear();
+    Py_RETURN_NONE;
+  }
+  int32_t *flag = c.flag(a[8]);
+  if (!c.ok || !rows_ok(q) || !rows_ok(k) || !rows_ok(v) || kr->dim() != 2 || qp->dim() != 1 || qp->size(0) < 1) Py_RETURN_NONE;
+  constexpr int64_t kNope = 128;
+  const int64_t N = q->size(0), heads = q->size(1), M = k->size(0), batch = qp->size(0) - 1;
+  const at::ScalarType type = q->scalar_type();
+  c.need(is16(code_of(type)) && k->scalar_type() == type && v->scalar_type() == type && kr->scalar_type() == type &&
+         q->size(2) == kNope + kRope && k->size(1) == heads && k->size(2) == kNope && v->sizes() == k->sizes() &&
+         kr->size(0) == M && kr->size(1) == kRope && kr->stride(1) == 1 && vector_of(qp, at::kInt, batch + 1) &&
+         vector_of(kp, at::kInt, batch + 1));
+  if (!c.ok || N == 0) Py_RETURN_NONE;
+  const c10::cuda::CUDAGuard guard(c.device);
+  void *stream = stream_of(c);
+  const auto ws = workspaces().find(Key(c.device.index(), stream));
+  const int64_t bytes = entries.prompt_workspace_bytes(N, M, batch, heads);
+  if (ws == workspaces().end() || bytes <= 0 || ws->second.numel() < bytes) Py_RETURN_NONE;
+  at::Tensor out = at::empty({N, heads, kNope}, q->options()), lse;
+  if (a[9] == Py_True) lse = at::empty({N, heads}, q->options().dtype(at::kFloat));
+  const int st = entries.latent_prompt_attention(
+      data(q), q->stride(0), q->stride(1), data(k), k->stride(0), k->stride(1), data(kr), kr->stride(0), data(v),
+      v->stride(0), v->stride(1), code_of(type), ints(qp), ints(kp), out.data_ptr(),
+      lse.defined() ? static_cast<float *>(lse.data_ptr()) : nullptr, N, M, batch, heads, static_cast<float>(scale),
+      a[7] == Py_True, ws->second.data_ptr(), ws->second.numel(), flag, stream);
+  if (st != 0) Py_RETURN_NONE;
+  return out_and_lse(std::move(out), std::move(lse));
+}
+
 // bind(addresses): the C entries in the order of Entries
 PyObject *bind(PyObject *, PyObject *const *a, Py_ssize_t n) {
   B200KV_ARGS(static_cast<Py_ssize_t>(sizeof(Entries) / sizeof(void *)))
@@ -649,6 +691,7 @@ PyMethodDef methods[] = {B200KV_METHOD(rotary),         B200KV_METHOD(kv_store),
                          B200KV_METHOD(tree_mask),      B200KV_METHOD(tree_attention), B200KV_METHOD(tree_commit),
                          B200KV_METHOD(extend_pages),   B200KV_METHOD(release_pages), B200KV_METHOD(tree_verify),
                          B200KV_METHOD(latent_store),   B200KV_METHOD(latent_commit), B200KV_METHOD(latent_attention),
+                         B200KV_METHOD(latent_prompt_attention),
                          B200KV_METHOD(bind),           B200KV_METHOD(set_workspace), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_fast", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

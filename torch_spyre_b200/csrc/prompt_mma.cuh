@@ -1,0 +1,786 @@
+// Tensor-core kernel of prompt attention (prompt_attention.cu has the operator):
+// heads with keys of 128 own and 64 shared elements, values of 128.
+//
+// The rows of a sequence and head are cut into Q tiles of 128, two of which form a
+// block; a block's tokens are cut into tiles of 128.  The blocks' tiles, all
+// sequences and heads one after the other, form one line that is cut into equal
+// shares, one per CTA; a block cut by a share's end is joined by prompt_join_kernel.
+//
+// Inside a CTA two streams run side by side, each with its own warpgroup, score
+// buffer S and accumulator O in TMEM: the block's two Q tiles over every token
+// tile, or, with one Q tile, alternate token tiles, whose states are merged when
+// the block ends.  Per tile: S = Q K^T (12 products of 16 elements), the warpgroup
+// (thread = row) masks and exponentiates, P goes back into S's columns in 16 bits,
+// O += P V with P as the TMEM operand.  O is only rescaled when a row's maximum
+// has risen by more than 2^8.
+//
+// Shared memory holds two Q tiles and eight columns of 64 elements x 128 tokens: a
+// K tile is three (two of the head's, one of the shared part), a V tile two, each
+// freed by itself, so that the next tile's come in while this one's are in use.
+//
+// Warps: 0-3 and 4-7 the two softmax warpgroups, 8 the TMA producer, 9 the MMA issuer.
+#pragma once
+
+#include "prompt_attention.h"
+#include "umma.cuh"
+
+namespace b200kv {
+namespace prompt {
+
+using namespace umma;
+
+constexpr int kThreads = 384;
+constexpr int kRegsSoftmax = 208, kRegsIssue = 80;  // a thread, after setmaxnreg (384 threads of 168 at launch)
+constexpr int kTile = 128;                          // rows of a Q tile, tokens of a K or V tile
+constexpr int kCol = kTile * 128;                   // bytes of a column of 64 elements
+constexpr int kColsQ = 3, kColsV = 2, kSlots = 8;
+constexpr int kOffQ = 3072;
+constexpr int kOffSlots = kOffQ + 2 * kColsQ * kCol;
+constexpr int kSmem = kOffSlots + kSlots * kCol;
+constexpr float kLazyLog2 = 8.f;
+static_assert(kSmem <= 227 * 1024, "shared memory per CTA");
+
+// TMEM columns
+constexpr uint32_t kTmemCols = 512;
+__device__ __forceinline__ uint32_t col_s(int w) { return uint32_t(w) * 128u; }
+__device__ __forceinline__ uint32_t col_o(int w) { return 256u + uint32_t(w) * 128u; }
+
+struct Seq {
+  int q0, rows, kv0, len, blocks;
+  int past;  // tokens before the first row's own (may be negative)
+  int end;   // the first row of q that is a later sequence's
+};
+struct Start {
+  Seq s;
+  int b, head, block, u0;
+};
+
+struct Ctrl {
+  uint64_t full[kSlots], empty[kSlots];
+  uint64_t q_full, q_empty;
+  uint64_t s_full[2], p_ready[2], o_full[2];
+  uint32_t tmem;
+  int per, total;  // units of a share, of the line
+  Start start;
+  int scan[32];
+  unsigned bad_piece;  // last piece (counted from 1) that met a non-finite value in a V row
+  float2 ml[2][kTile];
+};
+static_assert(sizeof(Ctrl) <= kOffQ, "control block");
+
+__device__ __forceinline__ void bar_pair() { asm volatile("bar.sync 1, 256;" ::: "memory"); }  // both warpgroups
+
+// -------------------------------------------------------------------- plan --
+__device__ __forceinline__ Seq load_seq(const Args &a, int b, bool report) {
+  Seq s;
+  s.q0 = __ldg(a.q_indptr + b);
+  s.kv0 = __ldg(a.kv_indptr + b);
+  const int end = __ldg(a.q_indptr + b + 1), kv_end = __ldg(a.kv_indptr + b + 1);
+  const bool bad = s.q0 < 0 || end < s.q0 || end > a.total_q || s.kv0 < 0 || kv_end < s.kv0 || kv_end > a.total_kv ||
+                   (b == 0 && s.q0 != 0) || (b == a.batch - 1 && end != a.total_q);
+  s.q0 = min(max(s.q0, 0), a.total_q);
+  s.rows = min(max(end, s.q0), a.total_q) - s.q0;
+  s.end = b == a.batch - 1 ? a.total_q : min(max(end, 0), a.total_q);
+  s.kv0 = min(max(s.kv0, 0), a.total_kv);
+  s.len = min(max(kv_end, s.kv0), a.total_kv) - s.kv0;
+  s.past = s.len - s.rows;
+  if (bad && report && a.error_flag) atomicOr(a.error_flag, B200KV_DEVERR_BAD_LEN);
+  s.blocks = (s.rows + 2 * kTile - 1) / (2 * kTile);
+  return s;
+}
+// Token tiles of block k: what its last row sees (one at least, which may be masked whole).
+__device__ __forceinline__ int block_tiles(const Args &a, const Seq &s, int k) {
+  const int seen = a.causal ? s.past + min(s.rows, (k + 1) * 2 * kTile) : s.len;
+  return max((seen + kTile - 1) / kTile, 1);
+}
+// The line is cut by cost: a step over a token tile counts 2 with one Q tile and 4
+// with two, a block's beginning and end 9 and 13.
+__device__ __forceinline__ bool two_tiles(const Seq &s, int k) { return s.rows - k * 2 * kTile > kTile; }
+__device__ __forceinline__ int step_units(const Seq &s, int k) { return two_tiles(s, k) ? 4 : 2; }
+__device__ __forceinline__ int begin_units(const Seq &s, int k) { return two_tiles(s, k) ? 13 : 9; }
+__device__ __forceinline__ int block_units(const Args &a, const Seq &s, int k) {
+  return begin_units(s, k) + step_units(s, k) * block_tiles(a, s, k);
+}
+__device__ __forceinline__ int head_units(const Args &a, const Seq &s) {
+  if (s.blocks == 0) return 0;
+  // without a mask all blocks have as many tiles, and only the last may be of one Q tile
+  if (!a.causal) return (s.blocks - 1) * block_units(a, s, 0) + block_units(a, s, s.blocks - 1);
+  int n = 0;
+  for (int k = 0; k < s.blocks; ++k) n += block_units(a, s, k);
+  return n;
+}
+
+// The blocks of a CTA's share, one piece (a block, or the part of it in this
+// share) at a time.  Every role walks the same sequence.
+struct Walk {
+  Seq s;
+  int b, head, block, u0, tiles, t0, t1;  // piece: token tiles [t0, t1) of `tiles`
+  int end;                                // of the share
+
+  __device__ __forceinline__ void init(const Ctrl &c) {
+    const Start &f = c.start;
+    s = f.s, b = f.b, head = f.head, block = f.block, u0 = f.u0;
+    t1 = 0;
+    end = min(c.total, (static_cast<int>(blockIdx.x) + 1) * c.per);
+  }
+  // Tile t belongs to the share that holds its first unit.
+  __device__ __forceinline__ int tile_from(int unit) const {
+    const int w = step_units(s, block), x = unit - u0 - begin_units(s, block);
+    return x <= 0 ? 0 : min(tiles, (x + w - 1) / w);
+  }
+  __device__ __forceinline__ bool next(const Args &a, const Ctrl &c) {
+    const int first = static_cast<int>(blockIdx.x) * c.per;
+    for (;;) {
+      if (first >= c.total || u0 >= end) return false;
+      tiles = block_tiles(a, s, block);
+      t0 = tile_from(first);
+      t1 = tile_from(end);
+      if (t0 < t1) return true;
+      advance(a);
+    }
+  }
+  __device__ __forceinline__ void advance(const Args &a) {
+    u0 += block_units(a, s, block);
+    if (u0 >= end) return;
+    if (++block >= s.blocks) {
+      block = 0;
+      if (++head >= a.heads) {
+        head = 0;
+        do s = load_seq(a, ++b, false);
+        while (s.rows == 0);
+      }
+    }
+  }
+  __device__ __forceinline__ bool two() const { return two_tiles(s, block); }
+  __device__ __forceinline__ int share_of(int t, int per) const {
+    return (u0 + begin_units(s, block) + t * step_units(s, block)) / per;
+  }
+};
+
+// Rows of q that no sequence has (all of them flagged): they see nothing.
+template <typename T>
+__device__ __noinline__ void clear_rows(const Args &a, bool all) {
+  for (int b = 0; b < a.batch; ++b) {
+    const Seq s = load_seq(a, b, false);
+    const int first = b == 0 ? 0 : s.q0, end = all ? (b == 0 ? a.total_q : 0) : s.end;
+    for (int t = first + blockIdx.x; t < end; t += gridDim.x) {
+      if (!all && t >= s.q0 && t < s.q0 + s.rows) continue;
+      uint4 *out = reinterpret_cast<uint4 *>(static_cast<T *>(a.out) + static_cast<int64_t>(t) * a.heads * kDim);
+      for (int i = threadIdx.x; i < a.heads * (kDim / 8); i += blockDim.x) out[i] = make_uint4(0, 0, 0, 0);
+      if (!a.lse) continue;
+      for (int h = threadIdx.x; h < a.heads; h += blockDim.x) a.lse[static_cast<int64_t>(t) * a.heads + h] = -CUDART_INF_F;
+    }
+  }
+}
+
+// The line's length, a share's, and where this CTA's begins; all threads call it,
+// a barrier follows.  The counts fit 31 bits (the host checks) where no two
+// sequences have the same row or token: with offsets that descend nothing has a sequence.
+template <typename T>
+__device__ __forceinline__ void make_plan(const Args &a, Ctrl &c) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int each = (a.batch + kThreads - 1) / kThreads;
+  const int b0 = tid * each, b1 = min(b0 + each, a.batch);
+  Seq s{};
+  int mine = 0;
+  bool unclaimed = false, descends = false;
+  for (int b = b0; b < b1; ++b) {
+    descends = descends || __ldg(a.q_indptr + b + 1) < __ldg(a.q_indptr + b) || __ldg(a.kv_indptr + b + 1) < __ldg(a.kv_indptr + b);
+  }
+  const bool none = __syncthreads_or(descends);
+  for (int b = b0; b < b1; ++b) {
+    s = load_seq(a, b, blockIdx.x == 0);
+    if (!none) mine += head_units(a, s) * a.heads;
+    unclaimed = unclaimed || (b == 0 && s.q0 > 0) || s.q0 + s.rows < s.end;
+  }
+  int incl = mine;
+#pragma unroll
+  for (int m = 1; m < 32; m <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, incl, m);
+    if (lane >= m) incl += y;
+  }
+  if (lane == 31) c.scan[warp] = incl;
+  if (__syncthreads_or(unclaimed || none)) clear_rows<T>(a, none);
+  int total = 0, before = 0;
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) {
+    if (w < warp) before += c.scan[w];
+    total += c.scan[w];
+  }
+  // (at least a step, so that a share inside a block holds the start of a tile)
+  const int per = max(4, static_cast<int>((static_cast<unsigned>(total) + gridDim.x - 1) / gridDim.x));
+  const int first = static_cast<int>(blockIdx.x) * per;
+  int at = before + incl - mine;
+  if (first >= at && first < at + mine) {
+    int b = b0, hu = 0;
+    for (;; ++b) {
+      if (each > 1) s = load_seq(a, b, false);
+      hu = head_units(a, s);
+      if (first < at + hu * a.heads) break;
+      at += hu * a.heads;
+    }
+    const int head = (first - at) / hu;
+    at += head * hu;
+    int block = 0;
+    if (!a.causal) {
+      const int n = block_units(a, s, 0);
+      block = min((first - at) / n, s.blocks - 1);
+      at += block * n;
+    } else {
+      for (int n; first >= at + (n = block_units(a, s, block)); ++block) at += n;
+    }
+    c.start = Start{s, b, head, block, at};
+  }
+  if (tid == 0) {
+    c.per = per;
+    c.total = total;
+  }
+}
+
+// ------------------------------------------------------------------- roles --
+__device__ __forceinline__ void producer(const Args &a, Ctrl &c, uint8_t *smem, const CUtensorMap *qm,
+                                         const CUtensorMap *km, const CUtensorMap *rm, const CUtensorMap *vm) {
+  const int lane = threadIdx.x & 31;
+  bool dead = false;
+  uint32_t slot = 0, pieces = 0;  // columns issued, pieces begun
+  Walk w;
+  w.init(c);
+  while (w.next(a, c)) {
+    const bool two = w.two();
+    wait(&c.q_empty, (pieces & 1u) ^ 1u, dead, a.error_flag);
+    if ((dead = __any_sync(0xffffffffu, dead))) break;
+    const int n = (two ? 2 : 1) * kColsQ;
+    if (lane == 0) mbar_arrive_expect_tx(&c.q_full, uint32_t(n) * kCol);
+    __syncwarp();
+    if (lane < n)
+      tma_3d(smem + kOffQ + lane * kCol, qm, &c.q_full, lane % kColsQ * 64, w.head,
+             w.s.q0 + (2 * w.block + lane / kColsQ) * kTile);
+    ++pieces;
+    auto issue = [&](const CUtensorMap *map, int x, int head, int t) {
+      if (dead) return;
+      const uint32_t s = slot % kSlots;
+      wait(&c.empty[s], ((slot / kSlots) & 1u) ^ 1u, dead, a.error_flag);
+      if ((dead = __any_sync(0xffffffffu, dead))) return;
+      if (lane == 0) {
+        mbar_arrive_expect_tx(&c.full[s], kCol);
+        tma_3d(smem + kOffSlots + s * kCol, map, &c.full[s], x, head, w.s.kv0 + t * kTile);
+      }
+      ++slot;
+    };
+    auto issue_k = [&](int t) {
+      issue(km, 0, w.head, t);
+      issue(km, 64, w.head, t);
+      issue(rm, 0, 0, t);
+    };
+    // K leads V by one tile per stream that needs it: the order the MMA warp consumes them in
+    const int lead = two ? 1 : 2;
+    for (int t = w.t0; t < min(w.t0 + lead, w.t1); ++t) issue_k(t);
+    for (int t = w.t0; t < w.t1; ++t) {
+      issue(vm, 0, w.head, t);
+      issue(vm, 64, w.head, t);
+      if (t + lead < w.t1) issue_k(t + lead);
+    }
+    if (dead) break;
+    w.advance(a);
+  }
+  if (dead) {  // the copies under way, with a limit
+    bool late = false;
+    if (pieces > 0) wait(&c.q_full, (pieces - 1) & 1u, late, a.error_flag);
+    for (uint32_t n = slot - min(slot, uint32_t(kSlots)); n < slot; ++n)
+      wait(&c.full[n % kSlots], (n / kSlots) & 1u, late, a.error_flag);
+  }
+  // the last arrival that the MMAs owe this CTA: not before it may the CTA end
+  if (lane == 0 && pieces > 0) {
+    bool late = false;
+    wait(&c.q_empty, (pieces & 1u) ^ 1u, late, a.error_flag);
+  }
+  __syncwarp();
+}
+
+// One warp, converged, issues every MMA from an elected lane.
+template <typename T>
+__device__ __forceinline__ void mma_issuer(const Args &a, Ctrl &c, uint8_t *smem, uint32_t tmem_any) {
+  constexpr uint32_t kBase =
+      (1u << 4) | (std::is_same<T, __half>::value ? 0u : (1u << 7) | (1u << 10)) | (uint32_t(kTile >> 4) << 24);
+  constexpr uint32_t kIdescQK = kBase | (uint32_t(kTile >> 3) << 17);
+  constexpr uint32_t kIdescPV = kBase | (1u << 16) | (uint32_t(64 >> 3) << 17);  // V: N-major, a column at a time
+  bool dead = false;
+  uint32_t slot = 0, pieces = 0, p_uses[2] = {0, 0};
+  const uint32_t go = elect_one(), tmem = uniform(tmem_any);
+  const uint32_t qbase = smem_u32(smem + kOffQ), sbase = smem_u32(smem + kOffSlots);
+  const uint32_t negate = a.scale < 0.f ? 1u << 13 : 0u;  // a negative scale turns Q's sign
+  auto done = [&](uint64_t *bar) {
+    if (go) commit(bar);
+  };
+  auto ready = [&](uint32_t n) {
+    wait(&c.full[n % kSlots], (n / kSlots) & 1u, dead, a.error_flag);
+    fence_after();
+    return uniform(sbase + (n % kSlots) * kCol);
+  };
+  // Scores of Q tile `qtile` from the K tile at slot k; frees it when `last`.
+  auto qk = [&](int w, int qtile, uint32_t k, bool last) {
+    const uint32_t qd = desc_kmajor(qbase + qtile * kColsQ * kCol);
+#pragma unroll
+    for (int col = 0; col < kColsQ; ++col) {
+      const uint32_t kd = desc_kmajor(ready(k + col));
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        mma_ss(tmem + col_s(w), qd + ((col * kCol + i * 32) >> 4), kd + (i * 32 >> 4), kIdescQK | negate, col + i > 0, go);
+      if (last) done(&c.empty[(k + col) % kSlots]);
+    }
+    done(&c.s_full[w]);
+  };
+  auto pv = [&](int w, uint32_t v, bool first, bool last) {
+    wait(&c.p_ready[w], p_uses[w]++ & 1u, dead, a.error_flag);
+    fence_after();
+#pragma unroll
+    for (int col = 0; col < kColsV; ++col) {
+      const uint32_t vd = desc_kmajor(ready(v + col));
+#pragma unroll
+      for (int i = 0; i < kTile / 16; ++i)
+        mma_ts(tmem + col_o(w) + 64 * col, tmem + col_s(w) + i * 8, vd + (i * 2048 >> 4), kIdescPV, !first || i > 0, go);
+      if (last) done(&c.empty[(v + col) % kSlots]);
+    }
+  };
+  Walk w;
+  w.init(c);
+  while (w.next(a, c)) {
+    wait(&c.q_full, pieces++ & 1u, dead, a.error_flag);
+    fence_after();
+    const int n = w.t1 - w.t0;
+    if (w.two()) {
+      // both streams over every tile; a column is free when the second has used it
+      qk(0, 0, slot, false);
+      qk(1, 1, slot, true);
+      slot += kColsQ;
+      for (int t = 0; t < n; ++t) {
+        const uint32_t v = slot, k = slot + kColsV;
+        const bool more = t + 1 < n;
+        pv(0, v, t == 0, false);
+        if (more)
+          qk(0, 0, k, false);
+        else
+          done(&c.o_full[0]);
+        pv(1, v, t == 0, true);
+        if (more)
+          qk(1, 1, k, true);
+        else
+          done(&c.o_full[1]);
+        slot += kColsV + (more ? kColsQ : 0);
+      }
+    } else {
+      // stream t & 1 takes tile t
+      qk(0, 0, slot, true);
+      slot += kColsQ;
+      if (n > 1) {
+        qk(1, 0, slot, true);
+        slot += kColsQ;
+      }
+      for (int t = 0; t < n; ++t) {
+        const int w0 = t & 1;
+        pv(w0, slot, t < 2, true);
+        slot += kColsV;
+        if (t + 2 < n) {
+          qk(w0, 0, slot, true);
+          slot += kColsQ;
+        } else {
+          done(&c.o_full[w0]);
+        }
+      }
+    }
+    done(&c.q_empty);
+    w.advance(a);
+  }
+  __syncwarp();
+}
+
+// Moves the running maximum when a row's has risen far enough, O and l with it.
+__device__ __forceinline__ void follow(uint32_t to, float mt, bool first, bool live, float &m, float &l) {
+  const bool rise = mt > m + (first ? 0.f : kLazyLog2);
+  if (!first && __any_sync(0xffffffffu, rise && live)) {
+    const float keep = rise ? ex2(m - mt) : 1.f;
+    l *= keep;
+#pragma unroll 1
+    for (int i = 0; i < kDim; i += 16) {
+      uint32_t r[16];
+      tmem_ld16(to + i, r);
+      wait_ld(r);
+#pragma unroll
+      for (int j = 0; j < 16; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * keep);
+      tmem_st16(to + i, r);
+    }
+  }
+  if (rise) m = mt;
+}
+
+template <bool kTail>
+__device__ __forceinline__ float mask_max(uint32_t (&s)[32], uint32_t vis) {
+  if (kTail) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) s[j] = vis >> j & 1u ? s[j] : 0xff800000u;  // -inf
+  }
+  float t = __uint_as_float(s[0]);
+#pragma unroll
+  for (int j = 1; j < 31; j += 2) t = fmaxf(fmaxf(t, __uint_as_float(s[j])), __uint_as_float(s[j + 1]));
+  return fmaxf(t, __uint_as_float(s[31]));
+}
+
+// Scores of a row's 128 tokens -> weights, in place in TMEM.  kTail: the row sees
+// the first `seen` of them.
+template <typename T, bool kTail>
+__device__ __forceinline__ void weigh(uint32_t ts, uint32_t to, int seen, float cl, bool first, bool live, float &m, float &l) {
+  uint32_t s[4][32];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) tmem_ld32(ts + 32 * i, s[i]);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) wait_ld(s[i]);
+  float top[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) top[i] = mask_max<kTail>(s[i], kTail ? low_bits(seen - 32 * i) : ~0u);
+  follow(to, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * cl, first, live, m, l);
+  const float minus = m == -CUDART_INF_F ? 0.f : -m;
+  float2 sum[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    sum[i] = make_float2(0.f, 0.f);
+    uint32_t p[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const float2 x = make_float2(__uint_as_float(s[i][2 * j]), __uint_as_float(s[i][2 * j + 1]));
+      const float2 y = fma2(x, make_float2(cl, cl), make_float2(minus, minus));
+      const float2 e = make_float2(ex2(y.x), ex2(y.y));
+      sum[i] = add2(sum[i], e);
+      p[j] = pack2(e.x, e.y, T());
+    }
+    tmem_st16(ts + 16 * i, p);
+  }
+  const float2 t = add2(add2(sum[0], sum[1]), add2(sum[2], sum[3]));
+  l += t.x + t.y;
+  wait_st();
+}
+
+// Adds the non-finite V elements of tokens [from, to) to a row that has been
+// written, to its partial sums or its output.
+template <typename T>
+__device__ __noinline__ void repair_row(const Args &a, const Seq &s, int head, int from, int to, int d0, int d1, float *part,
+                                        T *out) {
+  for (int p = from; p < to; ++p) {
+    const T *row = static_cast<const T *>(a.v) + (s.kv0 + p) * a.v_st + head * a.v_sh;
+    for (int d = d0; d < d1; ++d) {
+      const float v = to_float(row[d]);
+      if (fabsf(v) < CUDART_INF_F) continue;
+      if (part)
+        part[d / 4 * 1024 + d % 4] += v;
+      else
+        from_float(out[d], to_float(out[d]) + v);
+    }
+  }
+}
+
+// One softmax warpgroup (w = 0 or 1); thread = row of its Q tile.
+template <typename T>
+__device__ __forceinline__ void softmax(const Args &a, Ctrl &c, uint8_t *smem, uint32_t tmem, int w) {
+  const int tid = threadIdx.x & 127, lane = tid & 31, warp = tid >> 5;
+  const uint32_t quad = tmem + (uint32_t(warp * 32) << 16);
+  const uint32_t ts = quad + col_s(w), to = quad + col_o(w);
+  // (a scale of zero: too small to move a score, and -inf stays -inf)
+  const float cl = fmaxf(fabsf(a.scale) * 1.44269504088896341f, 1e-37f);
+  bool dead = false;
+  uint32_t s_uses = 0, o_uses[2] = {0, 0}, slot = 0;
+  unsigned piece = 0;
+  Walk wk;
+  wk.init(c);
+  while (wk.next(a, c)) {
+    ++piece;
+    const bool two = wk.two();
+    const int n = wk.t1 - wk.t0, lead = two ? 1 : 2;
+    const int len = wk.s.len, row0 = (2 * wk.block + (two ? w : 0)) * kTile;
+    const int row = row0 + tid;
+    const bool live = row < wk.s.rows;
+    const bool warp_live = __any_sync(0xffffffffu, live);
+    // what this row sees, and what all rows of the Q tile see
+    const int seen = a.causal ? min(wk.s.past + row + 1, len) : len;
+    const int common = a.causal ? min(max(wk.s.past + row0 + 1, 0), len) : len;
+    float m = -CUDART_INF_F, l = 0.f;
+    const int step = two ? 1 : 2, tfirst = wk.t0 + (two ? 0 : w);
+    for (int t = tfirst; t < wk.t1; t += step) {
+      const int pos = t * kTile;
+      const bool tail = pos + kTile > common;
+      wait(&c.s_full[w], s_uses++ & 1u, dead, a.error_flag);
+      fence_after();
+      if (warp_live) {
+        if (tail)
+          weigh<T, true>(ts, to, seen - pos, cl, t == tfirst, live, m, l);
+        else
+          weigh<T, false>(ts, to, kTile, cl, t == tfirst, live, m, l);
+      }
+      if (tail) {
+        // V rows past the sequence's end are another's and become zeros, so that weights of
+        // zero meet finite values; so do non-finite elements that not every row sees
+        const int i = t - wk.t0;
+        const uint32_t v = slot + kColsQ * min(n, i + lead) + kColsV * i;
+        const int from = max(common - pos, 0), end = len - pos;
+        for (int col = 0; col < kColsV; ++col) {
+          const uint32_t vs = v + col;
+          wait(&c.full[vs % kSlots], (vs / kSlots) & 1u, dead, a.error_flag);
+          uint8_t *base = smem + kOffSlots + vs % kSlots * kCol + tid * 16;
+#pragma unroll 1
+          for (int k = min(from, max(end, 0)) / 16; k < 8; ++k) {  // 16 bytes per thread: row = 16 k + tid / 8
+            uint4 *at = reinterpret_cast<uint4 *>(base + k * 2048);
+            const int vrow = 16 * k + (tid >> 3);
+            if (vrow >= end) {
+              *at = make_uint4(0, 0, 0, 0);
+            } else if (vrow >= from) {
+              uint4 x = *at;
+              if (!any_non_finite<T>(x)) continue;
+              atomicMax(&c.bad_piece, piece);  // before the element goes: the other stream looks too
+              __threadfence_block();
+              drop_non_finite<T>(x);
+              *at = x;
+            }
+          }
+        }
+        fence_async_smem();
+      }
+      fence_before();
+      __syncwarp();
+      if (lane == 0) arrive(&c.p_ready[w]);
+    }
+    slot += (kColsQ + kColsV) * n;
+
+    // -------------------------------------------------------- end of piece --
+    const bool split = wk.t0 > 0 || wk.t1 < wk.tiles;
+    const int pslot = 2 * blockIdx.x + (wk.t0 > 0 ? 0 : 1);  // one of each kind per share
+    auto o_wait = [&](int k) {
+      wait(&c.o_full[k], o_uses[k]++ & 1u, dead, a.error_flag);
+      fence_after();
+    };
+    float keep0 = 1.f, keep1 = 0.f;
+    const bool both = !two && n > 1;
+    int d0 = 0, d1 = kDim;
+    if (two) {
+      o_wait(w);
+      ++o_uses[1 - w];
+    } else {
+      c.ml[w][tid] = make_float2(m, l);
+      o_wait(0);
+      if (both) o_wait(1);
+      bar_pair();
+      const float2 x = c.ml[0][tid], y = c.ml[1][tid];
+      m = fmaxf(x.x, y.x);
+      const float mm = m == -CUDART_INF_F ? 0.f : m;
+      keep0 = ex2(x.x - mm);
+      keep1 = ex2(y.x - mm);
+      l = x.y * keep0;
+      if (both) l = fmaf(y.y, keep1, l);
+      d0 = w * (kDim / 2);
+      d1 = d0 + kDim / 2;
+    }
+    const int64_t orow = static_cast<int64_t>(wk.s.q0 + row) * a.heads + wk.head;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const int prow = (two ? w : 0) * kTile + tid;
+    if (warp_live) {
+#pragma unroll 1
+      for (int d = d0; d < d1; d += 16) {
+        uint32_t r[16];
+        tmem_ld16(two ? to + d : quad + col_o(0) + d, r);
+        wait_ld(r);
+        if (!two) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * keep0);
+          if (both) {
+            uint32_t r1[16];
+            tmem_ld16(quad + col_o(1) + d, r1);
+            wait_ld(r1);
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              r[j] = __float_as_uint(fmaf(__uint_as_float(r1[j]), keep1, __uint_as_float(r[j])));
+          }
+        }
+        if (live && split) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            *reinterpret_cast<uint4 *>(a.part_o + ((static_cast<int64_t>(pslot) * (kDim / 4) + d / 4 + j) * 256 + prow) * 4) =
+                make_uint4(r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
+        } else if (live) {
+          T *out = static_cast<T *>(a.out) + orow * kDim + d;
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            float f[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) f[k] = l == 0.f ? 0.f : __uint_as_float(r[8 * j + k]) * inv;
+            *reinterpret_cast<uint4 *>(out + 8 * j) = pack8(f, T());
+          }
+        }
+        __syncwarp();
+      }
+    }
+    // (from what the first row of the block does not see: the other stream may have taken
+    // elements out that all rows of this one see; added twice they are what they are)
+    const int hidden = a.causal ? min(max(wk.s.past + 2 * wk.block * kTile + 1, 0), len) : len;
+    if (live && *reinterpret_cast<volatile unsigned *>(&c.bad_piece) >= piece)
+      repair_row<T>(a, wk.s, wk.head, max(wk.t0 * kTile, hidden), min(wk.t1 * kTile, seen), d0, d1,
+                    split ? a.part_o + (static_cast<int64_t>(pslot) * (kDim / 4) * 256 + prow) * 4 : nullptr,
+                    static_cast<T *>(a.out) + orow * kDim);
+    if (live && (two || w == 0)) {
+      if (split)
+        a.part_ml[static_cast<int64_t>(pslot) * 256 + prow] = make_float2(m, l);
+      else if (a.lse)
+        a.lse[orow] = l == 0.f ? -CUDART_INF_F : (m + log2f(l)) * 0.69314718055994530942f;
+    }
+    // the second share of a split block describes it to the join
+    if (wk.t0 > 0 && w == 0 && tid == 0) {
+      const int first = wk.share_of(0, c.per);
+      if (static_cast<int>(blockIdx.x) == first + 1) {
+        Join j;
+        j.rows0 = wk.s.q0;
+        j.row0 = 2 * wk.block * kTile;
+        j.rows = min(wk.s.rows - j.row0, 2 * kTile);
+        j.head = wk.head;
+        j.first_cta = first;
+        j.last_cta = wk.share_of(wk.tiles - 1, c.per);
+        a.joins[blockIdx.x] = j;
+      }
+    }
+    fence_before();
+    if (!two) bar_pair();  // both have read O and ml before either goes on
+    fence_after();
+    wk.advance(a);
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 1)
+    prompt_kernel(const __grid_constant__ CUtensorMap qm, const __grid_constant__ CUtensorMap km,
+                  const __grid_constant__ CUtensorMap rm, const __grid_constant__ CUtensorMap vm,
+                  const __grid_constant__ Args a) {
+  extern __shared__ __align__(1024) uint8_t smem[];
+  Ctrl &c = *reinterpret_cast<Ctrl *>(smem);
+  const int tid = threadIdx.x, warp = tid >> 5;
+  if (tid == 0) {
+    prefetch_tensormap(&qm);
+    prefetch_tensormap(&km);
+    prefetch_tensormap(&rm);
+    prefetch_tensormap(&vm);
+    for (int i = 0; i < kSlots; ++i) {
+      mbar_init(&c.full[i], 1);
+      mbar_init(&c.empty[i], 1);
+    }
+    mbar_init(&c.q_full, 1);
+    mbar_init(&c.q_empty, 1);
+    for (int w = 0; w < 2; ++w) {
+      mbar_init(&c.s_full[w], 1);
+      mbar_init(&c.p_ready[w], 4);
+      mbar_init(&c.o_full[w], 1);
+    }
+    fence_mbar_init();
+    c.bad_piece = 0;
+  }
+  if (warp == 9) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&c.tmem)),
+                 "r"(kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (tid == 0) a.joins[blockIdx.x].rows = 0;  // no block begins to be split here, unless the epilogue says so
+  make_plan<T>(a, c);
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = c.tmem;
+  if (warp < 8) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
+    softmax<T>(a, c, smem, tmem, warp >> 2);
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsIssue));
+    if (warp == 8)
+      producer(a, c, smem, &qm, &km, &rm, &vm);
+    else if (warp == 9)
+      mma_issuer<T>(a, c, smem, tmem);
+  }
+  fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+  }
+}
+
+// ------------------------------------------------------------------- join --
+// Blocks cut by CTA boundaries: out = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i
+// over the pieces in order (the same bits every time).  One CTA per boundary and
+// 32 rows; lane = row, warp = an eighth of the head.
+template <typename T>
+__global__ void __launch_bounds__(256) prompt_join_kernel(const __grid_constant__ Args a) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const Join j = a.joins[blockIdx.x];
+  const int prow = blockIdx.y * 32 + (threadIdx.x & 31);
+  if (prow >= j.rows) return;
+  constexpr int kPer = kDim / 8 / 4;
+  const int d4 = (threadIdx.x >> 5) * kPer;
+  float M = -CUDART_INF_F, l = 0.f;
+  float4 o[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int x = j.first_cta; x <= j.last_cta; ++x) {
+    const int64_t s = 2 * x + (x == j.first_cta ? 1 : 0);
+    const float2 ml = a.part_ml[s * 256 + prow];
+    const float top = fmaxf(M, ml.x), mm = top == -CUDART_INF_F ? 0.f : top;
+    const float old = exp2f(M - mm), keep = exp2f(ml.x - mm);
+    M = top;
+    l = fmaf(ml.y, keep, l * old);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const float4 v = *reinterpret_cast<const float4 *>(a.part_o + ((s * (kDim / 4) + d4 + i) * 256 + prow) * 4);
+      o[i].x = fmaf(v.x, keep, o[i].x * old), o[i].y = fmaf(v.y, keep, o[i].y * old);
+      o[i].z = fmaf(v.z, keep, o[i].z * old), o[i].w = fmaf(v.w, keep, o[i].w * old);
+    }
+  }
+  const int64_t orow = (j.rows0 + j.row0 + prow) * a.heads + j.head;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  T *out = static_cast<T *>(a.out) + orow * kDim + 4 * d4;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const bool none = l == 0.f;
+    const uint32_t lo = pack2(none ? 0.f : o[i].x * inv, none ? 0.f : o[i].y * inv, T());
+    const uint32_t hi = pack2(none ? 0.f : o[i].z * inv, none ? 0.f : o[i].w * inv, T());
+    *reinterpret_cast<uint2 *>(out + 4 * i) = make_uint2(lo, hi);
+  }
+  if (threadIdx.x < 32 && a.lse) a.lse[orow] = l == 0.f ? -CUDART_INF_F : (M + log2f(l)) * 0.69314718055994530942f;
+}
+
+// ----------------------------------------------------------------- launch --
+template <typename T>
+int launch(const CUtensorMap &qm, const CUtensorMap &km, const CUtensorMap &rm, const CUtensorMap &vm, const Args &a, int ctas,
+           cudaStream_t stream) {
+  static int configured[64] = {0};
+  int dev = 0;
+  B200KV_CUDA_TRY(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= 64) return set_error(B200KV_ERR_UNSUPPORTED, "device ordinal %d", dev);
+  if (!__atomic_load_n(&configured[dev], __ATOMIC_ACQUIRE)) {
+    B200KV_CUDA_TRY(cudaFuncSetAttribute(prompt_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
+    __atomic_store_n(&configured[dev], 1, __ATOMIC_RELEASE);
+  }
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(ctas));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kSmem;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  B200KV_CUDA_TRY(cudaLaunchKernelEx(&cfg, prompt_kernel<T>, qm, km, rm, vm, a));
+  cfg.gridDim = dim3(static_cast<unsigned>(ctas), 8);
+  cfg.blockDim = dim3(256);
+  cfg.dynamicSmemBytes = 0;
+  B200KV_CUDA_TRY(cudaLaunchKernelEx(&cfg, prompt_join_kernel<T>, a));
+  return B200KV_OK;
+}
+
+}  // namespace prompt
+}  // namespace b200kv

@@ -296,3 +296,102 @@ def latent_attention(
         pair = _attend(*args, return_lse) if plain else torch.ops.b200kv.latent_attention(*args)
     out, lse = pair
     return (out, lse) if return_lse else out
+
+
+def _check_heads(t: torch.Tensor, name: str, like: torch.Tensor, rows: int, width: int) -> None:
+    if t.dim() != 3 or t.shape != (rows, like.shape[1], width) or t.dtype != like.dtype or t.stride(2) != 1 \
+            or t.device != like.device:
+        raise ValueError(f"{name} must be [{rows}, {like.shape[1]}, {width}] of q's dtype with contiguous rows on its "
+                         f"device, got {tuple(t.shape)} {t.dtype}")
+
+
+def _latent_prompt_attention_impl(
+    q: torch.Tensor,
+    k_nope: torch.Tensor,
+    k_rope: torch.Tensor,
+    v: torch.Tensor,
+    q_indptr: torch.Tensor,
+    kv_indptr: torch.Tensor,
+    scale: float,
+    causal: bool,
+    error_flag: Optional[torch.Tensor],
+) -> tuple[torch.Tensor, torch.Tensor]:
+    return _attend_prompt(q, k_nope, k_rope, v, q_indptr, kv_indptr, scale, causal, error_flag, True)
+
+
+def _attend_prompt(q, k_nope, k_rope, v, q_indptr, kv_indptr, scale, causal, error_flag, want_lse):
+    _require_cuda(q, k_nope, k_rope, v, q_indptr, kv_indptr)
+    if q.dim() != 3 or q.shape[2] != NOPE + ROPE or q.dtype not in DTYPES_16 or q.stride(2) != 1:
+        raise ValueError(f"q must be fp16 or bf16 [N, H, {NOPE + ROPE}] with contiguous rows, got {tuple(q.shape)} {q.dtype}")
+    N, H, _ = q.shape
+    M, device, dtype = k_nope.shape[0], q.device, q.dtype
+    _check_heads(k_nope, "k_nope", q, M, NOPE)
+    _check_heads(v, "v", q, M, NOPE)
+    if k_rope.shape != (M, ROPE) or k_rope.dtype != dtype or k_rope.stride(1) != 1 or k_rope.device != device:
+        raise ValueError(f"k_rope must be [{M}, {ROPE}] of q's dtype with contiguous rows on its device, got "
+                         f"{tuple(k_rope.shape)} {k_rope.dtype}")
+    B = q_indptr.shape[0] - 1 if q_indptr.dim() == 1 else -1
+    if B < 0:
+        raise ValueError("q_indptr must be int32 [B + 1]")
+    for indptr, name in ((q_indptr, "q_indptr"), (kv_indptr, "kv_indptr")):
+        if indptr.dtype != torch.int32 or indptr.shape != (B + 1,) or not indptr.is_contiguous() \
+                or indptr.device != device:
+            raise ValueError(f"{name} must be a contiguous int32 [{B + 1}] tensor on q's device")
+    out = torch.empty((N, H, NOPE), dtype=dtype, device=device)
+    lse = torch.empty((N, H), dtype=torch.float32, device=device) if want_lse else None
+    if N == 0:
+        return out, lse
+    wbytes = _lib.lib().b200kv_prompt_workspace_bytes(N, M, B, H)
+    ws = workspace_for(device, wbytes) if wbytes > 0 else torch.empty(0, dtype=torch.uint8, device=device)
+    if wbytes > 0:
+        _eager.fast.set_workspace(ws)
+    launch("b200kv_latent_prompt_attention", device, q.data_ptr(), q.stride(0), q.stride(1), k_nope.data_ptr(),
+           k_nope.stride(0), k_nope.stride(1), k_rope.data_ptr(), k_rope.stride(0), v.data_ptr(), v.stride(0), v.stride(1),
+           DTYPE_CODES[dtype], q_indptr.data_ptr(), kv_indptr.data_ptr(), out.data_ptr(), _ptr(lse), N, M, B, H, scale,
+           causal, ws.data_ptr(), ws.numel(), flag_ptr(error_flag, device))
+    _maybe_check_flag(error_flag, "latent_prompt_attention")
+    return out, lse
+
+
+_latent_prompt_attention_op = torch.library.custom_op("b200kv::latent_prompt_attention", _latent_prompt_attention_impl,
+                                                      mutates_args=(), device_types="cuda")
+
+
+@_latent_prompt_attention_op.register_fake
+def _(q, k_nope, k_rope, v, q_indptr, kv_indptr, scale, causal, error_flag):
+    return q.new_empty((*q.shape[:2], NOPE)), q.new_empty(q.shape[:2], dtype=torch.float32)
+
+
+def latent_prompt_attention(
+    q: torch.Tensor,
+    k_nope: torch.Tensor,
+    k_rope: torch.Tensor,
+    v: torch.Tensor,
+    q_indptr: torch.Tensor,
+    kv_indptr: torch.Tensor,
+    scale: Optional[float] = None,
+    causal: bool = True,
+    return_lse: bool = False,
+    error_flag: Optional[torch.Tensor] = None,
+):
+    """Attention of prompts (or chunks of them), expanded form: each head has keys and
+    values of its own, multiplied out of the latent rows, and all share k_rope.
+
+    q [N, H, 192] (128 own, 64 rotary), k_nope and v [M, H, 128] (halves of one
+    product will do: strides are free), k_rope [M, 64], all fp16 or all bf16.
+    Sequence b has rows q_indptr[b] .. q_indptr[b + 1] - 1 and tokens kv_indptr[b] ..
+    kv_indptr[b + 1] - 1 (int32 [B + 1] both); its rows are the last of its tokens, so
+    with ``causal`` row i of n sees the first m - n + i + 1 of m.  Without, all of
+    them: the past of a chunk, read back by :func:`latent_load`, whose result and
+    log-sum-exps :func:`torch_spyre_b200.merge_attention_states` joins with the
+    chunk's own (it takes fp16 or fp32 outputs).  Returns out [N, H, 128] (and the natural-log LSE [N, H] fp32); a
+    row that sees nothing gets zeros and -inf.  scale defaults to 1 / sqrt(192)."""
+    if scale is None:
+        scale = 1.0 / math.sqrt(NOPE + ROPE)
+    args = (q, k_nope, k_rope, v, q_indptr, kv_indptr, float(scale), bool(causal), error_flag)
+    pair = None if _eager.compiling() else _eager.fast.latent_prompt_attention(*args, bool(return_lse))
+    if pair is None:
+        plain = direct(q, k_nope, k_rope, v, q_indptr, kv_indptr)
+        pair = _attend_prompt(*args, return_lse) if plain else torch.ops.b200kv.latent_prompt_attention(*args)
+    out, lse = pair
+    return (out, lse) if return_lse else out
