@@ -43,6 +43,7 @@ constexpr int kOffRope = kOffP + 2 * kStickTile;
 constexpr int kOffSlots = kOffRope + kStickTile;
 constexpr int kSmem = kOffSlots + kSlots * kPair;
 static_assert(kSmem <= 227 * 1024, "shared memory per CTA");
+static_assert(kSlots == 2 * kPairs, "page n has pairs (n & 1) * kPairs ..");
 
 // TMEM columns: O^T, 64 for each 128 latent elements, and two score buffers
 constexpr uint32_t kTmemCols = 512;
@@ -59,7 +60,7 @@ struct Start {  // where a share of the line begins: in block `block`, whose uni
 };
 
 struct Ctrl {
-  uint64_t full[kSlots], empty[kSlots], rope_full, rope_empty;
+  uint64_t full[4], empty[4], rope_empty;  // halves of the two pages held (the rotary stick comes with the first)
   uint64_t q_full, q_empty;
   uint64_t s_full[2], p_ready[2], p_free[2], o_full, o_empty;
   uint32_t tmem;
@@ -272,7 +273,7 @@ __device__ __forceinline__ void producer(const Args &a, Ctrl &c, uint8_t *smem, 
   uint64_t policy_again;
   asm volatile("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(policy_again));
   bool dead = false;
-  uint32_t pairs = 0, tiles = 0, pieces = 0;  // issued
+  uint32_t halves = 0, pieces = 0;  // issued
   Walk w;
   w.init(a, c);
   while (w.next(a)) {
@@ -288,31 +289,28 @@ __device__ __forceinline__ void producer(const Args &a, Ctrl &c, uint8_t *smem, 
       tma_3d(smem + kOffQ + lane * kStickTile, lane < kSticks - 1 ? qm : rm, &c.q_full, lane < kSticks - 1 ? lane * 64 : 0,
              head0, w.s.q0 + w.block * a.tile_nodes);
     ++pieces;
-    for (int t = w.t0; t < w.t1; ++t, ++tiles) {
+    for (int t = w.t0; t < w.t1 && !dead; ++t) {
       if (t / 32 > window) {
         ids = ids_next;
         ids_next = load_ids(a, w.b, ++window + 1, pages);
       }
       const int id = __shfl_sync(0xffffffffu, ids, t & 31);
       const int page = id < 0 ? a.num_blocks : id;  // an invalid id reads past the last page: zeros
-      wait(&c.rope_empty, (tiles & 1u) ^ 1u, dead, a.error_flag);
-      if ((dead = __any_sync(0xffffffffu, dead))) break;
-      if (lane == 0) {
-        mbar_arrive_expect_tx(&c.rope_full, kStickTile);
-        tma_load_3d(smem + kOffRope, sm, &c.rope_full, 0, (kSticks - 1) * kTile, page, policy);
-      }
-      for (int j = 0; j < kPairs; ++j, ++pairs) {
-        const uint32_t slot = pairs % kSlots;
-        wait(&c.empty[slot], ((pairs / kSlots) & 1u) ^ 1u, dead, a.error_flag);
+#pragma unroll
+      for (int h = 0; h < 2; ++h, ++halves) {
+        // halves 2n and 2n + 1 are page n's
+        const uint32_t n = halves >> 1, b = halves & 3u;
+        if (h == 0) wait(&c.rope_empty, (n & 1u) ^ 1u, dead, a.error_flag);
+        wait(&c.empty[b], ((n >> 1) & 1u) ^ 1u, dead, a.error_flag);
         if ((dead = __any_sync(0xffffffffu, dead))) break;
         if (lane == 0) {
-          mbar_arrive_expect_tx(&c.full[slot], kPair);
-          tma_load_3d(smem + kOffSlots + slot * kPair, pm, &c.full[slot], 0, j * 2 * kTile, page, policy);
+          uint8_t *to = smem + kOffSlots + b * 2 * kPair;
+          mbar_arrive_expect_tx(&c.full[b], 2 * kPair + (h == 0 ? kStickTile : 0));
+          if (h == 0) tma_load_3d(smem + kOffRope, sm, &c.full[b], 0, (kSticks - 1) * kTile, page, policy);
+          tma_load_3d(to, pm, &c.full[b], 0, h * 4 * kTile, page, policy);
+          tma_load_3d(to + kPair, pm, &c.full[b], 0, h * 4 * kTile + 2 * kTile, page, policy);
         }
-      }
-      if (dead) {
-        ++tiles;
-        break;
+        __syncwarp();
       }
     }
     if (dead) break;
@@ -321,9 +319,7 @@ __device__ __forceinline__ void producer(const Args &a, Ctrl &c, uint8_t *smem, 
   if (dead) {  // the copies under way, with a limit
     bool late = false;
     if (pieces > 0) wait(&c.q_full, (pieces - 1) & 1u, late, a.error_flag);
-    if (tiles > 0) wait(&c.rope_full, (tiles - 1) & 1u, late, a.error_flag);
-    for (uint32_t n = pairs - min(pairs, uint32_t(kSlots)); n < pairs; ++n)
-      wait(&c.full[n % kSlots], (n / kSlots) & 1u, late, a.error_flag);
+    for (uint32_t n = halves - min(halves, 4u); n < halves; ++n) wait(&c.full[n & 3u], (n >> 2) & 1u, late, a.error_flag);
   }
   // the last arrival that the MMAs owe this CTA: not before it may the CTA end
   if (lane == 0 && pieces > 0) {
@@ -334,18 +330,22 @@ __device__ __forceinline__ void producer(const Args &a, Ctrl &c, uint8_t *smem, 
 }
 
 // One warp, converged, issues every MMA from an elected lane.  Scores run up to
-// one page ahead of the values; of the two, what is ready goes first.
+// one page ahead of the values; of the two, what is ready goes first.  A decision
+// costs little beside the MMAs' own time (1150 clocks for a page's scores, 770 for its
+// values): all lanes test the same barrier (14 clocks; barriers of their own would take
+// 13 a lane), and one shuffle makes turn and buffer uniform, from which all operands
+// follow (an MMA whose descriptors come from ordinary registers takes 60 to 80
+// clocks to issue, twice its own time).
 template <typename T>
 __device__ __forceinline__ void mma_issuer(const Args &a, Ctrl &c, uint8_t *smem, uint32_t tmem_any) {
   constexpr uint32_t kBase = (1u << 4) | (std::is_same<T, __half>::value ? 0u : (1u << 7) | (1u << 10));
   constexpr uint32_t kIdescQK = kBase | (uint32_t(kTile >> 3) << 17) | (uint32_t(kTileRows >> 4) << 24);
   constexpr uint32_t kIdescPV = kBase | (1u << 15) | (uint32_t(128 >> 4) << 24);  // A (V^T): M-major
   const uint32_t go = elect_one(), tmem = uniform(tmem_any);
-  const uint32_t negate = a.scale < 0.f ? 1u << 13 : 0u;  // a negative scale turns Q's sign
-  const uint32_t qd = desc_kmajor(uniform(smem_u32(smem + kOffQ)));
-  const uint32_t pd = desc_kmajor(uniform(smem_u32(smem + kOffP)));
-  const uint32_t rd = desc_kmajor(uniform(smem_u32(smem + kOffRope)));
-  const uint32_t slots = uniform(smem_u32(smem + kOffSlots));
+  const uint32_t idesc_qk = kIdescQK | (a.scale < 0.f ? 1u << 13 : 0u);  // a negative scale turns Q's sign
+  const uint32_t qd = desc_kmajor(smem_u32(smem + kOffQ)), rd = desc_kmajor(smem_u32(smem + kOffRope));
+  const uint32_t pd = desc_kmajor(smem_u32(smem + kOffP)), kd = desc_kmajor(smem_u32(smem + kOffSlots));
+  const uint32_t vd = (smem_u32(smem + kOffSlots) >> 4) | (uint32_t(kStickTile >> 4) << 16);
   auto done = [&](uint64_t *bar) {
     if (go) commit(bar);
   };
@@ -354,83 +354,78 @@ __device__ __forceinline__ void mma_issuer(const Args &a, Ctrl &c, uint8_t *smem
   wp = wq;
   bool more = wq.next(a), left = wp.next(a);
   int tq = wq.t0, tp = wp.t0;
-  uint32_t nq = 0, np = 0;            // pages whose scores are complete, whose values are
-  uint32_t sub = 0;                   // the next part of page nq: the rotary stick, then the pairs
+  uint32_t nq = 0, np = 0;  // pages whose scores are complete, whose values are
+  uint32_t half = 0;        // of page nq: the next half of its scores
   uint32_t piece_q = 0, piece_p = 0;
   uint32_t idle = 0;
   uint64_t since = 0;
-  while (left) {
-    bool moved = false;
-    if (np < nq) {
-      const bool first = tp == wp.t0;
-      bool ready = mbar_test(&c.p_ready[np & 1], (np >> 1) & 1u);
-      if (first) ready = ready && mbar_test(&c.o_empty, (piece_p & 1u) ^ 1u);
-      if (__all_sync(0xffffffffu, ready)) {
-        fence_after();
-        const uint32_t idesc = kIdescPV | (uint32_t((wp.rows(a) + 15) / 16 * 2) << 17);
-        const uint32_t p = pd + ((np & 1u) * kStickTile >> 4);
-#pragma unroll 1
-        for (int m = 0; m < kPairs; ++m) {
-          const uint32_t slot = (np * kPairs + m) % kSlots;
-          const uint32_t vd = ((slots + slot * kPair) >> 4) | (uint32_t(kStickTile >> 4) << 16);
+  uint32_t idesc_pv = uniform(kIdescPV | (uint32_t((wp.rows(a) + 15) / 16 * 2) << 17));
+  // what this warp does next: nothing, values, the first or second half of scores; | 4 in the odd buffer, | 8 adding up
+  for (;;) {
+    uint32_t turn = left ? 0 : 16;
+    if (np < nq && mbar_test(&c.p_ready[np & 1u], (np >> 1) & 1u) &&
+        (tp > wp.t0 || mbar_test(&c.o_empty, (piece_p & 1u) ^ 1u)))
+      turn = 1 | (np & 1u) << 2 | (tp > wp.t0 ? 8 : 0);
+    else if (more && nq <= np + 1 && mbar_test(&c.full[(nq & 1u) * 2 + half], (nq >> 1) & 1u) &&
+             (half || tq > wq.t0 || mbar_test(&c.q_full, piece_q & 1u)))
+      turn = (2 + half) | (nq & 1u) << 2;
+    turn = uniform(turn);
+    const uint32_t odd = (turn >> 2) & 1u;
+    if ((turn & 3) == 1) {
+      fence_after();
+      const uint32_t p = pd + (odd * kStickTile >> 4), v = vd + (odd * kPairs * kPair >> 4);
 #pragma unroll
-          for (int k = 0; k < kTile / 16; ++k)
-            mma_ss(tmem + col_o(m), vd + (k * 2048 >> 4), p + (k * 32 >> 4), idesc, !first || k > 0, go);
-          done(&c.empty[slot]);
-        }
-        done(&c.p_free[np & 1]);
-        ++np;
-        if (++tp >= wp.t1) {
-          done(&c.o_full);
-          ++piece_p;
-          wp.advance(a);
-          left = wp.next(a);
-          tp = wp.t0;
-        }
-        moved = true;
+      for (int m = 0; m < kPairs; ++m) {
+#pragma unroll
+        for (int k = 0; k < kTile / 16; ++k)
+          mma_ss(tmem + col_o(m), v + (m * kPair + k * 2048 >> 4), p + (k * 32 >> 4), idesc_pv, k > 0 ? 1 : turn & 8, go);
+        if (m & 1) done(&c.empty[odd * 2 + m / 2]);
       }
-    }
-    if (!moved && more && nq <= np + 1) {
-      const uint32_t slot = (nq * kPairs + sub - 1) % kSlots;
-      bool ready;
-      if (sub == 0)
-        ready = mbar_test(&c.rope_full, nq & 1u) && (tq > wq.t0 || mbar_test(&c.q_full, piece_q & 1u));
-      else
-        ready = mbar_test(&c.full[slot], ((nq * kPairs + sub - 1) / kSlots) & 1u);
-      if (__all_sync(0xffffffffu, ready)) {
-        fence_after();
-        const uint32_t s = tmem + col_s(nq & 1);
-        if (sub == 0) {
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            mma_ss(s, qd + ((kSticks - 1) * kStickTile + k * 32 >> 4), rd + (k * 32 >> 4), kIdescQK | negate, k > 0, go);
-          done(&c.rope_empty);
-          ++sub;
-        } else {
-          const uint32_t q = qd + ((sub - 1) * kPair >> 4), kd = desc_kmajor(slots + slot * kPair);
-#pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const uint32_t off = ((k >> 2) * kStickTile + (k & 3) * 32) >> 4;
-            mma_ss(s, q + off, kd + off, kIdescQK | negate, 1, go);
-          }
-          if (++sub > kPairs) {
-            sub = 0;
-            done(&c.s_full[nq & 1]);
-            ++nq;
-            if (++tq >= wq.t1) {
-              done(&c.q_empty);
-              ++piece_q;
-              wq.advance(a);
-              more = wq.next(a);
-              tq = wq.t0;
-            }
-          }
-        }
-        moved = true;
+      done(&c.p_free[odd]);
+      ++np;
+      if (++tp >= wp.t1) {
+        done(&c.o_full);
+        ++piece_p;
+        wp.advance(a);
+        left = wp.next(a);
+        tp = wp.t0;
+        idesc_pv = uniform(kIdescPV | (uint32_t((wp.rows(a) + 15) / 16 * 2) << 17));
       }
-    }
-    if (moved) {
       idle = 0;
+    } else if ((turn & 3) != 0) {
+      fence_after();
+      const uint32_t s = tmem + col_s(0) + odd * 64, k0 = kd + (odd * kPairs * kPair >> 4);
+      if ((turn & 3) == 2) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          mma_ss(s, qd + ((kSticks - 1) * kStickTile + k * 32 >> 4), rd + (k * 32 >> 4), idesc_qk, k > 0, go);
+        done(&c.rope_empty);
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+          const uint32_t off = ((k >> 2) * kStickTile + (k & 3) * 32) >> 4;
+          mma_ss(s, qd + off, k0 + off, idesc_qk, 1, go);
+        }
+        half = 1;
+      } else {
+#pragma unroll
+        for (int k = 16; k < 32; ++k) {
+          const uint32_t off = ((k >> 2) * kStickTile + (k & 3) * 32) >> 4;
+          mma_ss(s, qd + off, k0 + off, idesc_qk, 1, go);
+        }
+        done(&c.s_full[odd]);
+        half = 0;
+        ++nq;
+        if (++tq >= wq.t1) {
+          done(&c.q_empty);
+          ++piece_q;
+          wq.advance(a);
+          more = wq.next(a);
+          tq = wq.t0;
+        }
+      }
+      idle = 0;
+    } else if (turn == 16) {
+      break;
     } else if ((++idle & 1023u) == 0) {
       const uint64_t now = global_timer_ns();
       if (idle == 1024u) since = now;
@@ -603,7 +598,8 @@ __device__ __forceinline__ void softmax(const Args &a, Ctrl &c, uint8_t *smem, u
         // every row sees (repair_row)
         const int from = max(common - pos, 0), end = len - pos;
         for (int j = 0; j < kPairs; ++j) {
-          uint8_t *v = smem + kOffSlots + (n * kPairs + j) % kSlots * kPair + tid * 16;
+          if ((j & 1) == 0) wait(&c.full[(n & 1) * 2 + j / 2], (n >> 1) & 1u, dead, a.error_flag);
+          uint8_t *v = smem + kOffSlots + ((n & 1) * kPairs + j) * kPair + tid * 16;
 #pragma unroll 1
           for (int k = min(from, end) / 16; k < 4; ++k)
             for (int st = 0; st < 2; ++st) {
@@ -708,11 +704,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     prefetch_tensormap(&rm);
     prefetch_tensormap(&pm);
     prefetch_tensormap(&sm);
-    for (int i = 0; i < kSlots; ++i) {
+    for (int i = 0; i < 4; ++i) {
       mbar_init(&c.full[i], 1);
       mbar_init(&c.empty[i], 1);
     }
-    mbar_init(&c.rope_full, 1);
     mbar_init(&c.rope_empty, 1);
     mbar_init(&c.q_full, 1);
     mbar_init(&c.q_empty, 1);
