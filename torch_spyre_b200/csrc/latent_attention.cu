@@ -4,11 +4,12 @@
 //   out[t, h] = sum_p exp(s_p - m) c'_p / sum_p exp(s_p - m),  m = max_p s_p;
 // a row that sees nothing is zero with lse = -inf.
 //
-// latent_mma.cuh has the kernels; here are the C entries and the tensor maps.
+// latent_mma.cuh and latent_pair.cuh have the kernels; here are the C entries, the
+// tensor maps and the launches.
 #include <cmath>
 
 #include "decode_common.cuh"
-#include "latent_mma.cuh"
+#include "latent_pair.cuh"
 
 namespace b200kv {
 namespace {
@@ -38,13 +39,49 @@ Workspace workspace_of() {
   return w;
 }
 
+// The attention (on single SMs or on pairs) and the join behind it.
+template <typename T>
+int launch(const CUtensorMap &qm, const CUtensorMap &rm, const CUtensorMap &pm, const CUtensorMap &sm,
+           const latent::Args &a, bool pairs, int ctas, cudaStream_t stream) {
+  const auto kernel = pairs ? latent::pair::latent_pair_kernel<T> : latent::latent_kernel<T>;
+  const int smem = pairs ? latent::pair::kSmem : latent::kSmem;
+  static int configured[2][64] = {{0}};
+  int dev = 0;
+  B200KV_CUDA_TRY(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= 64) return set_error(B200KV_ERR_UNSUPPORTED, "device ordinal %d", dev);
+  if (!__atomic_load_n(&configured[pairs][dev], __ATOMIC_ACQUIRE)) {
+    B200KV_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    __atomic_store_n(&configured[pairs][dev], 1, __ATOMIC_RELEASE);
+  }
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 2;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(ctas));
+  cfg.blockDim = dim3(latent::kThreads);
+  cfg.dynamicSmemBytes = static_cast<size_t>(smem);
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = pairs ? 2 : 1;
+  B200KV_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, qm, rm, pm, sm, a));
+  cfg.gridDim = dim3(static_cast<unsigned>(ctas), static_cast<unsigned>((a.box_nodes * a.head_box + 7) / 8));
+  cfg.blockDim = dim3(256);
+  cfg.dynamicSmemBytes = 0;
+  cfg.numAttrs = 1;
+  B200KV_CUDA_TRY(cudaLaunchKernelEx(&cfg, latent::latent_join_kernel<T>, a));
+  return B200KV_OK;
+}
+
 }  // namespace
 }  // namespace b200kv
 
 using namespace b200kv;
 
 extern "C" int64_t b200kv_latent_workspace_bytes(int64_t total_q, int64_t batch, int64_t num_heads) {
-  if (total_q < 0 || batch < 0 || num_heads <= 0 || num_heads > latent::kMaxParts * latent::kTileRows) return -1;
+  if (total_q < 0 || batch < 0 || num_heads <= 0 || num_heads > latent::kMaxHeads) return -1;
   return workspace_of().total;
 }
 
@@ -59,7 +96,7 @@ extern "C" int b200kv_latent_attention(const void *q_latent, int64_t q_latent_st
   clear_error();
   B200KV_CHECK_ARG(dtype == B200KV_F16 || dtype == B200KV_BF16, "dtype %d is not fp16 or bf16", dtype);
   B200KV_CHECK_ARG(num_heads > 0, "num_heads %lld out of range", (long long)num_heads);
-  if (num_heads > latent::kMaxParts * latent::kTileRows)
+  if (num_heads > latent::kMaxHeads)
     return set_error(B200KV_ERR_UNSUPPORTED, "%lld heads unsupported (<= 512)", (long long)num_heads);
   B200KV_CHECK_ARG(batch >= 0 && total_q >= 0 && total_q * num_heads < (int64_t{1} << 31),
                    "batch or total_q * num_heads out of range");
@@ -73,9 +110,12 @@ extern "C" int b200kv_latent_attention(const void *q_latent, int64_t q_latent_st
                    (long long)mask_words, (long long)max_nodes);
   B200KV_CHECK_ARG(std::isfinite(scale), "scale must be finite");
   latent::Args a{};
-  a.parts = static_cast<int>((num_heads + 63) / 64);
   a.head_box = static_cast<int>(num_heads < 64 ? num_heads : 64);
   a.tile_nodes = 64 / a.head_box;
+  // Blocks of more than 64 rows, as far as the host knows, go to pairs of SMs.
+  const bool pairs = num_heads > 64 || total_q > batch * a.tile_nodes;
+  a.stride = pairs ? 2 * static_cast<int>((num_heads + 127) / 128) : 1;
+  a.block_nodes = pairs && num_heads <= 64 ? 2 * a.tile_nodes : a.tile_nodes;
   // the kernel counts its units of work in 31 bits
   if ((batch + total_q / a.tile_nodes + 1) * (max_blocks_per_seq + latent::kBegin) >= (int64_t{1} << 31))
     return set_error(B200KV_ERR_UNSUPPORTED, "2^31 or more steps of rows and tokens");
@@ -127,10 +167,10 @@ extern "C" int b200kv_latent_attention(const void *q_latent, int64_t q_latent_st
   if ((st = q_map(&qm, q_latent, q_latent_stride_t, q_latent_stride_h, latent::kRank)) != B200KV_OK) return st;
   if ((st = q_map(&rm, q_rope, q_rope_stride_t, q_rope_stride_h, latent::kRope)) != B200KV_OK) return st;
   if ((st = pool_map(&pm, 2)) != B200KV_OK || (st = pool_map(&sm, 1)) != B200KV_OK) return st;
-  const int ctas = (sms < latent::kMaxCtas ? sms : latent::kMaxCtas) / a.parts * a.parts;
+  const int ctas = (sms < latent::kMaxCtas ? sms : latent::kMaxCtas) / a.stride * a.stride;
   if (ctas == 0) return set_error(B200KV_ERR_UNSUPPORTED, "a GPU of %d SMs", sms);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   const WorkspaceLock lock(workspace);
-  return dtype == B200KV_F16 ? latent::launch<__half>(qm, rm, pm, sm, a, ctas, s)
-                             : latent::launch<__nv_bfloat16>(qm, rm, pm, sm, a, ctas, s);
+  return dtype == B200KV_F16 ? launch<__half>(qm, rm, pm, sm, a, pairs, ctas, s)
+                             : launch<__nv_bfloat16>(qm, rm, pm, sm, a, pairs, ctas, s);
 }

@@ -10,14 +10,14 @@ constexpr int kRank = B200KV_LATENT_RANK, kRope = B200KV_LATENT_ROPE, kRow = kRa
 constexpr int kSticks = kRow / 64;
 constexpr int kMaxCtas = 148;  // one CTA per SM of a B200
 constexpr int kTileRows = 64;  // rows of q that a CTA holds
-constexpr int kMaxParts = 8;
+constexpr int kMaxHeads = 512;
 
 // A block of rows whose token tiles are spread over shares first .. last; its
 // partials are in slot 2 * cta + 1 of the first share's CTA and slots 2 * cta of
 // the others'.
 struct Join {
   int64_t rows0;  // first row of q of the sequence
-  int node0, nodes, first, last;
+  int node0, nodes, head0, first, last, pad;
 };
 
 struct Args {
@@ -30,9 +30,10 @@ struct Args {
   void *out;  // contiguous [N, H, 512]
   float *lse;
   int total_q, batch, heads, max_blocks, max_nodes, num_blocks;
-  int parts;       // CTAs that share a node's heads, 64 each; 1 where there are up to 64
-  int head_box;    // heads of a Q tile
-  int tile_nodes;  // nodes of a Q tile
+  int stride;       // CTAs of a share: they walk the same blocks, each with rows of its own
+  int head_box;     // heads of a Q tile (a CTA's rows)
+  int tile_nodes;   // nodes of a Q tile
+  int block_nodes;  // nodes of a block
   int box_nodes;   // nodes of a TMA box of Q (no more than a sequence can have)
   float scale;
   int32_t *error_flag;

@@ -13,16 +13,23 @@
 // rows on M it would take all 512.  V^T is the page as it lies (tokens are the
 // reduction, their 64-element sticks M-major), P goes through shared memory.
 //
-// The cache's page is loaded once, as four pairs of sticks and the rotary stick;
-// a pair is free again once O has taken it.  Eight pairs are held, so the MMA
-// warp takes whichever is ready first: the next page's scores, stick by stick as
-// they arrive, or this page's values, as soon as its weights are there.
+// The cache's page is loaded once, in two halves (the rotary stick with the first),
+// and its slots are free again once O has taken it.  Two pages are held: one warp
+// issues the next page's scores as its halves arrive, another this page's values as
+// soon as its weights are there.
 //
 // The blocks' pages, all sequences one after the other, form one line that is cut
 // into equal shares; blocks cut by a share's end are joined by latent_join_kernel.
 //
-// Warps: 0-3 softmax and output (thread = row: lanes 0-15 of warp w have rows
-// 16w .. 16w + 15, where an M = 64 accumulator lies), 4 TMA producer, 5 MMA issuer.
+// Bound, up to 64 rows: memory; the products take 1920 of the 3080 clocks that a page's
+// 74 KB take at the copy rate on every SM.  What costs beside that are the hand-overs:
+// a wait for a barrier that is already complete takes some 200 clocks of a warp's time
+// between products, so there are few of them, and roles that would wait for one another
+// are warps of their own.
+//
+// Warps: 0-7 softmax and output (warp w: lanes 0-15 of quadrant w % 4 have rows
+// 16 (w % 4) .., where an M = 64 accumulator lies, and half w / 4 of a page's tokens),
+// 8 TMA producer, 9 issues the scores' MMAs, 10 the values'.
 #pragma once
 
 #include "latent_attention.h"
@@ -33,7 +40,8 @@ namespace latent {
 
 using namespace umma;
 
-constexpr int kThreads = 192;
+constexpr int kThreads = 384;  // (one warp without a role here, the pairs' relay there)
+constexpr int kSoftmaxWarps = 8;
 constexpr int kTile = kPageTokens;
 constexpr int kStickTile = kTile * 128, kPair = 2 * kStickTile, kPairs = 4, kSlots = 8;
 constexpr float kLazyLog2 = 8.f;
@@ -59,15 +67,19 @@ struct Start {  // where a share of the line begins: in block `block`, whose uni
   int b, block, u0;
 };
 
+struct Plan {
+  int per, total;  // units of a share, of the line
+  Start start;
+  int scan[kThreads / 32];
+};
+
 struct Ctrl {
   uint64_t full[4], empty[4], rope_empty;  // halves of the two pages held (the rotary stick comes with the first)
   uint64_t q_full, q_empty;
   uint64_t s_full[2], p_ready[2], p_free[2], o_full, o_empty;
   uint32_t tmem;
-  int per, total;  // units of a share, of the line
-  Start start;
-  int scan[kThreads / 32];
-  unsigned bad_piece;  // last piece (counted from 1) that met a non-finite value in a node's row
+  Plan plan;
+  float top[2][kTileRows];  // maxima, then sums, of the halves of a row's tokens
   float factor[kTileRows];  // of O's columns
   int row_at[kTileRows];    // row of out, -1: none
 };
@@ -84,10 +96,25 @@ __device__ __forceinline__ bool mbar_test(uint64_t *bar, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
-__device__ __forceinline__ void bar_softmax() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+// Waits, with a limit, until `ready` (which tests barriers side by side) holds.
+template <typename Ready>
+__device__ __forceinline__ void wait_until(Ready ready, bool &dead, int32_t *flag) {
+  if (dead || ready()) return;
+  uint64_t t0 = 0;
+  for (uint32_t i = 1;; ++i) {
+    if (ready()) return;
+    if ((i & 1023u) != 0) continue;
+    const uint64_t now = global_timer_ns();
+    if (t0 == 0) t0 = now;
+    if (now - t0 > kWaitLimitNs) break;
+  }
+  dead = true;
+  if (flag) atomicOr(flag, B200KV_DEVERR_TIMEOUT);
+}
+__device__ __forceinline__ void bar_softmax() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 __device__ __forceinline__ bool any_softmax(bool x) {
   uint32_t r;
-  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, 1, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
                : "=r"(r)
                : "r"(uint32_t(x))
                : "memory");
@@ -111,45 +138,51 @@ __device__ __forceinline__ Seq load_seq(const Args &a, int b, bool report) {
   bad = bad || s.nodes > most;
   s.nodes = min(s.nodes, most);
   if (bad && report && a.error_flag) atomicOr(a.error_flag, B200KV_DEVERR_BAD_LEN);
-  s.blocks = (s.nodes + a.tile_nodes - 1) / a.tile_nodes;
+  s.blocks = (s.nodes + a.block_nodes - 1) / a.block_nodes;
   return s;
 }
-// Pages of block k: what its last node can see.
+// Token tiles (of kStep tokens) of block k: what its last node can see.
+template <int kStep>
 __device__ __forceinline__ int block_tiles(const Args &a, const Seq &s, int k) {
-  const int nodes = a.mask ? s.nodes : min(s.nodes, (k + 1) * a.tile_nodes);
-  return (s.ctx + nodes + kTile - 1) / kTile;
+  const int nodes = a.mask ? s.nodes : min(s.nodes, (k + 1) * a.block_nodes);
+  return (s.ctx + nodes + kStep - 1) / kStep;
 }
-// The line is cut by cost: a page counts one, a block's beginning and end kBegin.
+// The line is cut by cost: a tile counts one, a block's beginning and end kBegin.
 constexpr int kBegin = 4;
-__device__ __forceinline__ int block_units(const Args &a, const Seq &s, int k) { return kBegin + block_tiles(a, s, k); }
+template <int kStep>
+__device__ __forceinline__ int block_units(const Args &a, const Seq &s, int k) {
+  return kBegin + block_tiles<kStep>(a, s, k);
+}
+template <int kStep>
 __device__ __forceinline__ int seq_units(const Args &a, const Seq &s) {
-  if (a.mask) return s.blocks > 0 ? s.blocks * block_units(a, s, 0) : 0;
+  if (a.mask) return s.blocks > 0 ? s.blocks * block_units<kStep>(a, s, 0) : 0;
   int n = 0;
-  for (int k = 0; k < s.blocks; ++k) n += block_units(a, s, k);
+  for (int k = 0; k < s.blocks; ++k) n += block_units<kStep>(a, s, k);
   return n;
 }
 
 // The blocks of a share, one piece (a block, or the part of it in this share) at
 // a time.  Every role walks the same sequence.
+template <int kStep>
 struct Walk {
   Seq s;
-  int b, block, u0, tiles, t0, t1;  // piece: pages [t0, t1) of `tiles`
+  int b, block, u0, tiles, t0, t1;  // piece: token tiles [t0, t1) of `tiles`
   int first, end;                   // of the share
 
-  __device__ __forceinline__ void init(const Args &a, const Ctrl &c) {
+  __device__ __forceinline__ void init(const Args &a, const Plan &c) {
     const Start &f = c.start;
     s = f.s, b = f.b, block = f.block, u0 = f.u0;
     t0 = t1 = 0;
-    const int share = static_cast<int>(blockIdx.x) / a.parts;
+    const int share = static_cast<int>(blockIdx.x) / a.stride;
     first = share * c.per;
     end = min(c.total, first + c.per);
   }
-  // Page t belongs to the share that holds its unit; the begin goes with the first.
+  // Tile t belongs to the share that holds its unit; the begin goes with the first.
   __device__ __forceinline__ int tile_from(int unit) const { return min(max(unit - u0 - kBegin, 0), tiles); }
   __device__ __forceinline__ bool next(const Args &a) {
     for (;;) {
       if (u0 >= end || first >= end) return false;
-      tiles = block_tiles(a, s, block);
+      tiles = block_tiles<kStep>(a, s, block);
       t0 = tile_from(first);
       t1 = tile_from(end);
       if (t0 < t1) return true;
@@ -157,7 +190,7 @@ struct Walk {
     }
   }
   __device__ __forceinline__ void advance(const Args &a) {
-    u0 += block_units(a, s, block);
+    u0 += block_units<kStep>(a, s, block);
     if (u0 >= end) return;
     if (++block >= s.blocks) {
       block = 0;
@@ -190,8 +223,8 @@ __device__ __noinline__ void clear_rows(const Args &a, bool all) {
 // The line's length, a share's, and where this CTA's begins; all threads call it,
 // a barrier follows.  (With a q_indptr that descends nothing has a sequence: its
 // sequences could have the same rows, and the counts pass 31 bits.)
-template <typename T>
-__device__ __forceinline__ void make_plan(const Args &a, Ctrl &c) {
+template <typename T, int kStep>
+__device__ __forceinline__ void make_plan(const Args &a, Plan &c) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int each = (a.batch + kThreads - 1) / kThreads;
   const int b0 = tid * each, b1 = min(b0 + each, a.batch);
@@ -200,7 +233,7 @@ __device__ __forceinline__ void make_plan(const Args &a, Ctrl &c) {
   bool unclaimed = false, descends = false;
   for (int b = b0; b < b1; ++b) {
     s = load_seq(a, b, blockIdx.x == 0);
-    mine += seq_units(a, s);
+    mine += seq_units<kStep>(a, s);
     unclaimed = unclaimed || (b == 0 && s.q0 > 0) || s.q0 + s.nodes < s.end;
     descends = descends || s.end < s.q0;
   }
@@ -223,25 +256,25 @@ __device__ __forceinline__ void make_plan(const Args &a, Ctrl &c) {
     total += c.scan[w];
   }
   if (none) total = mine = 0;
-  const int shares = static_cast<int>(gridDim.x) / a.parts;
+  const int shares = static_cast<int>(gridDim.x) / a.stride;
   const int per = max(2, static_cast<int>((static_cast<unsigned>(total) + shares - 1) / shares));
-  const int first = static_cast<int>(blockIdx.x) / a.parts * per;
+  const int first = static_cast<int>(blockIdx.x) / a.stride * per;
   int at = before + incl - mine;
   if (first >= at && first < at + mine) {
     int b = b0;
     for (;; ++b) {
       if (each > 1) s = load_seq(a, b, false);
-      const int n = seq_units(a, s);
+      const int n = seq_units<kStep>(a, s);
       if (first < at + n) break;
       at += n;
     }
     int block = 0;
     if (a.mask) {
-      const int n = block_units(a, s, 0);
+      const int n = block_units<kStep>(a, s, 0);
       block = (first - at) / n;
       at += block * n;
     } else {
-      for (int n; first >= at + (n = block_units(a, s, block)); ++block) at += n;
+      for (int n; first >= at + (n = block_units<kStep>(a, s, block)); ++block) at += n;
     }
     c.start = Start{s, b, block, at};
   }
@@ -267,18 +300,18 @@ __device__ __forceinline__ int load_ids(const Args &a, int b, int window, int pa
 __device__ __forceinline__ void producer(const Args &a, Ctrl &c, uint8_t *smem, const CUtensorMap *qm,
                                          const CUtensorMap *rm, const CUtensorMap *pm, const CUtensorMap *sm) {
   const int lane = threadIdx.x & 31;
-  const int head0 = static_cast<int>(blockIdx.x) % a.parts * a.head_box;
+  const int head0 = static_cast<int>(blockIdx.x) % a.stride * a.head_box;
   const uint32_t q_bytes = static_cast<uint32_t>(a.box_nodes * a.head_box * 128);
   const uint64_t policy_once = l2_policy_evict_first();
   uint64_t policy_again;
   asm volatile("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(policy_again));
   bool dead = false;
   uint32_t halves = 0, pieces = 0;  // issued
-  Walk w;
-  w.init(a, c);
+  Walk<kTile> w;
+  w.init(a, c.plan);
   while (w.next(a)) {
     // pages that one block of one CTA reads leave L2 first
-    const uint64_t policy = a.parts > 1 || w.s.blocks > 1 ? policy_again : policy_once;
+    const uint64_t policy = a.stride > 1 || w.s.blocks > 1 ? policy_again : policy_once;
     const int pages = (w.s.ctx + w.s.nodes + kPageTokens - 1) / kPageTokens;
     int window = w.t0 / 32, ids = load_ids(a, w.b, window, pages), ids_next = load_ids(a, w.b, window + 1, pages);
     wait(&c.q_empty, (pieces & 1u) ^ 1u, dead, a.error_flag);
@@ -329,111 +362,101 @@ __device__ __forceinline__ void producer(const Args &a, Ctrl &c, uint8_t *smem, 
   __syncwarp();
 }
 
-// One warp, converged, issues every MMA from an elected lane.  Scores run up to
-// one page ahead of the values; of the two, what is ready goes first.  A decision
-// costs little beside the MMAs' own time (1150 clocks for a page's scores, 770 for its
-// values): all lanes test the same barrier (14 clocks; barriers of their own would take
-// 13 a lane), and one shuffle makes turn and buffer uniform, from which all operands
-// follow (an MMA whose descriptors come from ordinary registers takes 60 to 80
-// clocks to issue, twice its own time).
+// The two MMA warps, converged, issue from an elected lane.  Operands are made uniform
+// first: an MMA whose descriptors come from ordinary registers takes 60 to 80 clocks to
+// issue, twice its own time.
 template <typename T>
-__device__ __forceinline__ void mma_issuer(const Args &a, Ctrl &c, uint8_t *smem, uint32_t tmem_any) {
-  constexpr uint32_t kBase = (1u << 4) | (std::is_same<T, __half>::value ? 0u : (1u << 7) | (1u << 10));
-  constexpr uint32_t kIdescQK = kBase | (uint32_t(kTile >> 3) << 17) | (uint32_t(kTileRows >> 4) << 24);
-  constexpr uint32_t kIdescPV = kBase | (1u << 15) | (uint32_t(128 >> 4) << 24);  // A (V^T): M-major
+constexpr uint32_t kIdesc = (1u << 4) | (std::is_same<T, __half>::value ? 0u : (1u << 7) | (1u << 10));
+
+template <typename T>
+__device__ __forceinline__ void score_issuer(const Args &a, Ctrl &c, uint8_t *smem, uint32_t tmem_any) {
   const uint32_t go = elect_one(), tmem = uniform(tmem_any);
-  const uint32_t idesc_qk = kIdescQK | (a.scale < 0.f ? 1u << 13 : 0u);  // a negative scale turns Q's sign
+  const uint32_t idesc = kIdesc<T> | (uint32_t(kTile >> 3) << 17) | (uint32_t(kTileRows >> 4) << 24) |
+                         (a.scale < 0.f ? 1u << 13 : 0u);  // a negative scale turns Q's sign
   const uint32_t qd = desc_kmajor(smem_u32(smem + kOffQ)), rd = desc_kmajor(smem_u32(smem + kOffRope));
-  const uint32_t pd = desc_kmajor(smem_u32(smem + kOffP)), kd = desc_kmajor(smem_u32(smem + kOffSlots));
+  const uint32_t kd = desc_kmajor(smem_u32(smem + kOffSlots));
+  auto done = [&](uint64_t *bar) {
+    if (go) commit(bar);
+  };
+  bool dead = false;
+  uint32_t n = 0, pieces = 0;  // pages, pieces
+  Walk<kTile> w;
+  w.init(a, c.plan);
+  while (w.next(a)) {
+    for (int t = w.t0; t < w.t1; ++t, ++n) {
+      const uint32_t odd = uniform(n & 1u);
+      // this score buffer is free once the page before last has weights
+      wait_until(
+          [&] {
+            const bool free = n < 2 || mbar_test(&c.p_ready[odd], ((n - 2) >> 1) & 1u);
+            const bool q = t > w.t0 || mbar_test(&c.q_full, pieces & 1u);
+            return free & q & mbar_test(&c.full[2 * odd], (n >> 1) & 1u);
+          },
+          dead, a.error_flag);
+      fence_after();
+      const uint32_t s = tmem + col_s(0) + odd * 64, k0 = kd + (odd * kPairs * kPair >> 4);
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        mma_ss(s, qd + ((kSticks - 1) * kStickTile + k * 32 >> 4), rd + (k * 32 >> 4), idesc, k > 0, go);
+      done(&c.rope_empty);
+#pragma unroll
+      for (int k = 0; k < 16; ++k) {
+        const uint32_t off = ((k >> 2) * kStickTile + (k & 3) * 32) >> 4;
+        mma_ss(s, qd + off, k0 + off, idesc, 1, go);
+      }
+      wait_until([&] { return mbar_test(&c.full[2 * odd + 1], (n >> 1) & 1u); }, dead, a.error_flag);
+      fence_after();
+#pragma unroll
+      for (int k = 16; k < 32; ++k) {
+        const uint32_t off = ((k >> 2) * kStickTile + (k & 3) * 32) >> 4;
+        mma_ss(s, qd + off, k0 + off, idesc, 1, go);
+      }
+      done(&c.s_full[odd]);
+    }
+    done(&c.q_empty);
+    ++pieces;
+    w.advance(a);
+  }
+  __syncwarp();
+}
+
+template <typename T>
+__device__ __forceinline__ void value_issuer(const Args &a, Ctrl &c, uint8_t *smem, uint32_t tmem_any) {
+  const uint32_t go = elect_one(), tmem = uniform(tmem_any);
+  const uint32_t pd = desc_kmajor(smem_u32(smem + kOffP));
   const uint32_t vd = (smem_u32(smem + kOffSlots) >> 4) | (uint32_t(kStickTile >> 4) << 16);
   auto done = [&](uint64_t *bar) {
     if (go) commit(bar);
   };
-  Walk wq, wp;  // the pieces that scores and values are at
-  wq.init(a, c);
-  wp = wq;
-  bool more = wq.next(a), left = wp.next(a);
-  int tq = wq.t0, tp = wp.t0;
-  uint32_t nq = 0, np = 0;  // pages whose scores are complete, whose values are
-  uint32_t half = 0;        // of page nq: the next half of its scores
-  uint32_t piece_q = 0, piece_p = 0;
-  uint32_t idle = 0;
-  uint64_t since = 0;
-  uint32_t idesc_pv = uniform(kIdescPV | (uint32_t((wp.rows(a) + 15) / 16 * 2) << 17));
-  // what this warp does next: nothing, values, the first or second half of scores; | 4 in the odd buffer, | 8 adding up
-  for (;;) {
-    uint32_t turn = left ? 0 : 16;
-    if (np < nq && mbar_test(&c.p_ready[np & 1u], (np >> 1) & 1u) &&
-        (tp > wp.t0 || mbar_test(&c.o_empty, (piece_p & 1u) ^ 1u)))
-      turn = 1 | (np & 1u) << 2 | (tp > wp.t0 ? 8 : 0);
-    else if (more && nq <= np + 1 && mbar_test(&c.full[(nq & 1u) * 2 + half], (nq >> 1) & 1u) &&
-             (half || tq > wq.t0 || mbar_test(&c.q_full, piece_q & 1u)))
-      turn = (2 + half) | (nq & 1u) << 2;
-    turn = uniform(turn);
-    const uint32_t odd = (turn >> 2) & 1u;
-    if ((turn & 3) == 1) {
+  bool dead = false;
+  uint32_t n = 0, pieces = 0;  // pages, pieces
+  Walk<kTile> w;
+  w.init(a, c.plan);
+  while (w.next(a)) {
+    // A (V^T): M-major; N: the rows there are
+    const uint32_t idesc = uniform(kIdesc<T> | (1u << 15) | (uint32_t(128 >> 4) << 24) | (uint32_t((w.rows(a) + 15) / 16 * 2) << 17));
+    for (int t = w.t0; t < w.t1; ++t, ++n) {
+      const uint32_t odd = uniform(n & 1u), later = uniform(t > w.t0);
+      wait_until(
+          [&] {
+            const bool free = t > w.t0 || mbar_test(&c.o_empty, (pieces & 1u) ^ 1u);
+            return free & mbar_test(&c.p_ready[odd], (n >> 1) & 1u);
+          },
+          dead, a.error_flag);
       fence_after();
       const uint32_t p = pd + (odd * kStickTile >> 4), v = vd + (odd * kPairs * kPair >> 4);
 #pragma unroll
       for (int m = 0; m < kPairs; ++m) {
 #pragma unroll
         for (int k = 0; k < kTile / 16; ++k)
-          mma_ss(tmem + col_o(m), v + (m * kPair + k * 2048 >> 4), p + (k * 32 >> 4), idesc_pv, k > 0 ? 1 : turn & 8, go);
+          mma_ss(tmem + col_o(m), v + (m * kPair + k * 2048 >> 4), p + (k * 32 >> 4), idesc, k > 0 ? 1 : later, go);
         if (m & 1) done(&c.empty[odd * 2 + m / 2]);
       }
       done(&c.p_free[odd]);
-      ++np;
-      if (++tp >= wp.t1) {
-        done(&c.o_full);
-        ++piece_p;
-        wp.advance(a);
-        left = wp.next(a);
-        tp = wp.t0;
-        idesc_pv = uniform(kIdescPV | (uint32_t((wp.rows(a) + 15) / 16 * 2) << 17));
-      }
-      idle = 0;
-    } else if ((turn & 3) != 0) {
-      fence_after();
-      const uint32_t s = tmem + col_s(0) + odd * 64, k0 = kd + (odd * kPairs * kPair >> 4);
-      if ((turn & 3) == 2) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          mma_ss(s, qd + ((kSticks - 1) * kStickTile + k * 32 >> 4), rd + (k * 32 >> 4), idesc_qk, k > 0, go);
-        done(&c.rope_empty);
-#pragma unroll
-        for (int k = 0; k < 16; ++k) {
-          const uint32_t off = ((k >> 2) * kStickTile + (k & 3) * 32) >> 4;
-          mma_ss(s, qd + off, k0 + off, idesc_qk, 1, go);
-        }
-        half = 1;
-      } else {
-#pragma unroll
-        for (int k = 16; k < 32; ++k) {
-          const uint32_t off = ((k >> 2) * kStickTile + (k & 3) * 32) >> 4;
-          mma_ss(s, qd + off, k0 + off, idesc_qk, 1, go);
-        }
-        done(&c.s_full[odd]);
-        half = 0;
-        ++nq;
-        if (++tq >= wq.t1) {
-          done(&c.q_empty);
-          ++piece_q;
-          wq.advance(a);
-          more = wq.next(a);
-          tq = wq.t0;
-        }
-      }
-      idle = 0;
-    } else if (turn == 16) {
-      break;
-    } else if ((++idle & 1023u) == 0) {
-      const uint64_t now = global_timer_ns();
-      if (idle == 1024u) since = now;
-      if (__any_sync(0xffffffffu, now - since > kWaitLimitNs)) {
-        if (go && a.error_flag) atomicOr(a.error_flag, B200KV_DEVERR_TIMEOUT);
-        break;
-      }
     }
+    done(&c.o_full);
+    ++pieces;
+    w.advance(a);
   }
   __syncwarp();
 }
@@ -471,60 +494,90 @@ __device__ __forceinline__ float mask_max(uint32_t (&s)[32], uint32_t vis) {
   return fmaxf(t, __uint_as_float(s[31]));
 }
 
-// O's columns times their factors; the four warps call it.
-static __device__ __noinline__ void rescale(const Ctrl &c, uint32_t quad, int rows) {
-  for (int m = 0; m < kPairs; ++m)
-    for (int j0 = 0; j0 < rows; j0 += 32) {
-      uint32_t r[32];
-      tmem_ld32(quad + col_o(m) + j0, r);
+// This warp's part of O, two of the four products, times its columns' factors.
+static __device__ __noinline__ void rescale(const Ctrl &c, uint32_t quad, int half, int rows) {
+#pragma unroll 1
+  for (int m = 2 * half; m < 2 * half + 2; ++m)
+#pragma unroll 1
+    for (int j0 = 0; j0 < rows; j0 += 16) {
+      uint32_t r[16];
+      tmem_ld16(quad + col_o(m) + j0, r);
       wait_ld(r);
 #pragma unroll
-      for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * c.factor[j0 + j]);
-      tmem_st32(quad + col_o(m) + j0, r);
+      for (int j = 0; j < 16; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * c.factor[j0 + j]);
+      tmem_st16(quad + col_o(m) + j0, r);
     }
   wait_st();
 }
 
-// Adds the non-finite elements of the piece's visible nodes to a row that has been
-// written, to its partial sums or its output.
+// Scores of 32 tokens -> weights in 16 bits, as 64 bytes of a row of P (`at`, with the
+// row's swizzle), and their sum.
 template <typename T>
-__device__ __noinline__ void repair_row(const Args &a, const Seq &s, int b, int node, int from, int to, float *part, T *out) {
-  for (int p = max(from, s.ctx); p < min(to, s.ctx + s.nodes); ++p) {
-    if (!(visible32(a, s, node, p) & 1u)) continue;
-    const int id = __ldg(a.block_table + static_cast<int64_t>(b) * a.bt_stride + p / kPageTokens);
-    if (id < 0 || id >= a.num_blocks) continue;
-    const T *page = static_cast<const T *>(a.pool) + static_cast<int64_t>(id) * kRow * kPageTokens;
-    for (int d = 0; d < kRank; ++d) {
-      const float v = to_float(page[(d / 64 * kPageTokens + p % kPageTokens) * 64 + d % 64]);
-      if (fabsf(v) < CUDART_INF_F) continue;
-      if (part)
-        part[d] += v;
-      else
-        from_float(out[d], to_float(out[d]) + v);
+__device__ __forceinline__ float put_weights(const uint32_t (&s)[32], float cl, float m, uint8_t *at, int chunk, int swizzle,
+                                             bool store) {
+  const float minus = m == -CUDART_INF_F ? 0.f : -m;
+  float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    uint32_t p[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 x = make_float2(__uint_as_float(s[8 * k + 2 * j]), __uint_as_float(s[8 * k + 2 * j + 1]));
+      const float2 y = fma2(x, make_float2(cl, cl), make_float2(minus, minus));
+      const float2 e = make_float2(ex2(y.x), ex2(y.y));
+      sum[j & 1] = add2(sum[j & 1], e);
+      p[j] = pack2(e.x, e.y, T());
     }
+    if (store) *reinterpret_cast<uint4 *>(at + (((chunk + k) ^ swizzle) << 4)) = make_uint4(p[0], p[1], p[2], p[3]);
   }
+  const float2 x = add2(sum[0], sum[1]);
+  return x.x + x.y;
+}
+
+// Rows of some of a page's sticks in shared memory: those from `end` on, past
+// the sequence's end, hold anything and become zeros, so that weights of zero meet
+// finite values; so do non-finite elements from `from` on, of nodes that not every row
+// sees (a row that sees such a node has its score, which is not finite either: NaN
+// everywhere, or no weight for it).  128 threads, 16 bytes each: row 16 k + tid / 8.
+template <typename T, int kOf>  // sticks
+__device__ __noinline__ void clean(uint8_t *half, int tid, int from, int end) {
+#pragma unroll 1
+  for (int st = 0; st < kOf; ++st)
+#pragma unroll 1
+    for (int k = min(from, max(end, 0)) / 16; k < 4; ++k) {
+      uint4 *cell = reinterpret_cast<uint4 *>(half + st * kStickTile + k * 2048 + tid * 16);
+      const int row = 16 * k + (tid >> 3);
+      if (row >= end) {
+        *cell = make_uint4(0, 0, 0, 0);
+      } else if (row >= from) {
+        uint4 x = *cell;
+        if (!any_non_finite<T>(x)) continue;
+        drop_non_finite<T>(x);
+        *cell = x;
+      }
+    }
 }
 
 // Softmax of the CTA's rows, and their output.
 template <typename T>
 __device__ __forceinline__ void softmax(const Args &a, Ctrl &c, uint8_t *smem, uint32_t tmem) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int row = 16 * warp + (lane & 15);
+  const int half = warp >> 2, row = 16 * (warp & 3) + (lane & 15);
   const bool has_row = lane < 16;
-  const uint32_t quad = tmem + (uint32_t(warp * 32) << 16);
-  const int part = static_cast<int>(blockIdx.x) % a.parts;
+  const uint32_t quad = tmem + (uint32_t((warp & 3) * 32) << 16);
+  const int head0 = static_cast<int>(blockIdx.x) % a.stride * a.head_box;
   // (a scale of zero: too small to move a score, and -inf stays -inf)
   const float cl = fmaxf(fabsf(a.scale) * 1.44269504088896341f, 1e-37f);
   bool dead = false;
   uint32_t n = 0;  // pages
   unsigned piece = 0;
-  Walk wk;
-  wk.init(a, c);
+  Walk<kTile> wk;
+  wk.init(a, c.plan);
   while (wk.next(a)) {
     ++piece;
     const int len = wk.s.ctx + wk.s.nodes, rows = wk.rows(a);
     const int node = wk.block * a.tile_nodes + row / a.head_box;
-    const int head = part * a.head_box + row % a.head_box;
+    const int head = head0 + row % a.head_box;
     const bool live = has_row && row < rows && head < a.heads;
     const bool warp_live = __any_sync(0xffffffffu, live);
     // tokens before this one are seen by every row of the tile
@@ -533,89 +586,42 @@ __device__ __forceinline__ void softmax(const Args &a, Ctrl &c, uint8_t *smem, u
     for (int t = wk.t0; t < wk.t1; ++t, ++n) {
       const int pos = t * kTile;
       const bool first = t == wk.t0, tail = pos + kTile > common;
-      uint32_t vis[2] = {~0u, ~0u};
-      if (tail && live) {
-        vis[0] = visible32(a, wk.s, node, pos);
-        vis[1] = visible32(a, wk.s, node, pos + 32);
-      }
+      const uint32_t vis = tail && live ? visible32(a, wk.s, node, pos + 32 * half) : ~0u;
       wait(&c.s_full[n & 1], (n >> 1) & 1u, dead, a.error_flag);
       fence_after();
-      uint32_t s[2][32];
+      uint32_t s[32];
       float mt = -CUDART_INF_F;
       if (warp_live) {
-        tmem_ld32(quad + col_s(n & 1), s[0]);
-        tmem_ld32(quad + col_s(n & 1) + 32, s[1]);
-        wait_ld(s[0]);
-        wait_ld(s[1]);
-        if (tail)
-          mt = fmaxf(mask_max<true>(s[0], vis[0]), mask_max<true>(s[1], vis[1])) * cl;
-        else
-          mt = fmaxf(mask_max<false>(s[0], ~0u), mask_max<false>(s[1], ~0u)) * cl;
+        tmem_ld32(quad + col_s(n & 1) + 32 * half, s);
+        wait_ld(s);
+        mt = (tail ? mask_max<true>(s, vis) : mask_max<false>(s, ~0u)) * cl;
       }
-      const bool rise = live && mt > m + (first ? 0.f : kLazyLog2);
-      if (!first && any_softmax(rise)) {
-        // O moves to the new maxima once the values before are in it
-        const float keep = rise ? ex2(m - mt) : 1.f;
-        l *= keep;
-        if (has_row) c.factor[row] = keep;
-        wait(&c.p_free[(n - 1) & 1], ((n - 1) >> 1) & 1u, dead, a.error_flag);
-        fence_after();
+      // the maximum is that of both halves of the row; it moves when either has risen far enough
+      if (first || any_softmax(live && mt > m + kLazyLog2)) {
+        if (has_row) c.top[half][row] = mt;
         bar_softmax();
-        rescale(c, quad, rows);
-        bar_softmax();
+        mt = fmaxf(mt, c.top[half ^ 1][row]);
+        const bool rise = live && mt > m + (first ? 0.f : kLazyLog2);
+        if (!first) {
+          // O moves to the new maxima once the values before are in it
+          const float keep = rise ? ex2(m - mt) : 1.f;
+          l *= keep;
+          if (has_row && half == 0) c.factor[row] = keep;
+          wait(&c.p_free[(n - 1) & 1], ((n - 1) >> 1) & 1u, dead, a.error_flag);
+          fence_after();
+          bar_softmax();
+          rescale(c, quad, half, rows);
+        }
+        if (rise) m = mt;
+        bar_softmax();  // (maxima and factors are read)
       }
-      if (rise) m = mt;
       // P's buffer is free once the values of two pages before are in O
       if (n >= 2) wait(&c.p_free[n & 1], ((n - 2) >> 1) & 1u, dead, a.error_flag);
-      if (warp_live) {
-        const float minus = m == -CUDART_INF_F ? 0.f : -m;
-        float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-        uint8_t *at = smem + kOffP + (n & 1) * kStickTile + row * 128;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          uint32_t p[16];
-#pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const float2 x = make_float2(__uint_as_float(s[i][2 * j]), __uint_as_float(s[i][2 * j + 1]));
-            const float2 y = fma2(x, make_float2(cl, cl), make_float2(minus, minus));
-            const float2 e = make_float2(ex2(y.x), ex2(y.y));
-            sum[j & 1] = add2(sum[j & 1], e);
-            p[j] = pack2(e.x, e.y, T());
-          }
-          if (has_row) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              *reinterpret_cast<uint4 *>(at + (((4 * i + k) ^ (row & 7)) << 4)) =
-                  make_uint4(p[4 * k], p[4 * k + 1], p[4 * k + 2], p[4 * k + 3]);
-          }
-        }
-        const float2 x = add2(sum[0], sum[1]);
-        l += x.x + x.y;
-      }
+      if (warp_live)
+        l += put_weights<T>(s, cl, m, smem + kOffP + (n & 1) * kStickTile + row * 128, 4 * half, row & 7, has_row);
       if (pos + kTile > min(common, len)) {
-        // the pool's rows past the sequence's end hold anything and become zeros, so that
-        // weights of zero meet finite values; so do non-finite elements of nodes that not
-        // every row sees (repair_row)
-        const int from = max(common - pos, 0), end = len - pos;
-        for (int j = 0; j < kPairs; ++j) {
-          if ((j & 1) == 0) wait(&c.full[(n & 1) * 2 + j / 2], (n >> 1) & 1u, dead, a.error_flag);
-          uint8_t *v = smem + kOffSlots + ((n & 1) * kPairs + j) * kPair + tid * 16;
-#pragma unroll 1
-          for (int k = min(from, end) / 16; k < 4; ++k)
-            for (int st = 0; st < 2; ++st) {
-              uint4 *cell = reinterpret_cast<uint4 *>(v + st * kStickTile + k * 2048);
-              const int vrow = 16 * k + (tid >> 3);
-              if (vrow >= end) {
-                *cell = make_uint4(0, 0, 0, 0);
-              } else if (vrow >= from) {
-                uint4 x = *cell;
-                if (!any_non_finite<T>(x)) continue;
-                atomicMax(&c.bad_piece, piece);
-                drop_non_finite<T>(x);
-                *cell = x;
-              }
-            }
-        }
+        wait(&c.full[(n & 1) * 2 + half], (n >> 1) & 1u, dead, a.error_flag);
+        clean<T, 4>(smem + kOffSlots + ((n & 1) * 2 + half) * 2 * kPair, tid & 127, max(common - pos, 0), len - pos);
       }
       fence_async_smem();
       fence_before();
@@ -627,7 +633,10 @@ __device__ __forceinline__ void softmax(const Args &a, Ctrl &c, uint8_t *smem, u
     const bool split = wk.t0 > 0 || wk.t1 < wk.tiles;
     const int64_t pslot = 2 * blockIdx.x + (wk.t0 > 0 ? 0 : 1);  // one of each kind per share
     const int64_t orow = static_cast<int64_t>(wk.s.q0 + node) * a.heads + head;
-    if (has_row) {
+    if (has_row) c.top[half][row] = l;
+    bar_softmax();
+    if (has_row && half == 0) {
+      l = c.top[0][row] + c.top[1][row];
       c.factor[row] = split ? 1.f : (l == 0.f ? 0.f : 1.f / l);
       c.row_at[row] = live ? static_cast<int>(orow) : -1;
       if (live && split)
@@ -638,52 +647,51 @@ __device__ __forceinline__ void softmax(const Args &a, Ctrl &c, uint8_t *smem, u
     bar_softmax();
     wait(&c.o_full, (piece - 1) & 1u, dead, a.error_flag);
     fence_after();
-    for (int mblock = 0; mblock < kPairs; ++mblock)
 #pragma unroll 1
-      for (int j0 = 0; j0 < rows; j0 += 32) {
-        const int d = 128 * mblock + 32 * warp + lane;  // this lane's latent element
-        uint32_t r[32];
-        tmem_ld32(quad + col_o(mblock) + j0, r);
-        wait_ld(r);
-        if (split) {
-          float *to = a.part_o + (pslot * kTileRows + j0) * kRank + d;
+    for (int x = 0; x < 4; ++x) {
+      const int mblock = 2 * half + (x >> 1), j0 = (x & 1) * 32;
+      if (j0 >= rows) continue;
+      const int d = 128 * mblock + 32 * (warp & 3) + lane;  // this lane's latent element
+      uint32_t r[32];
+      tmem_ld32(quad + col_o(mblock) + j0, r);
+      wait_ld(r);
+      if (split) {
+        float *to = a.part_o + (pslot * kTileRows + j0) * kRank + d;
 #pragma unroll
-          for (int j = 0; j < 32; ++j)
-            if (c.row_at[j0 + j] >= 0) to[j * kRank] = __uint_as_float(r[j]);
-        } else {
-          // lanes in pairs: two neighbouring elements of every other row each
-          T *out = static_cast<T *>(a.out) + (d & ~1);
+        for (int j = 0; j < 32; ++j)
+          if (c.row_at[j0 + j] >= 0) to[j * kRank] = __uint_as_float(r[j]);
+      } else {
+        // lanes in pairs: two neighbouring elements of every other row each
+        T *out = static_cast<T *>(a.out) + (d & ~1);
 #pragma unroll
-          for (int j = 0; j < 32; j += 2) {
-            float x[2];
+        for (int j = 0; j < 32; j += 2) {
+          float y[2];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const float f = c.factor[j0 + j + i];
-              x[i] = f == 0.f ? 0.f : __uint_as_float(r[j + i]) * f;
-            }
-            const float other = __shfl_xor_sync(0xffffffffu, lane & 1 ? x[0] : x[1], 1);
-            const int to = c.row_at[j0 + j + (lane & 1)];
-            const uint32_t two = lane & 1 ? pack2(other, x[1], T()) : pack2(x[0], other, T());
-            if (to >= 0) *reinterpret_cast<uint32_t *>(out + static_cast<int64_t>(to) * kRank) = two;
+          for (int i = 0; i < 2; ++i) {
+            const float f = c.factor[j0 + j + i];
+            y[i] = f == 0.f ? 0.f : __uint_as_float(r[j + i]) * f;
           }
+          const float other = __shfl_xor_sync(0xffffffffu, lane & 1 ? y[0] : y[1], 1);
+          const int to = c.row_at[j0 + j + (lane & 1)];
+          const uint32_t two = lane & 1 ? pack2(other, y[1], T()) : pack2(y[0], other, T());
+          if (to >= 0) *reinterpret_cast<uint32_t *>(out + static_cast<int64_t>(to) * kRank) = two;
         }
       }
+    }
     fence_before();
     bar_softmax();  // (the factors and rows are read)
     if (lane == 0) arrive(&c.o_empty);
-    if (live && *reinterpret_cast<volatile unsigned *>(&c.bad_piece) >= piece)
-      repair_row<T>(a, wk.s, wk.b, node, wk.t0 * kTile, wk.t1 * kTile,
-                    split ? a.part_o + (pslot * kTileRows + row) * kRank : nullptr, static_cast<T *>(a.out) + orow * kRank);
     // the second share of a split block describes it to the join
     if (wk.t0 > 0 && tid == 0) {
-      const int first = wk.share_of(0, c.per), share = static_cast<int>(blockIdx.x) / a.parts;
+      const int first = wk.share_of(0, c.plan.per), share = static_cast<int>(blockIdx.x) / a.stride;
       if (share == first + 1) {
         Join j;
         j.rows0 = wk.s.q0;
         j.node0 = wk.block * a.tile_nodes;
         j.nodes = min(wk.s.nodes - j.node0, a.tile_nodes);
+        j.head0 = head0;
         j.first = first;
-        j.last = wk.share_of(wk.tiles - 1, c.per);
+        j.last = wk.share_of(wk.tiles - 1, c.plan.per);
         a.joins[blockIdx.x] = j;
       }
     }
@@ -713,15 +721,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(&c.q_empty, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&c.s_full[i], 1);
-      mbar_init(&c.p_ready[i], 4);
+      mbar_init(&c.p_ready[i], kSoftmaxWarps);
       mbar_init(&c.p_free[i], 1);
     }
     mbar_init(&c.o_full, 1);
-    mbar_init(&c.o_empty, 4);
+    mbar_init(&c.o_empty, kSoftmaxWarps);
     fence_mbar_init();
-    c.bad_piece = 0;
   }
-  if (warp == 5) {
+  if (warp == 9) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&c.tmem)),
                  "r"(kTmemCols)
                  : "memory");
@@ -730,20 +737,22 @@ __global__ void __launch_bounds__(kThreads, 1)
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (tid == 0) a.joins[blockIdx.x].nodes = 0;  // no block begins to be split here, unless the epilogue says so
-  make_plan<T>(a, c);
+  make_plan<T, kTile>(a, c.plan);
   fence_before();
   __syncthreads();
   fence_after();
   const uint32_t tmem = c.tmem;
-  if (warp < 4)
+  if (warp < kSoftmaxWarps)
     softmax<T>(a, c, smem, tmem);
-  else if (warp == 4)
+  else if (warp == 8)
     producer(a, c, smem, &qm, &rm, &pm, &sm);
-  else
-    mma_issuer<T>(a, c, smem, tmem);
+  else if (warp == 9)
+    score_issuer<T>(a, c, smem, tmem);
+  else if (warp == 10)
+    value_issuer<T>(a, c, smem, tmem);
   fence_before();
   __syncthreads();
-  if (warp == 5) {
+  if (warp == 9) {
     fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
   }
@@ -758,15 +767,15 @@ __global__ void __launch_bounds__(256) latent_join_kernel(const __grid_constant_
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const Join j = a.joins[blockIdx.x];
   const int row = blockIdx.y * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  const int part = static_cast<int>(blockIdx.x) % a.parts;
-  const int node = row / a.head_box, head = part * a.head_box + row % a.head_box;
+  const int part = static_cast<int>(blockIdx.x) % a.stride;
+  const int node = row / a.head_box, head = j.head0 + row % a.head_box;
   if (node >= j.nodes || head >= a.heads) return;
   float M = -CUDART_INF_F, l = 0.f;
   float4 o[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int x = j.first; x <= j.last; ++x) {
-    const int64_t slot = 2 * (x * a.parts + part) + (x == j.first ? 1 : 0);
+    const int64_t slot = 2 * (x * a.stride + part) + (x == j.first ? 1 : 0);
     const float2 ml = a.part_ml[slot * kTileRows + row];
     const float4 *v = reinterpret_cast<const float4 *>(a.part_o + (slot * kTileRows + row) * kRank) + lane;
     float4 p[4];
@@ -793,37 +802,6 @@ __global__ void __launch_bounds__(256) latent_join_kernel(const __grid_constant_
     *reinterpret_cast<uint2 *>(out + 128 * i) = make_uint2(lo, hi);
   }
   if (lane == 0 && a.lse) a.lse[orow] = l == 0.f ? -CUDART_INF_F : (M + log2f(l)) * 0.69314718055994530942f;
-}
-
-// ----------------------------------------------------------------- launch --
-template <typename T>
-int launch(const CUtensorMap &qm, const CUtensorMap &rm, const CUtensorMap &pm, const CUtensorMap &sm, const Args &a,
-           int ctas, cudaStream_t stream) {
-  static int configured[64] = {0};
-  int dev = 0;
-  B200KV_CUDA_TRY(cudaGetDevice(&dev));
-  if (dev < 0 || dev >= 64) return set_error(B200KV_ERR_UNSUPPORTED, "device ordinal %d", dev);
-  if (!__atomic_load_n(&configured[dev], __ATOMIC_ACQUIRE)) {
-    B200KV_CUDA_TRY(cudaFuncSetAttribute(latent_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
-    __atomic_store_n(&configured[dev], 1, __ATOMIC_RELEASE);
-  }
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(ctas));
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = kSmem;
-  cfg.stream = stream;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  B200KV_CUDA_TRY(cudaLaunchKernelEx(&cfg, latent_kernel<T>, qm, rm, pm, sm, a));
-  const int rows = a.box_nodes * a.head_box;
-  cfg.gridDim = dim3(static_cast<unsigned>(ctas), static_cast<unsigned>((rows + 7) / 8));
-  cfg.blockDim = dim3(256);
-  cfg.dynamicSmemBytes = 0;
-  B200KV_CUDA_TRY(cudaLaunchKernelEx(&cfg, latent_join_kernel<T>, a));
-  return B200KV_OK;
 }
 
 }  // namespace latent

@@ -1,0 +1,575 @@
+// Latent attention for blocks of up to 128 rows, on pairs of SMs (latent_mma.cuh
+// has what the two kernels share, and the one for up to 64 rows).
+//
+// With 64 rows on one SM the products are bound by shared memory: a page's scores
+// and values read 4 + 6 KB of operands where the tensor core needs half the time
+// for them.  So two CTAs of a cluster work as one (cta_group::2): each holds 64 of
+// the 128 rows and gives half of every product's other operand,
+//   S [128 rows, 128 tokens]  = Q K^T    each CTA one of two pages: its own tokens
+//   O [128 rows, 512]        += P V      each CTA half of the latent elements
+// at 32 and 64 clocks a product of 16, 2176 for 128 tokens, where its own operands
+// take 4 and 6 KB.  (One SM with 64 rows: 3800 clocks for 128 tokens.)
+//
+// A step's keys are read as they arrive, a pair of sticks at a time, and their slots
+// freed at once; its values, half of the elements of both pages, come again (out of
+// L2) when the weights are there.  So seven slots of 16 KB keep the products fed.
+//
+// An accumulator of 128 rows over two CTAs lies in each of them as 64 rows: lanes 0-63
+// have the first half of the columns, lanes 64-127 the second.  Warp w has the lanes of
+// quadrant w % 4, so rows 32 (w % 2) .. and half (w / 2) % 2 of a step's tokens and of
+// O's columns, and of those columns the first or second part by w / 4.
+//
+// Warps: 0-7 softmax and output, 8 TMA producer; in the first CTA 9 issues the scores'
+// MMAs for both, 10 the values'; in the second 11 tells the first of its arrivals.
+#pragma once
+
+#include "latent_mma.cuh"
+
+namespace b200kv {
+namespace latent {
+namespace pair {
+
+constexpr int kStep = 2 * kPageTokens;  // tokens of a step
+constexpr int kSlots = 7, kSlot = kPair;
+constexpr int kOffQ = 3072;
+constexpr int kOffP = kOffQ + kSticks * kStickTile;  // [2][2 pages][64 rows][64 tokens]
+constexpr int kOffRope = kOffP + 4 * kStickTile;
+constexpr int kOffSlots = kOffRope + kStickTile;
+constexpr int kSmem = kOffSlots + kSlots * kSlot;
+static_assert(kSmem <= 227 * 1024, "shared memory per CTA");
+
+// TMEM columns of a CTA: O, 128 for each 256 latent elements, and two score buffers
+__device__ __forceinline__ uint32_t col_o(int j) { return uint32_t(j) * 128u; }
+__device__ __forceinline__ uint32_t col_s(uint32_t b) { return 256u + b * 64u; }
+
+struct Ctrl {
+  // each CTA's own: what has arrived, what is free again, what is computed
+  uint64_t full[kSlots], empty[kSlots], rope_full, rope_empty, q_full, q_empty;
+  uint64_t s_full[2], p_free[2], o_full;
+  // the first CTA's: the second's arrivals, and both CTAs' weights and outputs
+  uint64_t peer[kSlots], rope_peer, q_peer, p_ready[2], o_empty;
+  uint32_t tmem;
+  Plan plan;
+  float top[4][kTileRows];  // maxima, then sums, of the quarters of a row's tokens
+};
+static_assert(sizeof(Ctrl) <= kOffQ, "control block");
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+}
+// An arrival at the first CTA's barrier.  What it tells of lies in shared memory, written
+// by the copy engine or behind fence.proxy.async, and is read by the tensor cores: the
+// order of shared memory that arrival and wait give is enough.  (A release and an
+// acquire of the cluster's scope order global memory too, and cost 1000 to 2000 clocks each.)
+__device__ __forceinline__ void arrive_first(uint64_t *bar) {
+  asm volatile(
+      "{\n\t.reg .b32 r;\n\tmapa.shared::cluster.u32 r, %0, 0;\n\tmbarrier.arrive.shared::cluster.b64 _, [r];\n\t}" ::"r"(
+          smem_u32(bar))
+      : "memory");
+}
+__device__ __forceinline__ void commit_both(uint64_t *bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)),
+      "h"(static_cast<uint16_t>(3))
+      : "memory");
+}
+__device__ __forceinline__ void mma_pair(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc, uint32_t go) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\t.reg .b64 a, b;\n\tsetp.ne.b32 p, %5, 0;\n\tsetp.ne.b32 e, %6, 0;\n\t"
+      "mov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\t"
+      "@e tcgen05.mma.cta_group::2.kind::f16 [%0], a, b, %4, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(kDescHi), "r"(idesc), "r"(acc), "r"(go)
+      : "memory");
+}
+
+// The rows of a CTA in the pair's block: nodes from node0 on, heads from head0 on.
+struct Rows {
+  int node0, nodes, head0;
+};
+__device__ __forceinline__ Rows rows_of(const Args &a, const Walk<kStep> &w) {
+  const int part = static_cast<int>(blockIdx.x) % a.stride;
+  Rows r;
+  if (a.heads > kTileRows) {  // a node's heads over the CTAs of the share
+    r.node0 = w.block;
+    r.head0 = part * kTileRows;
+  } else {
+    r.node0 = w.block * a.block_nodes + part * a.tile_nodes;
+    r.head0 = 0;
+  }
+  r.nodes = min(max(w.s.nodes - r.node0, 0), a.tile_nodes);
+  return r;
+}
+
+// The order of a piece's arrivals, which producer and relay share: the
+// rotary stick and four pairs of the keys of step t, one step ahead of the four parts
+// of the values.
+template <typename Keys, typename Values>
+__device__ __forceinline__ void in_order(const Walk<kStep> &w, Keys keys, Values values) {
+  keys(w.t0);
+  for (int t = w.t0; t < w.t1; ++t) {
+    if (t + 1 < w.t1) keys(t + 1);
+    values(t);
+  }
+}
+
+__device__ __forceinline__ void producer(const Args &a, Ctrl &c, uint8_t *smem, const CUtensorMap *qm,
+                                         const CUtensorMap *rm, const CUtensorMap *pm, const CUtensorMap *sm) {
+  const int lane = threadIdx.x & 31;
+  const int rank = static_cast<int>(cluster_rank());
+  const uint32_t q_bytes = static_cast<uint32_t>(a.box_nodes * a.head_box * 128);
+  bool dead = false;
+  uint32_t slots = 0, steps = 0, pieces = 0;  // issued
+  Walk<kStep> w;
+  w.init(a, c.plan);
+  while (!dead && w.next(a)) {
+    const int pages = (w.s.ctx + w.s.nodes + kPageTokens - 1) / kPageTokens;
+    int window = w.t0 / 16, ids = load_ids(a, w.b, window, pages), ids_next = load_ids(a, w.b, window + 1, pages);
+    int ids_before = ids;
+    wait(&c.q_empty, (pieces & 1u) ^ 1u, dead, a.error_flag);
+    if ((dead = __any_sync(0xffffffffu, dead))) break;
+    const Rows rows = rows_of(a, w);
+    if (lane == 0) mbar_arrive_expect_tx(&c.q_full, kSticks * q_bytes);
+    __syncwarp();
+    if (lane < kSticks)
+      tma_3d(smem + kOffQ + lane * kStickTile, lane < kSticks - 1 ? qm : rm, &c.q_full, lane < kSticks - 1 ? lane * 64 : 0,
+             rows.head0, w.s.q0 + rows.node0);
+    ++pieces;
+    // an invalid id, and a page past the sequence's, reads past the last page: zeros
+    auto page_of = [&](int have, int p) {
+      const int id = __shfl_sync(0xffffffffu, have, p & 31);
+      return id < 0 ? a.num_blocks : id;
+    };
+    auto load = [&](int row, int page) {
+      if (dead) return;
+      const uint32_t s = slots % kSlots;
+      wait(&c.empty[s], ((slots / kSlots) & 1u) ^ 1u, dead, a.error_flag);
+      if ((dead = __any_sync(0xffffffffu, dead))) return;
+      if (lane == 0) {
+        mbar_arrive_expect_tx(&c.full[s], kSlot);
+        tma_3d(smem + kOffSlots + s * kSlot, pm, &c.full[s], 0, row, page);
+      }
+      __syncwarp();
+      ++slots;
+    };
+    in_order(
+        w,
+        [&](int t) {
+          if (dead) return;
+          if (t / 16 > window) {  // keys lead, values follow by a step
+            ids_before = ids;
+            ids = ids_next;
+            ids_next = load_ids(a, w.b, ++window + 1, pages);
+          }
+          const int page = page_of(ids, 2 * t + rank);
+          wait(&c.rope_empty, (steps & 1u) ^ 1u, dead, a.error_flag);
+          if ((dead = __any_sync(0xffffffffu, dead))) return;
+          if (lane == 0) {
+            mbar_arrive_expect_tx(&c.rope_full, kStickTile);
+            tma_3d(smem + kOffRope, sm, &c.rope_full, 0, (kSticks - 1) * kTile, page);
+          }
+          __syncwarp();
+          ++steps;
+          for (int j = 0; j < kPairs; ++j) load(j * 2 * kTile, page);
+        },
+        [&](int t) {
+          const int have = t / 16 == window ? ids : ids_before;
+          const int page[2] = {page_of(have, 2 * t), page_of(have, 2 * t + 1)};
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int p = 0; p < 2; ++p) load((4 * j + 2 * rank) * kTile, page[p]);
+        });
+    w.advance(a);
+  }
+  if (dead) {  // the copies under way, with a limit
+    bool late = false;
+    if (pieces > 0) wait(&c.q_full, (pieces - 1) & 1u, late, a.error_flag);
+    if (steps > 0) wait(&c.rope_full, (steps - 1) & 1u, late, a.error_flag);
+    for (uint32_t n = slots - min(slots, uint32_t(kSlots)); n < slots; ++n)
+      wait(&c.full[n % kSlots], (n / kSlots) & 1u, late, a.error_flag);
+  }
+  // the last arrival that the MMAs owe this CTA: not before it may the CTA end
+  if (lane == 0 && pieces > 0) {
+    bool late = false;
+    wait(&c.q_empty, (pieces & 1u) ^ 1u, late, a.error_flag);
+  }
+  __syncwarp();
+}
+
+// The second CTA's arrivals, told to the first.
+__device__ __forceinline__ void relay(const Args &a, Ctrl &c) {
+  bool dead = false;
+  uint32_t slots = 0, steps = 0, pieces = 0;
+  Walk<kStep> w;
+  w.init(a, c.plan);
+  while (!dead && w.next(a)) {
+    wait(&c.q_full, pieces++ & 1u, dead, a.error_flag);
+    if (!dead) arrive_first(&c.q_peer);
+    auto slot = [&] {
+      wait(&c.full[slots % kSlots], (slots / kSlots) & 1u, dead, a.error_flag);
+      if (!dead) arrive_first(&c.peer[slots % kSlots]);
+      ++slots;
+    };
+    in_order(
+        w,
+        [&](int) {
+          wait(&c.rope_full, steps++ & 1u, dead, a.error_flag);
+          if (!dead) arrive_first(&c.rope_peer);
+          for (int j = 0; j < kPairs; ++j) slot();
+        },
+        [&](int) {
+          for (int j = 0; j < kPairs; ++j) slot();
+        });
+    w.advance(a);
+  }
+}
+
+// The two MMA warps of the first CTA, converged, issue for both CTAs from an elected lane.
+template <typename T>
+__device__ __forceinline__ void score_issuer(const Args &a, Ctrl &c, uint8_t *smem, uint32_t tmem_any) {
+  const uint32_t go = elect_one(), tmem = uniform(tmem_any);
+  const uint32_t idesc = kIdesc<T> | (uint32_t(128 >> 4) << 24) | (uint32_t(kStep >> 3) << 17) |
+                         (a.scale < 0.f ? 1u << 13 : 0u);  // a negative scale turns Q's sign
+  const uint32_t qd = desc_kmajor(smem_u32(smem + kOffQ)), rd = desc_kmajor(smem_u32(smem + kOffRope));
+  const uint32_t kd = desc_kmajor(smem_u32(smem + kOffSlots));
+  auto done = [&](uint64_t *bar) {
+    if (go) commit_both(bar);
+  };
+  bool dead = false;
+  uint32_t slots = 0, n = 0, pieces = 0;  // slots of the pieces before; steps; pieces
+  Walk<kStep> w;
+  w.init(a, c.plan);
+  while (w.next(a)) {
+    const int steps = w.t1 - w.t0;
+    for (int i = 0; i < steps; ++i, ++n) {
+      const uint32_t odd = uniform(n & 1u), at = slots + kPairs * (i + max(i - 1, 0));
+      const uint32_t s = tmem + col_s(0) + odd * 64;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t at0 = uniform((at + 2 * h) % kSlots), at1 = uniform((at + 2 * h + 1) % kSlots);
+        const uint32_t par0 = (at + 2 * h) / kSlots & 1u, par1 = (at + 2 * h + 1) / kSlots & 1u;
+        wait_until(
+            [&] {
+              bool ok = mbar_test(&c.full[at0], par0) & mbar_test(&c.peer[at0], par0) & mbar_test(&c.full[at1], par1) &
+                        mbar_test(&c.peer[at1], par1);
+              if (h == 0) {
+                // this score buffer is free once the step before last has weights
+                ok = ok & mbar_test(&c.rope_full, n & 1u) & mbar_test(&c.rope_peer, n & 1u);
+                if (n >= 2) ok = ok & mbar_test(&c.p_ready[odd], ((n - 2) >> 1) & 1u);
+                if (i == 0) ok = ok & mbar_test(&c.q_full, pieces & 1u) & mbar_test(&c.q_peer, pieces & 1u);
+              }
+              return ok;
+            },
+            dead, a.error_flag);
+        fence_after();
+        if (h == 0) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            mma_pair(s, qd + ((kSticks - 1) * kStickTile + k * 32 >> 4), rd + (k * 32 >> 4), idesc, k > 0, go);
+          done(&c.rope_empty);
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const uint32_t k0 = kd + ((j ? at1 : at0) * kSlot >> 4);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const uint32_t off = ((k >> 2) * kStickTile + (k & 3) * 32) >> 4;
+            mma_pair(s, qd + ((2 * h + j) * kPair >> 4) + off, k0 + off, idesc, 1, go);
+          }
+          done(&c.empty[j ? at1 : at0]);
+        }
+      }
+      done(&c.s_full[odd]);
+    }
+    done(&c.q_empty);
+    slots += 2 * kPairs * steps;
+    ++pieces;
+    w.advance(a);
+  }
+  __syncwarp();
+}
+
+template <typename T>
+__device__ __forceinline__ void value_issuer(const Args &a, Ctrl &c, uint8_t *smem, uint32_t tmem_any) {
+  constexpr uint32_t idesc = kIdesc<T> | (uint32_t(128 >> 4) << 24) | (1u << 16) | (uint32_t(256 >> 3) << 17);  // V: N-major
+  const uint32_t go = elect_one(), tmem = uniform(tmem_any);
+  const uint32_t pd = desc_kmajor(smem_u32(smem + kOffP));
+  const uint32_t vd = (smem_u32(smem + kOffSlots) >> 4) | (uint32_t(kStickTile >> 4) << 16);
+  auto done = [&](uint64_t *bar) {
+    if (go) commit_both(bar);
+  };
+  bool dead = false;
+  uint32_t slots = 0, n = 0, pieces = 0;
+  Walk<kStep> w;
+  w.init(a, c.plan);
+  while (w.next(a)) {
+    const int steps = w.t1 - w.t0;
+    for (int i = 0; i < steps; ++i, ++n) {
+      const uint32_t odd = uniform(n & 1u), later = uniform(i > 0);
+      const uint32_t at = slots + kPairs * (min(steps, i + 2) + i);
+      const uint32_t p0 = pd + (odd * 2 * kStickTile >> 4);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const uint32_t at0 = uniform((at + 2 * j) % kSlots), at1 = uniform((at + 2 * j + 1) % kSlots);
+        const uint32_t par0 = (at + 2 * j) / kSlots & 1u, par1 = (at + 2 * j + 1) / kSlots & 1u;
+        wait_until(
+            [&] {
+              bool ok = mbar_test(&c.full[at0], par0) & mbar_test(&c.peer[at0], par0) & mbar_test(&c.full[at1], par1) &
+                        mbar_test(&c.peer[at1], par1);
+              if (j == 0) {
+                ok = ok & mbar_test(&c.p_ready[odd], (n >> 1) & 1u);
+                if (i == 0) ok = ok & mbar_test(&c.o_empty, (pieces & 1u) ^ 1u);
+              }
+              return ok;
+            },
+            dead, a.error_flag);
+        fence_after();
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+          const uint32_t v = vd + ((p ? at1 : at0) * kSlot >> 4);
+#pragma unroll
+          for (int k = 0; k < kTile / 16; ++k)
+            mma_pair(tmem + col_o(j), p0 + (p * kStickTile + k * 32 >> 4), v + (k * 2048 >> 4), idesc, p + k > 0 ? 1 : later,
+                     go);
+          done(&c.empty[p ? at1 : at0]);
+        }
+      }
+      done(&c.p_free[odd]);
+    }
+    done(&c.o_full);
+    slots += 2 * kPairs * steps;
+    ++pieces;
+    w.advance(a);
+  }
+  __syncwarp();
+}
+
+// This thread's columns of O, of its row, times `keep`.
+static __device__ __noinline__ void rescale(uint32_t at, float keep) {
+#pragma unroll 1
+  for (int i = 0; i < 128; i += 16) {
+    uint32_t r[16];
+    tmem_ld16(at + i, r);
+    wait_ld(r);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * keep);
+    tmem_st16(at + i, r);
+  }
+  wait_st();
+}
+
+// Softmax of the CTA's rows, and their output.
+template <typename T>
+__device__ __forceinline__ void softmax(const Args &a, Ctrl &c, uint8_t *smem, uint32_t tmem) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int row = tid & 63, half = (warp >> 1) & 1, part = warp >> 2;  // of the tokens: page `half`, 32 tokens `part`
+  const int quarter = 2 * half + part;
+  const uint32_t quad = tmem + (uint32_t((warp & 3) * 32) << 16);
+  // (a scale of zero: too small to move a score, and -inf stays -inf)
+  const float cl = fmaxf(fabsf(a.scale) * 1.44269504088896341f, 1e-37f);
+  bool dead = false;
+  uint32_t n = 0, slots = 0;  // steps; slots of the pieces before
+  unsigned piece = 0;
+  Walk<kStep> wk;
+  wk.init(a, c.plan);
+  while (wk.next(a)) {
+    ++piece;
+    const int len = wk.s.ctx + wk.s.nodes, steps = wk.t1 - wk.t0;
+    const Rows r = rows_of(a, wk);
+    const int node = r.node0 + row / a.head_box, head = r.head0 + row % a.head_box;
+    const bool live = row < r.nodes * a.head_box && head < a.heads;
+    const bool warp_live = __any_sync(0xffffffffu, live);
+    // tokens before this one are seen by every row of the block
+    const int common = wk.s.ctx + (a.mask ? 0 : wk.block * a.block_nodes + 1);
+    float m = -CUDART_INF_F, l = 0.f;
+    for (int t = wk.t0; t < wk.t1; ++t, ++n) {
+      const bool first = t == wk.t0, tail = t * kStep + kStep > common;
+      const uint32_t vis = tail && live ? visible32(a, wk.s, node, t * kStep + 32 * quarter) : ~0u;
+      wait(&c.s_full[n & 1], (n >> 1) & 1u, dead, a.error_flag);
+      fence_after();
+      uint32_t s[32];
+      float mt = -CUDART_INF_F;
+      if (warp_live) {
+        tmem_ld32(quad + col_s(n & 1) + 32 * part, s);
+        wait_ld(s);
+        mt = (tail ? mask_max<true>(s, vis) : mask_max<false>(s, ~0u)) * cl;
+      }
+      // the maximum is that of all quarters of the row; it moves when one has risen far enough
+      if (first || any_softmax(live && mt > m + kLazyLog2)) {
+        c.top[quarter][row] = mt;
+        bar_softmax();
+        mt = fmaxf(fmaxf(c.top[0][row], c.top[1][row]), fmaxf(c.top[2][row], c.top[3][row]));
+        const bool rise = live && mt > m + (first ? 0.f : kLazyLog2);
+        if (!first) {
+          // O moves to the new maximum once the values before are in it
+          const float keep = rise ? ex2(m - mt) : 1.f;
+          l *= keep;
+          wait(&c.p_free[(n - 1) & 1], ((n - 1) >> 1) & 1u, dead, a.error_flag);
+          fence_after();
+          if (warp_live) rescale(quad + col_o(part), keep);
+        }
+        if (rise) m = mt;
+        bar_softmax();  // (the maxima are read)
+      }
+      // P's buffer is free once the values of two steps before are in O
+      if (n >= 2) wait(&c.p_free[n & 1], ((n - 2) >> 1) & 1u, dead, a.error_flag);
+      if (warp_live)
+        l += put_weights<T>(s, cl, m, smem + kOffP + ((n & 1) * 2 + half) * kStickTile + row * 128, 4 * part, row & 7, true);
+      if (t * kStep + kStep > min(common, len)) {
+        // (this CTA's values, half of the elements: slots of two sticks, of either page by turns)
+        const int i = t - wk.t0;
+        for (int p = 0; p < 2; ++p) {
+          const uint32_t vs = slots + kPairs * (min(steps, i + 2) + i) + 2 * part + p;
+          wait(&c.full[vs % kSlots], (vs / kSlots) & 1u, dead, a.error_flag);
+          const int start = t * kStep + p * kTile;
+          clean<T, 2>(smem + kOffSlots + vs % kSlots * kSlot, tid & 127, max(common - start, 0), len - start);
+        }
+      }
+      fence_async_smem();
+      fence_before();
+      __syncwarp();
+      if (lane == 0) arrive_first(&c.p_ready[n & 1]);
+    }
+    slots += 2 * kPairs * steps;
+
+    // -------------------------------------------------------- end of piece --
+    const bool split = wk.t0 > 0 || wk.t1 < wk.tiles;
+    const int64_t pslot = 2 * blockIdx.x + (wk.t0 > 0 ? 0 : 1);  // one of each kind per share
+    const int64_t orow = static_cast<int64_t>(wk.s.q0 + node) * a.heads + head;
+    c.top[quarter][row] = l;
+    bar_softmax();
+    l = (c.top[0][row] + c.top[1][row]) + (c.top[2][row] + c.top[3][row]);
+    const float inv = split ? 1.f : (l == 0.f ? 0.f : 1.f / l);
+    if (live && quarter == 0) {
+      if (split)
+        a.part_ml[pslot * kTileRows + row] = make_float2(m, l);
+      else if (a.lse)
+        a.lse[orow] = l == 0.f ? -CUDART_INF_F : (m + log2f(l)) * 0.69314718055994530942f;
+    }
+    wait(&c.o_full, (piece - 1) & 1u, dead, a.error_flag);
+    fence_after();
+    // column x of product `part` is element 256 part + 128 half + x of this lane's row
+    if (warp_live) {
+      const int d0 = 256 * part + 128 * half;
+#pragma unroll 1
+      for (int x = 0; x < 128; x += 32) {
+        uint32_t o[32];
+        tmem_ld32(quad + col_o(part) + x, o);
+        wait_ld(o);
+        if (live && split) {
+          float4 *to = reinterpret_cast<float4 *>(a.part_o + (pslot * kTileRows + row) * kRank + d0 + x);
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            to[j] = make_float4(__uint_as_float(o[4 * j]), __uint_as_float(o[4 * j + 1]), __uint_as_float(o[4 * j + 2]),
+                                __uint_as_float(o[4 * j + 3]));
+        } else if (live) {
+          T *to = static_cast<T *>(a.out) + orow * kRank + d0 + x;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            float f[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) f[k] = inv == 0.f ? 0.f : __uint_as_float(o[8 * j + k]) * inv;
+            *reinterpret_cast<uint4 *>(to + 8 * j) = pack8(f, T());
+          }
+        }
+        __syncwarp();
+      }
+    }
+    fence_before();
+    bar_softmax();  // (the sums are read)
+    if (lane == 0) arrive_first(&c.o_empty);
+    // the second share of a split block describes it to the join
+    if (wk.t0 > 0 && tid == 0) {
+      const int first = wk.share_of(0, c.plan.per), share = static_cast<int>(blockIdx.x) / a.stride;
+      if (share == first + 1) {
+        Join j;
+        j.rows0 = wk.s.q0;
+        j.node0 = r.node0;
+        j.nodes = r.nodes;
+        j.head0 = r.head0;
+        j.first = first;
+        j.last = wk.share_of(wk.tiles - 1, c.plan.per);
+        a.joins[blockIdx.x] = j;
+      }
+    }
+    wk.advance(a);
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 1)
+    latent_pair_kernel(const __grid_constant__ CUtensorMap qm, const __grid_constant__ CUtensorMap rm,
+                       const __grid_constant__ CUtensorMap pm, const __grid_constant__ CUtensorMap sm,
+                       const __grid_constant__ Args a) {
+  extern __shared__ __align__(1024) uint8_t smem[];
+  Ctrl &c = *reinterpret_cast<Ctrl *>(smem);
+  const int tid = threadIdx.x, warp = tid >> 5;
+  if (tid == 0) {
+    prefetch_tensormap(&qm);
+    prefetch_tensormap(&rm);
+    prefetch_tensormap(&pm);
+    prefetch_tensormap(&sm);
+    for (int i = 0; i < kSlots; ++i) {
+      mbar_init(&c.full[i], 1);
+      mbar_init(&c.empty[i], 1);
+      mbar_init(&c.peer[i], 1);
+    }
+    mbar_init(&c.rope_full, 1);
+    mbar_init(&c.rope_empty, 1);
+    mbar_init(&c.rope_peer, 1);
+    mbar_init(&c.q_full, 1);
+    mbar_init(&c.q_empty, 1);
+    mbar_init(&c.q_peer, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&c.s_full[i], 1);
+      mbar_init(&c.p_ready[i], 2 * kSoftmaxWarps);
+      mbar_init(&c.p_free[i], 1);
+    }
+    mbar_init(&c.o_full, 1);
+    mbar_init(&c.o_empty, 2 * kSoftmaxWarps);
+    fence_mbar_init();
+  }
+  if (warp == 9) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&c.tmem)),
+                 "r"(kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (tid == 0) a.joins[blockIdx.x].nodes = 0;  // no block begins to be split here, unless the epilogue says so
+  make_plan<T, kStep>(a, c.plan);
+  fence_before();
+  __syncthreads();
+  cluster_sync();
+  fence_after();
+  const uint32_t tmem = c.tmem;
+  const bool leads = cluster_rank() == 0;
+  if (warp < kSoftmaxWarps)
+    softmax<T>(a, c, smem, tmem);
+  else if (warp == 8)
+    producer(a, c, smem, &qm, &rm, &pm, &sm);
+  else if (warp == 9 && leads)
+    score_issuer<T>(a, c, smem, tmem);
+  else if (warp == 10 && leads)
+    value_issuer<T>(a, c, smem, tmem);
+  else if (warp == 11 && !leads && elect_one())
+    relay(a, c);
+  __syncwarp();
+  fence_before();
+  __syncthreads();
+  cluster_sync();  // neither CTA ends while the other's operands or barriers may be used
+  if (warp == 9) {
+    fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+  }
+}
+
+}  // namespace pair
+}  // namespace latent
+}  // namespace b200kv
