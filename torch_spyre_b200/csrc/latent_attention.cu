@@ -41,8 +41,8 @@ Workspace workspace_of() {
 
 // The attention (on single SMs or on pairs) and the join behind it.
 template <typename T>
-int launch(const CUtensorMap &qm, const CUtensorMap &rm, const CUtensorMap &pm, const CUtensorMap &sm,
-           const latent::Args &a, bool pairs, int ctas, cudaStream_t stream) {
+int launch(const CUtensorMap &qm, const CUtensorMap &rm, const CUtensorMap &hm, const CUtensorMap &pm,
+           const CUtensorMap &sm, const latent::Args &a, bool pairs, int ctas, cudaStream_t stream) {
   const auto kernel = pairs ? latent::pair::latent_pair_kernel<T> : latent::latent_kernel<T>;
   const int smem = pairs ? latent::pair::kSmem : latent::kSmem;
   static int configured[2][64] = {{0}};
@@ -66,7 +66,7 @@ int launch(const CUtensorMap &qm, const CUtensorMap &rm, const CUtensorMap &pm, 
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = pairs ? 2 : 1;
-  B200KV_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, qm, rm, pm, sm, a));
+  B200KV_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, qm, rm, hm, pm, sm, a));
   cfg.gridDim = dim3(static_cast<unsigned>(ctas), static_cast<unsigned>((a.box_nodes * a.head_box + 7) / 8));
   cfg.blockDim = dim3(256);
   cfg.dynamicSmemBytes = 0;
@@ -151,7 +151,7 @@ extern "C" int b200kv_latent_attention(const void *q_latent, int64_t q_latent_st
   a.part_ml = reinterpret_cast<float2 *>(base + ws.ml);
   a.part_o = reinterpret_cast<float *>(base + ws.o);
   const CUtensorMapDataType type = dtype == B200KV_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-  CUtensorMap qm, rm, pm, sm;
+  CUtensorMap qm, rm, hm, pm, sm;
   auto q_map = [&](CUtensorMap *map, const void *q, int64_t stride_t, int64_t stride_h, int64_t width) {
     // a dimension of one element may have any stride
     const int64_t sh = num_heads == 1 ? width : stride_h, st = total_q == 1 ? num_heads * width : stride_t;
@@ -166,11 +166,12 @@ extern "C" int b200kv_latent_attention(const void *q_latent, int64_t q_latent_st
   };
   if ((st = q_map(&qm, q_latent, q_latent_stride_t, q_latent_stride_h, latent::kRank)) != B200KV_OK) return st;
   if ((st = q_map(&rm, q_rope, q_rope_stride_t, q_rope_stride_h, latent::kRope)) != B200KV_OK) return st;
-  if ((st = pool_map(&pm, 2)) != B200KV_OK || (st = pool_map(&sm, 1)) != B200KV_OK) return st;
+  if ((st = pool_map(&hm, 4)) != B200KV_OK || (st = pool_map(&pm, 2)) != B200KV_OK || (st = pool_map(&sm, 1)) != B200KV_OK)
+    return st;
   const int ctas = (sms < latent::kMaxCtas ? sms : latent::kMaxCtas) / a.stride * a.stride;
   if (ctas == 0) return set_error(B200KV_ERR_UNSUPPORTED, "a GPU of %d SMs", sms);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   const WorkspaceLock lock(workspace);
-  return dtype == B200KV_F16 ? launch<__half>(qm, rm, pm, sm, a, pairs, ctas, s)
-                             : launch<__nv_bfloat16>(qm, rm, pm, sm, a, pairs, ctas, s);
+  return dtype == B200KV_F16 ? launch<__half>(qm, rm, hm, pm, sm, a, pairs, ctas, s)
+                             : launch<__nv_bfloat16>(qm, rm, hm, pm, sm, a, pairs, ctas, s);
 }

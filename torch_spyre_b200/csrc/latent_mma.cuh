@@ -297,21 +297,23 @@ __device__ __forceinline__ int load_ids(const Args &a, int b, int window, int pa
   return id;
 }
 
+// Brings page `id` into L2.
+__device__ __forceinline__ void page_ahead(const Args &a, int id) {
+  prefetch_l2(static_cast<const uint8_t *>(a.pool) + static_cast<int64_t>(id) * (kSticks * kStickTile), kSticks * kStickTile);
+}
+
 __device__ __forceinline__ void producer(const Args &a, Ctrl &c, uint8_t *smem, const CUtensorMap *qm,
-                                         const CUtensorMap *rm, const CUtensorMap *pm, const CUtensorMap *sm) {
+                                         const CUtensorMap *rm, const CUtensorMap *hm, const CUtensorMap *sm) {
   const int lane = threadIdx.x & 31;
   const int head0 = static_cast<int>(blockIdx.x) % a.stride * a.head_box;
   const uint32_t q_bytes = static_cast<uint32_t>(a.box_nodes * a.head_box * 128);
-  const uint64_t policy_once = l2_policy_evict_first();
-  uint64_t policy_again;
-  asm volatile("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(policy_again));
+  // a page is read once (by one block of one CTA) and leaves L2 first
+  const uint64_t policy = l2_policy_evict_first();
   bool dead = false;
   uint32_t halves = 0, pieces = 0;  // issued
   Walk<kTile> w;
   w.init(a, c.plan);
   while (w.next(a)) {
-    // pages that one block of one CTA reads leave L2 first
-    const uint64_t policy = a.stride > 1 || w.s.blocks > 1 ? policy_again : policy_once;
     const int pages = (w.s.ctx + w.s.nodes + kPageTokens - 1) / kPageTokens;
     int window = w.t0 / 32, ids = load_ids(a, w.b, window, pages), ids_next = load_ids(a, w.b, window + 1, pages);
     wait(&c.q_empty, (pieces & 1u) ^ 1u, dead, a.error_flag);
@@ -333,16 +335,19 @@ __device__ __forceinline__ void producer(const Args &a, Ctrl &c, uint8_t *smem, 
       for (int h = 0; h < 2; ++h, ++halves) {
         // halves 2n and 2n + 1 are page n's
         const uint32_t n = halves >> 1, b = halves & 3u;
-        if (h == 0) wait(&c.rope_empty, (n & 1u) ^ 1u, dead, a.error_flag);
-        wait(&c.empty[b], ((n >> 1) & 1u) ^ 1u, dead, a.error_flag);
+        wait_until(
+            [&] {
+              const bool r = h == 1 || mbar_test(&c.rope_empty, (n & 1u) ^ 1u);
+              return r & mbar_test(&c.empty[b], ((n >> 1) & 1u) ^ 1u);
+            },
+            dead, a.error_flag);
         if ((dead = __any_sync(0xffffffffu, dead))) break;
-        if (lane == 0) {
-          uint8_t *to = smem + kOffSlots + b * 2 * kPair;
-          mbar_arrive_expect_tx(&c.full[b], 2 * kPair + (h == 0 ? kStickTile : 0));
-          if (h == 0) tma_load_3d(smem + kOffRope, sm, &c.full[b], 0, (kSticks - 1) * kTile, page, policy);
-          tma_load_3d(to, pm, &c.full[b], 0, h * 4 * kTile, page, policy);
-          tma_load_3d(to + kPair, pm, &c.full[b], 0, h * 4 * kTile + 2 * kTile, page, policy);
-        }
+        if (lane == 0) mbar_arrive_expect_tx(&c.full[b], 2 * kPair + (h == 0 ? kStickTile : 0));
+        __syncwarp();
+        if (lane == 0)
+          tma_load_3d(smem + kOffSlots + b * 2 * kPair, hm, &c.full[b], 0, h * 4 * kTile, page, policy);
+        else if (lane == 1 && h == 0)
+          tma_load_3d(smem + kOffRope, sm, &c.full[b], 0, (kSticks - 1) * kTile, page, policy);
         __syncwarp();
       }
     }
@@ -702,15 +707,15 @@ __device__ __forceinline__ void softmax(const Args &a, Ctrl &c, uint8_t *smem, u
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 1)
     latent_kernel(const __grid_constant__ CUtensorMap qm, const __grid_constant__ CUtensorMap rm,
-                  const __grid_constant__ CUtensorMap pm, const __grid_constant__ CUtensorMap sm,
-                  const __grid_constant__ Args a) {
+                  const __grid_constant__ CUtensorMap hm, const __grid_constant__ CUtensorMap,
+                  const __grid_constant__ CUtensorMap sm, const __grid_constant__ Args a) {
   extern __shared__ __align__(1024) uint8_t smem[];
   Ctrl &c = *reinterpret_cast<Ctrl *>(smem);
   const int tid = threadIdx.x, warp = tid >> 5;
   if (tid == 0) {
     prefetch_tensormap(&qm);
     prefetch_tensormap(&rm);
-    prefetch_tensormap(&pm);
+    prefetch_tensormap(&hm);
     prefetch_tensormap(&sm);
     for (int i = 0; i < 4; ++i) {
       mbar_init(&c.full[i], 1);
@@ -745,7 +750,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp < kSoftmaxWarps)
     softmax<T>(a, c, smem, tmem);
   else if (warp == 8)
-    producer(a, c, smem, &qm, &rm, &pm, &sm);
+    producer(a, c, smem, &qm, &rm, &hm, &sm);
   else if (warp == 9)
     score_issuer<T>(a, c, smem, tmem);
   else if (warp == 10)

@@ -10,9 +10,9 @@
 // at 32 and 64 clocks a product of 16, 2176 for 128 tokens, where its own operands
 // take 4 and 6 KB.  (One SM with 64 rows: 3800 clocks for 128 tokens.)
 //
-// A step's keys are read as they arrive, a pair of sticks at a time, and their slots
-// freed at once; its values, half of the elements of both pages, come again (out of
-// L2) when the weights are there.  So seven slots of 16 KB keep the products fed.
+// A step's keys are read as they arrive, half a page at a time, and their slots freed at
+// once; its values, half of the elements of both pages, come again (out of L2) when the
+// weights are there.  So four slots of 32 KB keep the products fed.
 //
 // An accumulator of 128 rows over two CTAs lies in each of them as 64 rows: lanes 0-63
 // have the first half of the columns, lanes 64-127 the second.  Warp w has the lanes of
@@ -30,10 +30,11 @@ namespace latent {
 namespace pair {
 
 constexpr int kStep = 2 * kPageTokens;  // tokens of a step
-constexpr int kSlots = 7, kSlot = kPair;
+constexpr int kSlots = 4, kSlot = 2 * kPair;
+constexpr int kAhead = 2;  // steps that pages are in L2 before they are loaded
 constexpr int kOffQ = 3072;
-constexpr int kOffP = kOffQ + kSticks * kStickTile;  // [2][2 pages][64 rows][64 tokens]
-constexpr int kOffRope = kOffP + 4 * kStickTile;
+constexpr int kOffP = kOffQ + kSticks * kStickTile;  // [2 pages][64 rows][64 tokens]
+constexpr int kOffRope = kOffP + 2 * kStickTile;
 constexpr int kOffSlots = kOffRope + kStickTile;
 constexpr int kSmem = kOffSlots + kSlots * kSlot;
 static_assert(kSmem <= 227 * 1024, "shared memory per CTA");
@@ -44,10 +45,10 @@ __device__ __forceinline__ uint32_t col_s(uint32_t b) { return 256u + b * 64u; }
 
 struct Ctrl {
   // each CTA's own: what has arrived, what is free again, what is computed
-  uint64_t full[kSlots], empty[kSlots], rope_full, rope_empty, q_full, q_empty;
-  uint64_t s_full[2], p_free[2], o_full;
+  uint64_t full[kSlots], empty[kSlots], rope_empty, q_full, q_empty;
+  uint64_t s_full[2], p_free, o_full;
   // the first CTA's: the second's arrivals, and both CTAs' weights and outputs
-  uint64_t peer[kSlots], rope_peer, q_peer, p_ready[2], o_empty;
+  uint64_t peer[kSlots], q_peer, p_ready[2], o_empty;
   uint32_t tmem;
   Plan plan;
   float top[4][kTileRows];  // maxima, then sums, of the quarters of a row's tokens
@@ -105,20 +106,12 @@ __device__ __forceinline__ Rows rows_of(const Args &a, const Walk<kStep> &w) {
   return r;
 }
 
-// The order of a piece's arrivals, which producer and relay share: the
-// rotary stick and four pairs of the keys of step t, one step ahead of the four parts
-// of the values.
-template <typename Keys, typename Values>
-__device__ __forceinline__ void in_order(const Walk<kStep> &w, Keys keys, Values values) {
-  keys(w.t0);
-  for (int t = w.t0; t < w.t1; ++t) {
-    if (t + 1 < w.t1) keys(t + 1);
-    values(t);
-  }
-}
-
+// A piece's copies, in order: two halves of the keys of step t (with the first the
+// rotary stick), one step ahead of two halves of the values (so keys of step i > 0 begin
+// at slot 2 (2 i - 1) of the piece, values of step i of n at 2 (min(n, i + 2) + i)).
 __device__ __forceinline__ void producer(const Args &a, Ctrl &c, uint8_t *smem, const CUtensorMap *qm,
-                                         const CUtensorMap *rm, const CUtensorMap *pm, const CUtensorMap *sm) {
+                                         const CUtensorMap *rm, const CUtensorMap *hm, const CUtensorMap *pm,
+                                         const CUtensorMap *sm) {
   const int lane = threadIdx.x & 31;
   const int rank = static_cast<int>(cluster_rank());
   const uint32_t q_bytes = static_cast<uint32_t>(a.box_nodes * a.head_box * 128);
@@ -130,6 +123,13 @@ __device__ __forceinline__ void producer(const Args &a, Ctrl &c, uint8_t *smem, 
     const int pages = (w.s.ctx + w.s.nodes + kPageTokens - 1) / kPageTokens;
     int window = w.t0 / 16, ids = load_ids(a, w.b, window, pages), ids_next = load_ids(a, w.b, window + 1, pages);
     int ids_before = ids;
+    // (a page that these ids do not reach is not brought ahead)
+    auto ahead = [&](int t) {
+      if (t >= w.t1 || t / 16 > window + 1) return;
+      const int id = __shfl_sync(0xffffffffu, t / 16 > window ? ids_next : ids, (2 * t + rank) & 31);
+      if (lane == 2 && id >= 0) page_ahead(a, id);
+    };
+    for (int t = w.t0; t < w.t0 + kAhead; ++t) ahead(t);
     wait(&c.q_empty, (pieces & 1u) ^ 1u, dead, a.error_flag);
     if ((dead = __any_sync(0xffffffffu, dead))) break;
     const Rows rows = rows_of(a, w);
@@ -144,52 +144,57 @@ __device__ __forceinline__ void producer(const Args &a, Ctrl &c, uint8_t *smem, 
       const int id = __shfl_sync(0xffffffffu, have, p & 31);
       return id < 0 ? a.num_blocks : id;
     };
-    auto load = [&](int row, int page) {
-      if (dead) return;
+    // Keys: lane 0 the half `h` of a page, lane 1 with the first the rotary stick.  Values:
+    // lanes 0 and 1 two sticks of a page each.
+    auto load = [&](bool key, int h, int page) {
       const uint32_t s = slots % kSlots;
-      wait(&c.empty[s], ((slots / kSlots) & 1u) ^ 1u, dead, a.error_flag);
+      const bool rope = key && h == 0;
+      wait_until(
+          [&] {
+            const bool r = !rope || mbar_test(&c.rope_empty, (steps & 1u) ^ 1u);
+            return r & mbar_test(&c.empty[s], (slots / kSlots & 1u) ^ 1u);
+          },
+          dead, a.error_flag);
       if ((dead = __any_sync(0xffffffffu, dead))) return;
-      if (lane == 0) {
-        mbar_arrive_expect_tx(&c.full[s], kSlot);
-        tma_3d(smem + kOffSlots + s * kSlot, pm, &c.full[s], 0, row, page);
+      if (lane == 0) mbar_arrive_expect_tx(&c.full[s], kSlot + (rope ? kStickTile : 0));
+      __syncwarp();
+      uint8_t *to = smem + kOffSlots + s * kSlot;
+      if (key) {
+        if (lane == 0)
+          tma_3d(to, hm, &c.full[s], 0, h * 4 * kTile, page);
+        else if (lane == 1 && rope)
+          tma_3d(smem + kOffRope, sm, &c.full[s], 0, (kSticks - 1) * kTile, page);
+      } else if (lane < 2) {
+        tma_3d(to + lane * kPair, pm, &c.full[s], 0, (4 * h + 2 * rank) * kTile, page);
       }
       __syncwarp();
       ++slots;
+      steps += rope;
     };
-    in_order(
-        w,
-        [&](int t) {
-          if (dead) return;
-          if (t / 16 > window) {  // keys lead, values follow by a step
-            ids_before = ids;
-            ids = ids_next;
-            ids_next = load_ids(a, w.b, ++window + 1, pages);
-          }
-          const int page = page_of(ids, 2 * t + rank);
-          wait(&c.rope_empty, (steps & 1u) ^ 1u, dead, a.error_flag);
-          if ((dead = __any_sync(0xffffffffu, dead))) return;
-          if (lane == 0) {
-            mbar_arrive_expect_tx(&c.rope_full, kStickTile);
-            tma_3d(smem + kOffRope, sm, &c.rope_full, 0, (kSticks - 1) * kTile, page);
-          }
-          __syncwarp();
-          ++steps;
-          for (int j = 0; j < kPairs; ++j) load(j * 2 * kTile, page);
-        },
-        [&](int t) {
-          const int have = t / 16 == window ? ids : ids_before;
-          const int page[2] = {page_of(have, 2 * t), page_of(have, 2 * t + 1)};
-#pragma unroll
-          for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int p = 0; p < 2; ++p) load((4 * j + 2 * rank) * kTile, page[p]);
-        });
+    auto keys = [&](int t) {
+      if (t / 16 > window) {  // keys lead, values follow by a step
+        ids_before = ids;
+        ids = ids_next;
+        ids_next = load_ids(a, w.b, ++window + 1, pages);
+      }
+      const int page = page_of(ids, 2 * t + rank);
+      load(true, 0, page);
+      if (!dead) load(true, 1, page);
+      ahead(t + kAhead);
+    };
+    keys(w.t0);
+    for (int t = w.t0; t < w.t1 && !dead; ++t) {
+      if (t + 1 < w.t1) keys(t + 1);
+      if (dead) break;
+      const int page = page_of(t / 16 == window ? ids : ids_before, 2 * t + (lane & 1));
+      load(false, 0, page);
+      if (!dead) load(false, 1, page);
+    }
     w.advance(a);
   }
   if (dead) {  // the copies under way, with a limit
     bool late = false;
     if (pieces > 0) wait(&c.q_full, (pieces - 1) & 1u, late, a.error_flag);
-    if (steps > 0) wait(&c.rope_full, (steps - 1) & 1u, late, a.error_flag);
     for (uint32_t n = slots - min(slots, uint32_t(kSlots)); n < slots; ++n)
       wait(&c.full[n % kSlots], (n / kSlots) & 1u, late, a.error_flag);
   }
@@ -201,31 +206,39 @@ __device__ __forceinline__ void producer(const Args &a, Ctrl &c, uint8_t *smem, 
   __syncwarp();
 }
 
-// The second CTA's arrivals, told to the first.
+// The second CTA's arrivals, told to the first: a lane for every slot and one for Q,
+// each as often as it is filled.
 __device__ __forceinline__ void relay(const Args &a, Ctrl &c) {
-  bool dead = false;
-  uint32_t slots = 0, steps = 0, pieces = 0;
+  const uint32_t lane = threadIdx.x & 31;
+  uint32_t steps = 0, pieces = 0;
   Walk<kStep> w;
-  w.init(a, c.plan);
-  while (!dead && w.next(a)) {
-    wait(&c.q_full, pieces++ & 1u, dead, a.error_flag);
-    if (!dead) arrive_first(&c.q_peer);
-    auto slot = [&] {
-      wait(&c.full[slots % kSlots], (slots / kSlots) & 1u, dead, a.error_flag);
-      if (!dead) arrive_first(&c.peer[slots % kSlots]);
-      ++slots;
-    };
-    in_order(
-        w,
-        [&](int) {
-          wait(&c.rope_full, steps++ & 1u, dead, a.error_flag);
-          if (!dead) arrive_first(&c.rope_peer);
-          for (int j = 0; j < kPairs; ++j) slot();
-        },
-        [&](int) {
-          for (int j = 0; j < kPairs; ++j) slot();
-        });
-    w.advance(a);
+  for (w.init(a, c.plan); w.next(a); w.advance(a)) {
+    steps += w.t1 - w.t0;
+    ++pieces;
+  }
+  static_assert(kSlots == 4, "a step fills every slot once");
+  uint64_t *from = lane < kSlots ? &c.full[lane] : &c.q_full;
+  uint64_t *to = lane < kSlots ? &c.peer[lane] : &c.q_peer;
+  uint32_t left = lane < kSlots ? steps : (lane == kSlots ? pieces : 0);
+  uint32_t parity = 0, idle = 0;
+  uint64_t since = 0;
+  while (__any_sync(0xffffffffu, left > 0)) {
+    const bool ready = left > 0 && mbar_test(from, parity);
+    if (ready) {
+      arrive_first(to);
+      parity ^= 1u;
+      --left;
+    }
+    if (__any_sync(0xffffffffu, ready)) {
+      idle = 0;
+    } else if ((++idle & 1023u) == 0) {
+      const uint64_t now = global_timer_ns();
+      if (idle == 1024u) since = now;
+      if (__any_sync(0xffffffffu, now - since > kWaitLimitNs)) {  // (the first CTA's waits run out as well)
+        if (lane == 0 && a.error_flag) atomicOr(a.error_flag, B200KV_DEVERR_TIMEOUT);
+        break;
+      }
+    }
   }
 }
 
@@ -247,19 +260,16 @@ __device__ __forceinline__ void score_issuer(const Args &a, Ctrl &c, uint8_t *sm
   while (w.next(a)) {
     const int steps = w.t1 - w.t0;
     for (int i = 0; i < steps; ++i, ++n) {
-      const uint32_t odd = uniform(n & 1u), at = slots + kPairs * (i + max(i - 1, 0));
+      const uint32_t odd = uniform(n & 1u), at = slots + 2 * (i + max(i - 1, 0));
       const uint32_t s = tmem + col_s(0) + odd * 64;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        uint32_t at0 = uniform((at + 2 * h) % kSlots), at1 = uniform((at + 2 * h + 1) % kSlots);
-        const uint32_t par0 = (at + 2 * h) / kSlots & 1u, par1 = (at + 2 * h + 1) / kSlots & 1u;
+        const uint32_t slot = uniform((at + h) % kSlots), parity = (at + h) / kSlots & 1u;
         wait_until(
             [&] {
-              bool ok = mbar_test(&c.full[at0], par0) & mbar_test(&c.peer[at0], par0) & mbar_test(&c.full[at1], par1) &
-                        mbar_test(&c.peer[at1], par1);
+              bool ok = mbar_test(&c.full[slot], parity) & mbar_test(&c.peer[slot], parity);
               if (h == 0) {
                 // this score buffer is free once the step before last has weights
-                ok = ok & mbar_test(&c.rope_full, n & 1u) & mbar_test(&c.rope_peer, n & 1u);
                 if (n >= 2) ok = ok & mbar_test(&c.p_ready[odd], ((n - 2) >> 1) & 1u);
                 if (i == 0) ok = ok & mbar_test(&c.q_full, pieces & 1u) & mbar_test(&c.q_peer, pieces & 1u);
               }
@@ -273,21 +283,18 @@ __device__ __forceinline__ void score_issuer(const Args &a, Ctrl &c, uint8_t *sm
             mma_pair(s, qd + ((kSticks - 1) * kStickTile + k * 32 >> 4), rd + (k * 32 >> 4), idesc, k > 0, go);
           done(&c.rope_empty);
         }
+        const uint32_t k0 = kd + (slot * kSlot >> 4);
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const uint32_t k0 = kd + ((j ? at1 : at0) * kSlot >> 4);
-#pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const uint32_t off = ((k >> 2) * kStickTile + (k & 3) * 32) >> 4;
-            mma_pair(s, qd + ((2 * h + j) * kPair >> 4) + off, k0 + off, idesc, 1, go);
-          }
-          done(&c.empty[j ? at1 : at0]);
+        for (int k = 0; k < 16; ++k) {
+          const uint32_t off = ((k >> 2) * kStickTile + (k & 3) * 32) >> 4;
+          mma_pair(s, qd + (h * 2 * kPair >> 4) + off, k0 + off, idesc, 1, go);
         }
+        done(&c.empty[slot]);
       }
       done(&c.s_full[odd]);
     }
     done(&c.q_empty);
-    slots += 2 * kPairs * steps;
+    slots += kSlots * steps;
     ++pieces;
     w.advance(a);
   }
@@ -310,39 +317,34 @@ __device__ __forceinline__ void value_issuer(const Args &a, Ctrl &c, uint8_t *sm
   while (w.next(a)) {
     const int steps = w.t1 - w.t0;
     for (int i = 0; i < steps; ++i, ++n) {
-      const uint32_t odd = uniform(n & 1u), later = uniform(i > 0);
-      const uint32_t at = slots + kPairs * (min(steps, i + 2) + i);
-      const uint32_t p0 = pd + (odd * 2 * kStickTile >> 4);
+      const uint32_t later = uniform(i > 0), at = slots + 2 * (min(steps, i + 2) + i);
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const uint32_t at0 = uniform((at + 2 * j) % kSlots), at1 = uniform((at + 2 * j + 1) % kSlots);
-        const uint32_t par0 = (at + 2 * j) / kSlots & 1u, par1 = (at + 2 * j + 1) / kSlots & 1u;
+        const uint32_t slot = uniform((at + j) % kSlots), parity = (at + j) / kSlots & 1u;
         wait_until(
             [&] {
-              bool ok = mbar_test(&c.full[at0], par0) & mbar_test(&c.peer[at0], par0) & mbar_test(&c.full[at1], par1) &
-                        mbar_test(&c.peer[at1], par1);
+              bool ok = mbar_test(&c.full[slot], parity) & mbar_test(&c.peer[slot], parity);
               if (j == 0) {
-                ok = ok & mbar_test(&c.p_ready[odd], (n >> 1) & 1u);
+                ok = ok & mbar_test(&c.p_ready[n & 1u], (n >> 1) & 1u);
                 if (i == 0) ok = ok & mbar_test(&c.o_empty, (pieces & 1u) ^ 1u);
               }
               return ok;
             },
             dead, a.error_flag);
         fence_after();
+        const uint32_t v = vd + (slot * kSlot >> 4);
 #pragma unroll
-        for (int p = 0; p < 2; ++p) {
-          const uint32_t v = vd + ((p ? at1 : at0) * kSlot >> 4);
+        for (int p = 0; p < 2; ++p)
 #pragma unroll
           for (int k = 0; k < kTile / 16; ++k)
-            mma_pair(tmem + col_o(j), p0 + (p * kStickTile + k * 32 >> 4), v + (k * 2048 >> 4), idesc, p + k > 0 ? 1 : later,
-                     go);
-          done(&c.empty[p ? at1 : at0]);
-        }
+            mma_pair(tmem + col_o(j), pd + (p * kStickTile + k * 32 >> 4), v + (p * kPair + k * 2048 >> 4), idesc,
+                     p + k > 0 ? 1 : later, go);
+        done(&c.empty[slot]);
       }
-      done(&c.p_free[odd]);
+      done(&c.p_free);
     }
     done(&c.o_full);
-    slots += 2 * kPairs * steps;
+    slots += kSlots * steps;
     ++pieces;
     w.advance(a);
   }
@@ -409,25 +411,24 @@ __device__ __forceinline__ void softmax(const Args &a, Ctrl &c, uint8_t *smem, u
           // O moves to the new maximum once the values before are in it
           const float keep = rise ? ex2(m - mt) : 1.f;
           l *= keep;
-          wait(&c.p_free[(n - 1) & 1], ((n - 1) >> 1) & 1u, dead, a.error_flag);
+          wait(&c.p_free, (n - 1) & 1u, dead, a.error_flag);
           fence_after();
           if (warp_live) rescale(quad + col_o(part), keep);
         }
         if (rise) m = mt;
         bar_softmax();  // (the maxima are read)
       }
-      // P's buffer is free once the values of two steps before are in O
-      if (n >= 2) wait(&c.p_free[n & 1], ((n - 2) >> 1) & 1u, dead, a.error_flag);
+      // P is free once the values of the step before are in O
+      if (n >= 1) wait(&c.p_free, (n - 1) & 1u, dead, a.error_flag);
       if (warp_live)
-        l += put_weights<T>(s, cl, m, smem + kOffP + ((n & 1) * 2 + half) * kStickTile + row * 128, 4 * part, row & 7, true);
+        l += put_weights<T>(s, cl, m, smem + kOffP + half * kStickTile + row * 128, 4 * part, row & 7, true);
       if (t * kStep + kStep > min(common, len)) {
-        // (this CTA's values, half of the elements: slots of two sticks, of either page by turns)
-        const int i = t - wk.t0;
+        // (this CTA's values, half of the elements: a slot for each product, both pages)
+        const uint32_t vs = slots + 2 * (min(steps, t - wk.t0 + 2) + t - wk.t0) + part;
+        wait(&c.full[vs % kSlots], (vs / kSlots) & 1u, dead, a.error_flag);
         for (int p = 0; p < 2; ++p) {
-          const uint32_t vs = slots + kPairs * (min(steps, i + 2) + i) + 2 * part + p;
-          wait(&c.full[vs % kSlots], (vs / kSlots) & 1u, dead, a.error_flag);
           const int start = t * kStep + p * kTile;
-          clean<T, 2>(smem + kOffSlots + vs % kSlots * kSlot, tid & 127, max(common - start, 0), len - start);
+          clean<T, 2>(smem + kOffSlots + vs % kSlots * kSlot + p * kPair, tid & 127, max(common - start, 0), len - start);
         }
       }
       fence_async_smem();
@@ -435,7 +436,7 @@ __device__ __forceinline__ void softmax(const Args &a, Ctrl &c, uint8_t *smem, u
       __syncwarp();
       if (lane == 0) arrive_first(&c.p_ready[n & 1]);
     }
-    slots += 2 * kPairs * steps;
+    slots += kSlots * steps;
 
     // -------------------------------------------------------- end of piece --
     const bool split = wk.t0 > 0 || wk.t1 < wk.tiles;
@@ -504,14 +505,15 @@ __device__ __forceinline__ void softmax(const Args &a, Ctrl &c, uint8_t *smem, u
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 1)
     latent_pair_kernel(const __grid_constant__ CUtensorMap qm, const __grid_constant__ CUtensorMap rm,
-                       const __grid_constant__ CUtensorMap pm, const __grid_constant__ CUtensorMap sm,
-                       const __grid_constant__ Args a) {
+                       const __grid_constant__ CUtensorMap hm, const __grid_constant__ CUtensorMap pm,
+                       const __grid_constant__ CUtensorMap sm, const __grid_constant__ Args a) {
   extern __shared__ __align__(1024) uint8_t smem[];
   Ctrl &c = *reinterpret_cast<Ctrl *>(smem);
   const int tid = threadIdx.x, warp = tid >> 5;
   if (tid == 0) {
     prefetch_tensormap(&qm);
     prefetch_tensormap(&rm);
+    prefetch_tensormap(&hm);
     prefetch_tensormap(&pm);
     prefetch_tensormap(&sm);
     for (int i = 0; i < kSlots; ++i) {
@@ -519,17 +521,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&c.empty[i], 1);
       mbar_init(&c.peer[i], 1);
     }
-    mbar_init(&c.rope_full, 1);
     mbar_init(&c.rope_empty, 1);
-    mbar_init(&c.rope_peer, 1);
     mbar_init(&c.q_full, 1);
     mbar_init(&c.q_empty, 1);
     mbar_init(&c.q_peer, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&c.s_full[i], 1);
       mbar_init(&c.p_ready[i], 2 * kSoftmaxWarps);
-      mbar_init(&c.p_free[i], 1);
     }
+    mbar_init(&c.p_free, 1);
     mbar_init(&c.o_full, 1);
     mbar_init(&c.o_empty, 2 * kSoftmaxWarps);
     fence_mbar_init();
@@ -553,12 +553,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp < kSoftmaxWarps)
     softmax<T>(a, c, smem, tmem);
   else if (warp == 8)
-    producer(a, c, smem, &qm, &rm, &pm, &sm);
+    producer(a, c, smem, &qm, &rm, &hm, &pm, &sm);
   else if (warp == 9 && leads)
     score_issuer<T>(a, c, smem, tmem);
   else if (warp == 10 && leads)
     value_issuer<T>(a, c, smem, tmem);
-  else if (warp == 11 && !leads && elect_one())
+  else if (warp == 11 && !leads)
     relay(a, c);
   __syncwarp();
   fence_before();

@@ -114,6 +114,11 @@ __device__ __forceinline__ void tma_3d(void *dst, const CUtensorMap *map, uint64
       : "memory");
 }
 
+// Brings `bytes` (a multiple of 16, from a 16-byte aligned address) into L2.
+__device__ __forceinline__ void prefetch_l2(const void *at, uint32_t bytes) {
+  asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(at), "r"(bytes) : "memory");
+}
+
 // -------------------------------------------------------------- arithmetic --
 __device__ __forceinline__ uint32_t low_bits(int n) { return n >= 32 ? ~0u : (n <= 0 ? 0u : (1u << n) - 1u); }
 __device__ __forceinline__ float ex2(float x) {
