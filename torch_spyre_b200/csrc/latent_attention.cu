@@ -67,7 +67,7 @@ int launch(const CUtensorMap &qm, const CUtensorMap &rm, const CUtensorMap &hm, 
   cfg.attrs = attr;
   cfg.numAttrs = pairs ? 2 : 1;
   B200KV_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, qm, rm, hm, pm, sm, a));
-  cfg.gridDim = dim3(static_cast<unsigned>(ctas), static_cast<unsigned>((a.box_nodes * a.head_box + 7) / 8));
+  cfg.gridDim = dim3(static_cast<unsigned>(ctas), static_cast<unsigned>((a.box_nodes * a.head_box + 3) / 4));
   cfg.blockDim = dim3(256);
   cfg.dynamicSmemBytes = 0;
   cfg.numAttrs = 1;

@@ -765,48 +765,82 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 // ------------------------------------------------------------------- join --
 // Blocks cut by shares: out = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i over the
-// pieces in order (the same bits every time).  A warp per row, 8 rows a CTA.
+// pieces in order (the same bits every time).  A warp per row and half of its elements,
+// 4 rows a CTA.  The pieces' maxima and sums come first, one to a lane, so that the
+// sums over their elements are loads that wait for nothing, eight under way.
 template <typename T>
 __global__ void __launch_bounds__(256) latent_join_kernel(const __grid_constant__ Args a) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  __shared__ float weight[4][kMaxCtas];
   const Join j = a.joins[blockIdx.x];
-  const int row = blockIdx.y * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int row = blockIdx.y * 4 + (warp >> 1), half = warp & 1;
   const int part = static_cast<int>(blockIdx.x) % a.stride;
   const int node = row / a.head_box, head = j.head0 + row % a.head_box;
-  if (node >= j.nodes || head >= a.heads) return;
+  if (blockIdx.y * 4 / a.head_box >= j.nodes) return;  // (the whole CTA)
+  const bool live = node < j.nodes && head < a.heads;
+  const int pieces = j.last - j.first + 1;
+  // the partials of piece i are in slot first_slot + i * step, the first piece's in the odd one
+  const int64_t slot0 = 2 * (int64_t{j.first} * a.stride + part), step = 2 * a.stride;
   float M = -CUDART_INF_F, l = 0.f;
-  float4 o[4];
+  if (live) {
+    for (int i0 = 0; i0 < pieces; i0 += 32) {
+      const int i = i0 + lane;
+      if (i < pieces) M = fmaxf(M, a.part_ml[(slot0 + i * step + (i == 0)) * kTileRows + row].x);
+    }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int x = j.first; x <= j.last; ++x) {
-    const int64_t slot = 2 * (x * a.stride + part) + (x == j.first ? 1 : 0);
-    const float2 ml = a.part_ml[slot * kTileRows + row];
-    const float4 *v = reinterpret_cast<const float4 *>(a.part_o + (slot * kTileRows + row) * kRank) + lane;
-    float4 p[4];
+    for (int x = 16; x > 0; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
+    const float mm = M == -CUDART_INF_F ? 0.f : M;
+    for (int i0 = 0; i0 < pieces; i0 += 32) {
+      const int i = i0 + lane;
+      float w = 0.f, y = 0.f;
+      if (i < pieces) {
+        const float2 ml = a.part_ml[(slot0 + i * step + (i == 0)) * kTileRows + row];
+        w = exp2f(ml.x - mm);
+        y = ml.y * w;
+        weight[warp >> 1][i] = w;
+      }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) p[i] = v[32 * i];
-    const float top = fmaxf(M, ml.x), mm = top == -CUDART_INF_F ? 0.f : top;
-    const float old = exp2f(M - mm), keep = exp2f(ml.x - mm);
-    M = top;
-    l = fmaf(ml.y, keep, l * old);
+      for (int x = 16; x > 0; x >>= 1) y += __shfl_xor_sync(0xffffffffu, y, x);
+      l += y;
+    }
+  }
+  __syncthreads();  // (both warps of a row write the same weights)
+  if (!live) return;
+  const float4 *from = reinterpret_cast<const float4 *>(a.part_o) + row * (kRank / 4) + half * (kRank / 8) + lane;
+  float4 o[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
+  for (int i0 = 0; i0 < pieces; i0 += 4) {
+    float4 v[4][2];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      o[i].x = fmaf(p[i].x, keep, o[i].x * old), o[i].y = fmaf(p[i].y, keep, o[i].y * old);
-      o[i].z = fmaf(p[i].z, keep, o[i].z * old), o[i].w = fmaf(p[i].w, keep, o[i].w * old);
+    for (int k = 0; k < 4; ++k) {
+      const int i = min(i0 + k, pieces - 1);
+      const float4 *p = from + (slot0 + i * step + (i == 0)) * (kTileRows * kRank / 4);
+      v[k][0] = p[0];
+      v[k][1] = p[32];
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (i0 + k >= pieces) continue;
+      const float w = weight[warp >> 1][i0 + k];
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        o[x].x = fmaf(v[k][x].x, w, o[x].x), o[x].y = fmaf(v[k][x].y, w, o[x].y);
+        o[x].z = fmaf(v[k][x].z, w, o[x].z), o[x].w = fmaf(v[k][x].w, w, o[x].w);
+      }
     }
   }
   const int64_t orow = (j.rows0 + j.node0 + node) * a.heads + head;
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  T *out = static_cast<T *>(a.out) + orow * kRank + 4 * lane;
+  const bool none = l == 0.f;
+  const float inv = none ? 0.f : 1.f / l;
+  T *out = static_cast<T *>(a.out) + orow * kRank + half * (kRank / 2) + 4 * lane;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const bool none = l == 0.f;
-    const uint32_t lo = pack2(none ? 0.f : o[i].x * inv, none ? 0.f : o[i].y * inv, T());
-    const uint32_t hi = pack2(none ? 0.f : o[i].z * inv, none ? 0.f : o[i].w * inv, T());
-    *reinterpret_cast<uint2 *>(out + 128 * i) = make_uint2(lo, hi);
+  for (int x = 0; x < 2; ++x) {
+    const uint32_t lo = pack2(none ? 0.f : o[x].x * inv, none ? 0.f : o[x].y * inv, T());
+    const uint32_t hi = pack2(none ? 0.f : o[x].z * inv, none ? 0.f : o[x].w * inv, T());
+    *reinterpret_cast<uint2 *>(out + 128 * x) = make_uint2(lo, hi);
   }
-  if (lane == 0 && a.lse) a.lse[orow] = l == 0.f ? -CUDART_INF_F : (M + log2f(l)) * 0.69314718055994530942f;
+  if (lane == 0 && half == 0 && a.lse) a.lse[orow] = none ? -CUDART_INF_F : (M + log2f(l)) * 0.69314718055994530942f;
 }
 
 }  // namespace latent

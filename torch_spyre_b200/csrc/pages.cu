@@ -104,7 +104,7 @@ __device__ __forceinline__ int scan_block(int x, int *warps) {  // inclusive
 template <bool kRelease, bool kSlots>
 __global__ void __launch_bounds__(kThreads) pages_kernel(const PageArgs a) {
   __shared__ int32_t indptr[kMaxBatch + 1], counts[kMaxBatch];
-  __shared__ int warps[32], moved;
+  __shared__ int warps[32], moved, sums[kMaxBatch], firsts[kMaxBatch];
   const int b = threadIdx.x, lane = b & 31;
   if (b == 0) moved = 0;
   const int stack_in = a.free_count[0];
@@ -143,7 +143,8 @@ __global__ void __launch_bounds__(kThreads) pages_kernel(const PageArgs a) {
     if (kSlots) counts[b] = now;
     a.counts[b] = now;
   }
-  if (kRelease) __syncthreads();  // release counts down from its end
+  __syncthreads();  // (release counts down from its end)
+  // Page `at` of all that move is entry `from` of sequence `seq`.
   auto move = [&](int seq, int from, int at, int j) {
     int32_t *entry = a.table + seq * a.stride + from + j;
     if (kRelease) {
@@ -153,14 +154,21 @@ __global__ void __launch_bounds__(kThreads) pages_kernel(const PageArgs a) {
       *entry = __ldg(a.free_pages + stack - 1 - (at + j));
     }
   };
-  // few pages each: a thread for a sequence; many: its warp
-  if (__reduce_max_sync(0xffffffffu, n) <= 4) {
+  // few pages each: a thread for a sequence; many: a thread for a page, whose sequence is
+  // the first that the sum passes it at (256 prompts of up to 16 pages: a warp for a
+  // sequence after the other took 16 us, this 6)
+  sums[b] = served ? upto : INT_MAX;
+  firsts[b] = first - off;
+  if (!__syncthreads_or(n > 4)) {
     for (int j = 0; j < n; ++j) move(b, first, off, j);
   } else {
-    for (int s = 0; s < 32; ++s) {
-      const int m = __shfl_sync(0xffffffffu, n, s), f = __shfl_sync(0xffffffffu, first, s);
-      const int o = __shfl_sync(0xffffffffu, off, s);
-      for (int j = lane; j < m; j += 32) move(b - lane + s, f, o, j);
+    for (int k = b; k < moved; k += kThreads) {
+      int lo = 0, hi = a.batch - 1;
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (sums[mid] > k) hi = mid; else lo = mid + 1;
+      }
+      move(lo, firsts[lo] + k, k, 0);
     }
   }
   __syncthreads();
