@@ -15,10 +15,11 @@
 // has risen by more than 2^8.
 //
 // Shared memory holds two Q tiles and eight columns of 64 elements x 128 tokens: a
-// K tile is three (two of the head's, one of the shared part), a V tile two, each
-// freed by itself, so that the next tile's come in while this one's are in use.
+// K tile is three (two of the head's, one of the shared part), a V tile two, so
+// that the next tile's come in while this one's are in use.
 //
-// Warps: 0-3 and 4-7 the two softmax warpgroups, 8 the TMA producer, 9 the MMA issuer.
+// Warps: 0-3 and 4-7 the two softmax warpgroups, 8 the TMA producer, 9 and 10 issue the
+// streams' MMAs.
 #pragma once
 
 #include "prompt_attention.h"
@@ -56,7 +57,7 @@ struct Start {
 };
 
 struct Ctrl {
-  uint64_t full[kSlots], empty[kSlots];
+  uint64_t full[kSlots], empty[kSlots];  // (a slot is empty when both streams say so)
   uint64_t q_full, q_empty;
   uint64_t s_full[2], p_ready[2], o_full[2];
   uint32_t tmem;
@@ -237,16 +238,95 @@ __device__ __forceinline__ void make_plan(const Args &a, Ctrl &c) {
   }
 }
 
+// The columns' places, one tile after the other.  A V tile's two lie side by side (one
+// product reads both), so one that would begin in the last slot begins in the first, and
+// that slot is not used in its turn: every slot has a parity of its own.
+struct Ring {
+  uint32_t pos = 0, parities = 0;
+  struct Tile {
+    uint32_t at, parities;  // first slot, the slots' parities
+    __device__ __forceinline__ uint32_t slot(uint32_t c) const { return (at + c) % kSlots; }
+    __device__ __forceinline__ uint32_t parity(uint32_t c) const { return parities >> slot(c) & 1u; }
+  };
+  template <int kCols>
+  __device__ __forceinline__ Tile take() {
+    if (kCols == kColsV && pos == kSlots - 1) pos = 0;
+    const Tile t{pos, parities};
+    const uint32_t used = ((1u << kCols) - 1u) << pos;
+    parities ^= (used | used >> kSlots) & ((1u << kSlots) - 1u);
+    pos = (pos + kCols) % kSlots;
+    return t;
+  }
+  __device__ __forceinline__ Tile k() { return take<kColsQ>(); }
+  __device__ __forceinline__ Tile v() { return take<kColsV>(); }
+};
+__device__ __forceinline__ bool mbar_test(uint64_t *bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+// Waits, with a limit, until `ready` (which tests barriers side by side) holds.
+template <typename Ready>
+__device__ __forceinline__ void wait_until(Ready ready, bool &dead, int32_t *flag) {
+  if (dead || ready()) return;
+  uint64_t t0 = 0;
+  for (uint32_t i = 1;; ++i) {
+    if (ready()) return;
+    if ((i & 1023u) != 0) continue;
+    const uint64_t now = global_timer_ns();
+    if (t0 == 0) t0 = now;
+    if (now - t0 > kWaitLimitNs) break;
+  }
+  dead = true;
+  if (flag) atomicOr(flag, B200KV_DEVERR_TIMEOUT);
+}
+
 // ------------------------------------------------------------------- roles --
 __device__ __forceinline__ void producer(const Args &a, Ctrl &c, uint8_t *smem, const CUtensorMap *qm,
                                          const CUtensorMap *km, const CUtensorMap *rm, const CUtensorMap *vm) {
   const int lane = threadIdx.x & 31;
   bool dead = false;
-  uint32_t slot = 0, pieces = 0;  // columns issued, pieces begun
+  uint32_t pieces = 0;  // begun
+  Ring ring;
+  uint32_t loaded = 0, last = 0;  // slots with a copy that was issued, their parities
   Walk w;
   w.init(c);
   while (w.next(a, c)) {
     const bool two = w.two();
+    // a column to a lane
+    auto issue = [&](const Ring::Tile &tile, uint32_t cols, const CUtensorMap *map, int t) {
+      wait_until(
+          [&] {
+            bool ok = mbar_test(&c.empty[tile.slot(0)], tile.parity(0) ^ 1u) & mbar_test(&c.empty[tile.slot(1)], tile.parity(1) ^ 1u);
+            if (cols == 3) ok = ok & mbar_test(&c.empty[tile.slot(2)], tile.parity(2) ^ 1u);
+            return ok;
+          },
+          dead, a.error_flag);
+      if ((dead = __any_sync(0xffffffffu, dead))) return;
+      if (lane < static_cast<int>(cols)) {
+        const uint32_t s = tile.slot(lane);
+        mbar_arrive_expect_tx(&c.full[s], kCol);
+        tma_3d(smem + kOffSlots + s * kCol, lane == 2 ? rm : map, &c.full[s], lane == 1 ? 64 : 0, lane == 2 ? 0 : w.head,
+               w.s.kv0 + t * kTile);
+      }
+      __syncwarp();
+      for (uint32_t x = 0; x < cols; ++x) {
+        const uint32_t bit = 1u << tile.slot(x);
+        loaded |= bit;
+        last = (last & ~bit) | (tile.parities & bit);
+      }
+    };
+    // K leads V by one tile per stream that needs it
+    const int lead = two ? 1 : 2;
+    for (int t = w.t0; t < min(w.t0 + lead, w.t1) && !dead; ++t) issue(ring.k(), kColsQ, km, t);
+    // (the first keys may come before the piece before is done with Q)
+    if (dead) break;
     wait(&c.q_empty, (pieces & 1u) ^ 1u, dead, a.error_flag);
     if ((dead = __any_sync(0xffffffffu, dead))) break;
     const int n = (two ? 2 : 1) * kColsQ;
@@ -256,29 +336,9 @@ __device__ __forceinline__ void producer(const Args &a, Ctrl &c, uint8_t *smem, 
       tma_3d(smem + kOffQ + lane * kCol, qm, &c.q_full, lane % kColsQ * 64, w.head,
              w.s.q0 + (2 * w.block + lane / kColsQ) * kTile);
     ++pieces;
-    auto issue = [&](const CUtensorMap *map, int x, int head, int t) {
-      if (dead) return;
-      const uint32_t s = slot % kSlots;
-      wait(&c.empty[s], ((slot / kSlots) & 1u) ^ 1u, dead, a.error_flag);
-      if ((dead = __any_sync(0xffffffffu, dead))) return;
-      if (lane == 0) {
-        mbar_arrive_expect_tx(&c.full[s], kCol);
-        tma_3d(smem + kOffSlots + s * kCol, map, &c.full[s], x, head, w.s.kv0 + t * kTile);
-      }
-      ++slot;
-    };
-    auto issue_k = [&](int t) {
-      issue(km, 0, w.head, t);
-      issue(km, 64, w.head, t);
-      issue(rm, 0, 0, t);
-    };
-    // K leads V by one tile per stream that needs it: the order the MMA warp consumes them in
-    const int lead = two ? 1 : 2;
-    for (int t = w.t0; t < min(w.t0 + lead, w.t1); ++t) issue_k(t);
-    for (int t = w.t0; t < w.t1; ++t) {
-      issue(vm, 0, w.head, t);
-      issue(vm, 64, w.head, t);
-      if (t + lead < w.t1) issue_k(t + lead);
+    for (int t = w.t0; t < w.t1 && !dead; ++t) {
+      issue(ring.v(), kColsV, vm, t);
+      if (t + lead < w.t1 && !dead) issue(ring.k(), kColsQ, km, t + lead);
     }
     if (dead) break;
     w.advance(a);
@@ -286,8 +346,8 @@ __device__ __forceinline__ void producer(const Args &a, Ctrl &c, uint8_t *smem, 
   if (dead) {  // the copies under way, with a limit
     bool late = false;
     if (pieces > 0) wait(&c.q_full, (pieces - 1) & 1u, late, a.error_flag);
-    for (uint32_t n = slot - min(slot, uint32_t(kSlots)); n < slot; ++n)
-      wait(&c.full[n % kSlots], (n / kSlots) & 1u, late, a.error_flag);
+    for (uint32_t s = 0; s < kSlots; ++s)
+      if (loaded >> s & 1u) wait(&c.full[s], last >> s & 1u, late, a.error_flag);
   }
   // the last arrival that the MMAs owe this CTA: not before it may the CTA end
   if (lane == 0 && pieces > 0) {
@@ -297,99 +357,97 @@ __device__ __forceinline__ void producer(const Args &a, Ctrl &c, uint8_t *smem, 
   __syncwarp();
 }
 
-// One warp, converged, issues every MMA from an elected lane.
+// The MMA warp of stream w, converged, issues from an elected lane: scores of a tile,
+// then its values, then the next tile's scores, in the order that S and P share their
+// columns in.  While one stream's warpgroup has the scores, the other's products run.
 template <typename T>
-__device__ __forceinline__ void mma_issuer(const Args &a, Ctrl &c, uint8_t *smem, uint32_t tmem_any) {
+__device__ __forceinline__ void mma_issuer(const Args &a, Ctrl &c, uint8_t *smem, uint32_t tmem_any, int w) {
   constexpr uint32_t kBase =
       (1u << 4) | (std::is_same<T, __half>::value ? 0u : (1u << 7) | (1u << 10)) | (uint32_t(kTile >> 4) << 24);
   constexpr uint32_t kIdescQK = kBase | (uint32_t(kTile >> 3) << 17);
-  constexpr uint32_t kIdescPV = kBase | (1u << 16) | (uint32_t(64 >> 3) << 17);  // V: N-major, a column at a time
+  constexpr uint32_t kIdescPV = kBase | (1u << 16) | (uint32_t(kDim >> 3) << 17);  // V: N-major
   bool dead = false;
-  uint32_t slot = 0, pieces = 0, p_uses[2] = {0, 0};
-  const uint32_t go = elect_one(), tmem = uniform(tmem_any);
-  const uint32_t qbase = smem_u32(smem + kOffQ), sbase = smem_u32(smem + kOffSlots);
-  const uint32_t negate = a.scale < 0.f ? 1u << 13 : 0u;  // a negative scale turns Q's sign
+  uint32_t pieces = 0, p_uses = 0;
+  const uint32_t go = elect_one(), s_at = uniform(tmem_any + col_s(w)), o_at = uniform(tmem_any + col_o(w));
+  const uint32_t idesc_qk = kIdescQK | (a.scale < 0.f ? 1u << 13 : 0u);  // a negative scale turns Q's sign
+  const uint32_t kd = desc_kmajor(smem_u32(smem + kOffSlots));
+  const uint32_t vd = (smem_u32(smem + kOffSlots) >> 4) | (uint32_t(kCol >> 4) << 16);
   auto done = [&](uint64_t *bar) {
     if (go) commit(bar);
   };
-  auto ready = [&](uint32_t n) {
-    wait(&c.full[n % kSlots], (n / kSlots) & 1u, dead, a.error_flag);
-    fence_after();
-    return uniform(sbase + (n % kSlots) * kCol);
+  // a slot waits for both streams: the one that a tile is for alone says it twice
+  auto free = [&](const Ring::Tile &tile, uint32_t cols, bool alone) {
+    for (uint32_t x = 0; x < cols; ++x) {
+      done(&c.empty[tile.slot(x)]);
+      if (alone) done(&c.empty[tile.slot(x)]);
+    }
   };
-  // Scores of Q tile `qtile` from the K tile at slot k; frees it when `last`.
-  auto qk = [&](int w, int qtile, uint32_t k, bool last) {
-    const uint32_t qd = desc_kmajor(qbase + qtile * kColsQ * kCol);
+  auto qk = [&](const Ring::Tile &tile, int qtile, bool alone) {
+    wait_until(
+        [&] {
+          return mbar_test(&c.full[tile.slot(0)], tile.parity(0)) & mbar_test(&c.full[tile.slot(1)], tile.parity(1)) &
+                 mbar_test(&c.full[tile.slot(2)], tile.parity(2));
+        },
+        dead, a.error_flag);
+    fence_after();
+    const uint32_t qd = uniform(desc_kmajor(smem_u32(smem + kOffQ)) + (qtile * kColsQ * kCol >> 4)), at = uniform(tile.at);
 #pragma unroll
     for (int col = 0; col < kColsQ; ++col) {
-      const uint32_t kd = desc_kmajor(ready(k + col));
+      const uint32_t k0 = kd + ((at + col) % kSlots * kCol >> 4);
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        mma_ss(tmem + col_s(w), qd + ((col * kCol + i * 32) >> 4), kd + (i * 32 >> 4), kIdescQK | negate, col + i > 0, go);
-      if (last) done(&c.empty[(k + col) % kSlots]);
+        mma_ss(s_at, qd + ((col * kCol + i * 32) >> 4), k0 + (i * 32 >> 4), idesc_qk, col + i > 0, go);
     }
+    free(tile, kColsQ, alone);
     done(&c.s_full[w]);
   };
-  auto pv = [&](int w, uint32_t v, bool first, bool last) {
-    wait(&c.p_ready[w], p_uses[w]++ & 1u, dead, a.error_flag);
+  auto pv = [&](const Ring::Tile &tile, bool first, bool alone) {
+    wait_until(
+        [&] {
+          return mbar_test(&c.p_ready[w], p_uses & 1u) & mbar_test(&c.full[tile.slot(0)], tile.parity(0)) &
+                 mbar_test(&c.full[tile.slot(1)], tile.parity(1));
+        },
+        dead, a.error_flag);
+    ++p_uses;
     fence_after();
+    const uint32_t v = uniform(vd + (tile.at * kCol >> 4)), later = uniform(!first);
 #pragma unroll
-    for (int col = 0; col < kColsV; ++col) {
-      const uint32_t vd = desc_kmajor(ready(v + col));
-#pragma unroll
-      for (int i = 0; i < kTile / 16; ++i)
-        mma_ts(tmem + col_o(w) + 64 * col, tmem + col_s(w) + i * 8, vd + (i * 2048 >> 4), kIdescPV, !first || i > 0, go);
-      if (last) done(&c.empty[(v + col) % kSlots]);
-    }
+    for (int i = 0; i < kTile / 16; ++i) mma_ts(o_at, s_at + i * 8, v + (i * 2048 >> 4), kIdescPV, i > 0 ? 1 : later, go);
+    free(tile, kColsV, alone);
   };
-  Walk w;
-  w.init(c);
-  while (w.next(a, c)) {
+  Ring ring;
+  Walk wk;
+  wk.init(c);
+  while (wk.next(a, c)) {
     wait(&c.q_full, pieces++ & 1u, dead, a.error_flag);
-    fence_after();
-    const int n = w.t1 - w.t0;
-    if (w.two()) {
-      // both streams over every tile; a column is free when the second has used it
-      qk(0, 0, slot, false);
-      qk(1, 1, slot, true);
-      slot += kColsQ;
+    const int n = wk.t1 - wk.t0;
+    if (wk.two()) {
+      qk(ring.k(), w, false);
       for (int t = 0; t < n; ++t) {
-        const uint32_t v = slot, k = slot + kColsV;
-        const bool more = t + 1 < n;
-        pv(0, v, t == 0, false);
-        if (more)
-          qk(0, 0, k, false);
-        else
-          done(&c.o_full[0]);
-        pv(1, v, t == 0, true);
-        if (more)
-          qk(1, 1, k, true);
-        else
-          done(&c.o_full[1]);
-        slot += kColsV + (more ? kColsQ : 0);
+        const Ring::Tile v = ring.v();
+        pv(v, t == 0, false);
+        if (t + 1 < n) qk(ring.k(), w, false);
+        if (t + 2 == n || n == 1) done(&c.q_empty);
       }
+      done(&c.o_full[w]);
     } else {
       // stream t & 1 takes tile t
-      qk(0, 0, slot, true);
-      slot += kColsQ;
-      if (n > 1) {
-        qk(1, 0, slot, true);
-        slot += kColsQ;
-      }
+      Ring::Tile k[2] = {ring.k(), Ring::Tile{0, 0}};
+      if (n > 1) k[1] = ring.k();
+      if (w < n) qk(w == 0 ? k[0] : k[1], 0, true);
       for (int t = 0; t < n; ++t) {
-        const int w0 = t & 1;
-        pv(w0, slot, t < 2, true);
-        slot += kColsV;
+        const Ring::Tile v = ring.v();
+        const bool mine = (t & 1) == w;
+        if (mine) pv(v, t < 2, true);
         if (t + 2 < n) {
-          qk(w0, 0, slot, true);
-          slot += kColsQ;
-        } else {
-          done(&c.o_full[w0]);
+          const Ring::Tile next = ring.k();
+          if (mine) qk(next, 0, true);
         }
       }
+      if (w < n) done(&c.o_full[w]);
+      done(&c.q_empty);
     }
-    done(&c.q_empty);
-    w.advance(a);
+    wk.advance(a);
   }
   __syncwarp();
 }
@@ -486,7 +544,8 @@ __device__ __forceinline__ void softmax(const Args &a, Ctrl &c, uint8_t *smem, u
   // (a scale of zero: too small to move a score, and -inf stays -inf)
   const float cl = fmaxf(fabsf(a.scale) * 1.44269504088896341f, 1e-37f);
   bool dead = false;
-  uint32_t s_uses = 0, o_uses[2] = {0, 0}, slot = 0;
+  uint32_t s_uses = 0, o_uses[2] = {0, 0};
+  Ring ring;
   unsigned piece = 0;
   Walk wk;
   wk.init(c);
@@ -502,8 +561,12 @@ __device__ __forceinline__ void softmax(const Args &a, Ctrl &c, uint8_t *smem, u
     const int seen = a.causal ? min(wk.s.past + row + 1, len) : len;
     const int common = a.causal ? min(max(wk.s.past + row0 + 1, 0), len) : len;
     float m = -CUDART_INF_F, l = 0.f;
-    const int step = two ? 1 : 2, tfirst = wk.t0 + (two ? 0 : w);
-    for (int t = tfirst; t < wk.t1; t += step) {
+    const int tfirst = wk.t0 + (two ? 0 : w);
+    for (int i = 0; i < min(lead, n); ++i) ring.k();
+    for (int t = wk.t0; t < wk.t1; ++t) {
+      const Ring::Tile vt = ring.v();
+      if (t + lead < wk.t1) ring.k();
+      if (!two && ((t - wk.t0) & 1) != w) continue;
       const int pos = t * kTile;
       const bool tail = pos + kTile > common;
       wait(&c.s_full[w], s_uses++ & 1u, dead, a.error_flag);
@@ -517,13 +580,10 @@ __device__ __forceinline__ void softmax(const Args &a, Ctrl &c, uint8_t *smem, u
       if (tail) {
         // V rows past the sequence's end are another's and become zeros, so that weights of
         // zero meet finite values; so do non-finite elements that not every row sees
-        const int i = t - wk.t0;
-        const uint32_t v = slot + kColsQ * min(n, i + lead) + kColsV * i;
         const int from = max(common - pos, 0), end = len - pos;
         for (int col = 0; col < kColsV; ++col) {
-          const uint32_t vs = v + col;
-          wait(&c.full[vs % kSlots], (vs / kSlots) & 1u, dead, a.error_flag);
-          uint8_t *base = smem + kOffSlots + vs % kSlots * kCol + tid * 16;
+          wait(&c.full[vt.slot(col)], vt.parity(col), dead, a.error_flag);
+          uint8_t *base = smem + kOffSlots + vt.slot(col) * kCol + tid * 16;
 #pragma unroll 1
           for (int k = min(from, max(end, 0)) / 16; k < 8; ++k) {  // 16 bytes per thread: row = 16 k + tid / 8
             uint4 *at = reinterpret_cast<uint4 *>(base + k * 2048);
@@ -546,7 +606,6 @@ __device__ __forceinline__ void softmax(const Args &a, Ctrl &c, uint8_t *smem, u
       __syncwarp();
       if (lane == 0) arrive(&c.p_ready[w]);
     }
-    slot += (kColsQ + kColsV) * n;
 
     // -------------------------------------------------------- end of piece --
     const bool split = wk.t0 > 0 || wk.t1 < wk.tiles;
@@ -664,10 +723,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     prefetch_tensormap(&vm);
     for (int i = 0; i < kSlots; ++i) {
       mbar_init(&c.full[i], 1);
-      mbar_init(&c.empty[i], 1);
+      mbar_init(&c.empty[i], 2);
     }
     mbar_init(&c.q_full, 1);
-    mbar_init(&c.q_empty, 1);
+    mbar_init(&c.q_empty, 2);
     for (int w = 0; w < 2; ++w) {
       mbar_init(&c.s_full[w], 1);
       mbar_init(&c.p_ready[w], 4);
@@ -697,8 +756,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsIssue));
     if (warp == 8)
       producer(a, c, smem, &qm, &km, &rm, &vm);
-    else if (warp == 9)
-      mma_issuer<T>(a, c, smem, tmem);
+    else if (warp == 9 || warp == 10)
+      mma_issuer<T>(a, c, smem, tmem, warp - 9);
   }
   fence_before();
   __syncthreads();
