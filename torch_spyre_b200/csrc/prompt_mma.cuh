@@ -484,35 +484,42 @@ __device__ __forceinline__ float mask_max(uint32_t (&s)[32], uint32_t vis) {
 }
 
 // Scores of a row's 128 tokens -> weights, in place in TMEM.  kTail: the row sees
-// the first `seen` of them.
+// the first `seen` of them.  Two passes of short loops: laid out whole, the 128 scores
+// of a row are 600 instructions, which come slower than they run.
 template <typename T, bool kTail>
 __device__ __forceinline__ void weigh(uint32_t ts, uint32_t to, int seen, float cl, bool first, bool live, float &m, float &l) {
-  uint32_t s[4][32];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) tmem_ld32(ts + 32 * i, s[i]);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) wait_ld(s[i]);
-  float top[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) top[i] = mask_max<kTail>(s[i], kTail ? low_bits(seen - 32 * i) : ~0u);
-  follow(to, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * cl, first, live, m, l);
+  float mt = -CUDART_INF_F;
+#pragma unroll 1
+  for (int i = 0; i < 128; i += 32) {
+    uint32_t s[32];
+    tmem_ld32(ts + i, s);
+    wait_ld(s);
+    mt = fmaxf(mt, mask_max<kTail>(s, kTail ? low_bits(seen - i) : ~0u));
+  }
+  follow(to, mt * cl, first, live, m, l);
   const float minus = m == -CUDART_INF_F ? 0.f : -m;
-  float2 sum[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    sum[i] = make_float2(0.f, 0.f);
-    uint32_t p[16];
+  float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll 1
+  for (int i = 0; i < 128; i += 32) {
+    uint32_t s[32], p[16];
+    tmem_ld32(ts + i, s);
+    wait_ld(s);
+    const uint32_t vis = kTail ? low_bits(seen - i) : ~0u;
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
-      const float2 x = make_float2(__uint_as_float(s[i][2 * j]), __uint_as_float(s[i][2 * j + 1]));
+      float2 x = make_float2(__uint_as_float(s[2 * j]), __uint_as_float(s[2 * j + 1]));
+      if (kTail) {
+        x.x = vis >> (2 * j) & 1u ? x.x : -CUDART_INF_F;
+        x.y = vis >> (2 * j + 1) & 1u ? x.y : -CUDART_INF_F;
+      }
       const float2 y = fma2(x, make_float2(cl, cl), make_float2(minus, minus));
       const float2 e = make_float2(ex2(y.x), ex2(y.y));
-      sum[i] = add2(sum[i], e);
+      sum[j & 1] = add2(sum[j & 1], e);
       p[j] = pack2(e.x, e.y, T());
     }
-    tmem_st16(ts + 16 * i, p);
+    tmem_st16(ts + i / 2, p);  // (over scores that have been read)
   }
-  const float2 t = add2(add2(sum[0], sum[1]), add2(sum[2], sum[3]));
+  const float2 t = add2(sum[0], sum[1]);
   l += t.x + t.y;
   wait_st();
 }
