@@ -30,7 +30,7 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kThreads = 512, kWarps = kThreads / 32, kMaxCluster = 8, kMaxNodes = 1024;
+constexpr int kThreads = 256, kWarps = kThreads / 32, kMaxCluster = 8, kMaxNodes = 1024;
 
 struct VerifyArgs {
   const int32_t *parents;
@@ -53,6 +53,7 @@ struct Shared {
   // what the CTA's warps do next: the sum over row `row` with c and the `gone` ones, the last one or not
   double c;
   int row, num_gone, last;
+  int found;  // the thread that has the next token
 };
 
 // Weight of an element; what is not a positive number counts as 0.
@@ -63,22 +64,27 @@ __device__ __forceinline__ double weight(float p, float q, double c) {
 }
 
 template <int kVec, typename T>
-__device__ __forceinline__ void load_elements(const T *row, int x, int vocab, float (&f)[kVec]) {
+__device__ __forceinline__ void load_whole(const T *at, float (&f)[kVec]) {
   if constexpr (kVec == 1) {
-    f[0] = x < vocab ? to_float(row[x]) : 0.f;
+    f[0] = to_float(*at);
   } else {
-    if (x + kVec <= vocab) {
-      const uint4 v = __ldg(reinterpret_cast<const uint4 *>(row + x));
-      if constexpr (kVec == 4) {
-        f[0] = __uint_as_float(v.x), f[1] = __uint_as_float(v.y);
-        f[2] = __uint_as_float(v.z), f[3] = __uint_as_float(v.w);
-      } else {
-        unpack8(v, f, T());
-      }
+    const uint4 v = __ldg(reinterpret_cast<const uint4 *>(at));
+    if constexpr (kVec == 4) {
+      f[0] = __uint_as_float(v.x), f[1] = __uint_as_float(v.y);
+      f[2] = __uint_as_float(v.z), f[3] = __uint_as_float(v.w);
     } else {
-#pragma unroll
-      for (int i = 0; i < kVec; ++i) f[i] = x + i < vocab ? to_float(row[x + i]) : 0.f;
+      unpack8(v, f, T());
     }
+  }
+}
+// The same of a row's elements x .. x + kVec - 1, zeros past its end.
+template <int kVec, typename T>
+__device__ __forceinline__ void load_elements(const T *row, int x, int vocab, float (&f)[kVec]) {
+  if (x + kVec <= vocab) {
+    load_whole<kVec>(row + x, f);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) f[i] = x + i < vocab ? to_float(row[x + i]) : 0.f;
   }
 }
 
@@ -96,88 +102,134 @@ __device__ __forceinline__ void weights(const VerifyArgs &a, const Shared &s, in
   }
 }
 
-// This warp's part [x0, x1) of a row: contiguous, ascending with rank and warp.
+// A warp's part [x0, x1) of a row: contiguous, ascending with rank and warp.
 template <int kVec>
-__device__ __forceinline__ void part_of(int vocab, int ranks, int rank, int &x0, int &x1) {
+__device__ __forceinline__ void part_of(int vocab, int ranks, int rank, int warp, int &x0, int &x1) {
   const int step = 32 * kVec, steps = (vocab + step - 1) / step;
   const int each = (steps + ranks * kWarps - 1) / (ranks * kWarps);
-  const int64_t first = int64_t(rank * kWarps + (threadIdx.x >> 5)) * each * step;
+  const int64_t first = int64_t(rank * kWarps + warp) * each * step;
   x0 = static_cast<int>(min(first, int64_t(vocab)));
   x1 = static_cast<int>(min(first + int64_t(each) * step, int64_t(vocab)));
 }
 
-template <typename T, bool kDraft, int kVec>
-__device__ __noinline__ double sum_part(const VerifyArgs &a, const Shared &s, int row, double c, int gone, int x0, int x1) {
+// This lane's share of the sum over [x0, x1).  kKind: 0 nothing rejected (c = 0), 1 one
+// token rejected (c = 1), 2 anything.  The first two decide in fp32, where p > q is exact,
+// which elements have a weight: 9 instructions an element where the third takes 30.
+template <typename T, bool kDraft, int kVec, int kKind>
+__device__ __forceinline__ double sum_lane(const VerifyArgs &a, const Shared &s, int row, double c, int gone, int x0, int x1) {
   const T *p = static_cast<const T *>(a.target) + row * a.target_stride;
   const T *q = kDraft ? static_cast<const T *>(a.draft) + row * a.draft_stride : p;
-  constexpr int kAhead = kVec == 1 ? 8 : 4, kStep = 32 * kVec;
+  constexpr int kAhead = kVec == 1 ? 8 : 16 / kVec, kStep = 32 * kVec;
+  constexpr bool kQ = kDraft && kKind > 0;
   double sum = 0.0;
-  for (int x = x0 + static_cast<int>(threadIdx.x & 31) * kVec; x < x1; x += kAhead * kStep) {
+  auto add = [&](const float (&fp)[kVec], const float (&fq)[kVec], int x) {
+    if constexpr (kKind == 2) {
+      double w[kVec];
+      weights<T, kDraft, kVec>(a, s, row, c, gone, fp, fq, x, w);
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) sum += w[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) {
+        const bool has = fp[i] < CUDART_INF_F && fp[i] > (kKind == 1 ? fq[i] : 0.f) && (kKind == 0 || fq[i] > -CUDART_INF_F);
+        const double w = static_cast<double>(has ? fp[i] : 0.f);
+        sum += kKind == 1 ? w - static_cast<double>(has ? fq[i] : 0.f) : w;
+      }
+    }
+  };
+  const int full = min(x1, a.vocab / kVec * kVec);  // vectors before this are whole
+  int x = x0 + static_cast<int>(threadIdx.x & 31) * kVec, base = x0;
+  for (; base + kAhead * kStep <= full; base += kAhead * kStep, x += kAhead * kStep) {
     float fp[kAhead][kVec], fq[kAhead][kVec];
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
-      const int at = x + k * kStep < x1 ? x + k * kStep : a.vocab;  // (past the part: zeros)
-      load_elements<kVec>(p, at, a.vocab, fp[k]);
-      if (kDraft && c > 0.0) load_elements<kVec>(q, at, a.vocab, fq[k]);
+      load_whole<kVec>(p + x + k * kStep, fp[k]);
+      if (kQ) load_whole<kVec>(q + x + k * kStep, fq[k]);
     }
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k) {
-      double w[kVec];
-      weights<T, kDraft, kVec>(a, s, row, c, gone, fp[k], kDraft ? fq[k] : fp[k], x + k * kStep, w);
-#pragma unroll
-      for (int i = 0; i < kVec; ++i) sum += w[i];
-    }
+    for (int k = 0; k < kAhead; ++k) add(fp[k], kQ ? fq[k] : fp[k], x + k * kStep);
   }
+  for (; x < x1; x += kStep) {
+    float fp[kVec], fq[kVec];
+    load_elements<kVec>(p, x, a.vocab, fp);
+    if (kQ) load_elements<kVec>(q, x, a.vocab, fq);
+    add(fp, kQ ? fq : fp, x);
+  }
+  return sum;
+}
+template <typename T, bool kDraft, int kVec>
+__device__ __noinline__ double sum_part(const VerifyArgs &a, const Shared &s, int row, double c, int gone, int x0, int x1) {
+  double sum;
+  if (gone == 0 && c == 0.0)
+    sum = sum_lane<T, kDraft, kVec, 0>(a, s, row, c, gone, x0, x1);
+  else if (kDraft && c == 1.0)
+    sum = sum_lane<T, kDraft, kVec, 1>(a, s, row, c, gone, x0, x1);
+  else
+    sum = sum_lane<T, kDraft, kVec, 2>(a, s, row, c, gone, x0, x1);
 #pragma unroll
   for (int m = 16; m > 0; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
   return sum;
 }
 
-// The first element of this warp's part whose running sum is above t, or the last with a weight.
+// The first element of [x0, x1), a warp's part, whose running sum is above t, or the last
+// with a weight.  The whole CTA looks, a run of elements to a thread.  (One warp, 32
+// vectors at a time behind one another: 32 steps of a load and a scan, half of the
+// kernel's time at 131072 elements on 4 CTAs.)
 template <typename T, bool kDraft, int kVec>
-__device__ __noinline__ int find_in_part(const VerifyArgs &a, const Shared &s, int row, double c, int gone, int x0, int x1,
-                                         double t) {
+__device__ __noinline__ int find_in_part(const VerifyArgs &a, Shared &s, int row, double c, int gone, int x0, int x1, double t) {
   const T *p = static_cast<const T *>(a.target) + row * a.target_stride;
   const T *q = kDraft ? static_cast<const T *>(a.draft) + row * a.draft_stride : p;
-  const int lane = threadIdx.x & 31;
-  double before = 0.0;
-  int last = -1;
-  for (int x = x0; x < x1; x += 32 * kVec) {
-    const int at = x + lane * kVec;
-    float fp[kVec], fq[kVec];
-    load_elements<kVec>(p, min(at, a.vocab), a.vocab, fp);
-    if (kDraft && c > 0.0) load_elements<kVec>(q, min(at, a.vocab), a.vocab, fq);
-    double w[kVec];
-    weights<T, kDraft, kVec>(a, s, row, c, gone, fp, kDraft ? fq : fp, at, w);
-    double mine = 0.0;
-#pragma unroll
-    for (int i = 0; i < kVec; ++i) {
-      mine += w[i];
-      if (w[i] > 0.0) last = at + i;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int run = ((x1 - x0 + kThreads - 1) / kThreads + kVec - 1) / kVec * kVec;
+  const int first = min(x0 + tid * run, x1), end = min(first + run, x1);
+  auto each = [&](auto use) {
+    for (int x = first; x < end; x += kVec) {
+      float fp[kVec], fq[kVec];
+      load_elements<kVec>(p, x, a.vocab, fp);
+      if (kDraft && c > 0.0) load_elements<kVec>(q, x, a.vocab, fq);
+      double w[kVec];
+      weights<T, kDraft, kVec>(a, s, row, c, gone, fp, kDraft ? fq : fp, x, w);
+      if (!use(x, w)) return;
     }
-    double upto = mine;
+  };
+  double mine = 0.0;
+  each([&](int, const double (&w)[kVec]) {
 #pragma unroll
-    for (int m = 1; m < 32; m <<= 1) {
-      const double y = __shfl_up_sync(0xffffffffu, upto, m);
-      if (lane >= m) upto += y;
-    }
-    double run = before + (upto - mine);
-    int found = -1, tail = -1;
+    for (int i = 0; i < kVec; ++i) mine += w[i];
+    return true;
+  });
+  double upto = mine;
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) {
-      run += w[i];
-      if (w[i] > 0.0) {
-        tail = at + i;
-        if (found < 0 && run > t) found = at + i;
-      }
-    }
-    // (a lane whose sum passes t without one of its elements doing so, by rounding: its last)
-    if (found < 0 && mine > 0.0 && before + upto > t) found = tail;
-    const unsigned hit = __ballot_sync(0xffffffffu, found >= 0);
-    if (hit) return __shfl_sync(0xffffffffu, found, __ffs(hit) - 1);
-    before += __shfl_sync(0xffffffffu, upto, 31);
+  for (int m = 1; m < 32; m <<= 1) {
+    const double y = __shfl_up_sync(0xffffffffu, upto, m);
+    if (lane >= m) upto += y;
   }
-  return __reduce_max_sync(0xffffffffu, last);
+  if (tid == 0) s.found = kThreads, s.last = -1;
+  __syncthreads();  // (warp_sum is read by all before this)
+  if (lane == 31) s.warp_sum[warp] = upto;
+  __syncthreads();
+  double before = 0.0;
+  for (int w = 0; w < warp; ++w) before += s.warp_sum[w];
+  if (mine > 0.0) {
+    atomicMax(&s.last, tid);
+    if (before + upto > t) atomicMin(&s.found, tid);
+  }
+  __syncthreads();
+  if (tid != (s.found < kThreads ? s.found : s.last)) return -1;
+  // (its sum may pass t without one of its elements doing so, by rounding: its last)
+  int found = -1;
+  double sum = before + (upto - mine);
+  each([&](int x, const double (&w)[kVec]) {
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) {
+      if (!(w[i] > 0.0)) continue;
+      sum += w[i];
+      found = x + i;
+      if (sum > t) return false;
+    }
+    return true;
+  });
+  return found;
 }
 
 // The next child of `node` after node i (n: none); the whole warp calls it.
@@ -192,7 +244,7 @@ __device__ __forceinline__ int next_child(const Shared &s, int node, int i, int 
 }
 
 template <typename T, bool kDraft>
-__global__ void __launch_bounds__(kThreads) tree_verify_kernel(const VerifyArgs a) {
+__global__ void __launch_bounds__(kThreads, 4) tree_verify_kernel(const VerifyArgs a) {
   __shared__ Shared s;
   cg::cluster_group cluster = cg::this_cluster();
   const int ranks = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
@@ -240,9 +292,9 @@ __global__ void __launch_bounds__(kThreads) tree_verify_kernel(const VerifyArgs 
 
   int x0, x1;
   if (a.vectors)
-    part_of<16 / sizeof(T)>(a.vocab, ranks, rank, x0, x1);
+    part_of<16 / sizeof(T)>(a.vocab, ranks, rank, warp, x0, x1);
   else
-    part_of<1>(a.vocab, ranks, rank, x0, x1);
+    part_of<1>(a.vocab, ranks, rank, warp, x0, x1);
 
   // warp 0's state: the node reached, the last child tried, path length, c, S, rejected ones
   int cur = 0, at = 0, len = 1, gone = 0;
@@ -347,11 +399,14 @@ __global__ void __launch_bounds__(kThreads) tree_verify_kernel(const VerifyArgs 
         run += x;
         if (mine >= 0 && run > t) break;
       }
-      if (mine == warp) {
-        const int x = a.vectors ? find_in_part<T, kDraft, kVec>(a, s, row, coef, num_gone, x0, x1, t - before)
-                                : find_in_part<T, kDraft, 1>(a, s, row, coef, num_gone, x0, x1, t - before);
-        if (lane == 0) a.next[b] = x;
-      }
+      int y0, y1;  // that warp's part
+      if (a.vectors)
+        part_of<kVec>(a.vocab, ranks, rank, mine, y0, y1);
+      else
+        part_of<1>(a.vocab, ranks, rank, mine, y0, y1);
+      const int x = a.vectors ? find_in_part<T, kDraft, kVec>(a, s, row, coef, num_gone, y0, y1, t - before)
+                              : find_in_part<T, kDraft, 1>(a, s, row, coef, num_gone, y0, y1, t - before);
+      if (x >= 0) a.next[b] = x;
     }
     break;
   }
@@ -416,10 +471,10 @@ extern "C" int b200kv_tree_verify(const int32_t *parents, const int64_t *tokens,
   auto vectors = [&](const void *p, int64_t stride) { return aligned_to(p, 16) && (total_q <= 1 || stride % vec == 0); };
   a.vectors = vectors(target_probs, target_stride) && (!draft_probs || vectors(draft_probs, draft_stride));
   a.error_flag = error_flag;
-  // As many CTAs to a sequence as give every warp a step of the row, two to an SM at most in all.
+  // As many CTAs to a sequence as give every warp a step of the row, four to an SM at most in all.
   const int64_t steps = (vocab + 32 * vec - 1) / (32 * vec);
   int ranks = kMaxCluster;
-  while (ranks > 1 && (batch * ranks > 2 * sms || steps < ranks * kWarps)) ranks /= 2;
+  while (ranks > 1 && (batch * ranks > 4 * sms || steps < ranks * kWarps)) ranks /= 2;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   switch (dtype) {
     case B200KV_F16: return launch<__half>(a, ranks, s);
