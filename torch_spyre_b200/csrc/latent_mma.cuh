@@ -85,32 +85,6 @@ struct Ctrl {
 };
 static_assert(sizeof(Ctrl) <= kOffQ, "control block");
 
-__device__ __forceinline__ bool mbar_test(uint64_t *bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-// Waits, with a limit, until `ready` (which tests barriers side by side) holds.
-template <typename Ready>
-__device__ __forceinline__ void wait_until(Ready ready, bool &dead, int32_t *flag) {
-  if (dead || ready()) return;
-  uint64_t t0 = 0;
-  for (uint32_t i = 1;; ++i) {
-    if (ready()) return;
-    if ((i & 1023u) != 0) continue;
-    const uint64_t now = global_timer_ns();
-    if (t0 == 0) t0 = now;
-    if (now - t0 > kWaitLimitNs) break;
-  }
-  dead = true;
-  if (flag) atomicOr(flag, B200KV_DEVERR_TIMEOUT);
-}
 __device__ __forceinline__ void bar_softmax() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 __device__ __forceinline__ bool any_softmax(bool x) {
   uint32_t r;

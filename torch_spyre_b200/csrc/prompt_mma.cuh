@@ -6,20 +6,30 @@
 // sequences and heads one after the other, form one line that is cut into equal
 // shares, one per CTA; a block cut by a share's end is joined by prompt_join_kernel.
 //
-// Inside a CTA two streams run side by side, each with its own warpgroup, score
+// Inside a CTA two streams run side by side, each with its own eight warps, score
 // buffer S and accumulator O in TMEM: the block's two Q tiles over every token
 // tile, or, with one Q tile, alternate token tiles, whose states are merged when
-// the block ends.  Per tile: S = Q K^T (12 products of 16 elements), the warpgroup
-// (thread = row) masks and exponentiates, P goes back into S's columns in 16 bits,
-// O += P V with P as the TMEM operand.  O is only rescaled when a row's maximum
-// has risen by more than 2^8.
+// the block ends.  Per tile: S = Q K^T (12 products of 16 elements), the warps mask
+// and exponentiate, P goes back into S's columns in 16 bits, O += P V with P as the
+// TMEM operand.  O is only rescaled when a row's maximum has risen by more than 2^8.
+//
+// What bounds it: S and O leave no TMEM for a second S, so a stream's products (1280
+// clocks for a tile) and its softmax follow each other, and a step over a tile of both
+// streams takes 4700 clocks: 2250 for the products with the ways there and back, 2300
+// for the softmax (500 the maximum, 1550 the exponentials, 1024 of them on the
+// special-function units).  The other stream fills the gaps up to the 2560 clocks that
+// the products need.  Four prompts of 1000 to 4100 rows, 16 heads: 233 us; 250 with
+// four warps to a stream, a thread to a row, and products that the streams issue out of
+// turn (two chunks over 8192 tokens, 128 heads: 1440 to 1480 us either way).
+// Exponentials by a polynomial on the FMA units, for a quarter or a half of the
+// elements, and code laid out without loops were as fast or slower.
 //
 // Shared memory holds two Q tiles and eight columns of 64 elements x 128 tokens: a
 // K tile is three (two of the head's, one of the shared part), a V tile two, so
 // that the next tile's come in while this one's are in use.
 //
-// Warps: 0-3 and 4-7 the two softmax warpgroups, 8 the TMA producer, 9 and 10 issue the
-// streams' MMAs.
+// Warps: 0-7 and 8-15 the streams' softmax (a row is in two threads, each with half of a
+// tile's tokens and of O's columns), 16 the TMA producer, 17 and 18 issue the streams' MMAs.
 #pragma once
 
 #include "prompt_attention.h"
@@ -30,8 +40,8 @@ namespace prompt {
 
 using namespace umma;
 
-constexpr int kThreads = 384;
-constexpr int kRegsSoftmax = 208, kRegsIssue = 80;  // a thread, after setmaxnreg (384 threads of 168 at launch)
+constexpr int kThreads = 640;
+constexpr int kRegsSoftmax = 104, kRegsIssue = 64;  // a thread, after setmaxnreg (640 threads of 96 at launch)
 constexpr int kTile = 128;                          // rows of a Q tile, tokens of a K or V tile
 constexpr int kCol = kTile * 128;                   // bytes of a column of 64 elements
 constexpr int kColsQ = 3, kColsV = 2, kSlots = 8;
@@ -59,17 +69,19 @@ struct Start {
 struct Ctrl {
   uint64_t full[kSlots], empty[kSlots];  // (a slot is empty when both streams say so)
   uint64_t q_full, q_empty;
-  uint64_t s_full[2], p_ready[2], o_full[2];
+  uint64_t s_full[2], p_ready[2], o_full[2], turn[2];
   uint32_t tmem;
   int per, total;  // units of a share, of the line
   Start start;
   int scan[32];
   unsigned bad_piece;  // last piece (counted from 1) that met a non-finite value in a V row
-  float2 ml[2][kTile];
+  float top[2][2][kTile];  // streams' rows: the halves' maxima of a tile; sums, when a piece ends
 };
 static_assert(sizeof(Ctrl) <= kOffQ, "control block");
 
-__device__ __forceinline__ void bar_pair() { asm volatile("bar.sync 1, 256;" ::: "memory"); }  // both warpgroups
+__device__ __forceinline__ void bar_all() { asm volatile("bar.sync 1, 512;" ::: "memory"); }  // both streams' softmax
+// The two warps that have a stream's rows 32 q .. 32 q + 31.
+__device__ __forceinline__ void bar_rows(int w, int q) { asm volatile("bar.sync %0, 64;" ::"r"(2 + 4 * w + q) : "memory"); }
 
 // -------------------------------------------------------------------- plan --
 __device__ __forceinline__ Seq load_seq(const Args &a, int b, bool report) {
@@ -260,32 +272,6 @@ struct Ring {
   __device__ __forceinline__ Tile k() { return take<kColsQ>(); }
   __device__ __forceinline__ Tile v() { return take<kColsV>(); }
 };
-__device__ __forceinline__ bool mbar_test(uint64_t *bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-// Waits, with a limit, until `ready` (which tests barriers side by side) holds.
-template <typename Ready>
-__device__ __forceinline__ void wait_until(Ready ready, bool &dead, int32_t *flag) {
-  if (dead || ready()) return;
-  uint64_t t0 = 0;
-  for (uint32_t i = 1;; ++i) {
-    if (ready()) return;
-    if ((i & 1023u) != 0) continue;
-    const uint64_t now = global_timer_ns();
-    if (t0 == 0) t0 = now;
-    if (now - t0 > kWaitLimitNs) break;
-  }
-  dead = true;
-  if (flag) atomicOr(flag, B200KV_DEVERR_TIMEOUT);
-}
 
 // ------------------------------------------------------------------- roles --
 __device__ __forceinline__ void producer(const Args &a, Ctrl &c, uint8_t *smem, const CUtensorMap *qm,
@@ -359,7 +345,8 @@ __device__ __forceinline__ void producer(const Args &a, Ctrl &c, uint8_t *smem, 
 
 // The MMA warp of stream w, converged, issues from an elected lane: scores of a tile,
 // then its values, then the next tile's scores, in the order that S and P share their
-// columns in.  While one stream's warpgroup has the scores, the other's products run.
+// columns in.  While one stream's softmax has the scores, the other's products run: the
+// two issue in turn, since mixed they would both end late.
 template <typename T>
 __device__ __forceinline__ void mma_issuer(const Args &a, Ctrl &c, uint8_t *smem, uint32_t tmem_any, int w) {
   constexpr uint32_t kBase =
@@ -368,6 +355,8 @@ __device__ __forceinline__ void mma_issuer(const Args &a, Ctrl &c, uint8_t *smem
   constexpr uint32_t kIdescPV = kBase | (1u << 16) | (uint32_t(kDim >> 3) << 17);  // V: N-major
   bool dead = false;
   uint32_t pieces = 0, p_uses = 0;
+  uint32_t turns = 0;
+  bool owed = false;  // stream 0: the last group was the other's
   const uint32_t go = elect_one(), s_at = uniform(tmem_any + col_s(w)), o_at = uniform(tmem_any + col_o(w));
   const uint32_t idesc_qk = kIdescQK | (a.scale < 0.f ? 1u << 13 : 0u);  // a negative scale turns Q's sign
   const uint32_t kd = desc_kmajor(smem_u32(smem + kOffSlots));
@@ -382,14 +371,8 @@ __device__ __forceinline__ void mma_issuer(const Args &a, Ctrl &c, uint8_t *smem
       if (alone) done(&c.empty[tile.slot(x)]);
     }
   };
+  auto filled = [&](const Ring::Tile &tile, uint32_t x) { return mbar_test(&c.full[tile.slot(x)], tile.parity(x)); };
   auto qk = [&](const Ring::Tile &tile, int qtile, bool alone) {
-    wait_until(
-        [&] {
-          return mbar_test(&c.full[tile.slot(0)], tile.parity(0)) & mbar_test(&c.full[tile.slot(1)], tile.parity(1)) &
-                 mbar_test(&c.full[tile.slot(2)], tile.parity(2));
-        },
-        dead, a.error_flag);
-    fence_after();
     const uint32_t qd = uniform(desc_kmajor(smem_u32(smem + kOffQ)) + (qtile * kColsQ * kCol >> 4)), at = uniform(tile.at);
 #pragma unroll
     for (int col = 0; col < kColsQ; ++col) {
@@ -402,18 +385,30 @@ __device__ __forceinline__ void mma_issuer(const Args &a, Ctrl &c, uint8_t *smem
     done(&c.s_full[w]);
   };
   auto pv = [&](const Ring::Tile &tile, bool first, bool alone) {
-    wait_until(
-        [&] {
-          return mbar_test(&c.p_ready[w], p_uses & 1u) & mbar_test(&c.full[tile.slot(0)], tile.parity(0)) &
-                 mbar_test(&c.full[tile.slot(1)], tile.parity(1));
-        },
-        dead, a.error_flag);
     ++p_uses;
-    fence_after();
     const uint32_t v = uniform(vd + (tile.at * kCol >> 4)), later = uniform(!first);
 #pragma unroll
-    for (int i = 0; i < kTile / 16; ++i) mma_ts(o_at, s_at + i * 8, v + (i * 2048 >> 4), kIdescPV, i > 0 ? 1 : later, go);
+    for (int i = 0; i < kTile / 16; ++i) mma_ts(o_at, s_at + i / 4 * 64 + i % 4 * 8, v + (i * 2048 >> 4), kIdescPV, i > 0 ? 1 : later, go);
     free(tile, kColsV, alone);
+  };
+  // One group of a stream's products: the values of a tile, whose weights are ready, and
+  // the next tile's scores.  The streams issue groups in turn; `after`: behind one of the
+  // other stream's, `before`: one of the other's follows.
+  auto group = [&](bool after, bool before, const Ring::Tile *v, bool first, const Ring::Tile *k, int qtile, bool alone) {
+    wait_until(
+        [&] {
+          bool ok = !after || mbar_test(&c.turn[w], turns & 1u);
+          if (v) ok = ok & mbar_test(&c.p_ready[w], p_uses & 1u) & filled(*v, 0) & filled(*v, 1);
+          if (k) ok = ok & filled(*k, 0) & filled(*k, 1) & filled(*k, 2);
+          return ok;
+        },
+        dead, a.error_flag);
+    turns += after;
+    fence_after();
+    if (v) pv(*v, first, alone);
+    if (k) qk(*k, qtile, alone);
+    __syncwarp();
+    if (before && go) arrive(&c.turn[w ^ 1]);
   };
   Ring ring;
   Walk wk;
@@ -422,53 +417,41 @@ __device__ __forceinline__ void mma_issuer(const Args &a, Ctrl &c, uint8_t *smem
     wait(&c.q_full, pieces++ & 1u, dead, a.error_flag);
     const int n = wk.t1 - wk.t0;
     if (wk.two()) {
-      qk(ring.k(), w, false);
+      Ring::Tile k = ring.k();
+      group(w == 1 || owed, true, nullptr, false, &k, w, false);
       for (int t = 0; t < n; ++t) {
         const Ring::Tile v = ring.v();
-        pv(v, t == 0, false);
-        if (t + 1 < n) qk(ring.k(), w, false);
+        const bool more = t + 1 < n;
+        if (more) k = ring.k();
+        group(true, true, &v, t == 0, more ? &k : nullptr, w, false);
         if (t + 2 == n || n == 1) done(&c.q_empty);
       }
+      owed = w == 0;
       done(&c.o_full[w]);
     } else {
       // stream t & 1 takes tile t
+      const bool both = n > 1;
       Ring::Tile k[2] = {ring.k(), Ring::Tile{0, 0}};
-      if (n > 1) k[1] = ring.k();
-      if (w < n) qk(w == 0 ? k[0] : k[1], 0, true);
+      if (both) k[1] = ring.k();
+      if (w < n) {
+        group(w == 1 || owed, both, nullptr, false, w == 0 ? &k[0] : &k[1], 0, true);
+        owed = false;
+      }
       for (int t = 0; t < n; ++t) {
         const Ring::Tile v = ring.v();
-        const bool mine = (t & 1) == w;
-        if (mine) pv(v, t < 2, true);
-        if (t + 2 < n) {
-          const Ring::Tile next = ring.k();
-          if (mine) qk(next, 0, true);
-        }
+        const bool mine = (t & 1) == w, more = t + 2 < n;
+        Ring::Tile next{0, 0};
+        if (more) next = ring.k();
+        // (the piece's last group gives the turn to stream 0, which begins the next)
+        if (mine) group(both, both && (t + 1 < n || w == 1), &v, t < 2, more ? &next : nullptr, 0, true);
       }
+      if (both && w == 0) owed = n % 2 == 0;
       if (w < n) done(&c.o_full[w]);
       done(&c.q_empty);
     }
     wk.advance(a);
   }
   __syncwarp();
-}
-
-// Moves the running maximum when a row's has risen far enough, O and l with it.
-__device__ __forceinline__ void follow(uint32_t to, float mt, bool first, bool live, float &m, float &l) {
-  const bool rise = mt > m + (first ? 0.f : kLazyLog2);
-  if (!first && __any_sync(0xffffffffu, rise && live)) {
-    const float keep = rise ? ex2(m - mt) : 1.f;
-    l *= keep;
-#pragma unroll 1
-    for (int i = 0; i < kDim; i += 16) {
-      uint32_t r[16];
-      tmem_ld16(to + i, r);
-      wait_ld(r);
-#pragma unroll
-      for (int j = 0; j < 16; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * keep);
-      tmem_st16(to + i, r);
-    }
-  }
-  if (rise) m = mt;
 }
 
 template <bool kTail>
@@ -483,24 +466,47 @@ __device__ __forceinline__ float mask_max(uint32_t (&s)[32], uint32_t vis) {
   return fmaxf(t, __uint_as_float(s[31]));
 }
 
-// Scores of a row's 128 tokens -> weights, in place in TMEM.  kTail: the row sees
-// the first `seen` of them.  Two passes of short loops: laid out whole, the 128 scores
-// of a row are 600 instructions, which come slower than they run.
+// Scores of a row's 64 tokens of this half -> weights, in place in TMEM.  kTail: the row
+// sees the first `seen` of them.  ts: the row's 128 scores, to: this half of its O.
+//
+// Two passes of short loops: laid out whole, with a row's scores in registers, the code
+// comes slower than it runs.
 template <typename T, bool kTail>
-__device__ __forceinline__ void weigh(uint32_t ts, uint32_t to, int seen, float cl, bool first, bool live, float &m, float &l) {
+__device__ __forceinline__ void weigh(uint32_t ts, uint32_t to, int half, int seen, float cl, bool first, bool live,
+                                      float *top, const float *other, int w, int q, float &m, float &l) {
+  ts += 64 * half;
   float mt = -CUDART_INF_F;
 #pragma unroll 1
-  for (int i = 0; i < 128; i += 32) {
+  for (int i = 0; i < 64; i += 32) {
     uint32_t s[32];
     tmem_ld32(ts + i, s);
     wait_ld(s);
     mt = fmaxf(mt, mask_max<kTail>(s, kTail ? low_bits(seen - i) : ~0u));
   }
-  follow(to, mt * cl, first, live, m, l);
+  mt *= cl;
+  // (the row's maximum is that of both halves)
+  *top = mt;
+  bar_rows(w, q);
+  mt = fmaxf(mt, *other);
+  const bool rise = mt > m + (first ? 0.f : kLazyLog2);
+  if (!first && __any_sync(0xffffffffu, rise && live)) {
+    const float keep = rise ? ex2(m - mt) : 1.f;
+    l *= keep;
+#pragma unroll 1
+    for (int i = 0; i < kDim / 2; i += 16) {
+      uint32_t r[16];
+      tmem_ld16(to + i, r);
+      wait_ld(r);
+#pragma unroll
+      for (int j = 0; j < 16; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * keep);
+      tmem_st16(to + i, r);
+    }
+  }
+  if (rise) m = mt;
   const float minus = m == -CUDART_INF_F ? 0.f : -m;
   float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll 1
-  for (int i = 0; i < 128; i += 32) {
+  for (int i = 0; i < 64; i += 32) {
     uint32_t s[32], p[16];
     tmem_ld32(ts + i, s);
     wait_ld(s);
@@ -542,12 +548,13 @@ __device__ __noinline__ void repair_row(const Args &a, const Seq &s, int head, i
   }
 }
 
-// One softmax warpgroup (w = 0 or 1); thread = row of its Q tile.
+// The softmax of stream w; a thread has a row of its Q tile and a half of a tile's tokens.
 template <typename T>
 __device__ __forceinline__ void softmax(const Args &a, Ctrl &c, uint8_t *smem, uint32_t tmem, int w) {
-  const int tid = threadIdx.x & 127, lane = tid & 31, warp = tid >> 5;
-  const uint32_t quad = tmem + (uint32_t(warp * 32) << 16);
-  const uint32_t ts = quad + col_s(w), to = quad + col_o(w);
+  const int tid = threadIdx.x & 127, lane = tid & 31, q = tid >> 5, half = (threadIdx.x >> 7) & 1;
+  const uint32_t quad = tmem + (uint32_t(q * 32) << 16);
+  const uint32_t ts = quad + col_s(w), to = quad + col_o(w) + half * (kDim / 2);
+  float *top = &c.top[w][half][tid], *other = &c.top[w][half ^ 1][tid];
   // (a scale of zero: too small to move a score, and -inf stays -inf)
   const float cl = fmaxf(fabsf(a.scale) * 1.44269504088896341f, 1e-37f);
   bool dead = false;
@@ -580,31 +587,29 @@ __device__ __forceinline__ void softmax(const Args &a, Ctrl &c, uint8_t *smem, u
       fence_after();
       if (warp_live) {
         if (tail)
-          weigh<T, true>(ts, to, seen - pos, cl, t == tfirst, live, m, l);
+          weigh<T, true>(ts, to, half, seen - pos - 64 * half, cl, t == tfirst, live, top, other, w, q, m, l);
         else
-          weigh<T, false>(ts, to, kTile, cl, t == tfirst, live, m, l);
+          weigh<T, false>(ts, to, half, kTile, cl, t == tfirst, live, top, other, w, q, m, l);
       }
       if (tail) {
         // V rows past the sequence's end are another's and become zeros, so that weights of
         // zero meet finite values; so do non-finite elements that not every row sees
         const int from = max(common - pos, 0), end = len - pos;
-        for (int col = 0; col < kColsV; ++col) {
-          wait(&c.full[vt.slot(col)], vt.parity(col), dead, a.error_flag);
-          uint8_t *base = smem + kOffSlots + vt.slot(col) * kCol + tid * 16;
+        wait(&c.full[vt.slot(half)], vt.parity(half), dead, a.error_flag);
+        uint8_t *base = smem + kOffSlots + vt.slot(half) * kCol + tid * 16;
 #pragma unroll 1
-          for (int k = min(from, max(end, 0)) / 16; k < 8; ++k) {  // 16 bytes per thread: row = 16 k + tid / 8
-            uint4 *at = reinterpret_cast<uint4 *>(base + k * 2048);
-            const int vrow = 16 * k + (tid >> 3);
-            if (vrow >= end) {
-              *at = make_uint4(0, 0, 0, 0);
-            } else if (vrow >= from) {
-              uint4 x = *at;
-              if (!any_non_finite<T>(x)) continue;
-              atomicMax(&c.bad_piece, piece);  // before the element goes: the other stream looks too
-              __threadfence_block();
-              drop_non_finite<T>(x);
-              *at = x;
-            }
+        for (int k = min(from, max(end, 0)) / 16; k < 8; ++k) {  // 16 bytes per thread: row = 16 k + tid / 8
+          uint4 *at = reinterpret_cast<uint4 *>(base + k * 2048);
+          const int vrow = 16 * k + (tid >> 3);
+          if (vrow >= end) {
+            *at = make_uint4(0, 0, 0, 0);
+          } else if (vrow >= from) {
+            uint4 x = *at;
+            if (!any_non_finite<T>(x)) continue;
+            atomicMax(&c.bad_piece, piece);  // before the element goes: the other stream looks too
+            __threadfence_block();
+            drop_non_finite<T>(x);
+            *at = x;
           }
         }
         fence_async_smem();
@@ -621,26 +626,36 @@ __device__ __forceinline__ void softmax(const Args &a, Ctrl &c, uint8_t *smem, u
       wait(&c.o_full[k], o_uses[k]++ & 1u, dead, a.error_flag);
       fence_after();
     };
+    // (once O is full all of the stream's threads have read the last tile's maxima)
     float keep0 = 1.f, keep1 = 0.f;
     const bool both = !two && n > 1;
-    int d0 = 0, d1 = kDim;
+    int d0 = half * (kDim / 2), d1 = d0 + kDim / 2;
     if (two) {
       o_wait(w);
       ++o_uses[1 - w];
+      *top = l;
+      bar_rows(w, q);
+      l += *other;
+      bar_rows(w, q);
     } else {
-      c.ml[w][tid] = make_float2(m, l);
       o_wait(0);
       if (both) o_wait(1);
-      bar_pair();
-      const float2 x = c.ml[0][tid], y = c.ml[1][tid];
-      m = fmaxf(x.x, y.x);
+      bar_all();
+      *top = l;
+      bar_all();
+      const float l0 = c.top[0][0][tid] + c.top[0][1][tid], l1 = c.top[1][0][tid] + c.top[1][1][tid];
+      bar_all();
+      *top = m;
+      bar_all();
+      const float m0 = c.top[0][0][tid], m1 = both ? c.top[1][0][tid] : -CUDART_INF_F;
+      m = fmaxf(m0, m1);
       const float mm = m == -CUDART_INF_F ? 0.f : m;
-      keep0 = ex2(x.x - mm);
-      keep1 = ex2(y.x - mm);
-      l = x.y * keep0;
-      if (both) l = fmaf(y.y, keep1, l);
-      d0 = w * (kDim / 2);
-      d1 = d0 + kDim / 2;
+      keep0 = ex2(m0 - mm);
+      keep1 = ex2(m1 - mm);
+      l = l0 * keep0;
+      if (both) l = fmaf(l1, keep1, l);
+      d0 = (2 * w + half) * (kDim / 4);
+      d1 = d0 + kDim / 4;
     }
     const int64_t orow = static_cast<int64_t>(wk.s.q0 + row) * a.heads + wk.head;
     const float inv = l == 0.f ? 0.f : 1.f / l;
@@ -649,7 +664,7 @@ __device__ __forceinline__ void softmax(const Args &a, Ctrl &c, uint8_t *smem, u
 #pragma unroll 1
       for (int d = d0; d < d1; d += 16) {
         uint32_t r[16];
-        tmem_ld16(two ? to + d : quad + col_o(0) + d, r);
+        tmem_ld16(quad + col_o(two ? w : 0) + d, r);
         wait_ld(r);
         if (!two) {
 #pragma unroll
@@ -688,14 +703,14 @@ __device__ __forceinline__ void softmax(const Args &a, Ctrl &c, uint8_t *smem, u
       repair_row<T>(a, wk.s, wk.head, max(wk.t0 * kTile, hidden), min(wk.t1 * kTile, seen), d0, d1,
                     split ? a.part_o + (static_cast<int64_t>(pslot) * (kDim / 4) * 256 + prow) * 4 : nullptr,
                     static_cast<T *>(a.out) + orow * kDim);
-    if (live && (two || w == 0)) {
+    if (live && half == 0 && (two || w == 0)) {
       if (split)
         a.part_ml[static_cast<int64_t>(pslot) * 256 + prow] = make_float2(m, l);
       else if (a.lse)
         a.lse[orow] = l == 0.f ? -CUDART_INF_F : (m + log2f(l)) * 0.69314718055994530942f;
     }
     // the second share of a split block describes it to the join
-    if (wk.t0 > 0 && w == 0 && tid == 0) {
+    if (wk.t0 > 0 && threadIdx.x == 0) {
       const int first = wk.share_of(0, c.per);
       if (static_cast<int>(blockIdx.x) == first + 1) {
         Join j;
@@ -709,7 +724,10 @@ __device__ __forceinline__ void softmax(const Args &a, Ctrl &c, uint8_t *smem, u
       }
     }
     fence_before();
-    if (!two) bar_pair();  // both have read O and ml before either goes on
+    if (!two)
+      bar_all();  // all have read O before any goes on
+    else
+      bar_rows(w, q);
     fence_after();
     wk.advance(a);
   }
@@ -736,13 +754,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(&c.q_empty, 2);
     for (int w = 0; w < 2; ++w) {
       mbar_init(&c.s_full[w], 1);
-      mbar_init(&c.p_ready[w], 4);
+      mbar_init(&c.p_ready[w], 8);
       mbar_init(&c.o_full[w], 1);
+      mbar_init(&c.turn[w], 1);
     }
     fence_mbar_init();
     c.bad_piece = 0;
   }
-  if (warp == 9) {
+  if (warp == 17) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&c.tmem)),
                  "r"(kTmemCols)
                  : "memory");
@@ -756,19 +775,19 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   fence_after();
   const uint32_t tmem = c.tmem;
-  if (warp < 8) {
+  if (warp < 16) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
-    softmax<T>(a, c, smem, tmem, warp >> 2);
+    softmax<T>(a, c, smem, tmem, warp >> 3);
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsIssue));
-    if (warp == 8)
+    if (warp == 16)
       producer(a, c, smem, &qm, &km, &rm, &vm);
-    else if (warp == 9 || warp == 10)
-      mma_issuer<T>(a, c, smem, tmem, warp - 9);
+    else if (warp < 19)
+      mma_issuer<T>(a, c, smem, tmem, warp - 17);
   }
   fence_before();
   __syncthreads();
-  if (warp == 9) {
+  if (warp == 17) {
     fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
   }

@@ -24,6 +24,32 @@ __device__ __forceinline__ void wait(uint64_t *bar, uint32_t parity, bool &dead,
   dead = true;
   if (flag) atomicOr(flag, B200KV_DEVERR_TIMEOUT);
 }
+__device__ __forceinline__ bool mbar_test(uint64_t *bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+// Waits, with a limit, until `ready` (which tests barriers side by side) holds.
+template <typename Ready>
+__device__ __forceinline__ void wait_until(Ready ready, bool &dead, int32_t *flag) {
+  if (dead || ready()) return;
+  uint64_t t0 = 0;
+  for (uint32_t i = 1;; ++i) {
+    if (ready()) return;
+    if ((i & 1023u) != 0) continue;
+    const uint64_t now = global_timer_ns();
+    if (t0 == 0) t0 = now;
+    if (now - t0 > kWaitLimitNs) break;
+  }
+  dead = true;
+  if (flag) atomicOr(flag, B200KV_DEVERR_TIMEOUT);
+}
 __device__ __forceinline__ void arrive(uint64_t *bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
@@ -143,31 +169,6 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
       : "=f"(d.x), "=f"(d.y)
       : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return d;
-}
-
-// 2^x for two x in [-inf, 2^6], within 2.7e-6 of them (below 2^-125: 2^-125), off the
-// special-function units, which give 16 a clock: x = n + f with n the nearest integer
-// (Cody and Waite's reduction, the sum with 1.5 * 2^23 leaves n in its low bits), a
-// polynomial of degree 4 for 2^f on [-1/2, 1/2], fitted by Remez exchange for the least
-// relative error, and n added to its exponent.
-__device__ __forceinline__ float2 exp2_poly(float2 x) {
-  constexpr float kBig = 12582912.f;
-  x.x = fmaxf(x.x, -125.f), x.y = fmaxf(x.y, -125.f);
-  const float2 t = add2(x, make_float2(kBig, kBig));
-  const float2 n = add2(t, make_float2(-kBig, -kBig));
-  const float2 f = fma2(n, make_float2(-1.f, -1.f), x);
-  float2 p = fma2(f, make_float2(0.009570102f, 0.009570102f), make_float2(0.05591786f, 0.05591786f));
-  p = fma2(p, f, make_float2(0.24024745f, 0.24024745f));
-  p = fma2(p, f, make_float2(0.69312181f, 0.69312181f));
-  p = fma2(p, f, make_float2(0.99999926f, 0.99999926f));
-  return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23)),
-                     __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23)));
-}
-// The largest of three, NaN if one is.
-__device__ __forceinline__ float max3_nan(float a, float b, float c) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-  return r;
 }
 
 // Non-finite elements of a vector.
