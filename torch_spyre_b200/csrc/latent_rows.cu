@@ -11,7 +11,6 @@ namespace b200kv {
 namespace {
 
 constexpr int kRank = B200KV_LATENT_RANK, kRope = B200KV_LATENT_ROPE, kRow = kRank + kRope;
-constexpr int kHeadsPerWarp = 32;
 
 struct StoreArgs {
   const void *latent, *k_rope, *q_rope;
@@ -34,13 +33,16 @@ __device__ __forceinline__ int64_t row_at(int64_t slot, int e) {
 }
 
 // A warp per token: part 0 the latent row (16 elements a lane) and the key, the
-// others 32 heads' queries each.  Four lanes turn a row of 64: lane l has pairs
+// others kHeads heads' queries each.  Four lanes turn a row of 64: lane l has pairs
 // 8l .. 8l + 7, which are two 16-byte vectors in either layout, so that the eight
 // rows of a step need one set of cosines and sines.
 //
-// Bound: bytes.
-template <typename T, int kTurn>  // 0 none, 1 half, 2 interleaved
-__global__ void __launch_bounds__(256) latent_store_kernel(const StoreArgs a) {
+// Bound: bytes, and how many of them are asked for at a time: rows are loaded before
+// the angles, which wait for a position.  16381 tokens, L2 filled with other lines that have to be
+// written back: 16 heads 33.7 us with 16 heads to a warp (3.3 TB/s), 39.8 with 32; 128 heads 121 us with 16,
+// 103 with 32 (5.6 TB/s).
+template <typename T, int kTurn, int kHeads>  // kTurn: 0 none, 1 half, 2 interleaved
+__global__ void __launch_bounds__(256, kHeads == 16 ? 5 : 4) latent_store_kernel(const StoreArgs a) {
   const int lane = threadIdx.x & 31;
   const uint32_t unit = blockIdx.x * 8 + (threadIdx.x >> 5);
   const int t = static_cast<int>(unit / a.parts), part = static_cast<int>(unit % a.parts);
@@ -48,17 +50,19 @@ __global__ void __launch_bounds__(256) latent_store_kernel(const StoreArgs a) {
   const int l = lane & 3;
   const int e0 = kTurn == 2 ? 16 * l : 8 * l, e1 = kTurn == 2 ? e0 + 8 : e0 + 32;  // the lane's vectors
   float2 cs[8];
-  if (kTurn != 0) {
-    const int p_in = __ldg(a.positions + t);
+  const int p_in = kTurn != 0 ? __ldg(a.positions + t) : 0;
+  if (kTurn != 0 && part == 0 && lane == 0 && (p_in < 0 || p_in >= a.max_pos) && a.error_flag)
+    atomicOr(a.error_flag, B200KV_DEVERR_BAD_LEN);
+  auto angles = [&] {  // (called with the rows under way)
+    if (kTurn == 0) return;
     const int64_t p = p_in < 0 ? 0 : (p_in >= a.max_pos ? a.max_pos - 1 : p_in);
-    if (p != p_in && lane == 0 && part == 0 && a.error_flag) atomicOr(a.error_flag, B200KV_DEVERR_BAD_LEN);
     const float4 *row = reinterpret_cast<const float4 *>(a.table + p * (kRope / 2) + 8 * l);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float4 v = __ldg(row + i);
       cs[2 * i] = make_float2(v.x, v.y), cs[2 * i + 1] = make_float2(v.z, v.w);
     }
-  }
+  };
   auto turn = [&](uint4 &u, uint4 &v) {
     if (kTurn == 0) return;
     float x[8], y[8];
@@ -78,19 +82,20 @@ __global__ void __launch_bounds__(256) latent_store_kernel(const StoreArgs a) {
     v = pack8(y, T());
   };
   if (part > 0) {
-    const int h0 = (part - 1) * kHeadsPerWarp + (lane >> 2);
+    const int h0 = (part - 1) * kHeads + (lane >> 2);
     const T *q = static_cast<const T *>(a.q_rope) + t * a.q_sn;
     T *out = static_cast<T *>(a.q_out) + static_cast<int64_t>(t) * a.heads * kRope;
-    uint4 u[4], v[4];
+    uint4 u[kHeads / 8], v[kHeads / 8];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < kHeads / 8; ++i) {
       const int h = h0 + 8 * i;
       if (h >= a.heads) continue;
       u[i] = __ldg(reinterpret_cast<const uint4 *>(q + h * a.q_sh + e0));
       v[i] = __ldg(reinterpret_cast<const uint4 *>(q + h * a.q_sh + e1));
     }
+    angles();
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < kHeads / 8; ++i) {
       const int h = h0 + 8 * i;
       if (h >= a.heads) continue;
       turn(u[i], v[i]);
@@ -113,8 +118,13 @@ __global__ void __launch_bounds__(256) latent_store_kernel(const StoreArgs a) {
     const T *k = static_cast<const T *>(a.k_rope) + t * a.rope_sn;
     ku = __ldg(reinterpret_cast<const uint4 *>(k + e0));
     kv = __ldg(reinterpret_cast<const uint4 *>(k + e1));
+    angles();
   }
   if (a.weight) {
+    uint4 weight[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      weight[i] = __ldg(reinterpret_cast<const uint4 *>(static_cast<const T *>(a.weight) + 256 * i + 8 * lane));
     float f[2][8], sum = 0.f;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -128,7 +138,7 @@ __global__ void __launch_bounds__(256) latent_store_kernel(const StoreArgs a) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       float w[8];
-      unpack8(__ldg(reinterpret_cast<const uint4 *>(static_cast<const T *>(a.weight) + 256 * i + 8 * lane)), w, T());
+      unpack8(weight[i], w, T());
 #pragma unroll
       for (int j = 0; j < 8; ++j) f[i][j] = f[i][j] * by * w[j];
       raw[i] = pack8(f[i], T());
@@ -143,14 +153,21 @@ __global__ void __launch_bounds__(256) latent_store_kernel(const StoreArgs a) {
   }
 }
 
-template <typename T>
+template <typename T, int kHeads>
 void launch(const StoreArgs &a, int turn, unsigned grid, cudaStream_t s) {
   if (turn == 0)
-    latent_store_kernel<T, 0><<<grid, 256, 0, s>>>(a);
+    latent_store_kernel<T, 0, kHeads><<<grid, 256, 0, s>>>(a);
   else if (turn == 1)
-    latent_store_kernel<T, 1><<<grid, 256, 0, s>>>(a);
+    latent_store_kernel<T, 1, kHeads><<<grid, 256, 0, s>>>(a);
   else
-    latent_store_kernel<T, 2><<<grid, 256, 0, s>>>(a);
+    latent_store_kernel<T, 2, kHeads><<<grid, 256, 0, s>>>(a);
+}
+template <typename T>
+void launch(const StoreArgs &a, int turn, int heads, unsigned grid, cudaStream_t s) {
+  if (heads == 16)
+    launch<T, 16>(a, turn, grid, s);
+  else
+    launch<T, 32>(a, turn, grid, s);
 }
 
 }  // namespace
@@ -169,7 +186,8 @@ extern "C" int b200kv_latent_store(const void *latent, int64_t latent_stride_n, 
   B200KV_CHECK_ARG(num_tokens >= 0 && num_q_heads >= 0 && num_q_heads <= 65536 && num_blocks > 0 &&
                        num_blocks < (int64_t{1} << 40),
                    "num_tokens, num_q_heads or num_blocks out of range");
-  const int64_t parts = 1 + (num_q_heads + kHeadsPerWarp - 1) / kHeadsPerWarp;
+  const int per = num_q_heads <= 16 ? 16 : 32;  // heads of a warp
+  const int64_t parts = 1 + (num_q_heads + per - 1) / per;
   B200KV_CHECK_ARG(num_tokens * parts < (int64_t{1} << 31), "num_tokens %lld out of range", (long long)num_tokens);
   B200KV_CHECK_ARG(!table || max_pos > 0, "max_pos must be > 0");
   B200KV_CHECK_ARG(table || num_q_heads == 0, "q_rope is only taken to be turned: a table is needed");
@@ -196,9 +214,9 @@ extern "C" int b200kv_latent_store(const void *latent, int64_t latent_stride_n, 
   const int turn = !table ? 0 : (interleaved ? 2 : 1);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (dtype == B200KV_F16)
-    launch<__half>(a, turn, grid, s);
+    launch<__half>(a, turn, per, grid, s);
   else
-    launch<__nv_bfloat16>(a, turn, grid, s);
+    launch<__nv_bfloat16>(a, turn, per, grid, s);
   B200KV_CUDA_TRY(cudaGetLastError());
   return B200KV_OK;
 }
