@@ -37,12 +37,13 @@ __device__ __forceinline__ int64_t row_at(int64_t slot, int e) {
 // 8l .. 8l + 7, which are two 16-byte vectors in either layout, so that the eight
 // rows of a step need one set of cosines and sines.
 //
-// Bound: bytes, and how many of them are asked for at a time: rows are loaded before
-// the angles, which wait for a position.  16381 tokens, L2 filled with other lines that have to be
-// written back: 16 heads 33.7 us with 16 heads to a warp (3.3 TB/s), 39.8 with 32; 128 heads 121 us with 16,
-// 103 with 32 (5.6 TB/s).
+// Bound: bytes, and how many of them are asked for at a time: all that a warp loads but
+// the angles, which wait for a position, is under way before it waits for any of it
+// (one thing after the other: 32.0 instead of 27.8 us below).  16381 tokens, with an L2
+// full of lines that have to be written back first: 16 heads 27.8 us (3.9 TB/s), 29.9
+// with 32 heads to a warp; 128 heads 97.6 us with 32 (5.9 TB/s), 117 with 16.
 template <typename T, int kTurn, int kHeads>  // kTurn: 0 none, 1 half, 2 interleaved
-__global__ void __launch_bounds__(256, kHeads == 16 ? 5 : 4) latent_store_kernel(const StoreArgs a) {
+__global__ void __launch_bounds__(256, 4) latent_store_kernel(const StoreArgs a) {
   const int lane = threadIdx.x & 31;
   const uint32_t unit = blockIdx.x * 8 + (threadIdx.x >> 5);
   const int t = static_cast<int>(unit / a.parts), part = static_cast<int>(unit % a.parts);
@@ -51,8 +52,6 @@ __global__ void __launch_bounds__(256, kHeads == 16 ? 5 : 4) latent_store_kernel
   const int e0 = kTurn == 2 ? 16 * l : 8 * l, e1 = kTurn == 2 ? e0 + 8 : e0 + 32;  // the lane's vectors
   float2 cs[8];
   const int p_in = kTurn != 0 ? __ldg(a.positions + t) : 0;
-  if (kTurn != 0 && part == 0 && lane == 0 && (p_in < 0 || p_in >= a.max_pos) && a.error_flag)
-    atomicOr(a.error_flag, B200KV_DEVERR_BAD_LEN);
   auto angles = [&] {  // (called with the rows under way)
     if (kTurn == 0) return;
     const int64_t p = p_in < 0 ? 0 : (p_in >= a.max_pos ? a.max_pos - 1 : p_in);
@@ -105,10 +104,6 @@ __global__ void __launch_bounds__(256, kHeads == 16 ? 5 : 4) latent_store_kernel
     return;
   }
   const int64_t slot = __ldg(a.slots + t);
-  if (slot < 0 || slot >= a.num_slots) {
-    if (slot >= 0 && lane == 0 && a.error_flag) atomicOr(a.error_flag, B200KV_DEVERR_BAD_SLOT);
-    return;
-  }
   const T *x = static_cast<const T *>(a.latent) + t * a.latent_sn;
   T *pool = static_cast<T *>(a.pool);
   uint4 raw[2], ku, kv;
@@ -118,8 +113,15 @@ __global__ void __launch_bounds__(256, kHeads == 16 ? 5 : 4) latent_store_kernel
     const T *k = static_cast<const T *>(a.k_rope) + t * a.rope_sn;
     ku = __ldg(reinterpret_cast<const uint4 *>(k + e0));
     kv = __ldg(reinterpret_cast<const uint4 *>(k + e1));
-    angles();
   }
+  // (all of it is under way before the first of it is waited for)
+  if (kTurn != 0 && lane == 0 && (p_in < 0 || p_in >= a.max_pos) && a.error_flag)
+    atomicOr(a.error_flag, B200KV_DEVERR_BAD_LEN);
+  if (slot < 0 || slot >= a.num_slots) {
+    if (slot >= 0 && lane == 0 && a.error_flag) atomicOr(a.error_flag, B200KV_DEVERR_BAD_SLOT);
+    return;
+  }
+  if (lane < 4) angles();
   if (a.weight) {
     uint4 weight[2];
 #pragma unroll
