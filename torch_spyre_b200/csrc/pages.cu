@@ -34,11 +34,9 @@ __device__ __forceinline__ void report(const PageArgs &a, int bit) {
   if (a.error_flag) atomicOr(a.error_flag, bit);
 }
 
-// Committed tokens and new ones of sequence b, clamped to the table.
-__device__ __forceinline__ void lengths(const PageArgs &a, int b, int &ctx, int &nodes, bool &bad) {
+// Committed tokens and new ones (first .. end - 1) of a sequence, clamped to the table.
+__device__ __forceinline__ void lengths(const PageArgs &a, int first, int end, int &ctx, int &nodes, bool &bad) {
   const int cap = a.max_blocks * kPageTokens;
-  ctx = a.lens[b];
-  const int first = a.indptr[b], end = a.indptr[b + 1];
   bad = ctx < 0 || ctx > cap || first < 0 || end < first || end > a.total;
   ctx = min(max(ctx, 0), cap);
   nodes = bad ? 0 : end - first;
@@ -48,9 +46,17 @@ __device__ __forceinline__ void lengths(const PageArgs &a, int b, int &ctx, int 
   }
 }
 
-// The slots of a token, from a table and counts that are complete.  `indptr` and
-// `counts` may be copies in shared memory.
-__device__ __forceinline__ void place(const PageArgs &a, const int32_t *indptr, const int32_t *counts, int t) {
+// Depth of token t in its tree, less than 0 without a bit in its mask.
+__device__ __forceinline__ int depth_of(const PageArgs &a, int t) {
+  int depth = -1;
+  for (int64_t w = 0; w < a.words; ++w) depth += __popcll(__ldg(a.mask + t * a.words + w));
+  return depth;
+}
+
+// The slots of a token, from a table and counts that are complete.  `indptr`,
+// `counts` and `lens` may be copies in shared memory; `depth`: depth_of(t).
+__device__ __forceinline__ void place(const PageArgs &a, const int32_t *indptr, const int32_t *counts, const int32_t *lens,
+                                      int t, int depth) {
   int lo = 0, hi = a.batch - 1;  // the last sequence that begins at or before t
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
@@ -60,13 +66,8 @@ __device__ __forceinline__ void place(const PageArgs &a, const int32_t *indptr, 
   int pos = 0;
   const int first = indptr[lo];
   if (first >= 0 && first <= t && t < indptr[lo + 1] && indptr[lo + 1] <= a.total) {
-    const int cap = a.max_blocks * kPageTokens, ctx = min(max(__ldg(a.lens + lo), 0), cap), i = t - first;
-    int depth = i;
-    if (a.mask) {
-      depth = -1;
-      for (int64_t w = 0; w < a.words; ++w) depth += __popcll(__ldg(a.mask + t * a.words + w));
-      depth = max(depth, 0);
-    }
+    const int cap = a.max_blocks * kPageTokens, ctx = min(max(lens[lo], 0), cap), i = t - first;
+    depth = a.mask ? max(depth, 0) : i;
     pos = ctx + min(depth, INT_MAX - ctx);
     if (i < cap - ctx) {
       const int at = ctx + i, page = at / kPageTokens;
@@ -103,32 +104,38 @@ __device__ __forceinline__ int scan_block(int x, int *warps) {  // inclusive
 // One CTA: thread b has sequence b.  kSlots: places the tokens too.
 template <bool kRelease, bool kSlots>
 __global__ void __launch_bounds__(kThreads) pages_kernel(const PageArgs a) {
-  __shared__ int32_t indptr[kMaxBatch + 1], counts[kMaxBatch];
+  __shared__ int32_t indptr[kMaxBatch + 1], counts[kMaxBatch], lens[kMaxBatch];
   __shared__ int warps[32], moved, sums[kMaxBatch], firsts[kMaxBatch];
-  const int b = threadIdx.x, lane = b & 31;
-  if (b == 0) moved = 0;
+  const int b = threadIdx.x;
+  // all that is read without waiting for something else, first
   const int stack_in = a.free_count[0];
+  int owned_in = 0, len = 0, begin = 0, end = 0;
+  if (b < a.batch) {
+    owned_in = a.counts[b];
+    len = a.lens[b];
+    if (!kRelease) begin = a.indptr[b], end = a.indptr[b + 1];
+  }
+  const int depth = kSlots && a.mask && b < a.total ? depth_of(a, b) : 0;
+  if (b == 0) moved = 0;
   const int stack = min(max(stack_in, 0), a.capacity);
   if (b == 0 && stack != stack_in) report(a, B200KV_DEVERR_BAD_LEN);
   int first = 0, need = 0, owned = 0;
   if (b < a.batch) {
-    const int owned_in = a.counts[b];
     owned = min(max(owned_in, 0), a.max_blocks);
     bool bad;
     if (kRelease) {
-      const int keep = a.lens[b];
-      bad = keep < 0;
-      first = bad ? owned : min(owned, keep / kPageTokens + (keep % kPageTokens != 0));
+      bad = len < 0;
+      first = bad ? owned : min(owned, len / kPageTokens + (len % kPageTokens != 0));
       need = owned - first;
     } else {
-      int ctx, nodes;
-      lengths(a, b, ctx, nodes, bad);
-      first = owned;
-      need = max((ctx + nodes + kPageTokens - 1) / kPageTokens - owned, 0);
       if (kSlots) {
-        indptr[b] = a.indptr[b];
-        if (b == a.batch - 1) indptr[a.batch] = a.indptr[a.batch];
+        indptr[b] = begin, lens[b] = len;
+        if (b == a.batch - 1) indptr[a.batch] = end;
       }
+      int nodes;
+      lengths(a, begin, end, len, nodes, bad);
+      first = owned;
+      need = max((len + nodes + kPageTokens - 1) / kPageTokens - owned, 0);
     }
     if (bad || owned != owned_in) report(a, B200KV_DEVERR_BAD_LEN);
   }
@@ -174,12 +181,12 @@ __global__ void __launch_bounds__(kThreads) pages_kernel(const PageArgs a) {
   __syncthreads();
   if (b == 0) a.free_count[0] = kRelease ? stack + moved : stack - moved;
   if (kSlots)
-    for (int t = b; t < a.total; t += kThreads) place(a, indptr, counts, t);
+    for (int t = b; t < a.total; t += kThreads) place(a, indptr, counts, lens, t, t == b || !a.mask ? depth : depth_of(a, t));
 }
 
 __global__ void __launch_bounds__(256) slots_kernel(const PageArgs a) {
   const int t = blockIdx.x * 256 + threadIdx.x;
-  if (t < a.total) place(a, a.indptr, a.counts, t);
+  if (t < a.total) place(a, a.indptr, a.counts, a.lens, t, a.mask ? depth_of(a, t) : 0);
 }
 
 int check(const int32_t *table, int64_t stride, const int32_t *counts, const int32_t *free_pages, int64_t capacity,
