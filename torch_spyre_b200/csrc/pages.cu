@@ -107,6 +107,7 @@ __global__ void __launch_bounds__(kThreads) pages_kernel(const PageArgs a) {
   __shared__ int32_t indptr[kMaxBatch + 1], counts[kMaxBatch], lens[kMaxBatch];
   __shared__ int warps[32], moved, sums[kMaxBatch], firsts[kMaxBatch];
   const int b = threadIdx.x;
+  if (!kRelease && !kSlots) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // slots_kernel
   // all that is read without waiting for something else, first
   const int stack_in = a.free_count[0];
   int owned_in = 0, len = 0, begin = 0, end = 0;
@@ -186,7 +187,9 @@ __global__ void __launch_bounds__(kThreads) pages_kernel(const PageArgs a) {
 
 __global__ void __launch_bounds__(256) slots_kernel(const PageArgs a) {
   const int t = blockIdx.x * 256 + threadIdx.x;
-  if (t < a.total) place(a, a.indptr, a.counts, a.lens, t, a.mask ? depth_of(a, t) : 0);
+  const int depth = a.mask && t < a.total ? depth_of(a, t) : 0;
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // the table and the counts are pages_kernel's
+  if (t < a.total) place(a, a.indptr, a.counts, a.lens, t, depth);
 }
 
 int check(const int32_t *table, int64_t stride, const int32_t *counts, const int32_t *free_pages, int64_t capacity,
@@ -246,7 +249,16 @@ extern "C" int b200kv_extend_pages(int32_t *block_table, int64_t block_table_str
   } else {
     pages_kernel<false, false><<<1, kThreads, 0, s>>>(a);
     B200KV_CUDA_TRY(cudaGetLastError());
-    slots_kernel<<<static_cast<unsigned>((num_tokens + 255) / 256), 256, 0, s>>>(a);
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>((num_tokens + 255) / 256));
+    cfg.blockDim = dim3(256);
+    cfg.stream = s;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    B200KV_CUDA_TRY(cudaLaunchKernelEx(&cfg, slots_kernel, static_cast<const PageArgs>(a)));
   }
   B200KV_CUDA_TRY(cudaGetLastError());
   return B200KV_OK;
