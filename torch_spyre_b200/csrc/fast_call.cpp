@@ -541,6 +541,26 @@ PyObject *latent_store(PyObject *, PyObject *const *a, Py_ssize_t n) {
   return THPVariable_Wrap(std::move(out));
 }
 
+// latent_load(pool, slots, dtype code, error_flag) -> (latent, k_rope), -1: the pool's dtype
+PyObject *latent_load(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  B200KV_ARGS(4)
+  Call c;
+  const at::Tensor *pool = c.tensor(a[0]), *slots = c.tensor(a[1]);
+  int64_t code = c.integer(a[2]);
+  int32_t *flag = c.flag(a[3]);
+  if (!c.ok || !latent_pool_ok(pool) || slots->dim() != 1 || !vector_of(slots, at::kLong, slots->size(0))) Py_RETURN_NONE;
+  const int32_t own = code_of(pool->scalar_type());
+  if (code < 0) code = own;
+  if (code > 2) Py_RETURN_NONE;
+  const c10::cuda::CUDAGuard guard(c.device);
+  const at::ScalarType type = code == 0 ? at::kHalf : (code == 1 ? at::kBFloat16 : at::kFloat);
+  const at::Tensor out = at::empty({slots->size(0), kRank + kRope}, pool->options().dtype(type));
+  const int st = entries.kv_load(data(pool), own, nullptr, static_cast<const int64_t *>(data(slots)), out.data_ptr(),
+                                 static_cast<int32_t>(code), slots->size(0), kSticks, 64, pool->size(0), flag, stream_of(c));
+  if (st != 0) Py_RETURN_NONE;
+  return pack({out.slice(1, 0, kRank), out.slice(1, kRank)});
+}
+
 // latent_commit(pool, block_table, context_lens, path, path_lens, error_flag)
 PyObject *latent_commit(PyObject *, PyObject *const *a, Py_ssize_t n) {
   B200KV_ARGS(6)
@@ -690,7 +710,8 @@ PyObject *guarded(PyObject *self, PyObject *const *a, Py_ssize_t n) {
 PyMethodDef methods[] = {B200KV_METHOD(rotary),         B200KV_METHOD(kv_store),    B200KV_METHOD(kv_load),
                          B200KV_METHOD(tree_mask),      B200KV_METHOD(tree_attention), B200KV_METHOD(tree_commit),
                          B200KV_METHOD(extend_pages),   B200KV_METHOD(release_pages), B200KV_METHOD(tree_verify),
-                         B200KV_METHOD(latent_store),   B200KV_METHOD(latent_commit), B200KV_METHOD(latent_attention),
+                         B200KV_METHOD(latent_store),   B200KV_METHOD(latent_load), B200KV_METHOD(latent_commit),
+                         B200KV_METHOD(latent_attention),
                          B200KV_METHOD(latent_prompt_attention),
                          B200KV_METHOD(bind),           B200KV_METHOD(set_workspace), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_fast", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

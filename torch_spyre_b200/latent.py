@@ -148,6 +148,10 @@ def latent_load(pool: torch.Tensor, slots: torch.Tensor, dtype: Optional[torch.d
     """(latent [N, 512], k_rope [N, 64]) of the rows at ``slots``, two views of one
     contiguous [N, 576] tensor (dtype fp16, bf16 or fp32; default the pool's).
     Negative slots give rows of zeros."""
+    if not _eager.compiling():
+        pair = _eager.fast.latent_load(pool, slots, -1 if dtype is None else DTYPE_CODES.get(dtype, 99), error_flag)
+        if pair is not None:
+            return pair
     NB = _check_pool(pool)
     rows = kv_load(pool.view(NB, STICKS, 1, PAGE_TOKENS, 64), slots, dtype=dtype, error_flag=error_flag)
     rows = rows.view(-1, RANK + ROPE)
