@@ -71,7 +71,7 @@ int launch(const CUtensorMap &qm, const CUtensorMap &rm, const CUtensorMap &hm, 
   cfg.blockDim = dim3(256);
   cfg.dynamicSmemBytes = 0;
   cfg.numAttrs = 1;
-  B200KV_CUDA_TRY(cudaLaunchKernelEx(&cfg, latent::latent_join_kernel<T>, a));
+  B200KV_CUDA_TRY(cudaLaunchKernelEx(&cfg, pairs ? latent::latent_join_kernel<T, true> : latent::latent_join_kernel<T, false>, a));
   return B200KV_OK;
 }
 

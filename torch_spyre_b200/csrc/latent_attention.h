@@ -39,7 +39,7 @@ struct Args {
   int32_t *error_flag;
   Join *joins;      // [CTAs]
   float2 *part_ml;  // [2 * CTAs][64] (maximum in log2 units, sum)
-  float *part_o;    // [2 * CTAs][64][512]
+  float *part_o;    // [2 * CTAs][64][512], from pairs of SMs [2 * CTAs][128][64][4]
 };
 
 }  // namespace latent

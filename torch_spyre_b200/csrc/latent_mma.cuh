@@ -122,7 +122,7 @@ __device__ __forceinline__ int block_tiles(const Args &a, const Seq &s, int k) {
   return (s.ctx + nodes + kStep - 1) / kStep;
 }
 // The line is cut by cost: a tile counts one, a block's beginning and end kBegin.
-constexpr int kBegin = 4;
+constexpr int kBegin = 3;
 template <int kStep>
 __device__ __forceinline__ int block_units(const Args &a, const Seq &s, int k) {
   return kBegin + block_tiles<kStep>(a, s, k);
@@ -739,26 +739,29 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 // ------------------------------------------------------------------- join --
 // Blocks cut by shares: out = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i over the
-// pieces in order (the same bits every time).  A warp per row and half of its elements,
-// 4 rows a CTA.  The pieces' maxima and sums come first, one to a lane, so that the
-// sums over their elements are loads that wait for nothing, eight under way.
-template <typename T>
+// pieces in order (the same bits every time).  4 rows a CTA, 2 x 4 elements a thread.
+// The pieces' maxima and sums come first, one to a lane, so that the sums over their
+// elements are loads that wait for nothing, eight under way.
+template <typename T, bool kPairs>
 __global__ void __launch_bounds__(256) latent_join_kernel(const __grid_constant__ Args a) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   __shared__ float weight[4][kMaxCtas];
+  __shared__ float2 whole[4];  // rows' maxima and sums
   const Join j = a.joins[blockIdx.x];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int row = blockIdx.y * 4 + (warp >> 1), half = warp & 1;
   const int part = static_cast<int>(blockIdx.x) % a.stride;
-  const int node = row / a.head_box, head = j.head0 + row % a.head_box;
   if (blockIdx.y * 4 / a.head_box >= j.nodes) return;  // (the whole CTA)
-  const bool live = node < j.nodes && head < a.heads;
+  auto live = [&](int r) {
+    const int row = blockIdx.y * 4 + r;
+    return row / a.head_box < j.nodes && j.head0 + row % a.head_box < a.heads;
+  };
   const int pieces = j.last - j.first + 1;
   // the partials of piece i are in slot first_slot + i * step, the first piece's in the odd one
   const int64_t slot0 = 2 * (int64_t{j.first} * a.stride + part), step = 2 * a.stride;
-  float M = -CUDART_INF_F, l = 0.f;
-  if (live) {
+  if (warp < 4 && live(warp)) {
+    const int row = blockIdx.y * 4 + warp;
+    float M = -CUDART_INF_F, l = 0.f;
     for (int i0 = 0; i0 < pieces; i0 += 32) {
       const int i = i0 + lane;
       if (i < pieces) M = fmaxf(M, a.part_ml[(slot0 + i * step + (i == 0)) * kTileRows + row].x);
@@ -768,21 +771,28 @@ __global__ void __launch_bounds__(256) latent_join_kernel(const __grid_constant_
     const float mm = M == -CUDART_INF_F ? 0.f : M;
     for (int i0 = 0; i0 < pieces; i0 += 32) {
       const int i = i0 + lane;
-      float w = 0.f, y = 0.f;
+      float y = 0.f;
       if (i < pieces) {
         const float2 ml = a.part_ml[(slot0 + i * step + (i == 0)) * kTileRows + row];
-        w = exp2f(ml.x - mm);
+        const float w = exp2f(ml.x - mm);
         y = ml.y * w;
-        weight[warp >> 1][i] = w;
+        weight[warp][i] = w;
       }
 #pragma unroll
       for (int x = 16; x > 0; x >>= 1) y += __shfl_xor_sync(0xffffffffu, y, x);
       l += y;
     }
+    if (lane == 0) whole[warp] = make_float2(M, l);
   }
-  __syncthreads();  // (both warps of a row write the same weights)
-  if (!live) return;
-  const float4 *from = reinterpret_cast<const float4 *>(a.part_o) + row * (kRank / 4) + half * (kRank / 8) + lane;
+  __syncthreads();
+  // rows' elements as the kernel before laid them: neighbours in a warp, or for pairs
+  // (there a lane has a row) the 4 rows of 4 elements side by side
+  const int r = kPairs ? threadIdx.x & 3 : warp >> 1;
+  const int e = kPairs ? threadIdx.x >> 2 : (warp & 1) * 64 + lane, e_step = kPairs ? 64 : 32;  // in fours
+  if (!live(r)) return;
+  const int row = blockIdx.y * 4 + r;
+  const float4 *from = reinterpret_cast<const float4 *>(a.part_o) + (kPairs ? e * kTileRows + row : row * (kRank / 4) + e);
+  constexpr int kNext = kPairs ? 64 * kTileRows : 32;
   float4 o[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
   for (int i0 = 0; i0 < pieces; i0 += 4) {
     float4 v[4][2];
@@ -791,12 +801,12 @@ __global__ void __launch_bounds__(256) latent_join_kernel(const __grid_constant_
       const int i = min(i0 + k, pieces - 1);
       const float4 *p = from + (slot0 + i * step + (i == 0)) * (kTileRows * kRank / 4);
       v[k][0] = p[0];
-      v[k][1] = p[32];
+      v[k][1] = p[kNext];
     }
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       if (i0 + k >= pieces) continue;
-      const float w = weight[warp >> 1][i0 + k];
+      const float w = weight[r][i0 + k];
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         o[x].x = fmaf(v[k][x].x, w, o[x].x), o[x].y = fmaf(v[k][x].y, w, o[x].y);
@@ -804,17 +814,18 @@ __global__ void __launch_bounds__(256) latent_join_kernel(const __grid_constant_
       }
     }
   }
-  const int64_t orow = (j.rows0 + j.node0 + node) * a.heads + head;
+  const float M = whole[r].x, l = whole[r].y;
+  const int64_t orow = (j.rows0 + j.node0 + row / a.head_box) * a.heads + j.head0 + row % a.head_box;
   const bool none = l == 0.f;
   const float inv = none ? 0.f : 1.f / l;
-  T *out = static_cast<T *>(a.out) + orow * kRank + half * (kRank / 2) + 4 * lane;
+  T *out = static_cast<T *>(a.out) + orow * kRank + 4 * e;
 #pragma unroll
   for (int x = 0; x < 2; ++x) {
     const uint32_t lo = pack2(none ? 0.f : o[x].x * inv, none ? 0.f : o[x].y * inv, T());
     const uint32_t hi = pack2(none ? 0.f : o[x].z * inv, none ? 0.f : o[x].w * inv, T());
-    *reinterpret_cast<uint2 *>(out + 128 * x) = make_uint2(lo, hi);
+    *reinterpret_cast<uint2 *>(out + 4 * e_step * x) = make_uint2(lo, hi);
   }
-  if (lane == 0 && half == 0 && a.lse) a.lse[orow] = none ? -CUDART_INF_F : (M + log2f(l)) * 0.69314718055994530942f;
+  if (e == 0 && a.lse) a.lse[orow] = none ? -CUDART_INF_F : (M + log2f(l)) * 0.69314718055994530942f;
 }
 
 }  // namespace latent

@@ -31,7 +31,7 @@ namespace pair {
 
 constexpr int kStep = 2 * kPageTokens;  // tokens of a step
 constexpr int kSlots = 4, kSlot = 2 * kPair;
-constexpr int kAhead = 2;  // steps that pages are in L2 before they are loaded
+constexpr int kAhead = 1;  // steps that pages are in L2 before they are loaded (32 sequences: 61.4 us, with 2 64.4, with none 69.5)
 constexpr int kOffQ = 3072;
 constexpr int kOffP = kOffQ + kSticks * kStickTile;  // [2 pages][64 rows][64 tokens]
 constexpr int kOffRope = kOffP + 2 * kStickTile;
@@ -60,9 +60,12 @@ __device__ __forceinline__ uint32_t cluster_rank() {
   asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
   return r;
 }
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
-}
+// (Relaxed: what has to be seen across the pair is fenced, or has been waited for.  A
+// release would wait for the partials' stores as well: 1000 clocks and more.)
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
+// After a wait that ran out: this thread's arrivals at the other CTA's barriers have landed.
+__device__ __forceinline__ void fence_cluster() { asm volatile("fence.acq_rel.cluster;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
 // An arrival at the first CTA's barrier.  What it tells of lies in shared memory, written
 // by the copy engine or behind fence.proxy.async, and is read by the tensor cores: the
 // order of shared memory that arrival and wait give is enough.  (A release and an
@@ -129,7 +132,6 @@ __device__ __forceinline__ void producer(const Args &a, Ctrl &c, uint8_t *smem, 
       const int id = __shfl_sync(0xffffffffu, t / 16 > window ? ids_next : ids, (2 * t + rank) & 31);
       if (lane == 2 && id >= 0) page_ahead(a, id);
     };
-    for (int t = w.t0; t < w.t0 + kAhead; ++t) ahead(t);
     wait(&c.q_empty, (pieces & 1u) ^ 1u, dead, a.error_flag);
     if ((dead = __any_sync(0xffffffffu, dead))) break;
     const Rows rows = rows_of(a, w);
@@ -183,6 +185,7 @@ __device__ __forceinline__ void producer(const Args &a, Ctrl &c, uint8_t *smem, 
       ahead(t + kAhead);
     };
     keys(w.t0);
+    for (int t = w.t0; t < w.t0 + kAhead; ++t) ahead(t);
     for (int t = w.t0; t < w.t1 && !dead; ++t) {
       if (t + 1 < w.t1) keys(t + 1);
       if (dead) break;
@@ -236,6 +239,7 @@ __device__ __forceinline__ void relay(const Args &a, Ctrl &c) {
       if (idle == 1024u) since = now;
       if (__any_sync(0xffffffffu, now - since > kWaitLimitNs)) {  // (the first CTA's waits run out as well)
         if (lane == 0 && a.error_flag) atomicOr(a.error_flag, B200KV_DEVERR_TIMEOUT);
+        fence_cluster();
         break;
       }
     }
@@ -348,6 +352,8 @@ __device__ __forceinline__ void value_issuer(const Args &a, Ctrl &c, uint8_t *sm
     ++pieces;
     w.advance(a);
   }
+  // the last arrivals from the other CTA: not before them may this one end
+  if (pieces > 0) wait(&c.o_empty, (pieces & 1u) ^ 1u, dead, a.error_flag);
   __syncwarp();
 }
 
@@ -457,25 +463,39 @@ __device__ __forceinline__ void softmax(const Args &a, Ctrl &c, uint8_t *smem, u
     // column x of product `part` is element 256 part + 128 half + x of this lane's row
     if (warp_live) {
       const int d0 = 256 * part + 128 * half;
+      // (a lane's own row at a time, a store would touch 32 lines: partials lie by fours of
+      // elements, neighbouring rows side by side, and outputs go through P, which is free)
+      uint8_t *stage = smem + kOffP + warp * 2048;
+      const unsigned lives = __ballot_sync(0xffffffffu, live);
+      const int at = static_cast<int>(orow);  // (rows x heads are less than 2^31)
 #pragma unroll 1
       for (int x = 0; x < 128; x += 32) {
         uint32_t o[32];
         tmem_ld32(quad + col_o(part) + x, o);
         wait_ld(o);
-        if (live && split) {
-          float4 *to = reinterpret_cast<float4 *>(a.part_o + (pslot * kTileRows + row) * kRank + d0 + x);
+        if (split) {
+          if (live) {
+            float4 *to = reinterpret_cast<float4 *>(a.part_o) + (pslot * (kRank / 4) + (d0 + x) / 4) * kTileRows + row;
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            to[j] = make_float4(__uint_as_float(o[4 * j]), __uint_as_float(o[4 * j + 1]), __uint_as_float(o[4 * j + 2]),
-                                __uint_as_float(o[4 * j + 3]));
-        } else if (live) {
-          T *to = static_cast<T *>(a.out) + orow * kRank + d0 + x;
+            for (int j = 0; j < 8; ++j)
+              to[j * kTileRows] = make_float4(__uint_as_float(o[4 * j]), __uint_as_float(o[4 * j + 1]),
+                                              __uint_as_float(o[4 * j + 2]), __uint_as_float(o[4 * j + 3]));
+          }
+        } else {
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             float f[8];
 #pragma unroll
             for (int k = 0; k < 8; ++k) f[k] = inv == 0.f ? 0.f : __uint_as_float(o[8 * j + k]) * inv;
-            *reinterpret_cast<uint4 *>(to + 8 * j) = pack8(f, T());
+            *reinterpret_cast<uint4 *>(stage + lane * 64 + ((j ^ (lane >> 1)) & 3) * 16) = pack8(f, T());
+          }
+          __syncwarp();
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int from = 8 * k + lane / 4, j = lane % 4;
+            const int64_t to = __shfl_sync(0xffffffffu, at, from);
+            const uint4 v = *reinterpret_cast<const uint4 *>(stage + from * 64 + ((j ^ (from >> 1)) & 3) * 16);
+            if (lives >> from & 1u) *reinterpret_cast<uint4 *>(static_cast<T *>(a.out) + to * kRank + d0 + x + 8 * j) = v;
           }
         }
         __syncwarp();
@@ -500,6 +520,7 @@ __device__ __forceinline__ void softmax(const Args &a, Ctrl &c, uint8_t *smem, u
     }
     wk.advance(a);
   }
+  if (dead) fence_cluster();
 }
 
 template <typename T>
@@ -532,8 +553,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(&c.p_free, 1);
     mbar_init(&c.o_full, 1);
     mbar_init(&c.o_empty, 2 * kSoftmaxWarps);
-    fence_mbar_init();
+    fence_mbar_init();  // (of the cluster's scope)
   }
+  __syncwarp();
+  cluster_arrive();
   if (warp == 9) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&c.tmem)),
                  "r"(kTmemCols)
@@ -546,7 +569,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   make_plan<T, kStep>(a, c.plan);
   fence_before();
   __syncthreads();
-  cluster_sync();
+  cluster_wait();  // both CTAs' barriers are there
   fence_after();
   const uint32_t tmem = c.tmem;
   const bool leads = cluster_rank() == 0;
@@ -563,7 +586,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncwarp();
   fence_before();
   __syncthreads();
-  cluster_sync();  // neither CTA ends while the other's operands or barriers may be used
+  cluster_arrive();  // neither CTA ends while the other's operands or barriers may be used
+  cluster_wait();
   if (warp == 9) {
     fence_after();
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
