@@ -13,16 +13,16 @@
 namespace b200kv {
 namespace {
 
-// Rows of `width` elements of `heads` heads and `rows` tokens, a box of 64 elements x 128 tokens of a head.
+// Rows of `width` elements of `heads` heads and `rows` tokens, a box of 64 elements x `box_rows` tokens of a head.
 int encode(CUtensorMap *map, CUtensorMapDataType type, const void *base, int64_t width, int64_t heads, int64_t rows,
-           int64_t stride_h, int64_t stride_t) {
+           int64_t stride_h, int64_t stride_t, int box_rows) {
   EncodeTiledFn enc = encode_tiled_fn();
   if (!enc) return set_error(B200KV_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
   // a dimension of one element may have any stride
   const int64_t sh = heads == 1 ? width : stride_h, st = rows == 1 ? heads * width : stride_t;
   const cuuint64_t dims[3] = {static_cast<cuuint64_t>(width), static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(rows)};
   const cuuint64_t strides[2] = {static_cast<cuuint64_t>(sh * 2), static_cast<cuuint64_t>(st * 2)};
-  const cuuint32_t box[3] = {64, 1, prompt::kTile}, estr[3] = {1, 1, 1};
+  const cuuint32_t box[3] = {64, 1, static_cast<cuuint32_t>(box_rows)}, estr[3] = {1, 1, 1};
   const CUresult r = enc(map, type, 3, const_cast<void *>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return set_error(B200KV_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", static_cast<int>(r));
@@ -69,9 +69,9 @@ extern "C" int b200kv_latent_prompt_attention(const void *q, int64_t q_stride_t,
                    "batch, total_q * num_heads or total_kv out of range");
   if (batch > 1024) return set_error(B200KV_ERR_UNSUPPORTED, "batch %lld > 1024 unsupported", (long long)batch);
   B200KV_CHECK_ARG(std::isfinite(scale), "scale must be finite");
-  // the kernel counts its units of work in 31 bits: 13 + 4 a tile for a block of 256 rows, at most
-  const int64_t blocks = total_q / 256 + batch, tiles = total_kv / 128 + 1;
-  if ((blocks * 17 + 4 * (total_q / 256 * tiles + tiles + batch)) * num_heads >= (int64_t{1} << 31))
+  // the kernel counts its units of work in 31 bits: kBegin + 4 a tile for a block of 256 rows, at most
+  const int64_t blocks = total_q / 256 + batch, tiles = total_kv / prompt::kTok + 1;
+  if ((blocks * (prompt::kBegin2 + 4) + 4 * (total_q / 256 * tiles + tiles + batch)) * num_heads >= (int64_t{1} << 31))
     return set_error(B200KV_ERR_UNSUPPORTED, "2^31 or more steps of rows and tokens");
   if (total_q == 0) return B200KV_OK;
   B200KV_CHECK_ARG(batch > 0, "rows without a sequence");
@@ -110,15 +110,17 @@ extern "C" int b200kv_latent_prompt_attention(const void *q, int64_t q_stride_t,
   const bool none = total_kv == 0;
   const int64_t rows = none ? total_q : total_kv;
   CUtensorMap qm, km, rm, vm;
-  st = encode(&qm, type, q, prompt::kNope + prompt::kRope, num_heads, total_q, q_stride_h, q_stride_t);
+  st = encode(&qm, type, q, prompt::kNope + prompt::kRope, num_heads, total_q, q_stride_h, q_stride_t,
+              prompt::kTile);
   if (st == B200KV_OK)
     st = encode(&km, type, none ? q : k_nope, prompt::kNope, num_heads, rows, none ? q_stride_h : k_stride_h,
-                none ? q_stride_t : k_stride_t);
+                none ? q_stride_t : k_stride_t, prompt::kTok);
   if (st == B200KV_OK)
-    st = encode(&rm, type, none ? q : k_rope, prompt::kRope, 1, rows, 0, none ? q_stride_t : k_rope_stride_t);
+    st = encode(&rm, type, none ? q : k_rope, prompt::kRope, 1, rows, 0, none ? q_stride_t : k_rope_stride_t,
+                prompt::kTok);
   if (st == B200KV_OK)
     st = encode(&vm, type, none ? q : v, prompt::kDim, num_heads, rows, none ? q_stride_h : v_stride_h,
-                none ? q_stride_t : v_stride_t);
+                none ? q_stride_t : v_stride_t, prompt::kTok);
   if (st != B200KV_OK) return st;
   const int ctas = sms < prompt::kMaxCtas ? sms : prompt::kMaxCtas;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);

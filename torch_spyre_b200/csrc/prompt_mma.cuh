@@ -2,31 +2,35 @@
 // heads with keys of 128 own and 64 shared elements, values of 128.
 //
 // The rows of a sequence and head are cut into Q tiles of 128, two of which form a
-// block; a block's tokens are cut into tiles of 128.  The blocks' tiles, all
+// block; a block's tokens are cut into tiles of 80.  The blocks' tiles, all
 // sequences and heads one after the other, form one line that is cut into equal
 // shares, one per CTA; a block cut by a share's end is joined by prompt_join_kernel.
 //
-// Inside a CTA two streams run side by side, each with its own eight warps, score
-// buffer S and accumulator O in TMEM: the block's two Q tiles over every token
+// Inside a CTA two streams run side by side, each with its own eight warps, scores S,
+// weights P and accumulator O in TMEM: the block's two Q tiles over every token
 // tile, or, with one Q tile, alternate token tiles, whose states are merged when
-// the block ends.  Per tile: S = Q K^T (12 products of 16 elements), the warps mask
-// and exponentiate, P goes back into S's columns in 16 bits, O += P V with P as the
-// TMEM operand.  O is only rescaled when a row's maximum has risen by more than 2^8.
+// the block ends.  Per tile: S = Q K^T (12 products of 16 elements), the warps take S
+// into registers (then the next tile's S may come), mask and exponentiate, P goes to
+// TMEM in 16 bits, O += P V with P as the TMEM operand.  O is only rescaled when a
+// row's maximum has risen by more than 2^8.
 //
-// What bounds it: S and O leave no TMEM for a second S, so a stream's products (1280
-// clocks for a tile) and its softmax follow each other, and a step over a tile of both
-// streams takes 4700 clocks: 2250 for the products with the ways there and back, 2300
-// for the softmax (500 the maximum, 1550 the exponentials, 1024 of them on the
-// special-function units).  The other stream fills the gaps up to the 2560 clocks that
-// the products need.  Four prompts of 1000 to 4100 rows, 16 heads: 233 us; 250 with
-// four warps to a stream, a thread to a row, and products that the streams issue out of
-// turn (two chunks over 8192 tokens, 128 heads: 1440 to 1480 us either way).
+// 80 tokens, since a stream has 256 of TMEM's columns: 80 S, 40 P, 128 O.  (Tiles of 128 with P in
+// S's place have 25 % fewer clocks of products, 2560 for 128 tokens and both streams, but a
+// stream's products and softmax then follow one another: 233 us instead of 225 below, 1440
+// instead of 1345.)
+//
+// What bounds it: the softmax warps, which are never idle: of 2700 clocks for a tile of both
+// streams 200 to take S, 200 for the rows' maxima, 1300 to 1450 for exponentials (1280 of
+// the special-function units', which both streams use at once; in turns they are no
+// faster), 300 to write P, the rest waits and arrivals; the products take 1900.  Then the
+// power limit: in long runs the clock falls from 1965 to some 1600 MHz.  Four prompts of up to 4096 rows, 16
+// heads: 225 us; two chunks of 777 to 1024 rows over 4001 to 8000 tokens, 128 heads: 1345.
 // Exponentials by a polynomial on the FMA units, for a quarter or a half of the
-// elements, and code laid out without loops were as fast or slower.
+// elements, waits that sleep, and code laid out without loops were as fast or slower.
 //
-// Shared memory holds two Q tiles and eight columns of 64 elements x 128 tokens: a
+// Shared memory holds two Q tiles and twelve columns of 64 elements x 80 tokens: a
 // K tile is three (two of the head's, one of the shared part), a V tile two, so
-// that the next tile's come in while this one's are in use.
+// that the next tiles' come in while this one's are in use.
 //
 // Warps: 0-7 and 8-15 the streams' softmax (a row is in two threads, each with half of a
 // tile's tokens and of O's columns), 16 the TMA producer, 17 and 18 issue the streams' MMAs.
@@ -42,11 +46,13 @@ using namespace umma;
 
 constexpr int kThreads = 640;
 constexpr int kRegsSoftmax = 104, kRegsIssue = 64;  // a thread, after setmaxnreg (640 threads of 96 at launch)
-constexpr int kTile = 128;                          // rows of a Q tile, tokens of a K or V tile
-constexpr int kCol = kTile * 128;                   // bytes of a column of 64 elements
-constexpr int kColsQ = 3, kColsV = 2, kSlots = 8;
+constexpr int kTile = 128;                          // rows of a Q tile
+constexpr int kTok = 80, kHalf = kTok / 2;          // tokens of a K or V tile
+constexpr int kColQ = kTile * 128, kCol = kTok * 128;  // bytes of a column of 64 elements
+constexpr int kColsQ = 3, kColsV = 2, kSlots = 12;
+constexpr int kLead = 2;                            // tiles that keys are ahead of values
 constexpr int kOffQ = 3072;
-constexpr int kOffSlots = kOffQ + 2 * kColsQ * kCol;
+constexpr int kOffSlots = kOffQ + 2 * kColsQ * kColQ;
 constexpr int kSmem = kOffSlots + kSlots * kCol;
 constexpr float kLazyLog2 = 8.f;
 static_assert(kSmem <= 227 * 1024, "shared memory per CTA");
@@ -54,6 +60,7 @@ static_assert(kSmem <= 227 * 1024, "shared memory per CTA");
 // TMEM columns
 constexpr uint32_t kTmemCols = 512;
 __device__ __forceinline__ uint32_t col_s(int w) { return uint32_t(w) * 128u; }
+__device__ __forceinline__ uint32_t col_p(int w) { return uint32_t(w) * 128u + kTok; }
 __device__ __forceinline__ uint32_t col_o(int w) { return 256u + uint32_t(w) * 128u; }
 
 struct Seq {
@@ -69,7 +76,7 @@ struct Start {
 struct Ctrl {
   uint64_t full[kSlots], empty[kSlots];  // (a slot is empty when both streams say so)
   uint64_t q_full, q_empty;
-  uint64_t s_full[2], p_ready[2], o_full[2], turn[2];
+  uint64_t s_full[2], s_free[2], p_ready[2], p_free[2], o_full[2];
   uint32_t tmem;
   int per, total;  // units of a share, of the line
   Start start;
@@ -82,6 +89,15 @@ static_assert(sizeof(Ctrl) <= kOffQ, "control block");
 __device__ __forceinline__ void bar_all() { asm volatile("bar.sync 1, 512;" ::: "memory"); }  // both streams' softmax
 // The two warps that have a stream's rows 32 q .. 32 q + 31.
 __device__ __forceinline__ void bar_rows(int w, int q) { asm volatile("bar.sync %0, 64;" ::"r"(2 + 4 * w + q) : "memory"); }
+
+__device__ __forceinline__ bool any_rows(int w, int q, bool x) {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, %2, 64, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+               : "=r"(r)
+               : "r"(uint32_t(x)), "r"(2 + 4 * w + q)
+               : "memory");
+  return r != 0;
+}
 
 // -------------------------------------------------------------------- plan --
 __device__ __forceinline__ Seq load_seq(const Args &a, int b, bool report) {
@@ -104,13 +120,14 @@ __device__ __forceinline__ Seq load_seq(const Args &a, int b, bool report) {
 // Token tiles of block k: what its last row sees (one at least, which may be masked whole).
 __device__ __forceinline__ int block_tiles(const Args &a, const Seq &s, int k) {
   const int seen = a.causal ? s.past + min(s.rows, (k + 1) * 2 * kTile) : s.len;
-  return max((seen + kTile - 1) / kTile, 1);
+  return max((seen + kTok - 1) / kTok, 1);
 }
 // The line is cut by cost: a step over a token tile counts 2 with one Q tile and 4
-// with two, a block's beginning and end 9 and 13.
+// with two, a block's beginning and end kBegin[0] and [1].
+constexpr int kBegin1 = 18, kBegin2 = 26;
 __device__ __forceinline__ bool two_tiles(const Seq &s, int k) { return s.rows - k * 2 * kTile > kTile; }
 __device__ __forceinline__ int step_units(const Seq &s, int k) { return two_tiles(s, k) ? 4 : 2; }
-__device__ __forceinline__ int begin_units(const Seq &s, int k) { return two_tiles(s, k) ? 13 : 9; }
+__device__ __forceinline__ int begin_units(const Seq &s, int k) { return two_tiles(s, k) ? kBegin2 : kBegin1; }
 __device__ __forceinline__ int block_units(const Args &a, const Seq &s, int k) {
   return begin_units(s, k) + step_units(s, k) * block_tiles(a, s, k);
 }
@@ -299,7 +316,7 @@ __device__ __forceinline__ void producer(const Args &a, Ctrl &c, uint8_t *smem, 
         const uint32_t s = tile.slot(lane);
         mbar_arrive_expect_tx(&c.full[s], kCol);
         tma_3d(smem + kOffSlots + s * kCol, lane == 2 ? rm : map, &c.full[s], lane == 1 ? 64 : 0, lane == 2 ? 0 : w.head,
-               w.s.kv0 + t * kTile);
+               w.s.kv0 + t * kTok);
       }
       __syncwarp();
       for (uint32_t x = 0; x < cols; ++x) {
@@ -308,23 +325,21 @@ __device__ __forceinline__ void producer(const Args &a, Ctrl &c, uint8_t *smem, 
         last = (last & ~bit) | (tile.parities & bit);
       }
     };
-    // K leads V by one tile per stream that needs it
-    const int lead = two ? 1 : 2;
-    for (int t = w.t0; t < min(w.t0 + lead, w.t1) && !dead; ++t) issue(ring.k(), kColsQ, km, t);
+    for (int t = w.t0; t < min(w.t0 + kLead, w.t1) && !dead; ++t) issue(ring.k(), kColsQ, km, t);
     // (the first keys may come before the piece before is done with Q)
     if (dead) break;
     wait(&c.q_empty, (pieces & 1u) ^ 1u, dead, a.error_flag);
     if ((dead = __any_sync(0xffffffffu, dead))) break;
     const int n = (two ? 2 : 1) * kColsQ;
-    if (lane == 0) mbar_arrive_expect_tx(&c.q_full, uint32_t(n) * kCol);
+    if (lane == 0) mbar_arrive_expect_tx(&c.q_full, uint32_t(n) * kColQ);
     __syncwarp();
     if (lane < n)
-      tma_3d(smem + kOffQ + lane * kCol, qm, &c.q_full, lane % kColsQ * 64, w.head,
+      tma_3d(smem + kOffQ + lane * kColQ, qm, &c.q_full, lane % kColsQ * 64, w.head,
              w.s.q0 + (2 * w.block + lane / kColsQ) * kTile);
     ++pieces;
     for (int t = w.t0; t < w.t1 && !dead; ++t) {
       issue(ring.v(), kColsV, vm, t);
-      if (t + lead < w.t1 && !dead) issue(ring.k(), kColsQ, km, t + lead);
+      if (t + kLead < w.t1 && !dead) issue(ring.k(), kColsQ, km, t + kLead);
     }
     if (dead) break;
     w.advance(a);
@@ -343,21 +358,18 @@ __device__ __forceinline__ void producer(const Args &a, Ctrl &c, uint8_t *smem, 
   __syncwarp();
 }
 
-// The MMA warp of stream w, converged, issues from an elected lane: scores of a tile,
-// then its values, then the next tile's scores, in the order that S and P share their
-// columns in.  While one stream's softmax has the scores, the other's products run: the
-// two issue in turn, since mixed they would both end late.
+// The MMA warp of stream w, converged, issues from an elected lane: the next tile's
+// scores, which the softmax makes room for when it has taken this one's, then this one's
+// values, when its weights are there.
 template <typename T>
 __device__ __forceinline__ void mma_issuer(const Args &a, Ctrl &c, uint8_t *smem, uint32_t tmem_any, int w) {
   constexpr uint32_t kBase =
       (1u << 4) | (std::is_same<T, __half>::value ? 0u : (1u << 7) | (1u << 10)) | (uint32_t(kTile >> 4) << 24);
-  constexpr uint32_t kIdescQK = kBase | (uint32_t(kTile >> 3) << 17);
+  constexpr uint32_t kIdescQK = kBase | (uint32_t(kTok >> 3) << 17);
   constexpr uint32_t kIdescPV = kBase | (1u << 16) | (uint32_t(kDim >> 3) << 17);  // V: N-major
   bool dead = false;
-  uint32_t pieces = 0, p_uses = 0;
-  uint32_t turns = 0;
-  bool owed = false;  // stream 0: the last group was the other's
-  const uint32_t go = elect_one(), s_at = uniform(tmem_any + col_s(w)), o_at = uniform(tmem_any + col_o(w));
+  uint32_t pieces = 0, s_uses = 0, p_uses = 0;
+  const uint32_t go = elect_one(), s_at = uniform(tmem_any + col_s(w)), p_at = uniform(tmem_any + col_p(w)), o_at = uniform(tmem_any + col_o(w));
   const uint32_t idesc_qk = kIdescQK | (a.scale < 0.f ? 1u << 13 : 0u);  // a negative scale turns Q's sign
   const uint32_t kd = desc_kmajor(smem_u32(smem + kOffSlots));
   const uint32_t vd = (smem_u32(smem + kOffSlots) >> 4) | (uint32_t(kCol >> 4) << 16);
@@ -372,43 +384,36 @@ __device__ __forceinline__ void mma_issuer(const Args &a, Ctrl &c, uint8_t *smem
     }
   };
   auto filled = [&](const Ring::Tile &tile, uint32_t x) { return mbar_test(&c.full[tile.slot(x)], tile.parity(x)); };
+  // scores, once the softmax has taken those before out of their columns
   auto qk = [&](const Ring::Tile &tile, int qtile, bool alone) {
-    const uint32_t qd = uniform(desc_kmajor(smem_u32(smem + kOffQ)) + (qtile * kColsQ * kCol >> 4)), at = uniform(tile.at);
+    wait_until(
+        [&] {
+          const bool ok = filled(tile, 0) & filled(tile, 1) & filled(tile, 2);
+          return ok & (s_uses == 0 || mbar_test(&c.s_free[w], (s_uses - 1) & 1u));
+        },
+        dead, a.error_flag);
+    ++s_uses;
+    fence_after();
+    const uint32_t qd = uniform(desc_kmajor(smem_u32(smem + kOffQ)) + (qtile * kColsQ * kColQ >> 4)), at = uniform(tile.at);
 #pragma unroll
     for (int col = 0; col < kColsQ; ++col) {
       const uint32_t k0 = kd + ((at + col) % kSlots * kCol >> 4);
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        mma_ss(s_at, qd + ((col * kCol + i * 32) >> 4), k0 + (i * 32 >> 4), idesc_qk, col + i > 0, go);
+        mma_ss(s_at, qd + ((col * kColQ + i * 32) >> 4), k0 + (i * 32 >> 4), idesc_qk, col + i > 0, go);
     }
     free(tile, kColsQ, alone);
     done(&c.s_full[w]);
   };
   auto pv = [&](const Ring::Tile &tile, bool first, bool alone) {
+    wait_until([&] { return mbar_test(&c.p_ready[w], p_uses & 1u) & filled(tile, 0) & filled(tile, 1); }, dead, a.error_flag);
     ++p_uses;
+    fence_after();
     const uint32_t v = uniform(vd + (tile.at * kCol >> 4)), later = uniform(!first);
 #pragma unroll
-    for (int i = 0; i < kTile / 16; ++i) mma_ts(o_at, s_at + i / 4 * 64 + i % 4 * 8, v + (i * 2048 >> 4), kIdescPV, i > 0 ? 1 : later, go);
+    for (int i = 0; i < kTok / 16; ++i) mma_ts(o_at, p_at + i * 8, v + (i * 2048 >> 4), kIdescPV, i > 0 ? 1 : later, go);
     free(tile, kColsV, alone);
-  };
-  // One group of a stream's products: the values of a tile, whose weights are ready, and
-  // the next tile's scores.  The streams issue groups in turn; `after`: behind one of the
-  // other stream's, `before`: one of the other's follows.
-  auto group = [&](bool after, bool before, const Ring::Tile *v, bool first, const Ring::Tile *k, int qtile, bool alone) {
-    wait_until(
-        [&] {
-          bool ok = !after || mbar_test(&c.turn[w], turns & 1u);
-          if (v) ok = ok & mbar_test(&c.p_ready[w], p_uses & 1u) & filled(*v, 0) & filled(*v, 1);
-          if (k) ok = ok & filled(*k, 0) & filled(*k, 1) & filled(*k, 2);
-          return ok;
-        },
-        dead, a.error_flag);
-    turns += after;
-    fence_after();
-    if (v) pv(*v, first, alone);
-    if (k) qk(*k, qtile, alone);
-    __syncwarp();
-    if (before && go) arrive(&c.turn[w ^ 1]);
+    done(&c.p_free[w]);
   };
   Ring ring;
   Walk wk;
@@ -416,36 +421,30 @@ __device__ __forceinline__ void mma_issuer(const Args &a, Ctrl &c, uint8_t *smem
   while (wk.next(a, c)) {
     wait(&c.q_full, pieces++ & 1u, dead, a.error_flag);
     const int n = wk.t1 - wk.t0;
+    Ring::Tile k[2] = {ring.k(), Ring::Tile{0, 0}};
+    if (n > 1) k[1] = ring.k();
     if (wk.two()) {
-      Ring::Tile k = ring.k();
-      group(w == 1 || owed, true, nullptr, false, &k, w, false);
+      qk(k[0], w, false);
       for (int t = 0; t < n; ++t) {
         const Ring::Tile v = ring.v();
-        const bool more = t + 1 < n;
-        if (more) k = ring.k();
-        group(true, true, &v, t == 0, more ? &k : nullptr, w, false);
+        if (t + 1 < n) qk(k[1], w, false);
         if (t + 2 == n || n == 1) done(&c.q_empty);
+        if (t + 2 < n) k[1] = ring.k();
+        pv(v, t == 0, false);
       }
-      owed = w == 0;
       done(&c.o_full[w]);
     } else {
       // stream t & 1 takes tile t
-      const bool both = n > 1;
-      Ring::Tile k[2] = {ring.k(), Ring::Tile{0, 0}};
-      if (both) k[1] = ring.k();
-      if (w < n) {
-        group(w == 1 || owed, both, nullptr, false, w == 0 ? &k[0] : &k[1], 0, true);
-        owed = false;
-      }
+      if (w < n) qk(w == 0 ? k[0] : k[1], 0, true);
       for (int t = 0; t < n; ++t) {
         const Ring::Tile v = ring.v();
-        const bool mine = (t & 1) == w, more = t + 2 < n;
-        Ring::Tile next{0, 0};
-        if (more) next = ring.k();
-        // (the piece's last group gives the turn to stream 0, which begins the next)
-        if (mine) group(both, both && (t + 1 < n || w == 1), &v, t < 2, more ? &next : nullptr, 0, true);
+        const bool mine = (t & 1) == w;
+        if (t + 2 < n) {
+          const Ring::Tile next = ring.k();
+          if (mine) qk(next, 0, true);
+        }
+        if (mine) pv(v, t < 2, true);
       }
-      if (both && w == 0) owed = n % 2 == 0;
       if (w < n) done(&c.o_full[w]);
       done(&c.q_empty);
     }
@@ -454,79 +453,96 @@ __device__ __forceinline__ void mma_issuer(const Args &a, Ctrl &c, uint8_t *smem
   __syncwarp();
 }
 
-template <bool kTail>
-__device__ __forceinline__ float mask_max(uint32_t (&s)[32], uint32_t vis) {
+template <bool kTail, int kN>
+__device__ __forceinline__ float mask_max(uint32_t (&s)[kN], uint32_t vis) {
   if (kTail) {
 #pragma unroll
-    for (int j = 0; j < 32; ++j) s[j] = vis >> j & 1u ? s[j] : 0xff800000u;  // -inf
+    for (int j = 0; j < kN; ++j) s[j] = vis >> j & 1u ? s[j] : 0xff800000u;  // -inf
   }
   float t = __uint_as_float(s[0]);
 #pragma unroll
-  for (int j = 1; j < 31; j += 2) t = fmaxf(fmaxf(t, __uint_as_float(s[j])), __uint_as_float(s[j + 1]));
-  return fmaxf(t, __uint_as_float(s[31]));
+  for (int j = 1; j < kN - 1; j += 2) t = fmaxf(fmaxf(t, __uint_as_float(s[j])), __uint_as_float(s[j + 1]));
+  return fmaxf(t, __uint_as_float(s[kN - 1]));
+}
+// exp2(x * cl + minus) of kN scores, two to a word, their sum added to `sum`.
+template <typename T, int kN>
+__device__ __forceinline__ void weigh(const uint32_t (&s)[2 * kN], float cl, float minus, float2 (&sum)[2], uint32_t (&p)[kN]) {
+#pragma unroll
+  for (int j = 0; j < kN; ++j) {
+    const float2 x = make_float2(__uint_as_float(s[2 * j]), __uint_as_float(s[2 * j + 1]));
+    const float2 y = fma2(x, make_float2(cl, cl), make_float2(minus, minus));
+    const float2 e = make_float2(ex2(y.x), ex2(y.y));
+    sum[j & 1] = add2(sum[j & 1], e);
+    p[j] = pack2(e.x, e.y, T());
+  }
 }
 
-// Scores of a row's 64 tokens of this half -> weights, in place in TMEM.  kTail: the row
-// sees the first `seen` of them.  ts: the row's 128 scores, to: this half of its O.
-//
-// Two passes of short loops: laid out whole, with a row's scores in registers, the code
-// comes slower than it runs.
+// What a thread of the softmax keeps: a row of its stream's Q tile, half of a tile's tokens.
+struct Half {
+  uint32_t ts, tp, to;  // this half of the row's scores, weights, O
+  float *top;
+  const float *other;   // the halves' maxima
+  uint64_t *s_free, *p_free;
+  int w, q;
+  uint32_t tiles;       // of the stream, so far
+  float m, l;
+};
+// O moves to a new maximum once the values before are in it.
+__device__ __noinline__ void rescale(uint32_t to, float keep) {
+#pragma unroll 1
+  for (int i = 0; i < kDim / 2; i += 16) {
+    uint32_t r[16];
+    tmem_ld16(to + i, r);
+    wait_ld(r);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * keep);
+    tmem_st16(to + i, r);
+  }
+  wait_st();
+}
+// Scores of a row's 40 tokens of this half -> weights.  kTail: the row sees the first
+// `seen` of them.
 template <typename T, bool kTail>
-__device__ __forceinline__ void weigh(uint32_t ts, uint32_t to, int half, int seen, float cl, bool first, bool live,
-                                      float *top, const float *other, int w, int q, float &m, float &l) {
-  ts += 64 * half;
-  float mt = -CUDART_INF_F;
-#pragma unroll 1
-  for (int i = 0; i < 64; i += 32) {
-    uint32_t s[32];
-    tmem_ld32(ts + i, s);
-    wait_ld(s);
-    mt = fmaxf(mt, mask_max<kTail>(s, kTail ? low_bits(seen - i) : ~0u));
-  }
-  mt *= cl;
-  // (the row's maximum is that of both halves)
-  *top = mt;
-  bar_rows(w, q);
-  mt = fmaxf(mt, *other);
-  const bool rise = mt > m + (first ? 0.f : kLazyLog2);
-  if (!first && __any_sync(0xffffffffu, rise && live)) {
-    const float keep = rise ? ex2(m - mt) : 1.f;
-    l *= keep;
-#pragma unroll 1
-    for (int i = 0; i < kDim / 2; i += 16) {
-      uint32_t r[16];
-      tmem_ld16(to + i, r);
-      wait_ld(r);
-#pragma unroll
-      for (int j = 0; j < 16; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * keep);
-      tmem_st16(to + i, r);
+__device__ __forceinline__ void tile(Half &h, int seen, float cl, bool first, bool live, bool &dead, int32_t *flag) {
+  uint32_t s0[32], s1[8];
+  tmem_ld32(h.ts, s0);
+  tmem_ld8(h.ts + 32, s1);
+  wait_ld(s0);
+  wait_ld(s1);
+  fence_before();
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) arrive(h.s_free);  // the next tile's may come
+  float mt = fmaxf(mask_max<kTail>(s0, kTail ? low_bits(seen) : ~0u), mask_max<kTail>(s1, kTail ? low_bits(seen - 32) : ~0u)) * cl;
+  const uint32_t before = (h.tiles - 1) & 1u;  // parity of the tile before's products
+  // the row's maximum is that of both halves; it moves when one has risen far enough
+  if (any_rows(h.w, h.q, first || (live && mt > h.m + kLazyLog2))) {
+    *h.top = mt;
+    bar_rows(h.w, h.q);
+    mt = fmaxf(mt, *h.other);
+    const bool rise = mt > h.m + (first ? 0.f : kLazyLog2);
+    if (!first) {
+      const float keep = rise ? ex2(h.m - mt) : 1.f;
+      h.l *= keep;
+      wait(h.p_free, before, dead, flag);
+      __syncwarp();
+      fence_after();
+      rescale(h.to, keep);
     }
+    if (rise) h.m = mt;
   }
-  if (rise) m = mt;
-  const float minus = m == -CUDART_INF_F ? 0.f : -m;
+  const float minus = h.m == -CUDART_INF_F ? 0.f : -h.m;
   float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-#pragma unroll 1
-  for (int i = 0; i < 64; i += 32) {
-    uint32_t s[32], p[16];
-    tmem_ld32(ts + i, s);
-    wait_ld(s);
-    const uint32_t vis = kTail ? low_bits(seen - i) : ~0u;
-#pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      float2 x = make_float2(__uint_as_float(s[2 * j]), __uint_as_float(s[2 * j + 1]));
-      if (kTail) {
-        x.x = vis >> (2 * j) & 1u ? x.x : -CUDART_INF_F;
-        x.y = vis >> (2 * j + 1) & 1u ? x.y : -CUDART_INF_F;
-      }
-      const float2 y = fma2(x, make_float2(cl, cl), make_float2(minus, minus));
-      const float2 e = make_float2(ex2(y.x), ex2(y.y));
-      sum[j & 1] = add2(sum[j & 1], e);
-      p[j] = pack2(e.x, e.y, T());
-    }
-    tmem_st16(ts + i / 2, p);  // (over scores that have been read)
-  }
+  uint32_t p0[16], p1[4];
+  weigh<T>(s0, cl, minus, sum, p0);
+  const bool is_free = h.tiles == 0 || mbar_test(h.p_free, before);  // (an answer that takes as long as the rest)
+  weigh<T>(s1, cl, minus, sum, p1);
   const float2 t = add2(sum[0], sum[1]);
-  l += t.x + t.y;
+  h.l += t.x + t.y;
+  if (!is_free) wait(h.p_free, before, dead, flag);
+  __syncwarp();
+  fence_after();
+  tmem_st16(h.tp, p0);
+  tmem_st4(h.tp + 16, p1);
   wait_st();
 }
 
@@ -553,12 +569,13 @@ template <typename T>
 __device__ __forceinline__ void softmax(const Args &a, Ctrl &c, uint8_t *smem, uint32_t tmem, int w) {
   const int tid = threadIdx.x & 127, lane = tid & 31, q = tid >> 5, half = (threadIdx.x >> 7) & 1;
   const uint32_t quad = tmem + (uint32_t(q * 32) << 16);
-  const uint32_t ts = quad + col_s(w), to = quad + col_o(w) + half * (kDim / 2);
   float *top = &c.top[w][half][tid], *other = &c.top[w][half ^ 1][tid];
+  Half h{quad + col_s(w) + half * kHalf, quad + col_p(w) + half * (kHalf / 2), quad + col_o(w) + half * (kDim / 2),
+         top, other, &c.s_free[w], &c.p_free[w], w, q, 0, 0.f, 0.f};
   // (a scale of zero: too small to move a score, and -inf stays -inf)
   const float cl = fmaxf(fabsf(a.scale) * 1.44269504088896341f, 1e-37f);
   bool dead = false;
-  uint32_t s_uses = 0, o_uses[2] = {0, 0};
+  uint32_t o_uses[2] = {0, 0};
   Ring ring;
   unsigned piece = 0;
   Walk wk;
@@ -566,7 +583,7 @@ __device__ __forceinline__ void softmax(const Args &a, Ctrl &c, uint8_t *smem, u
   while (wk.next(a, c)) {
     ++piece;
     const bool two = wk.two();
-    const int n = wk.t1 - wk.t0, lead = two ? 1 : 2;
+    const int n = wk.t1 - wk.t0;
     const int len = wk.s.len, row0 = (2 * wk.block + (two ? w : 0)) * kTile;
     const int row = row0 + tid;
     const bool live = row < wk.s.rows;
@@ -574,23 +591,28 @@ __device__ __forceinline__ void softmax(const Args &a, Ctrl &c, uint8_t *smem, u
     // what this row sees, and what all rows of the Q tile see
     const int seen = a.causal ? min(wk.s.past + row + 1, len) : len;
     const int common = a.causal ? min(max(wk.s.past + row0 + 1, 0), len) : len;
-    float m = -CUDART_INF_F, l = 0.f;
+    h.m = -CUDART_INF_F, h.l = 0.f;
     const int tfirst = wk.t0 + (two ? 0 : w);
-    for (int i = 0; i < min(lead, n); ++i) ring.k();
+    for (int i = 0; i < min(kLead, n); ++i) ring.k();
     for (int t = wk.t0; t < wk.t1; ++t) {
       const Ring::Tile vt = ring.v();
-      if (t + lead < wk.t1) ring.k();
+      if (t + kLead < wk.t1) ring.k();
       if (!two && ((t - wk.t0) & 1) != w) continue;
-      const int pos = t * kTile;
-      const bool tail = pos + kTile > common;
-      wait(&c.s_full[w], s_uses++ & 1u, dead, a.error_flag);
+      const int pos = t * kTok;
+      const bool tail = pos + kTok > common;
+      wait(&c.s_full[w], h.tiles & 1u, dead, a.error_flag);
       fence_after();
       if (warp_live) {
         if (tail)
-          weigh<T, true>(ts, to, half, seen - pos - 64 * half, cl, t == tfirst, live, top, other, w, q, m, l);
+          tile<T, true>(h, seen - pos - kHalf * half, cl, t == tfirst, live, dead, a.error_flag);
         else
-          weigh<T, false>(ts, to, half, kTile, cl, t == tfirst, live, top, other, w, q, m, l);
+          tile<T, false>(h, kHalf, cl, t == tfirst, live, dead, a.error_flag);
+      } else {
+        // (no faster than the others: an arrival for the next tile would count for this one)
+        if (lane == 0) arrive(&c.s_free[w]);
+        if (h.tiles > 0) wait(&c.p_free[w], (h.tiles - 1) & 1u, dead, a.error_flag);
       }
+      ++h.tiles;
       if (tail) {
         // V rows past the sequence's end are another's and become zeros, so that weights of
         // zero meet finite values; so do non-finite elements that not every row sees
@@ -598,7 +620,7 @@ __device__ __forceinline__ void softmax(const Args &a, Ctrl &c, uint8_t *smem, u
         wait(&c.full[vt.slot(half)], vt.parity(half), dead, a.error_flag);
         uint8_t *base = smem + kOffSlots + vt.slot(half) * kCol + tid * 16;
 #pragma unroll 1
-        for (int k = min(from, max(end, 0)) / 16; k < 8; ++k) {  // 16 bytes per thread: row = 16 k + tid / 8
+        for (int k = min(from, max(end, 0)) / 16; k < kTok / 16; ++k) {  // 16 bytes per thread: row = 16 k + tid / 8
           uint4 *at = reinterpret_cast<uint4 *>(base + k * 2048);
           const int vrow = 16 * k + (tid >> 3);
           if (vrow >= end) {
@@ -627,6 +649,7 @@ __device__ __forceinline__ void softmax(const Args &a, Ctrl &c, uint8_t *smem, u
       fence_after();
     };
     // (once O is full all of the stream's threads have read the last tile's maxima)
+    float m = h.m, l = h.l;
     float keep0 = 1.f, keep1 = 0.f;
     const bool both = !two && n > 1;
     int d0 = half * (kDim / 2), d1 = d0 + kDim / 2;
@@ -700,7 +723,7 @@ __device__ __forceinline__ void softmax(const Args &a, Ctrl &c, uint8_t *smem, u
     // elements out that all rows of this one see; added twice they are what they are)
     const int hidden = a.causal ? min(max(wk.s.past + 2 * wk.block * kTile + 1, 0), len) : len;
     if (live && *reinterpret_cast<volatile unsigned *>(&c.bad_piece) >= piece)
-      repair_row<T>(a, wk.s, wk.head, max(wk.t0 * kTile, hidden), min(wk.t1 * kTile, seen), d0, d1,
+      repair_row<T>(a, wk.s, wk.head, max(wk.t0 * kTok, hidden), min(wk.t1 * kTok, seen), d0, d1,
                     split ? a.part_o + (static_cast<int64_t>(pslot) * (kDim / 4) * 256 + prow) * 4 : nullptr,
                     static_cast<T *>(a.out) + orow * kDim);
     if (live && half == 0 && (two || w == 0)) {
@@ -754,9 +777,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(&c.q_empty, 2);
     for (int w = 0; w < 2; ++w) {
       mbar_init(&c.s_full[w], 1);
+      mbar_init(&c.s_free[w], 8);
       mbar_init(&c.p_ready[w], 8);
+      mbar_init(&c.p_free[w], 1);
       mbar_init(&c.o_full[w], 1);
-      mbar_init(&c.turn[w], 1);
     }
     fence_mbar_init();
     c.bad_piece = 0;

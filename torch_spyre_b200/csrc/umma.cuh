@@ -79,6 +79,9 @@ __device__ __forceinline__ void tmem_ld16(uint32_t at, uint32_t (&r)[16]) {
       : B200KV_R8(r, 0), B200KV_R8(r, 8)
       : "r"(at));
 }
+__device__ __forceinline__ void tmem_ld8(uint32_t at, uint32_t (&r)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];" : B200KV_R8(r, 0) : "r"(at));
+}
 #define B200KV_RW8(r, i) "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]), \
                          "+r"(r[i + 6]), "+r"(r[i + 7])
 // The loaded registers go through the wait, so that no use of them is moved before it.
@@ -88,6 +91,9 @@ __device__ __forceinline__ void wait_ld(uint32_t (&r)[32]) {
 }
 __device__ __forceinline__ void wait_ld(uint32_t (&r)[16]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" : B200KV_RW8(r, 0), B200KV_RW8(r, 8));
+}
+__device__ __forceinline__ void wait_ld(uint32_t (&r)[8]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" : B200KV_RW8(r, 0));
 }
 __device__ __forceinline__ void tmem_st32(uint32_t at, const uint32_t (&r)[32]) {
   asm volatile(
@@ -100,6 +106,9 @@ __device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t (&r)[16]) 
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(at),
       B200KV_W8(r, 0), B200KV_W8(r, 8));
+}
+__device__ __forceinline__ void tmem_st4(uint32_t at, const uint32_t (&r)[4]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]));
 }
 
 // ---------------------------------------------------------------- operands --
