@@ -833,7 +833,7 @@ B200KV_API int64_t b200kv_latent_workspace_bytes(int64_t total_q, int64_t batch,
  *             elements; 16-byte aligned, strides positive multiples of 8
  *   out       contiguous [total_q, H, 512]; lse fp32 [total_q, H] or NULL
  * Supported: H <= 512, batch <= 1024, total_q * H < 2^31, max_blocks_per_seq < 2^24
- * and (batch + total_q / max(1, 64 / H) + 1) * (max_blocks_per_seq + 4) < 2^31. */
+ * and (batch + total_q / max(1, 64 / H) + 1) * (max_blocks_per_seq + 3) < 2^31. */
 B200KV_API int b200kv_latent_attention(const void *q_latent, int64_t q_latent_stride_t,
                                        int64_t q_latent_stride_h, const void *q_rope,
                                        int64_t q_rope_stride_t, int64_t q_rope_stride_h,

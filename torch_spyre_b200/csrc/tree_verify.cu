@@ -21,7 +21,7 @@
 //
 // Bound: the bytes of a row of p and q per sequence (more where a tree's node
 // rejects several children), or, for few sequences, latency.  128 chains of 4 over 131072
-// elements, fp32: 43 us, 134 MB of rows in 23 of them (5.8 TB/s), the walk before and the
+// elements, fp32: 44 us, 134 MB of rows in 23 of them (5.8 TB/s), the walk before and the
 // exchange and the search behind take 7 and 8; 16 trees of up to 32 nodes over 32000: 23 us.
 #include <cooperative_groups.h>
 
@@ -253,6 +253,8 @@ __global__ void __launch_bounds__(kThreads, 4) tree_verify_kernel(const VerifyAr
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int b = blockIdx.y;
   const bool tells = rank == 0 && tid == 0;
+  // (waited for before another CTA's shared memory is written: it has to have begun)
+  if (ranks > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
   auto report = [&](int bit) {
     if (a.error_flag) atomicOr(a.error_flag, bit);
   };
@@ -358,6 +360,7 @@ __global__ void __launch_bounds__(kThreads, 4) tree_verify_kernel(const VerifyAr
       if (tid == 0) s.cta_sum[pass & 1][0] = total;
       __syncthreads();
     } else {
+      if (pass == 0) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
       if (tid < ranks) {
         double sum = 0.0;
 #pragma unroll
