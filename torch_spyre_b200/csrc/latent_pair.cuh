@@ -35,7 +35,7 @@ namespace pair {
 constexpr int kStep = 2 * kPageTokens;  // tokens of a step
 constexpr int kSlots = 4, kSlot = 2 * kPair;
 constexpr int kAhead = 1;  // steps that pages are in L2 before they are loaded (32 sequences: 61.4 us, with 2 64.4, with none 69.5)
-constexpr int kOffQ = 3072;
+constexpr int kOffQ = 3 * 1024;
 constexpr int kOffP = kOffQ + kSticks * kStickTile;  // [2 pages][64 rows][64 tokens]
 constexpr int kOffRope = kOffP + 2 * kStickTile;
 constexpr int kOffSlots = kOffRope + kStickTile;

@@ -51,7 +51,7 @@ constexpr int kTok = 80, kHalf = kTok / 2;          // tokens of a K or V tile
 constexpr int kColQ = kTile * 128, kCol = kTok * 128;  // bytes of a column of 64 elements
 constexpr int kColsQ = 3, kColsV = 2, kSlots = 12;
 constexpr int kLead = 2;                            // tiles that keys are ahead of values
-constexpr int kOffQ = 3072;
+constexpr int kOffQ = 3 * 1024;
 constexpr int kOffSlots = kOffQ + 2 * kColsQ * kColQ;
 constexpr int kSmem = kOffSlots + kSlots * kCol;
 constexpr float kLazyLog2 = 8.f;
