@@ -198,3 +198,25 @@ def test_repeat_graph_and_operator():
     captured.zero_()
     graph.replay()
     assert torch.equal(captured, first)
+
+
+def test_a_graph_follows_the_offsets():
+    # the plan is made on the device: other prompts of the same numbers of rows and tokens in all
+    case = Case([300, 700, 64], [400, 700, 1000], 4, seed=24)
+    tsb.latent_prompt_attention(*case.args())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = tsb.latent_prompt_attention(*case.args())
+    for q_ptr, kv_ptr in (((0, 1, 1000, 1064), (0, 1, 1900, 2100)), ((0, 0, 1064, 1064), (0, 500, 2000, 2100)),
+                          ((0, 400, 500, 1064), (0, 300, 600, 2100))):
+        case.q_indptr.copy_(torch.tensor(q_ptr, dtype=torch.int32))
+        case.kv_indptr.copy_(torch.tensor(kv_ptr, dtype=torch.int32))
+        graph.replay()
+        assert torch.equal(captured, tsb.latent_prompt_attention(*case.args()))
+
+
+@pytest.mark.parametrize("heads", [37, 100])
+def test_many_short_blocks_to_a_share(heads):
+    # blocks of one and two Q tiles, with warps that have no row, one after the other on every SM
+    new = [1, 70, 33, 129, 161, 300, 44, 257, 96, 5]
+    check(Case(new, [n + p for n, p in zip(new, [0, 79, 80, 0, 33, 1, 500, 7, 160, 81])], heads, seed=heads))
