@@ -21,8 +21,8 @@
 //
 // Bound: the bytes of a row of p and q per sequence (more where a tree's node
 // rejects several children), or, for few sequences, latency.  128 chains of 4 over 131072
-// elements, fp32: 44 us, 134 MB of rows in 23 of them (5.8 TB/s), the walk before and the
-// exchange and the search behind take 7 and 8; 16 trees of up to 32 nodes over 32000: 23 us.
+// elements, fp32: 43 us, 134 MB of rows in 23 of them (5.8 TB/s), the walk before and the
+// exchange and the search behind take 7 and 8; 16 trees of up to 32 nodes over 32000: 22 us.
 #include <cooperative_groups.h>
 
 #include "rows.cuh"
@@ -56,6 +56,7 @@ struct Shared {
   double c;
   int row, num_gone, last;
   int found;  // the thread that has the next token
+  uint64_t landed[2];  // all CTAs' sums of a pass
 };
 
 // Weight of an element; what is not a positive number counts as 0.
@@ -234,6 +235,26 @@ __device__ __noinline__ int find_in_part(const VerifyArgs &a, Shared &s, int row
   return found;
 }
 
+// A sum to the same place of CTA `rank` of the cluster, whose barrier counts its bytes.  (A barrier
+// of the whole cluster orders all memory, and takes 1500 clocks and more.)
+__device__ __forceinline__ void send(const double *to, const uint64_t *bar, int rank, double x) {
+  asm volatile(
+      "{\n\t.reg .b32 d, b;\n\tmapa.shared::cluster.u32 d, %0, %2;\n\tmapa.shared::cluster.u32 b, %1, %2;\n\t"
+      "st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.b64 [d], %3, [b];\n\t}" ::"r"(smem_u32(to)),
+      "r"(smem_u32(bar)), "r"(rank), "l"(__double_as_longlong(x))
+      : "memory");
+}
+
+// Waits for a pass's sums, with a limit.
+__device__ __forceinline__ bool landed(uint64_t *bar, uint32_t parity) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const uint64_t t0 = global_timer_ns();
+  for (uint32_t i = 1;; ++i) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((i & 255u) == 0 && global_timer_ns() - t0 > kWaitLimitNs) return false;
+  }
+}
+
 // The next child of `node` after node i (n: none); the whole warp calls it.
 __device__ __forceinline__ int next_child(const Shared &s, int node, int i, int n) {
   const int lane = threadIdx.x & 31;
@@ -254,7 +275,15 @@ __global__ void __launch_bounds__(kThreads, 4) tree_verify_kernel(const VerifyAr
   const int b = blockIdx.y;
   const bool tells = rank == 0 && tid == 0;
   // (waited for before another CTA's shared memory is written: it has to have begun)
-  if (ranks > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+  if (ranks > 1) {
+    if (tid == 0) {
+      mbar_init(&s.landed[0], 1);
+      mbar_init(&s.landed[1], 1);
+      fence_mbar_init();
+    }
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+  }
   auto report = [&](int bit) {
     if (a.error_flag) atomicOr(a.error_flag, bit);
   };
@@ -361,13 +390,18 @@ __global__ void __launch_bounds__(kThreads, 4) tree_verify_kernel(const VerifyAr
       __syncthreads();
     } else {
       if (pass == 0) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+      if (tid == 0) mbar_arrive_expect_tx(&s.landed[pass & 1], static_cast<uint32_t>(ranks) * 8u);
       if (tid < ranks) {
         double sum = 0.0;
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) sum += s.warp_sum[w];
-        *cluster.map_shared_rank(&s.cta_sum[pass & 1][rank], tid) = sum;
+        send(&s.cta_sum[pass & 1][rank], &s.landed[pass & 1], tid, sum);
       }
-      cluster.sync();
+      if (__syncthreads_or(!landed(&s.landed[pass & 1], (pass >> 1) & 1u))) {
+        if (tells) report(B200KV_DEVERR_TIMEOUT), a.next[b] = -1;
+        cluster.sync();  // (what the others send finds this CTA still there)
+        break;
+      }
       for (int r = 0; r < ranks; ++r) total += s.cta_sum[pass & 1][r];
     }
     if (!last) {
