@@ -71,7 +71,8 @@ __device__ __forceinline__ void place(const PageArgs &a, const int32_t *indptr, 
     const int cap = a.max_blocks * kPageTokens, ctx = min(max(lens[lo], 0), cap), i = t - first;
     depth = a.mask ? max(depth, 0) : i;
     pos = ctx + min(depth, INT_MAX - ctx);
-    if (i < cap - ctx) {
+    // (with a length that cannot be it has no slots: they would be those of committed tokens)
+    if (ctx == lens[lo] && i < cap - ctx) {
       const int at = ctx + i, page = at / kPageTokens;
       const int id = page < counts[lo] ? a.table[lo * a.stride + page] : -1;
       if (id >= 0) slot = int64_t(id) * kPageTokens + at % kPageTokens;
