@@ -729,9 +729,11 @@ B200KV_API int b200kv_tree_commit(void *k_pool, void *v_pool, int32_t pool_dtype
  * depth = i, or with tree_mask (int64 [num_tokens, mask_words], b200kv_tree_mask) the
  * number of its bits less one (0 for a pruned node).  Where the stack runs out
  * the sequence gets no page, nor do those after it that need any
- * (B200KV_DEVERR_NO_PAGES), and tokens without a page have slot -1.  Lengths
- * outside the table are clamped and such a sequence's tokens get slot -1, tokens that no sequence has get slot -1 and
- * position 0 (B200KV_DEVERR_BAD_LEN).  A page belongs to one sequence at a time.
+ * (B200KV_DEVERR_NO_PAGES), and tokens without a page have slot -1.  A sequence
+ * whose context_lens[b] is negative or past its row of the table takes no page, and its
+ * tokens have slot -1; of tokens that would pass the row the first that fit are
+ * placed; tokens that no sequence has get slot -1 and position 0 (all of them
+ * B200KV_DEVERR_BAD_LEN).  A page belongs to one sequence at a time.
  * batch <= 1024, max_blocks_per_seq < 2^21. */
 B200KV_API int b200kv_extend_pages(int32_t *block_table, int64_t block_table_stride,
                                    int32_t *page_counts, int32_t *free_pages, int64_t capacity,

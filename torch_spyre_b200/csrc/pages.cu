@@ -36,16 +36,16 @@ __device__ __forceinline__ void report(const PageArgs &a, int bit) {
   if (a.error_flag) atomicOr(a.error_flag, bit);
 }
 
-// Committed tokens and new ones (first .. end - 1) of a sequence, clamped to the table.
-__device__ __forceinline__ void lengths(const PageArgs &a, int first, int end, int &ctx, int &nodes, bool &bad) {
+// The pages that a sequence of ctx committed tokens and new ones (first .. end - 1) fills,
+// as far as its row of the table has room.  One whose length or offsets cannot be adds
+// nothing, and fills none: taken as the nearest that can be, a length past the table
+// would take all of its row from the stack.
+__device__ __forceinline__ int pages_of(const PageArgs &a, int first, int end, int ctx, bool &bad) {
   const int cap = a.max_blocks * kPageTokens;
   bad = ctx < 0 || ctx > cap || first < 0 || end < first || end > a.total;
-  ctx = min(max(ctx, 0), cap);
-  nodes = bad ? 0 : end - first;
-  if (nodes > cap - ctx) {
-    bad = true;
-    nodes = cap - ctx;
-  }
+  if (bad) return 0;
+  bad = end - first > cap - ctx;
+  return (ctx + min(end - first, cap - ctx) + kPageTokens - 1) / kPageTokens;
 }
 
 // Depth of token t in its tree, less than 0 without a bit in its mask.
@@ -136,10 +136,8 @@ __global__ void __launch_bounds__(kThreads) pages_kernel(const PageArgs a) {
         indptr[b] = begin, lens[b] = len;
         if (b == a.batch - 1) indptr[a.batch] = end;
       }
-      int nodes;
-      lengths(a, begin, end, len, nodes, bad);
       first = owned;
-      need = max((len + nodes + kPageTokens - 1) / kPageTokens - owned, 0);
+      need = max(pages_of(a, begin, end, len, bad) - owned, 0);
     }
     if (bad || owned != owned_in) report(a, B200KV_DEVERR_BAD_LEN);
   }

@@ -107,7 +107,8 @@ def extend_pages(
     token's position is its sequence's length plus its index, or with
     ``tree_mask`` (:func:`torch_spyre_b200.tree_mask`) plus its depth.  Tokens that
     got no page have slot -1, which :func:`torch_spyre_b200.kv_store` skips
-    (``DEVERR_NO_PAGES``)."""
+    (``DEVERR_NO_PAGES``); so have those of a sequence whose length is negative or
+    past its row of the table, which takes no page (``DEVERR_BAD_LEN``)."""
     args = (block_table, page_counts, free_pages, free_count, context_lens, q_indptr, int(num_tokens), tree_mask,
             error_flag)
     pair = None if _eager.compiling() else _eager.fast.extend_pages(*args)
