@@ -571,7 +571,7 @@ __device__ __forceinline__ void softmax(const Args &a, Ctrl &c, uint8_t *smem, u
       if (warp_live) {
         tmem_ld32(quad + col_s(n & 1) + 32 * half, s);
         wait_ld(s);
-        mt = (tail ? mask_max<true>(s, vis) : mask_max<false>(s, ~0u)) * cl;
+        mt = fmaf(tail ? mask_max<true>(s, vis) : mask_max<false>(s, ~0u), cl, -kWeightLog2<T>);
       }
       // the maximum is that of both halves of the row; it moves when either has risen far enough
       if (first || any_softmax(live && mt > m + kLazyLog2)) {

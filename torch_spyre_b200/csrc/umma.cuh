@@ -162,6 +162,16 @@ __device__ __forceinline__ float ex2(float x) {
   return r;
 }
 
+// Softmax weights enter the tensor cores in the 16 bits of the values: 2^(y - m), off by half a
+// step each (2^-8 of the weight in bf16, 2^-11 in fp16, at most), while the row's sum takes them as
+// they are.  m is the running maximum less kWeightLog2, where it may lag behind by 2^8.  bf16 has
+// fp32's exponents.  fp16 ends at 2^-24 below and 65504 above: with the largest weight at 1, a
+// weight below 2^-25 would be lost from the products and stay in the sum, and a flat
+// tail of 32768 tokens at 2^-23.5 of the loudest loses 29 % of its part.  At 2^7, and 2^15 before
+// the maximum follows, what is cut off a weight is at most 2^-32 of the largest.
+template <typename T>
+constexpr float kWeightLog2 = std::is_same<T, __half>::value ? 7.f : 0.f;
+
 // Two fp32 at a time.
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   float2 d;
