@@ -68,3 +68,21 @@ def test_absorbed(heads, dtype):
     indptr = torch.arange(batch + 1, dtype=torch.int32, device="cuda")
     out, lse = tsb.latent_attention(q[..., :512], q[..., 512:], pool, table, lens, indptr, scale=SCALE, return_lse=True)
     check(out, lse, loud, quiet, (lens + 1)[:, None].expand(batch, heads), dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("rows", [200, 100])
+def test_expanded(rows, dtype):
+    heads, g = 148, torch.Generator(device="cuda").manual_seed(rows)
+    loud, quiet = values(128, dtype, g)
+    k = torch.zeros((TOKENS, heads, 128), dtype=dtype, device="cuda")
+    k[0, :, 5] = 64
+    v = quiet.expand(TOKENS, heads, 128).contiguous()
+    v[0] = loud
+    q = torch.zeros((rows, heads, 192), dtype=dtype, device="cuda")
+    q[..., 5] = 1
+    ptr = [torch.tensor([0, n], dtype=torch.int32, device="cuda") for n in (rows, TOKENS)]
+    r = torch.zeros((TOKENS, 64), dtype=dtype, device="cuda")
+    out, lse = tsb.latent_prompt_attention(q, k, r, v, *ptr, scale=SCALE, return_lse=True)
+    seen = TOKENS - rows + 1 + torch.arange(rows, device="cuda")
+    check(out, lse, loud, quiet, seen[:, None].expand(rows, heads), dtype)

@@ -512,7 +512,8 @@ __device__ __forceinline__ void tile(Half &h, int seen, float cl, bool first, bo
   fence_before();
   __syncwarp();
   if ((threadIdx.x & 31) == 0) arrive(h.s_free);  // the next tile's may come
-  float mt = fmaxf(mask_max<kTail>(s0, kTail ? low_bits(seen) : ~0u), mask_max<kTail>(s1, kTail ? low_bits(seen - 32) : ~0u)) * cl;
+  float mt = fmaxf(mask_max<kTail>(s0, kTail ? low_bits(seen) : ~0u), mask_max<kTail>(s1, kTail ? low_bits(seen - 32) : ~0u));
+  mt = fmaf(mt, cl, -kWeightLog2<T>);
   const uint32_t before = (h.tiles - 1) & 1u;  // parity of the tile before's products
   // the row's maximum is that of both halves; it moves when one has risen far enough
   if (any_rows(h.w, h.q, first || (live && mt > h.m + kLazyLog2))) {
