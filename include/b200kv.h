@@ -866,7 +866,8 @@ B200KV_API int64_t b200kv_prompt_workspace_bytes(int64_t total_q, int64_t total_
  * B200KV_DEVERR_BAD_LEN; rows that no sequence has (all of them, where offsets descend)
  * are given as rows that see nothing.  Supported: H <= 65536, batch <= 1024, total_q * H
  * < 2^31, total_kv < 2^30 and, with T = total_kv / 80 + 1, (30 * (total_q / 256 + batch) +
- * 4 * (total_q / 256 * T + T + batch)) * H < 2^31. */
+ * 4 * (total_q / 256 * T + T + batch)) * H / SMs + 4 * T + 64 < 2^31 (8 million rows and as many
+ * tokens with 16 heads on 148 SMs). */
 B200KV_API int b200kv_latent_prompt_attention(
     const void *q, int64_t q_stride_t, int64_t q_stride_h, const void *k_nope, int64_t k_stride_t,
     int64_t k_stride_h, const void *k_rope, int64_t k_rope_stride_t, const void *v,

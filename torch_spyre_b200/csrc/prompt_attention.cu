@@ -69,10 +69,13 @@ extern "C" int b200kv_latent_prompt_attention(const void *q, int64_t q_stride_t,
                    "batch, total_q * num_heads or total_kv out of range");
   if (batch > 1024) return set_error(B200KV_ERR_UNSUPPORTED, "batch %lld > 1024 unsupported", (long long)batch);
   B200KV_CHECK_ARG(std::isfinite(scale), "scale must be finite");
-  // the kernel counts its units of work in 31 bits: kBegin + 4 a tile for a block of 256 rows, at most
+  // The kernel counts a share's units of work, and one more block's, in 31 bits: kBegin + 4 a tile for a
+  // block of 256 rows.  At most, that is: the rows of a batch meet their own sequences' tokens only.
   const int64_t blocks = total_q / 256 + batch, tiles = total_kv / prompt::kTok + 1;
-  if ((blocks * (prompt::kBegin2 + 4) + 4 * (total_q / 256 * tiles + tiles + batch)) * num_heads >= (int64_t{1} << 31))
-    return set_error(B200KV_ERR_UNSUPPORTED, "2^31 or more steps of rows and tokens");
+  const int64_t units = (blocks * (prompt::kBegin2 + 4) + 4 * (total_q / 256 * tiles + tiles + batch)) * num_heads;
+  auto countable = [&](int shares) { return units / shares + 4 * tiles + 64 < (int64_t{1} << 31); };
+  if (!countable(prompt::kMaxCtas))
+    return set_error(B200KV_ERR_UNSUPPORTED, "2^31 or more steps of rows and tokens for an SM");
   if (total_q == 0) return B200KV_OK;
   B200KV_CHECK_ARG(batch > 0, "rows without a sequence");
   B200KV_CHECK_ARG(q && q_indptr && kv_indptr && out && (total_kv == 0 || (k_nope && k_rope && v)), "null pointer argument");
@@ -94,6 +97,8 @@ extern "C" int b200kv_latent_prompt_attention(const void *q, int64_t q_stride_t,
   int dev = 0, sms = 0;
   int st = current_device_sm_count(&dev, &sms);
   if (st != B200KV_OK) return st;
+  const int ctas = sms < prompt::kMaxCtas ? sms : prompt::kMaxCtas;
+  if (!countable(ctas)) return set_error(B200KV_ERR_UNSUPPORTED, "2^31 or more steps of rows and tokens for an SM");
   prompt::Args a{};
   a.q_indptr = q_indptr, a.kv_indptr = kv_indptr;
   a.v = v, a.v_st = v_stride_t, a.v_sh = v_stride_h;
@@ -122,7 +127,6 @@ extern "C" int b200kv_latent_prompt_attention(const void *q, int64_t q_stride_t,
     st = encode(&vm, type, none ? q : v, prompt::kDim, num_heads, rows, none ? q_stride_h : v_stride_h,
                 none ? q_stride_t : v_stride_t, prompt::kTok);
   if (st != B200KV_OK) return st;
-  const int ctas = sms < prompt::kMaxCtas ? sms : prompt::kMaxCtas;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   const WorkspaceLock lock(workspace);
   return dtype == B200KV_F16 ? prompt::launch<__half>(qm, km, rm, vm, a, ctas, s)

@@ -68,7 +68,7 @@ struct Seq {
   int past;  // tokens before the first row's own (may be negative)
   int end;   // the first row of q that is a later sequence's
 };
-struct Start {
+struct Start {  // where a share begins: in a block whose units begin at u0, counted from the share's first
   Seq s;
   int b, head, block, u0;
 };
@@ -78,9 +78,9 @@ struct Ctrl {
   uint64_t q_full, q_empty;
   uint64_t s_full[2], s_free[2], p_ready[2], p_free[2], o_full[2];
   uint32_t tmem;
-  int per, total;  // units of a share, of the line
+  int per, end;  // units of a share, of this CTA's (the last may have fewer, or none)
   Start start;
-  int scan[32];
+  int64_t scan[kThreads / 32];
   unsigned bad_piece;  // last piece (counted from 1) that met a non-finite value in a V row
   float top[2][2][kTile];  // streams' rows: the halves' maxima of a tile; sums, when a piece ends
 };
@@ -131,11 +131,12 @@ __device__ __forceinline__ int begin_units(const Seq &s, int k) { return two_til
 __device__ __forceinline__ int block_units(const Args &a, const Seq &s, int k) {
   return begin_units(s, k) + step_units(s, k) * block_tiles(a, s, k);
 }
-__device__ __forceinline__ int head_units(const Args &a, const Seq &s) {
+// (The line is counted in 64 bits, a share and a block in 31: the host has bounded a share.)
+__device__ __forceinline__ int64_t head_units(const Args &a, const Seq &s) {
   if (s.blocks == 0) return 0;
   // without a mask all blocks have as many tiles, and only the last may be of one Q tile
-  if (!a.causal) return (s.blocks - 1) * block_units(a, s, 0) + block_units(a, s, s.blocks - 1);
-  int n = 0;
+  if (!a.causal) return static_cast<int64_t>(s.blocks - 1) * block_units(a, s, 0) + block_units(a, s, s.blocks - 1);
+  int64_t n = 0;
   for (int k = 0; k < s.blocks; ++k) n += block_units(a, s, k);
   return n;
 }
@@ -145,25 +146,24 @@ __device__ __forceinline__ int head_units(const Args &a, const Seq &s) {
 struct Walk {
   Seq s;
   int b, head, block, u0, tiles, t0, t1;  // piece: token tiles [t0, t1) of `tiles`
-  int end;                                // of the share
+  int end;                                // of the share; units count from its first
 
   __device__ __forceinline__ void init(const Ctrl &c) {
     const Start &f = c.start;
     s = f.s, b = f.b, head = f.head, block = f.block, u0 = f.u0;
     t1 = 0;
-    end = min(c.total, (static_cast<int>(blockIdx.x) + 1) * c.per);
+    end = c.end;
   }
   // Tile t belongs to the share that holds its first unit.
   __device__ __forceinline__ int tile_from(int unit) const {
     const int w = step_units(s, block), x = unit - u0 - begin_units(s, block);
     return x <= 0 ? 0 : min(tiles, (x + w - 1) / w);
   }
-  __device__ __forceinline__ bool next(const Args &a, const Ctrl &c) {
-    const int first = static_cast<int>(blockIdx.x) * c.per;
+  __device__ __forceinline__ bool next(const Args &a) {
     for (;;) {
-      if (first >= c.total || u0 >= end) return false;
+      if (end <= 0 || u0 >= end) return false;
       tiles = block_tiles(a, s, block);
-      t0 = tile_from(first);
+      t0 = tile_from(0);
       t1 = tile_from(end);
       if (t0 < t1) return true;
       advance(a);
@@ -183,7 +183,8 @@ struct Walk {
   }
   __device__ __forceinline__ bool two() const { return two_tiles(s, block); }
   __device__ __forceinline__ int share_of(int t, int per) const {
-    return (u0 + begin_units(s, block) + t * step_units(s, block)) / per;
+    const int x = u0 + begin_units(s, block) + t * step_units(s, block);
+    return static_cast<int>(blockIdx.x) + (x >= 0 ? x / per : -((per - 1 - x) / per));
   }
 };
 
@@ -204,15 +205,15 @@ __device__ __noinline__ void clear_rows(const Args &a, bool all) {
 }
 
 // The line's length, a share's, and where this CTA's begins; all threads call it,
-// a barrier follows.  The counts fit 31 bits (the host checks) where no two
-// sequences have the same row or token: with offsets that descend nothing has a sequence.
+// a barrier follows.  A share fits 31 bits (the host checks) where no two sequences have
+// the same row or token: with offsets that descend nothing has a sequence.
 template <typename T>
 __device__ __forceinline__ void make_plan(const Args &a, Ctrl &c) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int each = (a.batch + kThreads - 1) / kThreads;
   const int b0 = tid * each, b1 = min(b0 + each, a.batch);
   Seq s{};
-  int mine = 0;
+  int64_t mine = 0;
   bool unclaimed = false, descends = false;
   for (int b = b0; b < b1; ++b) {
     descends = descends || __ldg(a.q_indptr + b + 1) < __ldg(a.q_indptr + b) || __ldg(a.kv_indptr + b + 1) < __ldg(a.kv_indptr + b);
@@ -223,47 +224,48 @@ __device__ __forceinline__ void make_plan(const Args &a, Ctrl &c) {
     if (!none) mine += head_units(a, s) * a.heads;
     unclaimed = unclaimed || (b == 0 && s.q0 > 0) || s.q0 + s.rows < s.end;
   }
-  int incl = mine;
+  int64_t incl = mine;
 #pragma unroll
   for (int m = 1; m < 32; m <<= 1) {
-    const int y = __shfl_up_sync(0xffffffffu, incl, m);
+    const int64_t y = __shfl_up_sync(0xffffffffu, incl, m);
     if (lane >= m) incl += y;
   }
   if (lane == 31) c.scan[warp] = incl;
   if (__syncthreads_or(unclaimed || none)) clear_rows<T>(a, none);
-  int total = 0, before = 0;
+  int64_t total = 0, before = 0;
 #pragma unroll
   for (int w = 0; w < kThreads / 32; ++w) {
     if (w < warp) before += c.scan[w];
     total += c.scan[w];
   }
   // (at least a step, so that a share inside a block holds the start of a tile)
-  const int per = max(4, static_cast<int>((static_cast<unsigned>(total) + gridDim.x - 1) / gridDim.x));
-  const int first = static_cast<int>(blockIdx.x) * per;
-  int at = before + incl - mine;
+  const int per = max(4, static_cast<int>((total + gridDim.x - 1) / gridDim.x));
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * per;
+  int64_t at = before + incl - mine;
   if (first >= at && first < at + mine) {
-    int b = b0, hu = 0;
+    int64_t hu = 0;
+    int b = b0;
     for (;; ++b) {
       if (each > 1) s = load_seq(a, b, false);
       hu = head_units(a, s);
       if (first < at + hu * a.heads) break;
       at += hu * a.heads;
     }
-    const int head = (first - at) / hu;
+    const int head = static_cast<int>((first - at) / hu);
     at += head * hu;
     int block = 0;
     if (!a.causal) {
       const int n = block_units(a, s, 0);
-      block = min((first - at) / n, s.blocks - 1);
-      at += block * n;
+      block = static_cast<int>(min((first - at) / n, static_cast<int64_t>(s.blocks - 1)));
+      at += static_cast<int64_t>(block) * n;
     } else {
       for (int n; first >= at + (n = block_units(a, s, block)); ++block) at += n;
     }
-    c.start = Start{s, b, head, block, at};
+    c.start = Start{s, b, head, block, static_cast<int>(at - first)};
   }
   if (tid == 0) {
     c.per = per;
-    c.total = total;
+    c.end = static_cast<int>(max(min(total - first, static_cast<int64_t>(per)), int64_t{0}));
   }
 }
 
@@ -300,7 +302,7 @@ __device__ __forceinline__ void producer(const Args &a, Ctrl &c, uint8_t *smem, 
   uint32_t loaded = 0, last = 0;  // slots with a copy that was issued, their parities
   Walk w;
   w.init(c);
-  while (w.next(a, c)) {
+  while (w.next(a)) {
     const bool two = w.two();
     // a column to a lane
     auto issue = [&](const Ring::Tile &tile, uint32_t cols, const CUtensorMap *map, int t) {
@@ -418,7 +420,7 @@ __device__ __forceinline__ void mma_issuer(const Args &a, Ctrl &c, uint8_t *smem
   Ring ring;
   Walk wk;
   wk.init(c);
-  while (wk.next(a, c)) {
+  while (wk.next(a)) {
     wait(&c.q_full, pieces++ & 1u, dead, a.error_flag);
     const int n = wk.t1 - wk.t0;
     Ring::Tile k[2] = {ring.k(), Ring::Tile{0, 0}};
@@ -581,7 +583,7 @@ __device__ __forceinline__ void softmax(const Args &a, Ctrl &c, uint8_t *smem, u
   unsigned piece = 0;
   Walk wk;
   wk.init(c);
-  while (wk.next(a, c)) {
+  while (wk.next(a)) {
     ++piece;
     const bool two = wk.two();
     const int n = wk.t1 - wk.t0;
