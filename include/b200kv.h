@@ -174,6 +174,12 @@ B200KV_API int b200kv_lse_combine_f32(const void *part_o, int32_t part_elem_byte
                                       int64_t head_dim, void *out, float *lse_out,
                                       void *stream);
 
+/* The same with the parts' type (enum b200kv_dtype: fp16, bf16 or fp32); out is bf16 where
+ * the parts are, else fp16. */
+B200KV_API int b200kv_lse_combine(const void *part_o, int32_t dtype, const float *part_lse,
+                                  int64_t num_parts, int64_t rows, int64_t head_dim, void *out,
+                                  float *lse_out, void *stream);
+
 /*
  * q            fp16, element (b, h, d) at q[b * q_stride_b + h * q_stride_h + d]
  * k_pool/v_pool fp16 [num_blocks, num_kv_heads, D/64, 64, 64] (16-byte aligned)

@@ -388,7 +388,7 @@ def latent_prompt_attention(
     with ``causal`` row i of n sees the first m - n + i + 1 of m.  Without, all of
     them: the past of a chunk, read back by :func:`latent_load`, whose result and
     log-sum-exps :func:`torch_spyre_b200.merge_attention_states` joins with the
-    chunk's own (it takes fp16 or fp32 outputs).  Returns out [N, H, 128] (and the natural-log LSE [N, H] fp32); a
+    chunk's own.  Returns out [N, H, 128] (and the natural-log LSE [N, H] fp32); a
     row that sees nothing gets zeros and -inf.  scale defaults to 1 / sqrt(192)."""
     if scale is None:
         scale = 1.0 / math.sqrt(NOPE + ROPE)

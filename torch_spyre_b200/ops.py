@@ -485,27 +485,30 @@ def kv_unrelayout(pool, block_ids, num_tokens: int, error_flag=None) -> torch.Te
 
 
 # ------------------------------------------------------ merge split states --
+_PART_CODES = {getattr(torch, name): _lib.DTYPES[name] for name in ("float16", "bfloat16", "float32")}
+
+
 def merge_attention_states(outs, lses):
     """Merges attention outputs computed over disjoint KV sets of the same
-    queries: outs [n] of [..., D] (fp16 or fp32), lses [n] of [...] fp32
-    (natural-log LSE, -inf for an empty set) -> (out fp16 [..., D], lse fp32).
-    E.g. a shared prefix decoded once and each sequence's own pages decoded
-    separately (``b200kv_lse_combine_f32``)."""
+    queries: outs [n] of [..., D] (fp16, bf16 or fp32), lses [n] of [...] fp32
+    (natural-log LSE, -inf for an empty set) -> (out [..., D], bf16 where outs
+    are, else fp16; lse fp32).  E.g. a shared prefix decoded once and each
+    sequence's own pages decoded separately (``b200kv_lse_combine``)."""
     outs, lses = list(outs), list(lses)
     if not outs or len(outs) != len(lses):
         raise ValueError("need matching non-empty lists of outputs and LSEs")
     o = torch.stack([t.contiguous() for t in outs])
     l = torch.stack([t.contiguous().float() for t in lses])
     _require_cuda(o, l)
-    if o.dtype not in (torch.float16, torch.float32):
-        raise ValueError("outputs must be fp16 or fp32")
+    if o.dtype not in _PART_CODES:
+        raise ValueError(f"outputs must be fp16, bf16 or fp32, not {o.dtype}")
     D = o.shape[-1]
     rows = o[0].numel() // D
     if l[0].numel() != rows:
         raise ValueError("each LSE must have one value per output row")
-    out = torch.empty(o.shape[1:], dtype=torch.float16, device=o.device)
+    out = torch.empty(o.shape[1:], dtype=torch.bfloat16 if o.dtype == torch.bfloat16 else torch.float16, device=o.device)
     lse = torch.empty(l.shape[1:], dtype=torch.float32, device=o.device)
-    _lib.call("b200kv_lse_combine_f32", o.data_ptr(), o.element_size(), l.data_ptr(), o.shape[0], rows, D,
+    _lib.call("b200kv_lse_combine", o.data_ptr(), _PART_CODES[o.dtype], l.data_ptr(), o.shape[0], rows, D,
               out.data_ptr(), lse.data_ptr(), _stream_ptr(o.device))
     return out, lse
 
