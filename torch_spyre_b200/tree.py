@@ -196,6 +196,9 @@ def tree_attention(
 
 
 # ------------------------------------------------------------------- verify --
+MAX_NODES = 1024  # of a sequence
+
+
 def _check_probs(probs: torch.Tensor, name: str, nodes: int, device: torch.device) -> None:
     if probs.dim() != 2 or len(probs) != nodes or probs.dtype not in ROTARY_DTYPES or probs.device != device \
             or probs.shape[1] < 1 or (probs.shape[1] > 1 and probs.stride(1) != 1):
@@ -283,10 +286,11 @@ def tree_verify(
     64-bit arithmetic.
 
     Returns path int32 [B, max_path] (the nodes that stay, 0 first, then -1; at
-    most ``max_path``, default N), path_lens int32 [B], as :func:`tree_commit`
-    takes them, and next_tokens int64 [B].  At most 1024 nodes a sequence."""
+    most ``max_path``, default the smaller of N and 1024: the nodes of the deepest
+    draft are enough), path_lens int32 [B], as :func:`tree_commit` takes them, and
+    next_tokens int64 [B].  At most 1024 nodes a sequence."""
     if max_path is None:
-        max_path = max(1, parents.shape[0])
+        max_path = min(max(1, parents.shape[0]), MAX_NODES)
     args = (parents, tokens, q_indptr, target_probs, accept_u, sample_u, draft_probs, int(max_path), error_flag)
     out = None if _eager.compiling() else _eager.fast.tree_verify(*args)
     if out is None:
