@@ -160,6 +160,13 @@ B200KV_API int64_t b200kv_decode_workspace_bytes(int64_t batch, int64_t num_q_he
 B200KV_API int64_t b200kv_query_workspace_bytes(int64_t batch, int64_t num_q_heads,
                                                 int64_t num_kv_heads, int64_t head_dim);
 
+/* Sets this thread's mode for calls that a stream capture under way may refuse (enum
+ * cudaStreamCaptureMode: 0 global, 1 thread-local, 2 relaxed), and *mode to the one before.
+ * In the relaxed mode a workspace can be made and zeroed, on a stream that is not captured,
+ * while another is: a fill that the graph records comes with each of its replays,
+ * and not before the first. */
+B200KV_API int b200kv_exchange_capture_mode(int32_t *mode);
+
 /* Merge of attention outputs over disjoint KV sets through their
  * log-sum-exps (the split-KV combine, exposed): part_o [num_parts][rows]
  * [head_dim] (fp16 when part_elem_bytes is 2, fp32 when 4), part_lse fp32

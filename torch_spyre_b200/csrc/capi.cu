@@ -232,6 +232,15 @@ extern "C" int b200kv_stick_layout(const int64_t *host_size, const int64_t *host
   return B200KV_OK;
 }
 
+extern "C" int b200kv_exchange_capture_mode(int32_t *mode) {
+  clear_error();
+  B200KV_CHECK_ARG(mode && *mode >= 0 && *mode <= 2, "mode is null or not 0, 1 or 2");
+  cudaStreamCaptureMode m = static_cast<cudaStreamCaptureMode>(*mode);
+  B200KV_CUDA_TRY(cudaThreadExchangeStreamCaptureMode(&m));
+  *mode = static_cast<int32_t>(m);
+  return B200KV_OK;
+}
+
 extern "C" int64_t b200kv_device_size_in_bytes(const int64_t *device_size, int32_t device_rank) {
   if (!device_size || device_rank < 1) return -1;
   int64_t sticks = 1;

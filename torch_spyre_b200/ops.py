@@ -29,6 +29,7 @@ only implementation: CPU tensors are rejected, there is no fallback.
 
 from __future__ import annotations
 
+import ctypes
 import math
 import os
 from typing import Optional
@@ -63,6 +64,26 @@ def _require_cuda(*tensors: torch.Tensor) -> None:
             )
 
 
+def _zeros_beside_a_capture(nbytes: int) -> torch.Tensor:
+    """Zeros on the current device that the capture under way has no part in.  In the graph's
+    own memory they could share a place with what it computes before, and a recorded fill
+    would be repeated by every replay, and missing in a second graph that is replayed first."""
+    mode = ctypes.c_int32(2)  # relaxed: another stream may allocate and be waited for
+    _lib.call("b200kv_exchange_capture_mode", ctypes.byref(mode))
+    try:
+        for _ in range(64):
+            stream = torch.cuda.Stream()  # (one of a few, the captured one among them)
+            with torch.cuda.stream(stream):
+                if torch.cuda.is_current_stream_capturing():
+                    continue
+                ws = torch.zeros(nbytes, dtype=torch.uint8, device="cuda")
+            stream.synchronize()
+            return ws
+    finally:
+        _lib.call("b200kv_exchange_capture_mode", ctypes.byref(mode))
+    raise RuntimeError("every stream is being captured: call the operator once on this stream before the capture")
+
+
 def workspace_for(device: torch.device, nbytes: int) -> torch.Tensor:
     """Zero-initialised decode workspace cached per (device, stream).
 
@@ -76,7 +97,12 @@ def workspace_for(device: torch.device, nbytes: int) -> torch.Tensor:
     if ws is None or ws.numel() < nbytes:
         if ws is not None:
             _outgrown.append(ws)
-        ws = torch.zeros(1 << max(nbytes - 1, (1 << 20) - 1).bit_length(), dtype=torch.uint8, device=device)
+        size = 1 << max(nbytes - 1, (1 << 20) - 1).bit_length()
+        with torch.cuda.device(key[0]):
+            if torch.cuda.is_current_stream_capturing():
+                ws = _zeros_beside_a_capture(size)
+            else:
+                ws = torch.zeros(size, dtype=torch.uint8, device=device)
         _workspaces[key] = ws
     return ws
 
