@@ -112,10 +112,14 @@ extern "C" int b200kv_latent_attention(const void *q_latent, int64_t q_latent_st
   latent::Args a{};
   a.head_box = static_cast<int>(num_heads < 64 ? num_heads : 64);
   a.tile_nodes = 64 / a.head_box;
-  // Blocks of more than 64 rows, as far as the host knows, go to pairs of SMs (32 sequences, 128
-  // heads: 60 us, on single SMs 78; 8 trees, 128 heads: 101 and 158; 16 chains of 4, 32 heads: 35
-  // and 41), others to single ones (64 sequences, 16 heads: 67 us, on pairs 81; 300 short
-  // ones: 37 and 48).
+  // Blocks of more than 64 rows, as far as the host knows, go to pairs of SMs (when this was chosen: 32
+  // sequences, 128 heads: 60 us, in a form for single SMs 78; 8 trees, 128 heads: 101 and 158; 16
+  // chains of 4, 32 heads: 35 and 41), others to single ones (64 sequences, 16 heads: 67 us, on pairs 81;
+  // 300 short ones: 37 and 48).  More than 64 heads have the pairs alone, whose second CTA may be nearly
+  // empty: 32 sequences of 4000 tokens take 59 us with 65 heads, 61 with 128, 53 with 64 on single SMs.
+  // The host knows sums: a batch with few rows on average stays on single SMs though it has a large tree,
+  // whose blocks read its pages each.  63 single tokens over 4000 and a tree of 64 nodes over 8000, 16
+  // heads: 94 us, on pairs 96; the singles over 1000 and the tree over 60000: 221 and 129.
   const bool pairs = num_heads > 64 || total_q > batch * a.tile_nodes;
   a.stride = pairs ? 2 * static_cast<int>((num_heads + 127) / 128) : 1;
   a.block_nodes = pairs && num_heads <= 64 ? 2 * a.tile_nodes : a.tile_nodes;

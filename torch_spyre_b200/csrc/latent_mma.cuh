@@ -24,8 +24,8 @@
 // 74 KB take at the copy rate on every SM.  What costs beside that are the hand-overs:
 // a wait for a barrier that is already complete takes some 200 clocks of a warp's time
 // between products, so there are few of them, and roles that would wait for one another
-// are warps of their own.  64 sequences of up to 8192 tokens (321 MB), 16 heads: 67 us,
-// 4.8 TB/s with the plan (2 to 3 us), pieces' ends and the join (6.5 us by itself).
+// are warps of their own.  64 sequences of up to 8192 tokens (321 MB), 16 heads: 68 us,
+// 70 among other work, 4.7 TB/s with the plan (2 to 3 us), pieces' ends and the join (6.5 us by itself).
 //
 // Warps: 0-7 softmax and output (warp w: lanes 0-15 of quadrant w % 4 have rows
 // 16 (w % 4) .., where an M = 64 accumulator lies, and half w / 4 of a page's tokens),
@@ -280,7 +280,8 @@ __device__ __forceinline__ void producer(const Args &a, Ctrl &c, uint8_t *smem, 
                                          const CUtensorMap *rm, const CUtensorMap *hm, const CUtensorMap *sm) {
   const int lane = threadIdx.x & 31;
   const uint32_t q_bytes = static_cast<uint32_t>(a.box_nodes * a.head_box * 128);
-  // a page is read once (by one block of one CTA) and leaves L2 first
+  // a page is read once (by one block of one CTA; only a sequence of more nodes than a tile holds has
+  // several, which read it each) and leaves L2 first
   const uint64_t policy = l2_policy_evict_first();
   bool dead = false;
   uint32_t halves = 0, pieces = 0;  // issued

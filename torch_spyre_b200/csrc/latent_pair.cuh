@@ -9,9 +9,10 @@
 //   O [128 rows, 512]        += P V      each CTA half of the latent elements
 // at 32 and 64 clocks a product of 16, 2176 for 128 tokens, where its own operands
 // take 4 and 6 KB.  (One SM with 64 rows: 3800 clocks for 128 tokens.)  32 sequences of up
-// to 8192 tokens (170 MB), 128 heads: 60 us; first pieces run at HBM's rate (3300 clocks a step),
+// to 8192 tokens (170 MB), 128 heads: 64 us, 66 among other work; first pieces run at HBM's rate (3300 clocks a step),
 // 5 us pass before their first loads and 3 us at each piece's end, most of them 128 KB of
-// partials a CTA.  8 trees of up to 8 nodes over up to 16384 tokens: 101 us, 2400 clocks a step.
+// partials a CTA.  8 trees of up to 8 nodes over up to 16384 tokens: 103 us, 2400 clocks a step, 117
+// in long runs, in which the power limit lowers the clock.
 //
 // A step's keys are read as they arrive, half a page at a time, and their slots freed at
 // once; its values, half of the elements of both pages, come again (out of L2) when the

@@ -27,7 +27,7 @@ struct StoreArgs {
   int32_t *error_flag;
 };
 
-// Byte offset of element e (a multiple of 8) of the row at `slot`.
+// Offset, in elements, of element e (a multiple of 8) of the row at `slot`.
 __device__ __forceinline__ int64_t row_at(int64_t slot, int e) {
   return ((slot / kPageTokens * (kRow / 64) + e / 64) * kPageTokens + slot % kPageTokens) * 64 + e % 64;
 }

@@ -16,15 +16,15 @@
 //
 // 80 tokens, since a stream has 256 of TMEM's columns: 80 S, 40 P, 128 O.  (Tiles of 128 with P in
 // S's place have 25 % fewer clocks of products, 2560 for 128 tokens and both streams, but a
-// stream's products and softmax then follow one another: 233 us instead of 225 below, 1440
-// instead of 1345.)
+// stream's products and softmax then follow one another: 233 us for four prompts where these took 225, 1440
+// for two chunks and 1345.)
 //
 // What bounds it: the softmax warps, which are never idle: of 2700 clocks for a tile of both
 // streams 200 to take S, 200 for the rows' maxima, 1300 to 1450 for exponentials (1280 of
 // the special-function units', which both streams use at once; in turns they are no
 // faster), 300 to write P, the rest waits and arrivals; the products take 1900.  Then the
 // power limit: in long runs the clock falls from 1965 to some 1600 MHz.  Four prompts of up to 4096 rows, 16
-// heads: 225 us; two chunks of 777 to 1024 rows over 4001 to 8000 tokens, 128 heads: 1345.
+// heads: 219 us, in long runs 252; two chunks of 777 to 1024 rows over 4001 to 8000 tokens, 128 heads: 1325 and 1537.
 // Exponentials by a polynomial on the FMA units, for a quarter or a half of the
 // elements, waits that sleep, and code laid out without loops were as fast or slower.
 //

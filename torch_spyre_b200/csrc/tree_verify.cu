@@ -22,7 +22,10 @@
 // Bound: the bytes of a row of p and q per sequence (more where a tree's node
 // rejects several children), or, for few sequences, latency.  128 chains of 4 over 131072
 // elements, fp32: 43 us, 134 MB of rows in 23 of them (5.8 TB/s), the walk before and the
-// exchange and the search behind take 7 and 8; 16 trees of up to 32 nodes over 32000: 22 us.
+// exchange and the search behind take 7 and 8; 16 trees of up to 32 nodes over 32000: 20 us.
+// Chains over bf16 rows: 33 us, without the drafter's rows 34 (fp32 37); trees over bf16 rows 25, without the
+// drafter's 14.  (Four CTAs to an SM leave a thread 64 registers: with a drafter's rows 128 to 196
+// bytes of its state are spilled around the sums.)
 #include <cooperative_groups.h>
 
 #include "rows.cuh"
